@@ -331,6 +331,41 @@ int lowbit_grouped_mlp_forward(const void *x, const void *const *w_gate, const v
                                const int32_t *group_offsets, int n_groups, int64_t total_rows, int qtype,
                                int act_dtype, int64_t N, int64_t K, int act, void *stream);
 
+/* ---- products of two e4m3 operands with a scale for each block of 128
+ *
+ * The form in which block-scaled fp8 checkpoints hold their weights, multiplied on the fp8 matrix pipes: a weight [N, K] is row-major
+ * e4m3 codes (K a multiple of 16) with one float32 scale for each 128 x 128 block, scale[ceil(N / 128)][ceil(K / 128)]; the last
+ * blocks of a row or column may end short.  Activations are quantized in the call, by row, one scale for each 128 values:
+ * scale = a / 448, code = e4m3(x * 448 / a) to the nearest (ties to even), a = the block's largest magnitude, 2^-100 at least.  A block that
+ * holds a NaN or an infinity stands for NaN throughout.  All pointers are 16-byte aligned device memory (bias: any alignment).
+ * No counterpart in the reference, whose fp8 weights meet 16-bit activations (low_bit_linear.py:657-668). */
+
+/* codes [rows, K] and scale [rows, ceil(K / 128)] of x [rows, K], of any LOWBIT_DT_*. */
+int lowbit_block_fp8_quantize(const void *x, int dtype, int64_t rows, int64_t K, void *codes, float *scale, void *stream);
+/* codes and scales of `matrices` weights [N, K], one after the other; blocks of 128 x 128. */
+int lowbit_block_fp8_quantize_weight(const void *w, int dtype, int64_t matrices, int64_t N, int64_t K, void *codes, float *scale,
+                                     void *stream);
+/* y[M, N] = Q(x) * W^T (+ bias[N]); x, bias and y of `dtype`.  With 16-bit types the products run on the fp8 matrix pipes, which keep
+ * 13 bits below the largest of a few neighbouring products; with LOWBIT_DT_F32 they are summed in float32 throughout.  workspace:
+ * lowbit_block_fp8_linear_workspace_bytes bytes (0 for a few rows), contents undefined before and after. */
+size_t lowbit_block_fp8_linear_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K);
+int lowbit_block_fp8_linear(const void *x, const void *w, const float *w_scale, const void *bias, void *y, int dtype, int64_t M, int64_t N,
+                            int64_t K, void *workspace, size_t workspace_bytes, void *stream);
+/* The gradient that flows on to x, as if the quantization of x were the identity: grad_x[M, K] = grad[M, N] * dequant(W)[N, K], grad and
+ * grad_x f16 or bf16.  grad is not quantized: the products are exact, the sums float32, one rounding. */
+size_t lowbit_block_fp8_backward_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K);
+int lowbit_block_fp8_backward(const void *grad, const void *w, const float *w_scale, void *grad_x, int dtype, int64_t M, int64_t N, int64_t K,
+                              void *workspace, size_t workspace_bytes, void *stream);
+/* A mixture-of-experts block: y[t, :] = sum_j topk_weight[t, j] * (Q(act(g) .* u) * down[e]^T), (g | u) = Q(x_t) * gate_up[e]^T, e =
+ * topk_ids[t, j]; a pair whose id lies outside [0, n_experts) counts nothing.  gate_up [n_experts, 2 inter, hidden] (gate rows first)
+ * and down [n_experts, hidden, inter] are the experts' codes one after the other, their scales likewise; inter is a multiple of 128,
+ * hidden of 16.  act(g) .* u is quantized from float32.  Types and limits as in lowbit_experts_forward, pairs at most 2^21. */
+size_t lowbit_block_fp8_experts_workspace_bytes(int64_t tokens, int top_k, int n_experts, int64_t hidden, int64_t inter);
+int lowbit_block_fp8_experts(const void *x, const int64_t *topk_ids, const void *topk_weight, int weight_dtype, int64_t tokens, int top_k,
+                             int n_experts, const void *gate_up, const float *gate_up_scale, const void *down, const float *down_scale,
+                             void *workspace, size_t workspace_bytes, void *y, int act_dtype, int64_t hidden, int64_t inter, int act,
+                             void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -56,6 +56,19 @@ double narrow_time_us(int M, int N, int K, int qtype, bool linear);
 int gemm_splits(int M, int N, int K, size_t ws_bytes, int qtype);
 double gemm_time_us(int M, int N, int K, int splits, int qtype);
 bool gemm_prefers_tall(int qtype, int act_dtype, int M, int N, int K);
+int launch_block_fp8_rows(const void *x, int dtype, int64_t rows, int K, uint8_t *codes, int ldc, float *scale, int64_t row_step,
+                          int64_t block_step, hipStream_t st);
+int launch_block_fp8_weight(const void *w, int dtype, int64_t matrices, int N, int K, uint8_t *codes, float *scale, hipStream_t st);
+size_t block_fp8_linear_workspace_bytes(int dtype, int M, int N, int K);
+int launch_block_fp8_linear(const void *x, const uint8_t *w, const float *ws, const void *bias, void *y, int dtype, int M, int N, int K,
+                            uint8_t *space, hipStream_t st);
+size_t block_fp8_back_workspace_bytes(int dtype, int M, int N, int K);
+int launch_block_fp8_back(const void *grad, const uint8_t *w, const float *ws, void *gx, int dtype, int M, int N, int K, uint8_t *space,
+                          hipStream_t st);
+size_t block_fp8_experts_workspace_bytes(int tokens, int top_k, int n_exp, int H, int I);
+int launch_block_fp8_experts(const void *x, const int64_t *ids, const void *weight, int w_dtype, int tokens, int top_k, int n_exp,
+                             const uint8_t *gate_up, const float *gate_up_scale, const uint8_t *down, const float *down_scale, void *workspace,
+                             void *out, int act_dtype, int H, int I, int act, hipStream_t st);
 int launch_grouped_gemm(const void *x, const void *const *w, const void *const *w_up, void *y, const int32_t *offsets,
                         int n_groups, int total_rows, int qtype, int act_dtype, int N, int K, int act, void *workspace,
                         size_t workspace_bytes, hipStream_t st);
@@ -716,6 +729,116 @@ int lowbit_experts_forward(const void *x, const int64_t *topk_ids, const void *t
         return fail(LOWBIT_ESIZE, "%s: needs %zu bytes of 16-byte aligned workspace", what, need);
     return check_launch(launch_experts(x, topk_ids, topk_weight, weight_dtype, (int)tokens, top_k, n_experts, gates, ups, downs, workspace,
                                        y, qtype, act_dtype, (int)hidden, (int)inter, act, (hipStream_t)stream), what);
+}
+
+// ---- products with a scale for each block of 128
+
+// Sizes that the kernels' 32-bit arithmetic and grids hold: rows of fewer than 2^23 values, fewer than 2^22 rows of x.
+static int check_block_fp8(const char *what, int dtype, bool f32_too, int64_t M, int64_t N, int64_t K) {
+    if (dtype != LOWBIT_DT_F16 && dtype != LOWBIT_DT_BF16 && !(f32_too && dtype == LOWBIT_DT_F32))
+        return fail(LOWBIT_EDTYPE, "%s: unsupported element type", what);
+    if (M < 0 || N < 0 || K < 0) return fail(LOWBIT_EARG, "%s: negative shape", what);
+    if (K % 16) return fail(LOWBIT_ESHAPE, "%s: K=%lld is not a multiple of 16", what, (long long)K);
+    if (M >= (1 << 22) || N >= (1 << 23) || K >= (1 << 23)) return fail(LOWBIT_ESIZE, "%s: needs M < 2^22, N < 2^23 and K < 2^23", what);
+    return 0;
+}
+
+static int check_space(const char *what, const void *workspace, size_t bytes, size_t need) {
+    if (need && (!workspace || !aligned16(workspace) || bytes < need))
+        return fail(LOWBIT_ESIZE, "%s: needs %zu bytes of 16-byte aligned workspace", what, need);
+    return 0;
+}
+
+int lowbit_block_fp8_quantize(const void *x, int dtype, int64_t rows, int64_t K, void *codes, float *scale, void *stream) {
+    const char *what = "lowbit_block_fp8_quantize";
+    if (int rc = check_block_fp8(what, dtype, true, 0, 0, K)) return rc;
+    if (rows < 0) return fail(LOWBIT_EARG, "%s: negative shape", what);
+    if (rows == 0 || K == 0) return 0;
+    if (!x || !codes || !scale || !aligned16(x) || !aligned16(codes) || (((uintptr_t)scale) & 3))
+        return fail(LOWBIT_EARG, "%s: null or misaligned pointer", what);
+    if (rows > (int64_t)1 << 40) return fail(LOWBIT_ESIZE, "%s: too many rows", what);
+    return check_launch(launch_block_fp8_rows(x, dtype, rows, (int)K, (uint8_t *)codes, (int)K, scale, (K + 127) / 128, 1, (hipStream_t)stream), what);
+}
+
+int lowbit_block_fp8_quantize_weight(const void *w, int dtype, int64_t matrices, int64_t N, int64_t K, void *codes, float *scale,
+                                     void *stream) {
+    const char *what = "lowbit_block_fp8_quantize_weight";
+    if (int rc = check_block_fp8(what, dtype, true, 0, N, K)) return rc;
+    if (matrices < 0) return fail(LOWBIT_EARG, "%s: negative shape", what);
+    if (matrices == 0 || N == 0 || K == 0) return 0;
+    if (!w || !codes || !scale || !aligned16(w) || !aligned16(codes) || (((uintptr_t)scale) & 3))
+        return fail(LOWBIT_EARG, "%s: null or misaligned pointer", what);
+    if (matrices > 1 << 24) return fail(LOWBIT_ESIZE, "%s: too many matrices", what);
+    return check_launch(launch_block_fp8_weight(w, dtype, matrices, (int)N, (int)K, (uint8_t *)codes, scale, (hipStream_t)stream), what);
+}
+
+size_t lowbit_block_fp8_linear_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K) {
+    if (M <= 0 || N <= 0 || K <= 0 || M >= (1 << 22) || N >= (1 << 23) || K >= (1 << 23) || K % 16) return 0;
+    return block_fp8_linear_workspace_bytes(dtype, (int)M, (int)N, (int)K);
+}
+
+int lowbit_block_fp8_linear(const void *x, const void *w, const float *w_scale, const void *bias, void *y, int dtype, int64_t M, int64_t N,
+                            int64_t K, void *workspace, size_t workspace_bytes, void *stream) {
+    const char *what = "lowbit_block_fp8_linear";
+    if (int rc = check_block_fp8(what, dtype, true, M, N, K)) return rc;
+    if (M == 0 || N == 0) return 0;
+    if (K == 0) return fail(LOWBIT_ESHAPE, "%s: K must be positive", what);
+    if (!x || !w || !w_scale || !y || !aligned16(x) || !aligned16(w) || !aligned16(y) || (((uintptr_t)w_scale) & 3))
+        return fail(LOWBIT_EARG, "%s: null or misaligned pointer", what);
+    if (int rc = check_space(what, workspace, workspace_bytes, block_fp8_linear_workspace_bytes(dtype, (int)M, (int)N, (int)K))) return rc;
+    return check_launch(launch_block_fp8_linear(x, (const uint8_t *)w, w_scale, bias, y, dtype, (int)M, (int)N, (int)K, (uint8_t *)workspace,
+                                                (hipStream_t)stream), what);
+}
+
+size_t lowbit_block_fp8_backward_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K) {
+    if (M <= 0 || N <= 0 || K <= 0 || M >= (1 << 22) || N >= (1 << 23) || K >= (1 << 23) || K % 16) return 0;
+    return block_fp8_back_workspace_bytes(dtype, (int)M, (int)N, (int)K);
+}
+
+int lowbit_block_fp8_backward(const void *grad, const void *w, const float *w_scale, void *grad_x, int dtype, int64_t M, int64_t N, int64_t K,
+                              void *workspace, size_t workspace_bytes, void *stream) {
+    const char *what = "lowbit_block_fp8_backward";
+    if (int rc = check_block_fp8(what, dtype, false, M, N, K)) return rc;
+    if (M == 0 || K == 0) return 0;
+    if (N == 0) return fail(LOWBIT_ESHAPE, "%s: N must be positive", what);
+    if (!grad || !w || !w_scale || !grad_x || !aligned16(grad) || !aligned16(w) || !aligned16(grad_x) || (((uintptr_t)w_scale) & 3))
+        return fail(LOWBIT_EARG, "%s: null or misaligned pointer", what);
+    if (int rc = check_space(what, workspace, workspace_bytes, block_fp8_back_workspace_bytes(dtype, (int)M, (int)N, (int)K))) return rc;
+    return check_launch(launch_block_fp8_back(grad, (const uint8_t *)w, w_scale, grad_x, dtype, (int)M, (int)N, (int)K, (uint8_t *)workspace,
+                                              (hipStream_t)stream), what);
+}
+
+static bool block_fp8_experts_ok(int64_t tokens, int64_t top_k, int64_t n_experts, int64_t hidden, int64_t inter) {
+    return experts_sizes_ok(tokens, top_k, n_experts, hidden, inter) && tokens * top_k <= 1 << 21 && inter < 1 << 22;
+}
+
+size_t lowbit_block_fp8_experts_workspace_bytes(int64_t tokens, int top_k, int n_experts, int64_t hidden, int64_t inter) {
+    if (!block_fp8_experts_ok(tokens, top_k, n_experts, hidden, inter) || hidden % 16 || inter % 128) return 0;
+    return block_fp8_experts_workspace_bytes((int)tokens, top_k, n_experts, (int)hidden, (int)inter);
+}
+
+int lowbit_block_fp8_experts(const void *x, const int64_t *topk_ids, const void *topk_weight, int weight_dtype, int64_t tokens, int top_k,
+                             int n_experts, const void *gate_up, const float *gate_up_scale, const void *down, const float *down_scale,
+                             void *workspace, size_t workspace_bytes, void *y, int act_dtype, int64_t hidden, int64_t inter, int act,
+                             void *stream) {
+    const char *what = "lowbit_block_fp8_experts";
+    if (act_dtype != LOWBIT_DT_F16 && act_dtype != LOWBIT_DT_BF16) return fail(LOWBIT_EDTYPE, "%s: activations must be f16 or bf16", what);
+    if (weight_dtype != LOWBIT_DT_F16 && weight_dtype != LOWBIT_DT_BF16 && weight_dtype != LOWBIT_DT_F32)
+        return fail(LOWBIT_EDTYPE, "%s: routing weights must be f16, bf16 or f32", what);
+    if (act != LOWBIT_ACT_SILU && act != LOWBIT_ACT_GELU)
+        return fail(LOWBIT_EARG, "%s: activation must be LOWBIT_ACT_SILU or LOWBIT_ACT_GELU", what);
+    if (tokens == 0) return 0;
+    if (!block_fp8_experts_ok(tokens, top_k, n_experts, hidden, inter))
+        return fail(LOWBIT_ESIZE, "%s: top_k must be 1 .. 64, experts 1 .. 4096, pairs at most 2^21", what);
+    if (hidden % 16 || inter % 128) return fail(LOWBIT_ESHAPE, "%s: hidden must be a multiple of 16, inter of 128", what);
+    if (!x || !topk_ids || !topk_weight || !gate_up || !gate_up_scale || !down || !down_scale || !y || !aligned16(x) || !aligned16(y) ||
+        !aligned16(gate_up) || !aligned16(down) || (((uintptr_t)topk_ids) & 7) || (((uintptr_t)gate_up_scale | (uintptr_t)down_scale) & 3))
+        return fail(LOWBIT_EARG, "%s: null or misaligned pointer", what);
+    if (int rc = check_space(what, workspace, workspace_bytes, lowbit_block_fp8_experts_workspace_bytes(tokens, top_k, n_experts, hidden, inter)))
+        return rc;
+    return check_launch(launch_block_fp8_experts(x, topk_ids, topk_weight, weight_dtype, (int)tokens, top_k, n_experts, (const uint8_t *)gate_up,
+                                                 gate_up_scale, (const uint8_t *)down, down_scale, workspace, y, act_dtype, (int)hidden,
+                                                 (int)inter, act, (hipStream_t)stream), what);
 }
 
 static int grouped_any(const char *who, const void *x, const void *const *w, const void *const *w_up, void *y,

@@ -213,6 +213,18 @@ static void launch_combine(const void *y, const int32_t *pos, const void *weight
         hipLaunchKernelGGL((moe_combine_kernel<AT, __bf16>), grid, dim3(256), 0, st, (const AT *)y, pos, (const __bf16 *)weight, (AT *)out, top_k, N);
 }
 
+void launch_moe_combine(const void *y, const int32_t *pos, const void *weight, int w_dtype, void *out, int act_dtype, int tokens, int top_k,
+                        int N, hipStream_t st) {
+    if (act_dtype == DT_F16) launch_combine<_Float16>(y, pos, weight, w_dtype, out, tokens, top_k, N, st);
+    else launch_combine<__bf16>(y, pos, weight, w_dtype, out, tokens, top_k, N, st);
+}
+
+void launch_moe_route(const int64_t *ids, int pairs, int n_exp, int32_t *offsets, int32_t *order, int32_t *pos, hipStream_t st) {
+    const int waves = n_exp <= 512 ? 16 : 2;              // at most 48 KiB of counters
+    hipLaunchKernelGGL(moe_route_kernel, dim3(1), dim3(64 * waves), (size_t)n_exp * (waves + 1) * sizeof(int32_t), st, ids, pairs, n_exp,
+                       offsets, order, pos);
+}
+
 // Whether the pairs go through the streaming kernel, which reads an expert's weights once per pair: while there are no
 // more pairs than experts, so that few experts are read twice.  Measured (streaming / grouped, us): 60 experts of
 // [1408 x 2048] sym_int4 at 8 / 32 / 64 pairs 17 / 41, 40 / 71, 74 / 78; 8 experts of [14336 x 4096] fp8_e4m3 at 4 / 8 /
@@ -264,13 +276,11 @@ int launch_experts(const void *x, const int64_t *ids, const void *weight, int w_
                                act_dtype, hidden, inter, act, st);
     int32_t *const offsets = (int32_t *)(ws + at.offsets), *const order = (int32_t *)(ws + at.order), *const pos = (int32_t *)(ws + at.pos);
     void *const xs = ws + at.xs, *const y = ws + at.y;
-    const int waves = n_exp <= 512 ? 16 : 2;          // at most 48 KiB of counters
     if (pairs <= MOE_SORT_PAIRS && n_exp <= 512) {
         hipLaunchKernelGGL(moe_sort_gather_kernel, dim3(pairs + n_exp + 1), dim3(256), 0, st, ids, (const u32x4 *)x, pairs, n_exp, offsets,
                            pos, (u32x4 *)xs, top_k, hidden / 8);
     } else {
-        hipLaunchKernelGGL(moe_route_kernel, dim3(1), dim3(64 * waves), (size_t)n_exp * (waves + 1) * sizeof(int32_t), st, ids, pairs, n_exp,
-                           offsets, order, pos);
+        launch_moe_route(ids, pairs, n_exp, offsets, order, pos, st);
         hipLaunchKernelGGL(moe_gather_kernel, dim3(pairs), dim3(256), 0, st, (const u32x4 *)x, order, offsets + n_exp, (u32x4 *)xs, top_k,
                            hidden / 8);
     }
@@ -278,8 +288,7 @@ int launch_experts(const void *x, const int64_t *ids, const void *weight, int w_
         return rc;
     if (int rc = launch_grouped_gemm(h, downs, nullptr, y, offsets, n_exp, pairs, qtype, act_dtype, hidden, inter, 0, ws + at.split,
                                      at.bytes - at.split, st)) return rc;
-    if (act_dtype == DT_F16) launch_combine<_Float16>(y, pos, weight, w_dtype, out, tokens, top_k, hidden, st);
-    else launch_combine<__bf16>(y, pos, weight, w_dtype, out, tokens, top_k, hidden, st);
+    launch_moe_combine(y, pos, weight, w_dtype, out, act_dtype, tokens, top_k, hidden, st);
     return 0;
 }
 

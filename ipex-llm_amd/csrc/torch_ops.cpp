@@ -44,6 +44,14 @@ struct Api {
     decltype(&lowbit_backward_ws_applies) backward_ws_applies = nullptr;
     decltype(&lowbit_experts_workspace_bytes) experts_workspace_bytes = nullptr;
     decltype(&lowbit_experts_forward) experts_forward = nullptr;
+    decltype(&lowbit_block_fp8_quantize) block_fp8_quantize = nullptr;
+    decltype(&lowbit_block_fp8_quantize_weight) block_fp8_quantize_weight = nullptr;
+    decltype(&lowbit_block_fp8_linear) block_fp8_linear = nullptr;
+    decltype(&lowbit_block_fp8_linear_workspace_bytes) block_fp8_linear_workspace_bytes = nullptr;
+    decltype(&lowbit_block_fp8_backward) block_fp8_backward = nullptr;
+    decltype(&lowbit_block_fp8_backward_workspace_bytes) block_fp8_backward_workspace_bytes = nullptr;
+    decltype(&lowbit_block_fp8_experts) block_fp8_experts = nullptr;
+    decltype(&lowbit_block_fp8_experts_workspace_bytes) block_fp8_experts_workspace_bytes = nullptr;
 } api;
 
 constexpr size_t WORKSPACE_CAP = (size_t)256 << 20;      // most that a product borrows for split-K partial sums
@@ -275,6 +283,142 @@ Tensor experts(const Tensor &x_in, const Tensor &ids_in, const Tensor &weight_in
     return y;
 }
 
+// ---- e4m3 operands with a scale for each block of 128
+
+int64_t blocks(int64_t n) { return (n + 127) / 128; }
+
+// rows as the kernels read them: contiguous, from a 16-byte boundary on
+Tensor whole_rows(const Tensor &t) {
+    Tensor c = t.contiguous();
+    return ((uintptr_t)c.const_data_ptr() & 15) ? c.clone() : c;
+}
+
+// w holds e4m3 codes [.., N, K] and scale their scales, one per block of 128 x 128, on x's device
+bool is_block_fp8(const Tensor &w, const Tensor &scale, const Tensor &x, int64_t matrices) {
+    if (w.device() != x.device() || scale.device() != x.device() || w.layout() != at::kStrided || scale.layout() != at::kStrided ||
+        w.scalar_type() != at::kFloat8_e4m3fn || scale.scalar_type() != at::kFloat || w.dim() < 2 || w.dim() != scale.dim() ||
+        !w.is_contiguous() || !scale.is_contiguous() || ((uintptr_t)w.const_data_ptr() & 15)) return false;
+    const int64_t d = w.dim();
+    if (scale.size(d - 2) != blocks(w.size(d - 2)) || scale.size(d - 1) != blocks(w.size(d - 1)) || w.size(d - 1) % 16 || w.numel() == 0) return false;
+    if (d == 3 && (w.size(0) != matrices || scale.size(0) != matrices)) return false;
+    return d == (matrices ? 3 : 2) && !differentiable(w) && !differentiable(scale);
+}
+
+// codes and scales of x by row (weight false) or by 128 x 128; undefined tensors when this is not the plain case
+std::pair<Tensor, Tensor> block_fp8_quantize(const Tensor &x_in, bool weight) {
+    if (!on_gpu(x_in) || x_in.dim() < (weight ? 2 : 1) || x_in.numel() == 0 || x_in.size(-1) % 16 || dtype_code(x_in.scalar_type()) < 0) return {};
+    const Tensor x = whole_rows(x_in.detach());
+    const int64_t K = x.size(-1), N = weight ? x.size(-2) : 1;
+    c10::DeviceGuard guard(x.device());
+    at::DimVector shape(x.sizes().begin(), x.sizes().end());
+    shape.back() = blocks(K);
+    if (weight) shape[shape.size() - 2] = blocks(N);
+    const Tensor codes = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn)), scale = at::empty(shape, x.options().dtype(at::kFloat));
+    const int dt = dtype_code(x.scalar_type());
+    if (weight)
+        check(api.block_fp8_quantize_weight(x.const_data_ptr(), dt, x.numel() / (N * K), N, K, codes.data_ptr(), scale.data_ptr<float>(),
+                                            current_stream(x)), "lowbit_block_fp8_quantize_weight");
+    else
+        check(api.block_fp8_quantize(x.const_data_ptr(), dt, x.numel() / K, K, codes.data_ptr(), scale.data_ptr<float>(), current_stream(x)),
+              "lowbit_block_fp8_quantize");
+    return {codes, scale};
+}
+
+Tensor block_fp8_product(const Tensor &x, const Tensor &w, const Tensor &scale, const Tensor &bias) {
+    c10::DeviceGuard guard(x.device());
+    const int64_t N = w.size(0), K = w.size(1), M = x.numel() / K;
+    const int dt = dtype_code(x.scalar_type());
+    Tensor y = at::empty(with_last(x, N), x.options());
+    const size_t bytes = api.block_fp8_linear_workspace_bytes(dt, M, N, K);
+    const Tensor ws = bytes ? at::empty({(int64_t)bytes}, x.options().dtype(at::kByte)) : Tensor();
+    check(api.block_fp8_linear(x.const_data_ptr(), w.const_data_ptr(), scale.const_data_ptr<float>(), bias.defined() ? bias.const_data_ptr() : nullptr,
+                               y.data_ptr(), dt, M, N, K, bytes ? ws.data_ptr() : nullptr, bytes, current_stream(x)), "lowbit_block_fp8_linear");
+    return y;
+}
+
+// the weight in `dtype`, for what the kernels do not take
+Tensor block_fp8_dense(const Tensor &w, const Tensor &scale, at::ScalarType dtype) {
+    const Tensor rows = scale.repeat_interleave(128, 0).narrow(0, 0, w.size(0));
+    return w.to(at::kFloat).mul_(rows.repeat_interleave(128, 1).narrow(1, 0, w.size(1))).to(dtype);
+}
+
+// The gradient that flows on to x, the quantization of x counting as the identity.  Holds the weight as ProductBackward does.
+struct BlockFp8Backward : public torch::autograd::Node {
+    Tensor w, scale;
+    at::ScalarType dtype = at::kHalf;
+    at::DimVector x_shape;
+
+    std::string name() const override { return "BlockFp8LinearBackward"; }
+
+    torch::autograd::variable_list apply(torch::autograd::variable_list &&grads) override {
+        if (!task_should_compute_output(0)) return {Tensor()};
+        const int64_t N = w.size(0), K = w.size(1);
+        const Tensor grad = grads[0].defined() ? grads[0].to(dtype).reshape({-1, N})
+                                               : at::zeros({c10::multiply_integers(x_shape) / K, N}, w.options().dtype(dtype));
+        c10::DeviceGuard guard(grad.device());
+        if (grad.device() != w.device()) throw Failed("the block-scaled weight is not where the forward found it");
+        if (dtype == at::kFloat || differentiable(grad) || !nothing_watches(grad))     // (float32, a second derivative, a transform: the dense product)
+            return {at::matmul(grad, block_fp8_dense(w, scale, dtype)).view(x_shape)};
+        const Tensor g = whole_rows(grad);
+        const int64_t M = g.size(0);
+        const int dt = dtype_code(dtype);
+        Tensor gx = at::empty(x_shape, g.options());
+        const size_t bytes = api.block_fp8_backward_workspace_bytes(dt, M, N, K);
+        const Tensor ws = bytes ? at::empty({(int64_t)bytes}, g.options().dtype(at::kByte)) : Tensor();
+        check(api.block_fp8_backward(g.const_data_ptr(), w.const_data_ptr(), scale.const_data_ptr<float>(), gx.data_ptr(), dt, M, N, K,
+                                     bytes ? ws.data_ptr() : nullptr, bytes, current_stream(g)), "lowbit_block_fp8_backward");
+        return {gx};
+    }
+};
+
+// y = Q(x) W^T (+ bias), with the gradient to x where x wants one; an undefined tensor when this is not the plain case
+Tensor block_fp8_linear(const Tensor &x_in, const Tensor &w, const Tensor &scale, const Tensor &bias) {
+    if (!on_gpu(x_in) || x_in.dim() < 1 || x_in.numel() == 0 || dtype_code(x_in.scalar_type()) < 0 || !is_block_fp8(w, scale, x_in, 0) ||
+        w.size(1) != x_in.size(-1) || !nothing_watches(x_in) || x_in._fw_grad(/*level=*/0).defined()) return {};
+    if (bias.defined() && (bias.scalar_type() != x_in.scalar_type() || bias.device() != x_in.device() || bias.dim() != 1 ||
+                           bias.numel() != w.size(0) || !bias.is_contiguous() || differentiable(bias))) return {};
+    if (!x_in.requires_grad() || !c10::GradMode::is_enabled()) return block_fp8_product(whole_rows(x_in), w, scale, bias);
+    Tensor y;
+    auto node = std::shared_ptr<BlockFp8Backward>(new BlockFp8Backward(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(x_in));
+    node->w = w;
+    node->scale = scale;
+    node->dtype = x_in.scalar_type();
+    node->x_shape.assign(x_in.sizes().begin(), x_in.sizes().end());
+    {
+        c10::AutoGradMode no_grad(false);
+        y = block_fp8_product(whole_rows(x_in.detach()), w, scale, bias);
+    }
+    torch::autograd::set_history(y, node);
+    return y;
+}
+
+// the experts of a mixture-of-experts block; an undefined tensor when this is not the plain case
+Tensor block_fp8_experts(const Tensor &x_in, const Tensor &ids_in, const Tensor &weight_in, const Tensor &gate_up, const Tensor &gate_up_scale,
+                         const Tensor &down, const Tensor &down_scale, int act) {
+    if (!on_gpu(x_in) || x_in.dim() != 2 || gate_up.dim() != 3 || ids_in.dim() != 2 || ids_in.size(0) != x_in.size(0) || ids_in.numel() == 0 ||
+        !at::isIntegralType(ids_in.scalar_type(), /*includeBool=*/false) || weight_in.sizes() != ids_in.sizes() ||
+        ids_in.device() != x_in.device() || weight_in.device() != x_in.device() || differentiable(weight_in) || differentiable(x_in) ||
+        !nothing_watches(x_in)) return {};
+    const int64_t n_exp = gate_up.size(0), hidden = x_in.size(1), inter = gate_up.size(1) / 2;
+    if (!is_block_fp8(gate_up, gate_up_scale, x_in, n_exp) || !is_block_fp8(down, down_scale, x_in, n_exp) || gate_up.size(1) != 2 * inter ||
+        gate_up.size(2) != hidden || down.size(1) != hidden || down.size(2) != inter) return {};
+    const int dt = dtype_code(x_in.scalar_type()), wdt = dtype_code(weight_in.scalar_type());
+    if ((dt != LOWBIT_DT_F16 && dt != LOWBIT_DT_BF16) || wdt < 0) return {};
+    const int64_t tokens = ids_in.size(0), top_k = ids_in.size(1);
+    const size_t bytes = top_k > 64 || n_exp > 4096 ? 0 : api.block_fp8_experts_workspace_bytes(tokens, (int)top_k, (int)n_exp, hidden, inter);
+    if (!bytes) return {};                               // more than the library takes
+    const Tensor x = whole_rows(x_in), ids = ids_in.to(at::kLong).contiguous(), weight = weight_in.contiguous();
+    c10::DeviceGuard guard(x.device());
+    const Tensor ws = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
+    Tensor y = at::empty({tokens, hidden}, x.options());
+    check(api.block_fp8_experts(x.const_data_ptr(), ids.const_data_ptr<int64_t>(), weight.const_data_ptr(), wdt, tokens, (int)top_k, (int)n_exp,
+                                gate_up.const_data_ptr(), gate_up_scale.const_data_ptr<float>(), down.const_data_ptr(),
+                                down_scale.const_data_ptr<float>(), ws.data_ptr(), bytes, y.data_ptr(), dt, hidden, inter, act,
+                                current_stream(x)), "lowbit_block_fp8_experts");
+    return y;
+}
+
 // ---- large copies between pageable host memory and the GPU, through two pinned buffers
 //
 // A pageable copy by the runtime ran at 29 GB/s up and, into memory the process has not touched yet, 7.5 GB/s down
@@ -384,6 +528,27 @@ template <typename Fn> PyObject *answer(const char *name, Py_ssize_t got, Py_ssi
     END_HANDLE_TH_ERRORS
 }
 
+// The same for fn returning two tensors: a tuple, or None where they are undefined.
+template <typename Fn> PyObject *answer_pair(const char *name, Py_ssize_t got, Py_ssize_t want, Fn &&fn) {
+    std::pair<Tensor, Tensor> both;
+    PyObject *first = answer(name, got, want, [&] {
+        both = fn();
+        return both.first;
+    });
+    if (!first || first == Py_None) return first;
+    HANDLE_TH_ERRORS
+    PyObject *second = THPVariable_Wrap(std::move(both.second));
+    if (!second) {
+        Py_DECREF(first);
+        return nullptr;
+    }
+    PyObject *tuple = PyTuple_Pack(2, first, second);
+    Py_DECREF(first);
+    Py_DECREF(second);
+    return tuple;
+    END_HANDLE_TH_ERRORS
+}
+
 struct NoGil {
     PyThreadState *state = PyEval_SaveThread();
     ~NoGil() { PyEval_RestoreThread(state); }
@@ -406,6 +571,8 @@ PyObject *py_bind(PyObject *, PyObject *const *args, Py_ssize_t n) {
     } while (0)
     BIND(last_error); BIND(blob_bytes); BIND(tileable); BIND(linear_scratch_bytes); BIND(linear);
     BIND(gated_mlp); BIND(dequantize_rows); BIND(dequantize); BIND(backward_ws); BIND(backward_workspace_bytes); BIND(backward_ws_applies); BIND(experts_workspace_bytes); BIND(experts_forward);
+    BIND(block_fp8_quantize); BIND(block_fp8_quantize_weight); BIND(block_fp8_linear); BIND(block_fp8_linear_workspace_bytes);
+    BIND(block_fp8_backward); BIND(block_fp8_backward_workspace_bytes); BIND(block_fp8_experts); BIND(block_fp8_experts_workspace_bytes);
 #undef BIND
     Py_RETURN_NONE;
 }
@@ -486,6 +653,40 @@ PyObject *py_experts(PyObject *, PyObject *const *args, Py_ssize_t n) {
     });
 }
 
+// block_fp8_quantize(x, weight) -> (codes, scale) or None
+PyObject *py_block_fp8_quantize(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return answer_pair("block_fp8_quantize", n, 2, [&] {
+        const Args a{args, n};
+        const Tensor &x = a.tensor(0);
+        const bool weight = a.truth(1);
+        NoGil free;
+        return block_fp8_quantize(x, weight);
+    });
+}
+
+// block_fp8_linear(x, weight, scale, bias or None) -> y or None
+PyObject *py_block_fp8_linear(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return answer("block_fp8_linear", n, 4, [&] {
+        const Args a{args, n};
+        const Tensor &x = a.tensor(0), &w = a.tensor(1), &scale = a.tensor(2);
+        const Tensor bias = a.optional(3);
+        NoGil free;
+        return block_fp8_linear(x, w, scale, bias);
+    });
+}
+
+// block_fp8_experts(x, ids, weights, gate_up, gate_up_scale, down, down_scale, act) -> y or None
+PyObject *py_block_fp8_experts(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return answer("block_fp8_experts", n, 8, [&] {
+        const Args a{args, n};
+        const Tensor &x = a.tensor(0), &ids = a.tensor(1), &weight = a.tensor(2);
+        const Tensor &gu = a.tensor(3), &gus = a.tensor(4), &d = a.tensor(5), &ds = a.tensor(6);
+        const int act = (int)a.integer(7);
+        NoGil free;
+        return block_fp8_experts(x, ids, weight, gu, gus, d, ds, act);
+    });
+}
+
 // upload(host tensor, device index) -> the tensor on that GPU, or None; complete when it returns
 PyObject *py_upload(PyObject *, PyObject *const *args, Py_ssize_t n) {
     return answer("upload", n, 2, [&] {
@@ -528,7 +729,8 @@ PyObject *py_holds(PyObject *, PyObject *const *args, Py_ssize_t n) {
 }
 
 #define METHOD(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {METHOD(bind), METHOD(product), METHOD(linear), METHOD(linear_train), METHOD(gated), METHOD(embedding), METHOD(experts), METHOD(upload),
+PyMethodDef methods[] = {METHOD(bind), METHOD(product), METHOD(linear), METHOD(linear_train), METHOD(gated), METHOD(embedding), METHOD(experts), METHOD(block_fp8_quantize),
+                         METHOD(block_fp8_linear), METHOD(block_fp8_experts), METHOD(upload),
                          METHOD(download), METHOD(holds),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "lowbit_torch", "native host path of the low-bit layers", -1, methods};

@@ -431,6 +431,47 @@ _lib.lowbit_experts_forward.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_i
 _lib.lowbit_experts_forward.restype = c_int
 
 
+_lib.lowbit_block_fp8_quantize.argtypes = [c_void_p, c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p]
+_lib.lowbit_block_fp8_quantize_weight.argtypes = [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p]
+_lib.lowbit_block_fp8_linear.argtypes = [c_void_p] * 5 + [c_int, c_int64, c_int64, c_int64, c_void_p, c_size_t, c_void_p]
+_lib.lowbit_block_fp8_backward.argtypes = [c_void_p] * 4 + [c_int, c_int64, c_int64, c_int64, c_void_p, c_size_t, c_void_p]
+_lib.lowbit_block_fp8_experts.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p,
+                                          c_void_p, c_void_p, c_size_t, c_void_p, c_int, c_int64, c_int64, c_int, c_void_p]
+for _name in ("quantize", "quantize_weight", "linear", "backward", "experts"):
+    getattr(_lib, f"lowbit_block_fp8_{_name}").restype = c_int
+_lib.lowbit_block_fp8_linear_workspace_bytes.argtypes = [c_int, c_int64, c_int64, c_int64]
+_lib.lowbit_block_fp8_backward_workspace_bytes.argtypes = [c_int, c_int64, c_int64, c_int64]
+_lib.lowbit_block_fp8_experts_workspace_bytes.argtypes = [c_int64, c_int, c_int, c_int64, c_int64]
+for _name in ("linear", "backward", "experts"):
+    getattr(_lib, f"lowbit_block_fp8_{_name}_workspace_bytes").restype = c_size_t
+
+
+def lowbit_block_fp8_quantize(x, dtype, rows, k, codes, scale, stream):
+    _check(_lib.lowbit_block_fp8_quantize(x, dtype, rows, k, codes, scale, stream), "lowbit_block_fp8_quantize")
+
+
+def lowbit_block_fp8_quantize_weight(w, dtype, matrices, n, k, codes, scale, stream):
+    _check(_lib.lowbit_block_fp8_quantize_weight(w, dtype, matrices, n, k, codes, scale, stream), "lowbit_block_fp8_quantize_weight")
+
+
+def lowbit_block_fp8_linear(x, w, w_scale, bias, y, dtype, m, n, k, workspace, workspace_bytes, stream):
+    _check(_lib.lowbit_block_fp8_linear(x, w, w_scale, bias, y, dtype, m, n, k, workspace, workspace_bytes, stream),
+           "lowbit_block_fp8_linear")
+
+
+def lowbit_block_fp8_linear_workspace_bytes(dtype, m, n, k) -> int:
+    return _lib.lowbit_block_fp8_linear_workspace_bytes(dtype, m, n, k)
+
+
+def lowbit_block_fp8_backward(grad, w, w_scale, grad_x, dtype, m, n, k, workspace, workspace_bytes, stream):
+    _check(_lib.lowbit_block_fp8_backward(grad, w, w_scale, grad_x, dtype, m, n, k, workspace, workspace_bytes, stream),
+           "lowbit_block_fp8_backward")
+
+
+def lowbit_block_fp8_backward_workspace_bytes(dtype, m, n, k) -> int:
+    return _lib.lowbit_block_fp8_backward_workspace_bytes(dtype, m, n, k)
+
+
 def lowbit_dequantize_rows(w, rows, n_rows, dst, qtype, n, k, layout, out_dtype, stream):
     _check(_lib.lowbit_dequantize_rows(w, rows, n_rows, dst, qtype, n, k, layout, out_dtype, stream),
            "lowbit_dequantize_rows")

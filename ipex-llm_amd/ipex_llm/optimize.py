@@ -85,7 +85,14 @@ def unconverted_linears(state_dict):
     """Module names whose saved weight is still a dense matrix: they were excluded from the
     conversion when the model was saved and must be excluded again when it is rebuilt."""
     return [k[:-len(".weight")] for k, v in state_dict.items()
-            if k.endswith(".weight") and v.dim() == 2 and v.numel() > 0 and v.dtype != torch.uint8]
+            if k.endswith(".weight") and v.dim() == 2 and v.numel() > 0 and v.dtype not in (torch.uint8, torch.float8_e4m3fn)]
+
+
+def block_fp8_layers(state_dict):
+    """Module names whose saved weights have a scale for each 128 x 128 block, and whether q_proj / k_proj / v_proj were kept apart
+    when they were converted."""
+    names = {k[:-len(end)] for end in (".weight_scale_inv", ".gate_up_proj_scale_inv") for k in state_dict if k.endswith(end)}
+    return names, any(n.endswith("q_proj") for n in names)
 
 
 def load_low_bit(model, model_path):
@@ -98,8 +105,10 @@ def load_low_bit(model, model_path):
     if low_bit:
         from ipex_llm.transformers.convert import ggml_convert_low_bit
         qtype = ggml_tensor_qtype[low_bit]
+        block_fp8, apart = block_fp8_layers(state_dict)
         model = ggml_convert_low_bit(model, qtype=qtype, convert_shape_only=True,
-                                     modules_to_not_convert=unconverted_linears(state_dict))
+                                     modules_to_not_convert=unconverted_linears(state_dict),
+                                     disable_optimize_pre=apart, block_fp8=block_fp8)
     for param_name, param in state_dict.items():
         _assign(model, param_name, param)
     if low_bit:
@@ -111,7 +120,8 @@ def load_low_bit(model, model_path):
 def optimize_model(model, low_bit='sym_int4', optimize_llm=True, modules_to_not_convert=None,
                    cpu_embedding=False, **kwargs):
     """Replaces every nn.Linear of a PyTorch model by its low-bit counterpart
-    (reference: optimize.py:199-267; same arguments)."""
+    (reference: optimize.py:199-267; same arguments).  `block_fp8=True` with low_bit="fp8_e4m3": weights with a scale for each
+    128 x 128 block and activations quantized in the call (transformers/block_fp8.py)."""
     invalidInputError(low_bit is None or low_bit in ggml_tensor_qtype,
                       f"Unknown load_in_low_bit value: {low_bit}, expected:"
                       f" sym_int4, asym_int4, sym_int5, asym_int5 or sym_int8.")
@@ -136,7 +146,8 @@ def optimize_model(model, low_bit='sym_int4', optimize_llm=True, modules_to_not_
                                  optimize_model=optimize_llm,
                                  modules_to_not_convert=modules_to_not_convert,
                                  cpu_embedding=cpu_embedding,
-                                 disable_optimize_pre=kwargs.pop("disable_optimize_pre", False))
+                                 disable_optimize_pre=kwargs.pop("disable_optimize_pre", False),
+                                 block_fp8=kwargs.pop("block_fp8", False))
     model._bigdl_config = dict()
     model._bigdl_config["bigdl_transformers_low_bit"] = low_bit
     model.save_low_bit = types.MethodType(_save_low_bit, model)

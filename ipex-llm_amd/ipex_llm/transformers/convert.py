@@ -40,6 +40,13 @@ def is_gptq_linear(module) -> bool:
             and getattr(module, "bits", getattr(module, "w_bit", None)) == 4)
 
 
+def is_block_fp8(module, name="weight") -> bool:
+    """A layer (or, with the name of its 3-D parameter, an experts module) of a block-scaled fp8 checkpoint: e4m3 codes and a tensor
+    of scales beside them.  Recognised by its tensors, like a GPTQ layer."""
+    w = getattr(module, name, None)
+    return isinstance(w, torch.Tensor) and w.dtype == torch.float8_e4m3fn and isinstance(getattr(module, name + "_scale_inv", None), torch.Tensor)
+
+
 def is_linear_module(module):
     """(is_linear, (in_features, out_features, mp_group)): nn.Linear and 4-bit GPTQ / AWQ layers; the
     vLLM / DeepSpeed layer classes of the reference (convert.py:138-232) are not handled."""
@@ -137,17 +144,26 @@ def _replace_with_low_bit_linear(model, qtype, modules_to_not_convert=None,
                                  mixed_precision=False,
                                  act_order=False,
                                  enable_scale_search=False,
+                                 block_fp8=False,
                                  ):
+    """block_fp8: which layers (True: all; or a set of their full names) get e4m3 weights with a scale for each 128 x 128 and
+    activations quantized in the call (block_fp8.py) in place of qtype's format."""
+    from ipex_llm.transformers.block_fp8 import BlockFP8Experts, BlockFP8Linear
     from ipex_llm.transformers.low_bit_linear import BF16Linear, FP16Linear, FP4Params, LowBitLinear
     modules_to_not_convert = modules_to_not_convert or []
     has_been_replaced = False
+    only_fp8 = "layers with a scale for each 128 x 128 block hold e4m3: convert with load_in_low_bit='fp8_e4m3'"
 
     for name, module in model.named_children():
         is_linear, linear_args = is_linear_module(module)
         full_module_name = prefix_name + '.' + name if prefix_name != '' else name
+        wants_blocks = block_fp8 is True or (block_fp8 and full_module_name in block_fp8)
 
         # sub-string match, as in the reference: "0" also matches "10"
         if any(key in full_module_name for key in modules_to_not_convert):
+            continue
+
+        if isinstance(module, (BlockFP8Linear, BlockFP8Experts)):
             continue
 
         if is_linear and not isinstance(module, (LowBitLinear, FP16Linear, BF16Linear)):
@@ -155,7 +171,13 @@ def _replace_with_low_bit_linear(model, qtype, modules_to_not_convert=None,
             optimize_lm_head = (is_lm_head(name, model_config, out_features)
                                 and os.environ.get("IPEX_LLM_LAST_LM_HEAD", None) != "0")
             new_linear = None
-            if is_gptq_linear(module):
+            if is_block_fp8(module) or (wants_blocks and not is_gptq_linear(module)):
+                invalidInputError(qtype == ggml_tensor_qtype["fp8_e4m3"], only_fp8)
+                if in_features % 16 != 0:
+                    invalidInputError(not is_block_fp8(module), f"{full_module_name}: in_features must be a multiple of 16")
+                    continue
+                new_linear = BlockFP8Linear.from_linear(module, convert_shape_only, mp_group, optimize_lm_head)
+            elif is_gptq_linear(module):
                 # convert.py:511-545 of the reference: the codes are kept, only the packing changes
                 invalidInputError(qtype == ggml_tensor_qtype["asym_int4"],
                                   "GPTQ / AWQ layers convert to asym_int4 only")
@@ -232,6 +254,14 @@ def _replace_with_low_bit_linear(model, qtype, modules_to_not_convert=None,
             from ipex_llm.transformers.low_bit_linear import get_qk_size
             from ipex_llm.transformers.moe import LowBitExperts
             _, two_i, hidden = module.gate_up_proj.shape
+            scaled = is_block_fp8(module, "gate_up_proj") and is_block_fp8(module, "down_proj")
+            if scaled or (wants_blocks and hidden % 16 == 0 and two_i % 256 == 0):
+                invalidInputError(qtype == ggml_tensor_qtype["fp8_e4m3"], only_fp8)
+                model._modules[name] = BlockFP8Experts.from_fused(module, convert_shape_only).requires_grad_(False)
+                has_been_replaced = True
+                continue
+            if wants_blocks:
+                continue                                 # sizes that do not divide into blocks stay dense
             qk = get_qk_size(qtype)
             if hidden % 64 == 0 and (two_i // 2) % 64 == 0 and (not qk or (hidden % qk == 0 and (two_i // 2) % qk == 0)):
                 model._modules[name] = LowBitExperts.from_fused(module, qtype, convert_shape_only=convert_shape_only,
@@ -252,7 +282,7 @@ def _replace_with_low_bit_linear(model, qtype, modules_to_not_convert=None,
                 prefix_name=full_module_name, imatrix_data=imatrix_data,
                 embedding_qtype=embedding_qtype, model_config=model_config, torch_dtype=torch_dtype,
                 mixed_precision=mixed_precision, act_order=act_order,
-                enable_scale_search=enable_scale_search)
+                enable_scale_search=enable_scale_search, block_fp8=block_fp8)
             has_been_replaced = _flag or has_been_replaced
     return model, has_been_replaced
 
@@ -325,7 +355,10 @@ def ggml_convert_low_bit(model, qtype, optimize_model=True,
                          imatrix_data=None,
                          embedding_qtype=None,
                          mixed_precision=False,
-                         disable_optimize_pre=False):
+                         disable_optimize_pre=False,
+                         block_fp8=False):
+    invalidInputError(not block_fp8 or qtype == ggml_tensor_qtype["fp8_e4m3"],
+                      "block_fp8 makes e4m3 weights: use it with fp8_e4m3")
     if qtype in ggml_tensor_qtype.values():
         index = list(ggml_tensor_qtype.values()).index(qtype)
         logger.info(f"Converting the current model to {list(ggml_tensor_qtype.keys())[index]} format......")
@@ -344,7 +377,7 @@ def ggml_convert_low_bit(model, qtype, optimize_model=True,
             model, qtype, modules_to_not_convert, convert_shape_only, cpu_embedding,
             imatrix_data=imatrix_data, embedding_qtype=embedding_qtype, model_config=model_config,
             torch_dtype=torch_dtype, mixed_precision=mixed_precision, act_order=False,
-            enable_scale_search=enable_scale_search)
+            enable_scale_search=enable_scale_search, block_fp8=block_fp8)
         if not has_been_replaced:
             warnings.warn("No linear modules were found in your model. This can happen for some "
                           "architectures such as gpt2 that uses Conv1D instead of Linear layers.")
@@ -358,10 +391,11 @@ def ggml_convert_low_bit(model, qtype, optimize_model=True,
 
 def convert_bigdl_other_module(model, dtype):
     """Every leaf that is not one of our linears follows `dtype` (convert.py:1174-1182)."""
+    from ipex_llm.transformers.block_fp8 import BlockFP8Linear
     from ipex_llm.transformers.low_bit_linear import BF16Linear, FP16Linear, LowBitLinear
     for module in model.modules():
         if list(module.children()) == []:
-            if not isinstance(module, (LowBitLinear, FP16Linear, BF16Linear)):
+            if not isinstance(module, (LowBitLinear, FP16Linear, BF16Linear, BlockFP8Linear)):
                 module.to(dtype)
 
 

@@ -48,7 +48,8 @@ class _BaseAutoModelClass:
     @classmethod
     def from_pretrained(cls, *args, **kwargs):
         """Hugging Face from_pretrained plus load_in_4bit / load_in_low_bit / optimize_model /
-        modules_to_not_convert (reference: transformers/model.py:111-388)."""
+        modules_to_not_convert (reference: transformers/model.py:111-388), and block_fp8 (with "fp8_e4m3": weights with a
+        scale for each 128 x 128 block, activations quantized in the call)."""
         from transformers import PretrainedConfig
         pretrained_model_name_or_path = kwargs.get("pretrained_model_name_or_path", None) \
             if len(args) == 0 else args[0]
@@ -116,6 +117,7 @@ class _BaseAutoModelClass:
         mixed_precision = kwargs.pop("mixed_precision", False)
         disable_optimize_pre = kwargs.pop("disable_optimize_pre", False)
         embedding_qtype = kwargs.pop("embedding_qtype", None)
+        block_fp8 = kwargs.pop("block_fp8", False)
         if embedding_qtype is not None:
             # the reference documents 'q2_k' / 'q4_k' here (model.py:148); any qtype with a kernel works
             invalidInputError(embedding_qtype in ("sym_int4", "asym_int4", "sym_int8", "nf4", "fp8_e4m3"),
@@ -140,7 +142,8 @@ class _BaseAutoModelClass:
                                      torch_dtype=torch_dtype,
                                      embedding_qtype=embedding_qtype,
                                      mixed_precision=mixed_precision,
-                                     disable_optimize_pre=disable_optimize_pre)
+                                     disable_optimize_pre=disable_optimize_pre,
+                                     block_fp8=block_fp8)
         model.config.update({"bigdl_transformers_low_bit": q_k, "bigdl_disk_embedding": False})
         model.config.update({"tie_word_embeddings": False})
         model.save_low_bit = types.MethodType(save_low_bit, model)
@@ -167,15 +170,16 @@ class _BaseAutoModelClass:
                           " serialize the model using save_low_bit first.")
         invalidInputError(low_bit in ggml_tensor_qtype, f"Unknown bigdl_transformers_low_bit value: {low_bit}")
         qtype = ggml_tensor_qtype[low_bit]
-        from ipex_llm.optimize import unconverted_linears
+        from ipex_llm.optimize import block_fp8_layers, unconverted_linears
         state_dict = torch.load(os.path.join(pretrained_model_name_or_path, PYTORCH_MODEL_NAME),
                                 weights_only=True)
         with torch.device("meta"):
             model = cls.HF_Model.from_config(config)
         skip = list(modules_to_not_convert or []) + unconverted_linears(state_dict)
+        block_fp8, apart = block_fp8_layers(state_dict)
         model = ggml_convert_low_bit(model, qtype, optimize_model, device="meta",
                                      convert_shape_only=True, modules_to_not_convert=skip,
-                                     embedding_qtype=embedding_qtype)
+                                     embedding_qtype=embedding_qtype, disable_optimize_pre=apart, block_fp8=block_fp8)
         keys_file = os.path.join(pretrained_model_name_or_path, "load_keys.json")
         if os.path.isfile(keys_file):
             with open(keys_file) as f:

@@ -11,8 +11,9 @@ from ipex_llm.transformers.native_ops import ops
 
 def merge_linear(linears: List[torch.nn.Linear]) -> torch.nn.Linear:
     """One linear whose weight (and bias) is the row-wise concatenation of `linears`
-    (reference: models/common.py:22-37).  GPTQ layers (no `weight`) give None."""
-    if not all(isinstance(lin, torch.nn.Linear) and hasattr(lin, "weight") for lin in linears):
+    (reference: models/common.py:22-37).  GPTQ layers (no `weight`) give None, and so do block-scaled ones, whose
+    scales would have to be merged too."""
+    if not all(isinstance(lin, torch.nn.Linear) and hasattr(lin, "weight") and not hasattr(lin, "weight_scale_inv") for lin in linears):
         return None
     new_weight = torch.cat([lin.weight.data for lin in linears], dim=0)
     has_bias = linears[0].bias is not None

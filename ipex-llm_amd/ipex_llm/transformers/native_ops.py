@@ -13,7 +13,9 @@ from ipex_llm.utils.common import invalidInputError
 from ipex_llm.utils.utils import get_shared_lib_info
 
 _BOUND = ("last_error", "blob_bytes", "tileable", "linear_scratch_bytes", "linear", "gated_mlp", "dequantize_rows", "dequantize", "backward_ws", "backward_workspace_bytes", "backward_ws_applies",
-          "experts_workspace_bytes", "experts_forward")
+          "experts_workspace_bytes", "experts_forward", "block_fp8_quantize", "block_fp8_quantize_weight", "block_fp8_linear",
+          "block_fp8_linear_workspace_bytes", "block_fp8_backward", "block_fp8_backward_workspace_bytes", "block_fp8_experts",
+          "block_fp8_experts_workspace_bytes")
 
 
 def _load():

@@ -1,0 +1,171 @@
+"""Block-scaled fp8 without a GPU: refusals, conversion rules, what moves with a model and what does not."""
+import pytest
+import torch
+from torch import nn
+
+import block_fp8_util as u
+import ipex_llm.ggml.model.llama.llama_cpp as ggml
+from ipex_llm.transformers import block_fp8 as bf
+from ipex_llm.transformers.convert import ggml_convert_low_bit, is_block_fp8
+
+FP8 = 15
+lib = ggml._lib
+
+
+def scaled_linear(n, k, bias=False, seed=1):
+    w, ws = u.random_weight(torch.Generator().manual_seed(seed), n, k)
+    lin = nn.Linear(k, n, bias=bias)
+    lin.weight = nn.Parameter(w, requires_grad=False)
+    lin.weight_scale_inv = nn.Parameter(ws, requires_grad=False)
+    return lin
+
+
+def test_the_oracle_rounds_as_torch_does():
+    q = torch.linspace(-448, 448, 100003, dtype=torch.float64).float()
+    q = torch.cat([q, q * 2.0 ** -8, q * 2.0 ** -14, torch.tensor([17.0, 18.0, 19.0, 21.0, 2.0 ** -10, 3 * 2.0 ** -10])])
+    assert torch.equal(u.e4m3(q.double()), q.to(u.E4M3).double())
+
+
+def test_dequantize():
+    codes, scale = u.weight(torch.Generator().manual_seed(2), 300, 272)
+    assert torch.equal(bf.block_fp8_dequantize(codes, scale).double(), u.dense(codes, scale))
+    rows = torch.exp2(torch.arange(300 * 3) % 5).view(300, 3).float()
+    assert torch.equal(bf.block_fp8_dequantize(codes, rows, torch.bfloat16), (codes.double() * u.spread(rows, 300, 272, 1)).bfloat16())
+    with pytest.raises(RuntimeError, match="fit together"):
+        bf.block_fp8_dequantize(codes, scale[:2])
+    with pytest.raises(RuntimeError, match="fit together"):
+        bf.block_fp8_dequantize(codes.float(), scale)
+
+
+def test_host_tensors_are_refused():
+    w, ws = u.weight(torch.Generator().manual_seed(3), 16, 32)
+    x = torch.zeros((2, 32), dtype=torch.bfloat16)
+    for call in (lambda: bf.block_fp8_linear(x, w, ws), lambda: bf.block_fp8_quantize(x), lambda: bf.block_fp8_quantize_weight(x),
+                 lambda: bf.block_fp8_experts(x, torch.zeros((2, 1), dtype=torch.int64), torch.ones((2, 1)), w[None], ws[None], w[None], ws[None])):
+        with pytest.raises(RuntimeError, match="no CPU implementation"):
+            call()
+    with pytest.raises(RuntimeError, match="act is 0"):
+        bf.block_fp8_experts(x, x, x, w, ws, w, ws, act=2)
+
+
+P = 4096                                                     # an aligned address that nothing reads
+
+
+def test_abi_refuses_before_it_touches_the_gpu():
+    lin, back, q, qw, ex = (lib.lowbit_block_fp8_linear, lib.lowbit_block_fp8_backward, lib.lowbit_block_fp8_quantize,
+                            lib.lowbit_block_fp8_quantize_weight, lib.lowbit_block_fp8_experts)
+    assert lin(P, P, P, None, P, 3, 1, 16, 128, None, 0, None) == -4
+    assert lin(P, P, P, None, P, 0, -1, 16, 128, None, 0, None) == -1
+    assert lin(P, P, P, None, P, 0, 1, 16, 120, None, 0, None) == -5
+    assert lin(P, P, P, None, P, 0, 1 << 22, 16, 128, None, 0, None) == -3
+    assert lin(P, P, P, None, P, 0, 1, 16, 1 << 23, None, 0, None) == -3
+    assert lin(P, P, P, None, P, 0, 1, 16, 0, None, 0, None) == -5
+    assert lin(None, P, P, None, P, 0, 1, 16, 128, None, 0, None) == -1
+    assert lin(P + 8, P, P, None, P, 0, 1, 16, 128, None, 0, None) == -1
+    assert lin(P, P, P, None, P, 0, 100, 16, 128, None, 0, None) == -3          # without the workspace it asks for
+    assert b"workspace" in lib.lowbit_last_error()
+    assert lin(P, P, P, None, P, 0, 0, 16, 128, None, 0, None) == 0 == lin(P, P, P, None, P, 0, 5, 0, 128, None, 0, None)
+    assert back(P, P, P, P, 2, 1, 16, 128, None, 0, None) == -4                 # float32
+    assert back(P, P, P, P, 0, 1, 16, 100, None, 0, None) == -5
+    assert back(P, P, P, P, 0, 1, 0, 128, None, 0, None) == -5
+    assert back(P, P + 4, P, P, 0, 1, 16, 128, None, 0, None) == -1
+    assert back(P, P, P, P, 0, 0, 16, 128, None, 0, None) == 0
+    assert q(P, 3, 1, 128, P, P, None) == -4 and q(P, 0, 1, 8, P, P, None) == -5 and q(P, 0, -1, 16, P, P, None) == -1
+    assert q(P + 2, 0, 1, 16, P, P, None) == -1 and q(P, 0, 0, 16, P, P, None) == 0
+    assert qw(P, 3, 1, 16, 128, P, P, None) == -4 and qw(P, 0, 1, 16, 24, P, P, None) == -5 and qw(P, 0, -1, 16, 16, P, P, None) == -1
+    assert qw(P, 0, 1, 1 << 23, 16, P, P, None) == -3 and qw(P, 0, 0, 16, 16, P, P, None) == 0
+
+    def experts(x=P, wdt=0, tokens=4, top_k=2, n=4, dt=0, hidden=128, inter=128, act=0, ws=None, size=0):
+        return ex(x, P, P, wdt, tokens, top_k, n, P, P, P, P, ws, size, P, dt, hidden, inter, act, None)
+    assert experts(dt=2) == -4 and experts(wdt=3) == -4 and experts(act=2) == -1 and experts(tokens=0) == 0
+    assert experts(top_k=65) == -3 and experts(n=4097) == -3 and experts(tokens=1 << 21) == -3 and experts(tokens=-1) == -3
+    assert experts(hidden=24) == -5 and experts(inter=64) == -5 and experts(x=None) == -1
+    assert experts() == -3 and b"workspace" in lib.lowbit_last_error()
+    assert lib.lowbit_block_fp8_experts_workspace_bytes(4, 2, 4, 128, 64) == 0
+    assert lib.lowbit_block_fp8_linear_workspace_bytes(0, 100, 16, 100) == 0 < lib.lowbit_block_fp8_linear_workspace_bytes(0, 100, 16, 112)
+
+
+def test_conversion_replaces_block_scaled_layers_and_keeps_their_codes():
+    lin = scaled_linear(200, 272, bias=True)
+    assert is_block_fp8(lin) and not is_block_fp8(nn.Linear(16, 16))
+    codes, scales = lin.weight.data.clone(), lin.weight_scale_inv.data.clone()
+    model = ggml_convert_low_bit(nn.Sequential(lin, nn.ReLU()).eval(), FP8, torch_dtype=torch.bfloat16)
+    new = model[0]
+    assert type(new) is bf.BlockFP8Linear and not new.training and not any(p.requires_grad for p in new.parameters())
+    assert torch.equal(new.weight.float(), codes.float()) and torch.equal(new.weight_scale_inv, scales)
+    assert set(new.state_dict()) == {"weight", "weight_scale_inv", "bias"}
+    with pytest.raises(RuntimeError, match="fp8_e4m3"):
+        ggml_convert_low_bit(nn.Sequential(scaled_linear(32, 128)), 2)
+    bad = scaled_linear(200, 272)
+    bad.weight_scale_inv = nn.Parameter(torch.ones(1, 3), requires_grad=False)
+    with pytest.raises(RuntimeError, match="one scale for each block"):
+        ggml_convert_low_bit(nn.Sequential(bad), FP8)
+    again = ggml_convert_low_bit(model, FP8)
+    assert again[0] is new                                   # converted layers stay as they are
+
+
+def test_block_fp8_asks_for_fp8():
+    from ipex_llm import optimize_model
+    with pytest.raises(RuntimeError, match="use it with fp8_e4m3"):
+        optimize_model(nn.Sequential(nn.Linear(64, 64)), "sym_int4", block_fp8=True)
+
+
+def test_shape_only_conversion_of_dense_layers():
+    with torch.device("meta"):
+        model = nn.Sequential(nn.Linear(272, 200), nn.Linear(200, 100), nn.Linear(192, 64))
+    model = ggml_convert_low_bit(model, FP8, convert_shape_only=True, block_fp8=True)
+    assert type(model[0]) is bf.BlockFP8Linear and model[0].weight.shape == (200, 272) and model[0].weight_scale_inv.shape == (2, 3)
+    assert type(model[1]) is nn.Linear                       # 200 is no multiple of 16
+    with torch.device("meta"):
+        model = nn.Sequential(nn.Linear(256, 64), nn.Linear(256, 64))
+    model = ggml_convert_low_bit(model, FP8, convert_shape_only=True, block_fp8={"1"})
+    assert type(model[1]) is bf.BlockFP8Linear and type(model[0]).__name__ == "LowBitLinear"
+
+
+def test_codes_and_scales_keep_their_format_when_a_model_moves():
+    new = bf.BlockFP8Linear.from_linear(scaled_linear(130, 144, bias=True))
+    codes, scales = new.weight.data.clone(), new.weight_scale_inv.data.clone()
+    for move in (lambda m: m.half(), lambda m: m.to(torch.bfloat16), lambda m: m.double(), lambda m: m.to("cpu"), lambda m: m.float()):
+        m = move(new)
+        assert m.weight.dtype == u.E4M3 and m.weight_scale_inv.dtype == torch.float32
+        assert torch.equal(m.weight.float(), codes.float()) and torch.equal(m.weight_scale_inv, scales)
+    assert new.half().bias.dtype == torch.float16
+    assert new.to("meta").weight.device.type == "meta" and new.weight.dtype == u.E4M3
+
+
+def test_experts_module_from_dense_shapes_and_from_scaled_weights():
+    class Fused(nn.Module):
+        def __init__(self, e, h, i, dtype=torch.float32):
+            super().__init__()
+            self.gate_up_proj = nn.Parameter(torch.zeros((e, 2 * i, h)).to(dtype), requires_grad=False)
+            self.down_proj = nn.Parameter(torch.zeros((e, h, i)).to(dtype), requires_grad=False)
+            self.act_fn = nn.SiLU()
+
+    with torch.device("meta"):
+        model = nn.Sequential(Fused(3, 256, 128), Fused(3, 256, 64))
+    model = ggml_convert_low_bit(model, FP8, convert_shape_only=True, block_fp8=True)
+    assert type(model[0]) is bf.BlockFP8Experts and model[0].down_proj_scale_inv.shape == (3, 2, 1)
+    assert type(model[1]) is Fused                           # experts of 64 columns do not divide into blocks
+    fused = Fused(3, 256, 128, u.E4M3)
+    fused.gate_up_proj_scale_inv = nn.Parameter(torch.ones(3, 2, 2), requires_grad=False)
+    fused.down_proj_scale_inv = nn.Parameter(torch.ones(3, 2, 1), requires_grad=False)
+    model = ggml_convert_low_bit(nn.Sequential(fused).eval(), FP8)
+    assert type(model[0]) is bf.BlockFP8Experts and not model[0].training
+    with pytest.raises(RuntimeError, match="multiple of 16"):
+        bf.BlockFP8Experts(2, 24, 128, nn.SiLU())
+
+
+def test_block_scaled_projections_are_not_merged():
+    from ipex_llm.transformers.models.common import merge_linear
+    assert merge_linear([scaled_linear(128, 128), scaled_linear(128, 128)]) is None
+    assert merge_linear([nn.Linear(32, 16), nn.Linear(32, 16)]) is not None
+
+
+def test_saved_layers_are_found_again(tmp_path):
+    from ipex_llm.optimize import block_fp8_layers, unconverted_linears
+    model = nn.ModuleDict({"q_proj": bf.BlockFP8Linear.from_linear(scaled_linear(128, 128)), "head": nn.Linear(16, 16)})
+    state = model.state_dict()
+    assert block_fp8_layers(state) == ({"q_proj"}, True) and unconverted_linears(state) == ["head"]
+    torch.save(state, tmp_path / "m.bin")
+    again = torch.load(tmp_path / "m.bin", weights_only=True)
+    assert again["q_proj.weight"].dtype == u.E4M3
