@@ -1,0 +1,419 @@
+// The tiled product of block_fp8.h: codes of x and of the weight meet in LDS, 128 values of K at a time.
+//
+// A workgroup of WM x WN waves owns WM * TM * 16 rows of x by WN * TN * 16 weight rows.  A step's codes of both operands come by
+// LDS-DMA, one step ahead, into the other of two buffers; a step is one block of K, so a wave multiplies TM x TN results by one
+// instruction each, from zero, and adds them to the sums in float32 times the two scales.
+//
+// LDS holds rows of 128 bytes, the 16-byte chunk c of row r at slot c ^ swizzle(r): the DMA writes 8 rows of 8 slots at a time (lane
+// = 8 * row + slot, so the swizzle is in the lane's source address), and 16 lanes of a read, which take one chunk of 16
+// consecutive rows, cover all 64 banks: two rows are 256 bytes, and the eight rows of one parity have different slots.  (With slots that
+// repeat after four rows half of LDS' busy cycles were conflicts, 8192^3 in 567 us against SWIZZLED.)
+#pragma once
+#include "block_fp8.h"
+#include "lowbit_gemm.h"
+
+namespace lowbit {
+
+struct TiledArgs {
+    const uint8_t *x;                                        // codes, rows of ldx bytes, zeros past K
+    const float *xs;                                         // [KB][ldxs], rows of the result
+    const uint8_t *w;
+    const float *ws;
+    const void *bias;
+    void *y;
+    float *part;                                             // sums of a split: [split][M][pitch]
+    const int32_t *offsets, *order;                          // by expert: rows offsets[e] .. of the result; x row order[row] / top_k, or row
+    int64_t ldx;
+    int ldxs, M, N, K, KB, pitch;
+    int tiles_m, tiles_n, splits, split_blocks;
+    int n_exp, top_k, I, act;                                // UP: I columns of h
+    float *hs;                                               // UP: scales of h, [I / 128][ldhs]; its codes go to y
+    int ldhs;
+};
+
+enum TiledMode { TILED_PLAIN, TILED_PART, TILED_UP };
+
+__device__ inline int swizzle(int row) { return (row >> 1) & 7; }
+
+// 16 bytes per lane from base + off (or from the lanes' own addresses) to LDS at lds_at + 16 * lane.  Inline assembly, because the compiler
+// takes an LDS-DMA to alias every later LDS access and waits for it at once; here the wait is the one ahead of the step's barrier.
+__device__ inline void dma16(uint32_t off, uint64_t base, uint32_t lds_at) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(off), "s"(base), "s"(lds_at) : "memory", "m0");
+}
+__device__ inline void dma4(uint32_t off, uint64_t base, uint32_t lds_at) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" :: "v"(off), "s"(base), "s"(lds_at) : "memory", "m0");
+}
+__device__ inline void dma16_at(uint64_t address, uint32_t lds_at) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(address), "s"(lds_at) : "memory", "m0");
+}
+
+// (the other two counters untouched: 4 bits of lgkmcnt at 8)
+__device__ inline void wait_lds() { __builtin_amdgcn_s_waitcnt(0xC07F); }
+
+// codes of a lane as bfloat16, exactly: eight values per MFMA operand
+__device__ inline bf16x8 widen8(uint32_t w0, uint32_t w1) {
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, 1.0f, true);
+    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, 1.0f, true);
+    return {a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+template <bool EXACT> struct Operand;
+template <> struct Operand<false> {
+    i32x8 v;
+    __device__ void take(u32x4 lo, u32x4 hi) {
+        v = i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+    }
+    __device__ f32x4 dot(const Operand &o) const {
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(v, o.v, f32x4{}, 0, 0, 0, 0, 0, 0);
+    }
+};
+template <> struct Operand<true> {
+    bf16x8 v[4];
+    __device__ void take(u32x4 lo, u32x4 hi) {
+        v[0] = widen8(lo[0], lo[1]);
+        v[1] = widen8(lo[2], lo[3]);
+        v[2] = widen8(hi[0], hi[1]);
+        v[3] = widen8(hi[2], hi[3]);
+    }
+    __device__ f32x4 dot(const Operand &o) const { return mfma16(v[3], o.v[3], mfma16(v[2], o.v[2], mfma16(v[1], o.v[1], mfma16(v[0], o.v[0], f32x4{})))); }
+};
+
+template <typename OT> struct Stored;
+template <> struct Stored<float> {
+    static __device__ float of(float v) { return v; }
+};
+template <> struct Stored<_Float16> {
+    static __device__ _Float16 of(float v) { return (_Float16)v; }
+};
+template <> struct Stored<__bf16> {
+    static __device__ __bf16 of(float v) { return (__bf16)v; }
+};
+
+// BY_EXPERT: row tiles of one expert each.  GATHER: x rows by order[].  S: buffers in LDS.
+template <typename OT, bool EXACT, TiledMode MODE, bool BY_EXPERT, bool GATHER, int TM, int TN, int WM, int WN, int S, int MIN_WAVES>
+__global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void block_fp8_tiled_kernel(const TiledArgs p) {
+    constexpr int WAVES = WM * WN, BM = WM * TM * 16, BN = WN * TN * 16, XP = BM / 8, WP = BN / 8;
+    constexpr int PX = XP / WAVES, PW = WP / WAVES;
+    constexpr bool UP = MODE == TILED_UP;
+    constexpr int TH = TN / 2;                               // UP: a wave's tiles of the gate, and as many of u
+    // Two buffers: a step in two halves, each with a barrier (see the loop)
+    constexpr int HALVES = S == 2 ? 2 : 1, PH = PW / HALVES;
+    static_assert(WP % (WAVES * HALVES) == 0 && XP % WAVES == 0 && PX > 0 && BM / WAVES <= 64 && TN % 2 == 0 && (S > 2 || TN % 4 == 0 || TN == 2) &&
+                  (!UP || BN == 256), "whole pieces per wave");
+    constexpr uint32_t BUFFER = (BM + BN) * FP8_BLOCK, SCALES = BM * 4;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[S * (BUFFER + SCALES)];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+    const int wm = wave / WN, wn = wave % WN;
+
+    // Workgroups go to the XCDs in turn: each takes a run of the tiles, eight row tiles by as many columns as its CUs hold, so that
+    // its L2 serves every operand several times.
+    const uint32_t units = (uint32_t)(p.tiles_m * p.tiles_n * p.splits), xcd = blockIdx.x & 7;
+    const uint32_t unit = (uint32_t)((uint64_t)units * xcd >> 3) + (blockIdx.x >> 3);
+    if (unit >= (uint32_t)((uint64_t)units * (xcd + 1) >> 3)) return;
+    const int tile = (int)(unit / p.splits), split = (int)(unit - (uint32_t)tile * p.splits);
+    int tm, tn;
+    {
+        const int per = 8 * p.tiles_n, band = tile / per, at = tile - band * per, rows = p.tiles_m - band * 8 < 8 ? p.tiles_m - band * 8 : 8;
+        tn = at / rows;
+        tm = band * 8 + at - tn * rows;
+    }
+    int m0 = tm * BM, end = p.M, expert = 0;
+    if constexpr (BY_EXPERT) {
+        ExpertTile t;
+        if (!find_expert_tile<BM>(p.offsets, p.n_exp, tm, t)) return;
+        expert = __builtin_amdgcn_readfirstlane(t.expert);
+        m0 = __builtin_amdgcn_readfirstlane(t.first);
+        end = __builtin_amdgcn_readfirstlane(t.end);
+    }
+    const int n0 = tn * (UP ? FP8_BLOCK : BN), KB = p.KB;
+    const int b0 = split * p.split_blocks, b1 = MODE == TILED_PART && b0 + p.split_blocks < KB ? b0 + p.split_blocks : KB;
+
+    // ---- sources of this wave's pieces of 8 rows
+    uint32_t xoff[GATHER ? 1 : PX], woff[PW];
+    uint64_t xaddr[GATHER ? PX : 1];
+    const int piece_row = lane >> 3;
+    const uint64_t xbase = (uint64_t)(uintptr_t)p.x + (GATHER ? 0 : (uint64_t)m0 * p.ldx);
+#pragma unroll
+    for (int j = 0; j < PX; j++) {
+        const int row = (wave * PX + j) * 8 + piece_row, chunk = ((lane & 7) ^ swizzle(row)) * 16;
+        const int at = m0 + row < end ? m0 + row : end - 1;
+        if constexpr (GATHER) xaddr[j] = xbase + (uint64_t)(p.order[at] / p.top_k) * p.ldx + chunk;
+        else xoff[j] = (uint32_t)((at - m0) * p.ldx) + chunk;
+    }
+    const uint64_t wexpert = (uint64_t)(uintptr_t)p.w + (uint64_t)expert * p.N * p.K;
+    // Which weight row lies in row `at` of LDS: a wave column's tiles of 16, each lane quarter's four rows of them neighbours of its
+    // four in the next tile, so that a lane's results are neighbours in a row of y.  UP: tiles of the gate, then as many of u.
+    auto weight_row = [&](int at) -> int64_t {
+        const int col = at / (TN * 16), i = at / 16 % TN, q = at / 4 % 4, t = at % 4;
+        if constexpr (UP) return (int64_t)(i / TH) * p.I + n0 + col * (TH * 16) + q * (TH * 4) + i % TH * 4 + t;
+        const int n = n0 + col * (TN * 16) + i / 2 * 32 + q * 8 + i % 2 * 4 + t;
+        return n < p.N ? n : p.N - 1;
+    };
+    // Row of LDS where the wave's piece j starts: with two halves the first PH pieces are of the first half of every wave column's tiles
+    auto piece_at = [&](int j) {
+        const int id = wave * PH + j % PH;
+        return HALVES == 1 ? id * 8 : (id / TN) * (TN * 16) + j / PH * (TN * 8) + id % TN * 8;
+    };
+    uint32_t wchunk[2];                                      // of even and odd rows of eight: 8 rows more turn one bit of the swizzle
+#pragma unroll
+    for (int j = 0; j < 2; j++) wchunk[j] = ((lane & 7) ^ swizzle(j * 8 + piece_row)) * 16;
+    uint64_t wbase[UP ? PW : 1];
+    if constexpr (!UP) wbase[0] = wexpert + (uint64_t)n0 * p.K;
+#pragma unroll
+    for (int j = 0; j < PW; j++) {
+        const int first = piece_at(j);
+        const int64_t from = UP ? weight_row(first) : n0;    // (a piece is of one tile: the first of its rows is the lowest)
+        if constexpr (UP) wbase[j] = wexpert + (uint64_t)from * p.K;
+        woff[j] = (uint32_t)(weight_row(first + piece_row) - from) * p.K + wchunk[first / 8 & 1];
+    }
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds;
+    const uint32_t lds_x = lds0 + wave * PX * 1024, lds_w = lds0 + BM * FP8_BLOCK;
+    // x's scales of a block come the same way, BM / WAVES rows per wave (rows past the end: the last one's)
+    constexpr int RS = BM / WAVES;
+    const int srow = m0 + wave * RS + (lane < RS ? lane : 0);
+    const uint32_t soff = (uint32_t)(srow < end ? srow : end - 1) * 4, lds_s = lds0 + S * BUFFER + wave * RS * 4;
+    // Pieces of a block in the order in which a wave asks for them: x, its scales, weights.  They are asked for one at a time between the
+    // products: all at once, from all waves, they queue at the CU's address unit and the waves stand still (8192^3: 553 us against 489).
+    constexpr int PIECES = PX + 1 + PW;
+    auto fetch = [&](int kb, int which, int q) __attribute__((always_inline)) {
+        const uint32_t buffer = which * BUFFER;
+        if (q < PX) {
+            if constexpr (GATHER) dma16_at(xaddr[q] + (uint64_t)kb * FP8_BLOCK, lds_x + buffer + q * 1024);
+            else dma16(xoff[q], xbase + (uint64_t)kb * FP8_BLOCK, lds_x + buffer + q * 1024);
+        } else if (q == PX) {
+            if (lane < RS) dma4(soff, (uint64_t)(uintptr_t)(p.xs + (int64_t)kb * p.ldxs), lds_s + which * SCALES);
+        } else {
+            // A row that ends inside the block: in place of the chunks past its end the block's first one.  x has zeros there, so it
+            // counts nothing (a NaN among it is one of the row's own).
+            const int j = q - PX - 1, left = p.K - kb * FP8_BLOCK;
+            uint32_t off = woff[j];
+            if (left < FP8_BLOCK) {
+                const uint32_t chunk = wchunk[piece_at(j) / 8 & 1];
+                off -= chunk < (uint32_t)left ? 0u : chunk;
+            }
+            dma16(off, wbase[UP ? j : 0] + (uint64_t)kb * FP8_BLOCK, lds_w + buffer + piece_at(j) * FP8_BLOCK);
+        }
+    };
+
+    // ---- scales.  A weight's of up to 64 blocks lie in the lanes of one register
+    const int nb0 = UP ? n0 / FP8_BLOCK : (n0 + wn * TN * 16) / FP8_BLOCK, NB = fp8_blocks(p.N);
+    const float *const wscale = p.ws + ((int64_t)expert * NB + (nb0 < NB ? nb0 : NB - 1)) * KB;
+    const int64_t u_scale = UP ? (int64_t)(p.I / FP8_BLOCK) * KB : 0;
+    float wheld[UP ? 2 : 1];
+    auto hold = [&](int kb) __attribute__((always_inline)) {
+        const int b = kb + lane < KB ? kb + lane : KB - 1;
+        wheld[0] = wscale[b];
+        if constexpr (UP) wheld[1] = wscale[u_scale + b];
+        // (waited for here: a load that may be under way at the loop's head makes the compiler wait there for all, in every step)
+        asm volatile("" : "+v"(wheld[0]));
+        if constexpr (UP) asm volatile("" : "+v"(wheld[1]));
+    };
+    // ---- operands: lane (r, g) reads the chunks g and 4 + g of row r of a tile
+    const int xlo = (wm * TM * 16 + r) * FP8_BLOCK + (g ^ swizzle(r)) * 16, wlo = xlo + (BM + wn * TN * 16 - wm * TM * 16) * FP8_BLOCK;
+    auto read = [&](int lo, int tile, Operand<EXACT> &o) __attribute__((always_inline)) {
+        const uint8_t *const at = lds + tile * 16 * FP8_BLOCK;
+        o.take(*(const u32x4 *)(at + lo), *(const u32x4 *)(at + (lo ^ 64)));
+    };
+    auto read_x = [&](int buffer, int i, Operand<EXACT> &o) __attribute__((always_inline)) { read(xlo + buffer, i, o); };
+    auto read_w = [&](int buffer, int i, Operand<EXACT> &o) __attribute__((always_inline)) { read(wlo + buffer, i, o); };
+
+    // A step: TN tiles of TM products each.  A product is added while the next ones run, LAG instructions later; a tile's operands are read
+    // one tile ahead.  The barrier that publishes the next block stands ahead of the last tile, whose operands are in registers: its
+    // products cover the first reads of the next block (of x into the registers that they free), and the buffer that has been read is filled
+    // again from there on.  The order is fixed: left alone the compiler issues all products first and spills them.
+    //
+    // A load takes about as long as a step of the largest tile, so it is asked for more than a step ahead.  Where there is room for two
+    // buffers only, a second barrier stands in the middle: it frees x, which is in registers, and the first half of the weights, whose
+    // next block but one is asked for there; the second half's at the other barrier.  Each has a step and a half to arrive.
+    constexpr int COUNT = TN * TM, LAG = COUNT - TM < 3 ? COUNT - TM : 3, EARLY = PIECES - (HALVES - 1) * PH, TURN = HALVES == 2 ? (TN / 2 - 1) * TM : -1;
+    constexpr int IN_FLIGHT = HALVES == 2 ? PIECES : (S - 2) * PIECES;       // loads of this wave that a barrier leaves under way
+    constexpr int SLOTS = COUNT / HALVES, PER = ((HALVES == 2 ? EARLY : PIECES) + SLOTS - 1) / SLOTS;       // pieces asked for per product
+    static_assert(IN_FLIGHT < 64, "vmcnt has 6 bits");
+    f32x4 acc[TN][TM] = {};
+    Operand<EXACT> b[TM], a[2];
+    f32x4 d[LAG + 1];
+    float s[UP ? 2 : 1][TM], xs[TM];
+    auto read_xs = [&](int which) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < TM; i++) xs[i] = *(const float *)(lds + S * BUFFER + which * SCALES + ((wm * TM + i) * 16 + r) * 4);
+    };
+    auto scales = [&](int kb) __attribute__((always_inline)) {
+#pragma unroll
+        for (int h = 0; h < (UP ? 2 : 1); h++) {
+            const float sw = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wheld[h]), (kb - b0) & 63));
+#pragma unroll
+            for (int i = 0; i < TM; i++) s[h][i] = xs[i] * sw;
+        }
+    };
+    auto add = [&](int o) __attribute__((always_inline)) {
+        f32x4 &sum = acc[o / TM][o % TM];
+#pragma unroll
+        for (int j = 0; j < 4; j++) sum[j] = fmaf(s[UP ? o / TM / TH : 0][o % TM], d[o % (LAG + 1)][j], sum[j]);
+        asm volatile("" : "+v"(sum));                        // (here, and not behind the barrier, where nothing covers them)
+    };
+    // pieces first .. last - 1 of a block, PER of them in slot 0, 1, ..
+    auto fetch_slot = [&](int kb, int which, int first, int last, int slot) __attribute__((always_inline)) {
+#pragma unroll
+        for (int q = first + slot * PER; q < first + (slot + 1) * PER && q < last; q++) fetch(kb, which, q);
+    };
+    auto meet = [&]() __attribute__((always_inline)) {       // what was asked for IN_FLIGHT pieces ago is there, and every wave's reads are done
+        wait_loads_but<IN_FLIGHT>();
+        wait_lds();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    const int last = b1 - 1;                                 // (past it: this block again, whose products nobody adds)
+
+    hold(b0);
+    constexpr int AHEAD = S - 1;                             // whole blocks asked for ahead of the loop but for what slot 0 .. ask for
+#pragma unroll
+    for (int v = 0; v < AHEAD; v++)
+#pragma unroll
+        for (int q = 0; q < PIECES; q++) fetch(b0 + v < last ? b0 + v : last, v, q);
+    if constexpr (HALVES == 2) {
+#pragma unroll
+        for (int q = 0; q < EARLY; q++) fetch(b0 + 1 < last ? b0 + 1 : last, 1, q);
+        wait_loads_but<EARLY>();
+    } else wait_loads_but<(S - 2) * PIECES>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    int which = 0;
+#pragma unroll
+    for (int i = 0; i < TM; i++) read_x(0, i, b[i]);
+    read_w(0, 0, a[0]);
+    read_xs(0);
+#pragma unroll
+    for (int i = 0; i < TM; i++) {                           // what the last tile of a step before this one would have asked for
+        if constexpr (HALVES == 2) fetch_slot(b0 + 1 < last ? b0 + 1 : last, 1, EARLY, PIECES, i);
+        else fetch_slot(b0 + S - 1 < last ? b0 + S - 1 : last, S - 1, 0, PIECES, i);
+    }
+    for (int kb = b0;;) {
+        const int buffer = which * BUFFER, then = which + 1 < S ? which + 1 : 0, other = then * BUFFER;
+        const int late = kb + S - 1 < last ? kb + S - 1 : last, next = kb + S < last ? kb + S : last;
+        const int behind = which > 0 ? which - 1 : S - 1;    // the buffer that the step before this one freed
+        scales(kb);
+#pragma unroll
+        for (int o = 0; o < COUNT - TM; o++) {
+            const int t = o / TM, i = o % TM;
+            if (o == TURN) meet();
+            if (i == 0) read_w(buffer, t + 1, a[(t + 1) & 1]);
+            d[o % (LAG + 1)] = a[t & 1].dot(b[i]);
+            if (o >= LAG) add(o - LAG);
+            if constexpr (HALVES == 2) {
+                if (o < TURN) fetch_slot(late, behind, EARLY, PIECES, TM + o);
+                else fetch_slot(next, which, 0, EARLY, o - TURN);
+            } else fetch_slot(late, behind, 0, PIECES, TM + o);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        meet();
+#pragma unroll
+        for (int i = 0; i < TM; i++) {
+            const int o = COUNT - TM + i;
+            d[o % (LAG + 1)] = a[(TN - 1) & 1].dot(b[i]);
+            read_x(other, i, b[i]);
+            if (i == TM - 1) read_w(other, 0, a[TN & 1]);
+            add(o - LAG);
+            if constexpr (HALVES == 2) fetch_slot(next, which, EARLY, PIECES, i);
+            else fetch_slot(next, which, 0, PIECES, i);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        read_xs(then);
+#pragma unroll
+        for (int o = COUNT - LAG; o < COUNT; o++) add(o);
+        if (++kb >= b1) break;
+        if (((kb - b0) & 63) == 0) hold(kb);
+        which = then;
+    }
+    wait_all_loads();
+    __syncthreads();
+
+    // ---- results: lane = row r of tile i, columns 4 g .. 4 g + 3 of tile t's sixteen
+    if constexpr (UP) {
+        float *const most = (float *)lds;                    // [WN][BM] largest magnitudes, as bits
+        float h[TM][TH][4];
+#pragma unroll
+        for (int i = 0; i < TM; i++) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int t = 0; t < TH; t++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    h[i][t][j] = gate_act(acc[t][i][j], p.act) * acc[TH + t][i][j];
+                    m = max_u32(m, magnitude(h[i][t][j]));
+                }
+            m = max_u32(m, (uint32_t)__shfl_xor((int)m, 16));
+            m = max_u32(m, (uint32_t)__shfl_xor((int)m, 32));
+            if (g == 0) most[wn * BM + (wm * TM + i) * 16 + r] = __builtin_bit_cast(float, m);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < TM; i++) {
+            const int row = (wm * TM + i) * 16 + r, m = m0 + row;
+            uint32_t top = 0;
+#pragma unroll
+            for (int v = 0; v < WN; v++) top = max_u32(top, __builtin_bit_cast(uint32_t, most[v * BM + row]));
+            const float s = block_scale(top), inv = __builtin_amdgcn_rcpf(s);
+            uint32_t c[TH];
+#pragma unroll
+            for (int t = 0; t < TH; t++) c[t] = encode4(h[i][t][0] * inv, h[i][t][1] * inv, h[i][t][2] * inv, h[i][t][3] * inv);
+            if (m >= end) continue;
+            uint8_t *const to = (uint8_t *)p.y + (int64_t)m * p.I + n0 + wn * (TH * 16) + g * (TH * 4);
+            if constexpr (TH == 4) *(u32x4 *)to = u32x4{c[0], c[1], c[2], c[3]};
+            else if constexpr (TH == 2) *(u32x2 *)to = u32x2{c[0], c[1]};
+            else *(uint32_t *)to = c[0];
+            if (wn == 0 && g == 0) p.hs[(int64_t)(n0 / FP8_BLOCK) * p.ldhs + m] = s;
+        }
+    } else {
+        constexpr int PAIR = TN > 1 ? 2 : 1;
+        const bool vectors = MODE == TILED_PART || p.N % 8 == 0;
+#pragma unroll
+        for (int t = 0; t < TN; t += PAIR) {
+            const int n = n0 + wn * TN * 16 + (TN > 1 ? (t >> 1) * 32 + g * 8 : g * 4);
+            float add[4 * PAIR] = {};
+            if (MODE == TILED_PLAIN && p.bias) {
+#pragma unroll
+                for (int j = 0; j < 4 * PAIR; j++) add[j] = n + j < p.N ? (float)((const OT *)p.bias)[n + j] : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < TM; i++) {
+                const int m = m0 + (wm * TM + i) * 16 + r;
+                if (m >= end) continue;
+                if constexpr (MODE == TILED_PART) {
+                    float *const to = p.part + ((int64_t)split * p.M + m) * p.pitch + n;
+#pragma unroll
+                    for (int h = 0; h < PAIR; h++)
+                        if (n + 4 * h < p.pitch) *(f32x4 *)(to + 4 * h) = acc[t + h][i];
+                } else {
+                    OT *const to = (OT *)p.y + (int64_t)m * p.N + n;
+                    typedef OT out_v __attribute__((ext_vector_type(4 * PAIR)));
+                    out_v o;
+#pragma unroll
+                    for (int j = 0; j < 4 * PAIR; j++) o[j] = Stored<OT>::of(acc[t + j / 4][i][j & 3] + add[j]);
+                    if (vectors) {
+                        if (n < p.N) *(out_v *)to = o;
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4 * PAIR; j++)
+                            if (n + j < p.N) to[j] = o[j];
+                    }
+                }
+            }
+        }
+    }
+}
+
+template <typename OT, bool EXACT, TiledMode MODE, bool BY_EXPERT, bool GATHER, int TM, int TN, int WM, int WN, int S, int MIN_WAVES>
+void launch_tiled(TiledArgs p, hipStream_t st) {
+    constexpr int BM = WM * TM * 16, BN = WN * TN * 16;
+    if (!BY_EXPERT) p.tiles_m = (p.M + BM - 1) / BM;
+    p.tiles_n = MODE == TILED_UP ? p.I / FP8_BLOCK : (p.N + BN - 1) / BN;
+    if (MODE != TILED_PART) {
+        p.splits = 1;
+        p.split_blocks = p.KB;
+    }
+    const uint32_t units = (uint32_t)(p.tiles_m * p.tiles_n * p.splits);
+    hipLaunchKernelGGL((block_fp8_tiled_kernel<OT, EXACT, MODE, BY_EXPERT, GATHER, TM, TN, WM, WN, S, MIN_WAVES>), dim3((units + 7) / 8 * 8),
+                       dim3(64 * WM * WN), 0, st, p);
+}
+
+}  // namespace lowbit

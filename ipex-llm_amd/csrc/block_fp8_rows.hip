@@ -3,7 +3,7 @@
 // A workgroup owns 16 * T weight rows and up to 16 * MT rows of x; its waves take the blocks of K in turn and their sums meet in LDS.
 // A wave's loads are 16 rows x 64 contiguous bytes, STEPS blocks ahead of their use.  FUSED: x is quantized by each workgroup, into
 // LDS, while the first weights are on their way, which saves a launch; otherwise codes and scales of x come from memory (L2).
-#include "block_fp8.h"
+#include "block_fp8_tiled.h"
 
 namespace lowbit {
 
@@ -159,19 +159,43 @@ static bool fuses_rows(int M, int K) {
 
 static size_t codes_bytes(int M, int K) { return ((size_t)M * fp8_blocks(K) * FP8_BLOCK + 255) & ~(size_t)255; }
 
+// Up to here one pass of the weights through registers; beyond, tiles in LDS.
+static bool takes_few_rows(int M) { return M <= 64; }
+
+// codes of x, their scales, a split's sums
+struct LinearSpace {
+    size_t xs, part, bytes;
+};
+static LinearSpace linear_space(int M, int N, int K, const TiledPlan &plan) {
+    LinearSpace s;
+    s.xs = codes_bytes(M, K);
+    s.part = s.xs + (((size_t)M * fp8_blocks(K) * sizeof(float) + 255) & ~(size_t)255);
+    s.bytes = s.part + block_fp8_tiled_part_bytes(plan, M, N);
+    return s;
+}
+
 size_t block_fp8_linear_workspace_bytes(int dtype, int M, int N, int K) {
     if (fuses_rows(M, K)) return 0;
-    return codes_bytes(M, K) + (size_t)M * fp8_blocks(K) * sizeof(float);
+    const TiledPlan plan = takes_few_rows(M) ? TiledPlan{0, 1, 0.0f} : block_fp8_tiled_plan(dtype == DT_F32, M, N, K);
+    return linear_space(M, N, K, plan).bytes;
 }
 
 int launch_block_fp8_linear(const void *x, const uint8_t *w, const float *ws, const void *bias, void *y, int dtype, int M, int N, int K,
                             uint8_t *space, hipStream_t st) {
-    const bool fused = fuses_rows(M, K);
+    const bool fused = fuses_rows(M, K), few = takes_few_rows(M);
     const int KB = fp8_blocks(K), ldx = KB * FP8_BLOCK;
     RowsProduct p = {x, nullptr, w, ws, bias, y, M, N, K, KB, ldx, M};
     if (!fused) {
-        float *const xs = (float *)(space + codes_bytes(M, K));
+        const TiledPlan plan = few ? TiledPlan{0, 1, 0.0f} : block_fp8_tiled_plan(dtype == DT_F32, M, N, K);
+        const LinearSpace at = linear_space(M, N, K, plan);
+        float *const xs = (float *)(space + at.xs);
         if (int rc = launch_block_fp8_rows(x, dtype, M, K, space, ldx, xs, 1, M, st)) return rc;
+        if (!few) {
+            TiledArgs t{};
+            t.x = space; t.xs = xs; t.w = w; t.ws = ws; t.bias = bias; t.y = y; t.part = (float *)(space + at.part);
+            t.M = M; t.N = N; t.K = K;
+            return launch_block_fp8_tiled(t, dtype, plan, st);
+        }
         p.x = space;
         p.xs = xs;
     }

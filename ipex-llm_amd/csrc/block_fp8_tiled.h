@@ -1,0 +1,47 @@
+// The forms of the tiled product that launches choose from.
+#pragma once
+#include "block_fp8_gemm.h"
+
+namespace lowbit {
+
+// rows and weight rows of a tile, workgroups that a CU holds, and a step's time (us): with the GPU full, with one workgroup on a CU; the
+// same with float32 results, whose codes go through the bfloat16 MFMA
+struct TiledForm {
+    int rows, cols, per_cu;
+    float step_us, alone_us, exact_us, exact_alone_us;
+};
+enum { TILED_256, TILED_128_256, TILED_128, TILED_64, TILED_COUNT };
+static const TiledForm TILED_FORMS[TILED_COUNT] = {
+    {256, 256, 1, 1.75f, 1.70f, 4.4f, 4.2f},
+    {128, 256, 1, 1.00f, 0.92f, 2.2f, 2.1f},
+    {128, 128, 2, 1.05f, 0.62f, 2.2f, 1.2f},
+    {64, 128, 2, 0.68f, 0.40f, 1.2f, 0.7f},
+};
+
+struct TiledPlan {
+    int form, splits;
+    float us;
+};
+
+// One launch per form; the wave tiles are 64 x 128, 64 x 64, 64 x 64 and 32 x 64.
+template <typename OT, bool EXACT, TiledMode MODE> void launch_tiled_form(const TiledArgs &p, int form, hipStream_t st) {
+    if (form == TILED_256) {
+        // (widened operands of a 64 x 128 wave tile do not fit its registers)
+        if constexpr (EXACT) launch_tiled<OT, EXACT, MODE, false, false, 4, 4, 2, 4, 3, 2>(p, st);
+        else launch_tiled<OT, EXACT, MODE, false, false, 4, 8, 4, 2, 2, 2>(p, st);
+    } else if (form == TILED_128_256) launch_tiled<OT, EXACT, MODE, false, false, 4, 4, 2, 4, 3, 2>(p, st);
+    else if (form == TILED_128) launch_tiled<OT, EXACT, MODE, false, false, 4, 4, 2, 2, 2, 2>(p, st);
+    else launch_tiled<OT, EXACT, MODE, false, false, 2, 4, 2, 2, 3, 2>(p, st);
+}
+
+void launch_tiled_f16(const TiledArgs &p, int form, hipStream_t st);
+void launch_tiled_bf16(const TiledArgs &p, int form, hipStream_t st);
+void launch_tiled_f32(const TiledArgs &p, int form, hipStream_t st);
+void launch_tiled_part(const TiledArgs &p, int form, hipStream_t st);
+void launch_tiled_part_exact(const TiledArgs &p, int form, hipStream_t st);
+
+TiledPlan block_fp8_tiled_plan(bool exact, int M, int N, int K);
+size_t block_fp8_tiled_part_bytes(const TiledPlan &plan, int M, int N);
+int launch_block_fp8_tiled(TiledArgs p, int dtype, const TiledPlan &plan, hipStream_t st);
+
+}  // namespace lowbit
