@@ -4,27 +4,25 @@
 // A workgroup of the first product owns 128 columns of h = act(g) u, which are one block of h's rows: it has every value that the
 // block's scale depends on, so h leaves as codes and never as 16-bit numbers.
 //
-// Few pairs (DIRECT): each pair streams its expert's weights, two launches.  More: the pairs sorted by expert, and row tiles of one
-// expert (find_expert_tile).
-#include "block_fp8.h"
+// The first product's sums go through the bfloat16 MFMA, which is exact (block_fp8.h): what the fp8 instruction drops, 1e-5 of a sum, would put one
+// of 3000 values of h on the other side of the border between two codes, 1.5e-3 of the result, more than its rounding to bfloat16 costs.
+// While the experts' weights are what takes the time, that costs nothing.
+//
+// Few pairs: each pair streams its expert's weights, two launches.  More: the pairs sorted by expert, and tiles of rows of one expert
+// (block_fp8_gemm.h).
+#include "block_fp8_tiled.h"
 
 namespace lowbit {
 
 void launch_moe_route(const int64_t *ids, int pairs, int n_exp, int32_t *offsets, int32_t *order, int32_t *pos, hipStream_t st);
 void launch_moe_combine(const void *y, const int32_t *pos, const void *weight, int w_dtype, void *out, int act_dtype, int tokens, int top_k,
                         int N, hipStream_t st);
-int launch_block_fp8_rows(const void *x, int dtype, int64_t rows, int K, uint8_t *codes, int ldc, float *scale, int64_t row_step,
-                          int64_t block_step, hipStream_t st);
-
 struct ExpertsArgs {
-    const void *x;                                           // DIRECT: activations [tokens, H]; else their codes, rows of ldx bytes
-    const float *xs;                                         // [blocks of H][ldxs]
-    int ldx, ldxs;
+    const void *x;                                           // [tokens, H]
     const int64_t *ids;
-    const int32_t *offsets, *order;
     const uint8_t *gate_up, *down;
     const float *gate_up_scale, *down_scale;
-    uint8_t *h;                                              // codes [pairs, I], by pair (DIRECT) or by sorted position
+    uint8_t *h;                                              // codes [pairs, I], by pair (few pairs) or by sorted position
     float *hs;                                               // [blocks of I][ldh]
     int ldh;
     int n_exp, top_k, H, I, act;
@@ -37,27 +35,17 @@ __device__ inline void load_chunks(const uint8_t *row, int kb, int left, Codes &
 }
 
 // Wave w: 16 columns of g and the same of u, all of K.
-template <typename AT, int MT, bool DIRECT>
-__global__ __launch_bounds__(512) void block_fp8_expert_up_kernel(const ExpertsArgs p) {
-    constexpr int STEPS = MT == 1 ? 4 : 2;
+template <typename AT>
+__global__ __launch_bounds__(512) void block_fp8_expert_token_up_kernel(const ExpertsArgs p) {
+    constexpr int STEPS = 4;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    __shared__ uint32_t part[8][16 * MT];
+    __shared__ uint32_t part[8];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
     const int cb = blockIdx.x, KB = fp8_blocks(p.H);
-    int expert, first, end;
-    if constexpr (DIRECT) {
-        const int64_t e = p.ids[blockIdx.y];
-        if (e < 0 || e >= p.n_exp) return;                   // (the second product skips the pair)
-        expert = (int)e;
-        first = blockIdx.y;
-        end = first + 1;
-    } else {
-        ExpertTile t;
-        if (!find_expert_tile<16 * MT>(p.offsets, p.n_exp, blockIdx.y, t)) return;
-        expert = t.expert;
-        first = t.first;
-        end = t.end;
-    }
+    const int pair = blockIdx.y;
+    const int64_t e = p.ids[pair];
+    if (e < 0 || e >= p.n_exp) return;                       // (the second product skips the pair)
+    const int expert = (int)e;
     const uint8_t *const w = p.gate_up + (int64_t)expert * 2 * p.I * p.H;
     const uint8_t *row[2];
     const float *ws[2];
@@ -73,51 +61,30 @@ __global__ __launch_bounds__(512) void block_fp8_expert_up_kernel(const ExpertsA
 #pragma unroll
             for (int t = 0; t < 2; t++) load_chunks(row[t], s, p.H - s * FP8_BLOCK - g * 16, wc[s][t]);
 
-    const uint8_t *xrow[MT];
-    const float *xs;
-    int xs_at[MT], xs_step;
-    if constexpr (DIRECT) {
-        float *const xs_lds = (float *)(lds + KB * FP8_BLOCK);
-        for (int kb = threadIdx.x >> 3; kb < KB; kb += 64) {
-            const int k = kb * FP8_BLOCK + (threadIdx.x & 7) * 16;
-            float v[16] = {}, s;
-            if (k < p.H) load16((const AT *)p.x + (int64_t)(first / p.top_k) * p.H + k, v);
-            *(u32x4 *)(lds + k) = quantize16<AT>(v, s);
-            if ((threadIdx.x & 7) == 0) xs_lds[kb] = s;
-        }
-        __syncthreads();
-        xrow[0] = lds + g * 16;
-        xs = xs_lds;
-        xs_at[0] = 0;
-        xs_step = 1;
-    } else {
-        xs = p.xs;
-        xs_step = p.ldxs;
-#pragma unroll
-        for (int i = 0; i < MT; i++) {
-            const int at = first + i * 16 + r, token = p.order[at < end ? at : end - 1] / p.top_k;
-            xrow[i] = (const uint8_t *)p.x + (int64_t)token * p.ldx + g * 16;
-            xs_at[i] = token;
-        }
+    float *const xs = (float *)(lds + KB * FP8_BLOCK);
+    for (int kb = threadIdx.x >> 3; kb < KB; kb += 64) {
+        const int k = kb * FP8_BLOCK + (threadIdx.x & 7) * 16;
+        float v[16] = {}, s;
+        if (k < p.H) load16((const AT *)p.x + (int64_t)(pair / p.top_k) * p.H + k, v);
+        *(u32x4 *)(lds + k) = quantize16<AT>(v, s);
+        if ((threadIdx.x & 7) == 0) xs[kb] = s;
     }
+    __syncthreads();
 
-    f32x4 acc[2][MT] = {};
+    f32x4 acc[2] = {};
     for (int kb0 = 0; kb0 < KB; kb0 += STEPS) {
 #pragma unroll
         for (int s = 0; s < STEPS; s++) {
             const int kb = kb0 + s;
             if (kb >= KB) break;
+            const uint8_t *const xr = lds + kb * FP8_BLOCK + g * 16;     // (all 16 rows of the operand are the one)
+            const Codes xc = {*(const u32x4 *)xr, *(const u32x4 *)(xr + 64)};
 #pragma unroll
-            for (int i = 0; i < MT; i++) {
-                const Codes xc = {*(const u32x4 *)(xrow[i] + kb * FP8_BLOCK), *(const u32x4 *)(xrow[i] + kb * FP8_BLOCK + 64)};
-                const float sx = xs[(int64_t)kb * xs_step + xs_at[i]];
+            for (int t = 0; t < 2; t++) {
+                const float sc = xs[kb] * ws[t][kb];
+                const f32x4 d = block_dot<true>(wc[s][t], xc);
 #pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    const float sc = sx * ws[t][kb];
-                    const f32x4 d = block_dot<false>(wc[s][t], xc);
-#pragma unroll
-                    for (int j = 0; j < 4; j++) acc[t][i][j] = fmaf(sc, d[j], acc[t][i][j]);
-                }
+                for (int j = 0; j < 4; j++) acc[t][j] = fmaf(sc, d[j], acc[t][j]);
             }
             if (kb + STEPS < KB)
 #pragma unroll
@@ -125,32 +92,23 @@ __global__ __launch_bounds__(512) void block_fp8_expert_up_kernel(const ExpertsA
         }
     }
 
-    float h[MT][4];
+    float h[4];
+    uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < MT; i++) {
-        uint32_t m = 0;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            h[i][j] = gate_act(acc[0][i][j], p.act) * acc[1][i][j];
-            m = max_u32(m, magnitude(h[i][j]));
-        }
-        m = max_u32(m, (uint32_t)__shfl_xor((int)m, 16));
-        m = max_u32(m, (uint32_t)__shfl_xor((int)m, 32));
-        if (g == 0) part[wave][i * 16 + r] = m;
+    for (int j = 0; j < 4; j++) {
+        h[j] = gate_act(acc[0][j], p.act) * acc[1][j];
+        m = max_u32(m, magnitude(h[j]));
     }
+    m = max_u32(m, (uint32_t)__shfl_xor((int)m, 16));
+    m = max_u32(m, (uint32_t)__shfl_xor((int)m, 32));
+    if (lane == 0) part[wave] = m;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < MT; i++) {
-        uint32_t m = 0;
-#pragma unroll
-        for (int v = 0; v < 8; v++) m = max_u32(m, part[v][i * 16 + r]);
-        const float s = block_scale(m), inv = __builtin_amdgcn_rcpf(s);
-        const int at = first + i * 16 + r;
-        if (at >= end) continue;
-        *(uint32_t *)(p.h + (int64_t)at * p.I + cb * FP8_BLOCK + wave * 16 + g * 4) =
-            encode4(h[i][0] * inv, h[i][1] * inv, h[i][2] * inv, h[i][3] * inv);
-        if (wave == 0 && g == 0) p.hs[(int64_t)cb * p.ldh + at] = s;
-    }
+    for (int v = 0; v < 8; v++) m = max_u32(m, part[v]);
+    const float s = block_scale(m), inv = __builtin_amdgcn_rcpf(s);
+    if (r != 0) return;
+    *(uint32_t *)(p.h + (int64_t)pair * p.I + cb * FP8_BLOCK + wave * 16 + g * 4) = encode4(h[0] * inv, h[1] * inv, h[2] * inv, h[3] * inv);
+    if (wave == 0 && g == 0) p.hs[(int64_t)cb * p.ldh + pair] = s;
 }
 
 // One token's 16 columns per workgroup: the blocks of all its pairs are dealt to the waves.
@@ -196,50 +154,57 @@ __global__ __launch_bounds__(512) void block_fp8_expert_down_token_kernel(const 
     }
 }
 
-// 16 columns of up to 16 * MT rows of one expert; the waves share K.
-template <typename AT, int MT>
-__global__ __launch_bounds__(512) void block_fp8_expert_down_kernel(const ExpertsArgs p, AT *__restrict__ y) {
-    __shared__ f32x4 sums[8][MT][64];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
-    const int n0 = blockIdx.x * 16, IB = p.I / FP8_BLOCK, HB = fp8_blocks(p.H);
-    ExpertTile t;
-    if (!find_expert_tile<16 * MT>(p.offsets, p.n_exp, blockIdx.y, t)) return;
-    const uint8_t *const row = p.down + ((int64_t)t.expert * p.H + n0 + r) * p.I + g * 16;
-    const float *const ws = p.down_scale + ((int64_t)t.expert * HB + n0 / FP8_BLOCK) * IB;
-    int at[MT];
-#pragma unroll
-    for (int i = 0; i < MT; i++) at[i] = t.first + i * 16 + r < t.end ? t.first + i * 16 + r : t.end - 1;
-    f32x4 acc[MT] = {};
-    for (int kb = wave; kb < IB; kb += 8) {
-        Codes wc;
-        load_chunks(row, kb, FP8_BLOCK, wc);
-#pragma unroll
-        for (int i = 0; i < MT; i++) {
-            const uint8_t *const xr = p.h + (int64_t)at[i] * p.I + kb * FP8_BLOCK + g * 16;
-            const Codes xc = {*(const u32x4 *)xr, *(const u32x4 *)(xr + 64)};
-            const float sc = p.hs[(int64_t)kb * p.ldh + at[i]] * ws[kb];
-            const f32x4 d = block_dot<false>(wc, xc);
-#pragma unroll
-            for (int j = 0; j < 4; j++) acc[i][j] = fmaf(sc, d[j], acc[i][j]);
-        }
+// Codes and scales of the rows of x, and the pairs sorted by expert, in one launch: the first workgroups quantize (32 blocks each), the rest place
+// four pairs each.  A wave counts the pairs that come before its own - those of lower experts, and the earlier ones of its expert - as
+// moe_sort_gather_kernel does; waves pairs + e write offsets[e].
+constexpr int EXPERTS_SORT_PAIRS = 4096;
+template <typename AT>
+__global__ __launch_bounds__(256) void block_fp8_expert_rows_kernel(const AT *__restrict__ x, const int64_t *__restrict__ ids, uint8_t *__restrict__ codes,
+                                                                    float *__restrict__ scale, int32_t *__restrict__ offsets, int32_t *__restrict__ order,
+                                                                    int32_t *__restrict__ pos, int tokens, int pairs, int n_exp, int K, int KB,
+                                                                    int quantizing) {
+    if ((int)blockIdx.x < quantizing) {
+        const int64_t unit = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
+        if (unit >= (int64_t)tokens * KB) return;
+        const int row = (int)(unit / KB), kb = (int)(unit - (int64_t)row * KB), k = kb * FP8_BLOCK + (threadIdx.x & 7) * 16;
+        float v[16] = {}, s;
+        if (k < K) load16(x + (int64_t)row * K + k, v);
+        *(u32x4 *)(codes + (int64_t)row * KB * FP8_BLOCK + k) = quantize16<AT>(v, s);
+        if ((threadIdx.x & 7) == 0) scale[(int64_t)kb * tokens + row] = s;
+        return;
     }
+    const int lane = threadIdx.x & 63, b = (blockIdx.x - quantizing) * 4 + (threadIdx.x >> 6);
+    if (b > pairs + n_exp) return;
+    const bool is_pair = b < pairs;
+    const int64_t own = is_pair ? ids[b] : b - pairs;
+    int before = 0;
+    for (int j0 = lane; j0 - lane < pairs; j0 += 512) {
+        int64_t e[8];
 #pragma unroll
-    for (int i = 0; i < MT; i++) sums[wave][i][lane] = acc[i];
-    __syncthreads();
-    for (int o = threadIdx.x; o < MT * 64; o += 512) {
-        const int i = o >> 6, l = o & 63, m = t.first + i * 16 + (l & 15);
-        f32x4 v = {};
+        for (int i = 0; i < 8; i++) e[i] = j0 + i * 64 < pairs ? ids[j0 + i * 64] : -1;
 #pragma unroll
-        for (int w = 0; w < 8; w++) v += sums[w][i][l];
-        if (m >= t.end) continue;
-#pragma unroll
-        for (int j = 0; j < 4; j++) y[(int64_t)m * p.H + n0 + (l >> 4) * 4 + j] = to_at<AT>(v[j]);
+        for (int i = 0; i < 8; i++)
+            before += __popcll(__ballot(e[i] >= 0 && e[i] < n_exp && (e[i] < own || (is_pair && e[i] == own && j0 + i * 64 < b))));
     }
+    if (lane != 0) return;
+    if (!is_pair) {
+        offsets[own] = before;
+        return;
+    }
+    const bool valid = own >= 0 && own < n_exp;
+    pos[b] = valid ? before : -1;
+    if (valid) order[before] = b;
 }
 
 // While there are no more pairs than experts few of them share one, and each streams its weights; the row of x fits LDS.
 static bool direct(int tokens, int top_k, int n_exp, int H) {
     return ((int64_t)tokens * top_k <= n_exp || tokens == 1) && fp8_blocks(H) * (FP8_BLOCK + 4) <= 65536 - 4096;
+}
+
+// Rows of a tile: as many as an expert has in the mean, that no more weights are read twice than have to be, and few rows stand idle.
+static int expert_tile_rows(int pairs, int n_exp) {
+    const int mean = pairs / n_exp;
+    return mean <= 32 ? 32 : mean <= 64 ? 64 : 128;
 }
 
 struct ExpertsSpace {
@@ -275,14 +240,6 @@ size_t block_fp8_experts_workspace_bytes(int tokens, int top_k, int n_exp, int H
     return experts_space(tokens, top_k, n_exp, H, I).bytes;
 }
 
-template <typename AT> static void launch_up(const ExpertsArgs &p, bool one_each, int pairs, hipStream_t st) {
-    const int cols = p.I / FP8_BLOCK;
-    if (one_each)
-        hipLaunchKernelGGL((block_fp8_expert_up_kernel<AT, 1, true>), dim3(cols, pairs), dim3(512), (size_t)fp8_blocks(p.H) * (FP8_BLOCK + 4), st, p);
-    else
-        hipLaunchKernelGGL((block_fp8_expert_up_kernel<AT, 4, false>), dim3(cols, (pairs + 63) / 64 + p.n_exp), dim3(512), 0, st, p);
-}
-
 template <typename AT> static void launch_down_token(const ExpertsArgs &p, const void *weight, int w_dtype, void *out, int tokens, hipStream_t st) {
     const dim3 grid(p.H / 16, tokens), block(512);
     if (w_dtype == DT_F32)
@@ -298,19 +255,40 @@ template <typename AT> static int launch_experts_t(ExpertsArgs p, const ExpertsS
     const int pairs = tokens * p.top_k;
     const bool one_each = direct(tokens, p.top_k, p.n_exp, p.H);
     if (one_each) {
-        launch_up<AT>(p, true, pairs, st);
+        hipLaunchKernelGGL((block_fp8_expert_token_up_kernel<AT>), dim3(p.I / FP8_BLOCK, pairs), dim3(512), (size_t)fp8_blocks(p.H) * (FP8_BLOCK + 4), st, p);
         launch_down_token<AT>(p, weight, w_dtype, out, tokens, st);
         return 0;
     }
     int32_t *const offsets = (int32_t *)(ws + at.offsets), *const order = (int32_t *)(ws + at.order), *const pos = (int32_t *)(ws + at.pos);
-    if (int rc = launch_block_fp8_rows(p.x, act_dtype, tokens, p.H, ws + at.x, at.ldx, (float *)(ws + at.xs), 1, at.ldxs, st)) return rc;
-    launch_moe_route(p.ids, pairs, p.n_exp, offsets, order, pos, st);
-    p.x = ws + at.x;
-    p.xs = (float *)(ws + at.xs);
-    p.offsets = offsets;
-    p.order = order;
-    launch_up<AT>(p, false, pairs, st);
-    hipLaunchKernelGGL((block_fp8_expert_down_kernel<AT, 4>), dim3(p.H / 16, (pairs + 63) / 64 + p.n_exp), dim3(512), 0, st, p, (AT *)(ws + at.y));
+    const int KB = fp8_blocks(p.H), quantizing = (int)(((int64_t)tokens * KB + 31) / 32);
+    const bool sorts = pairs <= EXPERTS_SORT_PAIRS;
+    hipLaunchKernelGGL((block_fp8_expert_rows_kernel<AT>), dim3(quantizing + (sorts ? (pairs + p.n_exp + 4) / 4 : 0)), dim3(256), 0, st, (const AT *)p.x,
+                       p.ids, ws + at.x, (float *)(ws + at.xs), offsets, order, pos, tokens, pairs, p.n_exp, p.H, KB, quantizing);
+    if (!sorts) launch_moe_route(p.ids, pairs, p.n_exp, offsets, order, pos, st);
+
+    TiledArgs t{};
+    t.offsets = offsets; t.order = order; t.n_exp = p.n_exp; t.top_k = p.top_k; t.M = pairs; t.I = p.I; t.act = p.act;
+    TiledArgs u = t;
+    u.x = ws + at.x; u.xs = (float *)(ws + at.xs); u.ldx = at.ldx; u.ldxs = at.ldxs;
+    u.w = p.gate_up; u.ws = p.gate_up_scale; u.N = 2 * p.I; u.K = p.H; u.KB = KB;
+    u.y = p.h; u.hs = p.hs; u.ldhs = p.ldh;
+    TiledArgs d = t;
+    d.x = p.h; d.xs = p.hs; d.ldx = p.I; d.ldxs = p.ldh;
+    d.w = p.down; d.ws = p.down_scale; d.N = p.H; d.K = p.I; d.KB = p.I / FP8_BLOCK;
+    d.y = ws + at.y;
+    const int rows = expert_tile_rows(pairs, p.n_exp);
+    u.tiles_m = d.tiles_m = pairs / rows + (pairs < p.n_exp ? pairs : p.n_exp);      // at most
+    if ((int64_t)u.tiles_m * (p.I / FP8_BLOCK) > 0x7fffffff - 8 || (int64_t)d.tiles_m * ((p.H + 127) / 128) > 0x7fffffff - 8) return -3;
+    if (rows == 128) {
+        launch_tiled<AT, true, TILED_UP, true, true, 4, 4, 2, 4, 3, 2>(u, st);
+        launch_tiled<AT, false, TILED_PLAIN, true, false, 4, 4, 2, 4, 3, 2>(d, st);
+    } else if (rows == 64) {
+        launch_tiled<AT, true, TILED_UP, true, true, 2, 4, 2, 4, 3, 2>(u, st);
+        launch_tiled<AT, false, TILED_PLAIN, true, false, 2, 4, 2, 2, 3, 2>(d, st);
+    } else {
+        launch_tiled<AT, true, TILED_UP, true, true, 2, 4, 1, 4, 4, 1>(u, st);
+        launch_tiled<AT, false, TILED_PLAIN, true, false, 2, 2, 1, 4, 3, 2>(d, st);
+    }
     launch_moe_combine(ws + at.y, pos, weight, w_dtype, out, act_dtype, tokens, p.top_k, p.H, st);
     return 0;
 }
@@ -321,7 +299,7 @@ int launch_block_fp8_experts(const void *x, const int64_t *ids, const void *weig
     const ExpertsSpace at = experts_space(tokens, top_k, n_exp, H, I);
     uint8_t *const ws = (uint8_t *)workspace;
     ExpertsArgs p{};
-    p.x = x; p.ids = ids; p.ldx = at.ldx; p.ldxs = at.ldxs; p.ldh = at.ldh;
+    p.x = x; p.ids = ids; p.ldh = at.ldh;
     p.gate_up = gate_up; p.down = down; p.gate_up_scale = gate_up_scale; p.down_scale = down_scale;
     p.h = ws + at.h; p.hs = (float *)(ws + at.hs);
     p.n_exp = n_exp; p.top_k = top_k; p.H = H; p.I = I; p.act = act;

@@ -16,7 +16,7 @@ namespace lowbit {
 
 struct TiledArgs {
     const uint8_t *x;                                        // codes, rows of ldx bytes, zeros past K
-    const float *xs;                                         // [KB][ldxs], rows of the result
+    const float *xs;                                         // [KB][ldxs], by row of x
     const uint8_t *w;
     const float *ws;
     const void *bias;
@@ -169,8 +169,8 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void block_fp8_tiled_kerne
     const uint32_t lds_x = lds0 + wave * PX * 1024, lds_w = lds0 + BM * FP8_BLOCK;
     // x's scales of a block come the same way, BM / WAVES rows per wave (rows past the end: the last one's)
     constexpr int RS = BM / WAVES;
-    const int srow = m0 + wave * RS + (lane < RS ? lane : 0);
-    const uint32_t soff = (uint32_t)(srow < end ? srow : end - 1) * 4, lds_s = lds0 + S * BUFFER + wave * RS * 4;
+    const int sat = m0 + wave * RS + (lane < RS ? lane : 0), srow = sat < end ? sat : end - 1;
+    const uint32_t soff = (uint32_t)(GATHER ? p.order[srow] / p.top_k : srow) * 4, lds_s = lds0 + S * BUFFER + wave * RS * 4;
     // Pieces of a block in the order in which a wave asks for them: x, its scales, weights.  They are asked for one at a time between the
     // products: all at once, from all waves, they queue at the CU's address unit and the waves stand still (8192^3: 553 us against 489).
     constexpr int PIECES = PX + 1 + PW;
