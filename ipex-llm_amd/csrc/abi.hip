@@ -56,7 +56,7 @@ double narrow_time_us(int M, int N, int K, int qtype, bool linear);
 int gemm_splits(int M, int N, int K, size_t ws_bytes, int qtype);
 double gemm_time_us(int M, int N, int K, int splits, int qtype);
 bool gemm_prefers_tall(int qtype, int act_dtype, int M, int N, int K);
-int launch_block_fp8_rows(const void *x, int dtype, int64_t rows, int K, uint8_t *codes, int ldc, float *scale, int64_t row_step,
+int launch_block_fp8_rows(const void *x, int dtype, int64_t rows, int K, uint8_t *codes, int ldc, bool wide, float *scale, int64_t row_step,
                           int64_t block_step, hipStream_t st);
 int launch_block_fp8_weight(const void *w, int dtype, int64_t matrices, int N, int K, uint8_t *codes, float *scale, hipStream_t st);
 size_t block_fp8_linear_workspace_bytes(int dtype, int M, int N, int K);
@@ -757,7 +757,7 @@ int lowbit_block_fp8_quantize(const void *x, int dtype, int64_t rows, int64_t K,
     if (!x || !codes || !scale || !aligned16(x) || !aligned16(codes) || (((uintptr_t)scale) & 3))
         return fail(LOWBIT_EARG, "%s: null or misaligned pointer", what);
     if (rows > (int64_t)1 << 40) return fail(LOWBIT_ESIZE, "%s: too many rows", what);
-    return check_launch(launch_block_fp8_rows(x, dtype, rows, (int)K, (uint8_t *)codes, (int)K, scale, (K + 127) / 128, 1, (hipStream_t)stream), what);
+    return check_launch(launch_block_fp8_rows(x, dtype, rows, (int)K, (uint8_t *)codes, (int)K, false, scale, (K + 127) / 128, 1, (hipStream_t)stream), what);
 }
 
 int lowbit_block_fp8_quantize_weight(const void *w, int dtype, int64_t matrices, int64_t N, int64_t K, void *codes, float *scale,

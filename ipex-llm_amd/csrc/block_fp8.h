@@ -26,6 +26,12 @@ constexpr uint32_t FP8_LEAST_BITS = 27u << 23;
 
 __host__ __device__ inline int fp8_blocks(int k) { return (k + FP8_BLOCK - 1) / FP8_BLOCK; }
 
+// eight codes as bfloat16, exactly: an operand of the bfloat16 MFMA
+__device__ inline bf16x8 widen8(uint32_t w0, uint32_t w1) {
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, 1.0f, true);
+    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, 1.0f, true);
+    return {a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
 // 32 bytes of one row: chunks g and 4 + g of a block of 128.
 struct Codes {
     u32x4 lo, hi;
@@ -40,18 +46,10 @@ template <bool EXACT> __device__ inline f32x4 block_dot(const Codes &a, const Co
         return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(va, vb, zero, 0, 0, 0, 0, 0, 0);    // formats e4m3, no block exponents
     } else {
         f32x4 d = zero;
-        auto widen = [](uint32_t w0, uint32_t w1) {
-            bf16x8 v;
-            const f32x2 p = __builtin_amdgcn_cvt_pk_f32_fp8(w0, false), q = __builtin_amdgcn_cvt_pk_f32_fp8(w0, true);
-            const f32x2 r = __builtin_amdgcn_cvt_pk_f32_fp8(w1, false), s = __builtin_amdgcn_cvt_pk_f32_fp8(w1, true);
-            v[0] = (__bf16)p[0]; v[1] = (__bf16)p[1]; v[2] = (__bf16)q[0]; v[3] = (__bf16)q[1];
-            v[4] = (__bf16)r[0]; v[5] = (__bf16)r[1]; v[6] = (__bf16)s[0]; v[7] = (__bf16)s[1];
-            return v;
-        };
 #pragma unroll
-        for (int h = 0; h < 2; h++) d = mfma16(widen(a.lo[2 * h], a.lo[2 * h + 1]), widen(b.lo[2 * h], b.lo[2 * h + 1]), d);
+        for (int h = 0; h < 2; h++) d = mfma16(widen8(a.lo[2 * h], a.lo[2 * h + 1]), widen8(b.lo[2 * h], b.lo[2 * h + 1]), d);
 #pragma unroll
-        for (int h = 0; h < 2; h++) d = mfma16(widen(a.hi[2 * h], a.hi[2 * h + 1]), widen(b.hi[2 * h], b.hi[2 * h + 1]), d);
+        for (int h = 0; h < 2; h++) d = mfma16(widen8(a.hi[2 * h], a.hi[2 * h + 1]), widen8(b.hi[2 * h], b.hi[2 * h + 1]), d);
         return d;
     }
 }
@@ -131,8 +129,16 @@ template <typename AT> __device__ inline u32x4 quantize16(const float (&v)[16], 
     return c;
 }
 
+// 16 codes of a row to its k-th byte, or (WIDE) the same numbers in bfloat16
+template <bool WIDE> __device__ inline void store16(uint8_t *row, int k, u32x4 c) {
+    if constexpr (WIDE) {
+        *(bf16x8 *)(row + 2 * k) = widen8(c[0], c[1]);
+        *(bf16x8 *)(row + 2 * k + 16) = widen8(c[2], c[3]);
+    } else *(u32x4 *)(row + k) = c;
+}
+
 // Which rows a workgroup of a product grouped by expert works on: row tiles of ROWS rows, expert after expert; called by whole waves.
-// count = number of row tiles in all; returns false past the last.
+// Returns false past the last.
 struct ExpertTile {
     int expert, first, end;                                  // rows first .. end - 1 (end: the expert's, not the tile's)
 };
@@ -160,6 +166,15 @@ template <int ROWS> __device__ inline bool find_expert_tile(const int32_t *__res
         tile -= all;
     }
     return false;
+}
+
+// Number of row tiles of all experts.
+template <int ROWS> __device__ inline int count_expert_tiles(const int32_t *__restrict__ offsets, int n_exp) {
+    int all = 0;
+    for (int e = threadIdx.x & 63; e < n_exp; e += 64) all += (offsets[e + 1] - offsets[e] + ROWS - 1) / ROWS;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) all += __shfl_xor(all, d);
+    return __builtin_amdgcn_readfirstlane(all);
 }
 
 // act(g) * u in float32: hardware exp2 and reciprocal, 1 unit of 2^-24 each, ahead of a rounding to 4 bits

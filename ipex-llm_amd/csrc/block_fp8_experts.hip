@@ -154,7 +154,7 @@ __global__ __launch_bounds__(512) void block_fp8_expert_down_token_kernel(const 
     }
 }
 
-// Codes and scales of the rows of x, and the pairs sorted by expert, in one launch: the first workgroups quantize (32 blocks each), the rest place
+// The rows of x in codes (as bfloat16 numbers, see EXACT) and scales, and the pairs sorted by expert, in one launch: the first workgroups quantize (32 blocks each), the rest place
 // four pairs each.  A wave counts the pairs that come before its own - those of lower experts, and the earlier ones of its expert - as
 // moe_sort_gather_kernel does; waves pairs + e write offsets[e].
 constexpr int EXPERTS_SORT_PAIRS = 4096;
@@ -169,7 +169,7 @@ __global__ __launch_bounds__(256) void block_fp8_expert_rows_kernel(const AT *__
         const int row = (int)(unit / KB), kb = (int)(unit - (int64_t)row * KB), k = kb * FP8_BLOCK + (threadIdx.x & 7) * 16;
         float v[16] = {}, s;
         if (k < K) load16(x + (int64_t)row * K + k, v);
-        *(u32x4 *)(codes + (int64_t)row * KB * FP8_BLOCK + k) = quantize16<AT>(v, s);
+        store16<true>(codes + (int64_t)row * KB * (2 * FP8_BLOCK), k, quantize16<AT>(v, s));
         if ((threadIdx.x & 7) == 0) scale[(int64_t)kb * tokens + row] = s;
         return;
     }
@@ -220,7 +220,7 @@ static ExpertsSpace experts_space(int tokens, int top_k, int n_exp, int H, int I
         at += (bytes + 255) & ~(size_t)255;
         return here;
     };
-    w.ldx = fp8_blocks(H) * FP8_BLOCK;
+    w.ldx = fp8_blocks(H) * FP8_BLOCK * 2;
     w.ldxs = tokens;
     w.ldh = (int)pairs;
     w.h = take((size_t)pairs * I);
@@ -280,13 +280,13 @@ template <typename AT> static int launch_experts_t(ExpertsArgs p, const ExpertsS
     u.tiles_m = d.tiles_m = pairs / rows + (pairs < p.n_exp ? pairs : p.n_exp);      // at most
     if ((int64_t)u.tiles_m * (p.I / FP8_BLOCK) > 0x7fffffff - 8 || (int64_t)d.tiles_m * ((p.H + 127) / 128) > 0x7fffffff - 8) return -3;
     if (rows == 128) {
-        launch_tiled<AT, true, TILED_UP, true, true, 4, 4, 2, 4, 3, 2>(u, st);
+        launch_tiled<AT, true, TILED_UP, true, true, 4, 4, 2, 4, 2, 2>(u, st);
         launch_tiled<AT, false, TILED_PLAIN, true, false, 4, 4, 2, 4, 3, 2>(d, st);
     } else if (rows == 64) {
         launch_tiled<AT, true, TILED_UP, true, true, 2, 4, 2, 4, 3, 2>(u, st);
         launch_tiled<AT, false, TILED_PLAIN, true, false, 2, 4, 2, 2, 3, 2>(d, st);
     } else {
-        launch_tiled<AT, true, TILED_UP, true, true, 2, 4, 1, 4, 4, 1>(u, st);
+        launch_tiled<AT, true, TILED_UP, true, true, 2, 4, 1, 4, 3, 1>(u, st);
         launch_tiled<AT, false, TILED_PLAIN, true, false, 2, 2, 1, 4, 3, 2>(d, st);
     }
     launch_moe_combine(ws + at.y, pos, weight, w_dtype, out, act_dtype, tokens, p.top_k, p.H, st);

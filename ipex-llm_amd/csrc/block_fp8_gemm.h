@@ -7,7 +7,10 @@
 // LDS holds rows of 128 bytes, the 16-byte chunk c of row r at slot c ^ swizzle(r): the DMA writes 8 rows of 8 slots at a time (lane
 // = 8 * row + slot, so the swizzle is in the lane's source address), and 16 lanes of a read, which take one chunk of 16
 // consecutive rows, cover all 64 banks: two rows are 256 bytes, and the eight rows of one parity have different slots.  (With slots that
-// repeat after four rows half of LDS' busy cycles were conflicts, 8192^3 in 567 us against SWIZZLED.)
+// repeat after four rows half of LDS' busy cycles were conflicts.)
+//
+// EXACT, for sums that keep float32's 24 bits (block_fp8.h): the bfloat16 MFMA, four instructions of 32 values in place of one.  x comes as
+// bfloat16 numbers, rows of 256 bytes a block, and only the weight's codes are widened on the way from LDS, part by part.
 #pragma once
 #include "block_fp8.h"
 #include "lowbit_gemm.h"
@@ -15,7 +18,7 @@
 namespace lowbit {
 
 struct TiledArgs {
-    const uint8_t *x;                                        // codes, rows of ldx bytes, zeros past K
+    const uint8_t *x;                                        // codes (EXACT: their numbers in bfloat16), rows of ldx bytes, zeros past K
     const float *xs;                                         // [KB][ldxs], by row of x
     const uint8_t *w;
     const float *ws;
@@ -50,32 +53,22 @@ __device__ inline void dma16_at(uint64_t address, uint32_t lds_at) {
 // (the other two counters untouched: 4 bits of lgkmcnt at 8)
 __device__ inline void wait_lds() { __builtin_amdgcn_s_waitcnt(0xC07F); }
 
-// codes of a lane as bfloat16, exactly: eight values per MFMA operand
-__device__ inline bf16x8 widen8(uint32_t w0, uint32_t w1) {
-    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, 1.0f, true);
-    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, 1.0f, true);
-    return {a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+// The part of a lane's 32 codes that the p-th of four bfloat16 MFMAs takes
+__device__ inline bf16x8 widen_part(const Codes &c, int p) {
+    const u32x4 &h = p < 2 ? c.lo : c.hi;
+    return widen8(h[2 * (p & 1)], h[2 * (p & 1) + 1]);
 }
-template <bool EXACT> struct Operand;
-template <> struct Operand<false> {
-    i32x8 v;
-    __device__ void take(u32x4 lo, u32x4 hi) {
-        v = i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
-    }
-    __device__ f32x4 dot(const Operand &o) const {
-        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(v, o.v, f32x4{}, 0, 0, 0, 0, 0, 0);
-    }
+// A lane's values of x: codes, or (EXACT) the same numbers in bfloat16, part by part
+template <bool EXACT> struct XOperand;
+template <> struct XOperand<false> {
+    Codes v;
 };
-template <> struct Operand<true> {
+template <> struct XOperand<true> {
     bf16x8 v[4];
-    __device__ void take(u32x4 lo, u32x4 hi) {
-        v[0] = widen8(lo[0], lo[1]);
-        v[1] = widen8(lo[2], lo[3]);
-        v[2] = widen8(hi[0], hi[1]);
-        v[3] = widen8(hi[2], hi[3]);
-    }
-    __device__ f32x4 dot(const Operand &o) const { return mfma16(v[3], o.v[3], mfma16(v[2], o.v[2], mfma16(v[1], o.v[1], mfma16(v[0], o.v[0], f32x4{})))); }
 };
+__device__ inline i32x8 joined(const Codes &c) {
+    return {(int)c.lo[0], (int)c.lo[1], (int)c.lo[2], (int)c.lo[3], (int)c.hi[0], (int)c.hi[1], (int)c.hi[2], (int)c.hi[3]};
+}
 
 template <typename OT> struct Stored;
 template <> struct Stored<float> {
@@ -91,7 +84,8 @@ template <> struct Stored<__bf16> {
 // BY_EXPERT: row tiles of one expert each.  GATHER: x rows by order[].  S: buffers in LDS.
 template <typename OT, bool EXACT, TiledMode MODE, bool BY_EXPERT, bool GATHER, int TM, int TN, int WM, int WN, int S, int MIN_WAVES>
 __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void block_fp8_tiled_kernel(const TiledArgs p) {
-    constexpr int WAVES = WM * WN, BM = WM * TM * 16, BN = WN * TN * 16, XP = BM / 8, WP = BN / 8;
+    constexpr int WAVES = WM * WN, BM = WM * TM * 16, BN = WN * TN * 16;
+    constexpr int XB = EXACT ? 256 : 128, XR = 1024 / XB, XP = BM / XR, WP = BN / 8;   // bytes of a row of x, rows of a piece, pieces
     constexpr int PX = XP / WAVES, PW = WP / WAVES;
     constexpr bool UP = MODE == TILED_UP;
     constexpr int TH = TN / 2;                               // UP: a wave's tiles of the gate, and as many of u
@@ -99,22 +93,24 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void block_fp8_tiled_kerne
     constexpr int HALVES = S == 2 ? 2 : 1, PH = PW / HALVES;
     static_assert(WP % (WAVES * HALVES) == 0 && XP % WAVES == 0 && PX > 0 && BM / WAVES <= 64 && TN % 2 == 0 && (S > 2 || TN % 4 == 0 || TN == 2) &&
                   (!UP || BN == 256), "whole pieces per wave");
-    constexpr uint32_t BUFFER = (BM + BN) * FP8_BLOCK, SCALES = BM * 4;
+    constexpr uint32_t BUFFER = BM * XB + BN * FP8_BLOCK, SCALES = BM * 4;
     __shared__ __attribute__((aligned(16))) uint8_t lds[S * (BUFFER + SCALES)];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
     const int wm = wave / WN, wn = wave % WN;
 
     // Workgroups go to the XCDs in turn: each takes a run of the tiles, eight row tiles by as many columns as its CUs hold, so that
-    // its L2 serves every operand several times.
-    const uint32_t units = (uint32_t)(p.tiles_m * p.tiles_n * p.splits), xcd = blockIdx.x & 7;
+    // its L2 serves every operand several times.  By expert: all row tiles of a column side by side, those that there are (the launch
+    // counts what there may be at most; runs of tiles of which some do not exist would leave XCDs idle).
+    const int tiles_m = BY_EXPERT ? count_expert_tiles<BM>(p.offsets, p.n_exp) : p.tiles_m, tall = BY_EXPERT ? tiles_m : 8;
+    const uint32_t units = (uint32_t)(tiles_m * p.tiles_n * p.splits), xcd = blockIdx.x & 7;
     const uint32_t unit = (uint32_t)((uint64_t)units * xcd >> 3) + (blockIdx.x >> 3);
     if (unit >= (uint32_t)((uint64_t)units * (xcd + 1) >> 3)) return;
     const int tile = (int)(unit / p.splits), split = (int)(unit - (uint32_t)tile * p.splits);
     int tm, tn;
     {
-        const int per = 8 * p.tiles_n, band = tile / per, at = tile - band * per, rows = p.tiles_m - band * 8 < 8 ? p.tiles_m - band * 8 : 8;
+        const int per = tall * p.tiles_n, band = tile / per, at = tile - band * per, rows = tiles_m - band * tall < tall ? tiles_m - band * tall : tall;
         tn = at / rows;
-        tm = band * 8 + at - tn * rows;
+        tm = band * tall + at - tn * rows;
     }
     int m0 = tm * BM, end = p.M, expert = 0;
     if constexpr (BY_EXPERT) {
@@ -134,7 +130,7 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void block_fp8_tiled_kerne
     const uint64_t xbase = (uint64_t)(uintptr_t)p.x + (GATHER ? 0 : (uint64_t)m0 * p.ldx);
 #pragma unroll
     for (int j = 0; j < PX; j++) {
-        const int row = (wave * PX + j) * 8 + piece_row, chunk = ((lane & 7) ^ swizzle(row)) * 16;
+        const int row = (wave * PX + j) * XR + lane / (XB / 16), chunk = ((lane % (XB / 16)) ^ (EXACT ? row & 15 : swizzle(row))) * 16;
         const int at = m0 + row < end ? m0 + row : end - 1;
         if constexpr (GATHER) xaddr[j] = xbase + (uint64_t)(p.order[at] / p.top_k) * p.ldx + chunk;
         else xoff[j] = (uint32_t)((at - m0) * p.ldx) + chunk;
@@ -166,7 +162,7 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void block_fp8_tiled_kerne
         woff[j] = (uint32_t)(weight_row(first + piece_row) - from) * p.K + wchunk[first / 8 & 1];
     }
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds;
-    const uint32_t lds_x = lds0 + wave * PX * 1024, lds_w = lds0 + BM * FP8_BLOCK;
+    const uint32_t lds_x = lds0 + wave * PX * 1024, lds_w = lds0 + BM * XB;
     // x's scales of a block come the same way, BM / WAVES rows per wave (rows past the end: the last one's)
     constexpr int RS = BM / WAVES;
     const int sat = m0 + wave * RS + (lane < RS ? lane : 0), srow = sat < end ? sat : end - 1;
@@ -177,8 +173,8 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void block_fp8_tiled_kerne
     auto fetch = [&](int kb, int which, int q) __attribute__((always_inline)) {
         const uint32_t buffer = which * BUFFER;
         if (q < PX) {
-            if constexpr (GATHER) dma16_at(xaddr[q] + (uint64_t)kb * FP8_BLOCK, lds_x + buffer + q * 1024);
-            else dma16(xoff[q], xbase + (uint64_t)kb * FP8_BLOCK, lds_x + buffer + q * 1024);
+            if constexpr (GATHER) dma16_at(xaddr[q] + (uint64_t)kb * XB, lds_x + buffer + q * 1024);
+            else dma16(xoff[q], xbase + (uint64_t)kb * XB, lds_x + buffer + q * 1024);
         } else if (q == PX) {
             if (lane < RS) dma4(soff, (uint64_t)(uintptr_t)(p.xs + (int64_t)kb * p.ldxs), lds_s + which * SCALES);
         } else {
@@ -207,14 +203,21 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void block_fp8_tiled_kerne
         asm volatile("" : "+v"(wheld[0]));
         if constexpr (UP) asm volatile("" : "+v"(wheld[1]));
     };
-    // ---- operands: lane (r, g) reads the chunks g and 4 + g of row r of a tile
-    const int xlo = (wm * TM * 16 + r) * FP8_BLOCK + (g ^ swizzle(r)) * 16, wlo = xlo + (BM + wn * TN * 16 - wm * TM * 16) * FP8_BLOCK;
-    auto read = [&](int lo, int tile, Operand<EXACT> &o) __attribute__((always_inline)) {
-        const uint8_t *const at = lds + tile * 16 * FP8_BLOCK;
-        o.take(*(const u32x4 *)(at + lo), *(const u32x4 *)(at + (lo ^ 64)));
+    // ---- operands: lane (r, g) reads the chunks g and 4 + g of row r of a tile (EXACT: of x those of the same numbers, 2 g and 2 g + 1 and
+    // eight on; its sixteen slots are turned by the row)
+    const int wlo = BM * XB + (wn * TN * 16 + r) * FP8_BLOCK + (g ^ swizzle(r)) * 16;
+    const int xlo = (wm * TM * 16 + r) * XB + ((EXACT ? 2 * g : g) ^ (EXACT ? r : swizzle(r))) * 16;
+    auto read_x = [&](int buffer, int i, XOperand<EXACT> &o) __attribute__((always_inline)) {
+        const uint8_t *const at = lds + buffer + i * 16 * XB;
+        if constexpr (EXACT) {
+#pragma unroll
+            for (int c = 0; c < 4; c++) o.v[c] = *(const bf16x8 *)(at + (xlo ^ ((c & 1) * 16 + (c >> 1) * 128)));
+        } else o.v = Codes{*(const u32x4 *)(at + xlo), *(const u32x4 *)(at + (xlo ^ 64))};
     };
-    auto read_x = [&](int buffer, int i, Operand<EXACT> &o) __attribute__((always_inline)) { read(xlo + buffer, i, o); };
-    auto read_w = [&](int buffer, int i, Operand<EXACT> &o) __attribute__((always_inline)) { read(wlo + buffer, i, o); };
+    auto read_w = [&](int buffer, int i, Codes &o) __attribute__((always_inline)) {
+        const uint8_t *const at = lds + buffer + i * 16 * FP8_BLOCK;
+        o = Codes{*(const u32x4 *)(at + wlo), *(const u32x4 *)(at + (wlo ^ 64))};
+    };
 
     // A step: TN tiles of TM products each.  A product is added while the next ones run, LAG instructions later; a tile's operands are read
     // one tile ahead.  The barrier that publishes the next block stands ahead of the last tile, whose operands are in registers: its
@@ -224,13 +227,16 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void block_fp8_tiled_kerne
     // A load takes about as long as a step of the largest tile, so it is asked for more than a step ahead.  Where there is room for two
     // buffers only, a second barrier stands in the middle: it frees x, which is in registers, and the first half of the weights, whose
     // next block but one is asked for there; the second half's at the other barrier.  Each has a step and a half to arrive.
-    constexpr int COUNT = TN * TM, LAG = COUNT - TM < 3 ? COUNT - TM : 3, EARLY = PIECES - (HALVES - 1) * PH, TURN = HALVES == 2 ? (TN / 2 - 1) * TM : -1;
+    constexpr int COUNT = TN * TM, LAG = EXACT ? TM : COUNT - TM < 3 ? COUNT - TM : 3, PARTS = EXACT ? 4 : 1, EARLY = PIECES - (HALVES - 1) * PH, TURN = HALVES == 2 ? (TN / 2 - 1) * TM : -1;
     constexpr int IN_FLIGHT = HALVES == 2 ? PIECES : (S - 2) * PIECES;       // loads of this wave that a barrier leaves under way
     constexpr int SLOTS = COUNT / HALVES, PER = ((HALVES == 2 ? EARLY : PIECES) + SLOTS - 1) / SLOTS;       // pieces asked for per product
     static_assert(IN_FLIGHT < 64, "vmcnt has 6 bits");
     f32x4 acc[TN][TM] = {};
-    Operand<EXACT> b[TM], a[2];
-    f32x4 d[LAG + 1];
+    XOperand<EXACT> b[TM];
+    Codes a[2];
+    bf16x8 wide[2];                                          // EXACT: the part in use and the next one
+    constexpr int RING = EXACT ? 2 * TM : LAG + 1;
+    f32x4 d[RING];
     float s[UP ? 2 : 1][TM], xs[TM];
     auto read_xs = [&](int which) __attribute__((always_inline)) {
 #pragma unroll
@@ -247,13 +253,21 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void block_fp8_tiled_kerne
     auto add = [&](int o) __attribute__((always_inline)) {
         f32x4 &sum = acc[o / TM][o % TM];
 #pragma unroll
-        for (int j = 0; j < 4; j++) sum[j] = fmaf(s[UP ? o / TM / TH : 0][o % TM], d[o % (LAG + 1)][j], sum[j]);
+        for (int j = 0; j < 4; j++) sum[j] = fmaf(s[UP ? o / TM / TH : 0][o % TM], d[o % RING][j], sum[j]);
         asm volatile("" : "+v"(sum));                        // (here, and not behind the barrier, where nothing covers them)
     };
     // pieces first .. last - 1 of a block, PER of them in slot 0, 1, ..
     auto fetch_slot = [&](int kb, int which, int first, int last, int slot) __attribute__((always_inline)) {
 #pragma unroll
         for (int q = first + slot * PER; q < first + (slot + 1) * PER && q < last; q++) fetch(kb, which, q);
+    };
+    // part c of product (t, i); EXACT: the parts of a tile's products one after the other, the next part widened among the first of them
+    auto product = [&](int t, int i, int c, const Codes &w, const Codes &then) __attribute__((always_inline)) {
+        f32x4 &to = d[(t * TM + i) % RING];
+        if constexpr (EXACT) {
+            to = mfma16(wide[c & 1], b[i].v[c], c ? to : f32x4{});
+            if (i == 0) wide[(c + 1) & 1] = c < 3 ? widen_part(w, c + 1) : widen_part(then, 0);
+        } else to = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(joined(w), joined(b[i].v), f32x4{}, 0, 0, 0, 0, 0, 0);
     };
     auto meet = [&]() __attribute__((always_inline)) {       // what was asked for IN_FLIGHT pieces ago is there, and every wave's reads are done
         wait_loads_but<IN_FLIGHT>();
@@ -281,6 +295,7 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void block_fp8_tiled_kerne
 #pragma unroll
     for (int i = 0; i < TM; i++) read_x(0, i, b[i]);
     read_w(0, 0, a[0]);
+    if constexpr (EXACT) wide[0] = widen_part(a[0], 0);
     read_xs(0);
 #pragma unroll
     for (int i = 0; i < TM; i++) {                           // what the last tile of a step before this one would have asked for
@@ -293,30 +308,40 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void block_fp8_tiled_kerne
         const int behind = which > 0 ? which - 1 : S - 1;    // the buffer that the step before this one freed
         scales(kb);
 #pragma unroll
-        for (int o = 0; o < COUNT - TM; o++) {
-            const int t = o / TM, i = o % TM;
-            if (o == TURN) meet();
-            if (i == 0) read_w(buffer, t + 1, a[(t + 1) & 1]);
-            d[o % (LAG + 1)] = a[t & 1].dot(b[i]);
-            if (o >= LAG) add(o - LAG);
-            if constexpr (HALVES == 2) {
-                if (o < TURN) fetch_slot(late, behind, EARLY, PIECES, TM + o);
-                else fetch_slot(next, which, 0, EARLY, o - TURN);
-            } else fetch_slot(late, behind, 0, PIECES, TM + o);
-            __builtin_amdgcn_sched_barrier(0);
+        for (int t = 0; t < TN - 1; t++) {
+            if (t * TM == TURN) meet();
+            read_w(buffer, t + 1, a[(t + 1) & 1]);
+#pragma unroll
+            for (int c = 0; c < PARTS; c++)
+#pragma unroll
+                for (int i = 0; i < TM; i++) {
+                    const int o = t * TM + i;
+                    product(t, i, c, a[t & 1], a[(t + 1) & 1]);
+                    if (c == PARTS / 4 && o >= LAG) add(o - LAG);
+                    if (c == 0) {
+                        if constexpr (HALVES == 2) {
+                            if (o < TURN) fetch_slot(late, behind, EARLY, PIECES, TM + o);
+                            else fetch_slot(next, which, 0, EARLY, o - TURN);
+                        } else fetch_slot(late, behind, 0, PIECES, TM + o);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
         }
         meet();
+        read_w(other, 0, a[TN & 1]);
 #pragma unroll
-        for (int i = 0; i < TM; i++) {
-            const int o = COUNT - TM + i;
-            d[o % (LAG + 1)] = a[(TN - 1) & 1].dot(b[i]);
-            read_x(other, i, b[i]);
-            if (i == TM - 1) read_w(other, 0, a[TN & 1]);
-            add(o - LAG);
-            if constexpr (HALVES == 2) fetch_slot(next, which, EARLY, PIECES, i);
-            else fetch_slot(next, which, 0, PIECES, i);
-            __builtin_amdgcn_sched_barrier(0);
-        }
+        for (int c = 0; c < PARTS; c++)
+#pragma unroll
+            for (int i = 0; i < TM; i++) {
+                product(TN - 1, i, c, a[(TN - 1) & 1], a[TN & 1]);
+                if (c == PARTS - 1) read_x(other, i, b[i]);
+                if (c == PARTS / 4) add(COUNT - TM + i - LAG);
+                if (c == 0) {
+                    if constexpr (HALVES == 2) fetch_slot(next, which, EARLY, PIECES, i);
+                    else fetch_slot(next, which, 0, PIECES, i);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
         read_xs(then);
 #pragma unroll
         for (int o = COUNT - LAG; o < COUNT; o++) add(o);

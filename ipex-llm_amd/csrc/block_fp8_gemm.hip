@@ -43,8 +43,8 @@ static float tiled_us(int form, int M, int N, int KB, int splits, bool exact) {
 
 TiledPlan block_fp8_tiled_plan(bool exact, int M, int N, int K) {
     const int KB = fp8_blocks(K);
-    TiledPlan best = {0, 1, 0.0f};
-    for (int form = 0; form < TILED_COUNT; form++) {
+    TiledPlan best = {TILED_128_256, 1, 0.0f};
+    for (int form = exact ? TILED_128_256 : TILED_256; form < TILED_COUNT; form++) {
         static const int tried[] = {1, 2, 3, 4, 6, 8};
         for (int splits : tried) {
             if (splits > 1 && (KB < 2 * splits || (int64_t)cdiv(M, TILED_FORMS[form].rows) * cdiv(N, TILED_FORMS[form].cols) >= 512)) break;
@@ -75,7 +75,7 @@ void launch_block_fp8_reduce(const float *part, const void *bias, void *y, int d
 // p: x (codes), xs, w, ws, bias, y, M, N, K and, for splits, part
 int launch_block_fp8_tiled(TiledArgs p, int dtype, const TiledPlan &plan, hipStream_t st) {
     p.KB = fp8_blocks(p.K);
-    p.ldx = (int64_t)p.KB * FP8_BLOCK;
+    p.ldx = (int64_t)p.KB * FP8_BLOCK * (dtype == DT_F32 ? 2 : 1);
     p.ldxs = p.M;
     p.pitch = (p.N + 3) / 4 * 4;
     p.splits = plan.splits;

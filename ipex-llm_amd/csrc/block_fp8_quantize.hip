@@ -3,11 +3,13 @@
 // Both are bound by memory: an element is read once and its code written once.
 #include "block_fp8.h"
 
+#include <type_traits>
+
 namespace lowbit {
 
 // One block of a row per 8 lanes, 16 values per lane.  Codes go to rows of ldc bytes; past the row's end they are zeros up to whole
-// blocks where ldc has room for them (the products' own rows).  Scale of (row, block): scale[row * row_step + block * block_step].
-template <typename AT>
+// blocks where ldc has room for them (the products' own rows; WIDE: bfloat16 numbers in rows of 2 ldc bytes).  Scale of (row, block): scale[row * row_step + block * block_step].
+template <typename AT, bool WIDE>
 __global__ __launch_bounds__(256) void block_fp8_rows_kernel(const AT *__restrict__ x, uint8_t *__restrict__ codes, float *__restrict__ scale,
                                                              int64_t units, int K, int KB, int ldc, int64_t row_step, int64_t block_step) {
     const int64_t unit = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
@@ -18,23 +20,25 @@ __global__ __launch_bounds__(256) void block_fp8_rows_kernel(const AT *__restric
     if (k < K) load16(x + row * K + k, v);
     float s;
     const u32x4 c = quantize16<AT>(v, s);
-    if (k < ldc) *(u32x4 *)(codes + row * ldc + k) = c;
+    if (k < ldc) store16<WIDE>(codes + row * ldc * (WIDE ? 2 : 1), k, c);
     if ((threadIdx.x & 7) == 0) scale[row * row_step + kb * block_step] = s;
 }
 
-int launch_block_fp8_rows(const void *x, int dtype, int64_t rows, int K, uint8_t *codes, int ldc, float *scale, int64_t row_step,
+int launch_block_fp8_rows(const void *x, int dtype, int64_t rows, int K, uint8_t *codes, int ldc, bool wide, float *scale, int64_t row_step,
                           int64_t block_step, hipStream_t st) {
     const int KB = fp8_blocks(K);
     const int64_t units = rows * KB, groups = (units + 31) / 32;
     if (groups > 0x7fffffff) return -3;
     const dim3 grid((uint32_t)groups), block(256);
-    if (dtype == DT_F16)
-        hipLaunchKernelGGL((block_fp8_rows_kernel<_Float16>), grid, block, 0, st, (const _Float16 *)x, codes, scale, units, K, KB, ldc, row_step, block_step);
-    else if (dtype == DT_BF16)
-        hipLaunchKernelGGL((block_fp8_rows_kernel<__bf16>), grid, block, 0, st, (const __bf16 *)x, codes, scale, units, K, KB, ldc, row_step, block_step);
-    else if (dtype == DT_F32)
-        hipLaunchKernelGGL((block_fp8_rows_kernel<float>), grid, block, 0, st, (const float *)x, codes, scale, units, K, KB, ldc, row_step, block_step);
-    else return -4;
+    auto go = [&](auto *typed, auto w) {
+        using AT = typename std::remove_cv<typename std::remove_pointer<decltype(typed)>::type>::type;
+        hipLaunchKernelGGL((block_fp8_rows_kernel<AT, decltype(w)::value>), grid, block, 0, st, typed, codes, scale, units, K, KB, ldc, row_step, block_step);
+    };
+    if (dtype == DT_F16) go((const _Float16 *)x, std::false_type());
+    else if (dtype == DT_BF16) go((const __bf16 *)x, std::false_type());
+    else if (dtype != DT_F32) return -4;
+    else if (wide) go((const float *)x, std::true_type());
+    else go((const float *)x, std::false_type());
     return 0;
 }
 

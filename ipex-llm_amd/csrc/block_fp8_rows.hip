@@ -7,7 +7,7 @@
 
 namespace lowbit {
 
-int launch_block_fp8_rows(const void *x, int dtype, int64_t rows, int K, uint8_t *codes, int ldc, float *scale, int64_t row_step,
+int launch_block_fp8_rows(const void *x, int dtype, int64_t rows, int K, uint8_t *codes, int ldc, bool wide, float *scale, int64_t row_step,
                           int64_t block_step, hipStream_t st);
 
 struct RowsProduct {
@@ -157,18 +157,18 @@ static bool fuses_rows(int M, int K) {
     return M <= 4 && (size_t)M * (fp8_blocks(K) * FP8_BLOCK + 16) + (size_t)fp8_blocks(K) * 64 <= 65536;
 }
 
-static size_t codes_bytes(int M, int K) { return ((size_t)M * fp8_blocks(K) * FP8_BLOCK + 255) & ~(size_t)255; }
+static size_t codes_bytes(int M, int K, bool wide) { return ((size_t)M * fp8_blocks(K) * FP8_BLOCK * (wide ? 2 : 1) + 255) & ~(size_t)255; }
 
 // Up to here one pass of the weights through registers; beyond, tiles in LDS.
 static bool takes_few_rows(int M) { return M <= 64; }
 
-// codes of x, their scales, a split's sums
+// codes of x (float32 results of tiles: bfloat16 numbers), their scales, a split's sums
 struct LinearSpace {
     size_t xs, part, bytes;
 };
-static LinearSpace linear_space(int M, int N, int K, const TiledPlan &plan) {
+static LinearSpace linear_space(int M, int N, int K, bool wide, const TiledPlan &plan) {
     LinearSpace s;
-    s.xs = codes_bytes(M, K);
+    s.xs = codes_bytes(M, K, wide);
     s.part = s.xs + (((size_t)M * fp8_blocks(K) * sizeof(float) + 255) & ~(size_t)255);
     s.bytes = s.part + block_fp8_tiled_part_bytes(plan, M, N);
     return s;
@@ -177,7 +177,7 @@ static LinearSpace linear_space(int M, int N, int K, const TiledPlan &plan) {
 size_t block_fp8_linear_workspace_bytes(int dtype, int M, int N, int K) {
     if (fuses_rows(M, K)) return 0;
     const TiledPlan plan = takes_few_rows(M) ? TiledPlan{0, 1, 0.0f} : block_fp8_tiled_plan(dtype == DT_F32, M, N, K);
-    return linear_space(M, N, K, plan).bytes;
+    return linear_space(M, N, K, dtype == DT_F32 && !takes_few_rows(M), plan).bytes;
 }
 
 int launch_block_fp8_linear(const void *x, const uint8_t *w, const float *ws, const void *bias, void *y, int dtype, int M, int N, int K,
@@ -187,9 +187,10 @@ int launch_block_fp8_linear(const void *x, const uint8_t *w, const float *ws, co
     RowsProduct p = {x, nullptr, w, ws, bias, y, M, N, K, KB, ldx, M};
     if (!fused) {
         const TiledPlan plan = few ? TiledPlan{0, 1, 0.0f} : block_fp8_tiled_plan(dtype == DT_F32, M, N, K);
-        const LinearSpace at = linear_space(M, N, K, plan);
+        const bool wide = dtype == DT_F32 && !few;
+        const LinearSpace at = linear_space(M, N, K, wide, plan);
         float *const xs = (float *)(space + at.xs);
-        if (int rc = launch_block_fp8_rows(x, dtype, M, K, space, ldx, xs, 1, M, st)) return rc;
+        if (int rc = launch_block_fp8_rows(x, dtype, M, K, space, ldx, wide, xs, 1, M, st)) return rc;
         if (!few) {
             TiledArgs t{};
             t.x = space; t.xs = xs; t.w = w; t.ws = ws; t.bias = bias; t.y = y; t.part = (float *)(space + at.part);

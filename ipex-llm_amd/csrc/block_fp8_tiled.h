@@ -26,12 +26,11 @@ struct TiledPlan {
 // One launch per form; the wave tiles are 64 x 128, 64 x 64, 64 x 64 and 32 x 64.
 template <typename OT, bool EXACT, TiledMode MODE> void launch_tiled_form(const TiledArgs &p, int form, hipStream_t st) {
     if (form == TILED_256) {
-        // (widened operands of a 64 x 128 wave tile do not fit its registers)
-        if constexpr (EXACT) launch_tiled<OT, EXACT, MODE, false, false, 4, 4, 2, 4, 3, 2>(p, st);
-        else launch_tiled<OT, EXACT, MODE, false, false, 4, 8, 4, 2, 2, 2>(p, st);
-    } else if (form == TILED_128_256) launch_tiled<OT, EXACT, MODE, false, false, 4, 4, 2, 4, 3, 2>(p, st);
-    else if (form == TILED_128) launch_tiled<OT, EXACT, MODE, false, false, 4, 4, 2, 2, 2, 2>(p, st);
-    else launch_tiled<OT, EXACT, MODE, false, false, 2, 4, 2, 2, 3, 2>(p, st);
+        // (the operands of a 64 x 128 wave tile in bfloat16 do not fit its registers: no plan asks for it)
+        if constexpr (!EXACT) launch_tiled<OT, EXACT, MODE, false, false, 4, 8, 4, 2, 2, 2>(p, st);
+    } else if (form == TILED_128_256) launch_tiled<OT, EXACT, MODE, false, false, 4, 4, 2, 4, EXACT ? 2 : 3, 2>(p, st);
+    else if (form == TILED_128) launch_tiled<OT, EXACT, MODE, false, false, 4, 4, 2, 2, EXACT ? 3 : 2, EXACT ? 1 : 2>(p, st);
+    else launch_tiled<OT, EXACT, MODE, false, false, 2, 4, 2, 2, EXACT ? 2 : 3, 2>(p, st);
 }
 
 void launch_tiled_f16(const TiledArgs &p, int form, hipStream_t st);
