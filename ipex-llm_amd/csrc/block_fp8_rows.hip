@@ -1,8 +1,11 @@
-// Few rows of activations times a weight with a scale for each block of 128 (block_fp8.h): the weight streams past once.
+// Up to four rows of activations times a weight with a scale for each block of 128 (block_fp8.h): the weight streams past once, in one
+// launch.
 //
-// A workgroup owns 16 * T weight rows and up to 16 * MT rows of x; its waves take the blocks of K in turn and their sums meet in LDS.
-// A wave's loads are 16 rows x 64 contiguous bytes, STEPS blocks ahead of their use.  FUSED: x is quantized by each workgroup, into
-// LDS, while the first weights are on their way, which saves a launch; otherwise codes and scales of x come from memory (L2).
+// A workgroup owns 16 weight rows; its waves take the blocks of K in turn and their sums meet in LDS.  A wave's loads are 16 rows x 64
+// contiguous bytes, STEPS blocks ahead of their use.  x is quantized by each workgroup, into LDS, while the first weights are on their
+// way.  Loads return in order, so x is asked for ahead of them.  Bound by latency at the sizes of one token: of SMALL us at one row of [4096 x
+// 4096] an empty launch is 1.6.  More rows go to the tiles of block_fp8_gemm.h, which hide latency better than registers do: 40 rows on
+// [11008 x 4096] 28 us this way, 10.8 in tiles.
 #include "block_fp8_tiled.h"
 
 namespace lowbit {
@@ -11,200 +14,186 @@ int launch_block_fp8_rows(const void *x, int dtype, int64_t rows, int K, uint8_t
                           int64_t block_step, hipStream_t st);
 
 struct RowsProduct {
-    const void *x;                                           // FUSED: activations [M, K]; else codes, rows of ldx bytes
-    const float *xs;                                         // scales of the codes: [KB][ldm]
+    const void *x;                                           // [M, K]
     const uint8_t *w;
     const float *ws;
     const void *bias;
     void *y;
-    int M, N, K, KB, ldx, ldm;
+    int M, N, K, KB;
 };
 
-template <typename AT> __device__ inline AT narrow(float v) { return to_at<AT>(v); }
-template <> __device__ inline float narrow<float>(float v) { return v; }
+// 8 values of AT from memory (16-byte aligned)
+template <typename AT> struct Eight {
+    typedef AT type __attribute__((ext_vector_type(8)));
+};
 
-template <typename AT, int T, int MT, bool FUSED, int WAVES>
+template <typename AT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void block_fp8_few_rows_kernel(const RowsProduct p) {
     constexpr bool EXACT = sizeof(AT) == 4;
-    constexpr int STEPS = T * MT > 4 ? 2 : 4;                // blocks in flight per wave
+    constexpr int STEPS = 4;                                 // blocks in flight per wave
+    constexpr int HELD = EXACT ? 2 : 4;                      // pieces of x per thread that are asked for ahead of the weights
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
-    const int n0 = blockIdx.x * 16 * T, m0 = blockIdx.y * 16 * MT, KB = p.KB;
+    const int n0 = blockIdx.x * 16, KB = p.KB, M = p.M, N = p.N, K = p.K;
+    // (one wait for all arguments: left alone the compiler loads each where it is first used)
+    asm volatile("" :: "s"(p.x), "s"(p.w), "s"(p.ws), "s"(p.bias), "s"(p.y), "s"(M), "s"(N), "s"(K), "s"(KB));
 
-    const uint8_t *wrow[T];
-#pragma unroll
-    for (int t = 0; t < T; t++) {
-        const int n = n0 + t * 16 + r;
-        wrow[t] = p.w + (int64_t)(n < p.N ? n : p.N - 1) * p.K + g * 16;
-    }
-    const float *const ws = p.ws + (int64_t)(n0 / FP8_BLOCK) * KB;
-    auto load_w = [&](int kb, Codes (&c)[T]) {
-        const int left = p.K - kb * FP8_BLOCK - g * 16;      // bytes of the row from the lane's first chunk on
-#pragma unroll
-        for (int t = 0; t < T; t++) {
-            c[t] = Codes{};
-            if (left > 0) c[t].lo = ld<u32x4, true>(wrow[t] + kb * FP8_BLOCK);
-            if (left > 64) c[t].hi = ld<u32x4, true>(wrow[t] + kb * FP8_BLOCK + 64);
-        }
+    // pieces of 8 values of x, 16 to a block: thread, thread + 64 * WAVES, ...
+    using V8 = typename Eight<AT>::type;
+    const int pieces = M * KB * 16;
+    auto load_x = [&](int piece) __attribute__((always_inline)) {
+        const int row = piece / (KB * 16), k = (piece - row * KB * 16) * 8;
+        return k < K ? *(const V8 *)((const AT *)p.x + (int64_t)row * K + k) : V8{};
     };
-    Codes wc[STEPS][T];
-    float wsc[STEPS];
+    V8 held[HELD];
 #pragma unroll
-    for (int s = 0; s < STEPS; s++) {
-        const int kb = wave + s * WAVES;
-        if (kb < KB) {
-            load_w(kb, wc[s]);
-            wsc[s] = ws[kb];
-        }
+    for (int i = 0; i < HELD; i++) {
+        const int piece = threadIdx.x + i * 64 * WAVES;
+        held[i] = V8{};
+        if (piece < pieces) held[i] = load_x(piece);
     }
+    __builtin_amdgcn_sched_barrier(0);
 
-    // FUSED: codes of up to 16 rows in LDS, rows of KB * 128 + 16 bytes (16: rows start in other banks), then their scales [KB][16]
-    const int pitch = KB * FP8_BLOCK + 16, rows = p.M - m0 < 16 * MT ? p.M - m0 : 16 * MT;
-    float *const xs_lds = (float *)(lds + (size_t)rows * pitch);
-    if constexpr (FUSED) {
-        const int units = rows * KB;
-        for (int u = threadIdx.x >> 3; u < units; u += 8 * WAVES) {
-            const int row = u / KB, kb = u - row * KB, k = kb * FP8_BLOCK + (threadIdx.x & 7) * 16;
-            float v[16] = {}, s;
-            if (k < p.K) load16((const AT *)p.x + (int64_t)(m0 + row) * p.K + k, v);
-            *(u32x4 *)(lds + row * pitch + k) = quantize16<AT>(v, s);
-            if ((threadIdx.x & 7) == 0) xs_lds[kb * 16 + row] = s;
-        }
-        __syncthreads();
-    }
-    // rows past M repeat the last one; their results are not stored
-    const uint8_t *xrow[MT];
-    int xrow_at[MT];
+    const int n = n0 + r;
+    const uint8_t *const wrow = p.w + (int64_t)(n < N ? n : N - 1) * K;
+    // the scales of this wave's blocks in the lanes of a register (64 blocks per wave at most: see takes_few_rows); a scalar load per block
+    // would be waited for one after the other
+    const float wheld = p.ws[(int64_t)(n0 / FP8_BLOCK) * KB + (wave + lane * WAVES < KB ? wave + lane * WAVES : KB - 1)];
+    auto load_w = [&](int kb, Codes &c) __attribute__((always_inline)) {
+        // (chunks past the row's end: the block's first one, which meets zeros of x)
+        const int left = K - kb * FP8_BLOCK;
+        const uint8_t *const at = wrow + kb * FP8_BLOCK;
+        c.lo = ld<u32x4, true>(at + (g * 16 < left ? g * 16 : 0));
+        c.hi = ld<u32x4, true>(at + (64 + g * 16 < left ? 64 + g * 16 : 0));
+    };
+    Codes wc[STEPS];
 #pragma unroll
-    for (int i = 0; i < MT; i++) {
-        const int m = i * 16 + r, mm = m < rows ? m : rows - 1;
-        xrow_at[i] = FUSED ? mm : m0 + mm;
-        xrow[i] = FUSED ? lds + mm * pitch + g * 16 : (const uint8_t *)p.x + (int64_t)(m0 + mm) * p.ldx + g * 16;
-    }
+    for (int s = 0; s < STEPS; s++)
+        load_w(wave + s * WAVES < KB ? wave + s * WAVES : KB - 1, wc[s]);      // (past the last block: it again, not added)
+    __builtin_amdgcn_sched_barrier(0);
 
-    f32x4 acc[T][MT] = {};
-    for (int kb0 = wave; kb0 < KB; kb0 += WAVES * STEPS) {
+    // codes of x in LDS, rows of KB * 128 + 16 bytes (16: rows start in other banks), then the scales [KB][4]
+    const int pitch = KB * FP8_BLOCK + 16;
+    float *const xs = (float *)(lds + (size_t)M * pitch);
+    auto put_x = [&](int piece, const V8 &v) __attribute__((always_inline)) {
+        const int row = piece / (KB * 16), at = piece - row * KB * 16;
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) m = max_u32(m, magnitude((float)v[i]));
+        m = max_of_16(m);
+        const float scale = block_scale(m);
+        const Quotient<AT> q(scale, m);
+        *(u32x2 *)(lds + row * pitch + at * 8) = u32x2{encode4(q((float)v[0]), q((float)v[1]), q((float)v[2]), q((float)v[3])),
+                                                       encode4(q((float)v[4]), q((float)v[5]), q((float)v[6]), q((float)v[7]))};
+        if ((at & 15) == 0) xs[(at >> 4) * 4 + row] = scale;
+    };
+#pragma unroll
+    for (int i = 0; i < HELD; i++) {
+        const int piece = threadIdx.x + i * 64 * WAVES;
+        if (piece < pieces) put_x(piece, held[i]);           // (the 16 lanes of a block are in or out together)
+    }
+    for (int piece = threadIdx.x + HELD * 64 * WAVES; piece < pieces; piece += 64 * WAVES) put_x(piece, load_x(piece));
+    __syncthreads();
+
+    // (operand rows past M repeat the last one; their results are not stored)
+    const int row = r < M ? r : M - 1;
+    const uint8_t *const xrow = lds + row * pitch + g * 16;
+    f32x4 acc = {};
+    for (int i0 = 0; wave + i0 * WAVES < KB; i0 += STEPS) {
+        Codes xc[STEPS];
+        float sc[STEPS];
 #pragma unroll
         for (int s = 0; s < STEPS; s++) {
-            const int kb = kb0 + s * WAVES;
-            if (kb >= KB) break;
-            Codes xc[MT];
-            float scale[MT];
+            const int kb = wave + (i0 + s) * WAVES, in = kb < KB ? kb : KB - 1;
+            xc[s] = Codes{*(const u32x4 *)(xrow + in * FP8_BLOCK), *(const u32x4 *)(xrow + in * FP8_BLOCK + 64)};
+            sc[s] = xs[in * 4 + row] * __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wheld), i0 + s));
+        }
+        f32x4 d[STEPS];
 #pragma unroll
-            for (int i = 0; i < MT; i++) {
-                xc[i].lo = *(const u32x4 *)(xrow[i] + kb * FP8_BLOCK);
-                xc[i].hi = *(const u32x4 *)(xrow[i] + kb * FP8_BLOCK + 64);
-                scale[i] = FUSED ? xs_lds[kb * 16 + xrow_at[i]] : p.xs[(int64_t)kb * p.ldm + xrow_at[i]];
-            }
+        for (int s = 0; s < STEPS; s++) {
+            d[s] = block_dot<EXACT>(wc[s], xc[s]);
+            const int next = wave + (i0 + s + STEPS) * WAVES;
+            if (next < KB) load_w(next, wc[s]);
+        }
 #pragma unroll
-            for (int i = 0; i < MT; i++) {
-                const float sc = scale[i] * wsc[s];
+        for (int s = 0; s < STEPS; s++) {
+            const bool in = wave + (i0 + s) * WAVES < KB;
 #pragma unroll
-                for (int t = 0; t < T; t++) {
-                    const f32x4 d = block_dot<EXACT>(wc[s][t], xc[i]);
-#pragma unroll
-                    for (int j = 0; j < 4; j++) acc[t][i][j] = fmaf(sc, d[j], acc[t][i][j]);
-                }
-            }
-            const int next = kb + WAVES * STEPS;
-            if (next < KB) {
-                load_w(next, wc[s]);
-                wsc[s] = ws[next];
-            }
+            for (int j = 0; j < 4; j++) acc[j] = in ? fmaf(sc[s], d[s][j], acc[j]) : acc[j];
         }
     }
 
-    // the waves' sums, [wave][t * MT + i][lane]
-    if constexpr (FUSED) __syncthreads();                    // (they lie where the codes were)
-    f32x4 *const sums = (f32x4 *)lds;
-#pragma unroll
-    for (int t = 0; t < T; t++)
-#pragma unroll
-        for (int i = 0; i < MT; i++) sums[(wave * T * MT + t * MT + i) * 64 + lane] = acc[t][i];
+    // the waves' sums, [wave][row][16 columns]
+    __syncthreads();                                         // (they lie where the codes were)
+    float *const sums = (float *)lds;
+    if (r < M)
+        *(f32x4 *)(sums + (wave * 4 + r) * 16 + g * 4) = acc;
     __syncthreads();
-    for (int o = threadIdx.x; o < T * MT * 64; o += 64 * WAVES) {
-        f32x4 v = sums[o];
+    if ((int)threadIdx.x >= M * 16) return;
+    const int m = threadIdx.x >> 4, c = threadIdx.x & 15;
+    if (n0 + c >= N) return;
+    float v = 0.0f;
 #pragma unroll
-        for (int w = 1; w < WAVES; w++) v += sums[w * T * MT * 64 + o];
-        const int l = o & 63, i = (o >> 6) % MT, t = (o >> 6) / MT;
-        const int m = m0 + i * 16 + (l & 15), n = n0 + t * 16 + (l >> 4) * 4;
-        if (m >= p.M) continue;
-        AT *const out = (AT *)p.y + (int64_t)m * p.N + n;
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (n + j < p.N) out[j] = narrow<AT>(v[j] + (p.bias ? (float)((const AT *)p.bias)[n + j] : 0.0f));
-    }
+    for (int w = 0; w < WAVES; w++) v += sums[(w * 4 + m) * 16 + c];
+    if (p.bias) v += (float)((const AT *)p.bias)[n0 + c];
+    ((AT *)p.y)[(int64_t)m * N + n0 + c] = Stored<AT>::of(v);
 }
 
-template <typename AT, int T, int MT, bool FUSED, int WAVES> static void launch_few(const RowsProduct &p, hipStream_t st) {
-    size_t lds = (size_t)WAVES * T * MT * 64 * sizeof(f32x4);
-    const int rows = p.M < 16 * MT ? p.M : 16 * MT;
-    const size_t codes = (size_t)rows * (p.KB * FP8_BLOCK + 16) + (size_t)p.KB * 16 * sizeof(float);
-    if (FUSED && codes > lds) lds = codes;
-    const dim3 grid((p.N + 16 * T - 1) / (16 * T), (p.M + 16 * MT - 1) / (16 * MT));
-    hipLaunchKernelGGL((block_fp8_few_rows_kernel<AT, T, MT, FUSED, WAVES>), grid, dim3(64 * WAVES), lds, st, p);
+static size_t few_rows_lds(int M, int KB) {
+    const size_t codes = (size_t)M * (KB * FP8_BLOCK + 16) + (size_t)KB * 4 * sizeof(float);
+    return codes > 4096 ? codes : 4096;                      // (the sums of 16 waves)
 }
 
-template <typename AT> static void launch_few_rows_t(const RowsProduct &p, bool fused, hipStream_t st) {
-    if (fused) launch_few<AT, 1, 1, true, 8>(p, st);
-    else if (p.M <= 16) launch_few<AT, 1, 1, false, 8>(p, st);
-    else if (p.M <= 32) launch_few<AT, 1, 2, false, 8>(p, st);
-    else launch_few<AT, 2, 4, false, 8>(p, st);
+template <typename AT> static void launch_few_rows(const RowsProduct &p, hipStream_t st) {
+    const dim3 grid((p.N + 15) / 16);
+    const size_t lds = few_rows_lds(p.M, p.KB);
+    // Long walks of few workgroups: 16 waves each.  One row on [4096 x 11008] 13.3 us against 13.9, two on [4096 x 14336] 16.3 / 17.2; but
+    // one on [28672 x 8192] 53.3 / 49.9, on [4096 x 4096], where half of their loads would be of no block, 7.9 / 5.6.
+    if (p.KB > 64 && p.N <= 8192) hipLaunchKernelGGL((block_fp8_few_rows_kernel<AT, 16>), grid, dim3(1024), lds, st, p);
+    else hipLaunchKernelGGL((block_fp8_few_rows_kernel<AT, 8>), grid, dim3(512), lds, st, p);
 }
 
-// Rows that each workgroup quantizes by itself: their codes fit 64 KiB of LDS.
-static bool fuses_rows(int M, int K) {
-    return M <= 4 && (size_t)M * (fp8_blocks(K) * FP8_BLOCK + 16) + (size_t)fp8_blocks(K) * 64 <= 65536;
-}
+// Up to four rows whose codes fit 64 KiB of LDS; beyond, tiles.
+static bool takes_few_rows(int M, int K) { return M <= 4 && few_rows_lds(M, fp8_blocks(K)) <= 65536 && fp8_blocks(K) <= 512; }
 
-static size_t codes_bytes(int M, int K, bool wide) { return ((size_t)M * fp8_blocks(K) * FP8_BLOCK * (wide ? 2 : 1) + 255) & ~(size_t)255; }
-
-// Up to here one pass of the weights through registers; beyond, tiles in LDS.
-static bool takes_few_rows(int M) { return M <= 64; }
-
-// codes of x (float32 results of tiles: bfloat16 numbers), their scales, a split's sums
+// codes of x (float32 results: bfloat16 numbers), their scales, a split's sums
 struct LinearSpace {
     size_t xs, part, bytes;
 };
-static LinearSpace linear_space(int M, int N, int K, bool wide, const TiledPlan &plan) {
+static LinearSpace linear_space(bool wide, int M, int N, int K, const TiledPlan &plan) {
+    auto whole = [](size_t bytes) { return (bytes + 255) & ~(size_t)255; };
     LinearSpace s;
-    s.xs = codes_bytes(M, K, wide);
-    s.part = s.xs + (((size_t)M * fp8_blocks(K) * sizeof(float) + 255) & ~(size_t)255);
+    s.xs = whole((size_t)M * fp8_blocks(K) * FP8_BLOCK * (wide ? 2 : 1));
+    s.part = s.xs + whole((size_t)M * fp8_blocks(K) * sizeof(float));
     s.bytes = s.part + block_fp8_tiled_part_bytes(plan, M, N);
     return s;
 }
 
 size_t block_fp8_linear_workspace_bytes(int dtype, int M, int N, int K) {
-    if (fuses_rows(M, K)) return 0;
-    const TiledPlan plan = takes_few_rows(M) ? TiledPlan{0, 1, 0.0f} : block_fp8_tiled_plan(dtype == DT_F32, M, N, K);
-    return linear_space(M, N, K, dtype == DT_F32 && !takes_few_rows(M), plan).bytes;
+    if (takes_few_rows(M, K)) return 0;
+    const bool wide = dtype == DT_F32;
+    return linear_space(wide, M, N, K, block_fp8_tiled_plan(wide, M, N, K)).bytes;
 }
 
 int launch_block_fp8_linear(const void *x, const uint8_t *w, const float *ws, const void *bias, void *y, int dtype, int M, int N, int K,
                             uint8_t *space, hipStream_t st) {
-    const bool fused = fuses_rows(M, K), few = takes_few_rows(M);
-    const int KB = fp8_blocks(K), ldx = KB * FP8_BLOCK;
-    RowsProduct p = {x, nullptr, w, ws, bias, y, M, N, K, KB, ldx, M};
-    if (!fused) {
-        const TiledPlan plan = few ? TiledPlan{0, 1, 0.0f} : block_fp8_tiled_plan(dtype == DT_F32, M, N, K);
-        const bool wide = dtype == DT_F32 && !few;
-        const LinearSpace at = linear_space(M, N, K, wide, plan);
-        float *const xs = (float *)(space + at.xs);
-        if (int rc = launch_block_fp8_rows(x, dtype, M, K, space, ldx, wide, xs, 1, M, st)) return rc;
-        if (!few) {
-            TiledArgs t{};
-            t.x = space; t.xs = xs; t.w = w; t.ws = ws; t.bias = bias; t.y = y; t.part = (float *)(space + at.part);
-            t.M = M; t.N = N; t.K = K;
-            return launch_block_fp8_tiled(t, dtype, plan, st);
-        }
-        p.x = space;
-        p.xs = xs;
+    if (takes_few_rows(M, K)) {
+        const RowsProduct p = {x, w, ws, bias, y, M, N, K, fp8_blocks(K)};
+        if (dtype == DT_F16) launch_few_rows<_Float16>(p, st);
+        else if (dtype == DT_BF16) launch_few_rows<__bf16>(p, st);
+        else if (dtype == DT_F32) launch_few_rows<float>(p, st);
+        else return -4;
+        return 0;
     }
-    if (dtype == DT_F16) launch_few_rows_t<_Float16>(p, fused, st);
-    else if (dtype == DT_BF16) launch_few_rows_t<__bf16>(p, fused, st);
-    else if (dtype == DT_F32) launch_few_rows_t<float>(p, fused, st);
-    else return -4;
-    return 0;
+    const bool wide = dtype == DT_F32;
+    const TiledPlan plan = block_fp8_tiled_plan(wide, M, N, K);
+    const LinearSpace at = linear_space(wide, M, N, K, plan);
+    float *const xs = (float *)(space + at.xs);
+    if (int rc = launch_block_fp8_rows(x, dtype, M, K, space, fp8_blocks(K) * FP8_BLOCK, wide, xs, 1, M, st)) return rc;
+    TiledArgs t{};
+    t.x = space; t.xs = xs; t.w = w; t.ws = ws; t.bias = bias; t.y = y; t.part = (float *)(space + at.part);
+    t.M = M; t.N = N; t.K = K;
+    return launch_block_fp8_tiled(t, dtype, plan, st);
 }
 
 }  // namespace lowbit

@@ -10,12 +10,13 @@ struct TiledForm {
     int rows, cols, per_cu;
     float step_us, alone_us, exact_us, exact_alone_us;
 };
-enum { TILED_256, TILED_128_256, TILED_128, TILED_64, TILED_COUNT };
+enum { TILED_256, TILED_128_256, TILED_128, TILED_64, TILED_32, TILED_COUNT };
 static const TiledForm TILED_FORMS[TILED_COUNT] = {
-    {256, 256, 1, 1.75f, 1.70f, 4.4f, 4.2f},
-    {128, 256, 1, 1.00f, 0.92f, 2.2f, 2.1f},
-    {128, 128, 2, 1.05f, 0.62f, 2.2f, 1.2f},
-    {64, 128, 2, 0.68f, 0.40f, 1.2f, 0.7f},
+    {256, 256, 1, 1.81f, 1.69f, 0.0f, 0.0f},
+    {128, 256, 1, 1.30f, 0.97f, 2.07f, 1.59f},
+    {128, 128, 2, 1.01f, 0.66f, 2.77f, 1.21f},
+    {64, 128, 2, 0.82f, 0.41f, 1.07f, 0.77f},
+    {32, 128, 2, 0.66f, 0.32f, 0.73f, 0.53f},
 };
 
 struct TiledPlan {
@@ -23,14 +24,15 @@ struct TiledPlan {
     float us;
 };
 
-// One launch per form; the wave tiles are 64 x 128, 64 x 64, 64 x 64 and 32 x 64.
+// One launch per form; the wave tiles are 64 x 128, 64 x 64, 64 x 64, 32 x 64 and 32 x 32.
 template <typename OT, bool EXACT, TiledMode MODE> void launch_tiled_form(const TiledArgs &p, int form, hipStream_t st) {
     if (form == TILED_256) {
         // (the operands of a 64 x 128 wave tile in bfloat16 do not fit its registers: no plan asks for it)
         if constexpr (!EXACT) launch_tiled<OT, EXACT, MODE, false, false, 4, 8, 4, 2, 2, 2>(p, st);
     } else if (form == TILED_128_256) launch_tiled<OT, EXACT, MODE, false, false, 4, 4, 2, 4, EXACT ? 2 : 3, 2>(p, st);
     else if (form == TILED_128) launch_tiled<OT, EXACT, MODE, false, false, 4, 4, 2, 2, EXACT ? 3 : 2, EXACT ? 1 : 2>(p, st);
-    else launch_tiled<OT, EXACT, MODE, false, false, 2, 4, 2, 2, EXACT ? 2 : 3, 2>(p, st);
+    else if (form == TILED_64) launch_tiled<OT, EXACT, MODE, false, false, 2, 4, 2, 2, EXACT ? 2 : 3, 2>(p, st);
+    else launch_tiled<OT, EXACT, MODE, false, false, 2, 2, 1, 4, 3, 2>(p, st);
 }
 
 void launch_tiled_f16(const TiledArgs &p, int form, hipStream_t st);
