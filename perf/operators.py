@@ -219,15 +219,16 @@ def run(s):
 
 
 def _run_own(s):
-    if os.path.abspath("ipex-llm_amd") not in sys.path:
-        sys.path.insert(0, os.path.abspath("ipex-llm_amd"))    # the package lives beside this folder, in the working directory
-    from ipex_llm.transformers.block_fp8 import (block_fp8_experts, block_fp8_linear, block_fp8_quantize,
-                                                 block_fp8_quantize_weight)
+    calls = getattr(_run_own, "calls", None)
+    if calls is None:                                      # a user's program imports the package once
+        sys.path.insert(0, os.path.abspath("ipex-llm_amd"))    # it lives beside this folder, in the working directory
+        import ipex_llm.transformers.block_fp8 as calls
+        _run_own.calls = calls
     if s["kind"] == "quantize":
-        return block_fp8_quantize(s["x"]) if s["rows"] else block_fp8_quantize_weight(s["x"])
+        return calls.block_fp8_quantize(s["x"]) if s["rows"] else calls.block_fp8_quantize_weight(s["x"])
     if s["kind"] == "experts":
-        return block_fp8_experts(s["x"], s["ids"], s["p"], s["gate_up"], s["gate_up_scale"], s["down"], s["down_scale"])
-    y = block_fp8_linear(s["x"], s["w"], s["scale"], s["bias"])
+        return calls.block_fp8_experts(s["x"], s["ids"], s["p"], s["gate_up"], s["gate_up_scale"], s["down"], s["down_scale"])
+    y = calls.block_fp8_linear(s["x"], s["w"], s["scale"], s["bias"])
     if s["kind"] == "linear":
         return y
     return y.detach(), torch.autograd.grad(y, s["x"], s["grad"])[0]
