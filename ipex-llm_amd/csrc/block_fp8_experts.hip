@@ -28,67 +28,91 @@ struct ExpertsArgs {
     int n_exp, top_k, H, I, act;
 };
 
-__device__ inline void load_chunks(const uint8_t *row, int kb, int left, Codes &c) {
-    c = Codes{};
-    if (left > 0) c.lo = ld<u32x4, true>(row + kb * FP8_BLOCK);
-    if (left > 64) c.hi = ld<u32x4, true>(row + kb * FP8_BLOCK + 64);
+// Both chunks of a lane (block_fp8.h) of one block of a row; past the row's end the block's first chunk, which meets zeros of x
+__device__ inline Codes load_chunks(const uint8_t *row, int kb, int g, int K) {
+    const int left = K - kb * FP8_BLOCK;
+    const uint8_t *const at = row + kb * FP8_BLOCK;
+    return Codes{ld<u32x4, true>(at + (g * 16 < left ? g * 16 : 0)), ld<u32x4, true>(at + (64 + g * 16 < left ? 64 + g * 16 : 0))};
 }
 
-// Wave w: 16 columns of g and the same of u, all of K.
+__device__ inline float lane_value(float held, int l) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, held), l));
+}
+
+// One pair: a workgroup's wave w has 16 columns of g and the same of u, all of K, STEPS blocks in flight.  x is quantized by each workgroup.
+// Bound by memory: two experts of [14336 x 4096], 235 MB, in UPTIME us.
 template <typename AT>
 __global__ __launch_bounds__(512) void block_fp8_expert_token_up_kernel(const ExpertsArgs p) {
     constexpr int STEPS = 4;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     __shared__ uint32_t part[8];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
-    const int cb = blockIdx.x, KB = fp8_blocks(p.H);
-    const int pair = blockIdx.y;
+    const int cb = blockIdx.x, pair = blockIdx.y, H = p.H, KB = fp8_blocks(H);
     const int64_t e = p.ids[pair];
     if (e < 0 || e >= p.n_exp) return;                       // (the second product skips the pair)
-    const int expert = (int)e;
-    const uint8_t *const w = p.gate_up + (int64_t)expert * 2 * p.I * p.H;
+
+    // the row's first 8192 values are asked for ahead of the weights: loads return in order
+    const AT *const x = (const AT *)p.x + (int64_t)(pair / p.top_k) * H;
+    float v[16] = {};
+    const int own = (int)threadIdx.x * 16;
+    if (own < H) load16(x + own, v);
+    __builtin_amdgcn_sched_barrier(0);
+
+    const uint8_t *const w = p.gate_up + e * 2 * p.I * H;
     const uint8_t *row[2];
     const float *ws[2];
+    float held[2];
 #pragma unroll
     for (int t = 0; t < 2; t++) {
-        row[t] = w + (int64_t)(t * p.I + cb * FP8_BLOCK + wave * 16 + r) * p.H + g * 16;
-        ws[t] = p.gate_up_scale + ((int64_t)expert * 2 * (p.I / FP8_BLOCK) + t * (p.I / FP8_BLOCK) + cb) * KB;
+        row[t] = w + (int64_t)(t * p.I + cb * FP8_BLOCK + wave * 16 + r) * H;
+        ws[t] = p.gate_up_scale + ((e * 2 + t) * (p.I / FP8_BLOCK) + cb) * KB;
+        held[t] = ws[t][lane < KB ? lane : KB - 1];          // scales of 64 blocks in the lanes of a register
     }
     Codes wc[STEPS][2];
 #pragma unroll
     for (int s = 0; s < STEPS; s++)
-        if (s < KB)
 #pragma unroll
-            for (int t = 0; t < 2; t++) load_chunks(row[t], s, p.H - s * FP8_BLOCK - g * 16, wc[s][t]);
+        for (int t = 0; t < 2; t++) wc[s][t] = load_chunks(row[t], s < KB ? s : KB - 1, g, H);
+    __builtin_amdgcn_sched_barrier(0);
 
     float *const xs = (float *)(lds + KB * FP8_BLOCK);
-    for (int kb = threadIdx.x >> 3; kb < KB; kb += 64) {
-        const int k = kb * FP8_BLOCK + (threadIdx.x & 7) * 16;
-        float v[16] = {}, s;
-        if (k < p.H) load16((const AT *)p.x + (int64_t)(pair / p.top_k) * p.H + k, v);
+    for (int k = own; k < KB * FP8_BLOCK; k += 512 * 16) {
+        if (k != own) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) v[i] = 0.0f;
+            if (k < H) load16(x + k, v);
+        }
+        float s;
         *(u32x4 *)(lds + k) = quantize16<AT>(v, s);
-        if ((threadIdx.x & 7) == 0) xs[kb] = s;
+        if ((threadIdx.x & 7) == 0) xs[k / FP8_BLOCK] = s;
     }
     __syncthreads();
 
     f32x4 acc[2] = {};
     for (int kb0 = 0; kb0 < KB; kb0 += STEPS) {
+        if ((kb0 & 63) == 0 && kb0 != 0)
+#pragma unroll
+            for (int t = 0; t < 2; t++) held[t] = ws[t][kb0 + lane < KB ? kb0 + lane : KB - 1];
+        Codes xc[STEPS];
+        float sx[STEPS];
 #pragma unroll
         for (int s = 0; s < STEPS; s++) {
-            const int kb = kb0 + s;
-            if (kb >= KB) break;
-            const uint8_t *const xr = lds + kb * FP8_BLOCK + g * 16;     // (all 16 rows of the operand are the one)
-            const Codes xc = {*(const u32x4 *)xr, *(const u32x4 *)(xr + 64)};
+            const int in = kb0 + s < KB ? kb0 + s : KB - 1;
+            const uint8_t *const xr = lds + in * FP8_BLOCK + g * 16;     // (all 16 rows of the operand are the one)
+            xc[s] = Codes{*(const u32x4 *)xr, *(const u32x4 *)(xr + 64)};
+            sx[s] = xs[in];
+        }
+#pragma unroll
+        for (int s = 0; s < STEPS; s++) {
+            const bool in = kb0 + s < KB;                    // (past the last block: it again, not added)
 #pragma unroll
             for (int t = 0; t < 2; t++) {
-                const float sc = xs[kb] * ws[t][kb];
-                const f32x4 d = block_dot<true>(wc[s][t], xc);
+                const f32x4 d = block_dot<true>(wc[s][t], xc[s]);
+                const float sc = sx[s] * lane_value(held[t], (kb0 + s) & 63);
 #pragma unroll
-                for (int j = 0; j < 4; j++) acc[t][j] = fmaf(sc, d[j], acc[t][j]);
+                for (int j = 0; j < 4; j++) acc[t][j] = in ? fmaf(sc, d[j], acc[t][j]) : acc[t][j];
+                if (kb0 + s + STEPS < KB) wc[s][t] = load_chunks(row[t], kb0 + s + STEPS, g, H);
             }
-            if (kb + STEPS < KB)
-#pragma unroll
-                for (int t = 0; t < 2; t++) load_chunks(row[t], kb + STEPS, p.H - (kb + STEPS) * FP8_BLOCK - g * 16, wc[s][t]);
         }
     }
 
@@ -111,47 +135,63 @@ __global__ __launch_bounds__(512) void block_fp8_expert_token_up_kernel(const Ex
     if (wave == 0 && g == 0) p.hs[(int64_t)cb * p.ldh + pair] = s;
 }
 
-// One token's 16 columns per workgroup: the blocks of all its pairs are dealt to the waves.
+// One token's 16 columns per workgroup: the blocks of all its pairs are dealt to the waves, STEPS of them in flight per wave.  Bound by
+// memory: two experts of [4096 x 14336], 117 MB, in DOWNTIME us.
 template <typename AT, typename PT>
 __global__ __launch_bounds__(512) void block_fp8_expert_down_token_kernel(const ExpertsArgs p, const PT *__restrict__ weight, AT *__restrict__ out) {
     constexpr int STEPS = 4;
-    __shared__ f32x4 sums[8][4];
+    __shared__ float sums[8][16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
-    const int n0 = blockIdx.x * 16, token = blockIdx.y, IB = p.I / FP8_BLOCK, HB = fp8_blocks(p.H), units = p.top_k * IB;
+    const int n0 = blockIdx.x * 16, token = blockIdx.y, I = p.I, IB = I / FP8_BLOCK, HB = fp8_blocks(p.H), top_k = p.top_k;
+    // the pairs' experts (-1: none) and weights in the lanes of registers: top_k is 64 at most
+    const int pair0 = token * top_k;
+    int expert = -1;
+    float route = 0.0f;
+    if (lane < top_k) {
+        const int64_t e = p.ids[pair0 + lane];
+        expert = e >= 0 && e < p.n_exp ? (int)e : -1;
+        route = (float)weight[pair0 + lane];
+    }
+    const uint64_t valid = __ballot(expert >= 0);
+    const int units = top_k * IB;
+    struct Unit {
+        Codes w, x;
+        float scale;
+    };
+    // unit u: block u % IB of pair u / IB; one of no expert, or past the last, counts nothing
+    auto load = [&](int u, Unit &t) __attribute__((always_inline)) {
+        const int j = u / IB, kb = u - j * IB;
+        t.scale = 0.0f;
+        t.w = Codes{};
+        t.x = Codes{};
+        if (u < units && (valid >> j & 1)) {                 // (the same for the whole wave)
+            const int64_t e = __builtin_amdgcn_readlane(expert, j);
+            t.w = load_chunks(p.down + (e * p.H + n0 + r) * I, kb, g, I);
+            const uint8_t *const xr = p.h + (int64_t)(pair0 + j) * I + kb * FP8_BLOCK + g * 16;
+            t.x = Codes{*(const u32x4 *)xr, *(const u32x4 *)(xr + 64)};
+            t.scale = p.hs[(int64_t)kb * p.ldh + pair0 + j] * p.down_scale[(e * HB + n0 / FP8_BLOCK) * IB + kb] * lane_value(route, j);
+        }
+    };
+    Unit unit[STEPS];
+#pragma unroll
+    for (int s = 0; s < STEPS; s++) load(wave + s * 8, unit[s]);
     f32x4 acc = {};
-    const int n = n0 + r;
     for (int u0 = wave; u0 < units; u0 += 8 * STEPS) {
-        Codes wc[STEPS], xc[STEPS];
-        float sc[STEPS];
 #pragma unroll
         for (int s = 0; s < STEPS; s++) {
-            const int u = u0 + s * 8, j = u / IB, kb = u - j * IB, pair = token * p.top_k + j;
-            const int64_t e = u < units ? p.ids[pair] : -1;
-            wc[s] = Codes{};
-            xc[s] = Codes{};
-            sc[s] = 0.0f;
-            if (e < 0 || e >= p.n_exp) continue;
-            load_chunks(p.down + ((int64_t)e * p.H + n) * p.I + g * 16, kb, FP8_BLOCK, wc[s]);
-            const uint8_t *const xr = p.h + (int64_t)pair * p.I + kb * FP8_BLOCK + g * 16;
-            xc[s].lo = *(const u32x4 *)xr;
-            xc[s].hi = *(const u32x4 *)(xr + 64);
-            sc[s] = p.hs[(int64_t)kb * p.ldh + pair] * p.down_scale[((int64_t)e * HB + n0 / FP8_BLOCK) * IB + kb] * (float)weight[pair];
-        }
+            const f32x4 d = block_dot<false>(unit[s].w, unit[s].x);
 #pragma unroll
-        for (int s = 0; s < STEPS; s++) {
-            const f32x4 d = block_dot<false>(wc[s], xc[s]);
-#pragma unroll
-            for (int j = 0; j < 4; j++) acc[j] = fmaf(sc[s], d[j], acc[j]);
+            for (int j = 0; j < 4; j++) acc[j] = fmaf(unit[s].scale, d[j], acc[j]);
+            load(u0 + (s + STEPS) * 8, unit[s]);
         }
     }
-    if (r == 0) sums[wave][g] = acc;
+    if (r == 0) *(f32x4 *)&sums[wave][g * 4] = acc;
     __syncthreads();
-    if (threadIdx.x < 16) {
-        float v = 0.0f;
+    if (threadIdx.x >= 16) return;
+    float v = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 8; w++) v += sums[w][threadIdx.x >> 2][threadIdx.x & 3];
-        out[(int64_t)token * p.H + n0 + threadIdx.x] = to_at<AT>(v);
-    }
+    for (int w = 0; w < 8; w++) v += sums[w][threadIdx.x];
+    out[(int64_t)token * p.H + n0 + threadIdx.x] = to_at<AT>(v);
 }
 
 // The rows of x in codes (as bfloat16 numbers, see EXACT) and scales, and the pairs sorted by expert, in one launch: the first workgroups quantize (32 blocks each), the rest place
@@ -201,10 +241,28 @@ static bool direct(int tokens, int top_k, int n_exp, int H) {
     return ((int64_t)tokens * top_k <= n_exp || tokens == 1) && fp8_blocks(H) * (FP8_BLOCK + 4) <= 65536 - 4096;
 }
 
-// Rows of a tile: as many as an expert has in the mean, that no more weights are read twice than have to be, and few rows stand idle.
-static int expert_tile_rows(int pairs, int n_exp) {
-    const int mean = pairs / n_exp;
-    return mean <= 32 ? 32 : mean <= 64 ? 64 : 128;
+// The forms of the two products.
+//
+// First: tiles of 64 rows (waves of 32 x 64) up to 64 rows per expert in the mean, of 128 (waves of 64 x 64) beyond; a wave without rows
+// costs little.  Whole blocks, us: 16 rows per expert, 8 of [14336 x 4096], 342 against 362 of 128; 28, 64 of [1408 x 2048], 135 / 146;
+// 50, 8 of [14336 x 4096], 338 / 345; 94, 4 of [4608 x 640], 60 / 55; 128, 8 of [14336 x 4096], 521 / 510; 512 1557 / 1374.
+//
+// Second: the dense forms by estimated time (tiled_walk_us); of an expert's last tile half is taken to be rows, pairs / rows + experts / 2
+// tiles.  16 rows for each of 8 experts of [4096 x 14336] 323 us in tiles of 32 rows against 358 of 256, 512 rows 1582 / 1328.
+static bool up_takes_64(int pairs, int n_exp) { return pairs <= 64 * n_exp; }
+static int down_form(int pairs, int n_exp, int H, int I) {
+    const int64_t extra = (pairs < n_exp ? pairs : n_exp + 1) / 2;
+    int best = TILED_32;
+    float least = 0.0f;
+    for (int form = 0; form < TILED_COUNT; form++) {
+        const TiledForm &f = TILED_FORMS[form];
+        const float us = tiled_walk_us(f.step_us, f.alone_us, f.per_cu, (pairs / f.rows + extra) * ((H + f.cols - 1) / f.cols), I / FP8_BLOCK);
+        if (form == 0 || us < least) {
+            least = us;
+            best = form;
+        }
+    }
+    return best;
 }
 
 struct ExpertsSpace {
@@ -260,7 +318,9 @@ template <typename AT> static int launch_experts_t(ExpertsArgs p, const ExpertsS
         return 0;
     }
     int32_t *const offsets = (int32_t *)(ws + at.offsets), *const order = (int32_t *)(ws + at.order), *const pos = (int32_t *)(ws + at.pos);
-    const int KB = fp8_blocks(p.H), quantizing = (int)(((int64_t)tokens * KB + 31) / 32);
+    const int KB = fp8_blocks(p.H);
+    if ((int64_t)tokens * KB > (int64_t)1 << 34) return -3;
+    const int quantizing = (int)(((int64_t)tokens * KB + 31) / 32);
     const bool sorts = pairs <= EXPERTS_SORT_PAIRS;
     hipLaunchKernelGGL((block_fp8_expert_rows_kernel<AT>), dim3(quantizing + (sorts ? (pairs + p.n_exp + 4) / 4 : 0)), dim3(256), 0, st, (const AT *)p.x,
                        p.ids, ws + at.x, (float *)(ws + at.xs), offsets, order, pos, tokens, pairs, p.n_exp, p.H, KB, quantizing);
@@ -276,19 +336,14 @@ template <typename AT> static int launch_experts_t(ExpertsArgs p, const ExpertsS
     d.x = p.h; d.xs = p.hs; d.ldx = p.I; d.ldxs = p.ldh;
     d.w = p.down; d.ws = p.down_scale; d.N = p.H; d.K = p.I; d.KB = p.I / FP8_BLOCK;
     d.y = ws + at.y;
-    const int rows = expert_tile_rows(pairs, p.n_exp);
-    u.tiles_m = d.tiles_m = pairs / rows + (pairs < p.n_exp ? pairs : p.n_exp);      // at most
+    const bool small = up_takes_64(pairs, p.n_exp);
+    const int form = down_form(pairs, p.n_exp, p.H, p.I), used = pairs < p.n_exp ? pairs : p.n_exp;
+    u.tiles_m = pairs / (small ? 64 : 128) + used;           // at most
+    d.tiles_m = pairs / TILED_FORMS[form].rows + used;
     if ((int64_t)u.tiles_m * (p.I / FP8_BLOCK) > 0x7fffffff - 8 || (int64_t)d.tiles_m * ((p.H + 127) / 128) > 0x7fffffff - 8) return -3;
-    if (rows == 128) {
-        launch_tiled<AT, true, TILED_UP, true, true, 4, 4, 2, 4, 2, 2>(u, st);
-        launch_tiled<AT, false, TILED_PLAIN, true, false, 4, 4, 2, 4, 3, 2>(d, st);
-    } else if (rows == 64) {
-        launch_tiled<AT, true, TILED_UP, true, true, 2, 4, 2, 4, 3, 2>(u, st);
-        launch_tiled<AT, false, TILED_PLAIN, true, false, 2, 4, 2, 2, 3, 2>(d, st);
-    } else {
-        launch_tiled<AT, true, TILED_UP, true, true, 2, 4, 1, 4, 3, 1>(u, st);
-        launch_tiled<AT, false, TILED_PLAIN, true, false, 2, 2, 1, 4, 3, 2>(d, st);
-    }
+    if (small) launch_tiled<AT, true, TILED_UP, true, true, 2, 4, 2, 4, 3, 2>(u, st);
+    else launch_tiled<AT, true, TILED_UP, true, true, 4, 4, 2, 4, 2, 2>(u, st);
+    launch_tiled_form<AT, false, TILED_PLAIN, true>(d, form, st);
     launch_moe_combine(ws + at.y, pos, weight, w_dtype, out, act_dtype, tokens, p.top_k, p.H, st);
     return 0;
 }

@@ -302,6 +302,28 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void block_fp8_tiled_kerne
         if constexpr (HALVES == 2) fetch_slot(b0 + 1 < last ? b0 + 1 : last, 1, EARLY, PIECES, i);
         else fetch_slot(b0 + S - 1 < last ? b0 + S - 1 : last, S - 1, 0, PIECES, i);
     }
+    // A wave whose rows are all past the end loads its share and keeps the barriers: a tile of up to half its rows takes little more than half
+    // the time, where an expert's last one would otherwise cost as much as a whole one.
+    if (m0 + wm * TM * 16 >= end) {
+        for (int kb = b0; kb < b1; kb++) {
+            const int late = kb + S - 1 < last ? kb + S - 1 : last, next = kb + S < last ? kb + S : last, behind = which > 0 ? which - 1 : S - 1;
+#pragma unroll
+            for (int o = 0; o < COUNT - TM; o++) {
+                if (o == TURN) meet();
+                if constexpr (HALVES == 2) {
+                    if (o < TURN) fetch_slot(late, behind, EARLY, PIECES, TM + o);
+                    else fetch_slot(next, which, 0, EARLY, o - TURN);
+                } else fetch_slot(late, behind, 0, PIECES, TM + o);
+            }
+            meet();
+#pragma unroll
+            for (int i = 0; i < TM; i++) {
+                if constexpr (HALVES == 2) fetch_slot(next, which, EARLY, PIECES, i);
+                else fetch_slot(next, which, 0, PIECES, i);
+            }
+            which = which + 1 < S ? which + 1 : 0;
+        }
+    } else
     for (int kb = b0;;) {
         const int buffer = which * BUFFER, then = which + 1 < S ? which + 1 : 0, other = then * BUFFER;
         const int late = kb + S - 1 < last ? kb + S - 1 : last, next = kb + S < last ? kb + S : last;

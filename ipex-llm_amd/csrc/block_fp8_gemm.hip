@@ -28,18 +28,22 @@ __global__ __launch_bounds__(256) void block_fp8_reduce_kernel(const f32x4 *__re
 
 static int cdiv(int a, int b) { return (a + b - 1) / b; }
 
-// Estimated time in us: rounds of workgroups over the GPU, each a walk of `steps` blocks, and what a launch, its first loads and its
-// stores take.  A step is shorter on a CU that runs one workgroup where two fit, and while few CUs share the memory.  The constants are
-// fitted to 5000 timed launches of 550 sizes, 5 to 8192 rows by 256 to 28672 by 512 to 16384; the pick is 1 % above the fastest of the forms
-// and splits on average, 17 % at worst.
+// Rounds of workgroups over the GPU, each a walk of `steps` blocks.  A step is shorter on a CU that runs one workgroup where two fit, and
+// while few CUs share the memory.
+float tiled_walk_us(float step_us, float alone_us, int per_cu, int64_t units, int steps) {
+    const int slots = 256 * per_cu;
+    const int64_t rounds = units / slots, rest = units - rounds * slots;
+    return steps * (rounds * step_us + (!rest ? 0.0f : rest <= 256 ? alone_us : step_us));
+}
+
+// Estimated time in us: the walks, and what a launch, its first loads and its stores take; with splits the sums, written and read in
+// float32.  The constants are fitted to 5000 timed launches of 550 sizes, 5 to 8192 rows by 256 to 28672 by 512 to 16384; the pick is 1 %
+// above the fastest of the forms and splits on average, 17 % at worst.
 static float tiled_us(int form, int M, int N, int KB, int splits, bool exact) {
     const TiledForm &f = TILED_FORMS[form];
-    const int slots = 256 * f.per_cu, steps = cdiv(KB, splits);
-    const int64_t units = (int64_t)cdiv(M, f.rows) * cdiv(N, f.cols) * splits, rounds = units / slots, rest = units - rounds * slots;
-    float per_step = exact ? f.exact_us : f.step_us;
-    const float alone = rest ? (rest <= 256 ? (exact ? f.exact_alone_us : f.alone_us) : per_step) : 0.0f;
-    float us = steps * (rounds * per_step + alone) + (exact ? 5.1f : 5.6f);
-    if (splits > 1) us += (exact ? 1.6f : 1.4f) + (float)splits * M * N * 8.0f / 5.0e6f;   // (float32 sums, written and read)
+    const int64_t units = (int64_t)cdiv(M, f.rows) * cdiv(N, f.cols) * splits;
+    float us = tiled_walk_us(exact ? f.exact_us : f.step_us, exact ? f.exact_alone_us : f.alone_us, f.per_cu, units, cdiv(KB, splits)) + (exact ? 5.1f : 5.6f);
+    if (splits > 1) us += (exact ? 1.6f : 1.4f) + (float)splits * M * N * 8.0f / 5.0e6f;
     return us;
 }
 

@@ -25,14 +25,14 @@ struct TiledPlan {
 };
 
 // One launch per form; the wave tiles are 64 x 128, 64 x 64, 64 x 64, 32 x 64 and 32 x 32.
-template <typename OT, bool EXACT, TiledMode MODE> void launch_tiled_form(const TiledArgs &p, int form, hipStream_t st) {
+template <typename OT, bool EXACT, TiledMode MODE, bool BY_EXPERT = false> void launch_tiled_form(const TiledArgs &p, int form, hipStream_t st) {
     if (form == TILED_256) {
         // (the operands of a 64 x 128 wave tile in bfloat16 do not fit its registers: no plan asks for it)
-        if constexpr (!EXACT) launch_tiled<OT, EXACT, MODE, false, false, 4, 8, 4, 2, 2, 2>(p, st);
-    } else if (form == TILED_128_256) launch_tiled<OT, EXACT, MODE, false, false, 4, 4, 2, 4, EXACT ? 2 : 3, 2>(p, st);
-    else if (form == TILED_128) launch_tiled<OT, EXACT, MODE, false, false, 4, 4, 2, 2, EXACT ? 3 : 2, EXACT ? 1 : 2>(p, st);
-    else if (form == TILED_64) launch_tiled<OT, EXACT, MODE, false, false, 2, 4, 2, 2, EXACT ? 2 : 3, 2>(p, st);
-    else launch_tiled<OT, EXACT, MODE, false, false, 2, 2, 1, 4, 3, 2>(p, st);
+        if constexpr (!EXACT) launch_tiled<OT, EXACT, MODE, BY_EXPERT, false, 4, 8, 4, 2, 2, 2>(p, st);
+    } else if (form == TILED_128_256) launch_tiled<OT, EXACT, MODE, BY_EXPERT, false, 4, 4, 2, 4, EXACT ? 2 : 3, 2>(p, st);
+    else if (form == TILED_128) launch_tiled<OT, EXACT, MODE, BY_EXPERT, false, 4, 4, 2, 2, EXACT ? 3 : 2, EXACT ? 1 : 2>(p, st);
+    else if (form == TILED_64) launch_tiled<OT, EXACT, MODE, BY_EXPERT, false, 2, 4, 2, 2, EXACT ? 2 : 3, 2>(p, st);
+    else launch_tiled<OT, EXACT, MODE, BY_EXPERT, false, 2, 2, 1, 4, 3, 2>(p, st);
 }
 
 void launch_tiled_f16(const TiledArgs &p, int form, hipStream_t st);
@@ -41,6 +41,8 @@ void launch_tiled_f32(const TiledArgs &p, int form, hipStream_t st);
 void launch_tiled_part(const TiledArgs &p, int form, hipStream_t st);
 void launch_tiled_part_exact(const TiledArgs &p, int form, hipStream_t st);
 
+// Estimated time (us) of `units` tiles of a form that walk `steps` blocks each
+float tiled_walk_us(float step_us, float alone_us, int per_cu, int64_t units, int steps);
 TiledPlan block_fp8_tiled_plan(bool exact, int M, int N, int K);
 size_t block_fp8_tiled_part_bytes(const TiledPlan &plan, int M, int N);
 int launch_block_fp8_tiled(TiledArgs p, int dtype, const TiledPlan &plan, hipStream_t st);

@@ -204,6 +204,12 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const AT *__restrict__
 template <typename AT>
 static void launch_combine(const void *y, const int32_t *pos, const void *weight, int w_dtype, void *out, int tokens, int top_k,
                            int N, hipStream_t st) {
+    for (; tokens > 65535; tokens -= 65535) {                // (a grid's second dimension ends there)
+        launch_combine<AT>(y, pos, weight, w_dtype, out, 65535, top_k, N, st);
+        pos += (int64_t)65535 * top_k;
+        weight = (const uint8_t *)weight + (int64_t)65535 * top_k * (w_dtype == DT_F32 ? 4 : 2);
+        out = (AT *)out + (int64_t)65535 * N;
+    }
     const dim3 grid((N / 8 + 255) / 256, tokens);
     if (w_dtype == DT_F32)
         hipLaunchKernelGGL((moe_combine_kernel<AT, float>), grid, dim3(256), 0, st, (const AT *)y, pos, (const float *)weight, (AT *)out, top_k, N);
