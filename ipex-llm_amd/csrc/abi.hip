@@ -60,6 +60,9 @@ int launch_block_fp8_rows(const void *x, int dtype, int64_t rows, int K, uint8_t
                           int64_t block_step, hipStream_t st);
 int launch_block_fp8_weight(const void *w, int dtype, int64_t matrices, int N, int K, uint8_t *codes, float *scale, hipStream_t st);
 size_t block_fp8_linear_workspace_bytes(int dtype, int M, int N, int K);
+void block_fp8_linear_plan(int dtype, int M, int N, int K, int *plan3);
+void block_fp8_back_plan(int M, int N, int K, int *plan3);
+void block_fp8_experts_plan(int tokens, int top_k, int n_exp, int H, int I, int *plan4);
 int launch_block_fp8_linear(const void *x, const uint8_t *w, const float *ws, const void *bias, void *y, int dtype, int M, int N, int K,
                             uint8_t *space, hipStream_t st);
 size_t block_fp8_back_workspace_bytes(int dtype, int M, int N, int K);
@@ -790,6 +793,15 @@ int lowbit_block_fp8_linear(const void *x, const void *w, const float *w_scale, 
                                                 (hipStream_t)stream), what);
 }
 
+int lowbit_block_fp8_plan(int dtype, int backward, int64_t M, int64_t N, int64_t K, int *plan3) {
+    const char *what = "lowbit_block_fp8_plan";
+    if (int rc = check_block_fp8(what, dtype, !backward, M, N, K)) return rc;
+    if (M == 0 || N == 0 || K == 0 || !plan3) return fail(LOWBIT_EARG, "%s: sizes must be positive, plan3 not null", what);
+    if (backward) block_fp8_back_plan((int)M, (int)N, (int)K, plan3);
+    else block_fp8_linear_plan(dtype, (int)M, (int)N, (int)K, plan3);
+    return 0;
+}
+
 size_t lowbit_block_fp8_backward_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K) {
     if (M <= 0 || N <= 0 || K <= 0 || M >= (1 << 22) || N >= (1 << 23) || K >= (1 << 23) || K % 16) return 0;
     return block_fp8_back_workspace_bytes(dtype, (int)M, (int)N, (int)K);
@@ -815,6 +827,13 @@ static bool block_fp8_experts_ok(int64_t tokens, int64_t top_k, int64_t n_expert
 size_t lowbit_block_fp8_experts_workspace_bytes(int64_t tokens, int top_k, int n_experts, int64_t hidden, int64_t inter) {
     if (!block_fp8_experts_ok(tokens, top_k, n_experts, hidden, inter) || hidden % 16 || inter % 128) return 0;
     return block_fp8_experts_workspace_bytes((int)tokens, top_k, n_experts, (int)hidden, (int)inter);
+}
+
+int lowbit_block_fp8_experts_plan(int64_t tokens, int top_k, int n_experts, int64_t hidden, int64_t inter, int *plan4) {
+    if (tokens <= 0 || !block_fp8_experts_ok(tokens, top_k, n_experts, hidden, inter) || hidden % 16 || inter % 128 || !plan4)
+        return fail(LOWBIT_EARG, "lowbit_block_fp8_experts_plan: sizes that lowbit_block_fp8_experts does not take, or plan4 null");
+    block_fp8_experts_plan((int)tokens, top_k, n_experts, (int)hidden, (int)inter, plan4);
+    return 0;
 }
 
 int lowbit_block_fp8_experts(const void *x, const int64_t *topk_ids, const void *topk_weight, int weight_dtype, int64_t tokens, int top_k,

@@ -230,32 +230,49 @@ __global__ __launch_bounds__(256) void block_fp8_pad_kernel(const uint16_t *__re
 
 static int cdiv(int a, int b) { return (a + b - 1) / b; }
 
-// Tiles of 128 x 256 and, while those leave the GPU idle, of 64 x 128, two to a CU; blocks of N split where they do too.
+// Rows and columns of a tile, workgroups that a CU holds, and a block's time (us) with the GPU full and with one workgroup on a CU.  Each wave
+// takes all rows of its tile and 32 columns of it, so that a weight is widened once: at 2048 x 4096 (N) x 11008 waves of 64 x 64 in the
+// first form take 195 us where these take 189.
+struct BackForm {
+    int rows, cols, per_cu;
+    float block_us, alone_us;
+};
+enum { BACK_128, BACK_64, BACK_32, BACK_COUNT };
+static const BackForm BACK_FORMS[BACK_COUNT] = {{128, 256, 1, 1.85f, 1.74f}, {64, 128, 2, 1.10f, 0.71f}, {32, 128, 2, 0.85f, 0.64f}};
+
+// The form and the splits of N with the smallest estimate: rounds of workgroups over the GPU, and the sum of the splits, written and read in
+// float32.  The constants are fitted to 15000 timed launches of 775 sizes, 1 to 8192 rows by 256 to 16384 (N, K); on as many others the pick
+// is 0.5 % above the fastest form and split on average, 34 % at worst (1.5 us).
 struct BackPlan {
-    bool large;
-    int splits;
+    int form, splits;
 };
 static BackPlan back_plan(int M, int N, int K) {
     const int NB = fp8_blocks(N);
-    BackPlan best = {true, 1};
+    BackPlan best = {BACK_128, 1};
     float least = 0.0f;
-    for (int large = 1; large >= 0; large--) {
+    for (int form = 0; form < BACK_COUNT; form++) {
+        const BackForm &f = BACK_FORMS[form];
         static const int tried[] = {1, 2, 3, 4, 6, 8};
-        const int64_t tiles = large ? (int64_t)cdiv(M, 128) * cdiv(K, 256) : (int64_t)cdiv(M, 64) * cdiv(K, 128);
+        const int64_t tiles = (int64_t)cdiv(M, f.rows) * cdiv(K, f.cols);
         for (int splits : tried) {
             if (splits > 1 && (NB < splits || tiles >= 512 || (size_t)splits * M * K * 4 > (size_t)256 << 20)) break;
-            const int64_t units = tiles * splits, slots = large ? 256 : 512, rounds = units / slots, rest = units - rounds * slots;
-            const float full = large ? 1.9f : 1.2f, alone = !rest ? 0.0f : large ? 1.8f : rest <= 256 ? 0.8f : 1.2f;
-            float us = cdiv(NB, splits) * (rounds * full + alone) + 4.0f;
-            if (splits > 1) us += 2.0f + (float)splits * M * K * 8.0f / 4.0e6f;
+            float us = tiled_walk_us(f.block_us, f.alone_us, f.per_cu, tiles * splits, cdiv(NB, splits)) + 6.3f;
+            if (splits > 1) us += 1.6f + (float)splits * M * K * 8.0f / 5.0e6f;
             if (least == 0.0f || us < least) {
                 least = us;
-                best = {large != 0, splits};
+                best = {form, splits};
             }
         }
     }
-    best.splits = cdiv(NB, cdiv(NB, best.splits));
+    best.splits = cdiv(NB, cdiv(NB, best.splits));           // (every split has a block)
     return best;
+}
+
+void block_fp8_back_plan(int M, int N, int K, int *plan3) {
+    const BackPlan plan = back_plan(M, N, K);
+    plan3[0] = BACK_FORMS[plan.form].rows;
+    plan3[1] = BACK_FORMS[plan.form].cols;
+    plan3[2] = plan.splits;
 }
 
 static bool padded(int N) { return N % 8 != 0; }
@@ -268,11 +285,12 @@ size_t block_fp8_back_workspace_bytes(int dtype, int M, int N, int K) {
 
 void launch_block_fp8_reduce(const float *part, const void *bias, void *y, int dtype, int M, int N, int splits, hipStream_t st);
 
-template <typename AT, bool PART> static void launch_back(const BackArgs &p, bool large, hipStream_t st) {
+template <typename AT, bool PART> static void launch_back(const BackArgs &p, int form, hipStream_t st) {
     const uint32_t units = (uint32_t)(p.tiles_m * p.tiles_k * p.splits);
     const dim3 grid((units + 7) / 8 * 8);
-    if (large) hipLaunchKernelGGL((block_fp8_back_kernel<AT, PART, 4, 4, 2, 4, 4, 2>), grid, dim3(512), 0, st, p);
-    else hipLaunchKernelGGL((block_fp8_back_kernel<AT, PART, 2, 4, 2, 2, 4, 2>), grid, dim3(256), 0, st, p);
+    if (form == BACK_128) hipLaunchKernelGGL((block_fp8_back_kernel<AT, PART, 8, 2, 1, 8, 4, 2>), grid, dim3(512), 0, st, p);
+    else if (form == BACK_64) hipLaunchKernelGGL((block_fp8_back_kernel<AT, PART, 4, 2, 1, 4, 4, 2>), grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((block_fp8_back_kernel<AT, PART, 2, 2, 1, 4, 5, 2>), grid, dim3(256), 0, st, p);
 }
 
 int launch_block_fp8_back(const void *grad, const uint8_t *w, const float *ws, void *gx, int dtype, int M, int N, int K, uint8_t *space,
@@ -280,7 +298,7 @@ int launch_block_fp8_back(const void *grad, const uint8_t *w, const float *ws, v
     if (dtype != DT_F16 && dtype != DT_BF16) return -4;
     const BackPlan plan = back_plan(M, N, K);
     BackArgs p = {grad, w, ws, gx, (float *)(space + padded_bytes(M, N)), N, M, N, K, fp8_blocks(N), fp8_blocks(K),
-                  cdiv(M, plan.large ? 128 : 64), cdiv(K, plan.large ? 256 : 128), plan.splits, cdiv(fp8_blocks(N), plan.splits)};
+                  cdiv(M, BACK_FORMS[plan.form].rows), cdiv(K, BACK_FORMS[plan.form].cols), plan.splits, cdiv(fp8_blocks(N), plan.splits)};
     if ((int64_t)p.tiles_m * p.tiles_k * p.splits > 0x7fffffff - 8) return -3;
     if (padded(N)) {
         p.ldg = cdiv(N, BACK_STEP) * BACK_STEP;
@@ -291,11 +309,11 @@ int launch_block_fp8_back(const void *grad, const uint8_t *w, const float *ws, v
         p.g = space;
     }
     if (plan.splits > 1) {
-        if (dtype == DT_F16) launch_back<_Float16, true>(p, plan.large, st);
-        else launch_back<__bf16, true>(p, plan.large, st);
+        if (dtype == DT_F16) launch_back<_Float16, true>(p, plan.form, st);
+        else launch_back<__bf16, true>(p, plan.form, st);
         launch_block_fp8_reduce(p.part, nullptr, gx, dtype, M, K, plan.splits, st);
-    } else if (dtype == DT_F16) launch_back<_Float16, false>(p, plan.large, st);
-    else launch_back<__bf16, false>(p, plan.large, st);
+    } else if (dtype == DT_F16) launch_back<_Float16, false>(p, plan.form, st);
+    else launch_back<__bf16, false>(p, plan.form, st);
     return 0;
 }
 

@@ -40,7 +40,7 @@ __device__ inline float lane_value(float held, int l) {
 }
 
 // One pair: a workgroup's wave w has 16 columns of g and the same of u, all of K, STEPS blocks in flight.  x is quantized by each workgroup.
-// Bound by memory: two experts of [14336 x 4096], 235 MB, in UPTIME us.
+// Bound by memory: two experts of [14336 x 4096], 235 MB, in 47 us.
 template <typename AT>
 __global__ __launch_bounds__(512) void block_fp8_expert_token_up_kernel(const ExpertsArgs p) {
     constexpr int STEPS = 4;
@@ -136,7 +136,7 @@ __global__ __launch_bounds__(512) void block_fp8_expert_token_up_kernel(const Ex
 }
 
 // One token's 16 columns per workgroup: the blocks of all its pairs are dealt to the waves, STEPS of them in flight per wave.  Bound by
-// memory: two experts of [4096 x 14336], 117 MB, in DOWNTIME us.
+// memory: two experts of [4096 x 14336], 117 MB, in 25 us.
 template <typename AT, typename PT>
 __global__ __launch_bounds__(512) void block_fp8_expert_down_token_kernel(const ExpertsArgs p, const PT *__restrict__ weight, AT *__restrict__ out) {
     constexpr int STEPS = 4;
@@ -263,6 +263,17 @@ static int down_form(int pairs, int n_exp, int H, int I) {
         }
     }
     return best;
+}
+
+void block_fp8_experts_plan(int tokens, int top_k, int n_exp, int H, int I, int *plan4) {
+    const int pairs = tokens * top_k;
+    plan4[0] = plan4[1] = plan4[2] = plan4[3] = 0;
+    if (direct(tokens, top_k, n_exp, H)) return;
+    const TiledForm &down = TILED_FORMS[down_form(pairs, n_exp, H, I)];
+    plan4[0] = up_takes_64(pairs, n_exp) ? 64 : 128;
+    plan4[1] = down.rows;
+    plan4[2] = down.cols;
+    plan4[3] = pairs > EXPERTS_SORT_PAIRS;
 }
 
 struct ExpertsSpace {

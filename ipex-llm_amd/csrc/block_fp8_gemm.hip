@@ -50,7 +50,8 @@ static float tiled_us(int form, int M, int N, int KB, int splits, bool exact) {
 TiledPlan block_fp8_tiled_plan(bool exact, int M, int N, int K) {
     const int KB = fp8_blocks(K);
     TiledPlan best = {TILED_128_256, 1, 0.0f};
-    for (int form = exact ? TILED_128_256 : TILED_256; form < TILED_COUNT; form++) {
+    for (int form = 0; form < TILED_COUNT; form++) {
+        if (exact && TILED_FORMS[form].exact_us == 0.0f) continue;
         static const int tried[] = {1, 2, 3, 4, 6, 8};
         for (int splits : tried) {
             if (splits > 1 && (KB < 2 * splits || (int64_t)cdiv(M, TILED_FORMS[form].rows) * cdiv(N, TILED_FORMS[form].cols) >= 512)) break;

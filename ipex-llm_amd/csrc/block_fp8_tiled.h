@@ -5,7 +5,8 @@
 namespace lowbit {
 
 // rows and weight rows of a tile, workgroups that a CU holds, and a step's time (us): with the GPU full, with one workgroup on a CU; the
-// same with float32 results, whose codes go through the bfloat16 MFMA
+// same with float32 results, whose codes go through the bfloat16 MFMA (0: no such form; waves of 64 x 64 on a tile of 128 x 128 take 2.8 us
+// there, and no size would choose them)
 struct TiledForm {
     int rows, cols, per_cu;
     float step_us, alone_us, exact_us, exact_alone_us;
@@ -14,7 +15,7 @@ enum { TILED_256, TILED_128_256, TILED_128, TILED_64, TILED_32, TILED_COUNT };
 static const TiledForm TILED_FORMS[TILED_COUNT] = {
     {256, 256, 1, 1.81f, 1.69f, 0.0f, 0.0f},
     {128, 256, 1, 1.30f, 0.97f, 2.07f, 1.59f},
-    {128, 128, 2, 1.01f, 0.66f, 2.77f, 1.21f},
+    {128, 128, 2, 1.01f, 0.66f, 0.0f, 0.0f},
     {64, 128, 2, 0.82f, 0.41f, 1.07f, 0.77f},
     {32, 128, 2, 0.66f, 0.32f, 0.73f, 0.53f},
 };
@@ -30,8 +31,9 @@ template <typename OT, bool EXACT, TiledMode MODE, bool BY_EXPERT = false> void 
         // (the operands of a 64 x 128 wave tile in bfloat16 do not fit its registers: no plan asks for it)
         if constexpr (!EXACT) launch_tiled<OT, EXACT, MODE, BY_EXPERT, false, 4, 8, 4, 2, 2, 2>(p, st);
     } else if (form == TILED_128_256) launch_tiled<OT, EXACT, MODE, BY_EXPERT, false, 4, 4, 2, 4, EXACT ? 2 : 3, 2>(p, st);
-    else if (form == TILED_128) launch_tiled<OT, EXACT, MODE, BY_EXPERT, false, 4, 4, 2, 2, EXACT ? 3 : 2, EXACT ? 1 : 2>(p, st);
-    else if (form == TILED_64) launch_tiled<OT, EXACT, MODE, BY_EXPERT, false, 2, 4, 2, 2, EXACT ? 2 : 3, 2>(p, st);
+    else if (form == TILED_128) {
+        if constexpr (!EXACT) launch_tiled<OT, EXACT, MODE, BY_EXPERT, false, 4, 4, 2, 2, 2, 2>(p, st);
+    } else if (form == TILED_64) launch_tiled<OT, EXACT, MODE, BY_EXPERT, false, 2, 4, 2, 2, EXACT ? 2 : 3, 2>(p, st);
     else launch_tiled<OT, EXACT, MODE, BY_EXPERT, false, 2, 2, 1, 4, 3, 2>(p, st);
 }
 

@@ -472,6 +472,26 @@ def lowbit_block_fp8_backward_workspace_bytes(dtype, m, n, k) -> int:
     return _lib.lowbit_block_fp8_backward_workspace_bytes(dtype, m, n, k)
 
 
+_lib.lowbit_block_fp8_plan.argtypes = [c_int, c_int, c_int64, c_int64, c_int64, ctypes.POINTER(c_int)]
+_lib.lowbit_block_fp8_plan.restype = c_int
+_lib.lowbit_block_fp8_experts_plan.argtypes = [c_int64, c_int, c_int, c_int64, c_int64, ctypes.POINTER(c_int)]
+_lib.lowbit_block_fp8_experts_plan.restype = c_int
+
+
+def lowbit_block_fp8_plan(dtype, backward, m, n, k):
+    """(rows, columns of a tile (0, 0: the kernel of few rows), parts of the sum) of what lowbit_block_fp8_linear or _backward runs."""
+    plan3 = (c_int * 3)()
+    _check(_lib.lowbit_block_fp8_plan(dtype, backward, m, n, k, plan3), "lowbit_block_fp8_plan")
+    return tuple(plan3)
+
+
+def lowbit_block_fp8_experts_plan(tokens, top_k, n_experts, hidden, inter):
+    """(rows of a tile of the first product, rows, columns of one of the second (0: pair by pair), whether the sort has its own launches)."""
+    plan4 = (c_int * 4)()
+    _check(_lib.lowbit_block_fp8_experts_plan(tokens, top_k, n_experts, hidden, inter, plan4), "lowbit_block_fp8_experts_plan")
+    return tuple(plan4)
+
+
 def lowbit_dequantize_rows(w, rows, n_rows, dst, qtype, n, k, layout, out_dtype, stream):
     _check(_lib.lowbit_dequantize_rows(w, rows, n_rows, dst, qtype, n, k, layout, out_dtype, stream),
            "lowbit_dequantize_rows")

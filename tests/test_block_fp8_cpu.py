@@ -169,3 +169,42 @@ def test_saved_layers_are_found_again(tmp_path):
     torch.save(state, tmp_path / "m.bin")
     again = torch.load(tmp_path / "m.bin", weights_only=True)
     assert again["q_proj.weight"].dtype == u.E4M3
+
+
+def test_sizes_of_the_gpu_tests_reach_every_kernel():
+    f32, bf16 = ggml.DT_F32, ggml.DT_BF16
+
+    def kinds(plans):
+        return {(rows, cols, splits > 1) for rows, cols, splits in plans}
+
+    every = {(rows, cols, split) for rows, cols in [(32, 128), (64, 128), (128, 256)] for split in (False, True)}
+    few = {(0, 0, False)}
+    more = {(rows, cols, split) for rows, cols in [(128, 128), (256, 256)] for split in (False, True)}
+    assert kinds(ggml.lowbit_block_fp8_plan(f32, 0, *s) for s in u.SHAPES + u.TILES) == every | few
+    assert kinds(ggml.lowbit_block_fp8_plan(bf16, 0, *s) for s in u.SHAPES + u.TILES) == every | few | more
+    assert kinds(ggml.lowbit_block_fp8_plan(bf16, 1, *s) for s in u.BACK_SHAPES + u.BACK_TILES) == every
+    plans = {ggml.lowbit_block_fp8_experts_plan(*s) for s in u.EXPERTS + u.EXPERT_TILES}
+    assert {p[0] for p in plans} == {0, 64, 128} and {p[3] for p in plans} == {0, 1}
+    assert {p[1:3] for p in plans} == {(0, 0), (32, 128), (64, 128), (128, 128), (128, 256), (256, 256)}
+
+
+def test_plans_hold_for_any_size():
+    """Whatever the size: a tile that is there, no empty part of the sum, and no more workspace than codes, scales and 256 MB of sums."""
+    for m in (1, 4, 5, 31, 128, 1000, 8192, (1 << 22) - 1):
+        for n in (1, 7, 128, 4097, 28672, (1 << 23) - 1):
+            for k in (16, 128, 144, 4096, 16384, (1 << 23) - 16):
+                for dtype in (ggml.DT_F16, ggml.DT_F32):
+                    rows, cols, splits = ggml.lowbit_block_fp8_plan(dtype, 0, m, n, k)
+                    assert (rows == 0) == (cols == 0) and 1 <= splits <= 8 and splits <= u.blocks(k)
+                    parts = -(-u.blocks(k) // splits)
+                    assert parts * (splits - 1) < u.blocks(k)
+                    bound = m * u.blocks(k) * (128 * (2 if dtype == ggml.DT_F32 else 1) + 4) + (256 << 20) + 1024
+                    assert ggml.lowbit_block_fp8_linear_workspace_bytes(dtype, m, n, k) <= bound
+                rows, cols, splits = ggml.lowbit_block_fp8_plan(ggml.DT_BF16, 1, m, n, k)
+                assert rows and cols and -(-u.blocks(n) // splits) * (splits - 1) < u.blocks(n)
+                assert ggml.lowbit_block_fp8_backward_workspace_bytes(ggml.DT_BF16, m, n, k) <= m * (n + 64) * 2 + (256 << 20) + 1024
+    for call in (lambda: ggml.lowbit_block_fp8_plan(ggml.DT_F32, 1, 1, 16, 16), lambda: ggml.lowbit_block_fp8_plan(ggml.DT_F16, 0, 0, 16, 16),
+                 lambda: ggml.lowbit_block_fp8_plan(ggml.DT_F16, 0, 1, 16, 24), lambda: ggml.lowbit_block_fp8_experts_plan(0, 1, 1, 16, 128),
+                 lambda: ggml.lowbit_block_fp8_experts_plan(1, 65, 1, 16, 128)):
+        with pytest.raises(Exception):
+            call()

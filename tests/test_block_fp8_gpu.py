@@ -106,9 +106,7 @@ def test_every_finite_bfloat16_rounds_to_the_nearest_code():
 
 # ---------------------------------------------------------------- products
 
-SHAPES = [(1, 16, 16), (1, 1, 128), (1, 40, 128), (2, 130, 272), (3, 4096, 512), (4, 129, 4096), (5, 64, 2112), (16, 300, 1024), (17, 100, 640),
-          (32, 256, 384), (33, 257, 1152), (64, 128, 4096), (65, 136, 1024), (100, 520, 528), (129, 384, 256), (200, 1000, 400),
-          (257, 272, 1536), (520, 640, 2048), (1030, 528, 384)]
+SHAPES = u.SHAPES
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
@@ -123,6 +121,12 @@ def test_product_is_exact_where_no_order_of_summation_rounds(dtype, m, n, k):
     assert y.dtype == dtype and torch.equal(y.cpu(), want.to(dtype))
     y = bf.block_fp8_linear(xd, wd, sd, bias.cuda())
     assert torch.equal(y.cpu(), (want + bias.double()).to(dtype))
+
+
+@pytest.mark.parametrize("m,n,k", u.TILES)
+@pytest.mark.parametrize("dtype", ALL, ids=ids)
+def test_product_in_tiles_of_every_form(dtype, m, n, k):
+    test_product_is_exact_where_no_order_of_summation_rounds(dtype, m, n, k)
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 512, 4096), (8, 300, 1040), (40, 1000, 4096), (130, 640, 2112), (600, 1100, 2048)])
@@ -192,8 +196,7 @@ def test_nothing_is_written_past_the_result(m, n, k):
 
 # ---------------------------------------------------------------- gradient
 
-BACK = [(1, 16, 16), (1, 130, 128), (5, 128, 272), (17, 300, 400), (64, 257, 640), (77, 1200, 1024), (130, 33, 2112), (200, 1000, 144),
-        (300, 512, 512), (520, 264, 1040)]
+BACK = u.BACK_SHAPES
 
 
 @pytest.mark.parametrize("m,n,k", BACK)
@@ -206,6 +209,12 @@ def test_gradient_is_grad_times_the_weight(dtype, m, n, k):
     y = bf.block_fp8_linear(x, w.cuda(), ws.cuda())
     got, = torch.autograd.grad(y, x, grad.cuda())
     assert got.dtype == dtype and torch.equal(got.cpu(), (grad.double() @ u.dense(w, ws)).to(dtype))
+
+
+@pytest.mark.parametrize("m,n,k", u.BACK_TILES)
+@pytest.mark.parametrize("dtype", HALF, ids=ids)
+def test_gradient_in_tiles_of_every_form(dtype, m, n, k):
+    test_gradient_is_grad_times_the_weight(dtype, m, n, k)
 
 
 @pytest.mark.parametrize("dtype", HALF, ids=ids)
@@ -346,14 +355,18 @@ def check_experts(case, dtype, act=0):
     return got
 
 
-EXPERTS = [(1, 2, 8, 128, 128), (1, 1, 1, 16, 128), (1, 8, 8, 400, 256), (2, 2, 16, 256, 384), (3, 4, 4, 272, 128), (40, 2, 5, 512, 256),
-           (130, 3, 4, 144, 384), (300, 2, 70, 256, 128), (17, 5, 3, 384, 256), (600, 1, 2, 640, 512)]
+EXPERTS = u.EXPERTS
 
 
 @pytest.mark.parametrize("tokens,top_k,n_exp,hidden,inter", EXPERTS)
 @pytest.mark.parametrize("dtype", HALF, ids=ids)
 def test_experts(dtype, tokens, top_k, n_exp, hidden, inter):
     check_experts(expert_case(tokens + hidden, tokens, top_k, n_exp, hidden, inter, dtype), dtype, act=tokens % 2)
+
+
+@pytest.mark.parametrize("tokens,top_k,n_exp,hidden,inter", u.EXPERT_TILES)
+def test_experts_in_tiles_of_every_form(tokens, top_k, n_exp, hidden, inter):
+    check_experts(expert_case(tokens, tokens, top_k, n_exp, hidden, inter, torch.bfloat16), torch.bfloat16)
 
 
 @pytest.mark.parametrize("tokens", [1, 3, 50])
