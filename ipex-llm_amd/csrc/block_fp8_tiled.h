@@ -11,13 +11,14 @@ struct TiledForm {
     int rows, cols, per_cu;
     float step_us, alone_us, exact_us, exact_alone_us;
 };
-enum { TILED_256, TILED_128_256, TILED_128, TILED_64, TILED_32, TILED_COUNT };
+enum { TILED_256, TILED_192_256, TILED_128_256, TILED_128, TILED_64, TILED_32, TILED_COUNT };
 static const TiledForm TILED_FORMS[TILED_COUNT] = {
-    {256, 256, 1, 1.81f, 1.69f, 0.0f, 0.0f},
-    {128, 256, 1, 1.30f, 0.97f, 2.07f, 1.59f},
-    {128, 128, 2, 1.01f, 0.66f, 0.0f, 0.0f},
-    {64, 128, 2, 0.82f, 0.41f, 1.07f, 0.77f},
-    {32, 128, 2, 0.66f, 0.32f, 0.73f, 0.53f},
+    {256, 256, 1, 1.89f, 1.48f, 0.0f, 0.0f},
+    {192, 256, 1, 1.44f, 1.19f, 0.0f, 0.0f},
+    {128, 256, 1, 1.24f, 0.85f, 2.07f, 1.59f},
+    {128, 128, 2, 1.01f, 0.60f, 0.0f, 0.0f},
+    {64, 128, 2, 0.72f, 0.40f, 1.07f, 0.77f},
+    {32, 128, 2, 0.59f, 0.31f, 0.73f, 0.53f},
 };
 
 struct TiledPlan {
@@ -25,11 +26,14 @@ struct TiledPlan {
     float us;
 };
 
-// One launch per form; the wave tiles are 64 x 128, 64 x 64, 64 x 64, 32 x 64 and 32 x 32.
+// One launch per form; the wave tiles are 64 x 128, 96 x 64, 64 x 64, 64 x 64, 32 x 64 and 32 x 32.
 template <typename OT, bool EXACT, TiledMode MODE, bool BY_EXPERT = false> void launch_tiled_form(const TiledArgs &p, int form, hipStream_t st) {
     if (form == TILED_256) {
         // (the operands of a 64 x 128 wave tile in bfloat16 do not fit its registers: no plan asks for it)
         if constexpr (!EXACT) launch_tiled<OT, EXACT, MODE, BY_EXPERT, false, 4, 8, 4, 2, 2, 2>(p, st);
+    } else if (form == TILED_192_256) {
+        // (rows of x in bfloat16 do not fit LDS twice)
+        if constexpr (!EXACT) launch_tiled<OT, EXACT, MODE, BY_EXPERT, false, 6, 4, 2, 4, 2, 2>(p, st);
     } else if (form == TILED_128_256) launch_tiled<OT, EXACT, MODE, BY_EXPERT, false, 4, 4, 2, 4, EXACT ? 2 : 3, 2>(p, st);
     else if (form == TILED_128) {
         if constexpr (!EXACT) launch_tiled<OT, EXACT, MODE, BY_EXPERT, false, 4, 4, 2, 2, 2, 2>(p, st);
