@@ -423,6 +423,111 @@ def test_experts_gradients_run_expert_by_expert():
     assert (gx.cpu().double() - wx).norm() <= 1e-3 * wx.norm() and (gp.cpu().double() - wp).norm() <= 1e-3 * wp.norm()
 
 
+# ---------------------------------------------------------------- what a product must keep apart
+
+@pytest.mark.parametrize("m,n,k", [(1, 33, 144), (3, 130, 272), (40, 257, 400), (300, 129, 144), (1347, 1459, 144)])
+@pytest.mark.parametrize("dtype", ALL, ids=ids)
+def test_nan_stays_in_its_row_and_column(dtype, m, n, k):
+    """NaN in a row of x (a padded batch's), in the weight's last row and in a block's scale: the results that they belong to and no others,
+    also where a tile or a block ends inside."""
+    g = gen(m + k)
+    x, (w, ws) = u.activations(g, m, k, dtype), u.weight(g, n, k, base=-8)
+    grad = torch.randint(-8, 9, (m, n), generator=g).to(dtype)
+    want, back = x.double() @ u.dense(w, ws).t(), grad.double() @ u.dense(w, ws)
+    bad_x, bad_w, bad_g = x.clone(), w.clone(), grad.clone()
+    bad_w.view(torch.uint8)[n - 1, k - 1] = 0x7f
+    if m > 1:
+        bad_x[m - 1, k - 1], bad_g[m - 1, n - 1] = math.nan, math.nan
+    leaf = bad_x.cuda().requires_grad_()
+    y = bf.block_fp8_linear(leaf, bad_w.cuda(), ws.cuda())
+    got, = torch.autograd.grad(y, leaf, bad_g.cuda())
+    want[:, n - 1], back[:, k - 1] = math.nan, math.nan
+    if m > 1:
+        want[m - 1], back[m - 1] = math.nan, math.nan
+    assert same(y.detach().cpu(), want.to(dtype)) and same(got.cpu(), back.to(dtype))
+    scale = ws.clone()
+    scale[-1, -1] = math.nan
+    y = bf.block_fp8_linear(x.cuda(), w.cuda(), scale.cuda()).cpu()
+    first = (n - 1) // 128 * 128
+    assert y[:, first:].isnan().all() and torch.equal(y[:, :first], (x.double() @ u.dense(w, ws).t()).to(dtype)[:, :first])
+
+
+def test_scales_of_zero_and_negative_ones():
+    g = gen(21)
+    x, (w, ws) = u.activations(g, 50, 512, torch.bfloat16), u.weight(g, 300, 512, base=-8)
+    ws[0, 1], ws[1], ws[2, 3] = 0, 0, -ws[2, 3]
+    assert torch.equal(bf.block_fp8_linear(x.cuda(), w.cuda(), ws.cuda()).cpu(), (x.double() @ u.dense(w, ws).t()).bfloat16())
+
+
+# ---------------------------------------------------------------- offsets past 32 bits
+
+def test_weights_of_more_than_2_to_32_codes():
+    n, k, tail = (1 << 18) + 200, 16384, 200                     # the last 200 rows lie past 2^32
+    g = gen(22)
+    w, ws = torch.zeros((n, k), dtype=torch.uint8, device="cuda").view(u.E4M3), torch.zeros((u.blocks(n), k // 128), device="cuda")
+    part, scale = u.weight(g, tail, k, base=-10)
+    w[n - tail:].copy_(part.cuda())
+    ws[-2:].copy_(scale.cuda())
+    assert (n - tail) % 128 == 0
+    for m in (1, 40, 300):
+        x = u.activations(g, m, k, torch.bfloat16, spread_bits=0).cuda()
+        y = bf.block_fp8_linear(x, w, ws)
+        assert torch.equal(y[:, n - tail:], bf.block_fp8_linear(x, part.cuda(), scale.cuda())) and not y[:, :n - tail].any()
+        del y
+    x = u.activations(g, 33, k, torch.bfloat16, spread_bits=0).cuda().requires_grad_()
+    grad = torch.zeros((33, n), dtype=torch.bfloat16, device="cuda")
+    grad[:, n - tail:] = torch.randint(-8, 9, (33, tail), generator=g).cuda().bfloat16()
+    got, = torch.autograd.grad(bf.block_fp8_linear(x, w, ws), x, grad)
+    assert torch.equal(got.cpu(), (grad[:, n - tail:].cpu().double() @ u.dense(part, scale)).bfloat16())
+    dense = torch.zeros((n, k), dtype=torch.bfloat16, device="cuda")
+    dense[n - 7:] = torch.randn((7, k), generator=g).cuda().bfloat16()
+    codes, scales = bf.block_fp8_quantize_weight(dense)
+    last, last_scale = bf.block_fp8_quantize_weight(dense[n - 72:])
+    assert torch.equal(codes[n - 72:].view(torch.uint8), last.view(torch.uint8)) and torch.equal(scales[-1:], last_scale)
+    codes, scales = bf.block_fp8_quantize(dense)
+    last, last_scale = bf.block_fp8_quantize(dense[n - 7:])
+    assert torch.equal(codes[n - 7:].view(torch.uint8), last.view(torch.uint8)) and torch.equal(scales[n - 7:], last_scale)
+
+
+def test_results_of_more_than_2_to_32_bytes():
+    g = gen(23)
+    m, n, k = 150000, 16384, 128                                 # y: 4.9 GB
+    w, ws = (t.cuda() for t in u.weight(g, n, k, base=-8))
+    x = torch.zeros((m, k), dtype=torch.bfloat16, device="cuda")
+    tail = u.activations(g, 300, k, torch.bfloat16).cuda()
+    x[m - 300:] = tail
+    y = bf.block_fp8_linear(x, w, ws)
+    assert torch.equal(y[m - 300:], bf.block_fp8_linear(tail, w, ws)) and not y[:m - 300].any()
+    del y
+    # the gradient of as many values: x [m, n], a weight [k, n]
+    w, ws = (t.cuda() for t in u.weight(g, k, n, base=-8))
+    x = torch.zeros((m, n), dtype=torch.bfloat16, device="cuda").requires_grad_()
+    grad = torch.zeros((m, k), dtype=torch.bfloat16, device="cuda")
+    grad[m - 300:] = torch.randint(-8, 9, (300, k), generator=g).cuda().bfloat16()
+    got, = torch.autograd.grad(bf.block_fp8_linear(x, w, ws), x, grad)
+    assert torch.equal(got[m - 300:].cpu(), (grad[m - 300:].cpu().double() @ u.dense(w.cpu(), ws.cpu())).bfloat16()) and not got[:m - 300].any()
+
+
+def test_experts_whose_weights_pass_2_to_32_codes():
+    g = gen(24)
+    n_exp, hidden, inter = 70, 4096, 8192                        # gate_up 4.7e9 codes, down 2.3e9
+    small = expert_case(25, 4, 2, 2, hidden, inter, torch.bfloat16)
+    big = []
+    for t in small[3:]:
+        whole = torch.zeros((n_exp, *t.shape[1:]), dtype=torch.uint8 if t.dtype == u.E4M3 else t.dtype, device="cuda")
+        whole = whole.view(u.E4M3) if t.dtype == u.E4M3 else whole
+        whole[n_exp - 2:].copy_(t.cuda())
+        big.append(whole)
+    for tokens in (1, 50):
+        x = u.activations(g, tokens, hidden, torch.bfloat16, spread_bits=0).cuda()
+        picks = torch.randint(0, 2, (tokens, 2), generator=g).cuda()
+        p = torch.rand((tokens, 2), generator=g).bfloat16().cuda()
+        got = bf.block_fp8_experts(x, picks + n_exp - 2, p, *big)
+        want = bf.block_fp8_experts(x, picks, p, *(t.cuda() for t in small[3:]))
+        # (another kernel may run the smaller case: rounded per pair or not)
+        assert (got.double() - want.double()).norm() <= 2.0 ** -7 * want.double().norm() and want.any()
+
+
 # ---------------------------------------------------------------- streams, graphs, together
 
 def test_another_stream_and_many_at_once():
