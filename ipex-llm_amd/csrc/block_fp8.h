@@ -129,6 +129,19 @@ template <typename AT> __device__ inline u32x4 quantize16(const float (&v)[16], 
     return c;
 }
 
+// One block of a row from 16 neighbouring lanes of 8 values each: their codes to LDS, and the block's scale (first: the block's first lane).
+template <typename AT, typename V8> __device__ inline void put8(const V8 &v, uint8_t *codes, float *scale, bool first) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) m = max_u32(m, magnitude((float)v[i]));
+    m = max_of_16(m);
+    const float s = block_scale(m);
+    const Quotient<AT> q(s, m);
+    *(u32x2 *)codes = u32x2{encode4(q((float)v[0]), q((float)v[1]), q((float)v[2]), q((float)v[3])),
+                            encode4(q((float)v[4]), q((float)v[5]), q((float)v[6]), q((float)v[7]))};
+    if (first) *scale = s;
+}
+
 // 16 codes of a row to its k-th byte, or (WIDE) the same numbers in bfloat16
 template <bool WIDE> __device__ inline void store16(uint8_t *row, int k, u32x4 c) {
     if constexpr (WIDE) {

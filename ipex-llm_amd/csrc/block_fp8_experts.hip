@@ -22,9 +22,7 @@ struct ExpertsArgs {
     const int64_t *ids;
     const uint8_t *gate_up, *down;
     const float *gate_up_scale, *down_scale;
-    uint8_t *h;                                              // codes [pairs, I], by pair (few pairs) or by sorted position
-    float *hs;                                               // [blocks of I][ldh]
-    int ldh;
+    uint8_t *h;                                              // few pairs: float32 [pairs, I]; else codes [pairs, I], by sorted position
     int n_exp, top_k, H, I, act;
 };
 
@@ -39,108 +37,99 @@ __device__ inline float lane_value(float held, int l) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, held), l));
 }
 
-// One pair: a workgroup's wave w has 16 columns of g and the same of u, all of K, STEPS blocks in flight.  x is quantized by each workgroup.
-// Bound by memory: two experts of [14336 x 4096], 235 MB, in 47 us.
+// One pair's 16 columns of h per workgroup: 16 rows of the gate and 16 of u.  The blocks of K are dealt to the waves, STEPS of them in flight
+// per wave, whose sums meet in LDS.  x is quantized by each workgroup; h leaves in float32, since its blocks are of 128 columns: with 128
+// columns per workgroup six experts of [1408 x 2048] would keep 66 CUs busy.  Bound by memory: two experts of [14336 x 4096], 235 MB, in 45 us.
 template <typename AT>
 __global__ __launch_bounds__(512) void block_fp8_expert_token_up_kernel(const ExpertsArgs p) {
-    constexpr int STEPS = 4;
+    constexpr int STEPS = 2, WAVES = 8, THREADS = 64 * WAVES, HELD = 2;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    __shared__ uint32_t part[8];
+    __shared__ float sums[WAVES][2][16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
-    const int cb = blockIdx.x, pair = blockIdx.y, H = p.H, KB = fp8_blocks(H);
+    const int c0 = blockIdx.x * 16, pair = blockIdx.y, H = p.H, KB = fp8_blocks(H);
     const int64_t e = p.ids[pair];
     if (e < 0 || e >= p.n_exp) return;                       // (the second product skips the pair)
 
-    // the row's first 8192 values are asked for ahead of the weights: loads return in order
-    const AT *const x = (const AT *)p.x + (int64_t)(pair / p.top_k) * H;
-    float v[16] = {};
-    const int own = (int)threadIdx.x * 16;
-    if (own < H) load16(x + own, v);
+    // x is asked for ahead of the weights: loads return in order
+    using V8 = typename Vec8<AT>::type;
+    const V8 *const x = (const V8 *)((const AT *)p.x + (int64_t)(pair / p.top_k) * H);
+    const int pieces = KB * 16;
+    V8 first[HELD];
+#pragma unroll
+    for (int i = 0; i < HELD; i++) {
+        const int at = threadIdx.x + i * THREADS;
+        first[i] = at * 8 < H ? x[at] : V8{};
+    }
     __builtin_amdgcn_sched_barrier(0);
 
-    const uint8_t *const w = p.gate_up + e * 2 * p.I * H;
     const uint8_t *row[2];
     const float *ws[2];
     float held[2];
+    auto hold = [&](int i) __attribute__((always_inline)) {  // the scales of this wave's blocks i .. i + 63 in the lanes of a register
+        const int kb = wave + (i + lane) * WAVES;
+#pragma unroll
+        for (int t = 0; t < 2; t++) held[t] = ws[t][kb < KB ? kb : KB - 1];
+    };
 #pragma unroll
     for (int t = 0; t < 2; t++) {
-        row[t] = w + (int64_t)(t * p.I + cb * FP8_BLOCK + wave * 16 + r) * H;
-        ws[t] = p.gate_up_scale + ((e * 2 + t) * (p.I / FP8_BLOCK) + cb) * KB;
-        held[t] = ws[t][lane < KB ? lane : KB - 1];          // scales of 64 blocks in the lanes of a register
+        row[t] = p.gate_up + (e * 2 * p.I + t * p.I + c0 + r) * H;
+        ws[t] = p.gate_up_scale + ((e * 2 + t) * (p.I / FP8_BLOCK) + c0 / FP8_BLOCK) * KB;
     }
+    hold(0);
     Codes wc[STEPS][2];
 #pragma unroll
     for (int s = 0; s < STEPS; s++)
 #pragma unroll
-        for (int t = 0; t < 2; t++) wc[s][t] = load_chunks(row[t], s < KB ? s : KB - 1, g, H);
+        for (int t = 0; t < 2; t++) wc[s][t] = load_chunks(row[t], wave + s * WAVES < KB ? wave + s * WAVES : KB - 1, g, H);
     __builtin_amdgcn_sched_barrier(0);
 
     float *const xs = (float *)(lds + KB * FP8_BLOCK);
-    for (int k = own; k < KB * FP8_BLOCK; k += 512 * 16) {
-        if (k != own) {
+    auto put = [&](int at, const V8 &v) __attribute__((always_inline)) { put8<AT>(v, lds + at * 8, xs + (at >> 4), (at & 15) == 0); };
 #pragma unroll
-            for (int i = 0; i < 16; i++) v[i] = 0.0f;
-            if (k < H) load16(x + k, v);
-        }
-        float s;
-        *(u32x4 *)(lds + k) = quantize16<AT>(v, s);
-        if ((threadIdx.x & 7) == 0) xs[k / FP8_BLOCK] = s;
-    }
+    for (int i = 0; i < HELD; i++)
+        if ((int)threadIdx.x + i * THREADS < pieces) put(threadIdx.x + i * THREADS, first[i]);    // (the 16 lanes of a block are in or out together)
+    for (int at = threadIdx.x + HELD * THREADS; at < pieces; at += THREADS) put(at, at * 8 < H ? x[at] : V8{});
     __syncthreads();
 
     f32x4 acc[2] = {};
-    for (int kb0 = 0; kb0 < KB; kb0 += STEPS) {
-        if ((kb0 & 63) == 0 && kb0 != 0)
-#pragma unroll
-            for (int t = 0; t < 2; t++) held[t] = ws[t][kb0 + lane < KB ? kb0 + lane : KB - 1];
-        Codes xc[STEPS];
-        float sx[STEPS];
+    for (int i0 = 0; wave + i0 * WAVES < KB; i0 += STEPS) {
+        if ((i0 & 63) == 0 && i0 != 0) hold(i0);
 #pragma unroll
         for (int s = 0; s < STEPS; s++) {
-            const int in = kb0 + s < KB ? kb0 + s : KB - 1;
+            const int kb = wave + (i0 + s) * WAVES, in = kb < KB ? kb : KB - 1, next = kb + STEPS * WAVES;
             const uint8_t *const xr = lds + in * FP8_BLOCK + g * 16;     // (all 16 rows of the operand are the one)
-            xc[s] = Codes{*(const u32x4 *)xr, *(const u32x4 *)(xr + 64)};
-            sx[s] = xs[in];
-        }
-#pragma unroll
-        for (int s = 0; s < STEPS; s++) {
-            const bool in = kb0 + s < KB;                    // (past the last block: it again, not added)
+            const Codes xc = {*(const u32x4 *)xr, *(const u32x4 *)(xr + 64)};
+            const float sx = xs[in];                         // (past the last block: it again, not added)
 #pragma unroll
             for (int t = 0; t < 2; t++) {
-                const f32x4 d = block_dot<true>(wc[s][t], xc[s]);
-                const float sc = sx[s] * lane_value(held[t], (kb0 + s) & 63);
+                const f32x4 d = block_dot<true>(wc[s][t], xc);
+                const float sc = sx * lane_value(held[t], (i0 + s) & 63);
 #pragma unroll
-                for (int j = 0; j < 4; j++) acc[t][j] = in ? fmaf(sc, d[j], acc[t][j]) : acc[t][j];
-                if (kb0 + s + STEPS < KB) wc[s][t] = load_chunks(row[t], kb0 + s + STEPS, g, H);
+                for (int j = 0; j < 4; j++) acc[t][j] = kb < KB ? fmaf(sc, d[j], acc[t][j]) : acc[t][j];
+                if (next < KB) wc[s][t] = load_chunks(row[t], next, g, H);
             }
         }
     }
-
-    float h[4];
-    uint32_t m = 0;
+    if (r == 0)
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        h[j] = gate_act(acc[0][j], p.act) * acc[1][j];
-        m = max_u32(m, magnitude(h[j]));
-    }
-    m = max_u32(m, (uint32_t)__shfl_xor((int)m, 16));
-    m = max_u32(m, (uint32_t)__shfl_xor((int)m, 32));
-    if (lane == 0) part[wave] = m;
+        for (int t = 0; t < 2; t++) *(f32x4 *)&sums[wave][t][g * 4] = acc[t];
     __syncthreads();
+    if (threadIdx.x >= 16) return;
+    float v[2] = {};
 #pragma unroll
-    for (int v = 0; v < 8; v++) m = max_u32(m, part[v]);
-    const float s = block_scale(m), inv = __builtin_amdgcn_rcpf(s);
-    if (r != 0) return;
-    *(uint32_t *)(p.h + (int64_t)pair * p.I + cb * FP8_BLOCK + wave * 16 + g * 4) = encode4(h[0] * inv, h[1] * inv, h[2] * inv, h[3] * inv);
-    if (wave == 0 && g == 0) p.hs[(int64_t)cb * p.ldh + pair] = s;
+    for (int w = 0; w < WAVES; w++)
+#pragma unroll
+        for (int t = 0; t < 2; t++) v[t] += sums[w][t][threadIdx.x];
+    ((float *)p.h)[(int64_t)pair * p.I + c0 + threadIdx.x] = gate_act(v[0], p.act) * v[1];
 }
 
-// One token's 16 columns per workgroup: the blocks of all its pairs are dealt to the waves, STEPS of them in flight per wave.  Bound by
-// memory: two experts of [4096 x 14336], 117 MB, in 25 us.
-template <typename AT, typename PT>
-__global__ __launch_bounds__(512) void block_fp8_expert_down_token_kernel(const ExpertsArgs p, const PT *__restrict__ weight, AT *__restrict__ out) {
-    constexpr int STEPS = 4;
-    __shared__ float sums[8][16];
+// One token's 16 columns per workgroup, which quantizes h of all its pairs; their blocks are dealt to the waves, STEPS of them in flight per
+// wave.  Bound by memory: two experts of [4096 x 14336], 117 MB, in 25 us.
+template <typename AT, typename PT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void block_fp8_expert_down_token_kernel(const ExpertsArgs p, const PT *__restrict__ weight, AT *__restrict__ out) {
+    constexpr int STEPS = 4, HELD = 4, THREADS = 64 * WAVES;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    __shared__ float sums[WAVES][16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
     const int n0 = blockIdx.x * 16, token = blockIdx.y, I = p.I, IB = I / FP8_BLOCK, HB = fp8_blocks(p.H), top_k = p.top_k;
     // the pairs' experts (-1: none) and weights in the lanes of registers: top_k is 64 at most
@@ -152,37 +141,66 @@ __global__ __launch_bounds__(512) void block_fp8_expert_down_token_kernel(const 
         expert = e >= 0 && e < p.n_exp ? (int)e : -1;
         route = (float)weight[pair0 + lane];
     }
-    const uint64_t valid = __ballot(expert >= 0);
-    const int units = top_k * IB;
-    struct Unit {
-        Codes w, x;
-        float scale;
-    };
-    // unit u: block u % IB of pair u / IB; one of no expert, or past the last, counts nothing
-    auto load = [&](int u, Unit &t) __attribute__((always_inline)) {
-        const int j = u / IB, kb = u - j * IB;
-        t.scale = 0.0f;
-        t.w = Codes{};
-        t.x = Codes{};
-        if (u < units && (valid >> j & 1)) {                 // (the same for the whole wave)
-            const int64_t e = __builtin_amdgcn_readlane(expert, j);
-            t.w = load_chunks(p.down + (e * p.H + n0 + r) * I, kb, g, I);
-            const uint8_t *const xr = p.h + (int64_t)(pair0 + j) * I + kb * FP8_BLOCK + g * 16;
-            t.x = Codes{*(const u32x4 *)xr, *(const u32x4 *)(xr + 64)};
-            t.scale = p.hs[(int64_t)kb * p.ldh + pair0 + j] * p.down_scale[(e * HB + n0 / FP8_BLOCK) * IB + kb] * lane_value(route, j);
-        }
-    };
-    Unit unit[STEPS];
+    // h of the pairs, one row after the other (what a pair of no expert left there is not used)
+    typedef float f32x8 __attribute__((ext_vector_type(8)));
+    const f32x8 *const h = (const f32x8 *)((const float *)p.h + (int64_t)pair0 * I);
+    const int units = top_k * IB, pieces = units * 16;
+    f32x8 first[HELD];
 #pragma unroll
-    for (int s = 0; s < STEPS; s++) load(wave + s * 8, unit[s]);
+    for (int i = 0; i < HELD; i++) {
+        const int at = threadIdx.x + i * THREADS;
+        first[i] = at < pieces ? h[at] : f32x8{};
+    }
+    __builtin_amdgcn_sched_barrier(0);
+
+    const uint64_t valid = __ballot(expert >= 0);
+    // unit u: block u % IB of pair u / IB; a wave's are wave, wave + WAVES, ..
+    float held;                                              // what the sums of units i .. i + 63 count, but for h's scale
+    auto hold = [&](int i) __attribute__((always_inline)) {
+        const int u = wave + (i + lane) * WAVES, j = u < units ? u / IB : 0, kb = u < units ? u - j * IB : 0;
+        const int e = __shfl(expert, j);
+        const float by = __shfl(route, j);
+        held = u < units && e >= 0 ? p.down_scale[((int64_t)e * HB + n0 / FP8_BLOCK) * IB + kb] * by : 0.0f;
+    };
+    hold(0);
+    auto load = [&](int u, Codes &w) __attribute__((always_inline)) {
+        const int j = u / IB, kb = u - j * IB;
+        if (u < units && (valid >> j & 1))                   // (the same for the whole wave)
+            w = load_chunks(p.down + ((int64_t)__builtin_amdgcn_readlane(expert, j) * p.H + n0 + r) * I, kb, g, I);
+    };
+    Codes wc[STEPS] = {};
+#pragma unroll
+    for (int s = 0; s < STEPS; s++) load(wave + s * WAVES, wc[s]);
+    __builtin_amdgcn_sched_barrier(0);
+
+    float *const hs = (float *)(lds + pieces * 8);
+    auto put = [&](int at, const f32x8 &v) __attribute__((always_inline)) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) m = max_u32(m, magnitude(v[i]));
+        const float s = block_scale(max_of_16(m)), inv = __builtin_amdgcn_rcpf(s);
+        *(u32x2 *)(lds + at * 8) = u32x2{encode4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv), encode4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv)};
+        if ((at & 15) == 0) hs[at >> 4] = s;
+    };
+#pragma unroll
+    for (int i = 0; i < HELD; i++)
+        if ((int)threadIdx.x + i * THREADS < pieces) put(threadIdx.x + i * THREADS, first[i]);
+    for (int at = threadIdx.x + HELD * THREADS; at < pieces; at += THREADS) put(at, h[at]);
+    __syncthreads();
+
     f32x4 acc = {};
-    for (int u0 = wave; u0 < units; u0 += 8 * STEPS) {
+    for (int i0 = 0; wave + i0 * WAVES < units; i0 += STEPS) {
+        if ((i0 & 63) == 0 && i0 != 0) hold(i0);
 #pragma unroll
         for (int s = 0; s < STEPS; s++) {
-            const f32x4 d = block_dot<false>(unit[s].w, unit[s].x);
+            const int u = wave + (i0 + s) * WAVES, in = u < units ? u : units - 1;
+            const uint8_t *const xr = lds + in * FP8_BLOCK + g * 16;
+            const f32x4 d = block_dot<false>(wc[s], Codes{*(const u32x4 *)xr, *(const u32x4 *)(xr + 64)});
+            const float sc = hs[in] * lane_value(held, (i0 + s) & 63);
+            const bool counts = u < units && (valid >> (in / IB) & 1);
 #pragma unroll
-            for (int j = 0; j < 4; j++) acc[j] = fmaf(unit[s].scale, d[j], acc[j]);
-            load(u0 + (s + STEPS) * 8, unit[s]);
+            for (int j = 0; j < 4; j++) acc[j] = counts ? fmaf(sc, d[j], acc[j]) : acc[j];
+            load(u + STEPS * WAVES, wc[s]);
         }
     }
     if (r == 0) *(f32x4 *)&sums[wave][g * 4] = acc;
@@ -190,7 +208,7 @@ __global__ __launch_bounds__(512) void block_fp8_expert_down_token_kernel(const 
     if (threadIdx.x >= 16) return;
     float v = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 8; w++) v += sums[w][threadIdx.x];
+    for (int w = 0; w < WAVES; w++) v += sums[w][threadIdx.x];
     out[(int64_t)token * p.H + n0 + threadIdx.x] = to_at<AT>(v);
 }
 
@@ -236,9 +254,12 @@ __global__ __launch_bounds__(256) void block_fp8_expert_rows_kernel(const AT *__
     if (valid) order[before] = b;
 }
 
-// While there are no more pairs than experts few of them share one, and each streams its weights; the row of x fits LDS.
-static bool direct(int tokens, int top_k, int n_exp, int H) {
-    return ((int64_t)tokens * top_k <= n_exp || tokens == 1) && fp8_blocks(H) * (FP8_BLOCK + 4) <= 65536 - 4096;
+// While there are no more pairs than experts few of them share one, and each streams its weights; the codes of a row of x and those of a
+// token's rows of h fit LDS.
+static size_t token_up_lds(int H) { return (size_t)fp8_blocks(H) * (FP8_BLOCK + 4); }
+static size_t token_down_lds(int top_k, int I) { return (size_t)top_k * (I / FP8_BLOCK) * (FP8_BLOCK + 4); }
+static bool direct(int tokens, int top_k, int n_exp, int H, int I) {
+    return ((int64_t)tokens * top_k <= n_exp || tokens == 1) && token_up_lds(H) <= 65536 - 4096 && token_down_lds(top_k, I) <= 65536 - 4096;
 }
 
 // The forms of the two products.
@@ -268,7 +289,7 @@ static int down_form(int pairs, int n_exp, int H, int I) {
 void block_fp8_experts_plan(int tokens, int top_k, int n_exp, int H, int I, int *plan4) {
     const int pairs = tokens * top_k;
     plan4[0] = plan4[1] = plan4[2] = plan4[3] = 0;
-    if (direct(tokens, top_k, n_exp, H)) return;
+    if (direct(tokens, top_k, n_exp, H, I)) return;
     const TiledForm &down = TILED_FORMS[down_form(pairs, n_exp, H, I)];
     plan4[0] = up_takes_64(pairs, n_exp) ? 64 : 128;
     plan4[1] = down.rows;
@@ -278,7 +299,7 @@ void block_fp8_experts_plan(int tokens, int top_k, int n_exp, int H, int I, int 
 
 struct ExpertsSpace {
     size_t h, hs, x, xs, offsets, order, pos, y, bytes;
-    int ldx, ldxs, ldh;
+    int ldx, ldxs;
 };
 static ExpertsSpace experts_space(int tokens, int top_k, int n_exp, int H, int I) {
     const int64_t pairs = (int64_t)tokens * top_k;
@@ -291,10 +312,10 @@ static ExpertsSpace experts_space(int tokens, int top_k, int n_exp, int H, int I
     };
     w.ldx = fp8_blocks(H) * FP8_BLOCK * 2;
     w.ldxs = tokens;
-    w.ldh = (int)pairs;
-    w.h = take((size_t)pairs * I);
-    w.hs = take((size_t)pairs * (I / FP8_BLOCK) * 4);
-    if (!direct(tokens, top_k, n_exp, H)) {
+    const bool one_each = direct(tokens, top_k, n_exp, H, I);
+    w.h = take((size_t)pairs * I * (one_each ? sizeof(float) : 1));
+    if (!one_each) {
+        w.hs = take((size_t)pairs * (I / FP8_BLOCK) * 4);
         w.x = take((size_t)tokens * w.ldx);
         w.xs = take((size_t)tokens * fp8_blocks(H) * 4);
         w.offsets = take((size_t)(n_exp + 1) * 4);
@@ -309,23 +330,24 @@ size_t block_fp8_experts_workspace_bytes(int tokens, int top_k, int n_exp, int H
     return experts_space(tokens, top_k, n_exp, H, I).bytes;
 }
 
-template <typename AT> static void launch_down_token(const ExpertsArgs &p, const void *weight, int w_dtype, void *out, int tokens, hipStream_t st) {
-    const dim3 grid(p.H / 16, tokens), block(512);
-    if (w_dtype == DT_F32)
-        hipLaunchKernelGGL((block_fp8_expert_down_token_kernel<AT, float>), grid, block, 0, st, p, (const float *)weight, (AT *)out);
-    else if (w_dtype == DT_F16)
-        hipLaunchKernelGGL((block_fp8_expert_down_token_kernel<AT, _Float16>), grid, block, 0, st, p, (const _Float16 *)weight, (AT *)out);
-    else
-        hipLaunchKernelGGL((block_fp8_expert_down_token_kernel<AT, __bf16>), grid, block, 0, st, p, (const __bf16 *)weight, (AT *)out);
+// 16 waves where there are no more workgroups than CUs: two experts of [4096 x 14336] 26 us
+template <typename AT, typename PT> static void launch_down_token(const ExpertsArgs &p, const PT *weight, AT *out, int tokens, hipStream_t st) {
+    const dim3 grid(p.H / 16, tokens);
+    const size_t lds = token_down_lds(p.top_k, p.I);
+    if ((int64_t)grid.x * tokens <= 256)
+        hipLaunchKernelGGL((block_fp8_expert_down_token_kernel<AT, PT, 16>), grid, dim3(1024), lds, st, p, weight, out);
+    else hipLaunchKernelGGL((block_fp8_expert_down_token_kernel<AT, PT, 8>), grid, dim3(512), lds, st, p, weight, out);
 }
 
 template <typename AT> static int launch_experts_t(ExpertsArgs p, const ExpertsSpace &at, uint8_t *ws, const void *weight, int w_dtype, void *out,
                                                    int act_dtype, int tokens, hipStream_t st) {
     const int pairs = tokens * p.top_k;
-    const bool one_each = direct(tokens, p.top_k, p.n_exp, p.H);
+    const bool one_each = direct(tokens, p.top_k, p.n_exp, p.H, p.I);
     if (one_each) {
-        hipLaunchKernelGGL((block_fp8_expert_token_up_kernel<AT>), dim3(p.I / FP8_BLOCK, pairs), dim3(512), (size_t)fp8_blocks(p.H) * (FP8_BLOCK + 4), st, p);
-        launch_down_token<AT>(p, weight, w_dtype, out, tokens, st);
+        hipLaunchKernelGGL((block_fp8_expert_token_up_kernel<AT>), dim3(p.I / 16, pairs), dim3(512), token_up_lds(p.H), st, p);
+        if (w_dtype == DT_F32) launch_down_token(p, (const float *)weight, (AT *)out, tokens, st);
+        else if (w_dtype == DT_F16) launch_down_token(p, (const _Float16 *)weight, (AT *)out, tokens, st);
+        else launch_down_token(p, (const __bf16 *)weight, (AT *)out, tokens, st);
         return 0;
     }
     int32_t *const offsets = (int32_t *)(ws + at.offsets), *const order = (int32_t *)(ws + at.order), *const pos = (int32_t *)(ws + at.pos);
@@ -342,9 +364,9 @@ template <typename AT> static int launch_experts_t(ExpertsArgs p, const ExpertsS
     TiledArgs u = t;
     u.x = ws + at.x; u.xs = (float *)(ws + at.xs); u.ldx = at.ldx; u.ldxs = at.ldxs;
     u.w = p.gate_up; u.ws = p.gate_up_scale; u.N = 2 * p.I; u.K = p.H; u.KB = KB;
-    u.y = p.h; u.hs = p.hs; u.ldhs = p.ldh;
+    u.y = p.h; u.hs = (float *)(ws + at.hs); u.ldhs = pairs;
     TiledArgs d = t;
-    d.x = p.h; d.xs = p.hs; d.ldx = p.I; d.ldxs = p.ldh;
+    d.x = p.h; d.xs = u.hs; d.ldx = p.I; d.ldxs = pairs;
     d.w = p.down; d.ws = p.down_scale; d.N = p.H; d.K = p.I; d.KB = p.I / FP8_BLOCK;
     d.y = ws + at.y;
     const bool small = up_takes_64(pairs, p.n_exp);
@@ -365,9 +387,9 @@ int launch_block_fp8_experts(const void *x, const int64_t *ids, const void *weig
     const ExpertsSpace at = experts_space(tokens, top_k, n_exp, H, I);
     uint8_t *const ws = (uint8_t *)workspace;
     ExpertsArgs p{};
-    p.x = x; p.ids = ids; p.ldh = at.ldh;
+    p.x = x; p.ids = ids;
     p.gate_up = gate_up; p.down = down; p.gate_up_scale = gate_up_scale; p.down_scale = down_scale;
-    p.h = ws + at.h; p.hs = (float *)(ws + at.hs);
+    p.h = ws + at.h;
     p.n_exp = n_exp; p.top_k = top_k; p.H = H; p.I = I; p.act = act;
     return act_dtype == DT_F16 ? launch_experts_t<_Float16>(p, at, ws, weight, w_dtype, out, act_dtype, tokens, st)
                                : launch_experts_t<__bf16>(p, at, ws, weight, w_dtype, out, act_dtype, tokens, st);

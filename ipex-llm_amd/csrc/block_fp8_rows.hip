@@ -77,15 +77,7 @@ __global__ __launch_bounds__(64 * WAVES) void block_fp8_few_rows_kernel(const Ro
     float *const xs = (float *)(lds + (size_t)M * pitch);
     auto put_x = [&](int piece, const V8 &v) __attribute__((always_inline)) {
         const int row = piece / (KB * 16), at = piece - row * KB * 16;
-        uint32_t m = 0;
-#pragma unroll
-        for (int i = 0; i < 8; i++) m = max_u32(m, magnitude((float)v[i]));
-        m = max_of_16(m);
-        const float scale = block_scale(m);
-        const Quotient<AT> q(scale, m);
-        *(u32x2 *)(lds + row * pitch + at * 8) = u32x2{encode4(q((float)v[0]), q((float)v[1]), q((float)v[2]), q((float)v[3])),
-                                                       encode4(q((float)v[4]), q((float)v[5]), q((float)v[6]), q((float)v[7]))};
-        if ((at & 15) == 0) xs[(at >> 4) * 4 + row] = scale;
+        put8<AT>(v, lds + row * pitch + at * 8, xs + (at >> 4) * 4 + row, (at & 15) == 0);
     };
 #pragma unroll
     for (int i = 0; i < HELD; i++) {
@@ -147,9 +139,11 @@ static size_t few_rows_lds(int M, int KB) {
 template <typename AT> static void launch_few_rows(const RowsProduct &p, hipStream_t st) {
     const dim3 grid((p.N + 15) / 16);
     const size_t lds = few_rows_lds(p.M, p.KB);
+    // Short walks, in which half of the loads of 8 waves would be of no block: 4 waves each.  One row on [6144 x 2048] 5.2 us against 7.2.
     // Long walks of few workgroups: 16 waves each.  One row on [4096 x 11008] 13.3 us against 13.9, two on [4096 x 14336] 16.3 / 17.2; but
     // one on [28672 x 8192] 53.3 / 49.9, on [4096 x 4096], where half of their loads would be of no block, 7.9 / 5.6.
-    if (p.KB > 64 && p.N <= 8192) hipLaunchKernelGGL((block_fp8_few_rows_kernel<AT, 16>), grid, dim3(1024), lds, st, p);
+    if (p.KB <= 16) hipLaunchKernelGGL((block_fp8_few_rows_kernel<AT, 4>), grid, dim3(256), lds, st, p);
+    else if (p.KB > 64 && p.N <= 8192) hipLaunchKernelGGL((block_fp8_few_rows_kernel<AT, 16>), grid, dim3(1024), lds, st, p);
     else hipLaunchKernelGGL((block_fp8_few_rows_kernel<AT, 8>), grid, dim3(512), lds, st, p);
 }
 
