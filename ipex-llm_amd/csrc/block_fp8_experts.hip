@@ -12,6 +12,8 @@
 // (block_fp8_gemm.h).
 #include "block_fp8_tiled.h"
 
+#include <math.h>
+
 namespace lowbit {
 
 void launch_moe_route(const int64_t *ids, int pairs, int n_exp, int32_t *offsets, int32_t *order, int32_t *pos, hipStream_t st);
@@ -254,12 +256,19 @@ __global__ __launch_bounds__(256) void block_fp8_expert_rows_kernel(const AT *__
     if (valid) order[before] = b;
 }
 
-// While there are no more pairs than experts few of them share one, and each streams its weights; the codes of a row of x and those of a
-// token's rows of h fit LDS.
+// Few pairs: each streams its expert's weights, which costs as many reads as there are pairs; the codes of a row of x and those of a token's
+// rows of h have to fit LDS.  Sorted by expert a weight is read once, by launches that take some 10 us more and leave a quarter of a round
+// of the first product's tiles idle.  The estimate counts the experts that tokens routed evenly would meet, at 5.5 TB/s.  Pair by pair /
+// sorted, us: 3 tokens through 2 of 8 of [14336 x 4096] 197 / 167, two tokens 134 / 148; 4 through 6 of 64 of [1408 x 2048] 44 / 45, 8 81 / 72;
+// 8 through 8 of 128 of [768 x 2048] 61 / 66, 12 89 / 79; 4 through 8 of 256 of [2048 x 7168] 260 / 251, 16 1028 / 784.
 static size_t token_up_lds(int H) { return (size_t)fp8_blocks(H) * (FP8_BLOCK + 4); }
 static size_t token_down_lds(int top_k, int I) { return (size_t)top_k * (I / FP8_BLOCK) * (FP8_BLOCK + 4); }
 static bool direct(int tokens, int top_k, int n_exp, int H, int I) {
-    return ((int64_t)tokens * top_k <= n_exp || tokens == 1) && token_up_lds(H) <= 65536 - 4096 && token_down_lds(top_k, I) <= 65536 - 4096;
+    if (token_up_lds(H) > 65536 - 4096 || token_down_lds(top_k, I) > 65536 - 4096) return false;
+    if (tokens == 1) return true;
+    if ((int64_t)tokens * top_k > n_exp) return false;
+    const double expert_us = 3.0 * H * I / 5.5e6, met = n_exp * (1.0 - pow(1.0 - (double)top_k / n_exp, tokens));
+    return (tokens * top_k - met) * expert_us <= 10.0 + 64.0 * 2 * FP8_BLOCK * H / 5.5e6;
 }
 
 // The forms of the two products.
