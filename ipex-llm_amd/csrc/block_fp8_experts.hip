@@ -17,8 +17,8 @@
 namespace lowbit {
 
 void launch_moe_route(const int64_t *ids, int pairs, int n_exp, int32_t *offsets, int32_t *order, int32_t *pos, hipStream_t st);
-void launch_moe_combine(const void *y, const int32_t *pos, const void *weight, int w_dtype, void *out, int act_dtype, int tokens, int top_k,
-                        int N, hipStream_t st);
+void launch_moe_combine_f32(const float *y, const int32_t *pos, const void *weight, int w_dtype, void *out, int act_dtype, int tokens, int top_k,
+                            int N, hipStream_t st);
 struct ExpertsArgs {
     const void *x;                                           // [tokens, H]
     const int64_t *ids;
@@ -330,7 +330,7 @@ static ExpertsSpace experts_space(int tokens, int top_k, int n_exp, int H, int I
         w.offsets = take((size_t)(n_exp + 1) * 4);
         w.order = take((size_t)pairs * 4);
         w.pos = take((size_t)pairs * 4);
-        w.y = take((size_t)pairs * H * 2);
+        w.y = take((size_t)pairs * H * sizeof(float));       // (rounded once, when a token's are summed: 16 bits would cost its precision twice)
     }
     w.bytes = at;
     return w;
@@ -385,8 +385,8 @@ template <typename AT> static int launch_experts_t(ExpertsArgs p, const ExpertsS
     if ((int64_t)u.tiles_m * (p.I / FP8_BLOCK) > 0x7fffffff - 8 || (int64_t)d.tiles_m * ((p.H + 127) / 128) > 0x7fffffff - 8) return -3;
     if (small) launch_tiled<AT, true, TILED_UP, true, true, 2, 4, 2, 4, 3, 2>(u, st);
     else launch_tiled<AT, true, TILED_UP, true, true, 4, 4, 2, 4, 2, 2>(u, st);
-    launch_tiled_form<AT, false, TILED_PLAIN, true>(d, form, st);
-    launch_moe_combine(ws + at.y, pos, weight, w_dtype, out, act_dtype, tokens, p.top_k, p.H, st);
+    launch_tiled_form<float, false, TILED_PLAIN, true>(d, form, st);
+    launch_moe_combine_f32((const float *)(ws + at.y), pos, weight, w_dtype, out, act_dtype, tokens, p.top_k, p.H, st);
     return 0;
 }
 

@@ -155,10 +155,10 @@ __global__ __launch_bounds__(256) void moe_sort_gather_kernel(const int64_t *__r
 }
 
 // U pairs of one token: their places and weights on their way together, then their rows; added in order.
-template <int U, typename AT, typename WT>
-__device__ inline void combine_pairs(float (&sum)[8], const AT *__restrict__ y, const int32_t *__restrict__ pos, const WT *__restrict__ weight,
+template <int U, typename YT, typename WT>
+__device__ inline void combine_pairs(float (&sum)[8], const YT *__restrict__ y, const int32_t *__restrict__ pos, const WT *__restrict__ weight,
                                      int N) {
-    using V8 = typename Vec8<AT>::type;
+    typedef YT V8 __attribute__((ext_vector_type(8)));
     int p[U];
     float w[U];
     V8 v[U];
@@ -180,8 +180,8 @@ __device__ inline void combine_pairs(float (&sum)[8], const AT *__restrict__ y, 
 // Eight columns of one token per lane.  Bound by latency (3.8 us in a trace at 472 pairs of 1664 columns, 1.6 MB): a pair's place, its weight and
 // its row one after the other, pair by pair, were three waits per pair; four pairs at a time are two (118 tokens, four of 10 experts
 // of [1024 x 1664] in asym_int4, the whole call 34.9 -> 33.6 us, 32 tokens, two of 13, 30.2 -> 29.0, 512 of [14336 x 4096] 498 -> 496).
-template <typename AT, typename WT>
-__global__ __launch_bounds__(256) void moe_combine_kernel(const AT *__restrict__ y, const int32_t *__restrict__ pos,
+template <typename YT, typename AT, typename WT>
+__global__ __launch_bounds__(256) void moe_combine_kernel(const YT *__restrict__ y, const int32_t *__restrict__ pos,
                                                           const WT *__restrict__ weight, AT *__restrict__ out, int top_k, int N) {
     using V8 = typename Vec8<AT>::type;
     const int t = blockIdx.y, n = (blockIdx.x * 256 + threadIdx.x) * 8;
@@ -201,28 +201,29 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const AT *__restrict__
     *(V8 *)(out + (int64_t)t * N + n) = o;
 }
 
-template <typename AT>
+template <typename YT, typename AT>
 static void launch_combine(const void *y, const int32_t *pos, const void *weight, int w_dtype, void *out, int tokens, int top_k,
                            int N, hipStream_t st) {
     for (; tokens > 65535; tokens -= 65535) {                // (a grid's second dimension ends there)
-        launch_combine<AT>(y, pos, weight, w_dtype, out, 65535, top_k, N, st);
+        launch_combine<YT, AT>(y, pos, weight, w_dtype, out, 65535, top_k, N, st);
         pos += (int64_t)65535 * top_k;
         weight = (const uint8_t *)weight + (int64_t)65535 * top_k * (w_dtype == DT_F32 ? 4 : 2);
         out = (AT *)out + (int64_t)65535 * N;
     }
     const dim3 grid((N / 8 + 255) / 256, tokens);
     if (w_dtype == DT_F32)
-        hipLaunchKernelGGL((moe_combine_kernel<AT, float>), grid, dim3(256), 0, st, (const AT *)y, pos, (const float *)weight, (AT *)out, top_k, N);
+        hipLaunchKernelGGL((moe_combine_kernel<YT, AT, float>), grid, dim3(256), 0, st, (const YT *)y, pos, (const float *)weight, (AT *)out, top_k, N);
     else if (w_dtype == DT_F16)
-        hipLaunchKernelGGL((moe_combine_kernel<AT, _Float16>), grid, dim3(256), 0, st, (const AT *)y, pos, (const _Float16 *)weight, (AT *)out, top_k, N);
+        hipLaunchKernelGGL((moe_combine_kernel<YT, AT, _Float16>), grid, dim3(256), 0, st, (const YT *)y, pos, (const _Float16 *)weight, (AT *)out, top_k, N);
     else
-        hipLaunchKernelGGL((moe_combine_kernel<AT, __bf16>), grid, dim3(256), 0, st, (const AT *)y, pos, (const __bf16 *)weight, (AT *)out, top_k, N);
+        hipLaunchKernelGGL((moe_combine_kernel<YT, AT, __bf16>), grid, dim3(256), 0, st, (const YT *)y, pos, (const __bf16 *)weight, (AT *)out, top_k, N);
 }
 
-void launch_moe_combine(const void *y, const int32_t *pos, const void *weight, int w_dtype, void *out, int act_dtype, int tokens, int top_k,
-                        int N, hipStream_t st) {
-    if (act_dtype == DT_F16) launch_combine<_Float16>(y, pos, weight, w_dtype, out, tokens, top_k, N, st);
-    else launch_combine<__bf16>(y, pos, weight, w_dtype, out, tokens, top_k, N, st);
+// of pairs' results in float32
+void launch_moe_combine_f32(const float *y, const int32_t *pos, const void *weight, int w_dtype, void *out, int act_dtype, int tokens, int top_k,
+                            int N, hipStream_t st) {
+    if (act_dtype == DT_F16) launch_combine<float, _Float16>(y, pos, weight, w_dtype, out, tokens, top_k, N, st);
+    else launch_combine<float, __bf16>(y, pos, weight, w_dtype, out, tokens, top_k, N, st);
 }
 
 void launch_moe_route(const int64_t *ids, int pairs, int n_exp, int32_t *offsets, int32_t *order, int32_t *pos, hipStream_t st) {
@@ -294,7 +295,8 @@ int launch_experts(const void *x, const int64_t *ids, const void *weight, int w_
         return rc;
     if (int rc = launch_grouped_gemm(h, downs, nullptr, y, offsets, n_exp, pairs, qtype, act_dtype, hidden, inter, 0, ws + at.split,
                                      at.bytes - at.split, st)) return rc;
-    launch_moe_combine(y, pos, weight, w_dtype, out, act_dtype, tokens, top_k, hidden, st);
+    if (act_dtype == DT_F16) launch_combine<_Float16, _Float16>(y, pos, weight, w_dtype, out, tokens, top_k, hidden, st);
+    else launch_combine<__bf16, __bf16>(y, pos, weight, w_dtype, out, tokens, top_k, hidden, st);
     return 0;
 }
 

@@ -346,12 +346,12 @@ def check_experts(case, dtype, act=0):
     got = bf.block_fp8_experts(x.cuda(), picks.cuda(), p.cuda(), gu.cuda(), gus.cuda(), dn.cuda(), dns.cuda(), act).cpu().double()
     want, slack, size = experts64(x, picks, p, gu, gus, dn, dns, act)
     unit = torch.finfo(dtype).eps / 2
-    # a pair's result and the sum are rounded to the type; the second product's instruction as in test_product_of_ordinary_numbers
-    limit = unit * want.norm() + unit * size.norm() + 3 ** 0.5 * 2.0 ** -13 * size.norm() + slack.norm() + 2.0 ** -18 * size.norm()
+    # the sum over a token's pairs is rounded to the type; the second product's instruction as in test_product_of_ordinary_numbers
+    limit = unit * want.norm() + 3 ** 0.5 * 2.0 ** -13 * size.norm() + slack.norm() + 2.0 ** -18 * size.norm()
     assert (got - want).norm() <= limit
     # nobody's row is another's: the same per token, with the statistics of a row
     per = (got - want).norm(dim=1) - slack.norm(dim=1)
-    assert (per <= (2 * unit + 4 * 3 ** 0.5 * 2.0 ** -13) * size.norm(dim=1) + 1e-30).all()
+    assert (per <= (unit + 4 * 3 ** 0.5 * 2.0 ** -13) * size.norm(dim=1) + 1e-30).all()
     return got
 
 
@@ -524,8 +524,8 @@ def test_experts_whose_weights_pass_2_to_32_codes():
         p = torch.rand((tokens, 2), generator=g).bfloat16().cuda()
         got = bf.block_fp8_experts(x, picks + n_exp - 2, p, *big)
         want = bf.block_fp8_experts(x, picks, p, *(t.cuda() for t in small[3:]))
-        # (another kernel may run the smaller case: rounded per pair or not)
-        assert (got.double() - want.double()).norm() <= 2.0 ** -7 * want.double().norm() and want.any()
+        # (another kernel may run the smaller case: each rounded once, sums in another order)
+        assert (got.double() - want.double()).norm() <= 2.1 * 2.0 ** -8 * want.double().norm() and want.any()
 
 
 # ---------------------------------------------------------------- streams, graphs, together
