@@ -273,13 +273,33 @@ static bool direct(int tokens, int top_k, int n_exp, int H, int I) {
 
 // The forms of the two products.
 //
-// First: tiles of 64 rows (waves of 32 x 64) up to 64 rows per expert in the mean, of 128 (waves of 64 x 64) beyond; a wave without rows
-// costs little.  Whole blocks, us: 16 rows per expert, 8 of [14336 x 4096], 342 against 362 of 128; 28, 64 of [1408 x 2048], 135 / 146;
-// 50, 8 of [14336 x 4096], 338 / 345; 94, 4 of [4608 x 640], 60 / 55; 128, 8 of [14336 x 4096], 521 / 510; 512 1557 / 1374.
+// First: tiles of 64, 96 or 128 rows (waves of 32, 48 and 64 x 64), one to a CU, by estimated time: of rows that tokens routed evenly would give
+// an expert, m with a deviation of sqrt(m), the tiles are the sum of the chances that there are more than 0, R, 2 R .. rows, and a round of
+// the GPU's CUs takes a step's time as often as K has blocks.  Whole blocks at 64 / 96 / 128 rows, us: 8 experts of [14336 x 4096], 64
+// rows each in the mean 349 / 312 / 333, 96 rows 438 / 434 / 389, 150 551 / 503 / 545, 512 1611 / 1451 / 1392; 64 of [1408 x 2048], 28 rows
+// 138 / 139 / 144, 84 246 / 206 / 220; 4 of [2304 x 640], 94 rows 28 / 31 / 32, 300 43 / 47 / 38.
 //
 // Second: the dense forms by estimated time (tiled_walk_us); of an expert's last tile half is taken to be rows, pairs / rows + experts / 2
 // tiles.  16 rows for each of 8 experts of [4096 x 14336] 323 us in tiles of 32 rows against 358 of 256, 512 rows 1582 / 1328.
-static bool up_takes_64(int pairs, int n_exp) { return pairs <= 64 * n_exp; }
+static int up_rows(int pairs, int n_exp, int I) {
+    static const struct {
+        int rows;
+        float step_us, alone_us;
+    } forms[] = {{64, 1.23f, 1.05f}, {96, 1.6f, 1.3f}, {128, 2.0f, 1.6f}};
+    const double mean = (double)pairs / n_exp;
+    int best = 0;
+    double least = 0.0;
+    for (const auto &f : forms) {
+        double tiles = 1.0;
+        for (int k = 1; (k - 2) * f.rows < mean; k++) tiles += 0.5 * erfc((k * f.rows - mean) / sqrt(2.0 * mean));
+        const double rounds = tiles * n_exp * (I / FP8_BLOCK) / 256.0, us = rounds <= 1.0 ? f.alone_us : rounds * f.step_us;
+        if (!best || us < least) {
+            least = us;
+            best = f.rows;
+        }
+    }
+    return best;
+}
 static int down_form(int pairs, int n_exp, int H, int I) {
     const int64_t extra = (pairs < n_exp ? pairs : n_exp + 1) / 2;
     int best = TILED_32;
@@ -300,7 +320,7 @@ void block_fp8_experts_plan(int tokens, int top_k, int n_exp, int H, int I, int 
     plan4[0] = plan4[1] = plan4[2] = plan4[3] = 0;
     if (direct(tokens, top_k, n_exp, H, I)) return;
     const TiledForm &down = TILED_FORMS[down_form(pairs, n_exp, H, I)];
-    plan4[0] = up_takes_64(pairs, n_exp) ? 64 : 128;
+    plan4[0] = up_rows(pairs, n_exp, I);
     plan4[1] = down.rows;
     plan4[2] = down.cols;
     plan4[3] = pairs > EXPERTS_SORT_PAIRS;
@@ -378,12 +398,12 @@ template <typename AT> static int launch_experts_t(ExpertsArgs p, const ExpertsS
     d.x = p.h; d.xs = u.hs; d.ldx = p.I; d.ldxs = pairs;
     d.w = p.down; d.ws = p.down_scale; d.N = p.H; d.K = p.I; d.KB = p.I / FP8_BLOCK;
     d.y = ws + at.y;
-    const bool small = up_takes_64(pairs, p.n_exp);
-    const int form = down_form(pairs, p.n_exp, p.H, p.I), used = pairs < p.n_exp ? pairs : p.n_exp;
-    u.tiles_m = pairs / (small ? 64 : 128) + used;           // at most
+    const int rows = up_rows(pairs, p.n_exp, p.I), form = down_form(pairs, p.n_exp, p.H, p.I), used = pairs < p.n_exp ? pairs : p.n_exp;
+    u.tiles_m = pairs / rows + used;           // at most
     d.tiles_m = pairs / TILED_FORMS[form].rows + used;
     if ((int64_t)u.tiles_m * (p.I / FP8_BLOCK) > 0x7fffffff - 8 || (int64_t)d.tiles_m * ((p.H + 127) / 128) > 0x7fffffff - 8) return -3;
-    if (small) launch_tiled<AT, true, TILED_UP, true, true, 2, 4, 2, 4, 3, 2>(u, st);
+    if (rows == 64) launch_tiled<AT, true, TILED_UP, true, true, 2, 4, 2, 4, 3, 2>(u, st);
+    else if (rows == 96) launch_tiled<AT, true, TILED_UP, true, true, 3, 4, 2, 4, 2, 2>(u, st);
     else launch_tiled<AT, true, TILED_UP, true, true, 4, 4, 2, 4, 2, 2>(u, st);
     launch_tiled_form<float, false, TILED_PLAIN, true>(d, form, st);
     launch_moe_combine_f32((const float *)(ws + at.y), pos, weight, w_dtype, out, act_dtype, tokens, p.top_k, p.H, st);

@@ -184,7 +184,7 @@ def test_sizes_of_the_gpu_tests_reach_every_kernel():
     assert kinds(ggml.lowbit_block_fp8_plan(bf16, 0, *s) for s in u.SHAPES + u.TILES) == every | few | more
     assert kinds(ggml.lowbit_block_fp8_plan(bf16, 1, *s) for s in u.BACK_SHAPES + u.BACK_TILES) == every
     plans = {ggml.lowbit_block_fp8_experts_plan(*s) for s in u.EXPERTS + u.EXPERT_TILES}
-    assert {p[0] for p in plans} == {0, 64, 128} and {p[3] for p in plans} == {0, 1}
+    assert {p[0] for p in plans} == {0, 64, 96, 128} and {p[3] for p in plans} == {0, 1}
     assert {p[1:3] for p in plans} == {(0, 0), (32, 128), (64, 128), (128, 128), (128, 256), (192, 256), (256, 256)}
 
 
