@@ -273,26 +273,30 @@ static bool direct(int tokens, int top_k, int n_exp, int H, int I) {
 
 // The forms of the two products.
 //
-// First: tiles of 64, 96 or 128 rows (waves of 32, 48 and 64 x 64), one to a CU, by estimated time: of rows that tokens routed evenly would give
-// an expert, m with a deviation of sqrt(m), the tiles are the sum of the chances that there are more than 0, R, 2 R .. rows, and a round of
-// the GPU's CUs takes a step's time as often as K has blocks.  Whole blocks at 64 / 96 / 128 rows, us: 8 experts of [14336 x 4096], 64
-// rows each in the mean 349 / 312 / 333, 96 rows 438 / 434 / 389, 150 551 / 503 / 545, 512 1611 / 1451 / 1392; 64 of [1408 x 2048], 28 rows
-// 138 / 139 / 144, 84 246 / 206 / 220; 4 of [2304 x 640], 94 rows 28 / 31 / 32, 300 43 / 47 / 38.
+// Both by estimated time, with the row tiles that tokens routed evenly would make: of m rows for an expert, with a deviation of sqrt(m), the
+// sum of the chances that there are more than 0, R, 2 R .. of them.
 //
-// Second: the dense forms by estimated time (tiled_walk_us); of an expert's last tile half is taken to be rows, pairs / rows + experts / 2
-// tiles.  16 rows for each of 8 experts of [4096 x 14336] 323 us in tiles of 32 rows against 358 of 256, 512 rows 1582 / 1328.
+// First: tiles of 64, 96 or 128 rows (waves of 32, 48 and 64 x 64), one to a CU.  Whole blocks at 64 / 96 / 128 rows, us: 8 experts of [14336 x
+// 4096], 64 rows each in the mean 349 / 312 / 333, 96 rows 438 / 434 / 389, 150 551 / 503 / 545, 512 1611 / 1451 / 1392; 64 of [1408 x
+// 2048], 28 rows 138 / 139 / 144, 84 246 / 206 / 220; 4 of [2304 x 640], 94 rows 28 / 31 / 32, 300 43 / 47 / 38.
+//
+// Second: the dense forms (tiled_walk_us).  16 rows for each of 8 experts of [4096 x 14336] 323 us in tiles of 32 rows against 358 of 256,
+// 512 rows 1582 / 1328; counting tiles this way and not as pairs / rows + experts / 2 took 80 rows from 342 to 320, 96 from 392 to 368.
+static double expert_tiles(int pairs, int n_exp, int rows) {
+    const double mean = (double)pairs / n_exp;
+    double tiles = 1.0;
+    for (int k = 1; (k - 2) * rows < mean; k++) tiles += 0.5 * erfc((k * rows - mean) / sqrt(2.0 * mean));
+    return tiles * (pairs < n_exp ? pairs : n_exp);
+}
 static int up_rows(int pairs, int n_exp, int I) {
     static const struct {
         int rows;
         float step_us, alone_us;
     } forms[] = {{64, 1.23f, 1.05f}, {96, 1.6f, 1.3f}, {128, 2.0f, 1.6f}};
-    const double mean = (double)pairs / n_exp;
     int best = 0;
     double least = 0.0;
     for (const auto &f : forms) {
-        double tiles = 1.0;
-        for (int k = 1; (k - 2) * f.rows < mean; k++) tiles += 0.5 * erfc((k * f.rows - mean) / sqrt(2.0 * mean));
-        const double rounds = tiles * n_exp * (I / FP8_BLOCK) / 256.0, us = rounds <= 1.0 ? f.alone_us : rounds * f.step_us;
+        const double rounds = expert_tiles(pairs, n_exp, f.rows) * (I / FP8_BLOCK) / 256.0, us = rounds <= 1.0 ? f.alone_us : rounds * f.step_us;
         if (!best || us < least) {
             least = us;
             best = f.rows;
@@ -301,12 +305,11 @@ static int up_rows(int pairs, int n_exp, int I) {
     return best;
 }
 static int down_form(int pairs, int n_exp, int H, int I) {
-    const int64_t extra = (pairs < n_exp ? pairs : n_exp + 1) / 2;
     int best = TILED_32;
     float least = 0.0f;
     for (int form = 0; form < TILED_COUNT; form++) {
         const TiledForm &f = TILED_FORMS[form];
-        const float us = tiled_walk_us(f.step_us, f.alone_us, f.per_cu, (pairs / f.rows + extra) * ((H + f.cols - 1) / f.cols), I / FP8_BLOCK);
+        const float us = tiled_walk_us(f.step_us, f.alone_us, f.per_cu, (int64_t)(expert_tiles(pairs, n_exp, f.rows) * ((H + f.cols - 1) / f.cols) + 0.5), I / FP8_BLOCK);
         if (form == 0 || us < least) {
             least = us;
             best = form;
