@@ -284,8 +284,10 @@ static bool direct(int tokens, int top_k, int n_exp, int H, int I) {
 // 512 rows 1582 / 1328; counting tiles this way and not as pairs / rows + experts / 2 took 80 rows from 342 to 320, 96 from 392 to 368.
 static double expert_tiles(int pairs, int n_exp, int rows) {
     const double mean = (double)pairs / n_exp;
-    double tiles = 1.0;
-    for (int k = 1; (k - 2) * rows < mean; k++) tiles += 0.5 * erfc((k * rows - mean) / sqrt(2.0 * mean));
+    const double spread = sqrt(2.0 * mean);
+    const int sure = (int)fmax(0.0, (mean - 4.0 * spread) / rows);
+    double tiles = 1.0 + sure;
+    for (int k = sure + 1; k * (double)rows < mean + 4.0 * spread; k++) tiles += 0.5 * erfc((k * (double)rows - mean) / spread);
     return tiles * (pairs < n_exp ? pairs : n_exp);
 }
 static int up_rows(int pairs, int n_exp, int I) {
