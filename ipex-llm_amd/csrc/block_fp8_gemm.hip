@@ -17,8 +17,8 @@ __global__ __launch_bounds__(256) void block_fp8_reduce_kernel(const f32x4 *__re
     out4 o;
 #pragma unroll
     for (int j = 0; j < 4; j++) o[j] = Stored<OT>::of(v[j] + (bias && n + j < N ? (float)bias[n + j] : 0.0f));
-    if (N % 4 == 0) {
-        *(out4 *)to = o;
+    if (n + 4 <= N) {
+        __builtin_memcpy(to, &o, sizeof(o));                 // (rows may start at odd places)
         return;
     }
 #pragma unroll
