@@ -13,12 +13,12 @@ struct TiledForm {
 };
 enum { TILED_256, TILED_192_256, TILED_128_256, TILED_128, TILED_64, TILED_32, TILED_COUNT };
 static const TiledForm TILED_FORMS[TILED_COUNT] = {
-    {256, 256, 1, 1.89f, 1.48f, 0.0f, 0.0f},
-    {192, 256, 1, 1.44f, 1.19f, 0.0f, 0.0f},
-    {128, 256, 1, 1.24f, 0.85f, 2.07f, 1.59f},
-    {128, 128, 2, 1.01f, 0.60f, 0.0f, 0.0f},
-    {64, 128, 2, 0.72f, 0.40f, 1.07f, 0.77f},
-    {32, 128, 2, 0.59f, 0.31f, 0.73f, 0.53f},
+    {256, 256, 1, 1.76f, 1.41f, 0.0f, 0.0f},
+    {192, 256, 1, 1.37f, 1.15f, 0.0f, 0.0f},
+    {128, 256, 1, 1.04f, 0.87f, 1.68f, 1.52f},
+    {128, 128, 2, 1.02f, 0.58f, 0.0f, 0.0f},
+    {64, 128, 2, 0.58f, 0.36f, 1.02f, 0.67f},
+    {32, 128, 2, 0.57f, 0.30f, 0.75f, 0.44f},
 };
 
 struct TiledPlan {

@@ -10,7 +10,7 @@ SHAPES = [(1, 16, 16), (1, 1, 128), (1, 40, 128), (2, 130, 272), (3, 4096, 512),
           (257, 272, 1536), (520, 640, 2048), (1030, 528, 384)]
 TILES = [(935, 1070, 144), (1075, 23, 2032), (1347, 1459, 128), (1398, 1532, 144), (2699, 21, 3088), (2250, 1806, 128), (2694, 141, 6704),
          (3466, 3630, 144), (4170, 910, 6672), (1378, 1462, 144), (2722, 19, 1968), (2606, 1590, 144), (2884, 130, 6560),
-         (3255, 2439, 144), (5480, 267, 6928), (4172, 941, 7232)]
+         (3255, 2439, 144), (5480, 267, 6928), (4172, 941, 7232), (4179, 139, 7424)]
 BACK_SHAPES = [(1, 16, 16), (1, 130, 128), (5, 128, 272), (17, 300, 400), (64, 257, 640), (77, 1200, 1024), (130, 33, 2112), (200, 1000, 144),
                (300, 512, 512), (520, 264, 1040)]
 BACK_TILES = [(130, 17, 7824), (33, 710, 3376), (558, 18, 7200), (135, 3885, 7312)]
