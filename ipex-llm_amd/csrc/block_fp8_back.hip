@@ -8,6 +8,9 @@
 // LDS 64 values at a time, as codes of x do in the forward (block_fp8_gemm.h has the layout, the order of loads and the barrier ahead
 // of the last tile, which are the same here).  A step is 64 values of n; two steps, a block, are summed from zero by the MFMA and
 // then added to the float32 sums times the block's scale, while the next block's first products run.
+//
+// Bound by the issue of MFMAs between barriers: 8192^3 975 to 1020 us, 1.1 PFLOP/s, where the library's dense product takes 850; 2048 x 4096
+// (N) x 11008 in 187, of which a tenth is the third round of 688 tiles.  Three buffers or five make no difference.
 #include "block_fp8_tiled.h"
 
 namespace lowbit {
