@@ -356,9 +356,9 @@ int lowbit_block_fp8_linear(const void *x, const void *w, const float *w_scale, 
 size_t lowbit_block_fp8_backward_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K);
 int lowbit_block_fp8_backward(const void *grad, const void *w, const float *w_scale, void *grad_x, int dtype, int64_t M, int64_t N, int64_t K,
                               void *workspace, size_t workspace_bytes, void *stream);
-/* What these two run as, for a size: plan3 = {rows, columns of a tile (0, 0: the kernel of few rows, that takes x as it is), parts that the
- * sum is split into}.  `backward`: lowbit_block_fp8_backward. */
-int lowbit_block_fp8_plan(int dtype, int backward, int64_t M, int64_t N, int64_t K, int *plan3);
+/* What these two run as, for a size: plan4 = {rows, columns of a tile (0, 0: the kernel of few rows, that takes x as it is), parts that the
+ * sum is split into, groups of waves that share a tile's part}.  `backward`: lowbit_block_fp8_backward. */
+int lowbit_block_fp8_plan(int dtype, int backward, int64_t M, int64_t N, int64_t K, int *plan4);
 /* A mixture-of-experts block: y[t, :] = sum_j topk_weight[t, j] * (Q(act(g) .* u) * down[e]^T), (g | u) = Q(x_t) * gate_up[e]^T, e =
  * topk_ids[t, j]; a pair whose id lies outside [0, n_experts) counts nothing.  gate_up [n_experts, 2 inter, hidden] (gate rows first)
  * and down [n_experts, hidden, inter] are the experts' codes one after the other, their scales likewise; inter is a multiple of 128,

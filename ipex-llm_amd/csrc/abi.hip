@@ -60,8 +60,8 @@ int launch_block_fp8_rows(const void *x, int dtype, int64_t rows, int K, uint8_t
                           int64_t block_step, hipStream_t st);
 int launch_block_fp8_weight(const void *w, int dtype, int64_t matrices, int N, int K, uint8_t *codes, float *scale, hipStream_t st);
 size_t block_fp8_linear_workspace_bytes(int dtype, int M, int N, int K);
-void block_fp8_linear_plan(int dtype, int M, int N, int K, int *plan3);
-void block_fp8_back_plan(int M, int N, int K, int *plan3);
+void block_fp8_linear_plan(int dtype, int M, int N, int K, int *plan4);
+void block_fp8_back_plan(int M, int N, int K, int *plan4);
 void block_fp8_experts_plan(int tokens, int top_k, int n_exp, int H, int I, int *plan4);
 int launch_block_fp8_linear(const void *x, const uint8_t *w, const float *ws, const void *bias, void *y, int dtype, int M, int N, int K,
                             uint8_t *space, hipStream_t st);
@@ -793,12 +793,12 @@ int lowbit_block_fp8_linear(const void *x, const void *w, const float *w_scale, 
                                                 (hipStream_t)stream), what);
 }
 
-int lowbit_block_fp8_plan(int dtype, int backward, int64_t M, int64_t N, int64_t K, int *plan3) {
+int lowbit_block_fp8_plan(int dtype, int backward, int64_t M, int64_t N, int64_t K, int *plan4) {
     const char *what = "lowbit_block_fp8_plan";
     if (int rc = check_block_fp8(what, dtype, !backward, M, N, K)) return rc;
-    if (M == 0 || N == 0 || K == 0 || !plan3) return fail(LOWBIT_EARG, "%s: sizes must be positive, plan3 not null", what);
-    if (backward) block_fp8_back_plan((int)M, (int)N, (int)K, plan3);
-    else block_fp8_linear_plan(dtype, (int)M, (int)N, (int)K, plan3);
+    if (M == 0 || N == 0 || K == 0 || !plan4) return fail(LOWBIT_EARG, "%s: sizes must be positive, plan4 not null", what);
+    if (backward) block_fp8_back_plan((int)M, (int)N, (int)K, plan4);
+    else block_fp8_linear_plan(dtype, (int)M, (int)N, (int)K, plan4);
     return 0;
 }
 

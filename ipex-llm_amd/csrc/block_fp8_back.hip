@@ -271,11 +271,12 @@ static BackPlan back_plan(int M, int N, int K) {
     return best;
 }
 
-void block_fp8_back_plan(int M, int N, int K, int *plan3) {
+void block_fp8_back_plan(int M, int N, int K, int *plan4) {
     const BackPlan plan = back_plan(M, N, K);
-    plan3[0] = BACK_FORMS[plan.form].rows;
-    plan3[1] = BACK_FORMS[plan.form].cols;
-    plan3[2] = plan.splits;
+    plan4[0] = BACK_FORMS[plan.form].rows;
+    plan4[1] = BACK_FORMS[plan.form].cols;
+    plan4[2] = plan.splits;
+    plan4[3] = 1;
 }
 
 static bool padded(int N) { return N % 8 != 0; }

@@ -311,6 +311,7 @@ static int down_form(int pairs, int n_exp, int H, int I) {
     float least = 0.0f;
     for (int form = 0; form < TILED_COUNT; form++) {
         const TiledForm &f = TILED_FORMS[form];
+        if (f.groups > 1) continue;                          // (an expert's last tile, of few rows, would hold a CU for twice as many waves)
         const float us = tiled_walk_us(f.step_us, f.alone_us, f.per_cu, (int64_t)(expert_tiles(pairs, n_exp, f.rows) * ((H + f.cols - 1) / f.cols) + 0.5), I / FP8_BLOCK);
         if (form == 0 || us < least) {
             least = us;

@@ -11,7 +11,8 @@
 //
 // Bound by the matrix pipes and the clock that the power limit leaves them (1.6 GHz at the largest sizes): 8192^3 448 us, 2.45 PFLOP/s, where
 // the library's product with a single scale takes 386; [28672 x 8192] by 8192 rows 1550 us, MFMAs on 66 % of the cycles, no LDS conflict.
-// A few hundred rows are bound by the latency of a step: 333 x 3211 x 2112 in float32 17 us.
+// A few hundred rows are bound by the latency of a step: two groups of waves that take half of a tile's blocks each, 333 x 3211 x 2112 in
+// float32 15 us against 17, 300 x 4096 x 4096 14.2 / 17.6, 40 x 11008 x 4096 11.7 against 13.3 in two splits and their sum.
 //
 // EXACT, for sums that keep float32's 24 bits (block_fp8.h): the bfloat16 MFMA, four instructions of 32 values in place of one.  x comes as
 // bfloat16 numbers, rows of 256 bytes a block, and only the weight's codes are widened on the way from LDS, part by part.
@@ -85,9 +86,10 @@ template <> struct Stored<__bf16> {
     static __device__ __bf16 of(float v) { return (__bf16)v; }
 };
 
-// BY_EXPERT: row tiles of one expert each.  GATHER: x rows by order[].  S: buffers in LDS.
-template <typename OT, bool EXACT, TiledMode MODE, bool BY_EXPERT, bool GATHER, int TM, int TN, int WM, int WN, int S, int MIN_WAVES>
-__global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void block_fp8_tiled_kernel(const TiledArgs p) {
+// BY_EXPERT: row tiles of one expert each.  GATHER: x rows by order[].  S: buffers in LDS.  KG: groups of WM x WN waves, each with buffers of
+// its own, that share a tile's blocks out among them and add their sums at the end.
+template <typename OT, bool EXACT, TiledMode MODE, bool BY_EXPERT, bool GATHER, int TM, int TN, int WM, int WN, int S, int MIN_WAVES, int KG = 1>
+__global__ __launch_bounds__(64 * WM * WN * KG, MIN_WAVES) void block_fp8_tiled_kernel(const TiledArgs p) {
     constexpr int WAVES = WM * WN, BM = WM * TM * 16, BN = WN * TN * 16;
     constexpr int XB = EXACT ? 256 : 128, XR = 1024 / XB, XP = BM / XR, WP = BN / 8;   // bytes of a row of x, rows of a piece, pieces
     constexpr int PX = XP / WAVES, PW = WP / WAVES;
@@ -95,12 +97,15 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void block_fp8_tiled_kerne
     constexpr int TH = TN / 2;                               // UP: a wave's tiles of the gate, and as many of u
     // Two buffers: a step in two halves, each with a barrier (see the loop)
     constexpr int HALVES = S == 2 ? 2 : 1, PH = PW / HALVES;
+    static_assert(KG == 1 || (KG == 2 && MODE != TILED_UP && !BY_EXPERT && (int)(S * (BM * XB + BN * FP8_BLOCK)) >= TM * TN * WAVES * 1024), "room for a group's sums");
     static_assert(WP % (WAVES * HALVES) == 0 && XP % WAVES == 0 && PX > 0 && BM / WAVES <= 64 && TN % 2 == 0 && (S > 2 || TN % 4 == 0 || TN == 2) &&
                   (!UP || BN == 256), "whole pieces per wave");
     constexpr uint32_t BUFFER = BM * XB + BN * FP8_BLOCK, SCALES = BM * 4;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[S * (BUFFER + SCALES)];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
-    const int wm = wave / WN, wn = wave % WN;
+    constexpr uint32_t OWN = S * (BUFFER + SCALES);          // a group's
+    __shared__ __attribute__((aligned(16))) uint8_t shared[KG * OWN];
+    const int lane = threadIdx.x & 63, in_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+    const int group = KG == 1 ? 0 : in_all / WAVES, wave = in_all - group * WAVES, wm = wave / WN, wn = wave % WN;
+    uint8_t *const lds = shared + group * OWN;
 
     // Workgroups go to the XCDs in turn: each takes a run of the tiles, eight row tiles by as many columns as its CUs hold, so that
     // its L2 serves every operand several times.  By expert: all row tiles of a column side by side, those that there are (the launch
@@ -125,7 +130,9 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void block_fp8_tiled_kerne
         end = __builtin_amdgcn_readfirstlane(t.end);
     }
     const int n0 = tn * (UP ? FP8_BLOCK : BN), KB = p.KB;
-    const int b0 = split * p.split_blocks, b1 = MODE == TILED_PART && b0 + p.split_blocks < KB ? b0 + p.split_blocks : KB;
+    // blocks of K: of this split, and of this group (an odd one out is the first group's; the other walks as far, and adds nothing for it)
+    const int from = split * p.split_blocks, to = MODE == TILED_PART && from + p.split_blocks < KB ? from + p.split_blocks : KB;
+    const int walk = (to - from + KG - 1) / KG, b0 = KG == 1 || group == 0 ? from : from + walk, stop = b0 + walk, b1 = stop < to ? stop : to;
 
     // ---- sources of this wave's pieces of 8 rows
     uint32_t xoff[GATHER ? 1 : PX], woff[PW];
@@ -251,7 +258,7 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void block_fp8_tiled_kerne
         for (int h = 0; h < (UP ? 2 : 1); h++) {
             const float sw = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wheld[h]), (kb - b0) & 63));
 #pragma unroll
-            for (int i = 0; i < TM; i++) s[h][i] = xs[i] * sw;
+            for (int i = 0; i < TM; i++) s[h][i] = KG == 1 || kb < b1 ? xs[i] * sw : 0.0f;
         }
     };
     auto add = [&](int o) __attribute__((always_inline)) {
@@ -309,7 +316,7 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void block_fp8_tiled_kerne
     // A wave whose rows are all past the end loads its share and keeps the barriers: a tile of up to half its rows takes little more than half
     // the time, where an expert's last one would otherwise cost as much as a whole one.
     if (m0 + wm * TM * 16 >= end) {
-        for (int kb = b0; kb < b1; kb++) {
+        for (int kb = b0; kb < stop; kb++) {
             const int late = kb + S - 1 < last ? kb + S - 1 : last, next = kb + S < last ? kb + S : last, behind = which > 0 ? which - 1 : S - 1;
 #pragma unroll
             for (int o = 0; o < COUNT - TM; o++) {
@@ -371,12 +378,22 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void block_fp8_tiled_kerne
         read_xs(then);
 #pragma unroll
         for (int o = COUNT - LAG; o < COUNT; o++) add(o);
-        if (++kb >= b1) break;
+        if (++kb >= stop) break;
         if (((kb - b0) & 63) == 0) hold(kb);
         which = then;
     }
     wait_all_loads();
     __syncthreads();
+    if constexpr (KG == 2) {
+        f32x4 *const sums = (f32x4 *)(shared + OWN) + wave * TN * TM * 64 + lane;
+        if (group == 1)
+#pragma unroll
+            for (int o = 0; o < COUNT; o++) sums[o * 64] = acc[o / TM][o % TM];
+        __syncthreads();
+        if (group == 1) return;
+#pragma unroll
+        for (int o = 0; o < COUNT; o++) acc[o / TM][o % TM] += sums[o * 64];
+    }
 
     // ---- results: lane = row r of tile i, columns 4 g .. 4 g + 3 of tile t's sixteen
     if constexpr (UP) {
@@ -454,7 +471,7 @@ __global__ __launch_bounds__(64 * WM * WN, MIN_WAVES) void block_fp8_tiled_kerne
     }
 }
 
-template <typename OT, bool EXACT, TiledMode MODE, bool BY_EXPERT, bool GATHER, int TM, int TN, int WM, int WN, int S, int MIN_WAVES>
+template <typename OT, bool EXACT, TiledMode MODE, bool BY_EXPERT, bool GATHER, int TM, int TN, int WM, int WN, int S, int MIN_WAVES, int KG = 1>
 void launch_tiled(TiledArgs p, hipStream_t st) {
     constexpr int BM = WM * TM * 16, BN = WN * TN * 16;
     if (!BY_EXPERT) p.tiles_m = (p.M + BM - 1) / BM;
@@ -464,8 +481,8 @@ void launch_tiled(TiledArgs p, hipStream_t st) {
         p.split_blocks = p.KB;
     }
     const uint32_t units = (uint32_t)(p.tiles_m * p.tiles_n * p.splits);
-    hipLaunchKernelGGL((block_fp8_tiled_kernel<OT, EXACT, MODE, BY_EXPERT, GATHER, TM, TN, WM, WN, S, MIN_WAVES>), dim3((units + 7) / 8 * 8),
-                       dim3(64 * WM * WN), 0, st, p);
+    hipLaunchKernelGGL((block_fp8_tiled_kernel<OT, EXACT, MODE, BY_EXPERT, GATHER, TM, TN, WM, WN, S, MIN_WAVES, KG>), dim3((units + 7) / 8 * 8),
+                       dim3(64 * WM * WN * KG), 0, st, p);
 }
 
 }  // namespace lowbit

@@ -169,14 +169,15 @@ size_t block_fp8_linear_workspace_bytes(int dtype, int M, int N, int K) {
     return linear_space(wide, M, N, K, block_fp8_tiled_plan(wide, M, N, K)).bytes;
 }
 
-void block_fp8_linear_plan(int dtype, int M, int N, int K, int *plan3) {
-    plan3[0] = plan3[1] = 0;
-    plan3[2] = 1;
+void block_fp8_linear_plan(int dtype, int M, int N, int K, int *plan4) {
+    plan4[0] = plan4[1] = 0;
+    plan4[2] = plan4[3] = 1;
     if (takes_few_rows(M, K)) return;
     const TiledPlan plan = block_fp8_tiled_plan(dtype == DT_F32, M, N, K);
-    plan3[0] = TILED_FORMS[plan.form].rows;
-    plan3[1] = TILED_FORMS[plan.form].cols;
-    plan3[2] = plan.splits;
+    plan4[0] = TILED_FORMS[plan.form].rows;
+    plan4[1] = TILED_FORMS[plan.form].cols;
+    plan4[2] = plan.splits;
+    plan4[3] = TILED_FORMS[plan.form].groups;
 }
 
 int launch_block_fp8_linear(const void *x, const uint8_t *w, const float *ws, const void *bias, void *y, int dtype, int M, int N, int K,

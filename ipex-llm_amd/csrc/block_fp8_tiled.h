@@ -4,21 +4,23 @@
 
 namespace lowbit {
 
-// rows and weight rows of a tile, workgroups that a CU holds, and a step's time (us): with the GPU full, with one workgroup on a CU; the
-// same with float32 results, whose codes go through the bfloat16 MFMA (0: no such form; waves of 64 x 64 on a tile of 128 x 128 take 2.8 us
-// there, and no size would choose them)
+// rows and weight rows of a tile, workgroups that a CU holds, groups of waves that share its blocks, and a step's time (us): with the GPU
+// full, with one workgroup on a CU; the same with float32 results, whose codes go through the bfloat16 MFMA (0: no such form; waves of 64 x
+// 64 on a tile of 128 x 128 take 2.8 us there, and no size would choose them)
 struct TiledForm {
-    int rows, cols, per_cu;
+    int rows, cols, per_cu, groups;
     float step_us, alone_us, exact_us, exact_alone_us;
 };
-enum { TILED_256, TILED_192_256, TILED_128_256, TILED_128, TILED_64, TILED_32, TILED_COUNT };
+enum { TILED_256, TILED_192_256, TILED_128_256, TILED_128, TILED_64, TILED_32, TILED_64_SHARED, TILED_64_64_SHARED, TILED_COUNT };
 static const TiledForm TILED_FORMS[TILED_COUNT] = {
-    {256, 256, 1, 1.76f, 1.41f, 0.0f, 0.0f},
-    {192, 256, 1, 1.37f, 1.15f, 0.0f, 0.0f},
-    {128, 256, 1, 1.04f, 0.87f, 1.68f, 1.52f},
-    {128, 128, 2, 1.02f, 0.58f, 0.0f, 0.0f},
-    {64, 128, 2, 0.58f, 0.36f, 1.02f, 0.67f},
-    {32, 128, 2, 0.57f, 0.30f, 0.75f, 0.44f},
+    {256, 256, 1, 1, 1.72f, 1.42f, 0.0f, 0.0f},
+    {192, 256, 1, 1, 1.39f, 1.04f, 0.0f, 0.0f},
+    {128, 256, 1, 1, 1.04f, 0.81f, 1.78f, 1.48f},
+    {128, 128, 2, 1, 1.00f, 0.56f, 0.0f, 0.0f},
+    {64, 128, 2, 1, 0.55f, 0.33f, 1.03f, 0.65f},
+    {32, 128, 2, 1, 0.55f, 0.30f, 0.80f, 0.44f},
+    {64, 128, 1, 2, 0.92f, 0.57f, 1.55f, 1.01f},
+    {64, 64, 1, 2, 0.77f, 0.39f, 0.74f, 0.65f},
 };
 
 struct TiledPlan {
@@ -26,7 +28,7 @@ struct TiledPlan {
     float us;
 };
 
-// One launch per form; the wave tiles are 64 x 128, 96 x 64, 64 x 64, 64 x 64, 32 x 64 and 32 x 32.
+// One launch per form; the wave tiles are 64 x 128, 96 x 64, 64 x 64, 64 x 64, 32 x 64, 32 x 32, 32 x 64 and 32 x 32.
 template <typename OT, bool EXACT, TiledMode MODE, bool BY_EXPERT = false> void launch_tiled_form(const TiledArgs &p, int form, hipStream_t st) {
     if (form == TILED_256) {
         // (the operands of a 64 x 128 wave tile in bfloat16 do not fit its registers: no plan asks for it)
@@ -38,7 +40,11 @@ template <typename OT, bool EXACT, TiledMode MODE, bool BY_EXPERT = false> void 
     else if (form == TILED_128) {
         if constexpr (!EXACT) launch_tiled<OT, EXACT, MODE, BY_EXPERT, false, 4, 4, 2, 2, 2, 2>(p, st);
     } else if (form == TILED_64) launch_tiled<OT, EXACT, MODE, BY_EXPERT, false, 2, 4, 2, 2, EXACT ? 2 : 3, 2>(p, st);
-    else launch_tiled<OT, EXACT, MODE, BY_EXPERT, false, 2, 2, 1, 4, 3, 2>(p, st);
+    else if (form == TILED_32) launch_tiled<OT, EXACT, MODE, BY_EXPERT, false, 2, 2, 1, 4, 3, 2>(p, st);
+    else if constexpr (!BY_EXPERT) {
+        if (form == TILED_64_SHARED) launch_tiled<OT, EXACT, MODE, BY_EXPERT, false, 2, 4, 2, 2, EXACT ? 2 : 3, 2, 2>(p, st);
+        else launch_tiled<OT, EXACT, MODE, BY_EXPERT, false, 2, 2, 2, 2, 3, 2, 2>(p, st);
+    }
 }
 
 void launch_tiled_f16(const TiledArgs &p, int form, hipStream_t st);

@@ -479,10 +479,11 @@ _lib.lowbit_block_fp8_experts_plan.restype = c_int
 
 
 def lowbit_block_fp8_plan(dtype, backward, m, n, k):
-    """(rows, columns of a tile (0, 0: the kernel of few rows), parts of the sum) of what lowbit_block_fp8_linear or _backward runs."""
-    plan3 = (c_int * 3)()
-    _check(_lib.lowbit_block_fp8_plan(dtype, backward, m, n, k, plan3), "lowbit_block_fp8_plan")
-    return tuple(plan3)
+    """What lowbit_block_fp8_linear or _backward runs: (rows, columns of a tile (0, 0: the kernel of few rows), parts of the sum, groups
+    of waves that share a tile's part)."""
+    plan4 = (c_int * 4)()
+    _check(_lib.lowbit_block_fp8_plan(dtype, backward, m, n, k, plan4), "lowbit_block_fp8_plan")
+    return tuple(plan4)
 
 
 def lowbit_block_fp8_experts_plan(tokens, top_k, n_experts, hidden, inter):

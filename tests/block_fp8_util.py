@@ -8,9 +8,9 @@ E4M3 = torch.float8_e4m3fn
 SHAPES = [(1, 16, 16), (1, 1, 128), (1, 40, 128), (2, 130, 272), (3, 4096, 512), (4, 129, 4096), (5, 64, 2112), (16, 300, 1024), (17, 100, 640),
           (32, 256, 384), (33, 257, 1152), (64, 128, 4096), (65, 136, 1024), (100, 520, 528), (129, 384, 256), (200, 1000, 400),
           (257, 272, 1536), (520, 640, 2048), (1030, 528, 384)]
-TILES = [(935, 1070, 144), (1075, 23, 2032), (1347, 1459, 128), (1398, 1532, 144), (2699, 21, 3088), (2250, 1806, 128), (2694, 141, 6704),
-         (3466, 3630, 144), (4170, 910, 6672), (1378, 1462, 144), (2722, 19, 1968), (2606, 1590, 144), (2884, 130, 6560),
-         (3255, 2439, 144), (5480, 267, 6928), (4172, 941, 7232), (4179, 139, 7424)]
+TILES = [(301, 702, 1040), (935, 1070, 144), (1075, 23, 2032), (644, 1546, 1184), (653, 454, 4672), (1925, 4007, 144), (6017, 275, 7200),
+         (2250, 1806, 128), (1606, 1155, 5280), (3255, 2439, 144), (5480, 267, 6928), (3466, 3630, 144), (1806, 2250, 17984),
+         (1347, 1459, 128), (66, 2005, 7952), (1297, 777, 400), (2884, 130, 6560), (2692, 135, 7840)]
 BACK_SHAPES = [(1, 16, 16), (1, 130, 128), (5, 128, 272), (17, 300, 400), (64, 257, 640), (77, 1200, 1024), (130, 33, 2112), (200, 1000, 144),
                (300, 512, 512), (520, 264, 1040)]
 BACK_TILES = [(130, 17, 7824), (33, 710, 3376), (558, 18, 7200), (135, 3885, 7312)]
@@ -19,7 +19,7 @@ EXPERTS = [(1, 2, 8, 128, 128), (1, 1, 1, 16, 128), (1, 8, 8, 400, 256), (2, 2, 
 EXPERT_TILES = [(39, 2, 70, 784, 128), (148, 1, 70, 800, 128), (56, 3, 70, 1712, 128), (1008, 4, 8, 160, 128), (897, 2, 20, 800, 128),
                 (476, 3, 20, 2112, 128), (3356, 1, 8, 3344, 128), (2079, 2, 70, 128, 256), (2131, 2, 3, 128, 128),
                 (225, 3, 20, 2064, 128), (488, 2, 20, 4016, 128), (399, 4, 20, 128, 896), (300, 2, 4, 640, 2304), (3000, 1, 7, 272, 1152),
-                (286, 2, 8, 2864, 128), (2461, 4, 70, 448, 256), (2314, 4, 70, 144, 256)]
+                (286, 2, 8, 2864, 128), (2461, 4, 70, 448, 256), (3676, 4, 70, 288, 128)]
 
 
 def blocks(n):

@@ -175,13 +175,15 @@ def test_sizes_of_the_gpu_tests_reach_every_kernel():
     f32, bf16 = ggml.DT_F32, ggml.DT_BF16
 
     def kinds(plans):
-        return {(rows, cols, splits > 1) for rows, cols, splits in plans}
+        return {(rows, cols, groups, splits > 1) for rows, cols, splits, groups in plans}
 
-    every = {(rows, cols, split) for rows, cols in [(32, 128), (64, 128), (128, 256)] for split in (False, True)}
-    few = {(0, 0, False)}
-    more = {(rows, cols, split) for rows, cols in [(128, 128), (192, 256), (256, 256)] for split in (False, True)}
-    assert kinds(ggml.lowbit_block_fp8_plan(f32, 0, *s) for s in u.SHAPES + u.TILES) == every | few
-    assert kinds(ggml.lowbit_block_fp8_plan(bf16, 0, *s) for s in u.SHAPES + u.TILES) == every | few | more
+    def both(*forms):
+        return {(*form, split) for form in forms for split in (False, True)}
+
+    every, few = both((32, 128, 1), (64, 128, 1), (128, 256, 1)), {(0, 0, 1, False)}
+    shared = both((64, 64, 2), (64, 128, 2))
+    assert kinds(ggml.lowbit_block_fp8_plan(f32, 0, *s) for s in u.SHAPES + u.TILES) == every | few | shared
+    assert kinds(ggml.lowbit_block_fp8_plan(bf16, 0, *s) for s in u.SHAPES + u.TILES) == every | few | shared | both((128, 128, 1), (192, 256, 1), (256, 256, 1))
     assert kinds(ggml.lowbit_block_fp8_plan(bf16, 1, *s) for s in u.BACK_SHAPES + u.BACK_TILES) == every
     plans = {ggml.lowbit_block_fp8_experts_plan(*s) for s in u.EXPERTS + u.EXPERT_TILES}
     assert {p[0] for p in plans} == {0, 64, 96, 128} and {p[3] for p in plans} == {0, 1}
@@ -194,13 +196,13 @@ def test_plans_hold_for_any_size():
         for n in (1, 7, 128, 4097, 28672, (1 << 23) - 1):
             for k in (16, 128, 144, 4096, 16384, (1 << 23) - 16):
                 for dtype in (ggml.DT_F16, ggml.DT_F32):
-                    rows, cols, splits = ggml.lowbit_block_fp8_plan(dtype, 0, m, n, k)
+                    rows, cols, splits, _ = ggml.lowbit_block_fp8_plan(dtype, 0, m, n, k)
                     assert (rows == 0) == (cols == 0) and 1 <= splits <= 8 and splits <= u.blocks(k)
                     parts = -(-u.blocks(k) // splits)
                     assert parts * (splits - 1) < u.blocks(k)
                     bound = m * u.blocks(k) * (128 * (2 if dtype == ggml.DT_F32 else 1) + 4) + (256 << 20) + 1024
                     assert ggml.lowbit_block_fp8_linear_workspace_bytes(dtype, m, n, k) <= bound
-                rows, cols, splits = ggml.lowbit_block_fp8_plan(ggml.DT_BF16, 1, m, n, k)
+                rows, cols, splits, _ = ggml.lowbit_block_fp8_plan(ggml.DT_BF16, 1, m, n, k)
                 assert rows and cols and -(-u.blocks(n) // splits) * (splits - 1) < u.blocks(n)
                 assert ggml.lowbit_block_fp8_backward_workspace_bytes(ggml.DT_BF16, m, n, k) <= m * (n + 64) * 2 + (256 << 20) + 1024
     for call in (lambda: ggml.lowbit_block_fp8_plan(ggml.DT_F32, 1, 1, 16, 16), lambda: ggml.lowbit_block_fp8_plan(ggml.DT_F16, 0, 0, 16, 16),
