@@ -1,6 +1,7 @@
 """Block-scaled fp8: quantizers, products, gradients and experts against 64 bits on the host."""
 import copy
 import math
+from concurrent.futures import ThreadPoolExecutor
 
 import pytest
 import torch
@@ -544,6 +545,32 @@ def test_another_stream_and_many_at_once():
     torch.cuda.synchronize()
     for i, y in got:
         assert torch.equal(y, want[(i + i // 3) % 3])
+
+
+def test_threads_with_streams_of_their_own():
+    g = gen(17)
+    w, ws = (t.cuda() for t in u.weight(g, 512, 1024, base=-8))
+    cases = []
+    for m in (2, 24, 70, 300):
+        x = u.activations(g, m, 1024, torch.bfloat16).cuda()
+        ex = [t.cuda() for t in expert_case(m, m, 2, 4, 256, 128, torch.bfloat16)]
+        grad = torch.randint(-8, 9, (m, 512), generator=g).bfloat16().cuda()
+        cases.append((x, ex, grad))
+
+    def all_of(x, ex, grad):
+        leaf = x.clone().requires_grad_()
+        y = bf.block_fp8_linear(leaf, w, ws)
+        return y.detach(), torch.autograd.grad(y, leaf, grad)[0], bf.block_fp8_experts(*ex), bf.block_fp8_quantize(x)[1]
+    want = [all_of(*c) for c in cases]
+    torch.cuda.synchronize()
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got = [all_of(*cases[i]) for _ in range(10)]
+            torch.cuda.current_stream().synchronize()
+        return all(torch.equal(a, b) for one in got for a, b in zip(one, want[i]))
+    with ThreadPoolExecutor(len(cases)) as pool:
+        assert all(pool.map(run, range(len(cases))))
 
 
 @pytest.mark.parametrize("m", [1, 20, 200])
