@@ -37,14 +37,14 @@ float tiled_walk_us(float step_us, float alone_us, int per_cu, int64_t units, in
 }
 
 // Estimated time in us: the walks, and what a launch, its first loads and its stores take; with splits the sums, written and read in
-// float32.  The constants are fitted to timed launches of 715 sizes (float32: 564), 5 to 8192 rows by 256 to 28672 by 512 to 16384; on
-// as many others the pick is 0.7 % above the fastest of the forms and splits on average, 28 % at worst.
+// float32.  The constants are fitted to timed launches of 705 sizes (float32: 462), weights from memory, 5 to 8192 rows by 256 to 28672 by
+// 512 to 16384; on as many others the pick is 0.9 % above the fastest of the forms and splits on average, 27 % at worst.
 static float tiled_us(int form, int M, int N, int KB, int splits, bool exact) {
     const TiledForm &f = TILED_FORMS[form];
     const int64_t units = (int64_t)cdiv(M, f.rows) * cdiv(N, f.cols) * splits;
-    float us = tiled_walk_us(exact ? f.exact_us : f.step_us, exact ? f.exact_alone_us : f.alone_us, f.per_cu, units, cdiv(cdiv(KB, splits), f.groups)) + (exact ? 4.8f : 5.5f);
-    if (f.groups > 1) us += 0.4f;
-    if (splits > 1) us += (exact ? 2.0f : 1.6f) + (float)splits * M * N * 8.0f / (exact ? 4.0e6f : 4.6e6f);
+    float us = tiled_walk_us(exact ? f.exact_us : f.step_us, exact ? f.exact_alone_us : f.alone_us, f.per_cu, units, cdiv(cdiv(KB, splits), f.groups)) + (exact ? 4.1f : 4.6f);
+    if (f.groups > 1) us += 0.6f;
+    if (splits > 1) us += 2.0f + (float)splits * M * N * 8.0f / (exact ? 3.8e6f : 4.9e6f);
     return us;
 }
 

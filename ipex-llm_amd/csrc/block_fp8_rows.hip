@@ -1,17 +1,21 @@
-// Up to four rows of activations times a weight with a scale for each block of 128 (block_fp8.h): the weight streams past once, in one
+// Up to sixteen rows of activations times a weight with a scale for each block of 128 (block_fp8.h): the weight streams past once, in one
 // launch.
 //
 // A workgroup owns 16 weight rows; its waves take the blocks of K in turn and their sums meet in LDS.  A wave's loads are 16 rows x 64
 // contiguous bytes, STEPS blocks ahead of their use.  x is quantized by each workgroup, into LDS, while the first weights are on their
 // way.  Loads return in order, so x is asked for ahead of them.  Bound by latency at the sizes of one token: of 5.6 us at one row of [4096 x
-// 4096] an empty launch is 1.6.  More rows go to the tiles of block_fp8_gemm.h, which hide latency better than registers do: 40 rows on
-// [11008 x 4096] 28 us this way, 10.8 in tiles.
+// 4096] an empty launch is 1.6.  More rows go to the tiles of block_fp8_gemm.h,
+// which quantize x once: 40 rows on [11008 x 4096] 28 us this way, 10.8 in tiles.
 #include "block_fp8_tiled.h"
+
+#include <math.h>
 
 namespace lowbit {
 
 int launch_block_fp8_rows(const void *x, int dtype, int64_t rows, int K, uint8_t *codes, int ldc, bool wide, float *scale, int64_t row_step,
                           int64_t block_step, hipStream_t st);
+
+constexpr int FEW_ROWS = 16;                                 // an MFMA's
 
 struct RowsProduct {
     const void *x;                                           // [M, K]
@@ -72,12 +76,12 @@ __global__ __launch_bounds__(64 * WAVES) void block_fp8_few_rows_kernel(const Ro
         load_w(wave + s * WAVES < KB ? wave + s * WAVES : KB - 1, wc[s]);      // (past the last block: it again, not added)
     __builtin_amdgcn_sched_barrier(0);
 
-    // codes of x in LDS, rows of KB * 128 + 16 bytes (16: rows start in other banks), then the scales [KB][4]
+    // codes of x in LDS, rows of KB * 128 + 16 bytes (16: rows start in other banks), then the scales [KB][FEW_ROWS]
     const int pitch = KB * FP8_BLOCK + 16;
     float *const xs = (float *)(lds + (size_t)M * pitch);
     auto put_x = [&](int piece, const V8 &v) __attribute__((always_inline)) {
         const int row = piece / (KB * 16), at = piece - row * KB * 16;
-        put8<AT>(v, lds + row * pitch + at * 8, xs + (at >> 4) * 4 + row, (at & 15) == 0);
+        put8<AT>(v, lds + row * pitch + at * 8, xs + (at >> 4) * FEW_ROWS + row, (at & 15) == 0);
     };
 #pragma unroll
     for (int i = 0; i < HELD; i++) {
@@ -98,7 +102,7 @@ __global__ __launch_bounds__(64 * WAVES) void block_fp8_few_rows_kernel(const Ro
         for (int s = 0; s < STEPS; s++) {
             const int kb = wave + (i0 + s) * WAVES, in = kb < KB ? kb : KB - 1;
             xc[s] = Codes{*(const u32x4 *)(xrow + in * FP8_BLOCK), *(const u32x4 *)(xrow + in * FP8_BLOCK + 64)};
-            sc[s] = xs[in * 4 + row] * __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wheld), i0 + s));
+            sc[s] = xs[in * FEW_ROWS + row] * __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wheld), i0 + s));
         }
         f32x4 d[STEPS];
 #pragma unroll
@@ -119,36 +123,49 @@ __global__ __launch_bounds__(64 * WAVES) void block_fp8_few_rows_kernel(const Ro
     __syncthreads();                                         // (they lie where the codes were)
     float *const sums = (float *)lds;
     if (r < M)
-        *(f32x4 *)(sums + (wave * 4 + r) * 16 + g * 4) = acc;
+        *(f32x4 *)(sums + (wave * FEW_ROWS + r) * 16 + g * 4) = acc;
     __syncthreads();
     if ((int)threadIdx.x >= M * 16) return;
     const int m = threadIdx.x >> 4, c = threadIdx.x & 15;
     if (n0 + c >= N) return;
     float v = 0.0f;
 #pragma unroll
-    for (int w = 0; w < WAVES; w++) v += sums[(w * 4 + m) * 16 + c];
+    for (int w = 0; w < WAVES; w++) v += sums[(w * FEW_ROWS + m) * 16 + c];
     if (p.bias) v += (float)((const AT *)p.bias)[n0 + c];
     ((AT *)p.y)[(int64_t)m * N + n0 + c] = Stored<AT>::of(v);
 }
 
 static size_t few_rows_lds(int M, int KB) {
-    const size_t codes = (size_t)M * (KB * FP8_BLOCK + 16) + (size_t)KB * 4 * sizeof(float);
-    return codes > 4096 ? codes : 4096;                      // (the sums of 16 waves)
+    const size_t codes = (size_t)M * (KB * FP8_BLOCK + 16) + (size_t)KB * FEW_ROWS * sizeof(float);
+    return codes > 16384 ? codes : 16384;                    // (the sums of 16 waves)
 }
+
+// Short walks, in which half of the loads of 8 waves would be of no block: 4 waves each.  One row on [6144 x 2048] 5.2 us against 7.2.
+// Long walks of few workgroups: 16 waves each.  One row on [4096 x 11008] 13.3 us against 13.9, two on [4096 x 14336] 16.3 / 17.2; but
+// one on [28672 x 8192] 53.3 / 49.9, on [4096 x 4096], where half of their loads would be of no block, 7.9 / 5.6.
+static int few_rows_waves(int N, int KB) { return KB <= 16 ? 4 : KB > 64 && N <= 8192 ? 16 : 8; }
 
 template <typename AT> static void launch_few_rows(const RowsProduct &p, hipStream_t st) {
     const dim3 grid((p.N + 15) / 16);
     const size_t lds = few_rows_lds(p.M, p.KB);
-    // Short walks, in which half of the loads of 8 waves would be of no block: 4 waves each.  One row on [6144 x 2048] 5.2 us against 7.2.
-    // Long walks of few workgroups: 16 waves each.  One row on [4096 x 11008] 13.3 us against 13.9, two on [4096 x 14336] 16.3 / 17.2; but
-    // one on [28672 x 8192] 53.3 / 49.9, on [4096 x 4096], where half of their loads would be of no block, 7.9 / 5.6.
-    if (p.KB <= 16) hipLaunchKernelGGL((block_fp8_few_rows_kernel<AT, 4>), grid, dim3(256), lds, st, p);
-    else if (p.KB > 64 && p.N <= 8192) hipLaunchKernelGGL((block_fp8_few_rows_kernel<AT, 16>), grid, dim3(1024), lds, st, p);
+    const int waves = few_rows_waves(p.N, p.KB);
+    if (waves == 4) hipLaunchKernelGGL((block_fp8_few_rows_kernel<AT, 4>), grid, dim3(256), lds, st, p);
+    else if (waves == 16) hipLaunchKernelGGL((block_fp8_few_rows_kernel<AT, 16>), grid, dim3(1024), lds, st, p);
     else hipLaunchKernelGGL((block_fp8_few_rows_kernel<AT, 8>), grid, dim3(512), lds, st, p);
 }
 
-// Up to four rows whose codes fit 64 KiB of LDS; beyond, tiles.
-static bool takes_few_rows(int M, int K) { return M <= 4 && few_rows_lds(M, fp8_blocks(K)) <= 65536 && fp8_blocks(K) <= 512; }
+// Rows whose codes fit 64 KiB of LDS: up to four always, up to sixteen where that is estimated shorter than tiles and the launch ahead of them.
+// What grows with the rows is x, which every workgroup reads and quantizes: 8 rows on [4096 x 4096] 8.3 us against 10.7 in tiles, 16 11.2 /
+// 11.2; 8 on [14336 x 4096] 21.6 / 16.2, on [1536 x 2048] 5.8 / 8.3.  Fitted to 540 sizes of 5 to 16 rows, weights from memory; the pick is 1 %
+// above the shorter way on average, 31 % at worst (tiles for all 19 %).
+static bool takes_few_rows(bool wide, int M, int N, int K) {
+    const int KB = fp8_blocks(K);
+    if (M > FEW_ROWS || KB > 512 || few_rows_lds(M, KB) > 65536) return false;
+    if (M <= 4) return true;
+    const float rounds = N > 4096 ? N / 4096.0f : 1.0f;      // of a workgroup per CU
+    const float bytes = (float)N * K, us = 3.1f + bytes / 5.6e6f + (wide ? 0.072f : 0.038f) * M * rounds * K / (64 * few_rows_waves(N, KB));
+    return us <= fmaxf(block_fp8_tiled_plan(wide, M, N, K).us, bytes / 5.4e6f + 4.0f) + 1.5f;
+}
 
 // codes of x (float32 results: bfloat16 numbers), their scales, a split's sums
 struct LinearSpace {
@@ -164,7 +181,7 @@ static LinearSpace linear_space(bool wide, int M, int N, int K, const TiledPlan 
 }
 
 size_t block_fp8_linear_workspace_bytes(int dtype, int M, int N, int K) {
-    if (takes_few_rows(M, K)) return 0;
+    if (takes_few_rows(dtype == DT_F32, M, N, K)) return 0;
     const bool wide = dtype == DT_F32;
     return linear_space(wide, M, N, K, block_fp8_tiled_plan(wide, M, N, K)).bytes;
 }
@@ -172,7 +189,7 @@ size_t block_fp8_linear_workspace_bytes(int dtype, int M, int N, int K) {
 void block_fp8_linear_plan(int dtype, int M, int N, int K, int *plan4) {
     plan4[0] = plan4[1] = 0;
     plan4[2] = plan4[3] = 1;
-    if (takes_few_rows(M, K)) return;
+    if (takes_few_rows(dtype == DT_F32, M, N, K)) return;
     const TiledPlan plan = block_fp8_tiled_plan(dtype == DT_F32, M, N, K);
     plan4[0] = TILED_FORMS[plan.form].rows;
     plan4[1] = TILED_FORMS[plan.form].cols;
@@ -182,7 +199,7 @@ void block_fp8_linear_plan(int dtype, int M, int N, int K, int *plan4) {
 
 int launch_block_fp8_linear(const void *x, const uint8_t *w, const float *ws, const void *bias, void *y, int dtype, int M, int N, int K,
                             uint8_t *space, hipStream_t st) {
-    if (takes_few_rows(M, K)) {
+    if (takes_few_rows(dtype == DT_F32, M, N, K)) {
         const RowsProduct p = {x, w, ws, bias, y, M, N, K, fp8_blocks(K)};
         if (dtype == DT_F16) launch_few_rows<_Float16>(p, st);
         else if (dtype == DT_BF16) launch_few_rows<__bf16>(p, st);

@@ -5,7 +5,8 @@ E4M3 = torch.float8_e4m3fn
 
 # Sizes of the GPU tests.  The larger ones are there for the kernels that only they reach: odd numbers of rows and columns, K and N that end
 # inside a block, and sums in parts.
-SHAPES = [(1, 16, 16), (1, 1, 128), (1, 40, 128), (2, 130, 272), (3, 4096, 512), (4, 129, 4096), (5, 64, 2112), (16, 300, 1024), (17, 100, 640),
+SHAPES = [(1, 16, 16), (1, 1, 128), (1, 40, 128), (2, 130, 272), (3, 4096, 512), (4, 129, 4096), (5, 64, 2112), (16, 300, 1024), (11, 530, 1040), (7, 4100, 512), (13, 257, 4096), (9, 40, 16),
+          (13, 17, 4832), (17, 100, 640),
           (32, 256, 384), (33, 257, 1152), (64, 128, 4096), (65, 136, 1024), (100, 520, 528), (129, 384, 256), (200, 1000, 400),
           (257, 272, 1536), (520, 640, 2048), (1030, 528, 384)]
 TILES = [(301, 702, 1040), (935, 1070, 144), (1075, 23, 2032), (644, 1546, 1184), (653, 454, 4672), (1925, 4007, 144), (6017, 275, 7200),

@@ -426,7 +426,7 @@ def test_experts_gradients_run_expert_by_expert():
 
 # ---------------------------------------------------------------- what a product must keep apart
 
-@pytest.mark.parametrize("m,n,k", [(1, 33, 144), (3, 130, 272), (40, 257, 400), (300, 129, 144), (1347, 1459, 144)])
+@pytest.mark.parametrize("m,n,k", [(1, 33, 144), (3, 130, 272), (14, 130, 272), (40, 257, 400), (300, 129, 144), (1347, 1459, 144)])
 @pytest.mark.parametrize("dtype", ALL, ids=ids)
 def test_nan_stays_in_its_row_and_column(dtype, m, n, k):
     """NaN in a row of x (a padded batch's), in the weight's last row and in a block's scale: the results that they belong to and no others,
