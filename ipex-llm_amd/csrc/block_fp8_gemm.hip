@@ -36,15 +36,17 @@ float tiled_walk_us(float step_us, float alone_us, int per_cu, int64_t units, in
     return steps * (rounds * step_us + (!rest ? 0.0f : rest <= 256 ? alone_us : step_us));
 }
 
-// Estimated time in us: the walks, and what a launch, its first loads and its stores take; with splits the sums, written and read in
-// float32.  The constants are fitted to timed launches of 705 sizes (float32: 462), weights from memory, 5 to 8192 rows by 256 to 28672 by
-// 512 to 16384; on as many others the pick is 0.9 % above the fastest of the forms and splits on average, 27 % at worst.
+// Estimated time in us: the walks; what a launch, its first loads and its stores take, and again the first loads of each further round; the
+// sums of two groups; with splits the sums written and read in float32.  The constants are fitted to timed launches of 705 sizes (float32:
+// 462), weights from memory, 5 to 8192 rows by 256 to 28672 by 512 to 16384; on as many others the pick is 0.9 % (0.6 %) above the
+// fastest of the forms and splits on average, 24 % at worst.
 static float tiled_us(int form, int M, int N, int KB, int splits, bool exact) {
     const TiledForm &f = TILED_FORMS[form];
-    const int64_t units = (int64_t)cdiv(M, f.rows) * cdiv(N, f.cols) * splits;
-    float us = tiled_walk_us(exact ? f.exact_us : f.step_us, exact ? f.exact_alone_us : f.alone_us, f.per_cu, units, cdiv(cdiv(KB, splits), f.groups)) + (exact ? 4.1f : 4.6f);
-    if (f.groups > 1) us += 0.6f;
-    if (splits > 1) us += 2.0f + (float)splits * M * N * 8.0f / (exact ? 3.8e6f : 4.9e6f);
+    const int64_t units = (int64_t)cdiv(M, f.rows) * cdiv(N, f.cols) * splits, further = (units - 1) / (256 * f.per_cu);
+    float us = tiled_walk_us(exact ? f.exact_us : f.step_us, exact ? f.exact_alone_us : f.alone_us, f.per_cu, units, cdiv(cdiv(KB, splits), f.groups));
+    us += (exact ? 4.1f : 4.6f) + 0.9f * further;
+    if (f.groups > 1) us += 0.45f;
+    if (splits > 1) us += 2.0f + (float)splits * M * N * 8.0f / (exact ? 3.9e6f : 5.0e6f);
     return us;
 }
 

@@ -13,14 +13,14 @@ struct TiledForm {
 };
 enum { TILED_256, TILED_192_256, TILED_128_256, TILED_128, TILED_64, TILED_32, TILED_64_SHARED, TILED_64_64_SHARED, TILED_COUNT };
 static const TiledForm TILED_FORMS[TILED_COUNT] = {
-    {256, 256, 1, 1, 1.73f, 1.47f, 0.0f, 0.0f},
+    {256, 256, 1, 1, 1.73f, 1.48f, 0.0f, 0.0f},
     {192, 256, 1, 1, 1.40f, 1.11f, 0.0f, 0.0f},
-    {128, 256, 1, 1, 1.09f, 0.75f, 1.92f, 1.46f},
-    {128, 128, 2, 1, 0.99f, 0.53f, 0.0f, 0.0f},
-    {64, 128, 2, 1, 0.70f, 0.39f, 1.03f, 0.60f},
-    {32, 128, 2, 1, 0.66f, 0.37f, 0.83f, 0.51f},
-    {64, 128, 1, 2, 0.96f, 0.62f, 1.55f, 1.02f},
-    {64, 64, 1, 2, 0.82f, 0.43f, 1.13f, 0.67f},
+    {128, 256, 1, 1, 1.03f, 0.83f, 1.82f, 1.43f},
+    {128, 128, 2, 1, 0.99f, 0.54f, 0.0f, 0.0f},
+    {64, 128, 2, 1, 0.68f, 0.37f, 1.00f, 0.60f},
+    {32, 128, 2, 1, 0.70f, 0.34f, 0.91f, 0.48f},
+    {64, 128, 1, 2, 0.86f, 0.65f, 1.16f, 1.05f},
+    {64, 64, 1, 2, 0.70f, 0.43f, 0.97f, 0.66f},
 };
 
 struct TiledPlan {

@@ -11,7 +11,8 @@ SHAPES = [(1, 16, 16), (1, 1, 128), (1, 40, 128), (2, 130, 272), (3, 4096, 512),
           (257, 272, 1536), (520, 640, 2048), (1030, 528, 384)]
 TILES = [(301, 702, 1040), (935, 1070, 144), (1075, 23, 2032), (644, 1546, 1184), (653, 454, 4672), (1925, 4007, 144), (6017, 275, 7200),
          (2250, 1806, 128), (1606, 1155, 5280), (3255, 2439, 144), (5480, 267, 6928), (3466, 3630, 144), (1806, 2250, 17984),
-         (1347, 1459, 128), (66, 2005, 7952), (1297, 777, 400), (2884, 130, 6560), (2692, 135, 7840)]
+         (1347, 1459, 128), (66, 2005, 7952), (1297, 777, 400), (2884, 130, 6560), (2692, 135, 7840),
+         (1350, 707, 1520), (69, 1348, 7696), (5, 2839, 32544)]
 BACK_SHAPES = [(1, 16, 16), (1, 130, 128), (5, 128, 272), (17, 300, 400), (64, 257, 640), (77, 1200, 1024), (130, 33, 2112), (200, 1000, 144),
                (300, 512, 512), (520, 264, 1040)]
 BACK_TILES = [(130, 17, 7824), (33, 710, 3376), (558, 18, 7200), (135, 3885, 7312)]
