@@ -368,8 +368,8 @@ int lowbit_block_fp8_experts(const void *x, const int64_t *topk_ids, const void 
                              int n_experts, const void *gate_up, const float *gate_up_scale, const void *down, const float *down_scale,
                              void *workspace, size_t workspace_bytes, void *y, int act_dtype, int64_t hidden, int64_t inter, int act,
                              void *stream);
-/* What it runs as: plan4 = {rows of a tile of the first product, rows and columns of one of the second (0: each pair streams its weights), 1 if the pairs
- * are sorted by launches of their own} */
+/* What it runs as: plan4 = {rows of a tile of the first product, rows and columns of one of the second (0: each pair streams its weights), 1 if a launch
+ * of its own places the pairs} */
 int lowbit_block_fp8_experts_plan(int64_t tokens, int top_k, int n_experts, int64_t hidden, int64_t inter, int *plan4);
 
 #ifdef __cplusplus

@@ -227,8 +227,17 @@ __global__ __launch_bounds__(64 * WM * WK, MIN_WAVES) void block_fp8_back_kernel
 
 // Rows of g that do not start at 16-byte boundaries: a copy in rows of ldg values, zeros past N.
 __global__ __launch_bounds__(256) void block_fp8_pad_kernel(const uint16_t *__restrict__ g, uint16_t *__restrict__ to, int N, int ldg) {
-    const int64_t m = blockIdx.y;
-    for (int n = blockIdx.x * 256 + threadIdx.x; n < ldg; n += gridDim.x * 256) to[m * ldg + n] = n < N ? g[m * N + n] : (uint16_t)0;
+    const int n = (blockIdx.x * 256 + threadIdx.x) * 8;
+    if (n >= ldg) return;
+    const uint16_t *const from = g + (int64_t)blockIdx.y * N + n;
+    u32x4 v = {};
+    if (n + 8 <= N) __builtin_memcpy(&v, from, sizeof(v));   // (rows start at odd places)
+    else {
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (n + j < N) v[j / 2] |= (uint32_t)from[j] << (16 * (j & 1));
+    }
+    *(u32x4 *)(to + (int64_t)blockIdx.y * ldg + n) = v;
 }
 
 static int cdiv(int a, int b) { return (a + b - 1) / b; }
@@ -307,7 +316,7 @@ int launch_block_fp8_back(const void *grad, const uint8_t *w, const float *ws, v
     if (padded(N)) {
         p.ldg = cdiv(N, BACK_STEP) * BACK_STEP;
         for (int m = 0; m < M; m += 65535) {
-            const dim3 grid(cdiv((int)p.ldg, 1024), M - m < 65535 ? M - m : 65535);
+            const dim3 grid(cdiv((int)p.ldg, 2048), M - m < 65535 ? M - m : 65535);
             hipLaunchKernelGGL(block_fp8_pad_kernel, grid, dim3(256), 0, st, (const uint16_t *)grad + (int64_t)m * N, (uint16_t *)space + m * p.ldg, N, (int)p.ldg);
         }
         p.g = space;

@@ -16,7 +16,6 @@
 
 namespace lowbit {
 
-void launch_moe_route(const int64_t *ids, int pairs, int n_exp, int32_t *offsets, int32_t *order, int32_t *pos, hipStream_t st);
 void launch_moe_combine_f32(const float *y, const int32_t *pos, const void *weight, int w_dtype, void *out, int act_dtype, int tokens, int top_k,
                             int N, hipStream_t st);
 struct ExpertsArgs {
@@ -214,15 +213,16 @@ __global__ __launch_bounds__(64 * WAVES) void block_fp8_expert_down_token_kernel
     out[(int64_t)token * p.H + n0 + threadIdx.x] = to_at<AT>(v);
 }
 
-// The rows of x in codes (as bfloat16 numbers, see EXACT) and scales, and the pairs sorted by expert, in one launch: the first workgroups quantize (32 blocks each), the rest place
-// four pairs each.  A wave counts the pairs that come before its own - those of lower experts, and the earlier ones of its expert - as
-// moe_sort_gather_kernel does; waves pairs + e write offsets[e].
-constexpr int EXPERTS_SORT_PAIRS = 4096;
-template <typename AT>
+// The rows of x in codes (as bfloat16 numbers, see EXACT) and scales, and the pairs' sort by expert or its first half, in one launch: the
+// first workgroups quantize (32 blocks each).  Of up to EXPERTS_SORT_PAIRS pairs the rest place four each: a wave counts the pairs that come
+// before its own - those of lower experts, and the earlier ones of its expert -, and waves pairs + e write offsets[e].  More: each counts a
+// chunk of pairs by expert, counts[chunk][e], for the launch that places them.
+constexpr int EXPERTS_SORT_PAIRS = 3200, EXPERTS_CHUNKS = 256;
+template <typename AT, bool PLACES>
 __global__ __launch_bounds__(256) void block_fp8_expert_rows_kernel(const AT *__restrict__ x, const int64_t *__restrict__ ids, uint8_t *__restrict__ codes,
                                                                     float *__restrict__ scale, int32_t *__restrict__ offsets, int32_t *__restrict__ order,
-                                                                    int32_t *__restrict__ pos, int tokens, int pairs, int n_exp, int K, int KB,
-                                                                    int quantizing) {
+                                                                    int32_t *__restrict__ pos, int32_t *__restrict__ counts, int tokens, int pairs,
+                                                                    int n_exp, int K, int KB, int quantizing, int chunk) {
     if ((int)blockIdx.x < quantizing) {
         const int64_t unit = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
         if (unit >= (int64_t)tokens * KB) return;
@@ -231,6 +231,19 @@ __global__ __launch_bounds__(256) void block_fp8_expert_rows_kernel(const AT *__
         if (k < K) load16(x + (int64_t)row * K + k, v);
         store16<true>(codes + (int64_t)row * KB * (2 * FP8_BLOCK), k, quantize16<AT>(v, s));
         if ((threadIdx.x & 7) == 0) scale[(int64_t)kb * tokens + row] = s;
+        return;
+    }
+    if constexpr (!PLACES) {
+        extern __shared__ int32_t seen[];                    // [n_exp]
+        const int c = blockIdx.x - quantizing, first = c * chunk, last = first + chunk < pairs ? first + chunk : pairs;
+        for (int e = threadIdx.x; e < n_exp; e += 256) seen[e] = 0;
+        __syncthreads();
+        for (int b = first + threadIdx.x; b < last; b += 256) {
+            const int64_t e = ids[b];
+            if (e >= 0 && e < n_exp) atomicAdd(&seen[e], 1);
+        }
+        __syncthreads();
+        for (int e = threadIdx.x; e < n_exp; e += 256) counts[(int64_t)c * n_exp + e] = seen[e];
         return;
     }
     const int lane = threadIdx.x & 63, b = (blockIdx.x - quantizing) * 4 + (threadIdx.x >> 6);
@@ -254,6 +267,91 @@ __global__ __launch_bounds__(256) void block_fp8_expert_rows_kernel(const AT *__
     const bool valid = own >= 0 && own < n_exp;
     pos[b] = valid ? before : -1;
     if (valid) order[before] = b;
+}
+
+// Places the pairs of a chunk per wave behind those of lower experts and of earlier chunks, in their order.  Every workgroup sums the chunks'
+// counts for itself; four waves each, since with sixteen the ranks of 64 pairs, 300 instructions, wait for one another (10 and 18 us).  6726
+// pairs over 4 experts 6.6 us, 32768 over 128 16, where one workgroup that sorts them all takes 17 and
+// some 200 (4096 tokens through 8 of 128 of [768 x 2048] 713 us so, 527 this way); 3600 over 64 6.6 where counting all
+// earlier pairs for each takes 9, 1800 2.5.
+__global__ __launch_bounds__(1024) void block_fp8_expert_place_kernel(const int64_t *__restrict__ ids, const int32_t *__restrict__ counts,
+                                                                      int32_t *__restrict__ offsets, int32_t *__restrict__ order,
+                                                                      int32_t *__restrict__ pos, int pairs, int n_exp, int chunks, int chunk) {
+    constexpr int U = 16;                                    // counts on their way together
+    extern __shared__ int32_t at[];                          // [n_exp] pairs of earlier chunks, [n_exp + 1] offsets, [waves][n_exp] next places
+    const int threads = blockDim.x, waves = threads >> 6, t = threadIdx.x, lane = t & 63, wave = t >> 6, c0 = blockIdx.x * waves;
+    int32_t *const before = at, *const total = at + n_exp, *const next = total + n_exp + 1;
+    for (int e = t; e < 2 * n_exp; e += threads) at[e] = 0;
+    __syncthreads();
+    const int parts = threads > n_exp ? threads / n_exp : 1, step = threads > n_exp ? n_exp : threads, part = t / step;
+    if (part < parts)
+        for (int e = t - part * step; e < n_exp; e += step) {
+            int earlier = 0, all = 0;
+            for (int c = part; c < chunks; c += parts * U) {
+                int n[U];
+#pragma unroll
+                for (int u = 0; u < U; u++) n[u] = c + u * parts < chunks ? counts[(int64_t)(c + u * parts) * n_exp + e] : 0;
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    all += n[u];
+                    earlier += c + u * parts < c0 ? n[u] : 0;
+                }
+            }
+            atomicAdd(&before[e], earlier);
+            atomicAdd(&total[e], all);
+        }
+    __syncthreads();
+    if (wave == 0) {                                         // total: from sums to offsets
+        int sum = 0;
+        for (int e0 = 0; e0 < n_exp; e0 += 64) {
+            const int own = e0 + lane < n_exp ? total[e0 + lane] : 0;
+            int upto = own;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const int up = __shfl_up(upto, d);
+                if (lane >= d) upto += up;
+            }
+            if (e0 + lane < n_exp) total[e0 + lane] = sum + upto - own;
+            sum += __builtin_amdgcn_readlane(upto, 63);
+        }
+        if (lane == 0) total[n_exp] = sum;
+    }
+    __syncthreads();
+    if (blockIdx.x == 0)
+        for (int e = t; e <= n_exp; e += threads) offsets[e] = total[e];
+    for (int e = t; e < n_exp; e += threads) {
+        int place = total[e] + before[e];
+        for (int w = 0; w < waves; w += U) {
+            int n[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) n[u] = c0 + w + u < chunks ? counts[(int64_t)(c0 + w + u) * n_exp + e] : 0;
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                if (w + u < waves) next[(w + u) * n_exp + e] = place;
+                place += n[u];
+            }
+        }
+    }
+    __syncthreads();
+    const int first = (c0 + wave) * chunk;                   // (a chunk past the last one starts behind the pairs)
+    for (int i = 0; i < chunk; i += 64) {
+        const int b = first + i + lane;
+        const int64_t id = b < pairs ? ids[b] : -1;
+        const int e = id >= 0 && id < n_exp ? (int)id : -1;
+        int rank = 0, same = 0;                              // among the 64 pairs of the same expert
+#pragma unroll
+        for (int l = 0; l < 64; l++) {
+            const bool equal = __builtin_amdgcn_readlane(e, l) == e;
+            same += equal;
+            rank += equal && l < lane;
+        }
+        const int place = e >= 0 ? next[wave * n_exp + e] + rank : -1;
+        __syncthreads();                                     // (places are read ahead of their update, and after the last one's)
+        if (e >= 0 && rank == same - 1) next[wave * n_exp + e] += same;
+        __syncthreads();
+        if (b < pairs) pos[b] = place;
+        if (e >= 0) order[place] = b;
+    }
 }
 
 // Few pairs: each streams its expert's weights, which costs as many reads as there are pairs; the codes of a row of x and those of a token's
@@ -333,7 +431,7 @@ void block_fp8_experts_plan(int tokens, int top_k, int n_exp, int H, int I, int 
 }
 
 struct ExpertsSpace {
-    size_t h, hs, x, xs, offsets, order, pos, y, bytes;
+    size_t h, hs, x, xs, offsets, order, pos, counts, y, bytes;
     int ldx, ldxs;
 };
 static ExpertsSpace experts_space(int tokens, int top_k, int n_exp, int H, int I) {
@@ -356,6 +454,7 @@ static ExpertsSpace experts_space(int tokens, int top_k, int n_exp, int H, int I
         w.offsets = take((size_t)(n_exp + 1) * 4);
         w.order = take((size_t)pairs * 4);
         w.pos = take((size_t)pairs * 4);
+        if (pairs > EXPERTS_SORT_PAIRS) w.counts = take((size_t)EXPERTS_CHUNKS * n_exp * 4);
         w.y = take((size_t)pairs * H * sizeof(float));       // (rounded once, when a token's are summed: 16 bits would cost its precision twice)
     }
     w.bytes = at;
@@ -389,10 +488,20 @@ template <typename AT> static int launch_experts_t(ExpertsArgs p, const ExpertsS
     const int KB = fp8_blocks(p.H);
     if ((int64_t)tokens * KB > (int64_t)1 << 34) return -3;
     const int quantizing = (int)(((int64_t)tokens * KB + 31) / 32);
-    const bool sorts = pairs <= EXPERTS_SORT_PAIRS;
-    hipLaunchKernelGGL((block_fp8_expert_rows_kernel<AT>), dim3(quantizing + (sorts ? (pairs + p.n_exp + 4) / 4 : 0)), dim3(256), 0, st, (const AT *)p.x,
-                       p.ids, ws + at.x, (float *)(ws + at.xs), offsets, order, pos, tokens, pairs, p.n_exp, p.H, KB, quantizing);
-    if (!sorts) launch_moe_route(p.ids, pairs, p.n_exp, offsets, order, pos, st);
+    int32_t *const counts = (int32_t *)(ws + at.counts);
+    const AT *const x = (const AT *)p.x;
+    float *const xs = (float *)(ws + at.xs);
+    if (pairs <= EXPERTS_SORT_PAIRS)
+        hipLaunchKernelGGL((block_fp8_expert_rows_kernel<AT, true>), dim3(quantizing + (pairs + p.n_exp + 4) / 4), dim3(256), 0, st, x, p.ids, ws + at.x,
+                           xs, offsets, order, pos, nullptr, tokens, pairs, p.n_exp, p.H, KB, quantizing, 0);
+    else {
+        const int chunk = ((pairs + EXPERTS_CHUNKS - 1) / EXPERTS_CHUNKS + 63) / 64 * 64, chunks = (pairs + chunk - 1) / chunk;
+        const int waves = p.n_exp <= 512 ? 4 : 1;            // at most 48 KiB
+        hipLaunchKernelGGL((block_fp8_expert_rows_kernel<AT, false>), dim3(quantizing + chunks), dim3(256), (size_t)p.n_exp * 4, st, x, p.ids, ws + at.x,
+                           xs, offsets, order, pos, counts, tokens, pairs, p.n_exp, p.H, KB, quantizing, chunk);
+        hipLaunchKernelGGL(block_fp8_expert_place_kernel, dim3((chunks + waves - 1) / waves), dim3(64 * waves), ((size_t)p.n_exp * (waves + 2) + 1) * 4, st,
+                           p.ids, counts, offsets, order, pos, pairs, p.n_exp, chunks, chunk);
+    }
 
     TiledArgs t{};
     t.offsets = offsets; t.order = order; t.n_exp = p.n_exp; t.top_k = p.top_k; t.M = pairs; t.I = p.I; t.act = p.act;

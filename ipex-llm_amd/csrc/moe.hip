@@ -226,12 +226,6 @@ void launch_moe_combine_f32(const float *y, const int32_t *pos, const void *weig
     else launch_combine<float, __bf16>(y, pos, weight, w_dtype, out, tokens, top_k, N, st);
 }
 
-void launch_moe_route(const int64_t *ids, int pairs, int n_exp, int32_t *offsets, int32_t *order, int32_t *pos, hipStream_t st) {
-    const int waves = n_exp <= 512 ? 16 : 2;              // at most 48 KiB of counters
-    hipLaunchKernelGGL(moe_route_kernel, dim3(1), dim3(64 * waves), (size_t)n_exp * (waves + 1) * sizeof(int32_t), st, ids, pairs, n_exp,
-                       offsets, order, pos);
-}
-
 // Whether the pairs go through the streaming kernel, which reads an expert's weights once per pair: while there are no
 // more pairs than experts, so that few experts are read twice.  Measured (streaming / grouped, us): 60 experts of
 // [1408 x 2048] sym_int4 at 8 / 32 / 64 pairs 17 / 41, 40 / 71, 74 / 78; 8 experts of [14336 x 4096] fp8_e4m3 at 4 / 8 /
@@ -283,11 +277,13 @@ int launch_experts(const void *x, const int64_t *ids, const void *weight, int w_
                                act_dtype, hidden, inter, act, st);
     int32_t *const offsets = (int32_t *)(ws + at.offsets), *const order = (int32_t *)(ws + at.order), *const pos = (int32_t *)(ws + at.pos);
     void *const xs = ws + at.xs, *const y = ws + at.y;
+    const int waves = n_exp <= 512 ? 16 : 2;          // at most 48 KiB of counters
     if (pairs <= MOE_SORT_PAIRS && n_exp <= 512) {
         hipLaunchKernelGGL(moe_sort_gather_kernel, dim3(pairs + n_exp + 1), dim3(256), 0, st, ids, (const u32x4 *)x, pairs, n_exp, offsets,
                            pos, (u32x4 *)xs, top_k, hidden / 8);
     } else {
-        launch_moe_route(ids, pairs, n_exp, offsets, order, pos, st);
+        hipLaunchKernelGGL(moe_route_kernel, dim3(1), dim3(64 * waves), (size_t)n_exp * (waves + 1) * sizeof(int32_t), st, ids, pairs, n_exp,
+                           offsets, order, pos);
         hipLaunchKernelGGL(moe_gather_kernel, dim3(pairs), dim3(256), 0, st, (const u32x4 *)x, order, offsets + n_exp, (u32x4 *)xs, top_k,
                            hidden / 8);
     }

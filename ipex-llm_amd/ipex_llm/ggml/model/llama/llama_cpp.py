@@ -487,7 +487,7 @@ def lowbit_block_fp8_plan(dtype, backward, m, n, k):
 
 
 def lowbit_block_fp8_experts_plan(tokens, top_k, n_experts, hidden, inter):
-    """(rows of a tile of the first product, rows, columns of one of the second (0: pair by pair), whether the sort has its own launches)."""
+    """(rows of a tile of the first product, rows, columns of one of the second (0: pair by pair), whether a launch of its own places the pairs)."""
     plan4 = (c_int * 4)()
     _check(_lib.lowbit_block_fp8_experts_plan(tokens, top_k, n_experts, hidden, inter, plan4), "lowbit_block_fp8_experts_plan")
     return tuple(plan4)

@@ -370,7 +370,7 @@ def test_experts_in_tiles_of_every_form(tokens, top_k, n_exp, hidden, inter):
     check_experts(expert_case(tokens, tokens, top_k, n_exp, hidden, inter, torch.bfloat16), torch.bfloat16)
 
 
-@pytest.mark.parametrize("tokens", [1, 3, 50])
+@pytest.mark.parametrize("tokens", [1, 3, 50, 1500])
 def test_experts_skip_indices_that_name_none_and_experts_without_rows(tokens):
     case = list(expert_case(4, tokens, 3, 6, 256, 256, torch.bfloat16))
     case[1] = torch.where(case[1] == 2, torch.tensor(4), case[1])
