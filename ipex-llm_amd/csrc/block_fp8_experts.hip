@@ -271,10 +271,9 @@ __global__ __launch_bounds__(256) void block_fp8_expert_rows_kernel(const AT *__
 
 // Places the pairs of a chunk per wave behind those of lower experts and of earlier chunks, in their order.  Every workgroup sums the chunks'
 // counts for itself; four waves each, since with sixteen the ranks of 64 pairs, 300 instructions, wait for one another (10 and 18 us).  6726
-// pairs over 4 experts 6.6 us, 32768 over 128 16, where one workgroup that sorts them all takes 17 and
-// some 200 (4096 tokens through 8 of 128 of [768 x 2048] 713 us so, 527 this way); 3600 over 64 6.6 where counting all
-// earlier pairs for each takes 9, 1800 2.5.
-__global__ __launch_bounds__(1024) void block_fp8_expert_place_kernel(const int64_t *__restrict__ ids, const int32_t *__restrict__ counts,
+// pairs over 4 experts 6.6 us, 32768 over 128 16, where one workgroup that sorts them all takes 17 and some 200 (4096 tokens through 8 of 128 of
+// [768 x 2048] 713 us so, 527 this way); 3600 over 64 6.6 where counting all earlier pairs for each takes 9, 1800 2.5.
+__global__ __launch_bounds__(256) void block_fp8_expert_place_kernel(const int64_t *__restrict__ ids, const int32_t *__restrict__ counts,
                                                                       int32_t *__restrict__ offsets, int32_t *__restrict__ order,
                                                                       int32_t *__restrict__ pos, int pairs, int n_exp, int chunks, int chunk) {
     constexpr int U = 16;                                    // counts on their way together
@@ -496,7 +495,7 @@ template <typename AT> static int launch_experts_t(ExpertsArgs p, const ExpertsS
                            xs, offsets, order, pos, nullptr, tokens, pairs, p.n_exp, p.H, KB, quantizing, 0);
     else {
         const int chunk = ((pairs + EXPERTS_CHUNKS - 1) / EXPERTS_CHUNKS + 63) / 64 * 64, chunks = (pairs + chunk - 1) / chunk;
-        const int waves = p.n_exp <= 512 ? 4 : 1;            // at most 48 KiB
+        const int waves = p.n_exp <= 2048 ? 4 : 1;           // at most 48 KiB
         hipLaunchKernelGGL((block_fp8_expert_rows_kernel<AT, false>), dim3(quantizing + chunks), dim3(256), (size_t)p.n_exp * 4, st, x, p.ids, ws + at.x,
                            xs, offsets, order, pos, counts, tokens, pairs, p.n_exp, p.H, KB, quantizing, chunk);
         hipLaunchKernelGGL(block_fp8_expert_place_kernel, dim3((chunks + waves - 1) / waves), dim3(64 * waves), ((size_t)p.n_exp * (waves + 2) + 1) * 4, st,

@@ -21,7 +21,7 @@ EXPERTS = [(1, 2, 8, 128, 128), (1, 1, 1, 16, 128), (1, 8, 8, 400, 256), (2, 2, 
 EXPERT_TILES = [(39, 2, 70, 784, 128), (148, 1, 70, 800, 128), (56, 3, 70, 1712, 128), (1008, 4, 8, 160, 128), (897, 2, 20, 800, 128),
                 (476, 3, 20, 2112, 128), (3356, 1, 8, 3344, 128), (2079, 2, 70, 128, 256), (2131, 2, 3, 128, 128),
                 (225, 3, 20, 2064, 128), (488, 2, 20, 4016, 128), (399, 4, 20, 128, 896), (300, 2, 4, 640, 2304), (3000, 1, 7, 272, 1152),
-                (286, 2, 8, 2864, 128), (2461, 4, 70, 448, 256), (3676, 4, 70, 288, 128), (1700, 2, 600, 16, 128), (1700, 2, 512, 16, 128),
+                (286, 2, 8, 2864, 128), (2461, 4, 70, 448, 256), (3676, 4, 70, 288, 128), (1700, 2, 600, 16, 128), (1700, 2, 512, 16, 128), (900, 4, 2100, 16, 128),
                 (9000, 2, 1, 16, 128)]
 
 
