@@ -15,14 +15,14 @@ TILES = [(301, 702, 1040), (935, 1070, 144), (1075, 23, 2032), (644, 1546, 1184)
          (1350, 707, 1520), (69, 1348, 7696), (5, 2839, 32544)]
 BACK_SHAPES = [(1, 16, 16), (1, 130, 128), (5, 128, 272), (17, 300, 400), (64, 257, 640), (77, 1200, 1024), (130, 33, 2112), (200, 1000, 144),
                (300, 512, 512), (520, 264, 1040)]
-BACK_TILES = [(130, 17, 7824), (33, 710, 3376), (558, 18, 7200), (135, 3885, 7312)]
+BACK_TILES = [(130, 17, 7824), (33, 710, 3376), (558, 18, 7200), (135, 3885, 7312), (66000, 17, 16)]
 EXPERTS = [(1, 2, 8, 128, 128), (1, 1, 1, 16, 128), (1, 8, 8, 400, 256), (2, 2, 16, 256, 384), (3, 4, 4, 272, 128), (40, 2, 5, 512, 256),
            (130, 3, 4, 144, 384), (300, 2, 70, 256, 128), (17, 5, 3, 384, 256), (600, 1, 2, 640, 512)]
 EXPERT_TILES = [(39, 2, 70, 784, 128), (148, 1, 70, 800, 128), (56, 3, 70, 1712, 128), (1008, 4, 8, 160, 128), (897, 2, 20, 800, 128),
                 (476, 3, 20, 2112, 128), (3356, 1, 8, 3344, 128), (2079, 2, 70, 128, 256), (2131, 2, 3, 128, 128),
                 (225, 3, 20, 2064, 128), (488, 2, 20, 4016, 128), (399, 4, 20, 128, 896), (300, 2, 4, 640, 2304), (3000, 1, 7, 272, 1152),
                 (286, 2, 8, 2864, 128), (2461, 4, 70, 448, 256), (3676, 4, 70, 288, 128), (1700, 2, 600, 16, 128), (1700, 2, 512, 16, 128), (900, 4, 2100, 16, 128),
-                (9000, 2, 1, 16, 128)]
+                (9000, 2, 1, 16, 128), (70000, 1, 2, 16, 128)]
 
 
 def blocks(n):
