@@ -190,11 +190,13 @@ template <int ROWS> __device__ inline int count_expert_tiles(const int32_t *__re
     return __builtin_amdgcn_readfirstlane(all);
 }
 
-// act(g) * u in float32: hardware exp2 and reciprocal, 1 unit of 2^-24 each, ahead of a rounding to 4 bits
+// act(g) in float32.  tanh-GELU as g * sigmoid(2 u), in which nothing cancels: 1 - 1 / (1 + e^2u) is zero from g of about -5 on, where the
+// values of a block may all lie.  Hardware exp2 and reciprocal are within 1 unit of 2^-24; the exponent's own rounding counts as many of them
+// as it is large: 2^-24 times |g| (SiLU) and some 6 |u| (GELU, whose u takes four roundings), ahead of a rounding to 4 bits.
 __device__ inline float gate_act(float g, int act) {
     if (act == 0) return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * g));
     const float u = 0.7978845608028654f * (g + 0.044715f * g * g * g);
-    return g * (1.0f - __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(2.8853900817779268f * u)));   // 0.5 g (1 + tanh u)
+    return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-2.8853900817779268f * u));           // 0.5 g (1 + tanh u)
 }
 
 }  // namespace lowbit
