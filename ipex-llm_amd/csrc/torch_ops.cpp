@@ -345,7 +345,7 @@ Tensor block_fp8_dense(const Tensor &w, const Tensor &scale, at::ScalarType dtyp
 // The gradient that flows on to x, the quantization of x counting as the identity.  Holds the weight as ProductBackward does.
 struct BlockFp8Backward : public torch::autograd::Node {
     Tensor w, scale;
-    at::ScalarType dtype = at::kHalf;
+    at::ScalarType dtype = at::kHalf, x_dtype = at::kHalf;   // what the gradient is multiplied in; x's own
     at::DimVector x_shape;
 
     std::string name() const override { return "BlockFp8LinearBackward"; }
@@ -353,13 +353,13 @@ struct BlockFp8Backward : public torch::autograd::Node {
     torch::autograd::variable_list apply(torch::autograd::variable_list &&grads) override {
         if (!task_should_compute_output(0)) return {Tensor()};
         const int64_t N = w.size(0), K = w.size(1);
-        const Tensor grad = grads[0].defined() ? grads[0].to(dtype).reshape({-1, N})
-                                               : at::zeros({c10::multiply_integers(x_shape) / K, N}, w.options().dtype(dtype));
+        const Tensor grad = grads[0].defined() ? grads[0].to(x_dtype).reshape({-1, N})
+                                               : at::zeros({c10::multiply_integers(x_shape) / K, N}, w.options().dtype(x_dtype));
         c10::DeviceGuard guard(grad.device());
         if (grad.device() != w.device()) throw Failed("the block-scaled weight is not where the forward found it");
         if (dtype == at::kFloat || differentiable(grad) || !nothing_watches(grad))     // (float32, a second derivative, a transform: the dense product)
-            return {at::matmul(grad, block_fp8_dense(w, scale, dtype)).view(x_shape)};
-        const Tensor g = whole_rows(grad);
+            return {at::matmul(grad, block_fp8_dense(w, scale, x_dtype)).view(x_shape)};
+        const Tensor g = whole_rows(grad.to(dtype));
         const int64_t M = g.size(0);
         const int dt = dtype_code(dtype);
         Tensor gx = at::empty(x_shape, g.options());
@@ -367,12 +367,13 @@ struct BlockFp8Backward : public torch::autograd::Node {
         const Tensor ws = bytes ? at::empty({(int64_t)bytes}, g.options().dtype(at::kByte)) : Tensor();
         check(api.block_fp8_backward(g.const_data_ptr(), w.const_data_ptr(), scale.const_data_ptr<float>(), gx.data_ptr(), dt, M, N, K,
                                      bytes ? ws.data_ptr() : nullptr, bytes, current_stream(g)), "lowbit_block_fp8_backward");
-        return {gx};
+        return {gx.to(x_dtype)};
     }
 };
 
-// y = Q(x) W^T (+ bias), with the gradient to x where x wants one; an undefined tensor when this is not the plain case
-Tensor block_fp8_linear(const Tensor &x_in, const Tensor &w, const Tensor &scale, const Tensor &bias) {
+// y = Q(x) W^T (+ bias), with the gradient to x where x wants one; an undefined tensor when this is not the plain case.  grad_dt: a 16-bit
+// type in which the gradient of a float32 product is multiplied, or x's own
+Tensor block_fp8_linear(const Tensor &x_in, const Tensor &w, const Tensor &scale, const Tensor &bias, int grad_dt) {
     if (!on_gpu(x_in) || x_in.dim() < 1 || x_in.numel() == 0 || dtype_code(x_in.scalar_type()) < 0 || !is_block_fp8(w, scale, x_in, 0) ||
         w.size(1) != x_in.size(-1) || !nothing_watches(x_in) || x_in._fw_grad(/*level=*/0).defined()) return {};
     if (bias.defined() && (bias.scalar_type() != x_in.scalar_type() || bias.device() != x_in.device() || bias.dim() != 1 ||
@@ -383,7 +384,8 @@ Tensor block_fp8_linear(const Tensor &x_in, const Tensor &w, const Tensor &scale
     node->set_next_edges(torch::autograd::collect_next_edges(x_in));
     node->w = w;
     node->scale = scale;
-    node->dtype = x_in.scalar_type();
+    node->x_dtype = x_in.scalar_type();
+    node->dtype = grad_dt == LOWBIT_DT_F16 ? at::kHalf : grad_dt == LOWBIT_DT_BF16 ? at::kBFloat16 : x_in.scalar_type();
     node->x_shape.assign(x_in.sizes().begin(), x_in.sizes().end());
     {
         c10::AutoGradMode no_grad(false);
@@ -664,14 +666,15 @@ PyObject *py_block_fp8_quantize(PyObject *, PyObject *const *args, Py_ssize_t n)
     });
 }
 
-// block_fp8_linear(x, weight, scale, bias or None) -> y or None
+// block_fp8_linear(x, weight, scale, bias or None, dtype code of the gradient's product) -> y or None
 PyObject *py_block_fp8_linear(PyObject *, PyObject *const *args, Py_ssize_t n) {
-    return answer("block_fp8_linear", n, 4, [&] {
+    return answer("block_fp8_linear", n, 5, [&] {
         const Args a{args, n};
         const Tensor &x = a.tensor(0), &w = a.tensor(1), &scale = a.tensor(2);
         const Tensor bias = a.optional(3);
+        const int grad_dt = (int)a.integer(4);
         NoGil free;
-        return block_fp8_linear(x, w, scale, bias);
+        return block_fp8_linear(x, w, scale, bias, grad_dt);
     });
 }
 

@@ -14,13 +14,14 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
+import ipex_llm.ggml.model.llama.llama_cpp as ggml
 from ipex_llm.transformers.native_ops import ops
 from ipex_llm.utils.common import invalidInputError
 
 E4M3 = torch.float8_e4m3fn
 BLOCK = 128
 _ACCEL = "cuda"
-_FLOATS = (torch.float16, torch.bfloat16, torch.float32)
+_FLOATS = {torch.float16: ggml.DT_F16, torch.bfloat16: ggml.DT_BF16, torch.float32: ggml.DT_F32}
 
 
 def _blocks(n: int) -> int:
@@ -86,7 +87,7 @@ def block_fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.
     float16 and bfloat16: sums in float32 of products on the fp8 matrix pipes, which drop what lies 13 bits below the largest of a few
     neighbouring products (1e-5 of a result); float32: exact products.  The result is rounded once.  Where x wants a gradient it is
     grad W, grad not quantized."""
-    y = ops.block_fp8_linear(x, weight, weight_scale, bias)
+    y = ops.block_fp8_linear(x, weight, weight_scale, bias, -1)
     if y is not None:
         return y
     what = "block_fp8_linear"
@@ -109,18 +110,30 @@ def block_fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.
     return torch.matmul(xf + (values - xf).detach(), dense.t()).to(x.dtype)
 
 
+def _exact_product(x, weight, scale, grad_dtype):
+    """The product of float32 rows; where they want a gradient, it is multiplied in `grad_dtype`."""
+    y = ops.block_fp8_linear(x, weight, scale, None, _FLOATS[grad_dtype])
+    return block_fp8_linear(x, weight, scale) if y is None else y
+
+
 def _expert_loop(x, top_k_index, top_k_weights, gate_up, gate_up_scale, down, down_scale, act_fn):
-    """Expert by expert: what differs from the native call is that act(g) * u is rounded to x's dtype before it is quantized."""
-    out = torch.zeros_like(x)
-    inter = gate_up.shape[1] // 2
-    for e in range(gate_up.shape[0]):
-        tok, slot = torch.where(top_k_index == e)
-        if tok.numel() == 0:
-            continue
-        gu = block_fp8_linear(x[tok], gate_up[e], gate_up_scale[e])
-        y = block_fp8_linear(act_fn(gu[:, :inter]) * gu[:, inter:], down[e], down_scale[e])
-        out = out.index_add(0, tok, (y * top_k_weights[tok, slot, None].to(y.dtype)).to(out.dtype))
-    return out
+    """Expert by expert, with what the native call keeps in float32 (g, u, act(g) * u, the pairs' results and their sum) kept so too, and
+    one rounding.  Where a gradient is wanted below 16-bit rows, the products of the backward take it in their type."""
+    (tokens, top_k), n_exp, inter = top_k_index.shape, gate_up.shape[0], gate_up.shape[1] // 2
+    expert = top_k_index.reshape(-1).long()
+    expert = expert.masked_fill((expert < 0) | (expert >= n_exp), n_exp)
+    order = expert.argsort(stable=True)
+    counts = torch.bincount(expert, minlength=n_exp + 1).tolist()
+    rows, ys = x.float()[torch.div(order, top_k, rounding_mode="floor")].split(counts), []
+    for e in range(n_exp):
+        if counts[e]:
+            gu = _exact_product(rows[e], gate_up[e], gate_up_scale[e], x.dtype)
+            ys.append(_exact_product(act_fn(gu[:, :inter]) * gu[:, inter:], down[e], down_scale[e], x.dtype))
+    if not ys:
+        return torch.zeros_like(x)
+    order = order[:len(order) - counts[n_exp]]
+    y = torch.cat(ys) * top_k_weights.reshape(-1)[order].float().unsqueeze(-1)
+    return y.new_zeros((tokens * top_k, x.shape[1])).index_copy(0, order, y).view(tokens, top_k, -1).sum(1).to(x.dtype)
 
 
 _ACTS = {0: F.silu, 1: lambda g: F.gelu(g, approximate="tanh")}
@@ -132,8 +145,9 @@ def block_fp8_experts(x: torch.Tensor, top_k_index: torch.Tensor, top_k_weights:
     e = top_k_index[t, j], p = top_k_weights.
 
     x [T, H]; top_k_index, top_k_weights [T, k]; gate_up [E, 2 I, H] (gate rows first) and down [E, H, I] codes with their scales, I a
-    multiple of 128; act 0 = SiLU, 1 = GELU (tanh form).  An index that names no expert counts nothing.  One native call in
-    float16 and bfloat16; float32, and x or weights that want a gradient, run expert by expert through block_fp8_linear."""
+    multiple of 128; act 0 = SiLU, 1 = GELU (tanh form).  An index that names no expert counts nothing.  act(g) u, the pairs' results and
+    their sum are float32, rounded once.  One native call in float16 and bfloat16; float32, x or weights that want a gradient, and more
+    than 64 experts per token, 4096 experts or 2^21 pairs, run expert by expert through block_fp8_linear."""
     invalidInputError(act in _ACTS, "block_fp8_experts: act is 0 (SiLU) or 1 (GELU, tanh form)")
     y = ops.block_fp8_experts(x, top_k_index, top_k_weights, gate_up, gate_up_scale, down, down_scale, act)
     if y is not None:

@@ -68,3 +68,91 @@ def test_gelu_of_gates_far_below_zero(dtype, tokens):
     unit = torch.finfo(dtype).eps / 2
     # (a result is rounded once; the second product drops bits as in any product)
     assert (got - want).norm() <= unit * want.norm() + slack.norm() + (3 ** 0.5 * 2.0 ** -13 + 2.0 ** -18) * size.norm()
+
+
+def expert_case(seed, tokens, top_k, n_exp, hidden, inter, dtype):
+    """Ordinary numbers, experts of which some get no token, and an index that names none."""
+    g = gen(seed)
+    x, p = torch.randn((tokens, hidden), generator=g).to(dtype), torch.rand((tokens, top_k), generator=g).to(dtype)
+    picks = torch.rand((tokens, n_exp - 1), generator=g).argsort(dim=1)[:, :top_k]
+    picks[-1, -1] = n_exp
+    return x, picks, p, *u.random_weight(g, 2 * inter, hidden, lead=(n_exp,)), *u.random_weight(g, hidden, inter, lead=(n_exp,))
+
+
+def near(got, case, act, dtype, drops=0.0):
+    """Rounded once, sums in float32: half a unit of the type; codes of h that may lie on either side of a border; a float32 sum of some
+    products of a few blocks, and `drops` for what the fp8 instruction leaves out."""
+    want, slack, size = experts64(*case, act, 2.0 ** -18)
+    unit = torch.finfo(dtype).eps / 2
+    assert (got.double().cpu() - want).norm() <= unit * want.norm() + slack.norm() + (drops + 2.0 ** -18) * size.norm()
+
+
+@pytest.mark.parametrize("tokens,top_k,n_exp,hidden,inter", [(1, 2, 4, 128, 128), (24, 3, 6, 400, 256), (64, 4, 9, 1024, 512)])
+@pytest.mark.parametrize("dtype", HALF, ids=ids)
+def test_experts_below_a_gradient_round_once_as_the_native_call_does(dtype, tokens, top_k, n_exp, hidden, inter):
+    case = expert_case(tokens, tokens, top_k, n_exp, hidden, inter, dtype)
+    on_gpu = [t.cuda() for t in case]
+    near(bf.block_fp8_experts(*on_gpu), case, 0, dtype, 3 ** 0.5 * 2.0 ** -13)
+    for which in (0, 2):                                     # x, the routing weights
+        leaves = list(on_gpu)
+        leaves[which] = on_gpu[which].clone().requires_grad_()
+        out = bf.block_fp8_experts(*leaves, tokens % 2)
+        assert out.dtype == dtype and out.requires_grad
+        near(out.detach(), case, tokens % 2, dtype)
+
+
+@pytest.mark.parametrize("dtype", HALF, ids=ids)
+def test_gradients_of_experts_in_16_bits(dtype):
+    tokens, n_exp, hidden, inter = 60, 5, 512, 384
+    case = expert_case(3, tokens, 2, n_exp, hidden, inter, dtype)
+    x, picks, p, gu, gus, dn, dns = case
+    leaf, weights = x.cuda().requires_grad_(), p.cuda().requires_grad_()
+    v = torch.randn((tokens, hidden), generator=gen(4)).to(dtype)
+    out = bf.block_fp8_experts(leaf, picks.cuda(), weights, *(t.cuda() for t in case[3:]))
+    gx, gp = torch.autograd.grad(out, (leaf, weights), v.cuda())
+    assert gx.dtype == dtype and gp.dtype == dtype
+    x64, p64, total = x.double().requires_grad_(), p.double().requires_grad_(), torch.zeros((tokens, hidden), dtype=torch.float64)
+    rows = x64 + (u.dense(*u.quantize(x, 1), 1) - x.double())        # the quantization counts as the identity
+    for e in range(n_exp):
+        t, j = torch.where(picks == e)
+        s = rows[t] @ u.dense(gu[e], gus[e]).t()
+        h = act64(s[:, :inter], 0) * s[:, inter:]
+        h = h + (u.dense(*u.quantize(h.detach(), 1), 1) - h.detach())
+        total = total.index_add(0, t, h @ u.dense(dn[e], dns[e]).t() * p64[t, j, None])
+    wx, wp = torch.autograd.grad(total, (x64, p64), v.double())
+    unit = torch.finfo(dtype).eps / 2
+    # on the way to x: p grad, the gradients of h and of (g | u), a pair's rows, and their sum are rounded; to p: once, of sums in float32 (and
+    # one code of h in 2^14 may be on the other side of a border: a step of 2^-3 of one of its terms, 2^-3 / sqrt(2^14) and less)
+    assert (gx.double().cpu() - wx).norm() <= 5 * unit * wx.norm()
+    assert (gp.double().cpu() - wp).norm() <= (unit + 2.0 ** -10) * wp.norm()
+    assert (gp[-1, -1] == 0).all()                           # of a pair that goes nowhere
+
+
+class _Relu(torch.nn.Module):
+    def forward(self, t):
+        return t.clamp(min=0)
+
+
+@pytest.mark.parametrize("dtype", HALF, ids=ids)
+def test_experts_that_no_kernel_takes_round_once_too(dtype):
+    """An activation of another kind, and more experts for a token than the library takes."""
+    case = expert_case(6, 20, 2, 5, 256, 128, dtype)
+    with torch.device("meta"):
+        module = bf.BlockFP8Experts(5, 256, 128, _Relu())
+    for name, t in zip(("gate_up_proj", "gate_up_proj_scale_inv", "down_proj", "down_proj_scale_inv"), case[3:]):
+        setattr(module, name, torch.nn.Parameter(t.cuda(), requires_grad=False))
+    got = module(*(t.cuda() for t in case[:3]))
+    relu = torch.zeros((20, 256), dtype=torch.float64)
+    x, picks, p, gu, gus, dn, dns = case
+    rows, exactly = u.dense(*u.quantize(x, 1), 1), torch.zeros((20, 256), dtype=torch.float64)
+    for e in range(5):
+        t, j = torch.where(picks == e)
+        s = rows[t] @ u.dense(gu[e], gus[e]).t()
+        y = u.dense(*u.quantize(s[:, :128].clamp(min=0) * s[:, 128:], 1), 1) @ u.dense(dn[e], dns[e]).t() * p[t, j].double()[:, None]
+        exactly.index_add_(0, t, y)
+        relu.index_add_(0, t, y.abs())
+    unit = torch.finfo(dtype).eps / 2
+    # (one code of h in 2^14 may be on the other side of a border, a step of 2^-3 of one of 128 terms)
+    assert (got.double().cpu() - exactly).norm() <= unit * exactly.norm() + 2.0 ** -12 * relu.norm()
+    many = expert_case(7, 3, 66, 70, 128, 128, dtype)
+    near(bf.block_fp8_experts(*(t.cuda() for t in many)), many, 0, dtype)
