@@ -47,6 +47,10 @@ def _check_weight(w, scale, x, what, dim=2):
     invalidInputError(not (torch.is_grad_enabled() and (w.requires_grad or scale.requires_grad)), f"{what}: weights and scales are frozen")
 
 
+def _differentiable(t):
+    return (t.requires_grad and torch.is_grad_enabled()) or torch.autograd.forward_ad.unpack_dual(t).tangent is not None
+
+
 def _quantized(x, weight, what):
     _check_input(x, what)
     invalidInputError(x.dim() >= (2 if weight else 1) and x.shape[-1] % 16 == 0, f"{what}: rows must be a multiple of 16 long")
@@ -85,7 +89,7 @@ def block_fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.
     """y = Q(x) W^T (+ bias) in x's dtype: x [.., K] is quantized by row, W = (weight, weight_scale) [N, K] in blocks of 128 x 128.
 
     float16 and bfloat16: sums in float32 of products on the fp8 matrix pipes, which drop what lies 13 bits below the largest of a few
-    neighbouring products (1e-5 of a result); float32: exact products.  The result is rounded once.  Where x wants a gradient it is
+    neighbouring products (1e-5 of a result); float32: exact products.  The result, with its bias, is rounded once.  Where x wants a gradient it is
     grad W, grad not quantized."""
     y = ops.block_fp8_linear(x, weight, weight_scale, bias, -1)
     if y is not None:
@@ -98,8 +102,16 @@ def block_fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.
     invalidInputError(bias is None or (bias.device == x.device and bias.shape == (n,)), f"{what}: the bias must be [{n}] on x's GPU")
     if x.numel() == 0:
         return x.new_empty((*x.shape[:-1], n)) + x.sum() * 0
-    if bias is not None:                                 # of another dtype, strided, or one that wants a gradient itself
-        return block_fp8_linear(x, weight, weight_scale) + bias.to(x.dtype)
+    if bias is not None and bias.dtype == x.dtype:           # strided, or one that wants a gradient itself
+        fixed = bias.detach().contiguous()
+        y = ops.block_fp8_linear(x, weight, weight_scale, fixed, -1)
+        if y is not None:
+            # (a zero that carries the gradient; an infinity among the bias would make it a NaN)
+            return y + (bias - fixed).nan_to_num() if _differentiable(bias) else y
+    elif bias is not None:                                   # of another dtype: added before the result is rounded
+        y = ops.block_fp8_linear(x.float(), weight, weight_scale, None, _FLOATS[x.dtype])
+        if y is not None:
+            return (y + bias).to(x.dtype)
     # a tangent, a transform or a dispatch mode wants to see the operators
     with torch.no_grad():
         a = F.pad(x.abs(), (0, -k % BLOCK)).unflatten(-1, (-1, BLOCK)).amax(-1).float().clamp(min=2.0 ** -100)
@@ -107,7 +119,8 @@ def block_fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.
         values = q * (a / 448).repeat_interleave(BLOCK, dim=-1)[..., :k]
         dense = block_fp8_dequantize(weight, weight_scale)
     xf = x.float()
-    return torch.matmul(xf + (values - xf).detach(), dense.t()).to(x.dtype)
+    y = torch.matmul(xf + (values - xf).detach(), dense.t())
+    return (y if bias is None else y + bias).to(x.dtype)
 
 
 def _exact_product(x, weight, scale, grad_dtype):

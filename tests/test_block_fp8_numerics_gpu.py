@@ -156,3 +156,36 @@ def test_experts_that_no_kernel_takes_round_once_too(dtype):
     assert (got.double().cpu() - exactly).norm() <= unit * exactly.norm() + 2.0 ** -12 * relu.norm()
     many = expert_case(7, 3, 66, 70, 128, 128, dtype)
     near(bf.block_fp8_experts(*(t.cuda() for t in many)), many, 0, dtype)
+
+
+@pytest.mark.parametrize("m", [1, 6, 40])
+@pytest.mark.parametrize("dtype", HALF, ids=ids)
+def test_a_bias_is_added_before_the_result_is_rounded(dtype, m):
+    """Of another type, strided, or one that is trained itself: sums that are exact in float32 but for the bias' own last bits."""
+    g = gen(m)
+    x, (w, ws) = u.activations(g, m, 512, dtype), u.weight(g, 200, 512, base=-8)
+    product = x.double() @ u.dense(w, ws).t()
+    xd, wd, sd = x.cuda(), w.cuda(), ws.cuda()
+    long = (torch.randint(-1 << 10, 1 << 10, (200,), generator=g) * 2.0 ** -8).float()    # exact beside multiples of 2^-10
+    for bias in (long, long.double()):
+        assert torch.equal(bf.block_fp8_linear(xd, wd, sd, bias.cuda()).cpu(), (product + bias.double()).to(dtype))
+    short = (torch.randint(-64, 65, (200,), generator=g) * 2.0 ** -6).to(dtype)
+    short[3] = -float("inf")
+    want = (product + short.double()).to(dtype)
+    strided = torch.stack([short, short], dim=1).cuda()[:, 0]
+    assert torch.equal(bf.block_fp8_linear(xd, wd, sd, strided).cpu(), want)
+    v = torch.randint(-8, 9, (m, 200), generator=g).to(dtype).cuda()
+    for bias in (short, long):
+        leaf, row = bias.cuda().requires_grad_(), xd.clone().requires_grad_()
+        for at in (xd, row):
+            y = bf.block_fp8_linear(at, wd, sd, leaf)
+            assert torch.equal(y.detach().cpu(), (product + bias.double()).to(dtype))
+            grads = torch.autograd.grad(y, (leaf, at) if at.requires_grad else (leaf,), v)
+            finite = bias.isfinite()
+            assert grads[0].dtype == bias.dtype and torch.equal(grads[0].cpu()[finite], v.cpu().double().sum(0).to(bias.dtype)[finite])
+            if at.requires_grad:
+                assert torch.equal(grads[1].cpu(), (v.cpu().double() @ u.dense(w, ws)).to(dtype))
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(short.cuda(), torch.full((200,), 2.0, dtype=dtype, device="cuda"))
+        y = torch.autograd.forward_ad.unpack_dual(bf.block_fp8_linear(xd, wd, sd, dual))
+    assert torch.equal(y.primal.cpu(), want) and (y.tangent[:, torch.arange(200) != 3] == 2).all()
