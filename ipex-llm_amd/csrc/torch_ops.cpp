@@ -306,7 +306,8 @@ bool is_block_fp8(const Tensor &w, const Tensor &scale, const Tensor &x, int64_t
 
 // codes and scales of x by row (weight false) or by 128 x 128; undefined tensors when this is not the plain case
 std::pair<Tensor, Tensor> block_fp8_quantize(const Tensor &x_in, bool weight) {
-    if (!on_gpu(x_in) || x_in.dim() < (weight ? 2 : 1) || x_in.numel() == 0 || x_in.size(-1) % 16 || dtype_code(x_in.scalar_type()) < 0) return {};
+    if (!on_gpu(x_in) || x_in.dim() < (weight ? 2 : 1) || x_in.numel() == 0 || x_in.size(-1) % 16 || dtype_code(x_in.scalar_type()) < 0 ||
+        !nothing_watches(x_in)) return {};
     const Tensor x = whole_rows(x_in.detach());
     const int64_t K = x.size(-1), N = weight ? x.size(-2) : 1;
     c10::DeviceGuard guard(x.device());

@@ -60,7 +60,24 @@ def _quantized(x, weight, what):
         if weight:
             shape[-2] = _blocks(shape[-2])
         return torch.empty(x.shape, dtype=E4M3, device=x.device), torch.empty(shape, dtype=torch.float32, device=x.device)
-    return ops.block_fp8_quantize(x, weight)
+    both = ops.block_fp8_quantize(x, weight)
+    return _quantize_steps(x.detach(), weight) if both is None else both
+
+
+def _spread(scale, shape, weight):
+    """One scale for each value of [.., R, K]."""
+    s = scale.repeat_interleave(BLOCK, dim=-1)[..., :shape[-1]]
+    return s.repeat_interleave(BLOCK, dim=-2)[..., :shape[-2], :] if weight else s
+
+
+def _quantize_steps(x, weight):
+    """The quantizers as torch operators, for a transform, a trace or a dispatch mode, which want to see them.  The quotient is rounded from
+    float64 to float32 and then to a code, as the kernels do."""
+    pad = F.pad(x.abs(), (0, -x.shape[-1] % BLOCK, 0, -x.shape[-2] % BLOCK) if weight else (0, -x.shape[-1] % BLOCK))
+    a = pad.unflatten(-1, (-1, BLOCK)).amax(-1)
+    a = (a.unflatten(-2, (-1, BLOCK)).amax(-2) if weight else a).float().clamp(min=2.0 ** -100)
+    # (by a tensor: a division by a number is a product with its reciprocal on the GPU, a unit off)
+    return (x.double() * 448 / _spread(a, x.shape, weight).double()).float().to(E4M3), a / torch.full_like(a, 448.0)
 
 
 def block_fp8_quantize(x: torch.Tensor):
@@ -78,11 +95,9 @@ def block_fp8_dequantize(codes: torch.Tensor, scale: torch.Tensor, dtype=torch.f
     """What block_fp8_quantize (scale [.., R, ceil(K / 128)]) or block_fp8_quantize_weight made, as numbers; on any device."""
     invalidInputError(codes.dtype == E4M3 and codes.dim() == scale.dim() and scale.shape[-1] == _blocks(codes.shape[-1]),
                       "block_fp8_dequantize: codes and scales do not fit together")
-    s = scale.repeat_interleave(BLOCK, dim=-1)[..., :codes.shape[-1]]
-    if codes.dim() > 1 and scale.shape[-2] != codes.shape[-2]:
-        invalidInputError(scale.shape[-2] == _blocks(codes.shape[-2]), "block_fp8_dequantize: codes and scales do not fit together")
-        s = s.repeat_interleave(BLOCK, dim=-2)[..., :codes.shape[-2], :]
-    return (codes.float() * s).to(dtype)
+    weight = codes.dim() > 1 and scale.shape[-2] != codes.shape[-2]
+    invalidInputError(not weight or scale.shape[-2] == _blocks(codes.shape[-2]), "block_fp8_dequantize: codes and scales do not fit together")
+    return (codes.float() * _spread(scale, codes.shape, weight)).to(dtype)
 
 
 def block_fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bias: torch.Tensor = None):
@@ -114,9 +129,7 @@ def block_fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.
             return (y + bias).to(x.dtype)
     # a tangent, a transform or a dispatch mode wants to see the operators
     with torch.no_grad():
-        a = F.pad(x.abs(), (0, -k % BLOCK)).unflatten(-1, (-1, BLOCK)).amax(-1).float().clamp(min=2.0 ** -100)
-        q = (x.double() * 448 / a.repeat_interleave(BLOCK, dim=-1)[..., :k].double()).float().to(E4M3).float()
-        values = q * (a / 448).repeat_interleave(BLOCK, dim=-1)[..., :k]
+        values = block_fp8_dequantize(*_quantize_steps(x, False))
         dense = block_fp8_dequantize(weight, weight_scale)
     xf = x.float()
     y = torch.matmul(xf + (values - xf).detach(), dense.t())

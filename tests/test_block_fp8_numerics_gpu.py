@@ -189,3 +189,33 @@ def test_a_bias_is_added_before_the_result_is_rounded(dtype, m):
         dual = torch.autograd.forward_ad.make_dual(short.cuda(), torch.full((200,), 2.0, dtype=dtype, device="cuda"))
         y = torch.autograd.forward_ad.unpack_dual(bf.block_fp8_linear(xd, wd, sd, dual))
     assert torch.equal(y.primal.cpu(), want) and (y.tangent[:, torch.arange(200) != 3] == 2).all()
+
+
+class _Seen(torch.utils._python_dispatch.TorchDispatchMode):
+    """Counts the operators that a call shows."""
+
+    def __init__(self):
+        super().__init__()
+        self.names = []
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        self.names.append(str(func))
+        return func(*args, **(kwargs or {}))
+
+
+@pytest.mark.parametrize("weight", [False, True], ids=["rows", "weight"])
+@pytest.mark.parametrize("dtype", ALL, ids=ids)
+def test_quantizers_under_a_trace_a_dispatch_mode_and_vmap(dtype, weight):
+    call = bf.block_fp8_quantize_weight if weight else bf.block_fp8_quantize
+    g = gen(31)
+    x, other = ((torch.randn((6, 130, 272), generator=g) * 3).to(dtype).cuda() for _ in range(2))
+    want = [t.float() for t in call(x)]
+    traced = torch.jit.trace(lambda t: tuple(v.float() for v in call(t)), other, check_trace=False)
+    assert all(torch.equal(a, b) for a, b in zip(traced(x), want))
+    with _Seen() as mode:
+        got = call(x)
+    assert len(mode.names) > 4 and all(torch.equal(a.float(), b) for a, b in zip(got, want))
+    got = torch.func.vmap(lambda t: tuple(v.float() for v in call(t)))(x)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    leaf = x.float().requires_grad_()
+    assert not any(t.requires_grad for t in call(leaf))
