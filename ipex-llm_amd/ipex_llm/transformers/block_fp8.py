@@ -142,10 +142,10 @@ def _exact_product(x, weight, scale, grad_dtype):
     return block_fp8_linear(x, weight, scale) if y is None else y
 
 
-def _expert_loop(x, top_k_index, top_k_weights, gate_up, gate_up_scale, down, down_scale, act_fn):
-    """Expert by expert, with what the native call keeps in float32 (g, u, act(g) * u, the pairs' results and their sum) kept so too, and
+def _expert_loop(x, top_k_index, top_k_weights, gate_up, gate_up_scale, down, down_scale, gate):
+    """Expert by expert, h = gate(g | u), with what the native call keeps in float32 (g, u, h, the pairs' results and their sum) kept so too, and
     one rounding.  Where a gradient is wanted below 16-bit rows, the products of the backward take it in their type."""
-    (tokens, top_k), n_exp, inter = top_k_index.shape, gate_up.shape[0], gate_up.shape[1] // 2
+    (tokens, top_k), n_exp = top_k_index.shape, gate_up.shape[0]
     expert = top_k_index.reshape(-1).long()
     expert = expert.masked_fill((expert < 0) | (expert >= n_exp), n_exp)
     order = expert.argsort(stable=True)
@@ -154,12 +154,19 @@ def _expert_loop(x, top_k_index, top_k_weights, gate_up, gate_up_scale, down, do
     for e in range(n_exp):
         if counts[e]:
             gu = _exact_product(rows[e], gate_up[e], gate_up_scale[e], x.dtype)
-            ys.append(_exact_product(act_fn(gu[:, :inter]) * gu[:, inter:], down[e], down_scale[e], x.dtype))
+            ys.append(_exact_product(gate(gu), down[e], down_scale[e], x.dtype))
     if not ys:
         return torch.zeros_like(x)
     order = order[:len(order) - counts[n_exp]]
     y = torch.cat(ys) * top_k_weights.reshape(-1)[order].float().unsqueeze(-1)
     return y.new_zeros((tokens * top_k, x.shape[1])).index_copy(0, order, y).view(tokens, top_k, -1).sum(1).to(x.dtype)
+
+
+def _gated(act_fn):
+    def gate(gu):
+        g, u = gu.chunk(2, dim=-1)
+        return act_fn(g) * u
+    return gate
 
 
 _ACTS = {0: F.silu, 1: lambda g: F.gelu(g, approximate="tanh")}
@@ -190,7 +197,7 @@ def block_fp8_experts(x: torch.Tensor, top_k_index: torch.Tensor, top_k_weights:
                       and not top_k_index.is_floating_point() and top_k_index.dtype != torch.bool
                       and top_k_index.device == x.device and top_k_weights.device == x.device,
                       f"{what}: whole indices and weights [tokens, k] on x's GPU")
-    return _expert_loop(x, top_k_index, top_k_weights, gate_up, gate_up_scale, down, down_scale, _ACTS[act])
+    return _expert_loop(x, top_k_index, top_k_weights, gate_up, gate_up_scale, down, down_scale, _gated(_ACTS[act]))
 
 
 class _KeepsFormat(nn.Module):
@@ -288,17 +295,22 @@ class BlockFP8Experts(_KeepsFormat):
         invalidInputError(hidden_dim % 16 == 0 and intermediate_dim % BLOCK == 0,
                           "BlockFP8Experts needs hidden_dim to be a multiple of 16 and intermediate_dim of 128")
         self.num_experts, self.hidden_dim, self.intermediate_dim, self.act_fn = num_experts, hidden_dim, intermediate_dim, act_fn
+        self.own_gate = None                             # h of (g | u), where it is not act_fn(g) * u (moe.gate_of)
         for name, n, k in (("gate_up_proj", 2 * intermediate_dim, hidden_dim), ("down_proj", hidden_dim, intermediate_dim)):
             setattr(self, name, _frozen(torch.empty((num_experts, n, k), dtype=E4M3)))
             setattr(self, name + "_scale_inv", _frozen(torch.empty((num_experts, _blocks(n), _blocks(k)), dtype=torch.float32)))
 
     @classmethod
     def from_fused(cls, module, convert_shape_only=False):
-        """From a module with dense or block-scaled `gate_up_proj` and `down_proj` and an `act_fn`."""
+        """From a module with dense or block-scaled `gate_up_proj` and `down_proj` and an `act_fn`, or a gate of its own, which is kept."""
         n_exp, two_i, hidden = module.gate_up_proj.shape
         invalidInputError(tuple(module.down_proj.shape) == (n_exp, hidden, two_i // 2), "gate_up_proj / down_proj shapes do not fit together")
+        from ipex_llm.transformers.moe import gate_of
+        known, gate = gate_of(module)
+        invalidInputError(known, "the experts' gate depends on tensors of the module, which its block-scaled form does not have")
         with torch.device("meta"):
             new = cls(n_exp, hidden, two_i // 2, module.act_fn)
+        new.own_gate = gate
         for name in ("gate_up_proj", "down_proj"):
             w, scale = getattr(module, name).data, getattr(module, name + "_scale_inv", None)
             if scale is None:
@@ -317,6 +329,6 @@ class BlockFP8Experts(_KeepsFormat):
             return torch.zeros_like(hidden_states)
         weights = (self.gate_up_proj, self.gate_up_proj_scale_inv, self.down_proj, self.down_proj_scale_inv)
         act = activation_code(self.act_fn)
-        if act is None:
-            return _expert_loop(hidden_states, top_k_index, top_k_weights, *weights, self.act_fn)
+        if act is None or self.own_gate is not None:
+            return _expert_loop(hidden_states, top_k_index, top_k_weights, *weights, self.own_gate or _gated(self.act_fn))
         return block_fp8_experts(hidden_states, top_k_index, top_k_weights, *weights, act)

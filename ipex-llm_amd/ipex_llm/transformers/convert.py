@@ -252,9 +252,11 @@ def _replace_with_low_bit_linear(model, qtype, modules_to_not_convert=None,
             # parameters instead of the nn.Linear layers per expert that the reference converts one by one
             # (convert.py:469-748 on transformers 4.37): the whole module is replaced.
             from ipex_llm.transformers.low_bit_linear import get_qk_size
-            from ipex_llm.transformers.moe import LowBitExperts
+            from ipex_llm.transformers.moe import LowBitExperts, gate_of
             _, two_i, hidden = module.gate_up_proj.shape
             scaled = is_block_fp8(module, "gate_up_proj") and is_block_fp8(module, "down_proj")
+            if not scaled and not gate_of(module)[0]:
+                continue                                 # a gate that cannot be taken over: the module stays dense
             if scaled or (wants_blocks and hidden % 16 == 0 and two_i % 256 == 0):
                 invalidInputError(qtype == ggml_tensor_qtype["fp8_e4m3"], only_fp8)
                 model._modules[name] = BlockFP8Experts.from_fused(module, convert_shape_only).requires_grad_(False)

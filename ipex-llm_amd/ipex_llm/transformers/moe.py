@@ -10,6 +10,7 @@ sum - or, while there are no more pairs than experts, two launches of the stream
 not take runs as torch operators around the two grouped launches (`_grouped_steps`).
 """
 import array
+import copy
 
 import torch
 import torch.nn as nn
@@ -204,6 +205,27 @@ def activation_code(act_fn):
     return None
 
 
+def gate_of(module):
+    """(known, gate) of a fused experts module.  gate: None where it computes act_fn(g) * u of (g | u), the columns of `gate_up_proj`'s
+    product; else its own `_apply_gate`, which may clamp g and u, add to u, or deal the columns otherwise.  Told by its results on numbers
+    small and large, not by its class.  The gate is bound to a copy of the module without its tensors; where it needs those, known is False."""
+    if not callable(getattr(module, "_apply_gate", None)):
+        return True, None
+    shell = copy.copy(module)
+    shell.__dict__.update(_parameters={}, _buffers={})
+    v = torch.tensor([0.25, 1.0, 3.0, 6.5, 7.5, 11.0, 50.0, 300.0, 1e4], device="cpu")
+    v = torch.cat([-v, torch.zeros(1, device="cpu"), v])
+    g, u = v.repeat_interleave(len(v)), v.repeat(len(v))
+    try:
+        with torch.no_grad():
+            got, plain = shell._apply_gate(torch.cat([g, u]).unsqueeze(0)), shell.act_fn(g) * u
+    except Exception:  # noqa: BLE001
+        return False, None
+    if not isinstance(got, torch.Tensor) or got.device != plain.device or got.shape != (1, len(g)):
+        return False, None
+    return True, None if torch.allclose(got[0].float(), plain.float(), rtol=1e-5, atol=1e-30) else shell._apply_gate
+
+
 class LowBitExperts(nn.Module):
     """The experts of a sparse mixture-of-experts block with low-bit weights.
 
@@ -215,14 +237,14 @@ class LowBitExperts(nn.Module):
     siblings).  This module takes that one's place: each expert's three weights become LowBitLinear layers
     (`gate[e]`, `up[e]`, `down[e]`, so that save_low_bit / load_low_bit carry them like any other), and on the GPU the
     call is one native call (see the head of this file).  With anything else - host tensors, float32 activations,
-    training, an activation the kernels do not know, shapes without a tiled layout - it is the per-expert loop over the
-    LowBitLinear layers."""
+    training, an activation the kernels do not know, a gate of the module's own, shapes without a tiled layout - it is the
+    per-expert loop over the LowBitLinear layers."""
 
     def __init__(self, num_experts, hidden_dim, intermediate_dim, qtype, act_fn, enable_scale_search=False):
         super().__init__()
         from ipex_llm.transformers.low_bit_linear import LowBitLinear
         self.num_experts, self.hidden_dim, self.intermediate_dim, self.qtype = num_experts, hidden_dim, intermediate_dim, qtype
-        self.act_fn = act_fn
+        self.act_fn, self.own_gate = act_fn, None
 
         def layers(in_f, out_f):
             return nn.ModuleList([LowBitLinear(in_f, out_f, qtype, bias=False, enable_scale_search=enable_scale_search)
@@ -239,7 +261,10 @@ class LowBitExperts(nn.Module):
         n_exp, two_i, hidden = gate_up.shape
         inter = two_i // 2
         invalidInputError(tuple(down.shape) == (n_exp, hidden, inter), "gate_up_proj / down_proj shapes do not fit together")
+        known, gate = gate_of(module)
+        invalidInputError(known, "the experts' gate depends on tensors of the module, which its low-bit form does not have")
         new = cls(n_exp, hidden, inter, qtype, module.act_fn, enable_scale_search)
+        new.own_gate = gate
         device = gate_up.device
 
         def param(w, in_features):
@@ -259,7 +284,7 @@ class LowBitExperts(nn.Module):
         """Pointer tables of the three projections, built on first use and again when a weight has moved; None where the
         call is not one for the grouped kernels."""
         if not x.is_cuda or x.dtype not in (torch.float16, torch.bfloat16) or self.training \
-                or activation_code(self.act_fn) is None:
+                or self.own_gate is not None or activation_code(self.act_fn) is None:
             return None
         tables = self.__dict__["_tables"]
         if tables is None or not all(t.holds(x.device) for t in tables):
@@ -292,6 +317,7 @@ class LowBitExperts(nn.Module):
             if tok.numel() == 0:
                 continue
             xe = hidden_states[tok]
-            he = self.down[e](self.act_fn(self.gate[e](xe)) * self.up[e](xe))
+            g, u = self.gate[e](xe), self.up[e](xe)
+            he = self.down[e](self.act_fn(g) * u if self.own_gate is None else self.own_gate(torch.cat([g, u], dim=-1)))
             out.index_add_(0, tok, (he * top_k_weights[tok, slot, None]).to(out.dtype))
         return out

@@ -210,3 +210,92 @@ def test_plans_hold_for_any_size():
                  lambda: ggml.lowbit_block_fp8_experts_plan(1, 65, 1, 16, 128)):
         with pytest.raises(Exception):
             call()
+
+
+class FusedExperts(nn.Module):
+    """Experts in one module, block-scaled or dense; `limit` and `alpha` change the gate, as some models' do."""
+
+    def __init__(self, e, h, i, limit=None, alpha=None, blocks=True):
+        super().__init__()
+        gen = torch.Generator().manual_seed(5)
+        self.act_fn, self.limit, self.alpha = nn.SiLU(), limit, alpha
+        for name, n, k in (("gate_up_proj", 2 * i, h), ("down_proj", h, i)):
+            w, ws = u.random_weight(gen, n, k, lead=(e,))
+            setattr(self, name, nn.Parameter(w if blocks else torch.randn((e, n, k), generator=gen) * 0.05, requires_grad=False))
+            if blocks:
+                setattr(self, name + "_scale_inv", nn.Parameter(ws, requires_grad=False))
+
+    def _apply_gate(self, gu):
+        g, v = gu.chunk(2, dim=-1)
+        if self.limit is not None:
+            g, v = g.clamp(max=self.limit), v.clamp(-self.limit, self.limit)
+        return self.act_fn(g) * v if self.alpha is None else (v + 1) * g * torch.sigmoid(g * self.alpha)
+
+
+GATES = [dict(limit=7.0), dict(limit=7.0, alpha=1.7), dict(limit=500.0), dict(alpha=1.7)]
+
+
+@pytest.mark.parametrize("own", GATES, ids=str)
+def test_experts_keep_a_gate_of_their_own(own, monkeypatch):
+    module = FusedExperts(3, 256, 128, **own).eval()
+    new = ggml_convert_low_bit(nn.Sequential(module).eval(), FP8)[0]
+    assert type(new) is bf.BlockFP8Experts
+    gu = torch.randn((9, 256), generator=torch.Generator().manual_seed(2)) * 30
+    assert torch.equal(new.own_gate(gu), module._apply_gate(gu))
+    held = [v for v in vars(new.own_gate.__self__).values() if isinstance(v, torch.Tensor)]
+    assert not held and not list(new.own_gate.__self__.parameters())      # a gate without the module's weights
+    # (the products by the formula: there is no GPU here)
+    monkeypatch.setattr(bf, "_exact_product", lambda x, w, s, dtype: (x.double() @ u.dense(w, s).t()).float())
+    x, picks = torch.randn((6, 256), generator=torch.Generator().manual_seed(3)) * 8, torch.tensor([[0, 2]] * 5 + [[1, 7]])
+    p, want = torch.full((6, 2), 0.5), torch.zeros((6, 256))
+    for e in range(3):
+        t, j = torch.where(picks == e)
+        gu = (x[t].double() @ u.dense(module.gate_up_proj[e], module.gate_up_proj_scale_inv[e]).t()).float()
+        want.index_add_(0, t, (module._apply_gate(gu).double() @ u.dense(module.down_proj[e], module.down_proj_scale_inv[e]).t()).float() * 0.5)
+    assert torch.allclose(new(x, picks, p), want, rtol=1e-4, atol=1e-4)
+
+
+def test_experts_with_the_plain_gate_or_none_run_in_the_native_call():
+    class NoGate(FusedExperts):
+        _apply_gate = None
+    for module in (FusedExperts(2, 256, 128), NoGate(2, 256, 128, limit=7.0)):
+        assert ggml_convert_low_bit(nn.Sequential(module), FP8)[0].own_gate is None
+
+
+class _GateOfTensors(FusedExperts):
+    def __init__(self, *args, **kwargs):
+        super().__init__(*args, **kwargs)
+        self.bound = nn.Parameter(torch.ones(1), requires_grad=False)
+
+    def _apply_gate(self, gu):
+        g, v = gu.chunk(2, dim=-1)
+        return self.act_fn(g) * v.clamp(max=self.bound)
+
+
+def test_a_gate_that_needs_the_modules_tensors():
+    with pytest.raises(RuntimeError, match="gate depends on tensors"):
+        ggml_convert_low_bit(nn.Sequential(_GateOfTensors(2, 256, 128)), FP8)
+    model = ggml_convert_low_bit(nn.Sequential(_GateOfTensors(2, 256, 128, blocks=False)), 2)
+    assert type(model[0]) is _GateOfTensors                  # dense experts stay as they are
+
+
+@pytest.mark.parametrize("own", GATES[:2], ids=str)
+def test_low_bit_experts_keep_a_gate_of_their_own(own):
+    from ipex_llm.transformers.moe import LowBitExperts
+    module = FusedExperts(3, 256, 128, blocks=False, **own).eval()
+    with torch.device("meta"):
+        shapes = FusedExperts(3, 256, 128, blocks=False, **own).eval()
+    new = LowBitExperts.from_fused(shapes.to("meta"), 2, convert_shape_only=True)
+    for layers, w in ((new.gate, module.gate_up_proj[:, :128]), (new.up, module.gate_up_proj[:, 128:]), (new.down, module.down_proj)):
+        for e in range(3):                                   # (dense layers in their place: there is no GPU here)
+            layers[e] = nn.Linear(*reversed(w[e].shape), bias=False)
+            layers[e].weight.data = w[e].clone()
+    x, picks = torch.randn((6, 256), generator=torch.Generator().manual_seed(3)) * 30, torch.tensor([[0, 2]] * 5 + [[1, 2]])
+    p, want = torch.full((6, 2), 0.5), torch.zeros((6, 256))
+    for e in range(3):
+        t, j = torch.where(picks == e)
+        want.index_add_(0, t, module._apply_gate(x[t] @ module.gate_up_proj[e].t()) @ module.down_proj[e].t() * 0.5)
+    with torch.no_grad():
+        got = new(x, picks, p)
+    assert torch.allclose(got, want, rtol=1e-4, atol=1e-4)
+    assert LowBitExperts.from_fused(FusedExperts(3, 256, 128, blocks=False).to("meta"), 2, convert_shape_only=True).own_gate is None
