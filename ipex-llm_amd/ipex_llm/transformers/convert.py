@@ -47,6 +47,29 @@ def is_block_fp8(module, name="weight") -> bool:
     return isinstance(w, torch.Tensor) and w.dtype == torch.float8_e4m3fn and isinstance(getattr(module, name + "_scale_inv", None), torch.Tensor)
 
 
+def check_block_fp8(module, full_name, names):
+    """Refuses a layer of a block-scaled checkpoint (`names`: its weights that is_block_fp8 knows) that computes something else than the
+    product of block_fp8.py: other blocks, a fixed scale of the activations, groups of columns, tensors of its own."""
+    tensors = {n: t for n, t in [*module._parameters.items(), *module._buffers.items()] if t is not None}
+    if not names:
+        codes = [n for n, t in tensors.items() if t.dtype in (torch.float8_e4m3fn, torch.float8_e5m2)]
+        scales = [n for n in tensors if any(n.startswith(c + "_scale") for c in codes)]
+        invalidInputError(not scales, f"{full_name}: fp8 codes with {scales}; those with a scale for each 128 x 128, `{(codes or ['weight'])[0]}"
+                                      "_scale_inv`, convert (modules_to_not_convert leaves a layer out)")
+        return
+    why = f"{full_name}: a block-scaled layer converts"
+    block, groups = getattr(module, "block_size", None), getattr(module, "n_groups", 1)
+    invalidInputError(block is None or tuple(block) == (128, 128), f"{why} with a scale for each 128 x 128, not {block}")
+    invalidInputError(getattr(module, "activation_scheme", "dynamic") == "dynamic",
+                      f"{why} with activation_scheme='dynamic': activations are quantized by their own blocks")
+    invalidInputError(groups == 1, f"{why} where all of x meets all of the weight, not in {groups} groups")
+    own = {"bias"}.union(names, (n + "_scale_inv" for n in names))
+    if "weight" not in names:
+        own |= {"gate_up_proj", "down_proj"}
+    more = [n for n in tensors if n not in own]
+    invalidInputError(not more, f"{why} with weight, scales and bias; it holds {more} beside them (modules_to_not_convert leaves it out)")
+
+
 def is_linear_module(module):
     """(is_linear, (in_features, out_features, mp_group)): nn.Linear and 4-bit GPTQ / AWQ layers; the
     vLLM / DeepSpeed layer classes of the reference (convert.py:138-232) are not handled."""
@@ -165,6 +188,9 @@ def _replace_with_low_bit_linear(model, qtype, modules_to_not_convert=None,
 
         if isinstance(module, (BlockFP8Linear, BlockFP8Experts)):
             continue
+        scaled = [n for n in ("weight", "gate_up_proj", "down_proj") if is_block_fp8(module, n)]
+        if isinstance(module, nn.Linear) or is_fused_experts(module):
+            check_block_fp8(module, full_module_name, scaled)
 
         if is_linear and not isinstance(module, (LowBitLinear, FP16Linear, BF16Linear)):
             in_features, out_features, mp_group = linear_args
@@ -254,7 +280,6 @@ def _replace_with_low_bit_linear(model, qtype, modules_to_not_convert=None,
             from ipex_llm.transformers.low_bit_linear import get_qk_size
             from ipex_llm.transformers.moe import LowBitExperts, gate_of
             _, two_i, hidden = module.gate_up_proj.shape
-            scaled = is_block_fp8(module, "gate_up_proj") and is_block_fp8(module, "down_proj")
             if not scaled and not gate_of(module)[0]:
                 continue                                 # a gate that cannot be taken over: the module stays dense
             if scaled or (wants_blocks and hidden % 16 == 0 and two_i % 256 == 0):

@@ -274,6 +274,8 @@ class _GateOfTensors(FusedExperts):
 
 def test_a_gate_that_needs_the_modules_tensors():
     with pytest.raises(RuntimeError, match="gate depends on tensors"):
+        bf.BlockFP8Experts.from_fused(_GateOfTensors(2, 256, 128))
+    with pytest.raises(RuntimeError, match="holds .'bound'"):
         ggml_convert_low_bit(nn.Sequential(_GateOfTensors(2, 256, 128)), FP8)
     model = ggml_convert_low_bit(nn.Sequential(_GateOfTensors(2, 256, 128, blocks=False)), 2)
     assert type(model[0]) is _GateOfTensors                  # dense experts stay as they are
@@ -299,3 +301,42 @@ def test_low_bit_experts_keep_a_gate_of_their_own(own):
         got = new(x, picks, p)
     assert torch.allclose(got, want, rtol=1e-4, atol=1e-4)
     assert LowBitExperts.from_fused(FusedExperts(3, 256, 128, blocks=False).to("meta"), 2, convert_shape_only=True).own_gate is None
+
+
+def held(module, **more):
+    for name, v in more.items():
+        setattr(module, name, nn.Parameter(v, requires_grad=False) if isinstance(v, torch.Tensor) else v)
+    return module
+
+
+OTHER_FORMS = [
+    ("dynamic", lambda: held(scaled_linear(256, 256), activation_scheme="static")),
+    ("activation_scale", lambda: held(scaled_linear(256, 256), activation_scale=torch.ones(1))),
+    ("2 groups", lambda: held(scaled_linear(256, 128), n_groups=2)),
+    ("128 x 128, not", lambda: held(scaled_linear(64, 64), block_size=(64, 64))),
+    ("rotation", lambda: held(scaled_linear(256, 256), rotation=torch.ones(256))),
+    ("dynamic", lambda: held(FusedExperts(2, 256, 128), activation_scheme="static")),
+    ("down_proj_activation_scale", lambda: held(FusedExperts(2, 256, 128), down_proj_activation_scale=torch.ones(2))),
+    ("gate_up_proj_bias", lambda: held(FusedExperts(2, 256, 128), gate_up_proj_bias=torch.ones(2, 256))),
+    ("weight_scale'", lambda: held(nn.Linear(256, 256), weight=torch.zeros(256, 256).to(u.E4M3), weight_scale=torch.ones(1))),
+]
+
+
+@pytest.mark.parametrize("message,make", OTHER_FORMS, ids=[f"{i}-{m}" for i, (m, _) in enumerate(OTHER_FORMS)])
+def test_other_forms_of_fp8_checkpoints_are_refused(message, make):
+    with pytest.raises(RuntimeError, match=message):
+        ggml_convert_low_bit(nn.ModuleDict({"layer": make()}), FP8)
+    model = ggml_convert_low_bit(nn.ModuleDict({"layer": make(), "other": scaled_linear(128, 128)}), FP8, modules_to_not_convert=["layer"])
+    assert type(model["layer"]) in (nn.Linear, FusedExperts) and type(model["other"]) is bf.BlockFP8Linear
+
+
+def test_block_scaled_layers_with_a_named_form_convert():
+    lin = held(scaled_linear(200, 272), activation_scheme="dynamic", block_size=[128, 128], n_groups=1)
+    powers = torch.exp2(torch.randint(-9, -5, (2, 3)).float())
+    lin.weight_scale_inv = nn.Parameter(powers.to(torch.float8_e8m0fnu), requires_grad=False)     # scales held as their exponents
+    new = ggml_convert_low_bit(nn.Sequential(lin), FP8)[0]
+    assert type(new) is bf.BlockFP8Linear and torch.equal(new.weight_scale_inv, powers)
+    dense = nn.Linear(256, 256)
+    dense.register_buffer("weight_scale_factor", torch.ones(1))           # not fp8: nothing of a checkpoint's
+    from ipex_llm.transformers.convert import check_block_fp8
+    check_block_fp8(dense, "dense", [])
