@@ -192,6 +192,8 @@ def _replace_with_low_bit_linear(model, qtype, modules_to_not_convert=None,
         if isinstance(module, nn.Linear) or is_fused_experts(module):
             check_block_fp8(module, full_module_name, scaled)
 
+        if is_linear and getattr(module, "n_groups", 1) != 1:
+            continue   # a linear in groups, each of which meets its own columns of x, stays as it is
         if is_linear and not isinstance(module, (LowBitLinear, FP16Linear, BF16Linear)):
             in_features, out_features, mp_group = linear_args
             optimize_lm_head = (is_lm_head(name, model_config, out_features)
@@ -280,8 +282,8 @@ def _replace_with_low_bit_linear(model, qtype, modules_to_not_convert=None,
             from ipex_llm.transformers.low_bit_linear import get_qk_size
             from ipex_llm.transformers.moe import LowBitExperts, gate_of
             _, two_i, hidden = module.gate_up_proj.shape
-            if not scaled and not gate_of(module)[0]:
-                continue                                 # a gate that cannot be taken over: the module stays dense
+            if not scaled and (not gate_of(module)[0] or any(getattr(module, n + "_bias", None) is not None for n in ("gate_up_proj", "down_proj"))):
+                continue                                 # a gate that cannot be taken over, biases: the module stays dense
             if scaled or (wants_blocks and hidden % 16 == 0 and two_i % 256 == 0):
                 invalidInputError(qtype == ggml_tensor_qtype["fp8_e4m3"], only_fp8)
                 model._modules[name] = BlockFP8Experts.from_fused(module, convert_shape_only).requires_grad_(False)

@@ -340,3 +340,12 @@ def test_block_scaled_layers_with_a_named_form_convert():
     dense.register_buffer("weight_scale_factor", torch.ones(1))           # not fp8: nothing of a checkpoint's
     from ipex_llm.transformers.convert import check_block_fp8
     check_block_fp8(dense, "dense", [])
+
+
+def test_dense_layers_that_compute_more_than_a_product_stay_dense():
+    with torch.device("meta"):
+        grouped, biased = held(nn.Linear(256, 128), n_groups=2), held(FusedExperts(2, 256, 128, blocks=False), gate_up_proj_bias=torch.ones(2, 256))
+        for qtype, block_fp8 in ((FP8, True), (FP8, False), (2, False)):
+            model = nn.ModuleDict({"grouped": grouped, "experts": biased, "other": nn.Linear(256, 128)})
+            model = ggml_convert_low_bit(model, qtype, convert_shape_only=True, block_fp8=block_fp8)
+            assert model["grouped"] is grouped and model["experts"] is biased and type(model["other"]) is not nn.Linear
