@@ -95,6 +95,11 @@ def block_fp8_layers(state_dict):
     return names, any(n.endswith("q_proj") for n in names)
 
 
+def unmerged_attentions(state_dict):
+    """Names of the modules whose q_proj was saved by itself, not as part of a qkv_proj."""
+    return {k.rpartition("q_proj.")[0].rstrip(".") for k in state_dict if ".q_proj." in "." + k}
+
+
 def load_low_bit(model, model_path):
     """Turns `model` (on cpu or meta) into the low-bit model saved under model_path."""
     low_bit = low_bit_sanity_check(model_path)
@@ -105,10 +110,9 @@ def load_low_bit(model, model_path):
     if low_bit:
         from ipex_llm.transformers.convert import ggml_convert_low_bit
         qtype = ggml_tensor_qtype[low_bit]
-        block_fp8, apart = block_fp8_layers(state_dict)
         model = ggml_convert_low_bit(model, qtype=qtype, convert_shape_only=True,
                                      modules_to_not_convert=unconverted_linears(state_dict),
-                                     disable_optimize_pre=apart, block_fp8=block_fp8)
+                                     keep_apart=unmerged_attentions(state_dict), block_fp8=block_fp8_layers(state_dict)[0])
     for param_name, param in state_dict.items():
         _assign(model, param_name, param)
     if low_bit:

@@ -330,11 +330,11 @@ def is_fused_experts(module):
 _MERGE_QKV_MODEL_TYPES = ("llama", "mistral", "qwen2", "gemma", "gemma2", "minicpm", "stablelm", "mllama")
 
 
-def _optimize_pre(model, qtype=None):
+def _optimize_pre(model, qtype=None, keep_apart=()):
     """Of the reference's pre-conversion passes (convert.py:880-1076) the one that belongs to the linear
     path: q_proj / k_proj / v_proj become one `qkv_proj`, so that a decode step streams them in one launch
     (convert.py:996-999 for Llama; the merge itself is models/common.py:40-52).  GPTQ checkpoints are left
-    alone, as in the reference (convert.py:954-960)."""
+    alone, as in the reference (convert.py:954-960), and so are the modules named in `keep_apart`."""
     config = getattr(model, "config", None)
     model_type = getattr(config, "model_type", None)
     if model_type not in _MERGE_QKV_MODEL_TYPES:
@@ -343,8 +343,8 @@ def _optimize_pre(model, qtype=None):
     if (qcfg.get("quant_method") if isinstance(qcfg, dict) else getattr(qcfg, "quant_method", None)) == "gptq":
         return model
     from ipex_llm.transformers.models.common import merge_qkv_base
-    for module in list(model.modules()):
-        if module.__class__.__name__.endswith("Attention"):
+    for name, module in list(model.named_modules()):
+        if module.__class__.__name__.endswith("Attention") and name not in keep_apart:
             merge_qkv_base(module, module.__class__)
     return model
 
@@ -385,7 +385,8 @@ def ggml_convert_low_bit(model, qtype, optimize_model=True,
                          embedding_qtype=None,
                          mixed_precision=False,
                          disable_optimize_pre=False,
-                         block_fp8=False):
+                         block_fp8=False,
+                         keep_apart=()):
     invalidInputError(not block_fp8 or qtype == ggml_tensor_qtype["fp8_e4m3"],
                       "block_fp8 makes e4m3 weights: use it with fp8_e4m3")
     if qtype in ggml_tensor_qtype.values():
@@ -396,7 +397,7 @@ def ggml_convert_low_bit(model, qtype, optimize_model=True,
     modules_to_not_convert = [] if modules_to_not_convert is None else modules_to_not_convert
 
     if optimize_model and not disable_optimize_pre:
-        model = _optimize_pre(model, qtype)
+        model = _optimize_pre(model, qtype, keep_apart)
 
     model_config = getattr(model, "config", None)
     enable_scale_search = use_scale_search(model_config, qtype)

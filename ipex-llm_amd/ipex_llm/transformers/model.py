@@ -170,16 +170,16 @@ class _BaseAutoModelClass:
                           " serialize the model using save_low_bit first.")
         invalidInputError(low_bit in ggml_tensor_qtype, f"Unknown bigdl_transformers_low_bit value: {low_bit}")
         qtype = ggml_tensor_qtype[low_bit]
-        from ipex_llm.optimize import block_fp8_layers, unconverted_linears
+        from ipex_llm.optimize import block_fp8_layers, unconverted_linears, unmerged_attentions
         state_dict = torch.load(os.path.join(pretrained_model_name_or_path, PYTORCH_MODEL_NAME),
                                 weights_only=True)
         with torch.device("meta"):
             model = cls.HF_Model.from_config(config)
         skip = list(modules_to_not_convert or []) + unconverted_linears(state_dict)
-        block_fp8, apart = block_fp8_layers(state_dict)
         model = ggml_convert_low_bit(model, qtype, optimize_model, device="meta",
                                      convert_shape_only=True, modules_to_not_convert=skip,
-                                     embedding_qtype=embedding_qtype, disable_optimize_pre=apart, block_fp8=block_fp8)
+                                     embedding_qtype=embedding_qtype, keep_apart=unmerged_attentions(state_dict),
+                                     block_fp8=block_fp8_layers(state_dict)[0])
         keys_file = os.path.join(pretrained_model_name_or_path, "load_keys.json")
         if os.path.isfile(keys_file):
             with open(keys_file) as f:

@@ -349,3 +349,32 @@ def test_dense_layers_that_compute_more_than_a_product_stay_dense():
             model = nn.ModuleDict({"grouped": grouped, "experts": biased, "other": nn.Linear(256, 128)})
             model = ggml_convert_low_bit(model, qtype, convert_shape_only=True, block_fp8=block_fp8)
             assert model["grouped"] is grouped and model["experts"] is biased and type(model["other"]) is not nn.Linear
+
+
+def tiny_llama():
+    from transformers import LlamaConfig, LlamaForCausalLM
+    torch.manual_seed(4)
+    return LlamaForCausalLM(LlamaConfig(hidden_size=256, intermediate_size=384, num_hidden_layers=3, num_attention_heads=4, num_key_value_heads=2,
+                                        vocab_size=64)).eval()
+
+
+@pytest.mark.parametrize("apart", [False, True], ids=["merged", "disable_optimize_pre"])
+def test_a_model_with_some_block_scaled_layers_saves_and_loads(apart, tmp_path):
+    """Layer 1's projections block-scaled, the others' q, k and v dense: merged where they may be, layer by layer."""
+    from ipex_llm import optimize_model
+    from ipex_llm.optimize import load_low_bit, unmerged_attentions
+    model = tiny_llama()
+    for part in (model.model.layers[1].self_attn, model.model.layers[1].mlp):
+        for name, lin in list(part.named_children()):
+            if isinstance(lin, nn.Linear):
+                setattr(part, name, scaled_linear(*lin.weight.shape))
+    model = optimize_model(model, "fp8_e4m3", modules_to_not_convert=["layers.0", "layers.2", "lm_head"], disable_optimize_pre=apart)
+    assert hasattr(model.model.layers[0].self_attn, "qkv_proj") != apart and not hasattr(model.model.layers[1].self_attn, "qkv_proj")
+    model.save_low_bit(str(tmp_path))
+    again = load_low_bit(tiny_llama(), str(tmp_path))
+    want, got = model.state_dict(), again.state_dict()
+    assert set(want) == set(got) and all(torch.equal(got[k].float(), v.float()) and got[k].dtype == v.dtype for k, v in want.items())
+    assert type(again.model.layers[1].self_attn.q_proj) is bf.BlockFP8Linear and type(again.model.layers[2].mlp.up_proj) is nn.Linear
+    every = {f"model.layers.{i}.self_attn" for i in range(3)}
+    assert unmerged_attentions(want) == (every if apart else {"model.layers.1.self_attn"})
+    assert unmerged_attentions({"q_proj.weight": 0, "a.xq_proj.weight": 0, "b.q_proj.bias": 0}) == {"", "b"}
