@@ -420,12 +420,14 @@ def ggml_convert_low_bit(model, qtype, optimize_model=True,
 
 
 def convert_bigdl_other_module(model, dtype):
-    """Every leaf that is not one of our linears follows `dtype` (convert.py:1174-1182)."""
+    """Every leaf that is not one of our linears follows `dtype` (convert.py:1174-1182).  One that holds 8-bit floating point codes, a layer
+    of a checkpoint that was left out of the conversion, keeps them: as numbers of another type they would have lost their scales."""
     from ipex_llm.transformers.block_fp8 import BlockFP8Linear
     from ipex_llm.transformers.low_bit_linear import BF16Linear, FP16Linear, LowBitLinear
     for module in model.modules():
         if list(module.children()) == []:
-            if not isinstance(module, (LowBitLinear, FP16Linear, BF16Linear, BlockFP8Linear)):
+            codes = any(p.is_floating_point() and p.element_size() == 1 for p in module.parameters(recurse=False))
+            if not codes and not isinstance(module, (LowBitLinear, FP16Linear, BF16Linear, BlockFP8Linear)):
                 module.to(dtype)
 
 

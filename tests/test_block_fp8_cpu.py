@@ -378,3 +378,13 @@ def test_a_model_with_some_block_scaled_layers_saves_and_loads(apart, tmp_path):
     every = {f"model.layers.{i}.self_attn" for i in range(3)}
     assert unmerged_attentions(want) == (every if apart else {"model.layers.1.self_attn"})
     assert unmerged_attentions({"q_proj.weight": 0, "a.xq_proj.weight": 0, "b.q_proj.bias": 0}) == {"", "b"}
+
+
+def test_layers_left_out_of_the_conversion_keep_their_codes():
+    model = nn.ModuleDict({"left": scaled_linear(128, 256, bias=True), "other": scaled_linear(128, 256), "norm": nn.LayerNorm(256), "experts": FusedExperts(2, 256, 128)})
+    codes, scales = model["left"].weight.data.clone(), model["left"].weight_scale_inv.data.clone()
+    model = ggml_convert_low_bit(model, FP8, torch_dtype=torch.bfloat16, modules_to_not_convert=["left", "experts"])
+    assert model["norm"].weight.dtype == torch.bfloat16 and type(model["other"]) is bf.BlockFP8Linear
+    left = model["left"]
+    assert left.weight.dtype == u.E4M3 and torch.equal(left.weight.float(), codes.float()) and torch.equal(left.weight_scale_inv, scales)
+    assert model["experts"].down_proj.dtype == u.E4M3 and model["experts"].down_proj_scale_inv.dtype == torch.float32
