@@ -42,6 +42,19 @@ def save_low_bit(self, *args, **kwargs):
         json.dump({"all_checkpoint_keys": list(state.keys())}, json_file)
 
 
+def _release_quantizer(model):
+    """A block-scaled checkpoint whose fp8 layers have all been converted is no longer its quantizer's: transformers would refuse
+    model.half() and float(), which keep codes and scales (block_fp8.py)."""
+    from ipex_llm.transformers.block_fp8 import E4M3, BlockFP8Experts, BlockFP8Linear
+    method = getattr(model, "quantization_method", None)
+    if getattr(method, "value", method) != "fp8":
+        return
+    for module in model.modules():
+        if not isinstance(module, (BlockFP8Linear, BlockFP8Experts)) and any(p.dtype == E4M3 for p in module.parameters(recurse=False)):
+            return
+    model.is_quantized, model.hf_quantizer = False, None
+
+
 class _BaseAutoModelClass:
     HF_Model = None
 
@@ -144,6 +157,7 @@ class _BaseAutoModelClass:
                                      mixed_precision=mixed_precision,
                                      disable_optimize_pre=disable_optimize_pre,
                                      block_fp8=block_fp8)
+        _release_quantizer(model)
         model.config.update({"bigdl_transformers_low_bit": q_k, "bigdl_disk_embedding": False})
         model.config.update({"tie_word_embeddings": False})
         model.save_low_bit = types.MethodType(save_low_bit, model)

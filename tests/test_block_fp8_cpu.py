@@ -388,3 +388,57 @@ def test_layers_left_out_of_the_conversion_keep_their_codes():
     left = model["left"]
     assert left.weight.dtype == u.E4M3 and torch.equal(left.weight.float(), codes.float()) and torch.equal(left.weight_scale_inv, scales)
     assert model["experts"].down_proj.dtype == u.E4M3 and model["experts"].down_proj_scale_inv.dtype == torch.float32
+
+
+def write_checkpoint(path, model, apart=("lm_head",)):
+    """A Hugging Face directory whose projections are block-scaled, but for those that `apart` names."""
+    from safetensors.torch import save_file
+    state = {}
+    for name, v in model.state_dict().items():
+        if name.endswith("proj.weight") and not any(a in name for a in apart):
+            codes, state[name + "_scale_inv"] = u.quantize(v, 128)
+            state[name] = codes.float().to(u.E4M3)
+        else:
+            state[name] = v.bfloat16()
+    model.config.architectures, model.config.dtype = [type(model).__name__], torch.bfloat16
+    model.config.quantization_config = {"quant_method": "fp8", "weight_block_size": [128, 128], "activation_scheme": "dynamic",
+                                        "modules_to_not_convert": list(apart)}
+    model.config.save_pretrained(path)
+    save_file({k: v.contiguous() for k, v in state.items()}, str(path / "model.safetensors"), metadata={"format": "pt"})
+    return state
+
+
+@pytest.mark.parametrize("apart", [("lm_head",), ("lm_head", "model.layers.0.self_attn")], ids=["all", "mixed"])
+def test_a_block_scaled_checkpoint_loads_moves_saves_and_loads(apart, tmp_path, monkeypatch):
+    from ipex_llm.transformers import AutoModelForCausalLM
+    held = write_checkpoint(tmp_path, tiny_llama(), apart)
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)          # transformers reads such a checkpoint where a GPU is
+    monkeypatch.setattr(torch.cuda, "get_device_capability", lambda *a: (9, 5))
+    model = AutoModelForCausalLM.from_pretrained(str(tmp_path), load_in_low_bit="fp8_e4m3", torch_dtype=torch.bfloat16,
+                                                 modules_to_not_convert=list(apart))
+    monkeypatch.undo()
+    layers = model.model.layers
+    assert type(layers[0].mlp.up_proj) is bf.BlockFP8Linear and type(layers[1].self_attn.q_proj) is bf.BlockFP8Linear
+    for move, dtype in ((model.half, torch.float16), (model.float, torch.float32), (model.bfloat16, torch.bfloat16)):
+        move()
+        assert model.model.embed_tokens.weight.dtype == dtype
+        for name, v in model.state_dict().items():
+            if name in held and held[name].dtype == u.E4M3:
+                assert v.dtype == u.E4M3 and torch.equal(v.float(), held[name].float())
+                assert torch.equal(model.state_dict()[name + "_scale_inv"], held[name + "_scale_inv"])
+    model.save_low_bit(str(tmp_path / "low"))
+    again = AutoModelForCausalLM.load_low_bit(str(tmp_path / "low"))
+    want, got = model.state_dict(), again.state_dict()
+    assert set(want) == set(got) and all(torch.equal(got[k].float(), v.float()) and got[k].dtype == v.dtype for k, v in want.items())
+    assert again.half().model.embed_tokens.weight.dtype == torch.float16
+
+
+def test_a_checkpoint_with_layers_left_to_its_quantizer_stays_its(tmp_path, monkeypatch):
+    from ipex_llm.transformers import AutoModelForCausalLM
+    write_checkpoint(tmp_path, tiny_llama())
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "get_device_capability", lambda *a: (9, 5))
+    model = AutoModelForCausalLM.from_pretrained(str(tmp_path), load_in_low_bit="fp8_e4m3", torch_dtype=torch.bfloat16,
+                                                 modules_to_not_convert=["lm_head", "layers.2"])
+    with pytest.raises(ValueError, match="half"):
+        model.half()                                         # would turn codes into numbers without their scales
