@@ -395,7 +395,13 @@ def write_checkpoint(path, model, apart=("lm_head",)):
     from safetensors.torch import save_file
     state = {}
     for name, v in model.state_dict().items():
-        if name.endswith("proj.weight") and not any(a in name for a in apart):
+        if v.dim() == 3:                                     # experts, one by one
+            for e, w in enumerate(v):
+                for part, t in zip(("gate_proj", "up_proj"), w.chunk(2)) if name.endswith("gate_up_proj") else (("down_proj", w),):
+                    at = f"{name.rpartition('.')[0]}.{e}.{part}.weight"
+                    codes, state[at + "_scale_inv"] = u.quantize(t, 128)
+                    state[at] = codes.float().to(u.E4M3)
+        elif name.endswith("proj.weight") and not any(a in name for a in apart):
             codes, state[name + "_scale_inv"] = u.quantize(v, 128)
             state[name] = codes.float().to(u.E4M3)
         else:
@@ -442,3 +448,30 @@ def test_a_checkpoint_with_layers_left_to_its_quantizer_stays_its(tmp_path, monk
                                                  modules_to_not_convert=["lm_head", "layers.2"])
     with pytest.raises(ValueError, match="half"):
         model.half()                                         # would turn codes into numbers without their scales
+
+
+def test_a_block_scaled_checkpoint_with_experts_loads_saves_and_loads(tmp_path, monkeypatch):
+    from transformers import Qwen3MoeConfig, Qwen3MoeForCausalLM
+    from ipex_llm.transformers import AutoModelForCausalLM
+    torch.manual_seed(5)
+    dense = Qwen3MoeForCausalLM(Qwen3MoeConfig(hidden_size=256, intermediate_size=384, moe_intermediate_size=128, num_experts=4, num_experts_per_tok=2,
+                                               num_hidden_layers=1, num_attention_heads=4, num_key_value_heads=2, vocab_size=64)).eval()
+    held = write_checkpoint(tmp_path, dense, ("lm_head", "mlp.gate"))
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "get_device_capability", lambda *a: (9, 5))
+    model = AutoModelForCausalLM.from_pretrained(str(tmp_path), load_in_low_bit="fp8_e4m3", torch_dtype=torch.bfloat16,
+                                                 modules_to_not_convert=["lm_head", "mlp.gate"])
+    monkeypatch.undo()
+    experts = model.model.layers[0].mlp.experts
+    assert type(experts) is bf.BlockFP8Experts and experts.own_gate is None
+    for e in range(4):
+        at = f"model.layers.0.mlp.experts.{e}."
+        gate_up = torch.cat([held[at + "gate_proj.weight"].float(), held[at + "up_proj.weight"].float()])
+        assert torch.equal(experts.gate_up_proj[e].float(), gate_up)
+        assert torch.equal(experts.gate_up_proj_scale_inv[e], torch.cat([held[at + p + ".weight_scale_inv"] for p in ("gate_proj", "up_proj")]))
+        assert torch.equal(experts.down_proj[e].float(), held[at + "down_proj.weight"].float())
+        assert torch.equal(experts.down_proj_scale_inv[e], held[at + "down_proj.weight_scale_inv"])
+    model.half().save_low_bit(str(tmp_path / "low"))
+    again = AutoModelForCausalLM.load_low_bit(str(tmp_path / "low"))
+    want, got = model.state_dict(), again.state_dict()
+    assert set(want) == set(got) and all(torch.equal(got[k].float(), v.float()) and got[k].dtype == v.dtype for k, v in want.items())
