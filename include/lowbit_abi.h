@@ -359,6 +359,8 @@ int lowbit_block_fp8_backward(const void *grad, const void *w, const float *w_sc
 /* What these two run as, for a size: plan4 = {rows, columns of a tile (0, 0: the kernel of few rows, that takes x as it is), parts that the
  * sum is split into, groups of waves that share a tile's part}.  `backward`: lowbit_block_fp8_backward. */
 int lowbit_block_fp8_plan(int dtype, int backward, int64_t M, int64_t N, int64_t K, int *plan4);
+/* Waves of a workgroup where lowbit_block_fp8_linear runs the kernel of few rows, 0 where it runs tiles (negative: an error). */
+int lowbit_block_fp8_waves(int dtype, int64_t M, int64_t N, int64_t K);
 /* A mixture-of-experts block: y[t, :] = sum_j topk_weight[t, j] * (Q(act(g) .* u) * down[e]^T), (g | u) = Q(x_t) * gate_up[e]^T, e =
  * topk_ids[t, j]; a pair whose id lies outside [0, n_experts) counts nothing.  gate_up [n_experts, 2 inter, hidden] (gate rows first)
  * and down [n_experts, hidden, inter] are the experts' codes one after the other, their scales likewise; inter is a multiple of 128,
@@ -371,6 +373,8 @@ int lowbit_block_fp8_experts(const void *x, const int64_t *topk_ids, const void 
 /* What it runs as: plan4 = {rows of a tile of the first product, rows and columns of one of the second (0: each pair streams its weights), 1 if a launch
  * of its own places the pairs} */
 int lowbit_block_fp8_experts_plan(int64_t tokens, int top_k, int n_experts, int64_t hidden, int64_t inter, int *plan4);
+/* Waves of a workgroup of its second launch where each pair streams its weights, 0 where the pairs are sorted (negative: an error). */
+int lowbit_block_fp8_experts_waves(int64_t tokens, int top_k, int n_experts, int64_t hidden, int64_t inter);
 
 #ifdef __cplusplus
 }

@@ -61,6 +61,8 @@ int launch_block_fp8_rows(const void *x, int dtype, int64_t rows, int K, uint8_t
 int launch_block_fp8_weight(const void *w, int dtype, int64_t matrices, int N, int K, uint8_t *codes, float *scale, hipStream_t st);
 size_t block_fp8_linear_workspace_bytes(int dtype, int M, int N, int K);
 void block_fp8_linear_plan(int dtype, int M, int N, int K, int *plan4);
+int block_fp8_linear_waves(int dtype, int M, int N, int K);
+int block_fp8_experts_waves(int tokens, int top_k, int n_exp, int H, int I);
 void block_fp8_back_plan(int M, int N, int K, int *plan4);
 void block_fp8_experts_plan(int tokens, int top_k, int n_exp, int H, int I, int *plan4);
 int launch_block_fp8_linear(const void *x, const uint8_t *w, const float *ws, const void *bias, void *y, int dtype, int M, int N, int K,
@@ -802,6 +804,13 @@ int lowbit_block_fp8_plan(int dtype, int backward, int64_t M, int64_t N, int64_t
     return 0;
 }
 
+int lowbit_block_fp8_waves(int dtype, int64_t M, int64_t N, int64_t K) {
+    const char *what = "lowbit_block_fp8_waves";
+    if (int rc = check_block_fp8(what, dtype, true, M, N, K)) return rc;
+    if (M == 0 || N == 0 || K == 0) return fail(LOWBIT_EARG, "%s: sizes must be positive", what);
+    return block_fp8_linear_waves(dtype, (int)M, (int)N, (int)K);
+}
+
 size_t lowbit_block_fp8_backward_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K) {
     if (M <= 0 || N <= 0 || K <= 0 || M >= (1 << 22) || N >= (1 << 23) || K >= (1 << 23) || K % 16) return 0;
     return block_fp8_back_workspace_bytes(dtype, (int)M, (int)N, (int)K);
@@ -834,6 +843,12 @@ int lowbit_block_fp8_experts_plan(int64_t tokens, int top_k, int n_experts, int6
         return fail(LOWBIT_EARG, "lowbit_block_fp8_experts_plan: sizes that lowbit_block_fp8_experts does not take, or plan4 null");
     block_fp8_experts_plan((int)tokens, top_k, n_experts, (int)hidden, (int)inter, plan4);
     return 0;
+}
+
+int lowbit_block_fp8_experts_waves(int64_t tokens, int top_k, int n_experts, int64_t hidden, int64_t inter) {
+    if (tokens <= 0 || !block_fp8_experts_ok(tokens, top_k, n_experts, hidden, inter) || hidden % 16 || inter % 128)
+        return fail(LOWBIT_EARG, "lowbit_block_fp8_experts_waves: sizes that lowbit_block_fp8_experts does not take");
+    return block_fp8_experts_waves((int)tokens, top_k, n_experts, (int)hidden, (int)inter);
 }
 
 int lowbit_block_fp8_experts(const void *x, const int64_t *topk_ids, const void *topk_weight, int weight_dtype, int64_t tokens, int top_k,

@@ -464,10 +464,17 @@ size_t block_fp8_experts_workspace_bytes(int tokens, int top_k, int n_exp, int H
 }
 
 // 16 waves where there are no more workgroups than CUs: two experts of [4096 x 14336] 26 us
+static int down_token_waves(int tokens, int H) { return (int64_t)(H / 16) * tokens <= 256 ? 16 : 8; }
+
+// waves of a workgroup of the second launch where each pair streams its weights; 0 where the pairs are sorted
+int block_fp8_experts_waves(int tokens, int top_k, int n_exp, int H, int I) {
+    return direct(tokens, top_k, n_exp, H, I) ? down_token_waves(tokens, H) : 0;
+}
+
 template <typename AT, typename PT> static void launch_down_token(const ExpertsArgs &p, const PT *weight, AT *out, int tokens, hipStream_t st) {
     const dim3 grid(p.H / 16, tokens);
     const size_t lds = token_down_lds(p.top_k, p.I);
-    if ((int64_t)grid.x * tokens <= 256)
+    if (down_token_waves(tokens, p.H) == 16)
         hipLaunchKernelGGL((block_fp8_expert_down_token_kernel<AT, PT, 16>), grid, dim3(1024), lds, st, p, weight, out);
     else hipLaunchKernelGGL((block_fp8_expert_down_token_kernel<AT, PT, 8>), grid, dim3(512), lds, st, p, weight, out);
 }

@@ -197,6 +197,11 @@ void block_fp8_linear_plan(int dtype, int M, int N, int K, int *plan4) {
     plan4[3] = TILED_FORMS[plan.form].groups;
 }
 
+// waves of a workgroup of the kernel of few rows; 0 where tiles run
+int block_fp8_linear_waves(int dtype, int M, int N, int K) {
+    return takes_few_rows(dtype == DT_F32, M, N, K) ? few_rows_waves(N, fp8_blocks(K)) : 0;
+}
+
 int launch_block_fp8_linear(const void *x, const uint8_t *w, const float *ws, const void *bias, void *y, int dtype, int M, int N, int K,
                             uint8_t *space, hipStream_t st) {
     if (takes_few_rows(dtype == DT_F32, M, N, K)) {

@@ -493,6 +493,26 @@ def lowbit_block_fp8_experts_plan(tokens, top_k, n_experts, hidden, inter):
     return tuple(plan4)
 
 
+_lib.lowbit_block_fp8_waves.argtypes = [c_int, c_int64, c_int64, c_int64]
+_lib.lowbit_block_fp8_waves.restype = c_int
+_lib.lowbit_block_fp8_experts_waves.argtypes = [c_int64, c_int, c_int, c_int64, c_int64]
+_lib.lowbit_block_fp8_experts_waves.restype = c_int
+
+
+def lowbit_block_fp8_waves(dtype, m, n, k):
+    """Waves of a workgroup of the kernel of few rows, 0 where lowbit_block_fp8_linear runs tiles."""
+    waves = _lib.lowbit_block_fp8_waves(dtype, m, n, k)
+    _check(min(waves, 0), "lowbit_block_fp8_waves")
+    return waves
+
+
+def lowbit_block_fp8_experts_waves(tokens, top_k, n_experts, hidden, inter):
+    """Waves of a workgroup of the second launch where each pair streams its weights, 0 where the pairs are sorted."""
+    waves = _lib.lowbit_block_fp8_experts_waves(tokens, top_k, n_experts, hidden, inter)
+    _check(min(waves, 0), "lowbit_block_fp8_experts_waves")
+    return waves
+
+
 def lowbit_dequantize_rows(w, rows, n_rows, dst, qtype, n, k, layout, out_dtype, stream):
     _check(_lib.lowbit_dequantize_rows(w, rows, n_rows, dst, qtype, n, k, layout, out_dtype, stream),
            "lowbit_dequantize_rows")

@@ -24,6 +24,10 @@ EXPERT_TILES = [(39, 2, 70, 784, 128), (148, 1, 70, 800, 128), (56, 3, 70, 1712,
                 (286, 2, 8, 2864, 128), (2461, 4, 70, 448, 256), (3676, 4, 70, 288, 128), (1700, 2, 600, 16, 128), (1700, 2, 512, 16, 128), (900, 4, 2100, 16, 128),
                 (9000, 2, 1, 16, 128), (70000, 1, 2, 16, 128)]
 
+# Rows of each number of waves of the kernel of few rows, and tokens of each of the experts' second launch
+FEW_ROWS = [(1, 40, 8336), (3, 130, 11008), (2, 17, 8208), (4, 64, 14336), (1, 8200, 8448), (2, 33, 272), (4, 40, 2048), (3, 70, 4112)]
+FEW_PAIRS = [(1, 2, 4, 4112, 128), (2, 2, 8, 4096, 256), (1, 3, 8, 7168, 384), (1, 2, 4, 4096, 256), (2, 2, 8, 2048, 128)]
+
 
 def blocks(n):
     return (n + 127) // 128

@@ -475,3 +475,14 @@ def test_a_block_scaled_checkpoint_with_experts_loads_saves_and_loads(tmp_path, 
     again = AutoModelForCausalLM.load_low_bit(str(tmp_path / "low"))
     want, got = model.state_dict(), again.state_dict()
     assert set(want) == set(got) and all(torch.equal(got[k].float(), v.float()) and got[k].dtype == v.dtype for k, v in want.items())
+
+
+def test_sizes_of_the_gpu_tests_reach_every_number_of_waves():
+    for dtype in (ggml.DT_F16, ggml.DT_BF16, ggml.DT_F32):
+        assert {ggml.lowbit_block_fp8_waves(dtype, *s) for s in u.FEW_ROWS} == {4, 8, 16}
+    assert {ggml.lowbit_block_fp8_experts_waves(*s) for s in u.FEW_PAIRS} == {8, 16}
+    assert ggml.lowbit_block_fp8_waves(ggml.DT_BF16, 100, 4096, 4096) == 0 == ggml.lowbit_block_fp8_experts_waves(100, 2, 8, 4096, 256)
+    for call in (lambda: ggml.lowbit_block_fp8_waves(ggml.DT_F16, 0, 16, 16), lambda: ggml.lowbit_block_fp8_waves(3, 1, 16, 16),
+                 lambda: ggml.lowbit_block_fp8_experts_waves(1, 65, 1, 16, 128)):
+        with pytest.raises(Exception, match="waves"):
+            call()

@@ -219,3 +219,21 @@ def test_quantizers_under_a_trace_a_dispatch_mode_and_vmap(dtype, weight):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     leaf = x.float().requires_grad_()
     assert not any(t.requires_grad for t in call(leaf))
+
+
+@pytest.mark.parametrize("m,n,k", u.FEW_ROWS)
+@pytest.mark.parametrize("dtype", ALL, ids=ids)
+def test_few_rows_of_every_number_of_waves(dtype, m, n, k):
+    g = gen(m + n)
+    x, (w, ws) = u.activations(g, m, k, dtype, spread_bits=0), u.weight(g, n, k, base=-8)
+    # every partial sum is a whole multiple of the least product, 2^-9, below 2^24 of them: exact in any order
+    assert (x.double().abs() @ u.dense(w, ws).abs().t()).max() < 2.0 ** 15
+    want = x.double() @ u.dense(w, ws).t()
+    assert torch.equal(bf.block_fp8_linear(x.cuda(), w.cuda(), ws.cuda()).cpu(), want.to(dtype))
+
+
+@pytest.mark.parametrize("tokens,top_k,n_exp,hidden,inter", u.FEW_PAIRS)
+@pytest.mark.parametrize("dtype", HALF, ids=ids)
+def test_few_pairs_of_every_number_of_waves(dtype, tokens, top_k, n_exp, hidden, inter):
+    case = expert_case(hidden, tokens, top_k, n_exp, hidden, inter, dtype)       # (the last pair's index names no expert)
+    near(bf.block_fp8_experts(*(t.cuda() for t in case), tokens % 2), case, tokens % 2, dtype, 3 ** 0.5 * 2.0 ** -13)
