@@ -18,7 +18,6 @@
 namespace lowbit {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int FP8_BLOCK = 128;
 constexpr float FP8_LEAST = 0x1p-100f;                       // least magnitude that a block's scale is made for
@@ -37,13 +36,15 @@ struct Codes {
     u32x4 lo, hi;
 };
 
+__device__ inline i32x8 joined(const Codes &c) {
+    return {(int)c.lo[0], (int)c.lo[1], (int)c.lo[2], (int)c.lo[3], (int)c.hi[0], (int)c.hi[1], (int)c.hi[2], (int)c.hi[3]};
+}
+
 // D[i][j] = sum over 128 of A[i][k] B[j][k]: lane l holds D[4 * (l >> 4) + 0..3][l & 15]
 template <bool EXACT> __device__ inline f32x4 block_dot(const Codes &a, const Codes &b) {
     const f32x4 zero = {};
     if constexpr (!EXACT) {
-        const i32x8 va = {(int)a.lo[0], (int)a.lo[1], (int)a.lo[2], (int)a.lo[3], (int)a.hi[0], (int)a.hi[1], (int)a.hi[2], (int)a.hi[3]};
-        const i32x8 vb = {(int)b.lo[0], (int)b.lo[1], (int)b.lo[2], (int)b.lo[3], (int)b.hi[0], (int)b.hi[1], (int)b.hi[2], (int)b.hi[3]};
-        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(va, vb, zero, 0, 0, 0, 0, 0, 0);    // formats e4m3, no block exponents
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(joined(a), joined(b), zero, 0, 0, 0, 0, 0, 0);     // formats e4m3, no block exponents
     } else {
         f32x4 d = zero;
 #pragma unroll

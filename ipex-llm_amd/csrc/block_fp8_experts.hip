@@ -38,6 +38,11 @@ __device__ inline float lane_value(float held, int l) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, held), l));
 }
 
+// Codes and scales of a row that the two kernels below keep in LDS, and the blocks that fit: at most 64 for each of 8 waves
+constexpr size_t ROW_LDS = 65536 - 4096, BLOCK_LDS = FP8_BLOCK + sizeof(float);
+constexpr int MOST_BLOCKS = (int)(ROW_LDS / BLOCK_LDS);
+static_assert(MOST_BLOCKS <= 8 * 64, "a wave's scales lie in the 64 lanes of a register");
+
 // One pair's 16 columns of h per workgroup: 16 rows of the gate and 16 of u.  The blocks of K are dealt to the waves, STEPS of them in flight
 // per wave, whose sums meet in LDS.  x is quantized by each workgroup; h leaves in float32, since its blocks are of 128 columns: with 128
 // columns per workgroup six experts of [1408 x 2048] would keep 66 CUs busy.  Bound by memory: two experts of [14336 x 4096], 235 MB, in 45 us.
@@ -64,19 +69,14 @@ __global__ __launch_bounds__(512) void block_fp8_expert_token_up_kernel(const Ex
     __builtin_amdgcn_sched_barrier(0);
 
     const uint8_t *row[2];
-    const float *ws[2];
     float held[2];
-    auto hold = [&](int i) __attribute__((always_inline)) {  // the scales of this wave's blocks i .. i + 63 in the lanes of a register
-        const int kb = wave + (i + lane) * WAVES;
-#pragma unroll
-        for (int t = 0; t < 2; t++) held[t] = ws[t][kb < KB ? kb : KB - 1];
-    };
 #pragma unroll
     for (int t = 0; t < 2; t++) {
         row[t] = p.gate_up + (e * 2 * p.I + t * p.I + c0 + r) * H;
-        ws[t] = p.gate_up_scale + ((e * 2 + t) * (p.I / FP8_BLOCK) + c0 / FP8_BLOCK) * KB;
+        // the scales of this wave's blocks in the lanes of a register (MOST_BLOCKS)
+        const float *const ws = p.gate_up_scale + ((e * 2 + t) * (p.I / FP8_BLOCK) + c0 / FP8_BLOCK) * KB;
+        held[t] = ws[wave + lane * WAVES < KB ? wave + lane * WAVES : KB - 1];
     }
-    hold(0);
     Codes wc[STEPS][2];
 #pragma unroll
     for (int s = 0; s < STEPS; s++)
@@ -94,7 +94,6 @@ __global__ __launch_bounds__(512) void block_fp8_expert_token_up_kernel(const Ex
 
     f32x4 acc[2] = {};
     for (int i0 = 0; wave + i0 * WAVES < KB; i0 += STEPS) {
-        if ((i0 & 63) == 0 && i0 != 0) hold(i0);
 #pragma unroll
         for (int s = 0; s < STEPS; s++) {
             const int kb = wave + (i0 + s) * WAVES, in = kb < KB ? kb : KB - 1, next = kb + STEPS * WAVES;
@@ -104,7 +103,7 @@ __global__ __launch_bounds__(512) void block_fp8_expert_token_up_kernel(const Ex
 #pragma unroll
             for (int t = 0; t < 2; t++) {
                 const f32x4 d = block_dot<true>(wc[s][t], xc);
-                const float sc = sx * lane_value(held[t], (i0 + s) & 63);
+                const float sc = sx * lane_value(held[t], i0 + s);
 #pragma unroll
                 for (int j = 0; j < 4; j++) acc[t][j] = kb < KB ? fmaf(sc, d[j], acc[t][j]) : acc[t][j];
                 if (next < KB) wc[s][t] = load_chunks(row[t], next, g, H);
@@ -156,14 +155,13 @@ __global__ __launch_bounds__(64 * WAVES) void block_fp8_expert_down_token_kernel
 
     const uint64_t valid = __ballot(expert >= 0);
     // unit u: block u % IB of pair u / IB; a wave's are wave, wave + WAVES, ..
-    float held;                                              // what the sums of units i .. i + 63 count, but for h's scale
-    auto hold = [&](int i) __attribute__((always_inline)) {
-        const int u = wave + (i + lane) * WAVES, j = u < units ? u / IB : 0, kb = u < units ? u - j * IB : 0;
+    float held;                                              // what their sums count, but for h's scale, in the lanes of a register (MOST_BLOCKS)
+    {
+        const int u = wave + lane * WAVES, j = u < units ? u / IB : 0, kb = u < units ? u - j * IB : 0;
         const int e = __shfl(expert, j);
         const float by = __shfl(route, j);
         held = u < units && e >= 0 ? p.down_scale[((int64_t)e * HB + n0 / FP8_BLOCK) * IB + kb] * by : 0.0f;
-    };
-    hold(0);
+    }
     auto load = [&](int u, Codes &w) __attribute__((always_inline)) {
         const int j = u / IB, kb = u - j * IB;
         if (u < units && (valid >> j & 1))                   // (the same for the whole wave)
@@ -191,13 +189,12 @@ __global__ __launch_bounds__(64 * WAVES) void block_fp8_expert_down_token_kernel
 
     f32x4 acc = {};
     for (int i0 = 0; wave + i0 * WAVES < units; i0 += STEPS) {
-        if ((i0 & 63) == 0 && i0 != 0) hold(i0);
 #pragma unroll
         for (int s = 0; s < STEPS; s++) {
             const int u = wave + (i0 + s) * WAVES, in = u < units ? u : units - 1;
             const uint8_t *const xr = lds + in * FP8_BLOCK + g * 16;
             const f32x4 d = block_dot<false>(wc[s], Codes{*(const u32x4 *)xr, *(const u32x4 *)(xr + 64)});
-            const float sc = hs[in] * lane_value(held, (i0 + s) & 63);
+            const float sc = hs[in] * lane_value(held, i0 + s);
             const bool counts = u < units && (valid >> (in / IB) & 1);
 #pragma unroll
             for (int j = 0; j < 4; j++) acc[j] = counts ? fmaf(sc, d[j], acc[j]) : acc[j];
@@ -358,10 +355,10 @@ __global__ __launch_bounds__(256) void block_fp8_expert_place_kernel(const int64
 // of the first product's tiles idle.  The estimate counts the experts that tokens routed evenly would meet, at 5.5 TB/s.  Pair by pair /
 // sorted, us: 3 tokens through 2 of 8 of [14336 x 4096] 197 / 167, two tokens 134 / 148; 4 through 6 of 64 of [1408 x 2048] 44 / 45, 8 81 / 72;
 // 8 through 8 of 128 of [768 x 2048] 61 / 66, 12 89 / 79; 4 through 8 of 256 of [2048 x 7168] 260 / 251, 16 1028 / 784.
-static size_t token_up_lds(int H) { return (size_t)fp8_blocks(H) * (FP8_BLOCK + 4); }
-static size_t token_down_lds(int top_k, int I) { return (size_t)top_k * (I / FP8_BLOCK) * (FP8_BLOCK + 4); }
+static size_t token_up_lds(int H) { return fp8_blocks(H) * BLOCK_LDS; }
+static size_t token_down_lds(int top_k, int I) { return (size_t)top_k * (I / FP8_BLOCK) * BLOCK_LDS; }
 static bool direct(int tokens, int top_k, int n_exp, int H, int I) {
-    if (token_up_lds(H) > 65536 - 4096 || token_down_lds(top_k, I) > 65536 - 4096) return false;
+    if (fp8_blocks(H) > MOST_BLOCKS || (int64_t)top_k * (I / FP8_BLOCK) > MOST_BLOCKS) return false;
     if (tokens == 1) return true;
     if ((int64_t)tokens * top_k > n_exp) return false;
     const double expert_us = 3.0 * H * I / 5.5e6, met = n_exp * (1.0 - pow(1.0 - (double)top_k / n_exp, tokens));

@@ -71,9 +71,6 @@ template <> struct XOperand<false> {
 template <> struct XOperand<true> {
     bf16x8 v[4];
 };
-__device__ inline i32x8 joined(const Codes &c) {
-    return {(int)c.lo[0], (int)c.lo[1], (int)c.lo[2], (int)c.lo[3], (int)c.hi[0], (int)c.hi[1], (int)c.hi[2], (int)c.hi[3]};
-}
 
 template <typename OT> struct Stored;
 template <> struct Stored<float> {

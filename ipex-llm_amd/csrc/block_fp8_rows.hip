@@ -60,7 +60,7 @@ __global__ __launch_bounds__(64 * WAVES) void block_fp8_few_rows_kernel(const Ro
 
     const int n = n0 + r;
     const uint8_t *const wrow = p.w + (int64_t)(n < N ? n : N - 1) * K;
-    // the scales of this wave's blocks in the lanes of a register (64 blocks per wave at most: see takes_few_rows); a scalar load per block
+    // the scales of this wave's blocks in the lanes of a register (64 blocks per wave at most: see few_rows_waves); a scalar load per block
     // would be waited for one after the other
     const float wheld = p.ws[(int64_t)(n0 / FP8_BLOCK) * KB + (wave + lane * WAVES < KB ? wave + lane * WAVES : KB - 1)];
     auto load_w = [&](int kb, Codes &c) __attribute__((always_inline)) {
@@ -143,6 +143,10 @@ static size_t few_rows_lds(int M, int KB) {
 // Short walks, in which half of the loads of 8 waves would be of no block: 4 waves each.  One row on [6144 x 2048] 5.2 us against 7.2.
 // Long walks of few workgroups: 16 waves each.  One row on [4096 x 11008] 13.3 us against 13.9, two on [4096 x 14336] 16.3 / 17.2; but
 // one on [28672 x 8192] 53.3 / 49.9, on [4096 x 4096], where half of their loads would be of no block, 7.9 / 5.6.
+//
+// A row's codes and scales fit 64 KiB of LDS, so that 8 waves have 64 blocks each at most, and so have 4.
+constexpr size_t FEW_LDS = 65536;
+static_assert(FEW_LDS / (FP8_BLOCK + FEW_ROWS * sizeof(float)) <= 8 * 64, "a wave's scales lie in the 64 lanes of a register");
 static int few_rows_waves(int N, int KB) { return KB <= 16 ? 4 : KB > 64 && N <= 8192 ? 16 : 8; }
 
 template <typename AT> static void launch_few_rows(const RowsProduct &p, hipStream_t st) {
@@ -160,7 +164,7 @@ template <typename AT> static void launch_few_rows(const RowsProduct &p, hipStre
 // above the shorter way on average, 31 % at worst (tiles for all 19 %).
 static bool takes_few_rows(bool wide, int M, int N, int K) {
     const int KB = fp8_blocks(K);
-    if (M > FEW_ROWS || KB > 512 || few_rows_lds(M, KB) > 65536) return false;
+    if (M > FEW_ROWS || few_rows_lds(M, KB) > FEW_LDS) return false;
     if (M <= 4) return true;
     const float rounds = N > 4096 ? N / 4096.0f : 1.0f;      // of a workgroup per CU
     const float bytes = (float)N * K, us = 3.1f + bytes / 5.6e6f + (wide ? 0.072f : 0.038f) * M * rounds * K / (64 * few_rows_waves(N, KB));
