@@ -346,7 +346,8 @@ int lowbit_block_fp8_quantize(const void *x, int dtype, int64_t rows, int64_t K,
 int lowbit_block_fp8_quantize_weight(const void *w, int dtype, int64_t matrices, int64_t N, int64_t K, void *codes, float *scale,
                                      void *stream);
 /* y[M, N] = Q(x) * W^T (+ bias[N]); x, bias and y of `dtype`.  With 16-bit types the products run on the fp8 matrix pipes, which keep
- * 13 bits below the largest of a few neighbouring products; with LOWBIT_DT_F32 they are summed in float32 throughout.  workspace:
+ * 13 bits below the largest of a few neighbouring products (1e-5 to 5e-5 of the norm of activations times weights; where large terms
+ * cancel, of the terms); with LOWBIT_DT_F32 they are summed in float32 throughout.  workspace:
  * lowbit_block_fp8_linear_workspace_bytes bytes (0 for a few rows), contents undefined before and after. */
 size_t lowbit_block_fp8_linear_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K);
 int lowbit_block_fp8_linear(const void *x, const void *w, const float *w_scale, const void *bias, void *y, int dtype, int64_t M, int64_t N,

@@ -1,7 +1,7 @@
 // The experts of a mixture-of-experts block with weights and activations in e4m3, a scale for each block of 128 (block_fp8.h):
 //     out_t = sum_j p_tj * (Q(act(g) u) down_e^T),  (g | u) = Q(x_t) gate_up_e^T,  e = ids_tj
 //
-// The first product's sums go through the bfloat16 MFMA, which is exact (block_fp8.h): what the fp8 instruction drops, 1e-5 of a sum, would put one
+// The first product's sums go through the bfloat16 MFMA, which is exact (block_fp8.h): what the fp8 instruction drops, 1e-5 and more of a sum, would put one
 // of 3000 values of h on the other side of the border between two codes, 1.5e-3 of the result, more than its rounding to bfloat16 costs.
 // While the experts' weights are what takes the time, that costs nothing.
 //
