@@ -25,6 +25,9 @@ constexpr int FP8_BLOCK = 128;
 constexpr float FP8_LEAST = 0x1p-100f;                       // least magnitude that a block's scale is made for
 constexpr uint32_t FP8_LEAST_BITS = 27u << 23;
 
+// A launch has fewer than 2^32 threads in a row of its grid
+constexpr int64_t most_groups(int threads) { return ((int64_t)1 << 32) / threads - 8; }
+
 __host__ __device__ inline int fp8_blocks(int k) { return (k + FP8_BLOCK - 1) / FP8_BLOCK; }
 
 // eight codes as bfloat16, exactly: an operand of the bfloat16 MFMA

@@ -312,7 +312,7 @@ int launch_block_fp8_back(const void *grad, const uint8_t *w, const float *ws, v
     const BackPlan plan = back_plan(M, N, K);
     BackArgs p = {grad, w, ws, gx, (float *)(space + padded_bytes(M, N)), N, M, N, K, fp8_blocks(N), fp8_blocks(K),
                   cdiv(M, BACK_FORMS[plan.form].rows), cdiv(K, BACK_FORMS[plan.form].cols), plan.splits, cdiv(fp8_blocks(N), plan.splits)};
-    if ((int64_t)p.tiles_m * p.tiles_k * p.splits > 0x7fffffff - 8) return -3;
+    if ((int64_t)p.tiles_m * p.tiles_k * p.splits > most_groups(512)) return -3;
     if (padded(N)) {
         p.ldg = cdiv(N, BACK_STEP) * BACK_STEP;
         for (int m = 0; m < M; m += 65535) {

@@ -489,7 +489,7 @@ template <typename AT> static int launch_experts_t(ExpertsArgs p, const ExpertsS
     }
     int32_t *const offsets = (int32_t *)(ws + at.offsets), *const order = (int32_t *)(ws + at.order), *const pos = (int32_t *)(ws + at.pos);
     const int KB = fp8_blocks(p.H);
-    if ((int64_t)tokens * KB > (int64_t)1 << 34) return -3;
+    if (((int64_t)tokens * KB + 31) / 32 + pairs + p.n_exp > most_groups(256)) return -3;
     const int quantizing = (int)(((int64_t)tokens * KB + 31) / 32);
     int32_t *const counts = (int32_t *)(ws + at.counts);
     const AT *const x = (const AT *)p.x;
@@ -519,7 +519,7 @@ template <typename AT> static int launch_experts_t(ExpertsArgs p, const ExpertsS
     const int rows = up_rows(pairs, p.n_exp, p.I), form = down_form(pairs, p.n_exp, p.H, p.I), used = pairs < p.n_exp ? pairs : p.n_exp;
     u.tiles_m = pairs / rows + used;           // at most
     d.tiles_m = pairs / TILED_FORMS[form].rows + used;
-    if ((int64_t)u.tiles_m * (p.I / FP8_BLOCK) > 0x7fffffff - 8 || (int64_t)d.tiles_m * ((p.H + 127) / 128) > 0x7fffffff - 8) return -3;
+    if ((int64_t)u.tiles_m * (p.I / FP8_BLOCK) > most_groups(512) || (int64_t)d.tiles_m * ((p.H + 127) / 128) > most_groups(512)) return -3;
     if (rows == 64) launch_tiled<AT, true, TILED_UP, true, true, 2, 4, 2, 4, 3, 2>(u, st);
     else if (rows == 96) launch_tiled<AT, true, TILED_UP, true, true, 3, 4, 2, 4, 2, 2>(u, st);
     else launch_tiled<AT, true, TILED_UP, true, true, 4, 4, 2, 4, 2, 2>(u, st);

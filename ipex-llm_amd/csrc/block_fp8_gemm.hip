@@ -91,7 +91,7 @@ int launch_block_fp8_tiled(TiledArgs p, int dtype, const TiledPlan &plan, hipStr
     p.splits = plan.splits;
     p.split_blocks = cdiv(p.KB, plan.splits);
     const TiledForm &f = TILED_FORMS[plan.form];
-    if ((int64_t)cdiv(p.M, f.rows) * cdiv(p.N, f.cols) * plan.splits > 0x7fffffff - 8) return -3;
+    if ((int64_t)cdiv(p.M, f.rows) * cdiv(p.N, f.cols) * plan.splits > most_groups(512)) return -3;
     if (plan.splits > 1) {
         if (dtype == DT_F32) launch_tiled_part_exact(p, plan.form, st);
         else launch_tiled_part(p, plan.form, st);

@@ -28,9 +28,15 @@ __global__ __launch_bounds__(256) void block_fp8_rows_kernel(const AT *__restric
 int launch_block_fp8_rows(const void *x, int dtype, int64_t rows, int K, uint8_t *codes, int ldc, bool wide, float *scale, int64_t row_step,
                           int64_t block_step, hipStream_t st) {
     const int KB = fp8_blocks(K);
-    const int64_t units = rows * KB, groups = (units + 31) / 32;
-    if (groups > 0x7fffffff) return -3;
-    const dim3 grid((uint32_t)groups), block(256);
+    const int64_t most = most_groups(256) * 32 / KB;
+    for (; rows > most; rows -= most) {
+        if (int rc = launch_block_fp8_rows(x, dtype, most, K, codes, ldc, wide, scale, row_step, block_step, st)) return rc;
+        x = (const uint8_t *)x + most * K * (dtype == DT_F32 ? 4 : 2);
+        codes += most * ldc * (wide ? 2 : 1);
+        scale += most * row_step;
+    }
+    const int64_t units = rows * KB;
+    const dim3 grid((uint32_t)((units + 31) / 32)), block(256);
     auto go = [&](auto *typed, auto w) {
         using AT = typename std::remove_cv<typename std::remove_pointer<decltype(typed)>::type>::type;
         hipLaunchKernelGGL((block_fp8_rows_kernel<AT, decltype(w)::value>), grid, block, 0, st, typed, codes, scale, units, K, KB, ldc, row_step, block_step);
@@ -83,7 +89,14 @@ __global__ __launch_bounds__(512) void block_fp8_weight_kernel(const AT *__restr
 
 int launch_block_fp8_weight(const void *w, int dtype, int64_t matrices, int N, int K, uint8_t *codes, float *scale, hipStream_t st) {
     const int KB = fp8_blocks(K), NB = fp8_blocks(N);
-    if (matrices * NB > 0x7fffffff / KB) return -3;
+    const int64_t most = most_groups(512) / ((int64_t)NB * KB);
+    if (most == 0) return -3;
+    for (; matrices > most; matrices -= most) {
+        if (int rc = launch_block_fp8_weight(w, dtype, most, N, K, codes, scale, st)) return rc;
+        w = (const uint8_t *)w + most * N * K * (dtype == DT_F32 ? 4 : 2);
+        codes += most * N * K;
+        scale += most * NB * KB;
+    }
     const dim3 grid((uint32_t)(matrices * NB * KB));
     auto go = [&](auto *typed) {
         using AT = typename std::remove_cv<typename std::remove_pointer<decltype(typed)>::type>::type;

@@ -486,3 +486,14 @@ def test_sizes_of_the_gpu_tests_reach_every_number_of_waves():
                  lambda: ggml.lowbit_block_fp8_experts_waves(1, 65, 1, 16, 128)):
         with pytest.raises(Exception, match="waves"):
             call()
+
+
+def test_sizes_past_a_launch_are_refused_by_the_library():
+    """One weight of 2^24 blocks, and experts whose rows or tiles pass 2^32 threads: by arithmetic, with nothing launched (there is no GPU)."""
+    assert lib.lowbit_block_fp8_quantize_weight(P, 0, 1, 1 << 20, 1 << 18, P, P, None) == -3 and b"too large" in lib.lowbit_last_error()
+    size = lib.lowbit_block_fp8_experts_workspace_bytes(1 << 21, 1, 2, 1 << 17, 128)
+    assert lib.lowbit_block_fp8_experts(P, P, P, 0, 1 << 21, 1, 2, P, P, P, P, P, size, P, 0, 1 << 17, 128, 0, None) == -3
+    size = lib.lowbit_block_fp8_linear_workspace_bytes(0, (1 << 22) - 1, (1 << 23) - 1, 128)
+    assert size < 1 << 31                                    # (2^27 tiles; their sums are never split)
+    size = lib.lowbit_block_fp8_backward_workspace_bytes(0, (1 << 22) - 1, 128, (1 << 23) - 16)
+    assert lib.lowbit_block_fp8_backward(P, P, P, P, 0, (1 << 22) - 1, 128, (1 << 23) - 16, P, size, None) == -3

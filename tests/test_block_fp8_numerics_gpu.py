@@ -346,3 +346,25 @@ def test_experts_in_tiles_of_every_form_in_float16(tokens, top_k, n_exp, hidden,
     # tokens with a routing weight of some 1e-5, are subnormal: half a step, 2^-25, for each of the row's
     per = (got - want).norm(dim=1) - slack.norm(dim=1)
     assert (per <= (unit + 4 * 3 ** 0.5 * 2.0 ** -13) * size.norm(dim=1) + 2.0 ** -25 * hidden ** 0.5).all()
+
+
+def test_more_blocks_than_a_launch_has_workgroups_for():
+    """9 million weights of one block each, and 537 million rows of one block: several launches, whose parts meet without a seam."""
+    n = 9_000_000
+    w = (torch.arange(n * 16, device="cuda", dtype=torch.int32) % 4093 - 2046).view(n, 1, 16).bfloat16()
+    codes, scale = bf.block_fp8_quantize_weight(w)
+    seam = (1 << 32) // 512 - 8
+    for part in (slice(0, 1000), slice(seam - 500, seam + 500), slice(n - 1000, n)):
+        want, ws = u.quantize(w[part].cpu(), 128)
+        assert torch.equal(codes[part].cpu().double(), want) and torch.equal(scale[part].cpu(), ws)
+    del w, codes, scale
+    seam = ((1 << 32) // 256 - 8) * 32
+    n = seam + 3000
+    x = torch.empty((n, 16), dtype=torch.bfloat16, device="cuda")
+    for at in range(0, n, 1 << 26):
+        part = x[at:at + (1 << 26)]
+        part.copy_((torch.arange(part.numel(), device="cuda", dtype=torch.int32) % 4093 - 2046).view_as(part))
+    codes, scale = bf.block_fp8_quantize(x)
+    for part in (slice(0, 1000), slice(seam - 500, seam + 500), slice(n - 1000, n)):
+        want, ws = u.quantize(x[part].cpu(), 1)
+        assert torch.equal(codes[part].cpu().double(), want) and torch.equal(scale[part].cpu(), ws)
