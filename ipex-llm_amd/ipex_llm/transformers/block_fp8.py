@@ -208,7 +208,6 @@ class _KeepsFormat(nn.Module):
 
     def _apply(self, fn, recurse=True):
         keep = {id(self._parameters[n]) for n in self._FORMAT if self._parameters.get(n) is not None}
-        keep |= {id(self._parameters[n].data) for n in self._FORMAT if self._parameters.get(n) is not None}
 
         def moved(t):
             out = fn(t)
