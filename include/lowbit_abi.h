@@ -365,7 +365,8 @@ int lowbit_block_fp8_waves(int dtype, int64_t M, int64_t N, int64_t K);
 /* A mixture-of-experts block: y[t, :] = sum_j topk_weight[t, j] * (Q(act(g) .* u) * down[e]^T), (g | u) = Q(x_t) * gate_up[e]^T, e =
  * topk_ids[t, j]; a pair whose id lies outside [0, n_experts) counts nothing.  gate_up [n_experts, 2 inter, hidden] (gate rows first)
  * and down [n_experts, hidden, inter] are the experts' codes one after the other, their scales likewise; inter is a multiple of 128,
- * hidden of 16.  act(g) .* u is quantized from float32.  Types and limits as in lowbit_experts_forward, pairs at most 2^21. */
+ * hidden of 16.  act(g) .* u is quantized from float32.  Types and limits as in lowbit_experts_forward, pairs at most 2^21.  The workspace
+ * holds 2 bytes for each value of x, one for each of act(g) .* u, and pairs' results in float32: a GiB of them, or 256 columns, at a time. */
 size_t lowbit_block_fp8_experts_workspace_bytes(int64_t tokens, int top_k, int n_experts, int64_t hidden, int64_t inter);
 int lowbit_block_fp8_experts(const void *x, const int64_t *topk_ids, const void *topk_weight, int weight_dtype, int64_t tokens, int top_k,
                              int n_experts, const void *gate_up, const float *gate_up_scale, const void *down, const float *down_scale,

@@ -35,6 +35,7 @@ struct TiledArgs {
     int ldxs, M, N, K, KB, pitch;
     int tiles_m, tiles_n, splits, split_blocks;
     int n_exp, top_k, I, act;                                // UP: I columns of h
+    int expert_rows;                                         // by expert: weight rows from one expert's to the next's, N of which the launch takes
     float *hs;                                               // UP: scales of h, [I / 128][ldhs]; its codes go to y
     int ldhs;
 };
@@ -143,7 +144,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, MIN_WAVES) void block_fp8_tiled_
         if constexpr (GATHER) xaddr[j] = xbase + (uint64_t)(p.order[at] / p.top_k) * p.ldx + chunk;
         else xoff[j] = (uint32_t)((at - m0) * p.ldx) + chunk;
     }
-    const uint64_t wexpert = (uint64_t)(uintptr_t)p.w + (uint64_t)expert * p.N * p.K;
+    const uint64_t wexpert = (uint64_t)(uintptr_t)p.w + (BY_EXPERT ? (uint64_t)expert * p.expert_rows * p.K : 0);
     // Which weight row lies in row `at` of LDS: a wave column's tiles of 16, each lane quarter's four rows of them neighbours of its
     // four in the next tile, so that a lane's results are neighbours in a row of y.  UP: tiles of the gate, then as many of u.
     auto weight_row = [&](int at) -> int64_t {
@@ -200,7 +201,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, MIN_WAVES) void block_fp8_tiled_
 
     // ---- scales.  A weight's of up to 64 blocks lie in the lanes of one register
     const int nb0 = UP ? n0 / FP8_BLOCK : (n0 + wn * TN * 16) / FP8_BLOCK, NB = fp8_blocks(p.N);
-    const float *const wscale = p.ws + ((int64_t)expert * NB + (nb0 < NB ? nb0 : NB - 1)) * KB;
+    const float *const wscale = p.ws + ((BY_EXPERT ? (int64_t)expert * fp8_blocks(p.expert_rows) : 0) + (nb0 < NB ? nb0 : NB - 1)) * KB;
     const int64_t u_scale = UP ? (int64_t)(p.I / FP8_BLOCK) * KB : 0;
     float wheld[UP ? 2 : 1];
     auto hold = [&](int kb) __attribute__((always_inline)) {

@@ -182,7 +182,7 @@ __device__ inline void combine_pairs(float (&sum)[8], const YT *__restrict__ y, 
 // of [1024 x 1664] in asym_int4, the whole call 34.9 -> 33.6 us, 32 tokens, two of 13, 30.2 -> 29.0, 512 of [14336 x 4096] 498 -> 496).
 template <typename YT, typename AT, typename WT>
 __global__ __launch_bounds__(256) void moe_combine_kernel(const YT *__restrict__ y, const int32_t *__restrict__ pos,
-                                                          const WT *__restrict__ weight, AT *__restrict__ out, int top_k, int N) {
+                                                          const WT *__restrict__ weight, AT *__restrict__ out, int top_k, int N, int pitch) {
     using V8 = typename Vec8<AT>::type;
     const int t = blockIdx.y, n = (blockIdx.x * 256 + threadIdx.x) * 8;
     if (n >= N) return;
@@ -198,32 +198,33 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const YT *__restrict__
     V8 o;
 #pragma unroll
     for (int i = 0; i < 8; i++) o[i] = to_at<AT>(sum[i]);
-    *(V8 *)(out + (int64_t)t * N + n) = o;
+    *(V8 *)(out + (int64_t)t * pitch + n) = o;
 }
 
+// y: pairs' rows of N values; out: rows of `pitch`, of which the call writes N
 template <typename YT, typename AT>
 static void launch_combine(const void *y, const int32_t *pos, const void *weight, int w_dtype, void *out, int tokens, int top_k,
-                           int N, hipStream_t st) {
+                           int N, int pitch, hipStream_t st) {
     for (; tokens > 65535; tokens -= 65535) {                // (a grid's second dimension ends there)
-        launch_combine<YT, AT>(y, pos, weight, w_dtype, out, 65535, top_k, N, st);
+        launch_combine<YT, AT>(y, pos, weight, w_dtype, out, 65535, top_k, N, pitch, st);
         pos += (int64_t)65535 * top_k;
         weight = (const uint8_t *)weight + (int64_t)65535 * top_k * (w_dtype == DT_F32 ? 4 : 2);
-        out = (AT *)out + (int64_t)65535 * N;
+        out = (AT *)out + (int64_t)65535 * pitch;
     }
     const dim3 grid((N / 8 + 255) / 256, tokens);
     if (w_dtype == DT_F32)
-        hipLaunchKernelGGL((moe_combine_kernel<YT, AT, float>), grid, dim3(256), 0, st, (const YT *)y, pos, (const float *)weight, (AT *)out, top_k, N);
+        hipLaunchKernelGGL((moe_combine_kernel<YT, AT, float>), grid, dim3(256), 0, st, (const YT *)y, pos, (const float *)weight, (AT *)out, top_k, N, pitch);
     else if (w_dtype == DT_F16)
-        hipLaunchKernelGGL((moe_combine_kernel<YT, AT, _Float16>), grid, dim3(256), 0, st, (const YT *)y, pos, (const _Float16 *)weight, (AT *)out, top_k, N);
+        hipLaunchKernelGGL((moe_combine_kernel<YT, AT, _Float16>), grid, dim3(256), 0, st, (const YT *)y, pos, (const _Float16 *)weight, (AT *)out, top_k, N, pitch);
     else
-        hipLaunchKernelGGL((moe_combine_kernel<YT, AT, __bf16>), grid, dim3(256), 0, st, (const YT *)y, pos, (const __bf16 *)weight, (AT *)out, top_k, N);
+        hipLaunchKernelGGL((moe_combine_kernel<YT, AT, __bf16>), grid, dim3(256), 0, st, (const YT *)y, pos, (const __bf16 *)weight, (AT *)out, top_k, N, pitch);
 }
 
 // of pairs' results in float32
 void launch_moe_combine_f32(const float *y, const int32_t *pos, const void *weight, int w_dtype, void *out, int act_dtype, int tokens, int top_k,
-                            int N, hipStream_t st) {
-    if (act_dtype == DT_F16) launch_combine<float, _Float16>(y, pos, weight, w_dtype, out, tokens, top_k, N, st);
-    else launch_combine<float, __bf16>(y, pos, weight, w_dtype, out, tokens, top_k, N, st);
+                            int N, int pitch, hipStream_t st) {
+    if (act_dtype == DT_F16) launch_combine<float, _Float16>(y, pos, weight, w_dtype, out, tokens, top_k, N, pitch, st);
+    else launch_combine<float, __bf16>(y, pos, weight, w_dtype, out, tokens, top_k, N, pitch, st);
 }
 
 // Whether the pairs go through the streaming kernel, which reads an expert's weights once per pair: while there are no
@@ -291,8 +292,8 @@ int launch_experts(const void *x, const int64_t *ids, const void *weight, int w_
         return rc;
     if (int rc = launch_grouped_gemm(h, downs, nullptr, y, offsets, n_exp, pairs, qtype, act_dtype, hidden, inter, 0, ws + at.split,
                                      at.bytes - at.split, st)) return rc;
-    if (act_dtype == DT_F16) launch_combine<_Float16, _Float16>(y, pos, weight, w_dtype, out, tokens, top_k, hidden, st);
-    else launch_combine<__bf16, __bf16>(y, pos, weight, w_dtype, out, tokens, top_k, hidden, st);
+    if (act_dtype == DT_F16) launch_combine<_Float16, _Float16>(y, pos, weight, w_dtype, out, tokens, top_k, hidden, hidden, st);
+    else launch_combine<__bf16, __bf16>(y, pos, weight, w_dtype, out, tokens, top_k, hidden, hidden, st);
     return 0;
 }
 

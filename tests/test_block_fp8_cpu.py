@@ -497,3 +497,14 @@ def test_sizes_past_a_launch_are_refused_by_the_library():
     assert size < 1 << 31                                    # (2^27 tiles; their sums are never split)
     size = lib.lowbit_block_fp8_backward_workspace_bytes(0, (1 << 22) - 1, 128, (1 << 23) - 16)
     assert lib.lowbit_block_fp8_backward(P, P, P, P, 0, (1 << 22) - 1, 128, (1 << 23) - 16, P, size, None) == -3
+
+
+def test_the_experts_workspace_is_bounded_beside_what_goes_in():
+    """Codes of x (as 16-bit numbers) and of h, and a GiB, or a KiB for each pair, of pairs' results: not all of them at once."""
+    for tokens, top_k, n_exp, hidden, inter in ((512, 8, 256, 7168, 2048), (4096, 8, 256, 7168, 2048), (32768, 8, 256, 7168, 2048),
+                                                (262144, 8, 128, 2048, 768), (1 << 21, 1, 8, 4096, 256), (100000, 2, 8, 4096, 14336)):
+        pairs = tokens * top_k
+        own = tokens * u.blocks(hidden) * (256 + 4) + pairs * (inter + inter // 32 + 8) + 4 * 257 * n_exp
+        bound = own + max(1 << 30, pairs * 1024) + (1 << 16)
+        assert lib.lowbit_block_fp8_experts_workspace_bytes(tokens, top_k, n_exp, hidden, inter) <= bound
+    assert lib.lowbit_block_fp8_experts_workspace_bytes(512, 8, 256, 7168, 2048) > 512 * 8 * 7168 * 4      # (all at once where they fit)

@@ -368,3 +368,17 @@ def test_more_blocks_than_a_launch_has_workgroups_for():
     for part in (slice(0, 1000), slice(seam - 500, seam + 500), slice(n - 1000, n)):
         want, ws = u.quantize(x[part].cpu(), 1)
         assert torch.equal(codes[part].cpu().double(), want) and torch.equal(scale[part].cpu(), ws)
+
+
+@pytest.mark.parametrize("tokens,top_k,n_exp,hidden,inter,parts", [(70000, 4, 5, 1040, 128, 2), (300000, 1, 3, 1552, 128, 3), (300000, 2, 3, 1296, 128, 6)])
+def test_pairs_results_of_more_than_a_gib_are_summed_in_parts(tokens, top_k, n_exp, hidden, inter, parts):
+    """Columns in several launches; as the same tokens in calls of their own, and as 64 bits for some."""
+    assert -(-hidden // max(256, (1 << 30) // (4 * tokens * top_k) // 256 * 256)) == parts
+    g = gen(hidden)
+    case = list(expert_case(hidden, 600, top_k, n_exp, hidden, inter, torch.bfloat16))
+    rows = torch.randint(0, 600, (tokens,), generator=g)
+    rows[:600], rows[-600:] = torch.arange(600), torch.arange(600)
+    on_gpu = [t.cuda() for t in case]
+    got = bf.block_fp8_experts(*(t[rows.cuda()] for t in on_gpu[:3]), *on_gpu[3:])
+    near(got[:600], case, 0, torch.bfloat16, 3 ** 0.5 * 2.0 ** -13)
+    assert torch.equal(got, got[:600][rows.cuda()])          # (a row's sums are the same wherever it stands)
