@@ -1,8 +1,8 @@
 // The tiled product of block_fp8.h: codes of x and of the weight meet in LDS, 128 values of K at a time.
 //
 // A workgroup of WM x WN waves owns WM * TM * 16 rows of x by WN * TN * 16 weight rows.  A step's codes of both operands come by
-// LDS-DMA, one step ahead, into the other of two buffers; a step is one block of K, so a wave multiplies TM x TN results by one
-// instruction each, from zero, and adds them to the sums in float32 times the two scales.
+// LDS-DMA into two buffers, asked for a step and a half ahead, or three, two steps ahead; a step is one block of K, so a wave multiplies
+// TM x TN results by one instruction each, from zero, and adds them to the sums in float32 times the two scales.
 //
 // LDS holds rows of 128 bytes, the 16-byte chunk c of row r at slot c ^ swizzle(r): the DMA writes 8 rows of 8 slots at a time (lane
 // = 8 * row + slot, so the swizzle is in the lane's source address), and 16 lanes of a read, which take one chunk of 16
@@ -12,7 +12,8 @@
 // Bound by the matrix pipes and the clock that the power limit leaves them (1.6 GHz at the largest sizes): 8192^3 448 us, 2.45 PFLOP/s, where
 // the library's product with a single scale takes 386; [28672 x 8192] by 8192 rows 1550 us, MFMAs on 66 % of the cycles, no LDS conflict.
 // A few hundred rows are bound by the latency of a step: two groups of waves that take half of a tile's blocks each, 333 x 3211 x 2112 in
-// float32 15 us against 17, 300 x 4096 x 4096 14.2 / 17.6, 40 x 11008 x 4096 11.7 against 13.3 in two splits and their sum.
+// float32 15 us against 17, 300 x 4096 x 4096 14.2 / 17.6, 40 x 11008 x 4096 11.7 against 13.3 in two splits and their sum (without the
+// launch of 2.5 us that quantizes the rows).
 //
 // EXACT, for sums that keep float32's 24 bits (block_fp8.h): the bfloat16 MFMA, four instructions of 32 values in place of one.  x comes as
 // bfloat16 numbers, rows of 256 bytes a block, and only the weight's codes are widened on the way from LDS, part by part.
