@@ -105,8 +105,8 @@ def block_fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.
 
     float16 and bfloat16: sums in float32 of products on the fp8 matrix pipes, which drop what lies 13 bits below the largest of a few
     neighbouring products (1e-5 to 5e-5 of the norm of activations times weights; where large terms cancel, of the terms); float32: exact
-    products, which 16-bit rows have as `block_fp8_linear(x.float(), ..).to(x.dtype)`.  The result, with its bias, is rounded once.  Where x wants a gradient it is
-    grad W, grad not quantized."""
+    products, which 16-bit rows have as `block_fp8_linear(x.float(), ..).to(x.dtype)`.  The result, with its bias, is rounded once.  Where
+    x wants a gradient it is grad W, grad not quantized."""
     y = ops.block_fp8_linear(x, weight, weight_scale, bias, -1)
     if y is not None:
         return y

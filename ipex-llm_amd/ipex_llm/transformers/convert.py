@@ -192,7 +192,7 @@ def _replace_with_low_bit_linear(model, qtype, modules_to_not_convert=None,
         if isinstance(module, nn.Linear) or is_fused_experts(module):
             check_block_fp8(module, full_module_name, scaled)
 
-        if is_linear and getattr(module, "n_groups", 1) != 1:
+        if isinstance(module, nn.Linear) and getattr(module, "n_groups", 1) != 1:
             continue   # a linear in groups, each of which meets its own columns of x, stays as it is
         if is_linear and not isinstance(module, (LowBitLinear, FP16Linear, BF16Linear)):
             in_features, out_features, mp_group = linear_args

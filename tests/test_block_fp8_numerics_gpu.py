@@ -382,3 +382,86 @@ def test_pairs_results_of_more_than_a_gib_are_summed_in_parts(tokens, top_k, n_e
     got = bf.block_fp8_experts(*(t[rows.cuda()] for t in on_gpu[:3]), *on_gpu[3:])
     near(got[:600], case, 0, torch.bfloat16, 3 ** 0.5 * 2.0 ** -13)
     assert torch.equal(got, got[:600][rows.cuda()])          # (a row's sums are the same wherever it stands)
+
+
+def test_tangents_through_experts():
+    """Of x and of the routing weights, in float32: the formula's, the quantization counting as the identity."""
+    case = expert_case(21, 12, 2, 4, 256, 128, torch.float32)
+    x, picks, p, gu, gus, dn, dns = case
+    g = gen(22)
+    tx, tp = torch.randn(x.shape, generator=g), torch.randn(p.shape, generator=g)
+    with torch.autograd.forward_ad.dual_level():
+        make = torch.autograd.forward_ad.make_dual
+        out = bf.block_fp8_experts(make(x.cuda(), tx.cuda()), picks.cuda(), make(p.cuda(), tp.cuda()), *(t.cuda() for t in case[3:]))
+        got = torch.autograd.forward_ad.unpack_dual(out).tangent.cpu().double()
+    want = torch.zeros((12, 256), dtype=torch.float64)
+    rows = u.dense(*u.quantize(x, 1), 1)
+    for e in range(4):
+        t, j = torch.where(picks == e)
+        w, d = u.dense(gu[e], gus[e]), u.dense(dn[e], dns[e])
+        s, ds = rows[t] @ w.t(), tx[t].double() @ w.t()
+        a, v = s[:, :128], s[:, 128:]
+        slope = torch.sigmoid(a) * (1 + a * (1 - torch.sigmoid(a)))
+        h, dh = act64(a, 0) * v, slope * ds[:, :128] * v + act64(a, 0) * ds[:, 128:]
+        hq = u.dense(*u.quantize(h, 1), 1)
+        want.index_add_(0, t, dh @ d.t() * p[t, j].double()[:, None] + hq @ d.t() * tp[t, j].double()[:, None])
+    # (one code of h in 2^14 may be on the other side of a border, a step of 2^-3 of one of its terms)
+    assert (got - want).norm() <= 2.0 ** -10 * want.norm()
+
+
+@pytest.mark.parametrize("dtype", ALL, ids=ids)
+def test_experts_with_a_gate_of_their_own_on_the_gpu(dtype):
+    from test_block_fp8_cpu import FusedExperts
+    from ipex_llm.transformers.convert import ggml_convert_low_bit
+    fused = FusedExperts(4, 256, 128, limit=0.5, alpha=1.7).eval()
+    new = ggml_convert_low_bit(torch.nn.Sequential(fused), 15, torch_dtype=dtype)[0].cuda()
+    g = gen(23)
+    x, p = torch.randn((20, 256), generator=g).to(dtype), torch.rand((20, 2), generator=g).to(dtype)
+    picks = torch.rand((20, 4), generator=g).argsort(dim=1)[:, :2]
+    got = new(x.cuda(), picks.cuda(), p.cuda()).cpu().double()
+    want, size, clamped = torch.zeros((20, 256), dtype=torch.float64), torch.zeros((20, 256), dtype=torch.float64), 0
+    rows = u.dense(*u.quantize(x, 1), 1)
+    for e in range(4):
+        t, j = torch.where(picks == e)
+        s = rows[t] @ u.dense(fused.gate_up_proj[e], fused.gate_up_proj_scale_inv[e]).t()
+        clamped += (s > 0.5).sum()
+        y = u.dense(*u.quantize(fused._apply_gate(s), 1), 1) @ u.dense(fused.down_proj[e], fused.down_proj_scale_inv[e]).t() * p[t, j].double()[:, None]
+        want.index_add_(0, t, y)
+        size.index_add_(0, t, y.abs())
+    assert clamped > 100
+    # (codes of h: as in test_experts_that_no_kernel_takes_round_once_too)
+    assert (got - want).norm() <= torch.finfo(dtype).eps / 2 * want.norm() + 2.0 ** -12 * size.norm()
+
+
+@pytest.mark.parametrize("kind", ["dense", "experts"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=ids)
+def test_a_block_scaled_checkpoint_runs(dtype, kind, tmp_path):
+    """Through from_pretrained, beside the dense model that holds the same numbers.  It differs by the quantization of each product's
+    activations: e4m3 keeps 4 bits, 0.026 of a value in the mean, independent over seven products of one or three layers' branches."""
+    from test_block_fp8_cpu import tiny_llama, write_checkpoint
+    from ipex_llm.transformers import AutoModelForCausalLM
+    if kind == "dense":
+        model, apart = tiny_llama(), ("lm_head",)
+    else:
+        from transformers import Qwen3MoeConfig, Qwen3MoeForCausalLM
+        torch.manual_seed(5)
+        model, apart = Qwen3MoeForCausalLM(Qwen3MoeConfig(hidden_size=256, intermediate_size=384, moe_intermediate_size=128, num_experts=4,
+                                                          num_experts_per_tok=4, num_hidden_layers=1, num_attention_heads=4,
+                                                          num_key_value_heads=2, vocab_size=64)).eval(), ("lm_head", "mlp.gate")
+    write_checkpoint(tmp_path, model, apart)
+    with torch.no_grad():
+        for name, v in model.named_parameters():             # what the codes stand for
+            if v.dim() == 3 or (name.endswith("proj.weight") and not any(a in name for a in apart)):
+                high = [v] if v.dim() == 2 else [part for w in v for part in (w.chunk(2) if name.endswith("gate_up_proj") else [w])]
+                for w in high:
+                    w.copy_(u.dense(*u.quantize(w, 128)))
+            else:
+                v.copy_(v.bfloat16())
+    loaded = AutoModelForCausalLM.from_pretrained(str(tmp_path), load_in_low_bit="fp8_e4m3", torch_dtype=dtype, modules_to_not_convert=list(apart))
+    loaded = loaded.cuda()
+    tokens = torch.randint(0, 64, (2, 9), generator=gen(24))
+    with torch.inference_mode():
+        want = model(tokens).logits
+        got = loaded(tokens.cuda()).logits.float().cpu()
+        again = loaded.to(torch.float16)(tokens.cuda()).logits.float().cpu() if dtype == torch.float32 else loaded.half()(tokens.cuda()).logits.float().cpu()
+    assert (got - want).norm() <= 0.1 * want.norm() and (again - want).norm() <= 0.1 * want.norm()
