@@ -85,7 +85,8 @@ def unconverted_linears(state_dict):
     """Module names whose saved weight is still a dense matrix: they were excluded from the
     conversion when the model was saved and must be excluded again when it is rebuilt."""
     return [k[:-len(".weight")] for k, v in state_dict.items()
-            if k.endswith(".weight") and v.dim() == 2 and v.numel() > 0 and v.dtype not in (torch.uint8, torch.float8_e4m3fn)]
+            if k.endswith(".weight") and v.dim() == 2 and v.numel() > 0 and v.dtype != torch.uint8
+            and not (v.dtype == torch.float8_e4m3fn and k + "_scale_inv" in state_dict)]
 
 
 def block_fp8_layers(state_dict):

@@ -508,3 +508,18 @@ def test_the_experts_workspace_is_bounded_beside_what_goes_in():
         bound = own + max(1 << 30, pairs * 1024) + (1 << 16)
         assert lib.lowbit_block_fp8_experts_workspace_bytes(tokens, top_k, n_exp, hidden, inter) <= bound
     assert lib.lowbit_block_fp8_experts_workspace_bytes(512, 8, 256, 7168, 2048) > 512 * 8 * 7168 * 4      # (all at once where they fit)
+
+
+def test_fp8_weights_without_scales_that_were_left_out_stay_left_out(tmp_path):
+    from ipex_llm import optimize_model
+    from ipex_llm.optimize import load_low_bit
+
+    def model():
+        plain = nn.Linear(128, 64, bias=False)
+        plain.weight = nn.Parameter(torch.arange(64 * 128).view(64, 128).remainder(9).float().to(u.E4M3), requires_grad=False)
+        return nn.ModuleDict({"plain": plain, "scaled": scaled_linear(128, 256)}).eval()
+    want = optimize_model(model(), "fp8_e4m3", modules_to_not_convert=["plain"])
+    want.save_low_bit(str(tmp_path))
+    again = load_low_bit(model(), str(tmp_path))
+    assert type(again["plain"]) is nn.Linear and type(again["scaled"]) is bf.BlockFP8Linear
+    assert again["plain"].weight.dtype == u.E4M3 and torch.equal(again["plain"].weight.float(), want["plain"].weight.float())
