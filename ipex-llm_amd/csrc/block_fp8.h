@@ -13,7 +13,8 @@
 // Of the norm of products of activations and normal weights that is 1.4e-5 (1.6 at most) for N(0, 1) activations, 2e-5 to 3.4e-5 where one
 // channel in 100 to 500 is 20 times as loud, 5e-5 (5.6) for lognormal ones of deviation 1.5: a hundredth to a thirtieth of what rounding to
 // bfloat16 costs, a fifteenth to a quarter of float16's.  Where large terms cancel it is as much of their root of squares, 3.5e-6 of it in
-// neighbours of opposite signs, and more of the result.  Results in float32 therefore go through the bfloat16 MFMA, which keeps 24 bits: codes are exact in bfloat16.
+// neighbours of opposite signs, and more of the result.  Results in float32 therefore go through the bfloat16 MFMA, which keeps 24 bits:
+// codes are exact in bfloat16.
 #pragma once
 #include "lowbit_mfma.h"
 
