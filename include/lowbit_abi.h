@@ -378,6 +378,37 @@ int lowbit_block_fp8_experts_plan(int64_t tokens, int top_k, int n_experts, int6
 /* Waves of a workgroup of its second launch where each pair streams its weights, 0 where the pairs are sorted (negative: an error). */
 int lowbit_block_fp8_experts_waves(int64_t tokens, int top_k, int n_experts, int64_t hidden, int64_t inter);
 
+/* ---- products of two operands in 8-bit integers with a scale for each row
+ *
+ * The form of checkpoints with 8-bit weights by output channel and activations by token: a weight [N, K] is row-major int8 codes (K a
+ * multiple of 16) with one float32 scale for each row, scale[N].  Activations are quantized in the call, by row: scale = a / 127, code =
+ * x * 127 / a to the nearest (ties to even, decided exactly), a = the row's largest magnitude, 2^-100 at least.  A row that holds a NaN or an
+ * infinity has the scale NaN and codes of zero.  Sums are whole numbers in 32 bits, exact up to K = 2^17, which is as far as the products go; every
+ * LOWBIT_DT_* takes the same product.  All pointers are 16-byte aligned device memory (bias: any alignment; scales: 4).  No counterpart in the
+ * reference, whose 8-bit weights meet 16-bit activations (low_bit_linear.py:657-668). */
+
+/* codes [rows, K] and scale [rows] of x [rows, K], of any LOWBIT_DT_*: activations by token or a weight by output channel.  K < 2^23. */
+int lowbit_row_int8_quantize(const void *x, int dtype, int64_t rows, int64_t K, void *codes, float *scale, void *stream);
+/* y[M, N] = Q(x) * W^T (+ bias[N]); x, bias and y of `dtype`; one rounding to it.  workspace: lowbit_row_int8_linear_workspace_bytes bytes (0 for a
+ * few rows), contents undefined before and after. */
+size_t lowbit_row_int8_linear_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K);
+int lowbit_row_int8_linear(const void *x, const void *w, const float *w_scale, const void *bias, void *y, int dtype, int64_t M, int64_t N,
+                           int64_t K, void *workspace, size_t workspace_bytes, void *stream);
+/* The same of rows that are codes [M, K] and scale [M] already; bias and y of `dtype`. */
+size_t lowbit_row_int8_product_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K);
+int lowbit_row_int8_product(const void *codes, const float *scale, const void *w, const float *w_scale, const void *bias, void *y, int dtype,
+                            int64_t M, int64_t N, int64_t K, void *workspace, size_t workspace_bytes, void *stream);
+/* The gradient that flows on to x, as if the quantization of x were the identity: grad_x[M, K] = (grad * w_scale)[M, N] * codes[N, K].  grad *
+ * w_scale is rounded to float16 relative to a power of two of each row (LOWBIT_DT_F32: to two of them, 22 bits), the sums are float32, one rounding.
+ * A row of grad with a NaN or an infinity gives NaN. */
+size_t lowbit_row_int8_backward_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K);
+int lowbit_row_int8_backward(const void *grad, const void *w, const float *w_scale, void *grad_x, int dtype, int64_t M, int64_t N, int64_t K,
+                             void *workspace, size_t workspace_bytes, void *stream);
+/* What the linear product and the gradient run as: plan4 as lowbit_block_fp8_plan's. */
+int lowbit_row_int8_plan(int dtype, int backward, int64_t M, int64_t N, int64_t K, int *plan4);
+/* Waves of a workgroup where lowbit_row_int8_linear runs the kernel of few rows, 0 where it runs tiles (negative: an error). */
+int lowbit_row_int8_waves(int64_t M, int64_t N, int64_t K);
+
 #ifdef __cplusplus
 }
 #endif

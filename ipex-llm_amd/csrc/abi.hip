@@ -74,6 +74,18 @@ size_t block_fp8_experts_workspace_bytes(int tokens, int top_k, int n_exp, int H
 int launch_block_fp8_experts(const void *x, const int64_t *ids, const void *weight, int w_dtype, int tokens, int top_k, int n_exp,
                              const uint8_t *gate_up, const float *gate_up_scale, const uint8_t *down, const float *down_scale, void *workspace,
                              void *out, int act_dtype, int H, int I, int act, hipStream_t st);
+int launch_row_int8_quantize(const void *x, int dtype, int64_t rows, int K, uint8_t *codes, int ldc, float *scale, hipStream_t st);
+size_t row_int8_linear_workspace_bytes(int M, int N, int K);
+void row_int8_linear_plan(int M, int N, int K, int *plan4);
+int row_int8_linear_waves(int M, int N, int K);
+int launch_row_int8_linear(const void *x, const uint8_t *w, const float *ws, const void *bias, void *y, int dtype, int M, int N, int K,
+                           uint8_t *space, hipStream_t st);
+size_t row_int8_product_workspace_bytes(int M, int N, int K);
+int launch_row_int8_product(const uint8_t *codes, const float *xs, const uint8_t *w, const float *ws, const void *bias, void *y, int dtype, int M,
+                            int N, int K, uint8_t *space, hipStream_t st);
+size_t row_int8_back_workspace_bytes(int dtype, int M, int N, int K);
+void row_int8_back_plan(int dtype, int M, int N, int K, int *plan4);
+int launch_row_int8_back(const void *grad, const uint8_t *w, const float *ws, void *gx, int dtype, int M, int N, int K, uint8_t *space, hipStream_t st);
 int launch_grouped_gemm(const void *x, const void *const *w, const void *const *w_up, void *y, const int32_t *offsets,
                         int n_groups, int total_rows, int qtype, int act_dtype, int N, int K, int act, void *workspace,
                         size_t workspace_bytes, hipStream_t st);
@@ -873,6 +885,102 @@ int lowbit_block_fp8_experts(const void *x, const int64_t *topk_ids, const void 
     return check_launch(launch_block_fp8_experts(x, topk_ids, topk_weight, weight_dtype, (int)tokens, top_k, n_experts, (const uint8_t *)gate_up,
                                                  gate_up_scale, (const uint8_t *)down, down_scale, workspace, y, act_dtype, (int)hidden,
                                                  (int)inter, act, (hipStream_t)stream), what);
+}
+
+// ---- products of 8-bit integers with a scale for each row
+
+// Sizes that the kernels' arithmetic and grids hold: whole sums of K products of 127 * 127 in 32 bits, fewer than 2^22 rows of x.
+static int check_row_int8(const char *what, int dtype, int64_t M, int64_t N, int64_t K) {
+    if (dtype != LOWBIT_DT_F16 && dtype != LOWBIT_DT_BF16 && dtype != LOWBIT_DT_F32) return fail(LOWBIT_EDTYPE, "%s: unsupported element type", what);
+    if (M < 0 || N < 0 || K < 0) return fail(LOWBIT_EARG, "%s: negative shape", what);
+    if (K % 16) return fail(LOWBIT_ESHAPE, "%s: K=%lld is not a multiple of 16", what, (long long)K);
+    if (M >= (1 << 22) || N >= (1 << 23) || K > (1 << 17)) return fail(LOWBIT_ESIZE, "%s: needs M < 2^22, N < 2^23 and K <= 2^17", what);
+    return 0;
+}
+
+static bool row_int8_ok(int dtype, int64_t M, int64_t N, int64_t K) {
+    return M > 0 && N > 0 && K > 0 && M < (1 << 22) && N < (1 << 23) && K <= (1 << 17) && K % 16 == 0 &&
+           (dtype == LOWBIT_DT_F16 || dtype == LOWBIT_DT_BF16 || dtype == LOWBIT_DT_F32);
+}
+
+static bool aligned4(const void *p) { return (((uintptr_t)p) & 3) == 0; }
+
+int lowbit_row_int8_quantize(const void *x, int dtype, int64_t rows, int64_t K, void *codes, float *scale, void *stream) {
+    const char *what = "lowbit_row_int8_quantize";
+    if (rows < 0) return fail(LOWBIT_EARG, "%s: negative shape", what);
+    if (K >= 0 && K % 16 == 0 && K >= (1 << 23)) return fail(LOWBIT_ESIZE, "%s: needs K < 2^23", what);
+    if (int rc = check_row_int8(what, dtype, 0, 0, K > (1 << 17) ? 16 : K)) return rc;
+    if (rows == 0 || K == 0) return 0;
+    if (!x || !codes || !scale || !aligned16(x) || !aligned16(codes) || !aligned4(scale)) return fail(LOWBIT_EARG, "%s: null or misaligned pointer", what);
+    if (rows > (int64_t)1 << 40) return fail(LOWBIT_ESIZE, "%s: too many rows", what);
+    return check_launch(launch_row_int8_quantize(x, dtype, rows, (int)K, (uint8_t *)codes, (int)K, scale, (hipStream_t)stream), what);
+}
+
+size_t lowbit_row_int8_linear_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K) {
+    return row_int8_ok(dtype, M, N, K) ? row_int8_linear_workspace_bytes((int)M, (int)N, (int)K) : 0;
+}
+
+int lowbit_row_int8_linear(const void *x, const void *w, const float *w_scale, const void *bias, void *y, int dtype, int64_t M, int64_t N,
+                           int64_t K, void *workspace, size_t workspace_bytes, void *stream) {
+    const char *what = "lowbit_row_int8_linear";
+    if (int rc = check_row_int8(what, dtype, M, N, K)) return rc;
+    if (M == 0 || N == 0) return 0;
+    if (K == 0) return fail(LOWBIT_ESHAPE, "%s: K must be positive", what);
+    if (!x || !w || !w_scale || !y || !aligned16(x) || !aligned16(w) || !aligned16(y) || !aligned4(w_scale))
+        return fail(LOWBIT_EARG, "%s: null or misaligned pointer", what);
+    if (int rc = check_space(what, workspace, workspace_bytes, row_int8_linear_workspace_bytes((int)M, (int)N, (int)K))) return rc;
+    return check_launch(launch_row_int8_linear(x, (const uint8_t *)w, w_scale, bias, y, dtype, (int)M, (int)N, (int)K, (uint8_t *)workspace,
+                                               (hipStream_t)stream), what);
+}
+
+size_t lowbit_row_int8_product_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K) {
+    return row_int8_ok(dtype, M, N, K) ? row_int8_product_workspace_bytes((int)M, (int)N, (int)K) : 0;
+}
+
+int lowbit_row_int8_product(const void *codes, const float *scale, const void *w, const float *w_scale, const void *bias, void *y, int dtype,
+                            int64_t M, int64_t N, int64_t K, void *workspace, size_t workspace_bytes, void *stream) {
+    const char *what = "lowbit_row_int8_product";
+    if (int rc = check_row_int8(what, dtype, M, N, K)) return rc;
+    if (M == 0 || N == 0) return 0;
+    if (K == 0) return fail(LOWBIT_ESHAPE, "%s: K must be positive", what);
+    if (!codes || !scale || !w || !w_scale || !y || !aligned16(codes) || !aligned16(w) || !aligned16(y) || !aligned4(w_scale) || !aligned4(scale))
+        return fail(LOWBIT_EARG, "%s: null or misaligned pointer", what);
+    if (int rc = check_space(what, workspace, workspace_bytes, row_int8_product_workspace_bytes((int)M, (int)N, (int)K))) return rc;
+    return check_launch(launch_row_int8_product((const uint8_t *)codes, scale, (const uint8_t *)w, w_scale, bias, y, dtype, (int)M, (int)N, (int)K,
+                                                (uint8_t *)workspace, (hipStream_t)stream), what);
+}
+
+int lowbit_row_int8_plan(int dtype, int backward, int64_t M, int64_t N, int64_t K, int *plan4) {
+    const char *what = "lowbit_row_int8_plan";
+    if (int rc = check_row_int8(what, dtype, M, N, K)) return rc;
+    if (M == 0 || N == 0 || K == 0 || !plan4) return fail(LOWBIT_EARG, "%s: sizes must be positive, plan4 not null", what);
+    if (backward) row_int8_back_plan(dtype, (int)M, (int)N, (int)K, plan4);
+    else row_int8_linear_plan((int)M, (int)N, (int)K, plan4);
+    return 0;
+}
+
+int lowbit_row_int8_waves(int64_t M, int64_t N, int64_t K) {
+    const char *what = "lowbit_row_int8_waves";
+    if (int rc = check_row_int8(what, LOWBIT_DT_F32, M, N, K)) return rc;
+    if (M == 0 || N == 0 || K == 0) return fail(LOWBIT_EARG, "%s: sizes must be positive", what);
+    return row_int8_linear_waves((int)M, (int)N, (int)K);
+}
+
+size_t lowbit_row_int8_backward_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K) {
+    return row_int8_ok(dtype, M, N, K) ? row_int8_back_workspace_bytes(dtype, (int)M, (int)N, (int)K) : 0;
+}
+
+int lowbit_row_int8_backward(const void *grad, const void *w, const float *w_scale, void *grad_x, int dtype, int64_t M, int64_t N, int64_t K,
+                             void *workspace, size_t workspace_bytes, void *stream) {
+    const char *what = "lowbit_row_int8_backward";
+    if (int rc = check_row_int8(what, dtype, M, N, K)) return rc;
+    if (M == 0 || K == 0) return 0;
+    if (N == 0) return fail(LOWBIT_ESHAPE, "%s: N must be positive", what);
+    if (!grad || !w || !w_scale || !grad_x || !aligned16(grad) || !aligned16(w) || !aligned16(grad_x) || !aligned4(w_scale))
+        return fail(LOWBIT_EARG, "%s: null or misaligned pointer", what);
+    if (int rc = check_space(what, workspace, workspace_bytes, row_int8_back_workspace_bytes(dtype, (int)M, (int)N, (int)K))) return rc;
+    return check_launch(launch_row_int8_back(grad, (const uint8_t *)w, w_scale, grad_x, dtype, (int)M, (int)N, (int)K, (uint8_t *)workspace,
+                                             (hipStream_t)stream), what);
 }
 
 static int grouped_any(const char *who, const void *x, const void *const *w, const void *const *w_up, void *y,

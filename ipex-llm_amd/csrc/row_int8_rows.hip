@@ -1,0 +1,252 @@
+// Up to sixteen rows of activations times a weight with a scale for each row (row_int8.h): the weight streams past once, in one launch.
+//
+// A workgroup owns 16 weight rows; its waves take the blocks of K in turn and their sums meet in LDS.  A wave's loads are 16 rows x 64
+// contiguous bytes, STEPS blocks ahead of their use.  x is quantized by each workgroup, into LDS, while the first weights are on their
+// way: its largest magnitudes by row first, then its codes.  Loads return in order, so x is asked for ahead of the weights.
+#include "row_int8_tiled.h"
+
+#include <math.h>
+
+namespace lowbit {
+
+constexpr int FEW_ROWS = 16;                                 // an MFMA's
+
+struct Int8Rows {
+    const void *x;                                           // [M, K]
+    const uint8_t *w;
+    const float *ws;
+    const void *bias;
+    void *y;
+    int M, N, K, KB;
+};
+
+template <typename AT> struct Eight {
+    typedef AT type __attribute__((ext_vector_type(8)));
+};
+
+template <typename V8> __device__ inline void widen_to(const V8 &v, float (&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) f[i] = (float)v[i];
+}
+
+template <typename AT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void row_int8_few_rows_kernel(const Int8Rows p) {
+    constexpr int STEPS = 4;                                 // blocks in flight per wave
+    constexpr int HELD = sizeof(AT) == 4 ? 2 : 4;            // pieces of x per thread that are asked for ahead of the weights
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    __shared__ uint32_t most[FEW_ROWS];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+    const int n0 = blockIdx.x * 16, KB = p.KB, M = p.M, N = p.N, K = p.K;
+    // (one wait for all arguments: left alone the compiler loads each where it is first used)
+    asm volatile("" :: "s"(p.x), "s"(p.w), "s"(p.ws), "s"(p.bias), "s"(p.y), "s"(M), "s"(N), "s"(K), "s"(KB));
+
+    // pieces of 8 values of x, 16 to a block: thread, thread + 64 * WAVES, ...
+    using V8 = typename Eight<AT>::type;
+    const int pieces = M * KB * 16;
+    auto load_x = [&](int piece) __attribute__((always_inline)) {
+        const int row = piece / (KB * 16), k = (piece - row * KB * 16) * 8;
+        return k < K ? *(const V8 *)((const AT *)p.x + (int64_t)row * K + k) : V8{};
+    };
+    V8 held[HELD];
+#pragma unroll
+    for (int i = 0; i < HELD; i++) {
+        const int piece = threadIdx.x + i * 64 * WAVES;
+        held[i] = V8{};
+        if (piece < pieces) held[i] = load_x(piece);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+
+    const int n = n0 + r;
+    const uint8_t *const wrow = p.w + (int64_t)(n < N ? n : N - 1) * K;
+    auto load_w = [&](int kb, Codes &c) __attribute__((always_inline)) {
+        // (chunks past the row's end: the block's first one, which meets zeros of x)
+        const int left = K - kb * INT8_BLOCK;
+        const uint8_t *const at = wrow + kb * INT8_BLOCK;
+        c.lo = ld<u32x4, true>(at + (g * 16 < left ? g * 16 : 0));
+        c.hi = ld<u32x4, true>(at + (64 + g * 16 < left ? 64 + g * 16 : 0));
+    };
+    Codes wc[STEPS];
+#pragma unroll
+    for (int s = 0; s < STEPS; s++)
+        load_w(wave + s * WAVES < KB ? wave + s * WAVES : KB - 1, wc[s]);      // (past the last block: it again, times zeros)
+    __builtin_amdgcn_sched_barrier(0);
+
+    // the rows' largest magnitudes
+    if (threadIdx.x < FEW_ROWS) most[threadIdx.x] = 0;
+    __syncthreads();
+    auto look = [&](int piece, const V8 &v) __attribute__((always_inline)) {
+        float f[8];
+        widen_to(v, f);
+        const uint32_t m = max_of_16(largest_of(f));         // (16 neighbouring lanes have pieces of one row)
+        if ((threadIdx.x & 15) == 0) atomicMax(&most[piece / (KB * 16)], m);
+    };
+#pragma unroll
+    for (int i = 0; i < HELD; i++) {
+        const int piece = threadIdx.x + i * 64 * WAVES;
+        if (piece < pieces) look(piece, held[i]);            // (the 16 lanes of a block are in or out together)
+    }
+    for (int piece = threadIdx.x + HELD * 64 * WAVES; piece < pieces; piece += 64 * WAVES) look(piece, load_x(piece));
+    __syncthreads();
+
+    // codes of x in LDS, rows of KB * 128 + 16 bytes (16: rows start in other banks)
+    const int pitch = KB * INT8_BLOCK + 16;
+    auto put_x = [&](int piece, const V8 &v) __attribute__((always_inline)) {
+        const int row = piece / (KB * 16), at = piece - row * KB * 16;
+        float f[8];
+        widen_to(v, f);
+        uint32_t c[2];
+        RowCoder{most[row]}(f, c);
+        *(u32x2 *)(lds + row * pitch + at * 8) = u32x2{c[0], c[1]};
+    };
+#pragma unroll
+    for (int i = 0; i < HELD; i++) {
+        const int piece = threadIdx.x + i * 64 * WAVES;
+        if (piece < pieces) put_x(piece, held[i]);
+    }
+    for (int piece = threadIdx.x + HELD * 64 * WAVES; piece < pieces; piece += 64 * WAVES) put_x(piece, load_x(piece));
+    __syncthreads();
+
+    // (operand rows past M repeat the last one; their results are not stored)
+    const uint8_t *const xrow = lds + (r < M ? r : M - 1) * pitch + g * 16;
+    i32x4 acc = {};
+    for (int i0 = 0; wave + i0 * WAVES < KB; i0 += STEPS) {
+#pragma unroll
+        for (int s = 0; s < STEPS; s++) {
+            const int kb = wave + (i0 + s) * WAVES, in = kb < KB ? kb : KB - 1, next = kb + STEPS * WAVES;
+            Codes xc = {*(const u32x4 *)(xrow + in * INT8_BLOCK), *(const u32x4 *)(xrow + in * INT8_BLOCK + 64)};
+            if (kb >= KB) xc = Codes{};
+            acc = int8_dot(wc[s], xc, acc);
+            if (next < KB) load_w(next, wc[s]);
+        }
+    }
+
+    // the waves' sums, [wave][row][16 columns]
+    __syncthreads();                                         // (they lie where the codes were)
+    int32_t *const sums = (int32_t *)lds;
+    if (r < M) *(i32x4 *)(sums + (wave * FEW_ROWS + r) * 16 + g * 4) = acc;
+    __syncthreads();
+    if ((int)threadIdx.x >= M * 16) return;
+    const int m = threadIdx.x >> 4, c = threadIdx.x & 15;
+    if (n0 + c >= N) return;
+    int32_t sum = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) sum += sums[(w * FEW_ROWS + m) * 16 + c];
+    float v = (float)sum * row_scale(most[m]) * p.ws[n0 + c];
+    if (p.bias) v += (float)((const AT *)p.bias)[n0 + c];
+    ((AT *)p.y)[(int64_t)m * N + n0 + c] = Stored<AT>::of(v);
+}
+
+static size_t few_rows_lds(int M, int KB) {
+    const size_t codes = (size_t)M * (KB * INT8_BLOCK + 16);
+    return codes > 16384 ? codes : 16384;                    // (the sums of 16 waves)
+}
+
+constexpr size_t FEW_LDS = 65536 - 64;
+static int few_rows_waves(int N, int KB) { return KB <= 16 ? 4 : KB > 64 && N <= 8192 ? 16 : 8; }
+
+template <typename AT> static void launch_few_rows(const Int8Rows &p, hipStream_t st) {
+    const dim3 grid((p.N + 15) / 16);
+    const size_t lds = few_rows_lds(p.M, p.KB);
+    const int waves = few_rows_waves(p.N, p.KB);
+    if (waves == 4) hipLaunchKernelGGL((row_int8_few_rows_kernel<AT, 4>), grid, dim3(256), lds, st, p);
+    else if (waves == 16) hipLaunchKernelGGL((row_int8_few_rows_kernel<AT, 16>), grid, dim3(1024), lds, st, p);
+    else hipLaunchKernelGGL((row_int8_few_rows_kernel<AT, 8>), grid, dim3(512), lds, st, p);
+}
+
+// Rows whose codes fit 64 KiB of LDS: up to four always, up to sixteen where that is estimated shorter than tiles and the launch ahead of them.
+static bool takes_few_rows(int M, int N, int K) {
+    const int KB = int8_blocks(K);
+    if (M > FEW_ROWS || few_rows_lds(M, KB) > FEW_LDS) return false;
+    if (M <= 4) return true;
+    const float rounds = N > 4096 ? N / 4096.0f : 1.0f;      // of a workgroup per CU
+    const float bytes = (float)N * K, us = 3.1f + bytes / 5.6e6f + 0.038f * M * rounds * K / (64 * few_rows_waves(N, KB));
+    return us <= fmaxf(row_int8_tiled_plan(M, N, K).us, bytes / 5.4e6f + 4.0f) + 1.5f;
+}
+
+// codes of x, their scales, a split's sums
+struct Int8Space {
+    size_t xs, part, bytes;
+};
+static Int8Space linear_space(int M, int N, int K, const Int8Plan &plan) {
+    auto whole = [](size_t bytes) { return (bytes + 255) & ~(size_t)255; };
+    Int8Space s;
+    s.xs = whole((size_t)M * int8_blocks(K) * INT8_BLOCK);
+    s.part = s.xs + whole((size_t)M * sizeof(float));
+    s.bytes = s.part + row_int8_part_bytes(plan, M, N);
+    return s;
+}
+
+size_t row_int8_linear_workspace_bytes(int M, int N, int K) {
+    return takes_few_rows(M, N, K) ? 0 : linear_space(M, N, K, row_int8_tiled_plan(M, N, K)).bytes;
+}
+
+// rows and columns of a tile (0, 0: the kernel of few rows), splits, groups
+void row_int8_linear_plan(int M, int N, int K, int *plan4) {
+    plan4[0] = plan4[1] = 0;
+    plan4[2] = plan4[3] = 1;
+    if (takes_few_rows(M, N, K)) return;
+    const Int8Plan plan = row_int8_tiled_plan(M, N, K);
+    plan4[0] = INT8_FORMS[plan.form].rows;
+    plan4[1] = INT8_FORMS[plan.form].cols;
+    plan4[2] = plan.splits;
+    plan4[3] = INT8_FORMS[plan.form].groups;
+}
+
+// waves of a workgroup of the kernel of few rows; 0 where tiles run
+int row_int8_linear_waves(int M, int N, int K) { return takes_few_rows(M, N, K) ? few_rows_waves(N, int8_blocks(K)) : 0; }
+
+int launch_row_int8_linear(const void *x, const uint8_t *w, const float *ws, const void *bias, void *y, int dtype, int M, int N, int K, uint8_t *space,
+                           hipStream_t st) {
+    if (takes_few_rows(M, N, K)) {
+        const Int8Rows p = {x, w, ws, bias, y, M, N, K, int8_blocks(K)};
+        if (dtype == DT_F16) launch_few_rows<_Float16>(p, st);
+        else if (dtype == DT_BF16) launch_few_rows<__bf16>(p, st);
+        else if (dtype == DT_F32) launch_few_rows<float>(p, st);
+        else return -4;
+        return 0;
+    }
+    const Int8Plan plan = row_int8_tiled_plan(M, N, K);
+    const Int8Space at = linear_space(M, N, K, plan);
+    float *const xs = (float *)(space + at.xs);
+    Int8Args t{};
+    t.ldx = (int64_t)int8_blocks(K) * INT8_BLOCK;
+    if (int rc = launch_row_int8_quantize(x, dtype, M, K, space, (int)t.ldx, xs, st)) return rc;
+    t.x = space; t.xs = xs; t.w = w; t.ws = ws; t.bias = bias; t.y = y; t.part = (int32_t *)(space + at.part);
+    t.M = M; t.N = N; t.K = K;
+    return launch_row_int8_tiled(t, dtype, plan, st);
+}
+
+// Rows of codes that do not fill whole blocks, in rows of ldx bytes with zeros past K; 16 bytes per thread.
+__global__ __launch_bounds__(256) void row_int8_pad_kernel(const u32x4 *__restrict__ codes, u32x4 *__restrict__ to, int64_t units, int quads, int ldq) {
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (id >= units) return;
+    const int64_t row = id / ldq;
+    const int q = (int)(id - row * ldq);
+    to[id] = q < quads ? codes[row * quads + q] : u32x4{};
+}
+
+static bool whole_blocks(int K) { return K % INT8_BLOCK == 0; }
+
+size_t row_int8_product_workspace_bytes(int M, int N, int K) {
+    const size_t padded = whole_blocks(K) ? 0 : (size_t)M * int8_blocks(K) * INT8_BLOCK;
+    return ((padded + 255) & ~(size_t)255) + row_int8_part_bytes(row_int8_tiled_plan(M, N, K), M, N);
+}
+
+int launch_row_int8_product(const uint8_t *codes, const float *xs, const uint8_t *w, const float *ws, const void *bias, void *y, int dtype, int M, int N,
+                            int K, uint8_t *space, hipStream_t st) {
+    Int8Args t{};
+    t.ldx = (int64_t)int8_blocks(K) * INT8_BLOCK;
+    t.x = codes;
+    if (!whole_blocks(K)) {
+        const int64_t units = M * (t.ldx / 16);
+        hipLaunchKernelGGL(row_int8_pad_kernel, dim3((uint32_t)((units + 255) / 256)), dim3(256), 0, st, (const u32x4 *)codes, (u32x4 *)space, units, K / 16,
+                           (int)(t.ldx / 16));
+        t.x = space;
+        space += (M * t.ldx + 255) & ~(int64_t)255;
+    }
+    t.xs = xs; t.w = w; t.ws = ws; t.bias = bias; t.y = y; t.part = (int32_t *)space;
+    t.M = M; t.N = N; t.K = K;
+    return launch_row_int8_tiled(t, dtype, row_int8_tiled_plan(M, N, K), st);
+}
+
+}  // namespace lowbit

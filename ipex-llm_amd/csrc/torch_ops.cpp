@@ -50,6 +50,13 @@ struct Api {
     decltype(&lowbit_block_fp8_linear_workspace_bytes) block_fp8_linear_workspace_bytes = nullptr;
     decltype(&lowbit_block_fp8_backward) block_fp8_backward = nullptr;
     decltype(&lowbit_block_fp8_backward_workspace_bytes) block_fp8_backward_workspace_bytes = nullptr;
+    decltype(&lowbit_row_int8_quantize) row_int8_quantize = nullptr;
+    decltype(&lowbit_row_int8_linear) row_int8_linear = nullptr;
+    decltype(&lowbit_row_int8_linear_workspace_bytes) row_int8_linear_workspace_bytes = nullptr;
+    decltype(&lowbit_row_int8_product) row_int8_product = nullptr;
+    decltype(&lowbit_row_int8_product_workspace_bytes) row_int8_product_workspace_bytes = nullptr;
+    decltype(&lowbit_row_int8_backward) row_int8_backward = nullptr;
+    decltype(&lowbit_row_int8_backward_workspace_bytes) row_int8_backward_workspace_bytes = nullptr;
     decltype(&lowbit_block_fp8_experts) block_fp8_experts = nullptr;
     decltype(&lowbit_block_fp8_experts_workspace_bytes) block_fp8_experts_workspace_bytes = nullptr;
 } api;
@@ -422,6 +429,116 @@ Tensor block_fp8_experts(const Tensor &x_in, const Tensor &ids_in, const Tensor 
     return y;
 }
 
+// ---- int8 operands with a scale for each row
+
+// w holds int8 codes [.., N, K] and scale their scales [.., N], on x's device
+bool is_row_int8(const Tensor &w, const Tensor &scale, const Tensor &x, int64_t matrices) {
+    if (w.device() != x.device() || scale.device() != x.device() || w.layout() != at::kStrided || scale.layout() != at::kStrided ||
+        w.scalar_type() != at::kChar || scale.scalar_type() != at::kFloat || w.dim() != (matrices ? 3 : 2) || scale.dim() != w.dim() - 1 ||
+        !w.is_contiguous() || !scale.is_contiguous() || ((uintptr_t)w.const_data_ptr() & 15) || w.numel() == 0 || w.size(-1) % 16) return false;
+    return scale.sizes() == w.sizes().slice(0, w.dim() - 1) && (!matrices || w.size(0) == matrices) && !differentiable(scale);
+}
+
+constexpr int64_t ROW_INT8_MOST_K = 1 << 17;
+
+// codes and scales of x by row; undefined tensors when this is not the plain case
+std::pair<Tensor, Tensor> row_int8_quantize(const Tensor &x_in) {
+    if (!on_gpu(x_in) || x_in.dim() < 1 || x_in.numel() == 0 || x_in.size(-1) % 16 || dtype_code(x_in.scalar_type()) < 0 ||
+        !nothing_watches(x_in)) return {};
+    const Tensor x = whole_rows(x_in.detach());
+    const int64_t K = x.size(-1);
+    c10::DeviceGuard guard(x.device());
+    const Tensor codes = at::empty(x.sizes(), x.options().dtype(at::kChar)),
+                 scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+    check(api.row_int8_quantize(x.const_data_ptr(), dtype_code(x.scalar_type()), x.numel() / K, K, codes.data_ptr(), scale.data_ptr<float>(),
+                                current_stream(x)), "lowbit_row_int8_quantize");
+    return {codes, scale};
+}
+
+// y in `dtype` of rows x (or of codes and their scales), whole as the kernels read them
+Tensor row_int8_any_product(const Tensor &x, const Tensor &xs, const Tensor &w, const Tensor &scale, const Tensor &bias, at::ScalarType dtype) {
+    c10::DeviceGuard guard(x.device());
+    const int64_t N = w.size(0), K = w.size(1), M = x.numel() / K;
+    const int dt = dtype_code(dtype);
+    Tensor y = at::empty(with_last(x, N), x.options().dtype(dtype));
+    const size_t bytes = (xs.defined() ? api.row_int8_product_workspace_bytes : api.row_int8_linear_workspace_bytes)(dt, M, N, K);
+    const Tensor ws = bytes ? at::empty({(int64_t)bytes}, x.options().dtype(at::kByte)) : Tensor();
+    const void *const b = bias.defined() ? bias.const_data_ptr() : nullptr;
+    if (xs.defined())
+        check(api.row_int8_product(x.const_data_ptr(), xs.const_data_ptr<float>(), w.const_data_ptr(), scale.const_data_ptr<float>(), b, y.data_ptr(), dt, M, N, K,
+                                   bytes ? ws.data_ptr() : nullptr, bytes, current_stream(x)), "lowbit_row_int8_product");
+    else
+        check(api.row_int8_linear(x.const_data_ptr(), w.const_data_ptr(), scale.const_data_ptr<float>(), b, y.data_ptr(), dt, M, N, K,
+                                  bytes ? ws.data_ptr() : nullptr, bytes, current_stream(x)), "lowbit_row_int8_linear");
+    return y;
+}
+
+// a bias that the kernels add themselves
+bool plain_bias(const Tensor &bias, const Tensor &x, at::ScalarType dtype, int64_t N) {
+    return !bias.defined() || (bias.scalar_type() == dtype && bias.device() == x.device() && bias.dim() == 1 && bias.numel() == N &&
+                               bias.is_contiguous() && !differentiable(bias));
+}
+
+// The gradient that flows on to x, the quantization of x counting as the identity.  Holds the weight as ProductBackward does.
+struct RowInt8Backward : public torch::autograd::Node {
+    Tensor w, scale;
+    at::ScalarType x_dtype = at::kHalf;
+    at::DimVector x_shape;
+
+    std::string name() const override { return "RowInt8LinearBackward"; }
+
+    torch::autograd::variable_list apply(torch::autograd::variable_list &&grads) override {
+        if (!task_should_compute_output(0)) return {Tensor()};
+        const int64_t N = w.size(0), K = w.size(1);
+        const Tensor grad = grads[0].defined() ? grads[0].to(x_dtype).reshape({-1, N})
+                                               : at::zeros({c10::multiply_integers(x_shape) / K, N}, w.options().dtype(x_dtype));
+        c10::DeviceGuard guard(grad.device());
+        if (grad.device() != w.device()) throw Failed("the int8 weight is not where the forward found it");
+        if (differentiable(grad) || !nothing_watches(grad))  // (a second derivative, a transform: the dense product)
+            return {at::matmul(grad.to(at::kFloat), w.to(at::kFloat).mul_(scale.unsqueeze(-1))).to(x_dtype).view(x_shape)};
+        const Tensor g = whole_rows(grad);
+        const int64_t M = g.size(0);
+        const int dt = dtype_code(x_dtype);
+        Tensor gx = at::empty(x_shape, g.options());
+        const size_t bytes = api.row_int8_backward_workspace_bytes(dt, M, N, K);
+        const Tensor ws = bytes ? at::empty({(int64_t)bytes}, g.options().dtype(at::kByte)) : Tensor();
+        check(api.row_int8_backward(g.const_data_ptr(), w.const_data_ptr(), scale.const_data_ptr<float>(), gx.data_ptr(), dt, M, N, K,
+                                    bytes ? ws.data_ptr() : nullptr, bytes, current_stream(g)), "lowbit_row_int8_backward");
+        return {gx};
+    }
+};
+
+// y = Q(x) W^T (+ bias), with the gradient to x where x wants one; an undefined tensor when this is not the plain case
+Tensor row_int8_linear(const Tensor &x_in, const Tensor &w, const Tensor &scale, const Tensor &bias) {
+    if (!on_gpu(x_in) || x_in.dim() < 1 || x_in.numel() == 0 || dtype_code(x_in.scalar_type()) < 0 || !is_row_int8(w, scale, x_in, 0) ||
+        w.size(1) != x_in.size(-1) || w.size(1) > ROW_INT8_MOST_K || !nothing_watches(x_in) || x_in._fw_grad(/*level=*/0).defined() ||
+        !plain_bias(bias, x_in, x_in.scalar_type(), w.size(0))) return {};
+    if (!x_in.requires_grad() || !c10::GradMode::is_enabled()) return row_int8_any_product(whole_rows(x_in), Tensor(), w, scale, bias, x_in.scalar_type());
+    Tensor y;
+    auto node = std::shared_ptr<RowInt8Backward>(new RowInt8Backward(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(x_in));
+    node->w = w;
+    node->scale = scale;
+    node->x_dtype = x_in.scalar_type();
+    node->x_shape.assign(x_in.sizes().begin(), x_in.sizes().end());
+    {
+        c10::AutoGradMode no_grad(false);
+        y = row_int8_any_product(whole_rows(x_in.detach()), Tensor(), w, scale, bias, x_in.scalar_type());
+    }
+    torch::autograd::set_history(y, node);
+    return y;
+}
+
+// the same product of codes and their scales, in the type of dtype code `dt`; an undefined tensor when this is not the plain case
+Tensor row_int8_product(const Tensor &codes, const Tensor &xs, const Tensor &w, const Tensor &scale, const Tensor &bias, int dt) {
+    const at::ScalarType dtype = dt == LOWBIT_DT_F16 ? at::kHalf : dt == LOWBIT_DT_BF16 ? at::kBFloat16 : at::kFloat;
+    if (!on_gpu(codes) || codes.scalar_type() != at::kChar || codes.dim() < 1 || codes.numel() == 0 || !is_row_int8(w, scale, codes, 0) ||
+        w.size(1) != codes.size(-1) || w.size(1) > ROW_INT8_MOST_K || xs.device() != codes.device() || xs.scalar_type() != at::kFloat ||
+        xs.sizes() != codes.sizes().slice(0, codes.dim() - 1) || differentiable(xs) || !nothing_watches(codes) || !nothing_watches(xs) ||
+        !plain_bias(bias, codes, dtype, w.size(0))) return {};
+    return row_int8_any_product(whole_rows(codes), xs.contiguous(), w, scale, bias, dtype);
+}
+
 // ---- large copies between pageable host memory and the GPU, through two pinned buffers
 //
 // A pageable copy by the runtime ran at 29 GB/s up and, into memory the process has not touched yet, 7.5 GB/s down
@@ -575,6 +692,8 @@ PyObject *py_bind(PyObject *, PyObject *const *args, Py_ssize_t n) {
     BIND(last_error); BIND(blob_bytes); BIND(tileable); BIND(linear_scratch_bytes); BIND(linear);
     BIND(gated_mlp); BIND(dequantize_rows); BIND(dequantize); BIND(backward_ws); BIND(backward_workspace_bytes); BIND(backward_ws_applies); BIND(experts_workspace_bytes); BIND(experts_forward);
     BIND(block_fp8_quantize); BIND(block_fp8_quantize_weight); BIND(block_fp8_linear); BIND(block_fp8_linear_workspace_bytes);
+    BIND(row_int8_quantize); BIND(row_int8_linear); BIND(row_int8_linear_workspace_bytes); BIND(row_int8_product);
+    BIND(row_int8_product_workspace_bytes); BIND(row_int8_backward); BIND(row_int8_backward_workspace_bytes);
     BIND(block_fp8_backward); BIND(block_fp8_backward_workspace_bytes); BIND(block_fp8_experts); BIND(block_fp8_experts_workspace_bytes);
 #undef BIND
     Py_RETURN_NONE;
@@ -691,6 +810,39 @@ PyObject *py_block_fp8_experts(PyObject *, PyObject *const *args, Py_ssize_t n) 
     });
 }
 
+// row_int8_quantize(x) -> (codes, scale) or None
+PyObject *py_row_int8_quantize(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return answer_pair("row_int8_quantize", n, 1, [&] {
+        const Args a{args, n};
+        const Tensor &x = a.tensor(0);
+        NoGil free;
+        return row_int8_quantize(x);
+    });
+}
+
+// row_int8_linear(x, weight, scale, bias or None) -> y or None
+PyObject *py_row_int8_linear(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return answer("row_int8_linear", n, 4, [&] {
+        const Args a{args, n};
+        const Tensor &x = a.tensor(0), &w = a.tensor(1), &scale = a.tensor(2);
+        const Tensor bias = a.optional(3);
+        NoGil free;
+        return row_int8_linear(x, w, scale, bias);
+    });
+}
+
+// row_int8_product(codes, scale of the rows, weight, scale, bias or None, dtype code) -> y or None
+PyObject *py_row_int8_product(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return answer("row_int8_product", n, 6, [&] {
+        const Args a{args, n};
+        const Tensor &codes = a.tensor(0), &xs = a.tensor(1), &w = a.tensor(2), &scale = a.tensor(3);
+        const Tensor bias = a.optional(4);
+        const int dt = (int)a.integer(5);
+        NoGil free;
+        return row_int8_product(codes, xs, w, scale, bias, dt);
+    });
+}
+
 // upload(host tensor, device index) -> the tensor on that GPU, or None; complete when it returns
 PyObject *py_upload(PyObject *, PyObject *const *args, Py_ssize_t n) {
     return answer("upload", n, 2, [&] {
@@ -734,7 +886,8 @@ PyObject *py_holds(PyObject *, PyObject *const *args, Py_ssize_t n) {
 
 #define METHOD(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {METHOD(bind), METHOD(product), METHOD(linear), METHOD(linear_train), METHOD(gated), METHOD(embedding), METHOD(experts), METHOD(block_fp8_quantize),
-                         METHOD(block_fp8_linear), METHOD(block_fp8_experts), METHOD(upload),
+                         METHOD(block_fp8_linear), METHOD(block_fp8_experts), METHOD(row_int8_quantize), METHOD(row_int8_linear), METHOD(row_int8_product),
+                         METHOD(upload),
                          METHOD(download), METHOD(holds),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "lowbit_torch", "native host path of the low-bit layers", -1, methods};

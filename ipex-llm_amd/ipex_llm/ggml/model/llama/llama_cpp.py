@@ -513,6 +513,64 @@ def lowbit_block_fp8_experts_waves(tokens, top_k, n_experts, hidden, inter):
     return waves
 
 
+_lib.lowbit_row_int8_quantize.argtypes = [c_void_p, c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p]
+_lib.lowbit_row_int8_linear.argtypes = [c_void_p] * 5 + [c_int, c_int64, c_int64, c_int64, c_void_p, c_size_t, c_void_p]
+_lib.lowbit_row_int8_product.argtypes = [c_void_p] * 6 + [c_int, c_int64, c_int64, c_int64, c_void_p, c_size_t, c_void_p]
+_lib.lowbit_row_int8_backward.argtypes = [c_void_p] * 4 + [c_int, c_int64, c_int64, c_int64, c_void_p, c_size_t, c_void_p]
+_lib.lowbit_row_int8_plan.argtypes = [c_int, c_int, c_int64, c_int64, c_int64, ctypes.POINTER(c_int)]
+_lib.lowbit_row_int8_waves.argtypes = [c_int64, c_int64, c_int64]
+for _name in ("quantize", "linear", "product", "backward", "plan", "waves"):
+    getattr(_lib, f"lowbit_row_int8_{_name}").restype = c_int
+for _name in ("linear", "product", "backward"):
+    getattr(_lib, f"lowbit_row_int8_{_name}_workspace_bytes").argtypes = [c_int, c_int64, c_int64, c_int64]
+    getattr(_lib, f"lowbit_row_int8_{_name}_workspace_bytes").restype = c_size_t
+
+
+def lowbit_row_int8_quantize(x, dtype, rows, k, codes, scale, stream):
+    _check(_lib.lowbit_row_int8_quantize(x, dtype, rows, k, codes, scale, stream), "lowbit_row_int8_quantize")
+
+
+def lowbit_row_int8_linear(x, w, w_scale, bias, y, dtype, m, n, k, workspace, workspace_bytes, stream):
+    _check(_lib.lowbit_row_int8_linear(x, w, w_scale, bias, y, dtype, m, n, k, workspace, workspace_bytes, stream), "lowbit_row_int8_linear")
+
+
+def lowbit_row_int8_linear_workspace_bytes(dtype, m, n, k) -> int:
+    return _lib.lowbit_row_int8_linear_workspace_bytes(dtype, m, n, k)
+
+
+def lowbit_row_int8_product(codes, scale, w, w_scale, bias, y, dtype, m, n, k, workspace, workspace_bytes, stream):
+    _check(_lib.lowbit_row_int8_product(codes, scale, w, w_scale, bias, y, dtype, m, n, k, workspace, workspace_bytes, stream),
+           "lowbit_row_int8_product")
+
+
+def lowbit_row_int8_product_workspace_bytes(dtype, m, n, k) -> int:
+    return _lib.lowbit_row_int8_product_workspace_bytes(dtype, m, n, k)
+
+
+def lowbit_row_int8_backward(grad, w, w_scale, grad_x, dtype, m, n, k, workspace, workspace_bytes, stream):
+    _check(_lib.lowbit_row_int8_backward(grad, w, w_scale, grad_x, dtype, m, n, k, workspace, workspace_bytes, stream),
+           "lowbit_row_int8_backward")
+
+
+def lowbit_row_int8_backward_workspace_bytes(dtype, m, n, k) -> int:
+    return _lib.lowbit_row_int8_backward_workspace_bytes(dtype, m, n, k)
+
+
+def lowbit_row_int8_plan(dtype, backward, m, n, k):
+    """What lowbit_row_int8_linear or _backward runs: (rows, columns of a tile (0, 0: the kernel of few rows), parts of the sum, groups
+    of waves that share a tile's part)."""
+    plan4 = (c_int * 4)()
+    _check(_lib.lowbit_row_int8_plan(dtype, backward, m, n, k, plan4), "lowbit_row_int8_plan")
+    return tuple(plan4)
+
+
+def lowbit_row_int8_waves(m, n, k):
+    """Waves of a workgroup of the kernel of few rows, 0 where lowbit_row_int8_linear runs tiles."""
+    waves = _lib.lowbit_row_int8_waves(m, n, k)
+    _check(min(waves, 0), "lowbit_row_int8_waves")
+    return waves
+
+
 def lowbit_dequantize_rows(w, rows, n_rows, dst, qtype, n, k, layout, out_dtype, stream):
     _check(_lib.lowbit_dequantize_rows(w, rows, n_rows, dst, qtype, n, k, layout, out_dtype, stream),
            "lowbit_dequantize_rows")

@@ -1,0 +1,98 @@
+"""Row-scaled int8 without a GPU: refusals, conversion rules, what moves with a model and what does not."""
+import pytest
+import torch
+
+import row_int8_util as u
+import ipex_llm.ggml.model.llama.llama_cpp as ggml
+from ipex_llm.transformers import row_int8 as ri
+
+lib = ggml._lib
+P = 4096                                                     # an aligned address that nothing reads
+EARG, ESIZE, EDTYPE, ESHAPE = -1, -3, -4, -5
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def test_dequantize():
+    codes, scale = u.weight(gen(2), 30, 272)
+    assert torch.equal(ri.row_int8_dequantize(codes, scale), codes.float() * scale.unsqueeze(-1))
+    assert ri.row_int8_dequantize(codes[0], scale[0], torch.bfloat16).dtype == torch.bfloat16
+    for bad in ((codes, scale[:2]), (codes.float(), scale), (codes, scale.unsqueeze(-1))):
+        with pytest.raises(RuntimeError, match="fit together"):
+            ri.row_int8_dequantize(*bad)
+
+
+def test_the_steps_of_the_quantizer_round_as_the_oracle_does():
+    for dtype in (torch.float16, torch.bfloat16, torch.float32):
+        x = (torch.randn((9, 272), generator=gen(1)) * 5).to(dtype)
+        x[0] = 0
+        x[1] = (torch.arange(272) % 255 - 127).to(dtype) / 2
+        x[2, 3], x[3, 4] = float("nan"), float("-inf")
+        codes, scale = ri._quantize_steps(x)
+        want, ws = u.quantize(x)
+        assert torch.equal(codes.long(), want) and torch.equal(scale.nan_to_num(nan=-1), ws.nan_to_num(nan=-1))
+
+
+def test_host_tensors_are_refused():
+    w, ws = u.weight(gen(3), 16, 32)
+    x = torch.zeros((2, 32), dtype=torch.bfloat16)
+    for call in (lambda: ri.row_int8_linear(x, w, ws), lambda: ri.row_int8_quantize(x),
+                 lambda: ri.row_int8_product(w[:2], ws[:2], w, ws)):
+        with pytest.raises(RuntimeError, match="no CPU implementation"):
+            call()
+    with pytest.raises(RuntimeError, match="unsupported dtype"):
+        ri.row_int8_product(w[:2], ws[:2], w, ws, dtype=torch.float64)
+
+
+def test_abi_refuses_before_it_touches_the_gpu():
+    lin, product, back, q = lib.lowbit_row_int8_linear, lib.lowbit_row_int8_product, lib.lowbit_row_int8_backward, lib.lowbit_row_int8_quantize
+    assert lin(P, P, P, None, P, 3, 1, 16, 128, None, 0, None) == EDTYPE
+    assert lin(P, P, P, None, P, 0, -1, 16, 128, None, 0, None) == EARG
+    assert lin(P, P, P, None, P, 0, 1, 16, 120, None, 0, None) == ESHAPE
+    assert lin(P, P, P, None, P, 0, 1 << 22, 16, 128, None, 0, None) == ESIZE
+    assert lin(P, P, P, None, P, 0, 1, 1 << 23, 128, None, 0, None) == ESIZE
+    assert lin(P, P, P, None, P, 0, 1, 16, (1 << 17) + 16, None, 0, None) == ESIZE
+    assert lin(P, P, P, None, P, 0, 1, 16, 0, None, 0, None) == ESHAPE
+    assert lin(P + 8, P, P, None, P, 0, 1, 16, 128, None, 0, None) == EARG
+    assert lin(P, P, None, None, P, 0, 1, 16, 128, None, 0, None) == EARG
+    assert lin(P, P, P + 2, None, P, 0, 1, 16, 128, None, 0, None) == EARG
+    need = lib.lowbit_row_int8_linear_workspace_bytes(1, 512, 256, 512)
+    assert need >= 512 * 512 + 512 * 4
+    assert lin(P, P, P, None, P, 1, 512, 256, 512, None, 0, None) == ESIZE
+    assert lin(P, P, P, None, P, 1, 512, 256, 512, P, need - 1, None) == ESIZE
+    assert lin(P, P, P, None, P, 1, 512, 256, 512, P + 8, need, None) == ESIZE
+    assert lin(None, None, None, None, None, 1, 0, 256, 512, None, 0, None) == 0
+    assert lin(None, None, None, None, None, 1, 7, 0, 512, None, 0, None) == 0
+    assert product(P, None, P, P, None, P, 1, 4, 16, 128, None, 0, None) == EARG
+    assert product(P, P, P, P, None, P, 5, 4, 16, 128, None, 0, None) == EDTYPE
+    assert product(P, P, P, P, None, P, 1, 4, 16, 144, None, 0, None) == ESIZE       # (rows that do not fill whole blocks are copied)
+    assert back(P, P, P, P, 1, 4, 16, 128, None, 0, None) == ESIZE
+    assert back(P, P, P, P, 1, 4, 0, 128, None, 0, None) == ESHAPE
+    assert back(P, P, P, P, 7, 4, 16, 128, None, 0, None) == EDTYPE
+    assert back(None, None, None, None, 1, 0, 16, 128, None, 0, None) == 0
+    assert q(P, 0, -1, 128, P, P, None) == EARG and q(P, 0, 1, 120, P, P, None) == ESHAPE and q(P, 9, 1, 128, P, P, None) == EDTYPE
+    assert q(P, 0, 1, 1 << 23, P, P, None) == ESIZE and q(P, 0, 1, -16, P, P, None) == EARG and q(P, 0, 1, 128, None, P, None) == EARG
+    assert q(None, 0, 0, 128, None, None, None) == 0 and q(None, 0, 5, 0, None, None, None) == 0
+    with pytest.raises(Exception, match="plan"):
+        ggml.lowbit_row_int8_plan(0, 0, 0, 16, 16)
+    with pytest.raises(Exception, match="waves"):
+        ggml.lowbit_row_int8_waves(1, 16, 24)
+
+
+def test_plans_cover_every_size():
+    """Whatever is asked for has a plan whose parts have blocks, and a workspace that holds them."""
+    for m in (1, 4, 5, 16, 17, 64, 300, 4000):
+        for n in (1, 64, 1000, 28672):
+            for k in (16, 128, 144, 4096, 1 << 17):
+                rows, cols, splits, groups = ggml.lowbit_row_int8_plan(1, 0, m, n, k)
+                assert (rows == 0) == (ggml.lowbit_row_int8_waves(m, n, k) > 0)
+                assert 1 <= splits <= (k + 127) // 128 and groups in (1, 2)
+                if rows:
+                    need = m * ((k + 127) // 128 * 128) + m * 4 + (splits * m * n * 4 if splits > 1 else 0)
+                    assert ggml.lowbit_row_int8_linear_workspace_bytes(1, m, n, k) >= need
+                for dtype, terms in ((0, 1), (2, 2)):
+                    splits = ggml.lowbit_row_int8_plan(dtype, 1, m, n, k)[2]
+                    assert 1 <= splits <= (n + 63) // 64 * terms
+                    assert ggml.lowbit_row_int8_backward_workspace_bytes(dtype, m, n, k) >= m * n * 2 * terms + (splits * m * k * 4 if splits > 1 else 0)

@@ -1,0 +1,200 @@
+"""Row-scaled int8: quantizer, products and gradients against whole numbers and 64 bits on the host."""
+import math
+
+import pytest
+import torch
+
+import row_int8_util as u
+from gpu_util import DT, ggml, stream
+from ipex_llm.transformers import row_int8 as ri
+
+pytestmark = pytest.mark.gpu
+HALF = [torch.float16, torch.bfloat16]
+ALL = HALF + [torch.float32]
+IDS = {torch.float16: "f16", torch.bfloat16: "bf16", torch.float32: "f32"}
+
+
+def ids(v):
+    return IDS.get(v) if isinstance(v, torch.dtype) else None
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def same(a, b):
+    """Equal values, NaN where NaN."""
+    return torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(nan=0.0), b.nan_to_num(nan=0.0))
+
+
+# ---------------------------------------------------------------- quantizer
+
+def awkward(x):
+    """Rows of every kind: zeros, one value, ties of the rounding, the least and largest numbers of the type."""
+    info = torch.finfo(x.dtype)
+    if x.shape[0] > 7:
+        x[0] = 0
+        x[1] = 0
+        x[1, -1] = 3.0
+        x[2] = (torch.arange(x.shape[1]) % 255 - 127).to(x.dtype)           # codes themselves
+        x[3] *= info.smallest_normal
+        x[4] = info.max
+        x[4, ::2] = info.tiny
+        x[5, 0] = info.smallest_normal / 4
+        x[5, 1:] = 0
+        x[6] = (torch.arange(x.shape[1]) % 255 - 127).to(x.dtype) / 2       # every other one half way between two codes
+        x[6, 0] = 127
+        x[7] = torch.linspace(-1, 1, x.shape[1]).to(x.dtype) * 14
+    return x
+
+
+@pytest.mark.parametrize("m,k", [(1, 16), (1, 128), (9, 144), (33, 1024), (10, 1040), (130, 2112), (300, 4096), (9, 4112), (8, 8208), (8, 28672), (8, 40016)])
+@pytest.mark.parametrize("dtype", ALL, ids=ids)
+def test_quantize(dtype, m, k):
+    x = awkward((torch.randn((m, k), generator=gen(m)) * 3).to(dtype))
+    codes, scale = ri.row_int8_quantize(x.cuda())
+    want, ws = u.quantize(x)
+    assert codes.dtype == torch.int8 and codes.shape == x.shape and scale.shape == (m,)
+    assert torch.equal(scale.cpu(), ws)
+    assert torch.equal(codes.cpu().long(), want)
+    assert torch.equal(ri.row_int8_dequantize(codes, scale).cpu(), codes.cpu().float() * ws.unsqueeze(-1))
+
+
+def test_quantize_decides_next_to_every_border_as_the_true_quotient_does():
+    """float32 values next to each border between two codes, on both sides and on it where it is a number."""
+    rows = []
+    for a in (1.0, 127.0, 254.0, 1.2345678, 3.1e38, 2.0 ** -90, 1.0 - 2.0 ** -24, 16777213.0):
+        top = torch.tensor(a, dtype=torch.float32)
+        border = ((torch.arange(-127, 127).double() + 0.5) * top.double() / 127).float()
+        near = torch.cat([border, torch.nextafter(border, torch.tensor(math.inf)), torch.nextafter(border, torch.tensor(-math.inf)), top.view(1), -top.view(1)])
+        rows.append(torch.nn.functional.pad(near, (0, -near.numel() % 16)))
+    x = torch.stack(rows)
+    codes, scale = ri.row_int8_quantize(x.cuda())
+    want, ws = u.quantize(x)
+    assert torch.equal(codes.cpu().long(), want) and torch.equal(scale.cpu(), ws)
+
+
+def test_quantize_every_finite_bfloat16():
+    """All magnitudes beside each of the mantissas that a row's largest value can have."""
+    v = torch.arange(0, 0x7f80, dtype=torch.int32).to(torch.int16).view(torch.bfloat16)
+    for mantissa in range(0, 128, 3):
+        top = torch.tensor(0x4300 + mantissa, dtype=torch.int32).to(torch.int16).view(torch.bfloat16)
+        x = v[v <= top]
+        x = torch.nn.functional.pad(x, (0, -x.numel() % 16)).view(1, -1)
+        codes, _ = ri.row_int8_quantize(x.cuda())
+        assert torch.equal(codes.cpu().long(), u.quantize(x)[0])
+
+
+@pytest.mark.parametrize("dtype", ALL, ids=ids)
+@pytest.mark.parametrize("m,n", [(5, 32), (40, 100)], ids=["few_rows", "tiles"])
+def test_rows_with_nan_and_infinity(dtype, m, n):
+    x = torch.randn((m, 400), generator=gen(3)).to(dtype)
+    x[0, 5], x[1, 200], x[1, 201], x[2, 399] = math.nan, math.inf, math.nan, -math.inf
+    codes, scale = ri.row_int8_quantize(x.cuda())
+    assert scale.cpu().isnan().tolist() == [True] * 3 + [False] * (m - 3) and not codes[:3].any()
+    w, ws = u.weight(gen(4), n, 400)
+    ws[7] = math.nan
+    y = ri.row_int8_linear(x.cuda(), w.cuda(), ws.cuda()).cpu()
+    assert same(y, u.product(x, w, ws))
+    assert y[:3].isnan().all() and y[:, 7].isnan().all() and y[3:, 8:].isfinite().all()
+
+
+# ---------------------------------------------------------------- products
+
+def check_product(dtype, m, n, k, seed=0):
+    g = gen(m * 7 + n + seed)
+    x = (torch.randn((m, k), generator=g) * torch.exp2(torch.randint(-3, 4, (m, 1), generator=g).float())).to(dtype)
+    w, ws = u.weight(g, n, k)
+    bias = torch.randn(n, generator=g).to(dtype)
+    xd, wd, sd, bd = x.cuda(), w.cuda(), ws.cuda(), bias.cuda()
+    y = ri.row_int8_linear(xd, wd, sd)
+    assert y.dtype == dtype and y.shape == (m, n)
+    assert torch.equal(y.cpu(), u.product(x, w, ws))
+    assert torch.equal(ri.row_int8_linear(xd, wd, sd, bd).cpu(), u.product(x, w, ws, bias))
+    assert torch.equal(ri.row_int8_product(*ri.row_int8_quantize(xd), wd, sd, bd, dtype).cpu(), u.product(x, w, ws, bias))
+
+
+@pytest.mark.parametrize("m,n,k", u.SHAPES)
+@pytest.mark.parametrize("dtype", ALL, ids=ids)
+def test_product_equals_its_float32_steps(dtype, m, n, k):
+    check_product(dtype, m, n, k)
+
+
+def test_longest_row():
+    """The largest sum that K = 2^17 can make, 127 * 127 * 2^17, still fits 32 bits."""
+    k = 1 << 17
+    for m in (1, 40):
+        x = torch.full((m, k), 2.0)
+        w = torch.full((33, k), 127, dtype=torch.int8)
+        w[1] = -127
+        ws = torch.ones(33)
+        y = ri.row_int8_linear(x.cuda(), w.cuda(), ws.cuda()).cpu()
+        assert torch.equal(y, u.product(x, w, ws))
+
+
+# ---------------------------------------------------------------- gradients
+
+def back_tolerance(dtype):
+    """Of the 2-norm.  Each g * ws: float32's product, and half a unit of 11 bits (float32: of 22) of values evenly spread in a binade,
+    1 / sqrt(12) of a unit at rms, 2^-11 * 0.29 * 1.4 at most; both average over a sum, so the result's share is the same.  Sums in float32, a rounding of
+    2^-24 for each of up to 300 instructions, their squares summed: sqrt(300) * 2^-24 = 1e-6.  The result: half a unit of its type."""
+    if dtype == torch.float32:
+        return 2.0 ** -22 + 1e-6 + 2.0 ** -24
+    return 2.0 ** -12 + 1e-6 + torch.finfo(dtype).eps / 2
+
+
+@pytest.mark.parametrize("m,n,k", u.BACK_SHAPES)
+@pytest.mark.parametrize("dtype", ALL, ids=ids)
+def test_gradient(dtype, m, n, k):
+    g = gen(m + n)
+    x = torch.randn((m, k), generator=g).to(dtype).cuda().requires_grad_()
+    w, ws = u.weight(g, n, k)
+    ws = ws * torch.exp2(torch.randint(-6, 7, (n,), generator=g).float())
+    grad = (torch.randn((m, n), generator=g) * torch.exp2(torch.randint(-9, 3, (m, 1), generator=g).float())).to(dtype)
+    y = ri.row_int8_linear(x, w.cuda(), ws.cuda())
+    gx, = torch.autograd.grad(y, x, grad.cuda())
+    want = (grad.double() * ws.double()) @ w.double()
+    assert gx.dtype == dtype and gx.shape == x.shape
+    off = (gx.cpu().double() - want).norm(dim=1)
+    assert (off <= back_tolerance(dtype) * want.norm(dim=1)).all(), (off / want.norm(dim=1)).max()
+
+
+@pytest.mark.parametrize("dtype", ALL, ids=ids)
+def test_gradient_rows_of_awkward_numbers(dtype):
+    info = torch.finfo(dtype)
+    g = gen(5)
+    w, ws = u.weight(g, 70, 144)
+    grad = torch.randn((8, 70), generator=g).to(dtype)
+    grad[0] = 0
+    grad[1] = 0
+    grad[1, 69] = info.max
+    grad[2] *= info.tiny
+    grad[3, 5], grad[4, 69], grad[5, 0] = math.nan, math.inf, -math.inf
+    x = torch.randn((8, 144), generator=g).to(dtype).cuda().requires_grad_()
+    gx, = torch.autograd.grad(ri.row_int8_linear(x, w.cuda(), ws.cuda()), x, grad.cuda())
+    gx = gx.cpu()
+    assert gx[3:6].isnan().all() and not gx[0].any()
+    want = (grad.double() * ws.double()) @ w.double()
+    for row in (1, 6, 7):
+        assert (gx[row].double() - want[row]).norm() <= back_tolerance(dtype) * want[row].norm()
+    # (the second row's products lie among the type's subnormals: a unit of those)
+    assert (gx[2].double() - want[2]).abs().max() <= info.tiny * info.eps + back_tolerance(dtype) * want[2].norm()
+
+
+def test_gradient_against_differences():
+    """The product is linear in x once x's codes are exact: differences of one code step against the gradient."""
+    g = gen(6)
+    w, ws = u.weight(g, 48, 64)
+    x = torch.randint(-100, 101, (3, 64), generator=g).float()
+    x[:, 0] = 127
+    grad = torch.randn((3, 48), generator=g)
+    wd, sd = w.cuda(), ws.cuda()
+    xd = x.cuda().requires_grad_()
+    gx, = torch.autograd.grad(ri.row_int8_linear(xd, wd, sd), xd, grad.cuda())
+    for row, col in [(0, 1), (1, 30), (2, 63)]:
+        step = torch.zeros_like(x)
+        step[row, col] = 1
+        up, down = (ri.row_int8_linear((x + s).cuda(), wd, sd).cpu().double() for s in (step, -step))
+        d = ((up - down) / 2 * grad.double()).sum()
+        # 48 results, each rounded to 2^-24 of itself
+        assert abs(gx[row, col].cpu().double() - d) <= 2.0 ** -22 * (up[row].abs() * grad[row].abs()).sum() + 1e-6 * gx[row].norm().cpu()
