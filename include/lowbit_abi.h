@@ -408,6 +408,45 @@ int lowbit_row_int8_backward(const void *grad, const void *w, const float *w_sca
 int lowbit_row_int8_plan(int dtype, int backward, int64_t M, int64_t N, int64_t K, int *plan4);
 /* Waves of a workgroup where lowbit_row_int8_linear runs the kernel of few rows, 0 where it runs tiles (negative: an error). */
 int lowbit_row_int8_waves(int64_t M, int64_t N, int64_t K);
+/* A mixture-of-experts block: y[t, :] = sum_j topk_weight[t, j] * (Q(act(g) .* u) * down[e]^T), (g | u) = Q(x_t) * gate_up[e]^T, e =
+ * topk_ids[t, j]; a pair whose id lies outside [0, n_experts) counts nothing.  gate_up [n_experts, 2 inter, hidden] (gate rows first)
+ * and down [n_experts, hidden, inter] are the experts' codes one after the other, their scales [n_experts, 2 inter] and [n_experts, hidden]
+ * (16-byte aligned); hidden and inter are multiples of 16, at most 2^17.  act(g) .* u, the pairs' results and their sum are float32.  Limits as in
+ * lowbit_experts_forward, pairs at most 2^21. */
+size_t lowbit_row_int8_experts_workspace_bytes(int64_t tokens, int top_k, int n_experts, int64_t hidden, int64_t inter);
+int lowbit_row_int8_experts(const void *x, const int64_t *topk_ids, const void *topk_weight, int weight_dtype, int64_t tokens, int top_k,
+                            int n_experts, const void *gate_up, const float *gate_up_scale, const void *down, const float *down_scale,
+                            void *workspace, size_t workspace_bytes, void *y, int act_dtype, int64_t hidden, int64_t inter, int act,
+                            void *stream);
+/* What it runs as: plan4 = {rows of a tile of the first product, rows and columns of one of the second (0: each pair streams its weights), 1 if a launch
+ * of its own places the pairs} */
+int lowbit_row_int8_experts_plan(int64_t tokens, int top_k, int n_experts, int64_t hidden, int64_t inter, int *plan4);
+/* Waves of a workgroup of its second launch where each pair streams its weights, 0 where the pairs are sorted (negative: an error). */
+int lowbit_row_int8_experts_waves(int64_t tokens, int top_k, int n_experts, int64_t hidden, int64_t inter);
+
+/* ---- the router of a mixture-of-experts block
+ *
+ * z = x[tokens, hidden] * router[n_experts, hidden]^T, s = softmax or sigmoid of z; topk_ids: the top_k largest z (s + bias[n_experts] where bias is
+ * not null), in descending order, ties to the lowest index, NaN above all numbers; topk_weight = factor * s of those, divided by their
+ * sum if renormalize.  Sums, z and s are float64, so that the choice depends on no order of summation.  hidden is a multiple of 8, n_experts at
+ * most 1024, top_k 64.  logits: z [tokens, n_experts] for the backward, or null. */
+#define LOWBIT_SCORE_SOFTMAX 0
+#define LOWBIT_SCORE_SIGMOID 1
+size_t lowbit_route_workspace_bytes(int64_t tokens, int n_experts, int64_t hidden);
+int lowbit_route(const void *x, int x_dtype, const void *router, int router_dtype, const float *bias, int64_t tokens, int n_experts, int64_t hidden,
+                 int top_k, int score, int renormalize, float factor, float *topk_weight, int64_t *topk_ids, double *logits, void *workspace,
+                 size_t workspace_bytes, void *stream);
+/* The gradients of x (in x_dtype) and of the router (in router_dtype), either may be null, for grad [tokens, top_k] of topk_weight; the choice counts as
+ * constant.  The gradient of z is rounded to float32, sums are float32, one rounding. */
+size_t lowbit_route_backward_workspace_bytes(int64_t tokens, int n_experts, int64_t hidden);
+int lowbit_route_backward(const float *grad, const double *logits, const int64_t *topk_ids, const void *x, int x_dtype, const void *router,
+                          int router_dtype, int64_t tokens, int n_experts, int64_t hidden, int top_k, int score, int renormalize, float factor,
+                          void *grad_x, void *grad_router, void *workspace, size_t workspace_bytes, void *stream);
+/* lowbit_route and lowbit_row_int8_experts in one call: a whole layer. */
+size_t lowbit_row_int8_moe_workspace_bytes(int64_t tokens, int top_k, int n_experts, int64_t hidden, int64_t inter);
+int lowbit_row_int8_moe(const void *x, const void *router, int router_dtype, const float *bias, int64_t tokens, int top_k, int n_experts, int score,
+                        int renormalize, float factor, const void *gate_up, const float *gate_up_scale, const void *down, const float *down_scale,
+                        void *workspace, size_t workspace_bytes, void *y, int act_dtype, int64_t hidden, int64_t inter, int act, void *stream);
 
 #ifdef __cplusplus
 }

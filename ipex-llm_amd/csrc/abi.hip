@@ -74,7 +74,7 @@ size_t block_fp8_experts_workspace_bytes(int tokens, int top_k, int n_exp, int H
 int launch_block_fp8_experts(const void *x, const int64_t *ids, const void *weight, int w_dtype, int tokens, int top_k, int n_exp,
                              const uint8_t *gate_up, const float *gate_up_scale, const uint8_t *down, const float *down_scale, void *workspace,
                              void *out, int act_dtype, int H, int I, int act, hipStream_t st);
-int launch_row_int8_quantize(const void *x, int dtype, int64_t rows, int K, uint8_t *codes, int ldc, float *scale, hipStream_t st);
+int launch_row_int8_quantize(const void *x, int dtype, int64_t rows, int K, uint8_t *codes, int ldc, float *scale, const int32_t *limit, hipStream_t st);
 size_t row_int8_linear_workspace_bytes(int M, int N, int K);
 void row_int8_linear_plan(int M, int N, int K, int *plan4);
 int row_int8_linear_waves(int M, int N, int K);
@@ -86,6 +86,18 @@ int launch_row_int8_product(const uint8_t *codes, const float *xs, const uint8_t
 size_t row_int8_back_workspace_bytes(int dtype, int M, int N, int K);
 void row_int8_back_plan(int dtype, int M, int N, int K, int *plan4);
 int launch_row_int8_back(const void *grad, const uint8_t *w, const float *ws, void *gx, int dtype, int M, int N, int K, uint8_t *space, hipStream_t st);
+size_t row_int8_experts_workspace_bytes(int tokens, int top_k, int n_exp, int H, int I);
+void row_int8_experts_plan(int tokens, int top_k, int n_exp, int H, int I, int *plan4);
+int row_int8_experts_waves(int tokens, int top_k, int n_exp, int H, int I);
+int launch_row_int8_experts(const void *x, const int64_t *ids, const void *weight, int w_dtype, int tokens, int top_k, int n_exp,
+                            const uint8_t *gate_up, const float *gate_up_scale, const uint8_t *down, const float *down_scale, void *workspace,
+                            void *out, int act_dtype, int H, int I, int act, hipStream_t st);
+size_t route_workspace_bytes(int T, int E, int H);
+int launch_route(const void *x, int x_dtype, const void *router, int r_dtype, const float *bias, int T, int E, int H, int top_k, bool sigmoid,
+                 bool renormalize, float factor, float *w, int64_t *ids, double *z, void *space, hipStream_t st);
+size_t route_backward_workspace_bytes(int T, int E, int H);
+int launch_route_backward(const float *grad, const double *z, const int64_t *ids, const void *x, int x_dtype, const void *router, int r_dtype, int T,
+                          int E, int H, int top_k, bool sigmoid, bool renormalize, float factor, void *gx, void *gr, uint8_t *space, hipStream_t st);
 int launch_grouped_gemm(const void *x, const void *const *w, const void *const *w_up, void *y, const int32_t *offsets,
                         int n_groups, int total_rows, int qtype, int act_dtype, int N, int K, int act, void *workspace,
                         size_t workspace_bytes, hipStream_t st);
@@ -913,7 +925,7 @@ int lowbit_row_int8_quantize(const void *x, int dtype, int64_t rows, int64_t K, 
     if (rows == 0 || K == 0) return 0;
     if (!x || !codes || !scale || !aligned16(x) || !aligned16(codes) || !aligned4(scale)) return fail(LOWBIT_EARG, "%s: null or misaligned pointer", what);
     if (rows > (int64_t)1 << 40) return fail(LOWBIT_ESIZE, "%s: too many rows", what);
-    return check_launch(launch_row_int8_quantize(x, dtype, rows, (int)K, (uint8_t *)codes, (int)K, scale, (hipStream_t)stream), what);
+    return check_launch(launch_row_int8_quantize(x, dtype, rows, (int)K, (uint8_t *)codes, (int)K, scale, nullptr, (hipStream_t)stream), what);
 }
 
 size_t lowbit_row_int8_linear_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K) {
@@ -981,6 +993,157 @@ int lowbit_row_int8_backward(const void *grad, const void *w, const float *w_sca
     if (int rc = check_space(what, workspace, workspace_bytes, row_int8_back_workspace_bytes(dtype, (int)M, (int)N, (int)K))) return rc;
     return check_launch(launch_row_int8_back(grad, (const uint8_t *)w, w_scale, grad_x, dtype, (int)M, (int)N, (int)K, (uint8_t *)workspace,
                                              (hipStream_t)stream), what);
+}
+
+static bool row_int8_experts_ok(int64_t tokens, int64_t top_k, int64_t n_experts, int64_t hidden, int64_t inter) {
+    return experts_sizes_ok(tokens, top_k, n_experts, hidden, inter) && tokens * top_k <= 1 << 21 && hidden <= 1 << 17 && inter <= 1 << 17;
+}
+
+size_t lowbit_row_int8_experts_workspace_bytes(int64_t tokens, int top_k, int n_experts, int64_t hidden, int64_t inter) {
+    if (!row_int8_experts_ok(tokens, top_k, n_experts, hidden, inter) || hidden % 16 || inter % 16) return 0;
+    return row_int8_experts_workspace_bytes((int)tokens, top_k, n_experts, (int)hidden, (int)inter);
+}
+
+int lowbit_row_int8_experts_plan(int64_t tokens, int top_k, int n_experts, int64_t hidden, int64_t inter, int *plan4) {
+    if (!row_int8_experts_ok(tokens, top_k, n_experts, hidden, inter) || hidden % 16 || inter % 16 || !plan4)
+        return fail(LOWBIT_EARG, "lowbit_row_int8_experts_plan: sizes that lowbit_row_int8_experts does not take, or plan4 null");
+    row_int8_experts_plan((int)tokens, top_k, n_experts, (int)hidden, (int)inter, plan4);
+    return 0;
+}
+
+int lowbit_row_int8_experts_waves(int64_t tokens, int top_k, int n_experts, int64_t hidden, int64_t inter) {
+    if (!row_int8_experts_ok(tokens, top_k, n_experts, hidden, inter) || hidden % 16 || inter % 16)
+        return fail(LOWBIT_EARG, "lowbit_row_int8_experts_waves: sizes that lowbit_row_int8_experts does not take");
+    return row_int8_experts_waves((int)tokens, top_k, n_experts, (int)hidden, (int)inter);
+}
+
+// What the experts' call and the whole layer's ask of their weights and sizes
+static int check_row_int8_experts(const char *what, int act_dtype, int64_t tokens, int top_k, int n_experts, const void *gate_up, const float *gate_up_scale,
+                                  const void *down, const float *down_scale, const void *x, const void *y, int64_t hidden, int64_t inter, int act) {
+    if (act_dtype != LOWBIT_DT_F16 && act_dtype != LOWBIT_DT_BF16 && act_dtype != LOWBIT_DT_F32) return fail(LOWBIT_EDTYPE, "%s: unsupported element type", what);
+    if (act != LOWBIT_ACT_SILU && act != LOWBIT_ACT_GELU)
+        return fail(LOWBIT_EARG, "%s: activation must be LOWBIT_ACT_SILU or LOWBIT_ACT_GELU", what);
+    if (!row_int8_experts_ok(tokens, top_k, n_experts, hidden, inter))
+        return fail(LOWBIT_ESIZE, "%s: top_k must be 1 .. 64, experts 1 .. 4096, pairs at most 2^21, hidden and inter 2^17", what);
+    if (hidden % 16 || inter % 16) return fail(LOWBIT_ESHAPE, "%s: hidden and inter must be multiples of 16", what);
+    if (!x || !gate_up || !gate_up_scale || !down || !down_scale || !y || !aligned16(x) || !aligned16(y) || !aligned16(gate_up) || !aligned16(down) ||
+        !aligned16(gate_up_scale) || !aligned16(down_scale))
+        return fail(LOWBIT_EARG, "%s: null or misaligned pointer", what);
+    return 0;
+}
+
+int lowbit_row_int8_experts(const void *x, const int64_t *topk_ids, const void *topk_weight, int weight_dtype, int64_t tokens, int top_k,
+                            int n_experts, const void *gate_up, const float *gate_up_scale, const void *down, const float *down_scale,
+                            void *workspace, size_t workspace_bytes, void *y, int act_dtype, int64_t hidden, int64_t inter, int act,
+                            void *stream) {
+    const char *what = "lowbit_row_int8_experts";
+    if (weight_dtype != LOWBIT_DT_F16 && weight_dtype != LOWBIT_DT_BF16 && weight_dtype != LOWBIT_DT_F32)
+        return fail(LOWBIT_EDTYPE, "%s: routing weights must be f16, bf16 or f32", what);
+    if (tokens == 0) return 0;
+    if (int rc = check_row_int8_experts(what, act_dtype, tokens, top_k, n_experts, gate_up, gate_up_scale, down, down_scale, x, y, hidden, inter, act)) return rc;
+    if (!topk_ids || !topk_weight || (((uintptr_t)topk_ids) & 7)) return fail(LOWBIT_EARG, "%s: null or misaligned pointer", what);
+    if (int rc = check_space(what, workspace, workspace_bytes, row_int8_experts_workspace_bytes((int)tokens, top_k, n_experts, (int)hidden, (int)inter)))
+        return rc;
+    return check_launch(launch_row_int8_experts(x, topk_ids, topk_weight, weight_dtype, (int)tokens, top_k, n_experts, (const uint8_t *)gate_up,
+                                                gate_up_scale, (const uint8_t *)down, down_scale, workspace, y, act_dtype, (int)hidden,
+                                                (int)inter, act, (hipStream_t)stream), what);
+}
+
+// ---- the router
+
+static bool float_type(int dtype) { return dtype == LOWBIT_DT_F16 || dtype == LOWBIT_DT_BF16 || dtype == LOWBIT_DT_F32; }
+
+static bool route_ok(int64_t tokens, int64_t n_experts, int64_t hidden) {
+    return tokens > 0 && tokens <= 1 << 21 && n_experts > 0 && n_experts <= 1024 && hidden > 0 && hidden <= 1 << 20 && hidden % 8 == 0;
+}
+
+static int check_route(const char *what, int x_dtype, int r_dtype, int64_t tokens, int n_experts, int64_t hidden, int top_k, int score) {
+    if (!float_type(x_dtype) || !float_type(r_dtype)) return fail(LOWBIT_EDTYPE, "%s: unsupported element type", what);
+    if (tokens < 0 || hidden <= 0 || n_experts <= 0) return fail(LOWBIT_EARG, "%s: sizes must be positive", what);
+    if (score != LOWBIT_SCORE_SOFTMAX && score != LOWBIT_SCORE_SIGMOID) return fail(LOWBIT_EARG, "%s: score must be LOWBIT_SCORE_SOFTMAX or LOWBIT_SCORE_SIGMOID", what);
+    if (hidden % 8) return fail(LOWBIT_ESHAPE, "%s: hidden=%lld is not a multiple of 8", what, (long long)hidden);
+    if (tokens > 1 << 21 || n_experts > 1024 || hidden > 1 << 20) return fail(LOWBIT_ESIZE, "%s: needs at most 2^21 tokens, 1024 experts and rows of 2^20", what);
+    if (top_k < 1 || top_k > 64 || top_k > n_experts) return fail(LOWBIT_ESIZE, "%s: top_k must be 1 .. 64 and at most the number of experts", what);
+    return 0;
+}
+
+size_t lowbit_route_workspace_bytes(int64_t tokens, int n_experts, int64_t hidden) {
+    return route_ok(tokens, n_experts, hidden) ? route_workspace_bytes((int)tokens, n_experts, (int)hidden) : 0;
+}
+
+int lowbit_route(const void *x, int x_dtype, const void *router, int router_dtype, const float *bias, int64_t tokens, int n_experts, int64_t hidden,
+                 int top_k, int score, int renormalize, float factor, float *topk_weight, int64_t *topk_ids, double *logits, void *workspace,
+                 size_t workspace_bytes, void *stream) {
+    const char *what = "lowbit_route";
+    if (int rc = check_route(what, x_dtype, router_dtype, tokens, n_experts, hidden, top_k, score)) return rc;
+    if (tokens == 0) return 0;
+    if (!x || !router || !topk_weight || !topk_ids || !aligned16(x) || !aligned16(router) || !aligned4(bias) || !aligned4(topk_weight) ||
+        (((uintptr_t)topk_ids | (uintptr_t)logits) & 7))
+        return fail(LOWBIT_EARG, "%s: null or misaligned pointer", what);
+    if (int rc = check_space(what, workspace, workspace_bytes, route_workspace_bytes((int)tokens, n_experts, (int)hidden))) return rc;
+    return check_launch(launch_route(x, x_dtype, router, router_dtype, bias, (int)tokens, n_experts, (int)hidden, top_k, score == LOWBIT_SCORE_SIGMOID,
+                                     renormalize != 0, factor, topk_weight, topk_ids, logits, workspace, (hipStream_t)stream), what);
+}
+
+size_t lowbit_route_backward_workspace_bytes(int64_t tokens, int n_experts, int64_t hidden) {
+    return route_ok(tokens, n_experts, hidden) ? route_backward_workspace_bytes((int)tokens, n_experts, (int)hidden) : 0;
+}
+
+int lowbit_route_backward(const float *grad, const double *logits, const int64_t *topk_ids, const void *x, int x_dtype, const void *router,
+                          int router_dtype, int64_t tokens, int n_experts, int64_t hidden, int top_k, int score, int renormalize, float factor,
+                          void *grad_x, void *grad_router, void *workspace, size_t workspace_bytes, void *stream) {
+    const char *what = "lowbit_route_backward";
+    if (int rc = check_route(what, x_dtype, router_dtype, tokens, n_experts, hidden, top_k, score)) return rc;
+    if (tokens == 0) return fail(LOWBIT_EARG, "%s: needs a token", what);
+    if (!grad || !logits || !topk_ids || !x || !router || !aligned16(x) || !aligned16(router) || !aligned4(grad) || !aligned16(grad_x) ||
+        !aligned16(grad_router) || (((uintptr_t)topk_ids | (uintptr_t)logits) & 7))
+        return fail(LOWBIT_EARG, "%s: null or misaligned pointer", what);
+    if (int rc = check_space(what, workspace, workspace_bytes, route_backward_workspace_bytes((int)tokens, n_experts, (int)hidden))) return rc;
+    return check_launch(launch_route_backward(grad, logits, topk_ids, x, x_dtype, router, router_dtype, (int)tokens, n_experts, (int)hidden, top_k,
+                                              score == LOWBIT_SCORE_SIGMOID, renormalize != 0, factor, grad_x, grad_router, (uint8_t *)workspace,
+                                              (hipStream_t)stream), what);
+}
+
+// ---- router and int8 experts in one call
+
+struct MoeSpace {
+    size_t weight, ids, rest, bytes;
+};
+static MoeSpace moe_space(int64_t tokens, int top_k, int n_experts, int64_t hidden, int64_t inter) {
+    auto whole = [](size_t bytes) { return (bytes + 255) & ~(size_t)255; };
+    const size_t route = route_workspace_bytes((int)tokens, n_experts, (int)hidden);
+    const size_t experts = row_int8_experts_workspace_bytes((int)tokens, top_k, n_experts, (int)hidden, (int)inter);
+    MoeSpace s;
+    s.weight = 0;
+    s.ids = whole((size_t)tokens * top_k * sizeof(float));
+    s.rest = s.ids + whole((size_t)tokens * top_k * sizeof(int64_t));
+    s.bytes = s.rest + (route > experts ? route : experts);  // (the router's sums are read before the experts write)
+    return s;
+}
+
+size_t lowbit_row_int8_moe_workspace_bytes(int64_t tokens, int top_k, int n_experts, int64_t hidden, int64_t inter) {
+    if (!route_ok(tokens, n_experts, hidden) || !row_int8_experts_ok(tokens, top_k, n_experts, hidden, inter) || hidden % 16 || inter % 16) return 0;
+    return moe_space(tokens, top_k, n_experts, hidden, inter).bytes;
+}
+
+int lowbit_row_int8_moe(const void *x, const void *router, int router_dtype, const float *bias, int64_t tokens, int top_k, int n_experts, int score,
+                        int renormalize, float factor, const void *gate_up, const float *gate_up_scale, const void *down, const float *down_scale,
+                        void *workspace, size_t workspace_bytes, void *y, int act_dtype, int64_t hidden, int64_t inter, int act, void *stream) {
+    const char *what = "lowbit_row_int8_moe";
+    if (int rc = check_route(what, act_dtype, router_dtype, tokens, n_experts, hidden, top_k, score)) return rc;
+    if (tokens == 0) return 0;
+    if (int rc = check_row_int8_experts(what, act_dtype, tokens, top_k, n_experts, gate_up, gate_up_scale, down, down_scale, x, y, hidden, inter, act)) return rc;
+    if (!router || !aligned16(router) || !aligned4(bias)) return fail(LOWBIT_EARG, "%s: null or misaligned pointer", what);
+    const MoeSpace at = moe_space(tokens, top_k, n_experts, hidden, inter);
+    if (int rc = check_space(what, workspace, workspace_bytes, at.bytes)) return rc;
+    uint8_t *const ws = (uint8_t *)workspace;
+    float *const weight = (float *)(ws + at.weight);
+    int64_t *const ids = (int64_t *)(ws + at.ids);
+    if (int rc = check_launch(launch_route(x, act_dtype, router, router_dtype, bias, (int)tokens, n_experts, (int)hidden, top_k, score == LOWBIT_SCORE_SIGMOID,
+                                           renormalize != 0, factor, weight, ids, nullptr, ws + at.rest, (hipStream_t)stream), what)) return rc;
+    return check_launch(launch_row_int8_experts(x, ids, weight, LOWBIT_DT_F32, (int)tokens, top_k, n_experts, (const uint8_t *)gate_up, gate_up_scale,
+                                                (const uint8_t *)down, down_scale, ws + at.rest, y, act_dtype, (int)hidden, (int)inter, act,
+                                                (hipStream_t)stream), what);
 }
 
 static int grouped_any(const char *who, const void *x, const void *const *w, const void *const *w_up, void *y,

@@ -183,7 +183,7 @@ __device__ inline void combine_pairs(float (&sum)[8], const YT *__restrict__ y, 
 template <typename YT, typename AT, typename WT>
 __global__ __launch_bounds__(256) void moe_combine_kernel(const YT *__restrict__ y, const int32_t *__restrict__ pos,
                                                           const WT *__restrict__ weight, AT *__restrict__ out, int top_k, int N, int pitch) {
-    using V8 = typename Vec8<AT>::type;
+    typedef AT V8 __attribute__((ext_vector_type(8)));
     const int t = blockIdx.y, n = (blockIdx.x * 256 + threadIdx.x) * 8;
     if (n >= N) return;
     float sum[8] = {};
@@ -197,7 +197,7 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const YT *__restrict__
     else if (left == 1) combine_pairs<1>(sum, y, pos, weight, N);
     V8 o;
 #pragma unroll
-    for (int i = 0; i < 8; i++) o[i] = to_at<AT>(sum[i]);
+    for (int i = 0; i < 8; i++) o[i] = (AT)sum[i];
     *(V8 *)(out + (int64_t)t * pitch + n) = o;
 }
 
@@ -224,6 +224,7 @@ static void launch_combine(const void *y, const int32_t *pos, const void *weight
 void launch_moe_combine_f32(const float *y, const int32_t *pos, const void *weight, int w_dtype, void *out, int act_dtype, int tokens, int top_k,
                             int N, int pitch, hipStream_t st) {
     if (act_dtype == DT_F16) launch_combine<float, _Float16>(y, pos, weight, w_dtype, out, tokens, top_k, N, pitch, st);
+    else if (act_dtype == DT_F32) launch_combine<float, float>(y, pos, weight, w_dtype, out, tokens, top_k, N, pitch, st);
     else launch_combine<float, __bf16>(y, pos, weight, w_dtype, out, tokens, top_k, N, pitch, st);
 }
 

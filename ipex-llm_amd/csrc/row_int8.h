@@ -86,4 +86,49 @@ __device__ inline uint32_t max_of_wave(uint32_t v) {
     return max_u32((uint32_t)__builtin_amdgcn_readlane((int)v, 0), (uint32_t)__builtin_amdgcn_readlane((int)v, 32));
 }
 
+// One row of K values by the threads t of WAVES waves, 16 values per thread and piece; what lies past the first HELD pieces is read again behind
+// the row's maximum.  Codes go to ldc bytes, zeros from K up to ldc.  Returns the scale.
+template <typename AT, int WAVES, int HELD> __device__ inline float quantize_row(const AT *__restrict__ from, uint8_t *__restrict__ to, int K, int ldc, int t) {
+    constexpr int STEP = 64 * WAVES * 16;
+    float v[HELD][16];
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < HELD; i++) {
+        const int k = i * STEP + t * 16;
+#pragma unroll
+        for (int j = 0; j < 16; j++) v[i][j] = 0.0f;
+        if (k < K) load16(from + k, v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < HELD; i++) m = max_u32(m, largest_of(v[i]));
+    for (int k = HELD * STEP + t * 16; k < K; k += STEP) {
+        float more[16];
+        load16(from + k, more);
+        m = max_u32(m, largest_of(more));
+    }
+    m = max_of_wave(m);
+    if constexpr (WAVES > 1) {
+        __shared__ uint32_t part[WAVES];
+        if ((t & 63) == 0) part[t >> 6] = m;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < WAVES; i++) m = max_u32(m, part[i]);
+    }
+    const RowCoder code(m);
+    auto put = [&](int k, const float (&u)[16]) __attribute__((always_inline)) {
+        if (k >= ldc) return;
+        uint32_t c[4];
+        code(u, c);
+        *(u32x4 *)(to + k) = u32x4{c[0], c[1], c[2], c[3]};
+    };
+#pragma unroll
+    for (int i = 0; i < HELD; i++) put(i * STEP + t * 16, v[i]);
+    for (int k = HELD * STEP + t * 16; k < ldc; k += STEP) {
+        float more[16] = {};
+        if (k < K) load16(from + k, more);
+        put(k, more);
+    }
+    return row_scale(m);
+}
+
 }  // namespace lowbit

@@ -210,7 +210,7 @@ int launch_row_int8_linear(const void *x, const uint8_t *w, const float *ws, con
     float *const xs = (float *)(space + at.xs);
     Int8Args t{};
     t.ldx = (int64_t)int8_blocks(K) * INT8_BLOCK;
-    if (int rc = launch_row_int8_quantize(x, dtype, M, K, space, (int)t.ldx, xs, st)) return rc;
+    if (int rc = launch_row_int8_quantize(x, dtype, M, K, space, (int)t.ldx, xs, nullptr, st)) return rc;
     t.x = space; t.xs = xs; t.w = w; t.ws = ws; t.bias = bias; t.y = y; t.part = (int32_t *)(space + at.part);
     t.M = M; t.N = N; t.K = K;
     return launch_row_int8_tiled(t, dtype, plan, st);

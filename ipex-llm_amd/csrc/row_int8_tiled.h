@@ -51,6 +51,6 @@ float tiled_walk_us(float step_us, float alone_us, int per_cu, int64_t units, in
 Int8Plan row_int8_tiled_plan(int M, int N, int K);
 size_t row_int8_part_bytes(const Int8Plan &plan, int M, int N);
 int launch_row_int8_tiled(Int8Args p, int dtype, const Int8Plan &plan, hipStream_t st);
-int launch_row_int8_quantize(const void *x, int dtype, int64_t rows, int K, uint8_t *codes, int ldc, float *scale, hipStream_t st);
+int launch_row_int8_quantize(const void *x, int dtype, int64_t rows, int K, uint8_t *codes, int ldc, float *scale, const int32_t *limit, hipStream_t st);
 
 }  // namespace lowbit

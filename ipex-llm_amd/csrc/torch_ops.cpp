@@ -13,7 +13,9 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/autograd.h>
 #include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/Event.h>
@@ -57,6 +59,14 @@ struct Api {
     decltype(&lowbit_row_int8_product_workspace_bytes) row_int8_product_workspace_bytes = nullptr;
     decltype(&lowbit_row_int8_backward) row_int8_backward = nullptr;
     decltype(&lowbit_row_int8_backward_workspace_bytes) row_int8_backward_workspace_bytes = nullptr;
+    decltype(&lowbit_row_int8_experts) row_int8_experts = nullptr;
+    decltype(&lowbit_row_int8_experts_workspace_bytes) row_int8_experts_workspace_bytes = nullptr;
+    decltype(&lowbit_row_int8_moe) row_int8_moe = nullptr;
+    decltype(&lowbit_row_int8_moe_workspace_bytes) row_int8_moe_workspace_bytes = nullptr;
+    decltype(&lowbit_route) route = nullptr;
+    decltype(&lowbit_route_workspace_bytes) route_workspace_bytes = nullptr;
+    decltype(&lowbit_route_backward) route_backward = nullptr;
+    decltype(&lowbit_route_backward_workspace_bytes) route_backward_workspace_bytes = nullptr;
     decltype(&lowbit_block_fp8_experts) block_fp8_experts = nullptr;
     decltype(&lowbit_block_fp8_experts_workspace_bytes) block_fp8_experts_workspace_bytes = nullptr;
 } api;
@@ -539,6 +549,161 @@ Tensor row_int8_product(const Tensor &codes, const Tensor &xs, const Tensor &w, 
     return row_int8_any_product(whole_rows(codes), xs.contiguous(), w, scale, bias, dtype);
 }
 
+// codes and scales of E experts that fit together: gate_up [E, 2 I, H], down [E, H, I]
+bool are_row_int8_experts(const Tensor &x, const Tensor &gate_up, const Tensor &gate_up_scale, const Tensor &down, const Tensor &down_scale) {
+    if (gate_up.dim() != 3 || down.dim() != 3 || gate_up.size(1) % 2) return false;
+    const int64_t n_exp = gate_up.size(0), hidden = x.size(1), inter = gate_up.size(1) / 2;
+    return is_row_int8(gate_up, gate_up_scale, x, n_exp) && is_row_int8(down, down_scale, x, n_exp) && gate_up.size(2) == hidden &&
+           down.size(1) == hidden && down.size(2) == inter;
+}
+
+// the experts of a mixture-of-experts block; an undefined tensor when this is not the plain case
+Tensor row_int8_experts(const Tensor &x_in, const Tensor &ids_in, const Tensor &weight_in, const Tensor &gate_up, const Tensor &gate_up_scale,
+                        const Tensor &down, const Tensor &down_scale, int act) {
+    if (!on_gpu(x_in) || x_in.dim() != 2 || ids_in.dim() != 2 || ids_in.size(0) != x_in.size(0) || ids_in.numel() == 0 ||
+        !at::isIntegralType(ids_in.scalar_type(), /*includeBool=*/false) || weight_in.sizes() != ids_in.sizes() ||
+        ids_in.device() != x_in.device() || weight_in.device() != x_in.device() || differentiable(weight_in) || differentiable(x_in) ||
+        !nothing_watches(x_in) || !nothing_watches(ids_in) || !nothing_watches(weight_in) ||
+        !are_row_int8_experts(x_in, gate_up, gate_up_scale, down, down_scale)) return {};
+    const int64_t n_exp = gate_up.size(0), hidden = x_in.size(1), inter = gate_up.size(1) / 2;
+    const int dt = dtype_code(x_in.scalar_type()), wdt = dtype_code(weight_in.scalar_type());
+    if (dt < 0 || wdt < 0) return {};
+    const int64_t tokens = ids_in.size(0), top_k = ids_in.size(1);
+    const size_t bytes = top_k > 64 || n_exp > 4096 ? 0 : api.row_int8_experts_workspace_bytes(tokens, (int)top_k, (int)n_exp, hidden, inter);
+    if (!bytes) return {};                               // more than the library takes
+    c10::DeviceGuard guard(x_in.device());
+    const Tensor x = whole_rows(x_in), ids = ids_in.to(at::kLong).contiguous(), weight = weight_in.contiguous(), gs = whole_rows(gate_up_scale),
+                 ds = whole_rows(down_scale);
+    const Tensor ws = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
+    Tensor y = at::empty({tokens, hidden}, x.options());
+    check(api.row_int8_experts(x.const_data_ptr(), ids.const_data_ptr<int64_t>(), weight.const_data_ptr(), wdt, tokens, (int)top_k, (int)n_exp,
+                               gate_up.const_data_ptr(), gs.const_data_ptr<float>(), down.const_data_ptr(), ds.const_data_ptr<float>(), ws.data_ptr(), bytes,
+                               y.data_ptr(), dt, hidden, inter, act, current_stream(x)), "lowbit_row_int8_experts");
+    return y;
+}
+
+// ---- the router of a mixture-of-experts block
+
+struct RouteRule {
+    int64_t top_k;
+    bool sigmoid, renormalize;
+    double factor;
+};
+
+// operands of a router on one GPU, of types and sizes that the library takes
+bool plain_route(const Tensor &x, const Tensor &router, const Tensor &bias, const RouteRule &rule) {
+    if (!on_gpu(x) || x.dim() != 2 || x.numel() == 0 || dtype_code(x.scalar_type()) < 0 || router.device() != x.device() || router.layout() != at::kStrided ||
+        router.dim() != 2 || router.numel() == 0 || dtype_code(router.scalar_type()) < 0 || router.size(1) != x.size(1) || !nothing_watches(x) ||
+        !nothing_watches(router) || x._fw_grad(/*level=*/0).defined() || router._fw_grad(/*level=*/0).defined()) return false;
+    if (bias.defined() && (bias.device() != x.device() || bias.dim() != 1 || bias.size(0) != router.size(0) || bias.scalar_type() != at::kFloat ||
+                           !nothing_watches(bias))) return false;
+    return rule.top_k >= 1 && rule.top_k <= 64 && rule.top_k <= router.size(0) &&
+           api.route_workspace_bytes(x.size(0), (int)std::min<int64_t>(router.size(0), 1 << 30), x.size(1)) > 0;
+}
+
+// the weights as torch operators of logits and choice, for a second derivative
+Tensor route_weights(const Tensor &x, const Tensor &router, const Tensor &ids, const RouteRule &rule) {
+    const Tensor z = at::matmul(x.to(at::kDouble), router.to(at::kDouble).t());
+    const Tensor c = (rule.sigmoid ? z.sigmoid() : z.softmax(-1)).gather(1, ids);
+    return ((rule.renormalize ? c / c.sum(-1, true) : c) * rule.factor).to(at::kFloat);
+}
+
+struct RouteBackward : public torch::autograd::Node {
+    torch::autograd::SavedVariable x_saved, router_saved;
+    Tensor ids, logits;
+    RouteRule rule{};
+
+    std::string name() const override { return "MoeRouteBackward"; }
+    void release_variables() override {
+        x_saved.reset_data();
+        router_saved.reset_data();
+        ids.reset();
+        logits.reset();
+    }
+
+    torch::autograd::variable_list apply(torch::autograd::variable_list &&grads) override {
+        const Tensor x = x_saved.unpack(), router = router_saved.unpack();
+        const int64_t T = x.size(0), H = x.size(1), E = router.size(0);
+        c10::DeviceGuard guard(x.device());
+        const Tensor grad = grads[0].defined() ? grads[0] : at::zeros(ids.sizes(), logits.options().dtype(at::kFloat));
+        const bool want_x = task_should_compute_output(0), want_r = task_should_compute_output(1);
+        if (!want_x && !want_r) return {Tensor(), Tensor()};
+        if (differentiable(grad) || !nothing_watches(grad) || c10::GradMode::is_enabled()) {
+            c10::AutoGradMode enabled(true);                 // (a second derivative, a transform: torch operators)
+            const bool create = differentiable(grad) || differentiable(x) || differentiable(router);
+            const Tensor xl = want_x && !x.requires_grad() ? x.detach().requires_grad_() : x, rl = want_r && !router.requires_grad() ? router.detach().requires_grad_() : router;
+            const Tensor w = route_weights(xl, rl, ids, rule);
+            torch::autograd::variable_list inputs;
+            if (want_x) inputs.push_back(xl);
+            if (want_r) inputs.push_back(rl);
+            auto g = torch::autograd::grad({w}, inputs, {grad}, /*retain_graph=*/true, create, /*allow_unused=*/false);
+            return {want_x ? g[0] : Tensor(), want_r ? g[want_x ? 1 : 0] : Tensor()};
+        }
+        const Tensor xr = whole_rows(x.detach()), rr = whole_rows(router.detach()), g = grad.to(at::kFloat).contiguous();
+        Tensor gx = want_x ? at::empty(xr.sizes(), xr.options()) : Tensor(), gr = want_r ? at::empty(rr.sizes(), rr.options()) : Tensor();
+        const size_t bytes = api.route_backward_workspace_bytes(T, (int)E, H);
+        const Tensor ws = at::empty({(int64_t)bytes}, xr.options().dtype(at::kByte));
+        check(api.route_backward(g.const_data_ptr<float>(), logits.const_data_ptr<double>(), ids.const_data_ptr<int64_t>(), xr.const_data_ptr(),
+                                 dtype_code(xr.scalar_type()), rr.const_data_ptr(), dtype_code(rr.scalar_type()), T, (int)E, H, (int)rule.top_k, rule.sigmoid,
+                                 rule.renormalize, (float)rule.factor, want_x ? gx.data_ptr() : nullptr, want_r ? gr.data_ptr() : nullptr, ws.data_ptr(), bytes,
+                                 current_stream(xr)), "lowbit_route_backward");
+        return {gx, gr};
+    }
+};
+
+// (weights [T, top_k], indices [T, top_k]); undefined tensors when this is not the plain case
+std::pair<Tensor, Tensor> route(const Tensor &x_in, const Tensor &router_in, const Tensor &bias_in, const RouteRule &rule) {
+    if (!plain_route(x_in, router_in, bias_in, rule)) return {};
+    c10::DeviceGuard guard(x_in.device());
+    const bool wants = c10::GradMode::is_enabled() && (x_in.requires_grad() || router_in.requires_grad());
+    const int64_t T = x_in.size(0), H = x_in.size(1), E = router_in.size(0);
+    Tensor w, ids, logits;
+    {
+        c10::AutoGradMode no_grad(false);
+        const Tensor x = whole_rows(x_in.detach()), router = whole_rows(router_in.detach()), bias = bias_in.defined() ? bias_in.detach().contiguous() : Tensor();
+        w = at::empty({T, rule.top_k}, x.options().dtype(at::kFloat));
+        ids = at::empty({T, rule.top_k}, x.options().dtype(at::kLong));
+        if (wants) logits = at::empty({T, E}, x.options().dtype(at::kDouble));
+        const size_t bytes = api.route_workspace_bytes(T, (int)E, H);
+        const Tensor ws = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
+        check(api.route(x.const_data_ptr(), dtype_code(x.scalar_type()), router.const_data_ptr(), dtype_code(router.scalar_type()),
+                        bias.defined() ? bias.const_data_ptr<float>() : nullptr, T, (int)E, H, (int)rule.top_k, rule.sigmoid, rule.renormalize,
+                        (float)rule.factor, w.data_ptr<float>(), ids.data_ptr<int64_t>(), wants ? logits.data_ptr<double>() : nullptr, ws.data_ptr(), bytes,
+                        current_stream(x)), "lowbit_route");
+    }
+    if (wants) {
+        auto node = std::shared_ptr<RouteBackward>(new RouteBackward(), torch::autograd::deleteNode);
+        node->set_next_edges(torch::autograd::collect_next_edges(x_in, router_in));
+        node->x_saved = torch::autograd::SavedVariable(x_in, /*is_output=*/false);
+        node->router_saved = torch::autograd::SavedVariable(router_in, /*is_output=*/false);
+        node->ids = ids;
+        node->logits = logits;
+        node->rule = rule;
+        torch::autograd::set_history(w, node);
+    }
+    return {w, ids};
+}
+
+// router and experts in one call; an undefined tensor when this is not the plain case
+Tensor row_int8_moe(const Tensor &x_in, const Tensor &router_in, const Tensor &bias_in, const RouteRule &rule, const Tensor &gate_up, const Tensor &gate_up_scale,
+                    const Tensor &down, const Tensor &down_scale, int act) {
+    if (!plain_route(x_in, router_in, bias_in, rule) || differentiable(x_in) || differentiable(router_in) ||
+        !are_row_int8_experts(x_in, gate_up, gate_up_scale, down, down_scale) || router_in.size(0) != gate_up.size(0)) return {};
+    const int64_t T = x_in.size(0), H = x_in.size(1), E = router_in.size(0), I = gate_up.size(1) / 2;
+    const size_t bytes = api.row_int8_moe_workspace_bytes(T, (int)rule.top_k, (int)E, H, I);
+    if (!bytes) return {};                               // more than the library takes
+    c10::DeviceGuard guard(x_in.device());
+    const Tensor x = whole_rows(x_in), router = whole_rows(router_in), bias = bias_in.defined() ? bias_in.contiguous() : Tensor(),
+                 gs = whole_rows(gate_up_scale), ds = whole_rows(down_scale);
+    const Tensor ws = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
+    Tensor y = at::empty({T, H}, x.options());
+    check(api.row_int8_moe(x.const_data_ptr(), router.const_data_ptr(), dtype_code(router.scalar_type()), bias.defined() ? bias.const_data_ptr<float>() : nullptr,
+                           T, (int)rule.top_k, (int)E, rule.sigmoid, rule.renormalize, (float)rule.factor, gate_up.const_data_ptr(), gs.const_data_ptr<float>(),
+                           down.const_data_ptr(), ds.const_data_ptr<float>(), ws.data_ptr(), bytes, y.data_ptr(), dtype_code(x.scalar_type()), H, I, act,
+                           current_stream(x)), "lowbit_row_int8_moe");
+    return y;
+}
+
 // ---- large copies between pageable host memory and the GPU, through two pinned buffers
 //
 // A pageable copy by the runtime ran at 29 GB/s up and, into memory the process has not touched yet, 7.5 GB/s down
@@ -625,6 +790,11 @@ struct Args {
         if (v == -1 && PyErr_Occurred()) { PyErr_Clear(); throw std::invalid_argument("an integer is expected"); }
         return v;
     }
+    double number(Py_ssize_t i) const {
+        const double v = PyFloat_AsDouble(a[i]);
+        if (v == -1.0 && PyErr_Occurred()) { PyErr_Clear(); throw std::invalid_argument("a number is expected"); }
+        return v;
+    }
     bool truth(Py_ssize_t i) const { return PyObject_IsTrue(a[i]) == 1; }
 };
 
@@ -693,6 +863,8 @@ PyObject *py_bind(PyObject *, PyObject *const *args, Py_ssize_t n) {
     BIND(gated_mlp); BIND(dequantize_rows); BIND(dequantize); BIND(backward_ws); BIND(backward_workspace_bytes); BIND(backward_ws_applies); BIND(experts_workspace_bytes); BIND(experts_forward);
     BIND(block_fp8_quantize); BIND(block_fp8_quantize_weight); BIND(block_fp8_linear); BIND(block_fp8_linear_workspace_bytes);
     BIND(row_int8_quantize); BIND(row_int8_linear); BIND(row_int8_linear_workspace_bytes); BIND(row_int8_product);
+    BIND(row_int8_experts); BIND(row_int8_experts_workspace_bytes); BIND(row_int8_moe); BIND(row_int8_moe_workspace_bytes);
+    BIND(route); BIND(route_workspace_bytes); BIND(route_backward); BIND(route_backward_workspace_bytes);
     BIND(row_int8_product_workspace_bytes); BIND(row_int8_backward); BIND(row_int8_backward_workspace_bytes);
     BIND(block_fp8_backward); BIND(block_fp8_backward_workspace_bytes); BIND(block_fp8_experts); BIND(block_fp8_experts_workspace_bytes);
 #undef BIND
@@ -843,6 +1015,46 @@ PyObject *py_row_int8_product(PyObject *, PyObject *const *args, Py_ssize_t n) {
     });
 }
 
+// row_int8_experts(x, ids, weights, gate_up, gate_up_scale, down, down_scale, act) -> y or None
+PyObject *py_row_int8_experts(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return answer("row_int8_experts", n, 8, [&] {
+        const Args a{args, n};
+        const Tensor &x = a.tensor(0), &ids = a.tensor(1), &weight = a.tensor(2);
+        const Tensor &gu = a.tensor(3), &gus = a.tensor(4), &d = a.tensor(5), &ds = a.tensor(6);
+        const int act = (int)a.integer(7);
+        NoGil free;
+        return row_int8_experts(x, ids, weight, gu, gus, d, ds, act);
+    });
+}
+
+RouteRule rule_of(const Args &a, Py_ssize_t first) { return {a.integer(first), a.truth(first + 1), a.truth(first + 2), a.number(first + 3)}; }
+
+// route(x, router, bias or None, top_k, sigmoid, renormalize, factor) -> (weights, indices) or None
+PyObject *py_route(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return answer_pair("route", n, 7, [&] {
+        const Args a{args, n};
+        const Tensor &x = a.tensor(0), &router = a.tensor(1);
+        const Tensor bias = a.optional(2);
+        const RouteRule rule = rule_of(a, 3);
+        NoGil free;
+        return route(x, router, bias, rule);
+    });
+}
+
+// row_int8_moe(x, router, bias or None, top_k, sigmoid, renormalize, factor, gate_up, gate_up_scale, down, down_scale, act) -> y or None
+PyObject *py_row_int8_moe(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return answer("row_int8_moe", n, 12, [&] {
+        const Args a{args, n};
+        const Tensor &x = a.tensor(0), &router = a.tensor(1);
+        const Tensor bias = a.optional(2);
+        const RouteRule rule = rule_of(a, 3);
+        const Tensor &gu = a.tensor(7), &gus = a.tensor(8), &d = a.tensor(9), &ds = a.tensor(10);
+        const int act = (int)a.integer(11);
+        NoGil free;
+        return row_int8_moe(x, router, bias, rule, gu, gus, d, ds, act);
+    });
+}
+
 // upload(host tensor, device index) -> the tensor on that GPU, or None; complete when it returns
 PyObject *py_upload(PyObject *, PyObject *const *args, Py_ssize_t n) {
     return answer("upload", n, 2, [&] {
@@ -887,6 +1099,7 @@ PyObject *py_holds(PyObject *, PyObject *const *args, Py_ssize_t n) {
 #define METHOD(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {METHOD(bind), METHOD(product), METHOD(linear), METHOD(linear_train), METHOD(gated), METHOD(embedding), METHOD(experts), METHOD(block_fp8_quantize),
                          METHOD(block_fp8_linear), METHOD(block_fp8_experts), METHOD(row_int8_quantize), METHOD(row_int8_linear), METHOD(row_int8_product),
+                         METHOD(row_int8_experts), METHOD(route), METHOD(row_int8_moe),
                          METHOD(upload),
                          METHOD(download), METHOD(holds),
                          {nullptr, nullptr, 0, nullptr}};

@@ -571,6 +571,50 @@ def lowbit_row_int8_waves(m, n, k):
     return waves
 
 
+_lib.lowbit_row_int8_experts.argtypes = _lib.lowbit_block_fp8_experts.argtypes
+_lib.lowbit_row_int8_experts_plan.argtypes = [c_int64, c_int, c_int, c_int64, c_int64, ctypes.POINTER(c_int)]
+_lib.lowbit_row_int8_experts_waves.argtypes = [c_int64, c_int, c_int, c_int64, c_int64]
+_lib.lowbit_route.argtypes = [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int64, c_int, c_int64, c_int, c_int, c_int, ctypes.c_float, c_void_p, c_void_p,
+                              c_void_p, c_void_p, c_size_t, c_void_p]
+_lib.lowbit_route_backward.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int64, c_int, c_int64, c_int, c_int, c_int,
+                                       ctypes.c_float, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]
+_lib.lowbit_row_int8_moe.argtypes = [c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int, c_int, c_int, c_int, ctypes.c_float, c_void_p, c_void_p, c_void_p,
+                                     c_void_p, c_void_p, c_size_t, c_void_p, c_int, c_int64, c_int64, c_int, c_void_p]
+for _name in ("row_int8_experts", "row_int8_experts_plan", "row_int8_experts_waves", "route", "route_backward", "row_int8_moe"):
+    getattr(_lib, f"lowbit_{_name}").restype = c_int
+for _name in ("row_int8_experts", "row_int8_moe"):
+    getattr(_lib, f"lowbit_{_name}_workspace_bytes").argtypes = [c_int64, c_int, c_int, c_int64, c_int64]
+for _name in ("route", "route_backward"):
+    getattr(_lib, f"lowbit_{_name}_workspace_bytes").argtypes = [c_int64, c_int, c_int64]
+for _name in ("row_int8_experts", "row_int8_moe", "route", "route_backward"):
+    getattr(_lib, f"lowbit_{_name}_workspace_bytes").restype = c_size_t
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+
+
+def lowbit_row_int8_experts_plan(tokens, top_k, n_experts, hidden, inter):
+    """(rows of a tile of the first product, rows, columns of one of the second (0: pair by pair), whether a launch of its own places the pairs)."""
+    plan4 = (c_int * 4)()
+    _check(_lib.lowbit_row_int8_experts_plan(tokens, top_k, n_experts, hidden, inter, plan4), "lowbit_row_int8_experts_plan")
+    return tuple(plan4)
+
+
+def lowbit_row_int8_experts_waves(tokens, top_k, n_experts, hidden, inter):
+    """Waves of a workgroup of the second launch where each pair streams its weights, 0 where the pairs are sorted."""
+    waves = _lib.lowbit_row_int8_experts_waves(tokens, top_k, n_experts, hidden, inter)
+    _check(min(waves, 0), "lowbit_row_int8_experts_waves")
+    return waves
+
+
+def lowbit_route(x, x_dtype, router, router_dtype, bias, tokens, n_experts, hidden, top_k, score, renormalize, factor, topk_weight, topk_ids, logits,
+                 workspace, workspace_bytes, stream):
+    _check(_lib.lowbit_route(x, x_dtype, router, router_dtype, bias, tokens, n_experts, hidden, top_k, score, renormalize, factor, topk_weight, topk_ids,
+                             logits, workspace, workspace_bytes, stream), "lowbit_route")
+
+
+def lowbit_route_workspace_bytes(tokens, n_experts, hidden) -> int:
+    return _lib.lowbit_route_workspace_bytes(tokens, n_experts, hidden)
+
+
 def lowbit_dequantize_rows(w, rows, n_rows, dst, qtype, n, k, layout, out_dtype, stream):
     _check(_lib.lowbit_dequantize_rows(w, rows, n_rows, dst, qtype, n, k, layout, out_dtype, stream),
            "lowbit_dequantize_rows")

@@ -30,6 +30,56 @@ def route_top_k(router_logits: torch.Tensor, top_k: int = 2):
     return weights, experts
 
 
+_SCORES = {"softmax": False, "sigmoid": True}
+_FLOATS = (torch.float16, torch.bfloat16, torch.float32)
+
+
+def _check_route(x, router, top_k, bias, score, what):
+    invalidInputError(score in _SCORES, f"{what}: score is 'softmax' or 'sigmoid', not {score!r}")
+    invalidInputError(isinstance(x, torch.Tensor) and x.device.type == "cuda", f"{what} needs a tensor on an MI355X: the kernels have no CPU implementation")
+    invalidInputError(isinstance(router, torch.Tensor) and router.device == x.device and x.dtype in _FLOATS and router.dtype in _FLOATS,
+                      f"{what}: x and the router must be float16, bfloat16 or float32 on one GPU")
+    invalidInputError(x.dim() >= 1 and router.dim() == 2 and router.shape[0] > 0 and x.shape[-1] == router.shape[1] and router.shape[1] % 8 == 0 and router.shape[1] > 0,
+                      f"{what}: x [.., hidden] and router [experts, hidden], hidden a multiple of 8, not {tuple(x.shape)} and {tuple(router.shape)}")
+    invalidInputError(router.shape[0] <= 1024 and router.shape[1] <= 1 << 20, f"{what}: at most 1024 experts and rows of 2^20")
+    invalidInputError(1 <= top_k <= min(64, router.shape[0]), f"{what}: top_k must be 1 .. 64 and at most the number of experts")
+    invalidInputError(bias is None or (isinstance(bias, torch.Tensor) and bias.device == x.device and bias.shape == (router.shape[0],)
+                                       and bias.is_floating_point()), f"{what}: the bias must hold a number for each expert, on x's GPU")
+
+
+def _route_steps(x, router, top_k, bias, score, renormalize, scale):
+    """moe_route as torch operators, for a tangent, a transform, a trace or a dispatch mode, which want to see them."""
+    z = x.double() @ router.double().t()
+    s = torch.sigmoid(z) if _SCORES[score] else torch.softmax(z, -1)
+    by = z if bias is None else s + bias.double()
+    index = torch.sort(by.detach(), dim=-1, descending=True, stable=True).indices[..., :top_k]
+    w = s.gather(-1, index)
+    return ((w / w.sum(-1, keepdim=True) if renormalize else w) * scale).float(), index
+
+
+def moe_route(x: torch.Tensor, router: torch.Tensor, top_k: int, bias: torch.Tensor = None, score: str = "softmax", renormalize: bool = True,
+              scale: float = 1.0):
+    """(weights, indices) [.., top_k], float32 and int64, of the experts that each row of x [.., hidden] is sent to, for the calls of experts of this
+    package (`LowBitExperts`, `block_fp8_experts`, `row_int8_experts`).
+
+    z = x router^T (router [experts, hidden]) and s = softmax(z) or sigmoid(z); chosen are the top_k largest z, in descending order - of s + bias
+    where a bias [experts] is given, a correction of the choice that the weights do not see -, ties to the lowest index, a NaN above all numbers.
+    weights = scale * s of those, divided by their sum if `renormalize`.  Sums and scores are float64 (csrc/route.hip), so that the choice depends on
+    no order of summation.  The gradient of the weights flows on to x and the router; the choice and the bias count as constant."""
+    invalidInputError(score in _SCORES, f"moe_route: score is 'softmax' or 'sigmoid', not {score!r}")
+    if isinstance(x, torch.Tensor) and isinstance(router, torch.Tensor):
+        rows = x if x.dim() == 2 else x.reshape(-1, x.shape[-1]) if x.dim() else x
+        fixed = bias.float() if isinstance(bias, torch.Tensor) and bias.is_floating_point() else bias
+        both = ops.route(rows, router, fixed, top_k, _SCORES[score], renormalize, float(scale))
+        if both is not None:
+            return both if x.dim() == 2 else tuple(t.view(*x.shape[:-1], top_k) for t in both)
+    _check_route(x, router, top_k, bias, score, "moe_route")
+    if x.numel() == 0:
+        return (x.float().sum(-1, keepdim=True) * 0 + torch.zeros(top_k, device=x.device),
+                torch.zeros((*x.shape[:-1], top_k), dtype=torch.int64, device=x.device))
+    return _route_steps(x, router, top_k, bias, score, renormalize, scale)
+
+
 class ExpertWeights:
     """Device pointers of one projection of every expert ([N, K] tiled blobs of one qtype)."""
 

@@ -16,7 +16,9 @@ _BOUND = ("last_error", "blob_bytes", "tileable", "linear_scratch_bytes", "linea
           "experts_workspace_bytes", "experts_forward", "block_fp8_quantize", "block_fp8_quantize_weight", "block_fp8_linear",
           "block_fp8_linear_workspace_bytes", "block_fp8_backward", "block_fp8_backward_workspace_bytes", "block_fp8_experts",
           "block_fp8_experts_workspace_bytes", "row_int8_quantize", "row_int8_linear", "row_int8_linear_workspace_bytes", "row_int8_product",
-          "row_int8_product_workspace_bytes", "row_int8_backward", "row_int8_backward_workspace_bytes")
+          "row_int8_product_workspace_bytes", "row_int8_backward", "row_int8_backward_workspace_bytes", "row_int8_experts",
+          "row_int8_experts_workspace_bytes", "row_int8_moe", "row_int8_moe_workspace_bytes", "route", "route_workspace_bytes", "route_backward",
+          "route_backward_workspace_bytes")
 
 
 def _load():

@@ -10,6 +10,7 @@ they keep, or of dense layers with `optimize_model(model, "sym_int8", row_int8=T
 Weights are frozen, as in LowBitLinear.  The gradient flows on to the activations, whose quantization counts as the identity.
 """
 import torch
+import torch.nn.functional as F
 
 import ipex_llm.ggml.model.llama.llama_cpp as ggml
 from ipex_llm.transformers.native_ops import ops
@@ -142,3 +143,87 @@ def row_int8_product(codes: torch.Tensor, scale: torch.Tensor, weight: torch.Ten
             return (y + bias).to(dtype)
     y = torch.matmul(codes.float(), weight.float().t()) * scale.unsqueeze(-1) * weight_scale
     return (y if bias is None else y + bias).to(dtype)
+
+
+def _expert_loop(x, top_k_index, top_k_weights, gate_up, gate_up_scale, down, down_scale, gate):
+    """Expert by expert, h = gate(g | u), with what the native call keeps in float32 (g, u, h, the pairs' results and their sum) kept so too, and
+    one rounding."""
+    (tokens, top_k), n_exp = top_k_index.shape, gate_up.shape[0]
+    expert = top_k_index.reshape(-1).long()
+    expert = expert.masked_fill((expert < 0) | (expert >= n_exp), n_exp)
+    order = expert.argsort(stable=True)
+    counts = torch.bincount(expert, minlength=n_exp + 1).tolist()
+    rows, ys = x.float()[torch.div(order, top_k, rounding_mode="floor")].split(counts), []
+    for e in range(n_exp):
+        if counts[e]:
+            gu = row_int8_linear(rows[e], gate_up[e], gate_up_scale[e])
+            ys.append(row_int8_linear(gate(gu), down[e], down_scale[e]))
+    if not ys:
+        return x * 0 + top_k_weights.sum().to(x.dtype) * 0
+    order = order[:len(order) - counts[n_exp]]
+    y = torch.cat(ys) * top_k_weights.reshape(-1)[order].float().unsqueeze(-1)
+    return y.new_zeros((tokens * top_k, x.shape[1])).index_copy(0, order, y).view(tokens, top_k, -1).sum(1).to(x.dtype)
+
+
+def _gated(act_fn):
+    def gate(gu):
+        g, u = gu.chunk(2, dim=-1)
+        return act_fn(g) * u
+    return gate
+
+
+_ACTS = {0: F.silu, 1: lambda g: F.gelu(g, approximate="tanh")}
+
+
+def _check_experts(x, gate_up, gate_up_scale, down, down_scale, what):
+    _check_input(x, what)
+    _check_weight(gate_up, gate_up_scale, x, what, 3)
+    _check_weight(down, down_scale, x, what, 3)
+    n_exp, two_i, hidden = gate_up.shape
+    invalidInputError(two_i % 2 == 0 and tuple(down.shape) == (n_exp, hidden, two_i // 2),
+                      f"{what}: gate_up [E, 2 I, H] and down [E, H, I] do not fit together")
+    invalidInputError(x.dim() == 2 and x.shape[1] == hidden, f"{what}: x must be [tokens, {hidden}]")
+
+
+def row_int8_experts(x: torch.Tensor, top_k_index: torch.Tensor, top_k_weights: torch.Tensor, gate_up: torch.Tensor,
+                     gate_up_scale: torch.Tensor, down: torch.Tensor, down_scale: torch.Tensor, act: int = 0):
+    """The experts of a mixture-of-experts block: out[t] = sum_j p[t, j] (Q(act(g) u) down[e]^T), (g | u) = Q(x[t]) gate_up[e]^T,
+    e = top_k_index[t, j], p = top_k_weights.
+
+    x [T, H]; top_k_index, top_k_weights [T, k]; gate_up [E, 2 I, H] (gate rows first) and down [E, H, I] codes with their scales [E, 2 I] and
+    [E, H]; act 0 = SiLU, 1 = GELU (tanh form).  An index that names no expert counts nothing.  act(g) u, the pairs' results and their sum are float32,
+    rounded once.  One native call; x or weights that want a gradient, and more than 64 experts per token, 4096 experts or 2^21 pairs, run
+    expert by expert through row_int8_linear."""
+    invalidInputError(act in _ACTS, "row_int8_experts: act is 0 (SiLU) or 1 (GELU, tanh form)")
+    y = ops.row_int8_experts(x, top_k_index, top_k_weights, gate_up, gate_up_scale, down, down_scale, act)
+    if y is not None:
+        return y
+    what = "row_int8_experts"
+    _check_experts(x, gate_up, gate_up_scale, down, down_scale, what)
+    invalidInputError(top_k_index.dim() == 2 and top_k_index.shape == top_k_weights.shape and top_k_index.shape[0] == x.shape[0]
+                      and not top_k_index.is_floating_point() and top_k_index.dtype != torch.bool
+                      and top_k_index.device == x.device and top_k_weights.device == x.device,
+                      f"{what}: whole indices and weights [tokens, k] on x's GPU")
+    return _expert_loop(x, top_k_index, top_k_weights, gate_up, gate_up_scale, down, down_scale, _gated(_ACTS[act]))
+
+
+def row_int8_moe(x: torch.Tensor, router: torch.Tensor, top_k: int, gate_up: torch.Tensor, gate_up_scale: torch.Tensor, down: torch.Tensor,
+                 down_scale: torch.Tensor, bias: torch.Tensor = None, score: str = "softmax", renormalize: bool = True, scale: float = 1.0,
+                 act: int = 0):
+    """A whole mixture-of-experts layer, moe.moe_route and row_int8_experts in one native call: x [T, H], router [E, H] (bias, score, renormalize
+    and scale are the router's), the experts' codes and scales as in row_int8_experts.  Where x or the router want a gradient it is the two calls."""
+    from ipex_llm.transformers.moe import _SCORES, _check_route, moe_route
+    what = "row_int8_moe"
+    invalidInputError(act in _ACTS, f"{what}: act is 0 (SiLU) or 1 (GELU, tanh form)")
+    invalidInputError(score in _SCORES, f"{what}: score is 'softmax' or 'sigmoid', not {score!r}")
+    fixed = bias.float() if isinstance(bias, torch.Tensor) and bias.is_floating_point() else bias
+    y = ops.row_int8_moe(x, router, fixed, top_k, _SCORES[score], renormalize, float(scale), gate_up, gate_up_scale, down, down_scale, act)
+    if y is not None:
+        return y
+    _check_experts(x, gate_up, gate_up_scale, down, down_scale, what)
+    _check_route(x, router, top_k, bias, score, what)
+    invalidInputError(router.shape[0] == gate_up.shape[0], f"{what}: the router has {router.shape[0]} rows for {gate_up.shape[0]} experts")
+    if x.numel() == 0:
+        return x * 0
+    weights, index = moe_route(x, router, top_k, bias, score, renormalize, scale)
+    return row_int8_experts(x, index, weights, gate_up, gate_up_scale, down, down_scale, act)

@@ -96,3 +96,65 @@ def test_plans_cover_every_size():
                     splits = ggml.lowbit_row_int8_plan(dtype, 1, m, n, k)[2]
                     assert 1 <= splits <= (n + 63) // 64 * terms
                     assert ggml.lowbit_row_int8_backward_workspace_bytes(dtype, m, n, k) >= m * n * 2 * terms + (splits * m * k * 4 if splits > 1 else 0)
+
+
+def test_experts_router_and_layer_refuse_before_they_touch_the_gpu():
+    ex, route, back, layer = lib.lowbit_row_int8_experts, lib.lowbit_route, lib.lowbit_route_backward, lib.lowbit_row_int8_moe
+
+    def experts(x=P, ids=P, weight=P, wdt=2, tokens=2, top_k=2, n_exp=4, gu=P, gus=P, d=P, ds=P, ws=P, bytes_=1 << 40, y=P, dt=1, hidden=128, inter=64, act=0):
+        return ex(x, ids, weight, wdt, tokens, top_k, n_exp, gu, gus, d, ds, ws, bytes_, y, dt, hidden, inter, act, None)
+    assert experts(dt=3) == EDTYPE and experts(wdt=9) == EDTYPE and experts(act=2) == EARG
+    assert experts(top_k=0) == ESIZE and experts(top_k=65) == ESIZE and experts(n_exp=4097) == ESIZE and experts(tokens=1 << 20, top_k=4) == ESIZE
+    assert experts(hidden=(1 << 17) + 16) == ESIZE and experts(inter=(1 << 17) + 16) == ESIZE and experts(tokens=-1) == ESIZE
+    assert experts(hidden=120) == ESHAPE and experts(inter=72) == ESHAPE
+    assert experts(x=P + 8) == EARG and experts(gus=P + 4) == EARG and experts(ids=P + 4) == EARG and experts(y=None) == EARG
+    assert experts(ws=None) == ESIZE and experts(bytes_=16) == ESIZE
+    assert experts(tokens=0, x=None, ids=None, y=None, ws=None) == 0
+    need = lib.lowbit_row_int8_experts_workspace_bytes
+    assert need(300, 2, 8, 512, 256) >= 600 * (5 * 256 + 4 * 512) + 300 * 512 and need(300, 2, 8, 512, 250) == 0 and need(0, 2, 8, 512, 256) == 0
+    assert need(1 << 20, 2, 8, 8192, 8192) <= (1 << 31) + (1 << 30)             # (tokens go in parts)
+
+    def router(x=P, xdt=1, r=P, rdt=1, bias=None, tokens=2, n_exp=8, hidden=64, top_k=2, score=0, w=P, ids=P, z=None, ws=P, bytes_=1 << 40):
+        return route(x, xdt, r, rdt, bias, tokens, n_exp, hidden, top_k, score, 1, 1.0, w, ids, z, ws, bytes_, None)
+    assert router(xdt=3) == EDTYPE and router(rdt=-1) == EDTYPE and router(score=2) == EARG and router(tokens=-1) == EARG and router(hidden=0) == EARG
+    assert router(hidden=60) == ESHAPE and router(n_exp=1025) == ESIZE and router(top_k=9) == ESIZE and router(top_k=0) == ESIZE
+    assert router(n_exp=100, top_k=65) == ESIZE and router(tokens=(1 << 21) + 1) == ESIZE
+    assert router(x=P + 4) == EARG and router(bias=P + 2) == EARG and router(z=P + 4) == EARG and router(w=None) == EARG
+    assert router(bytes_=8) == ESIZE and router(ws=None) == ESIZE
+    assert router(tokens=0, x=None, r=None) == 0
+    assert back(P, P, P, P, 1, P, 1, 0, 8, 64, 2, 0, 1, 1.0, P, P, P, 1 << 40, None) == EARG
+    assert back(P, None, P, P, 1, P, 1, 2, 8, 64, 2, 0, 1, 1.0, P, P, P, 1 << 40, None) == EARG
+    assert back(P, P, P, P, 1, P, 1, 2, 8, 64, 2, 0, 1, 1.0, P, P, P, 8, None) == ESIZE
+
+    def whole(x=P, r=P, rdt=1, bias=None, tokens=2, top_k=2, n_exp=8, score=0, gu=P, gus=P, d=P, ds=P, ws=P, bytes_=1 << 40, y=P, dt=1, hidden=128, inter=64, act=0):
+        return layer(x, r, rdt, bias, tokens, top_k, n_exp, score, 1, 1.0, gu, gus, d, ds, ws, bytes_, y, dt, hidden, inter, act, None)
+    assert whole(dt=7) == EDTYPE and whole(score=5) == EARG and whole(act=3) == EARG and whole(hidden=72) == ESHAPE and whole(top_k=9) == ESIZE
+    assert whole(r=None) == EARG and whole(gu=None) == EARG and whole(bytes_=100) == ESIZE and whole(n_exp=1030) == ESIZE
+    assert whole(tokens=0, x=None, y=None) == 0
+    assert lib.lowbit_row_int8_moe_workspace_bytes(2, 2, 8, 128, 64) >= need(2, 2, 8, 128, 64)
+
+
+def test_router_and_layers_refuse_host_tensors():
+    from ipex_llm.transformers import moe
+    x, router = torch.zeros((2, 32)), torch.zeros((4, 32))
+    w, ws = u.weight(gen(3), 32, 32, (4,))
+    with pytest.raises(RuntimeError, match="no CPU implementation"):
+        moe.moe_route(x, router, 2)
+    with pytest.raises(RuntimeError, match="score is"):
+        moe.moe_route(x, router, 2, score="relu")
+    with pytest.raises(RuntimeError, match="no CPU implementation"):
+        ri.row_int8_experts(x, torch.zeros((2, 1), dtype=torch.int64), torch.ones((2, 1)), w, ws, w[:, :, :16].contiguous(), ws)
+    with pytest.raises(RuntimeError, match="no CPU implementation"):
+        ri.row_int8_moe(x, router, 2, w, ws, w[:, :, :16].contiguous(), ws)
+
+
+def test_route_steps_are_the_formula():
+    from ipex_llm.transformers import moe
+    x, router, bias = torch.randn((5, 16), generator=gen(1)), torch.randn((6, 16), generator=gen(2)), torch.randn(6, generator=gen(3))
+    z = x.double() @ router.double().t()
+    w, index = moe._route_steps(x, router, 2, None, "softmax", True, 2.0)
+    top = z.topk(2, dim=-1)
+    assert torch.equal(index, top.indices) and torch.allclose(w.double(), 2 * torch.softmax(top.values, -1), atol=1e-7)
+    w, index = moe._route_steps(x, router, 3, bias, "sigmoid", False, 1.0)
+    assert torch.equal(index, (torch.sigmoid(z) + bias.double()).topk(3, dim=-1).indices)
+    assert torch.allclose(w.double(), torch.sigmoid(z).gather(1, index), atol=1e-7)
