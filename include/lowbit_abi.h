@@ -404,9 +404,10 @@ int lowbit_row_int8_product(const void *codes, const float *scale, const void *w
 size_t lowbit_row_int8_backward_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K);
 int lowbit_row_int8_backward(const void *grad, const void *w, const float *w_scale, void *grad_x, int dtype, int64_t M, int64_t N, int64_t K,
                              void *workspace, size_t workspace_bytes, void *stream);
-/* What the linear product and the gradient run as: plan4 as lowbit_block_fp8_plan's. */
+/* What the linear product and the gradient run as: plan4 as lowbit_block_fp8_plan's; tiles of 16 columns: the streaming kernel, which reads codes of up
+ * to 32 rows. */
 int lowbit_row_int8_plan(int dtype, int backward, int64_t M, int64_t N, int64_t K, int *plan4);
-/* Waves of a workgroup where lowbit_row_int8_linear runs the kernel of few rows, 0 where it runs tiles (negative: an error). */
+/* Waves of a workgroup where lowbit_row_int8_linear runs the kernel of few rows or the streaming one, 0 where it runs tiles (negative: an error). */
 int lowbit_row_int8_waves(int64_t M, int64_t N, int64_t K);
 /* A mixture-of-experts block: y[t, :] = sum_j topk_weight[t, j] * (Q(act(g) .* u) * down[e]^T), (g | u) = Q(x_t) * gate_up[e]^T, e =
  * topk_ids[t, j]; a pair whose id lies outside [0, n_experts) counts nothing.  gate_up [n_experts, 2 inter, hidden] (gate rows first)

@@ -285,14 +285,18 @@ __global__ __launch_bounds__(256) void row_int8_back_reduce_kernel(const f32x4 *
 
 static int cdiv(int a, int b) { return (a + b - 1) / b; }
 
-// Rows and columns of a tile, workgroups that a CU holds, and the time (us) of two steps with the GPU full and with one workgroup on a CU.  Each
-// wave takes all rows of its tile and 32 columns of it, so that a weight is widened once.
+// Rows and columns of a tile, workgroups that a CU holds, and a step's time (us) with the GPU full and with one workgroup on a CU.  In the first
+// three each wave takes all rows of its tile and 32 columns of it, so that a weight is widened once; the larger ones (waves of 64 x 64, 128 x 64 and
+// 96 x 64) read fewer operands from LDS for a product: 2048 x 4096 (N) x 11008 188 us in tiles of 128 x 256, 163 in 192 x 256, 8192 x 4096 x 4096 232 and
+// 210 in 256 x 256.  Fitted to 63 sizes, 16 to 8192 rows by 64 to 28672 (N) by 128 to 16384: the pick is 1.1 % above the fastest form and split on
+// average, 16 % at worst.
 struct Int8BackForm {
     int rows, cols, per_cu;
-    float block_us, alone_us;
+    float step_us, alone_us;
 };
-enum { BACK_128, BACK_64, BACK_32, BACK_COUNT };
-static const Int8BackForm BACK_FORMS[BACK_COUNT] = {{128, 256, 1, 1.85f, 1.74f}, {64, 128, 2, 1.10f, 0.71f}, {32, 128, 2, 0.85f, 0.64f}};
+enum { BACK_128, BACK_64, BACK_32, BACK_128_128, BACK_256, BACK_192, BACK_COUNT };
+static const Int8BackForm BACK_FORMS[BACK_COUNT] = {{128, 256, 1, 0.786f, 0.736f}, {64, 128, 2, 0.515f, 0.382f}, {32, 128, 2, 0.475f, 0.347f},
+                                                    {128, 128, 2, 0.814f, 0.615f}, {256, 256, 1, 1.35f, 1.32f}, {192, 256, 1, 1.093f, 1.068f}};
 
 struct Int8BackPlan {
     int form, splits;
@@ -306,8 +310,9 @@ static Int8BackPlan back_plan(int M, int steps, int K) {
         const int64_t tiles = (int64_t)cdiv(M, f.rows) * cdiv(K, f.cols);
         for (int splits : tried) {
             if (splits > 1 && (steps < 2 * splits || tiles >= 512 || (size_t)splits * M * K * 4 > (size_t)256 << 20)) break;
-            float us = tiled_walk_us(f.block_us, f.alone_us, f.per_cu, tiles * splits, cdiv(steps, splits)) * 0.5f + 6.3f;
-            if (splits > 1) us += 1.6f + (float)splits * M * K * 8.0f / 5.0e6f;
+            float us = tiled_walk_us(f.step_us, f.alone_us, f.per_cu, tiles * splits, cdiv(steps, splits)) + 3.4f + 0.83e-6f * M * K;
+            us += 0.16f * ((tiles * splits - 1) / (256 * f.per_cu));
+            if (splits > 1) us += 2.6f + (float)splits * M * K * 8.0f / 5.2e6f;
             if (least == 0.0f || us < least) {
                 least = us;
                 best = {form, splits};
@@ -350,7 +355,10 @@ template <typename OT, bool PART> static void launch_back(const Int8Back &p, int
     const dim3 grid((units + 7) / 8 * 8);
     if (form == BACK_128) hipLaunchKernelGGL((row_int8_back_kernel<OT, PART, 8, 2, 1, 8, 4, 2>), grid, dim3(512), 0, st, p);
     else if (form == BACK_64) hipLaunchKernelGGL((row_int8_back_kernel<OT, PART, 4, 2, 1, 4, 4, 2>), grid, dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((row_int8_back_kernel<OT, PART, 2, 2, 1, 4, 5, 2>), grid, dim3(256), 0, st, p);
+    else if (form == BACK_32) hipLaunchKernelGGL((row_int8_back_kernel<OT, PART, 2, 2, 1, 4, 5, 2>), grid, dim3(256), 0, st, p);
+    else if (form == BACK_128_128) hipLaunchKernelGGL((row_int8_back_kernel<OT, PART, 4, 4, 2, 2, 3, 2>), grid, dim3(256), 0, st, p);
+    else if (form == BACK_256) hipLaunchKernelGGL((row_int8_back_kernel<OT, PART, 8, 4, 2, 4, 3, 2>), grid, dim3(512), 0, st, p);
+    else hipLaunchKernelGGL((row_int8_back_kernel<OT, PART, 6, 4, 2, 4, 3, 2>), grid, dim3(512), 0, st, p);
 }
 
 int launch_row_int8_back(const void *grad, const uint8_t *w, const float *ws, void *gx, int dtype, int M, int N, int K, uint8_t *space, hipStream_t st) {

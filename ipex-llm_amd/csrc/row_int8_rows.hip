@@ -1,15 +1,13 @@
-// Up to sixteen rows of activations times a weight with a scale for each row (row_int8.h): the weight streams past once, in one launch.
+// Up to four rows of activations times a weight with a scale for each row (row_int8.h): the weight streams past once, in one launch.
 //
 // A workgroup owns 16 weight rows; its waves take the blocks of K in turn and their sums meet in LDS.  A wave's loads are 16 rows x 64
 // contiguous bytes, STEPS blocks ahead of their use.  x is quantized by each workgroup, into LDS, while the first weights are on their
 // way: its largest magnitudes by row first, then its codes.  Loads return in order, so x is asked for ahead of the weights.
 #include "row_int8_tiled.h"
 
-#include <math.h>
-
 namespace lowbit {
 
-constexpr int FEW_ROWS = 16;                                 // an MFMA's
+constexpr int FEW_ROWS = 4;
 
 struct Int8Rows {
     const void *x;                                           // [M, K]
@@ -136,31 +134,60 @@ __global__ __launch_bounds__(64 * WAVES) void row_int8_few_rows_kernel(const Int
     ((AT *)p.y)[(int64_t)m * N + n0 + c] = Stored<AT>::of(v);
 }
 
-static size_t few_rows_lds(int M, int KB) {
-    const size_t codes = (size_t)M * (KB * INT8_BLOCK + 16);
-    return codes > 16384 ? codes : 16384;                    // (the sums of 16 waves)
+static size_t few_rows_lds(int M, int KB, int waves) {
+    const size_t codes = (size_t)M * (KB * INT8_BLOCK + 16), sums = (size_t)waves * FEW_ROWS * 16 * sizeof(int32_t);
+    return codes > sums ? codes : sums;
 }
 
-constexpr size_t FEW_LDS = 65536 - 64;
-static int few_rows_waves(int N, int KB) { return KB <= 16 ? 4 : KB > 64 && N <= 8192 ? 16 : 8; }
-
-template <typename AT> static void launch_few_rows(const Int8Rows &p, hipStream_t st) {
+template <typename AT> static void launch_few_rows(const Int8Rows &p, int waves, hipStream_t st) {
     const dim3 grid((p.N + 15) / 16);
-    const size_t lds = few_rows_lds(p.M, p.KB);
-    const int waves = few_rows_waves(p.N, p.KB);
+    const size_t lds = few_rows_lds(p.M, p.KB, waves);
     if (waves == 4) hipLaunchKernelGGL((row_int8_few_rows_kernel<AT, 4>), grid, dim3(256), lds, st, p);
-    else if (waves == 16) hipLaunchKernelGGL((row_int8_few_rows_kernel<AT, 16>), grid, dim3(1024), lds, st, p);
     else hipLaunchKernelGGL((row_int8_few_rows_kernel<AT, 8>), grid, dim3(512), lds, st, p);
 }
 
-// Rows whose codes fit 64 KiB of LDS: up to four always, up to sixteen where that is estimated shorter than tiles and the launch ahead of them.
-static bool takes_few_rows(int M, int N, int K) {
+// Waves of a workgroup, by estimated time in us; 0 where codes of x, made by a launch of their own, and a product of those are estimated shorter,
+// or where x's codes do not fit 64 KiB of LDS.  What grows with the rows is x, which every workgroup reads and quantizes: on [4096 x 4096] one row
+// 6.1 against 6.3 and the launch ahead of it, 2.6; four 8.8 / 6.6 + 2.6; on [28672 x 8192] one 44.5 / 44.4 + 2.6, four 71 / 46 + 2.7; one on
+// [20000 x 512] 9.4 / 4.2 + 2.6.  Fitted to 80 sizes of 1 to 16 rows, within 11 and 17 % at rms; 16
+// waves would be the shortest at one row of very long weights only, [4096 x 11008] 13.7 against 14.3.
+constexpr size_t FEW_LDS = 65536 - 64;
+constexpr float ROWS_LAUNCH_US = 2.6f;
+static int few_rows_waves(int M, int N, int K, float codes_us) {
+    static const struct {
+        int waves;
+        float launch, further, block, row;
+    } fits[] = {{4, 3.0f, 0.09f, 0.077f, 0.136f}, {8, 4.0f, 1.9f, 0.053f, 0.183f}};
     const int KB = int8_blocks(K);
-    if (M > FEW_ROWS || few_rows_lds(M, KB) > FEW_LDS) return false;
-    if (M <= 4) return true;
-    const float rounds = N > 4096 ? N / 4096.0f : 1.0f;      // of a workgroup per CU
-    const float bytes = (float)N * K, us = 3.1f + bytes / 5.6e6f + 0.038f * M * rounds * K / (64 * few_rows_waves(N, KB));
-    return us <= fmaxf(row_int8_tiled_plan(M, N, K).us, bytes / 5.4e6f + 4.0f) + 1.5f;
+    const float units = (N + 15) / 16 / 256.0f, load = units > 1.0f ? units : 1.0f;
+    float least = codes_us + ROWS_LAUNCH_US;
+    int best = 0;
+    for (const auto &f : fits) {
+        if (M > FEW_ROWS || few_rows_lds(M, KB, f.waves) > FEW_LDS) continue;
+        const float us = f.launch + f.further * (load - 1.0f) + load * KB * (f.block + f.row * M / f.waves);
+        if (us < least) {
+            least = us;
+            best = f.waves;
+        }
+    }
+    return best;
+}
+
+// What a product of these sizes runs as.  A call asks twice, for the workspace and for the launch: the last sizes' plan, a microsecond's
+// estimates, is kept.
+struct LinearPlan {
+    int few;                                                 // waves of the kernel of few rows, or 0
+    Int8Plan plan;
+};
+static LinearPlan linear_plan(int M, int N, int K) {
+    static thread_local int last[3] = {};
+    static thread_local LinearPlan kept;
+    if (M != last[0] || N != last[1] || K != last[2]) {
+        kept.plan = row_int8_product_plan(M, N, K);
+        kept.few = few_rows_waves(M, N, K, kept.plan.us);
+        last[0] = M; last[1] = N; last[2] = K;
+    }
+    return kept;
 }
 
 // codes of x, their scales, a split's sums
@@ -177,35 +204,41 @@ static Int8Space linear_space(int M, int N, int K, const Int8Plan &plan) {
 }
 
 size_t row_int8_linear_workspace_bytes(int M, int N, int K) {
-    return takes_few_rows(M, N, K) ? 0 : linear_space(M, N, K, row_int8_tiled_plan(M, N, K)).bytes;
+    const LinearPlan p = linear_plan(M, N, K);
+    return p.few ? 0 : linear_space(M, N, K, p.plan).bytes;
 }
 
-// rows and columns of a tile (0, 0: the kernel of few rows), splits, groups
+// rows and columns of a tile (0, 0: the kernel of few rows; columns 16: the streaming kernel), splits, groups
 void row_int8_linear_plan(int M, int N, int K, int *plan4) {
     plan4[0] = plan4[1] = 0;
     plan4[2] = plan4[3] = 1;
-    if (takes_few_rows(M, N, K)) return;
-    const Int8Plan plan = row_int8_tiled_plan(M, N, K);
-    plan4[0] = INT8_FORMS[plan.form].rows;
-    plan4[1] = INT8_FORMS[plan.form].cols;
+    const LinearPlan p = linear_plan(M, N, K);
+    if (p.few) return;
+    const Int8Plan &plan = p.plan;
+    plan4[0] = plan.waves ? (M > 16 ? 32 : 16) : INT8_FORMS[plan.form].rows;
+    plan4[1] = plan.waves ? 16 : INT8_FORMS[plan.form].cols;
     plan4[2] = plan.splits;
-    plan4[3] = INT8_FORMS[plan.form].groups;
+    plan4[3] = plan.waves ? 1 : INT8_FORMS[plan.form].groups;
 }
 
-// waves of a workgroup of the kernel of few rows; 0 where tiles run
-int row_int8_linear_waves(int M, int N, int K) { return takes_few_rows(M, N, K) ? few_rows_waves(N, int8_blocks(K)) : 0; }
+// waves of a workgroup of the kernel of few rows or of the streaming kernel; 0 where tiles run
+int row_int8_linear_waves(int M, int N, int K) {
+    const LinearPlan p = linear_plan(M, N, K);
+    return p.few ? p.few : p.plan.waves;
+}
 
 int launch_row_int8_linear(const void *x, const uint8_t *w, const float *ws, const void *bias, void *y, int dtype, int M, int N, int K, uint8_t *space,
                            hipStream_t st) {
-    if (takes_few_rows(M, N, K)) {
+    const LinearPlan all = linear_plan(M, N, K);
+    if (const int waves = all.few) {
         const Int8Rows p = {x, w, ws, bias, y, M, N, K, int8_blocks(K)};
-        if (dtype == DT_F16) launch_few_rows<_Float16>(p, st);
-        else if (dtype == DT_BF16) launch_few_rows<__bf16>(p, st);
-        else if (dtype == DT_F32) launch_few_rows<float>(p, st);
+        if (dtype == DT_F16) launch_few_rows<_Float16>(p, waves, st);
+        else if (dtype == DT_BF16) launch_few_rows<__bf16>(p, waves, st);
+        else if (dtype == DT_F32) launch_few_rows<float>(p, waves, st);
         else return -4;
         return 0;
     }
-    const Int8Plan plan = row_int8_tiled_plan(M, N, K);
+    const Int8Plan &plan = all.plan;
     const Int8Space at = linear_space(M, N, K, plan);
     float *const xs = (float *)(space + at.xs);
     Int8Args t{};
@@ -213,7 +246,7 @@ int launch_row_int8_linear(const void *x, const uint8_t *w, const float *ws, con
     if (int rc = launch_row_int8_quantize(x, dtype, M, K, space, (int)t.ldx, xs, nullptr, st)) return rc;
     t.x = space; t.xs = xs; t.w = w; t.ws = ws; t.bias = bias; t.y = y; t.part = (int32_t *)(space + at.part);
     t.M = M; t.N = N; t.K = K;
-    return launch_row_int8_tiled(t, dtype, plan, st);
+    return launch_row_int8_codes(t, dtype, plan, st);
 }
 
 // Rows of codes that do not fill whole blocks, in rows of ldx bytes with zeros past K; 16 bytes per thread.
@@ -229,7 +262,7 @@ static bool whole_blocks(int K) { return K % INT8_BLOCK == 0; }
 
 size_t row_int8_product_workspace_bytes(int M, int N, int K) {
     const size_t padded = whole_blocks(K) ? 0 : (size_t)M * int8_blocks(K) * INT8_BLOCK;
-    return ((padded + 255) & ~(size_t)255) + row_int8_part_bytes(row_int8_tiled_plan(M, N, K), M, N);
+    return ((padded + 255) & ~(size_t)255) + row_int8_part_bytes(linear_plan(M, N, K).plan, M, N);
 }
 
 int launch_row_int8_product(const uint8_t *codes, const float *xs, const uint8_t *w, const float *ws, const void *bias, void *y, int dtype, int M, int N,
@@ -246,7 +279,7 @@ int launch_row_int8_product(const uint8_t *codes, const float *xs, const uint8_t
     }
     t.xs = xs; t.w = w; t.ws = ws; t.bias = bias; t.y = y; t.part = (int32_t *)space;
     t.M = M; t.N = N; t.K = K;
-    return launch_row_int8_tiled(t, dtype, row_int8_tiled_plan(M, N, K), st);
+    return launch_row_int8_codes(t, dtype, linear_plan(M, N, K).plan, st);
 }
 
 }  // namespace lowbit

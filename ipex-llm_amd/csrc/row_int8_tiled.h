@@ -10,24 +10,24 @@ struct Int8Form {
     int rows, cols, per_cu, groups;
     float step_us, alone_us;
 };
-enum { INT8_256, INT8_192_256, INT8_128_256, INT8_128, INT8_64, INT8_32, INT8_64_SHARED, INT8_64_64_SHARED, INT8_COUNT };
+enum { INT8_256, INT8_192_256, INT8_128_256, INT8_128, INT8_64, INT8_32, INT8_64_SHARED, INT8_COUNT };
 static const Int8Form INT8_FORMS[INT8_COUNT] = {
-    {256, 256, 1, 1, 1.73f, 1.48f},
-    {192, 256, 1, 1, 1.40f, 1.11f},
-    {128, 256, 1, 1, 1.03f, 0.83f},
-    {128, 128, 2, 1, 0.99f, 0.54f},
-    {64, 128, 2, 1, 0.68f, 0.37f},
-    {32, 128, 2, 1, 0.70f, 0.34f},
-    {64, 128, 1, 2, 0.86f, 0.65f},
-    {64, 64, 1, 2, 0.70f, 0.43f},
+    {256, 256, 1, 1, 1.20f, 1.04f},
+    {192, 256, 1, 1, 0.985f, 0.88f},
+    {128, 256, 1, 1, 0.76f, 0.71f},
+    {128, 128, 2, 1, 0.875f, 0.48f},
+    {64, 128, 2, 1, 0.645f, 0.31f},
+    {32, 128, 2, 1, 0.55f, 0.247f},
+    {64, 64, 1, 2, 0.76f, 0.455f},
 };
 
+// What a product of codes runs as: a form of tiles, or (waves > 0) the streaming kernel of row_int8_stream.h
 struct Int8Plan {
-    int form, splits;
+    int form, splits, waves;
     float us;
 };
 
-// One launch per form; the wave tiles are 64 x 128, 96 x 64, 64 x 64, 64 x 64, 32 x 64, 32 x 32, 32 x 64 and 32 x 32.
+// One launch per form; the wave tiles are 64 x 128, 96 x 64, 64 x 64, 64 x 64, 32 x 64, 32 x 32 and 32 x 32.
 template <typename OT, Int8Mode MODE, bool BY_EXPERT = false> void launch_int8_form(const Int8Args &p, int form, hipStream_t st) {
     if (form == INT8_256) launch_int8_tile<OT, MODE, BY_EXPERT, false, 4, 8, 4, 2, 2, 2>(p, st);
     else if (form == INT8_192_256) launch_int8_tile<OT, MODE, BY_EXPERT, false, 6, 4, 2, 4, 2, 2>(p, st);
@@ -35,10 +35,7 @@ template <typename OT, Int8Mode MODE, bool BY_EXPERT = false> void launch_int8_f
     else if (form == INT8_128) launch_int8_tile<OT, MODE, BY_EXPERT, false, 4, 4, 2, 2, 2, 2>(p, st);
     else if (form == INT8_64) launch_int8_tile<OT, MODE, BY_EXPERT, false, 2, 4, 2, 2, 3, 2>(p, st);
     else if (form == INT8_32) launch_int8_tile<OT, MODE, BY_EXPERT, false, 2, 2, 1, 4, 3, 2>(p, st);
-    else if constexpr (!BY_EXPERT) {
-        if (form == INT8_64_SHARED) launch_int8_tile<OT, MODE, BY_EXPERT, false, 2, 4, 2, 2, 3, 2, 2>(p, st);
-        else launch_int8_tile<OT, MODE, BY_EXPERT, false, 2, 2, 2, 2, 3, 2, 2>(p, st);
-    }
+    else if constexpr (!BY_EXPERT) launch_int8_tile<OT, MODE, BY_EXPERT, false, 2, 2, 2, 2, 3, 2, 2>(p, st);
 }
 
 void launch_int8_f16(const Int8Args &p, int form, hipStream_t st);
@@ -48,9 +45,9 @@ void launch_int8_part(const Int8Args &p, int form, hipStream_t st);
 
 // Estimated time (us) of `units` tiles of a form that walk `steps` blocks each (block_fp8_gemm.hip)
 float tiled_walk_us(float step_us, float alone_us, int per_cu, int64_t units, int steps);
-Int8Plan row_int8_tiled_plan(int M, int N, int K);
+Int8Plan row_int8_product_plan(int M, int N, int K);
 size_t row_int8_part_bytes(const Int8Plan &plan, int M, int N);
-int launch_row_int8_tiled(Int8Args p, int dtype, const Int8Plan &plan, hipStream_t st);
+int launch_row_int8_codes(Int8Args p, int dtype, const Int8Plan &plan, hipStream_t st);
 int launch_row_int8_quantize(const void *x, int dtype, int64_t rows, int K, uint8_t *codes, int ldc, float *scale, const int32_t *limit, hipStream_t st);
 
 }  // namespace lowbit
