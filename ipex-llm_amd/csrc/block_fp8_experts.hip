@@ -212,7 +212,7 @@ __global__ __launch_bounds__(64 * WAVES) void block_fp8_expert_down_token_kernel
 }
 
 // The rows of x in codes (as bfloat16 numbers, see EXACT) and scales, and the pairs' sort by expert or its first half, in one launch: the
-// first workgroups quantize (32 blocks each), the rest place pairs, or count them for the launch that does (expert_sort.h).
+// first workgroups quantize (32 blocks each); one more sorts the pairs, or as many as there are chunks count them for the launch that does (expert_sort.h).
 template <typename AT, bool PLACES>
 __global__ __launch_bounds__(256) void block_fp8_expert_rows_kernel(const AT *__restrict__ x, const int64_t *__restrict__ ids, uint8_t *__restrict__ codes,
                                                                     float *__restrict__ scale, int32_t *__restrict__ offsets, int32_t *__restrict__ order,
@@ -228,7 +228,7 @@ __global__ __launch_bounds__(256) void block_fp8_expert_rows_kernel(const AT *__
         if ((threadIdx.x & 7) == 0) scale[(int64_t)kb * tokens + row] = s;
         return;
     }
-    if constexpr (PLACES) place_pairs(ids, offsets, order, pos, pairs, n_exp, blockIdx.x - quantizing);
+    if constexpr (PLACES) sort_pairs(ids, offsets, order, pos, pairs, n_exp);
     else count_pairs(ids, counts, pairs, n_exp, chunk, blockIdx.x - quantizing);
 }
 
@@ -317,7 +317,7 @@ void block_fp8_experts_plan(int tokens, int top_k, int n_exp, int H, int I, int 
     plan4[0] = up_rows(pairs, n_exp, I);
     plan4[1] = down.rows;
     plan4[2] = down.cols;
-    plan4[3] = pairs > EXPERTS_SORT_PAIRS;
+    plan4[3] = !one_sorts(pairs, n_exp);
 }
 
 struct ExpertsSpace {
@@ -344,7 +344,7 @@ static ExpertsSpace experts_space(int tokens, int top_k, int n_exp, int H, int I
         w.offsets = take((size_t)(n_exp + 1) * 4);
         w.order = take((size_t)pairs * 4);
         w.pos = take((size_t)pairs * 4);
-        if (pairs > EXPERTS_SORT_PAIRS) w.counts = take((size_t)EXPERTS_CHUNKS * n_exp * 4);
+        if (!one_sorts(pairs, n_exp)) w.counts = take((size_t)EXPERTS_CHUNKS * n_exp * 4);
         w.y = take((size_t)pairs * down_columns(pairs, H) * sizeof(float));        // (rounded once, when a token's are summed: 16 bits would cost its precision twice)
     }
     w.bytes = at;
@@ -388,8 +388,8 @@ template <typename AT> static int launch_experts_t(ExpertsArgs p, const ExpertsS
     int32_t *const counts = (int32_t *)(ws + at.counts);
     const AT *const x = (const AT *)p.x;
     float *const xs = (float *)(ws + at.xs);
-    if (pairs <= EXPERTS_SORT_PAIRS)
-        hipLaunchKernelGGL((block_fp8_expert_rows_kernel<AT, true>), dim3(quantizing + (pairs + p.n_exp + 4) / 4), dim3(256), 0, st, x, p.ids, ws + at.x,
+    if (one_sorts(pairs, p.n_exp))
+        hipLaunchKernelGGL((block_fp8_expert_rows_kernel<AT, true>), dim3(quantizing + 1), dim3(256), sort_lds(p.n_exp), st, x, p.ids, ws + at.x,
                            xs, offsets, order, pos, nullptr, tokens, pairs, p.n_exp, p.H, KB, quantizing, 0);
     else {
         const int chunk = sort_chunk(pairs), chunks = (pairs + chunk - 1) / chunk;

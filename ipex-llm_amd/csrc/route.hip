@@ -159,8 +159,15 @@ template <int NR> __global__ __launch_bounds__(256) void route_select_kernel(con
         const int e = lane + 64 * i;
         z[i] = 0.0;
         if (e < p.E) {
-            z[i] = p.part[t * p.E + e];
-            for (int v = 1; v < p.splits; v++) z[i] += p.part[((int64_t)v * p.T + t) * p.E + e];
+            const double *const from = p.part + t * p.E + e;
+            const int64_t stride = (int64_t)p.T * p.E;
+            for (int v = 0; v < p.splits; v += 8) {          // (the parts on their way together, added in order)
+                double part[8];
+#pragma unroll
+                for (int u = 0; u < 8; u++) part[u] = v + u < p.splits ? from[(v + u) * stride] : 0.0;
+#pragma unroll
+                for (int u = 0; u < 8; u++) z[i] += part[u];
+            }
             if (p.z) p.z[t * p.E + e] = z[i];
         }
     }

@@ -88,7 +88,7 @@ __device__ inline uint32_t max_of_wave(uint32_t v) {
 
 // One row of K values by the threads t of WAVES waves, 16 values per thread and piece; what lies past the first HELD pieces is read again behind
 // the row's maximum.  Codes go to ldc bytes, zeros from K up to ldc.  Returns the scale.
-template <typename AT, int WAVES, int HELD> __device__ inline float quantize_row(const AT *__restrict__ from, uint8_t *__restrict__ to, int K, int ldc, int t) {
+template <typename AT, int WAVES, int HELD> __device__ __forceinline__ float quantize_row(const AT *__restrict__ from, uint8_t *__restrict__ to, int K, int ldc, int t) {
     constexpr int STEP = 64 * WAVES * 16;
     float v[HELD][16];
     uint32_t m = 0;

@@ -238,16 +238,17 @@ __global__ __launch_bounds__(64 * WAVES) void row_int8_expert_down_token_kernel(
     out[(int64_t)token * p.H + n0 + threadIdx.x] = Stored<AT>::of(v);
 }
 
-// The rows of x in codes and scales, a row per workgroup, and the pairs' sort by expert or its first half, in one launch (expert_sort.h).
+// The rows of x in codes and scales, a row per workgroup, and the pairs' sort by expert or its first half, in one launch (expert_sort.h).  The sort
+// goes first: it takes the longest.
 template <typename AT, bool PLACES>
 __global__ __launch_bounds__(256) void row_int8_expert_rows_kernel(const AT *__restrict__ x, const int64_t *__restrict__ ids, uint8_t *__restrict__ codes,
                                                                    float *__restrict__ scale, int32_t *__restrict__ offsets, int32_t *__restrict__ order,
                                                                    int32_t *__restrict__ pos, int32_t *__restrict__ counts, int tokens, int pairs,
-                                                                   int n_exp, int H, int ldc, int chunk) {
-    const int row = blockIdx.x;
-    if (row >= tokens) {
-        if constexpr (PLACES) place_pairs(ids, offsets, order, pos, pairs, n_exp, row - tokens);
-        else count_pairs(ids, counts, pairs, n_exp, chunk, row - tokens);
+                                                                   int n_exp, int H, int ldc, int chunk, int sorting) {
+    const int row = (int)blockIdx.x - sorting;
+    if (row < 0) {
+        if constexpr (PLACES) sort_pairs(ids, offsets, order, pos, pairs, n_exp);
+        else count_pairs(ids, counts, pairs, n_exp, chunk, blockIdx.x);
         return;
     }
     const float s = quantize_row<AT, 4, 1>(x + (int64_t)row * H, codes + (int64_t)row * ldc, H, ldc, threadIdx.x);
@@ -277,36 +278,36 @@ static double expert_tiles(int pairs, int n_exp, int rows) {
     for (int k = sure + 1; k * (double)rows < mean + 4.0 * spread; k++) tiles += 0.5 * erfc((k * (double)rows - mean) / spread);
     return tiles * (pairs < n_exp ? pairs : n_exp);
 }
-static int up_rows(int pairs, int n_exp, int I) {
-    static const struct {
-        int rows;
-        float step_us, alone_us;
-    } forms[] = {{64, 0.8f, 0.7f}, {128, 1.2f, 1.0f}};
+//
+// Both launches' times are fitted to 37 sizes, 4 to 4096 tokens through 1 to 8 of 4 to 160 experts, [256 to 14336 x 512 to 8192]: for each round of
+// workgroups over the GPU what goes by the tile, and by its steps for each whole one.  The picks are 2.6 % and 2.7 % above the fastest of fourteen
+// forms on average, 18 and 22 % at worst.  First product, us at 32 / 64 / 128 / 192 rows: 64 experts of [1408 x 2048], 47 rows each in the mean, 92 / 81 / 88 / 88, 8
+// of [14336 x 4096], 8 rows 162 / 162 / 163 / 174, 128 rows 327 / 277 / 260 / 220, 500 rows 1011 / 782 / 634 / 514.
+struct ExpertForm {
+    int rows, cols, per_cu;                                  // cols: of weight rows, half of which are u's in the first product
+    float tile_us, step_us;
+};
+enum { UP_32, UP_64, UP_128, UP_192 };
+static const ExpertForm UP_FORMS[4] = {{32, 128, 2, 3.83f, 0.635f}, {64, 128, 3, 2.68f, 1.05f}, {128, 128, 2, 4.35f, 0.995f}, {192, 256, 1, 5.42f, 1.15f}};
+enum { DOWN_64_64, DOWN_64, DOWN_128, DOWN_256 };
+static const ExpertForm DOWN_FORMS[4] = {{64, 64, 2, 3.53f, 0.565f}, {64, 128, 3, 4.62f, 0.85f}, {128, 256, 1, 5.97f, 0.98f}, {256, 256, 1, 7.6f, 1.105f}};
+
+static int expert_form(const ExpertForm (&forms)[4], int pairs, int n_exp, int N, int K) {
     int best = 0;
-    double least = 0.0;
-    for (const auto &f : forms) {
-        const double rounds = expert_tiles(pairs, n_exp, f.rows) * ((I + 127) / 128) / 256.0, us = rounds <= 1.0 ? f.alone_us : rounds * f.step_us;
-        if (!best || us < least) {
-            least = us;
-            best = f.rows;
-        }
-    }
-    return best;
-}
-static int down_form(int pairs, int n_exp, int H, int I) {
-    int best = INT8_32;
     float least = 0.0f;
-    for (int form = 0; form < INT8_COUNT; form++) {
-        const Int8Form &f = INT8_FORMS[form];
-        if (f.groups > 1) continue;                          // (an expert's last tile, of few rows, would hold a CU for twice as many waves)
-        const float us = tiled_walk_us(f.step_us, f.alone_us, f.per_cu, (int64_t)(expert_tiles(pairs, n_exp, f.rows) * ((H + f.cols - 1) / f.cols) + 0.5), int8_blocks(I));
-        if (form == 0 || us < least) {
+    for (int i = 0; i < 4; i++) {
+        const ExpertForm &f = forms[i];
+        const float rounds = (float)expert_tiles(pairs, n_exp, f.rows) * ((N + f.cols - 1) / f.cols) / (256 * f.per_cu);
+        const float us = (rounds > 1.0f ? rounds : 1.0f) * f.tile_us + ceilf(rounds) * f.step_us * int8_blocks(K);
+        if (i == 0 || us < least) {
             least = us;
-            best = form;
+            best = i;
         }
     }
     return best;
 }
+static int up_form(int pairs, int n_exp, int H, int I) { return expert_form(UP_FORMS, pairs, n_exp, 2 * I, H); }
+static int down_form(int pairs, int n_exp, int H, int I) { return expert_form(DOWN_FORMS, pairs, n_exp, H, I); }
 
 // Tokens that go through the sorted launches together: as many as keep h, its codes and the pairs' results within 2 GiB.
 constexpr int64_t EXPERTS_HELD = (int64_t)1 << 31;
@@ -319,11 +320,11 @@ void row_int8_experts_plan(int tokens, int top_k, int n_exp, int H, int I, int *
     plan4[0] = plan4[1] = plan4[2] = plan4[3] = 0;
     if (direct(tokens, top_k, n_exp, H, I)) return;
     const int pairs = tokens_at_once(tokens, top_k, H, I) * top_k;
-    const Int8Form &down = INT8_FORMS[down_form(pairs, n_exp, H, I)];
-    plan4[0] = up_rows(pairs, n_exp, I);
+    const ExpertForm &down = DOWN_FORMS[down_form(pairs, n_exp, H, I)];
+    plan4[0] = UP_FORMS[up_form(pairs, n_exp, H, I)].rows;
     plan4[1] = down.rows;
     plan4[2] = down.cols;
-    plan4[3] = pairs > EXPERTS_SORT_PAIRS;
+    plan4[3] = !one_sorts(pairs, n_exp);
 }
 
 struct ExpertsSpace {
@@ -350,7 +351,7 @@ static ExpertsSpace experts_space(int tokens, int top_k, int n_exp, int H, int I
         w.offsets = take((size_t)(n_exp + 1) * 4);
         w.order = take((size_t)pairs * 4);
         w.pos = take((size_t)pairs * 4);
-        if (pairs > EXPERTS_SORT_PAIRS) w.counts = take((size_t)EXPERTS_CHUNKS * n_exp * 4);
+        if (!one_sorts(pairs, n_exp)) w.counts = take((size_t)EXPERTS_CHUNKS * n_exp * 4);
         w.y = take((size_t)pairs * H * sizeof(float));       // (rounded once, when a token's are summed)
     }
     w.bytes = at;
@@ -383,13 +384,13 @@ template <typename AT> static int launch_sorted(Int8Experts p, const ExpertsSpac
     if ((int64_t)tokens + pairs + p.n_exp > most_groups(256)) return -3;
     const AT *const x = (const AT *)p.x;
     float *const xs = (float *)(ws + at.xs), *const hs = (float *)(ws + at.hs);
-    if (pairs <= EXPERTS_SORT_PAIRS)
-        hipLaunchKernelGGL((row_int8_expert_rows_kernel<AT, true>), dim3(tokens + (pairs + p.n_exp + 4) / 4), dim3(256), 0, st, x, p.ids, ws + at.x, xs, offsets,
-                           order, pos, nullptr, tokens, pairs, p.n_exp, p.H, ldx, 0);
+    if (one_sorts(pairs, p.n_exp))
+        hipLaunchKernelGGL((row_int8_expert_rows_kernel<AT, true>), dim3(1 + tokens), dim3(256), sort_lds(p.n_exp), st, x, p.ids, ws + at.x, xs, offsets, order,
+                           pos, nullptr, tokens, pairs, p.n_exp, p.H, ldx, 0, 1);
     else {
         const int chunk = sort_chunk(pairs), chunks = (pairs + chunk - 1) / chunk;
-        hipLaunchKernelGGL((row_int8_expert_rows_kernel<AT, false>), dim3(tokens + chunks), dim3(256), (size_t)p.n_exp * 4, st, x, p.ids, ws + at.x, xs,
-                           offsets, order, pos, counts, tokens, pairs, p.n_exp, p.H, ldx, chunk);
+        hipLaunchKernelGGL((row_int8_expert_rows_kernel<AT, false>), dim3(chunks + tokens), dim3(256), (size_t)p.n_exp * 4, st, x, p.ids, ws + at.x, xs,
+                           offsets, order, pos, counts, tokens, pairs, p.n_exp, p.H, ldx, chunk, chunks);
         launch_expert_place(p.ids, counts, offsets, order, pos, pairs, p.n_exp, st);
     }
 
@@ -405,14 +406,19 @@ template <typename AT> static int launch_sorted(Int8Experts p, const ExpertsSpac
     d.w = p.down; d.ws = p.down_scale; d.N = p.H; d.K = p.I; d.KB = int8_blocks(p.I);
     d.expert_rows = p.H;
     d.y = ws + at.y;
-    const int rows = up_rows(pairs, p.n_exp, p.I), form = down_form(pairs, p.n_exp, p.H, p.I), used = pairs < p.n_exp ? pairs : p.n_exp;
-    u.tiles_m = pairs / rows + used;                         // at most
-    d.tiles_m = pairs / INT8_FORMS[form].rows + used;
-    if ((int64_t)u.tiles_m * ((p.I + 127) / 128) > most_groups(512) || (int64_t)d.tiles_m * ((p.H + 127) / 128) > most_groups(512)) return -3;
-    if (rows == 64) launch_int8_tile<float, INT8_UP, true, true, 2, 4, 2, 4, 3, 2>(u, st);
-    else launch_int8_tile<float, INT8_UP, true, true, 4, 4, 2, 4, 3, 2>(u, st);
+    const int up = up_form(pairs, p.n_exp, p.H, p.I), down = down_form(pairs, p.n_exp, p.H, p.I), used = pairs < p.n_exp ? pairs : p.n_exp;
+    u.tiles_m = pairs / UP_FORMS[up].rows + used;            // at most
+    d.tiles_m = pairs / DOWN_FORMS[down].rows + used;
+    if ((int64_t)u.tiles_m * ((p.I + 63) / 64) > most_groups(512) || (int64_t)d.tiles_m * ((p.H + 63) / 64) > most_groups(512)) return -3;
+    if (up == UP_32) launch_int8_tile<float, INT8_UP, true, true, 2, 2, 1, 4, 4, 2>(u, st);
+    else if (up == UP_64) launch_int8_tile<float, INT8_UP, true, true, 2, 4, 2, 2, 2, 2>(u, st);
+    else if (up == UP_128) launch_int8_tile<float, INT8_UP, true, true, 4, 4, 2, 2, 2, 2>(u, st);
+    else launch_int8_tile<float, INT8_UP, true, true, 6, 4, 2, 4, 2, 2>(u, st);
     if (int rc = launch_row_int8_quantize(p.h, DT_F32, pairs, p.I, ws + at.codes, ldh, hs, offsets + p.n_exp, st)) return rc;
-    launch_int8_form<float, INT8_PLAIN, true>(d, form, st);
+    if (down == DOWN_64_64) launch_int8_tile<float, INT8_PLAIN, true, false, 2, 2, 2, 2, 4, 2>(d, st);
+    else if (down == DOWN_64) launch_int8_tile<float, INT8_PLAIN, true, false, 2, 4, 2, 2, 2, 2>(d, st);
+    else if (down == DOWN_128) launch_int8_tile<float, INT8_PLAIN, true, false, 4, 4, 2, 4, 3, 2>(d, st);
+    else launch_int8_tile<float, INT8_PLAIN, true, false, 4, 8, 4, 2, 2, 2>(d, st);
     launch_moe_combine_f32((const float *)(ws + at.y), pos, weight, w_dtype, out, act_dtype, tokens, p.top_k, p.H, p.H, st);
     return 0;
 }

@@ -29,6 +29,36 @@ struct Int8Args {
 
 enum Int8Mode { INT8_PLAIN, INT8_PART, INT8_UP };
 
+// Which tile a workgroup of a product grouped by expert works on: expert after expert, of each its columns in turn, of each column its row tiles of
+// ROWS rows side by side: they share its weights, and all of an expert's tiles its rows, mostly in one XCD's L2.  Called by whole waves; false past the last.
+struct ExpertUnit {
+    int expert, first, end, column;                          // rows first .. end - 1 (end: the expert's, not the tile's)
+};
+template <int ROWS> __device__ inline bool find_expert_unit(const int32_t *__restrict__ offsets, int n_exp, int unit, int tiles_n, ExpertUnit &u) {
+    const int lane = threadIdx.x & 63;
+    for (int e0 = 0; e0 < n_exp; e0 += 64) {
+        const int e = e0 + lane, from = e < n_exp ? offsets[e] : 0, to = e < n_exp ? offsets[e + 1] : 0, own = (to - from + ROWS - 1) / ROWS;
+        int upto = own;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int up = __shfl_up(upto, d);
+            if (lane >= d) upto += up;
+        }
+        const int all = __builtin_amdgcn_readlane(upto, 63);
+        if (unit < all * tiles_n) {
+            const int l = __builtin_ctzll(__ballot(upto * tiles_n > unit)), tiles = __builtin_amdgcn_readlane(own, l);
+            const int at = unit - (__builtin_amdgcn_readlane(upto, l) - tiles) * tiles_n;
+            u.expert = e0 + l;
+            u.column = at / tiles;
+            u.first = __builtin_amdgcn_readlane(from, l) + (at - u.column * tiles) * ROWS;
+            u.end = __builtin_amdgcn_readlane(to, l);
+            return true;
+        }
+        unit -= all * tiles_n;
+    }
+    return false;
+}
+
 // BY_EXPERT: row tiles of one expert each.  GATHER: x rows by order[].  S: buffers in LDS.  KG: groups of WM x WN waves, each with buffers of
 // its own, that share a tile's blocks out among them and add their sums at the end.
 template <typename OT, Int8Mode MODE, bool BY_EXPERT, bool GATHER, int TM, int TN, int WM, int WN, int S, int MIN_WAVES, int KG = 1>
@@ -49,24 +79,24 @@ __global__ __launch_bounds__(64 * WM * WN * KG, MIN_WAVES) void row_int8_tiled_k
     uint8_t *const lds = shared + group * OWN;
 
     // Runs of tiles to the XCDs in turn, so that an L2 serves every operand several times (block_fp8_gemm.h).
-    const int tiles_m = BY_EXPERT ? count_expert_tiles<BM>(p.offsets, p.n_exp) : p.tiles_m, tall = BY_EXPERT ? tiles_m : 8;
+    const int tiles_m = BY_EXPERT ? count_expert_tiles<BM>(p.offsets, p.n_exp) : p.tiles_m;
     const uint32_t units = (uint32_t)(tiles_m * p.tiles_n * p.splits), xcd = blockIdx.x & 7;
     const uint32_t unit = (uint32_t)((uint64_t)units * xcd >> 3) + (blockIdx.x >> 3);
     if (unit >= (uint32_t)((uint64_t)units * (xcd + 1) >> 3)) return;
-    const int tile = (int)(unit / p.splits), split = (int)(unit - (uint32_t)tile * p.splits);
-    int tm, tn;
-    {
-        const int per = tall * p.tiles_n, band = tile / per, at = tile - band * per, rows = tiles_m - band * tall < tall ? tiles_m - band * tall : tall;
-        tn = at / rows;
-        tm = band * tall + at - tn * rows;
-    }
-    int m0 = tm * BM, end = p.M, expert = 0;
+    int m0, tn, end = p.M, expert = 0, split = 0;
     if constexpr (BY_EXPERT) {
-        ExpertTile t;
-        if (!find_expert_tile<BM>(p.offsets, p.n_exp, tm, t)) return;
-        expert = __builtin_amdgcn_readfirstlane(t.expert);
-        m0 = __builtin_amdgcn_readfirstlane(t.first);
-        end = __builtin_amdgcn_readfirstlane(t.end);
+        ExpertUnit u;
+        if (!find_expert_unit<BM>(p.offsets, p.n_exp, (int)unit, p.tiles_n, u)) return;
+        expert = __builtin_amdgcn_readfirstlane(u.expert);
+        m0 = __builtin_amdgcn_readfirstlane(u.first);
+        end = __builtin_amdgcn_readfirstlane(u.end);
+        tn = __builtin_amdgcn_readfirstlane(u.column);
+    } else {
+        const int tile = (int)(unit / p.splits), per = 8 * p.tiles_n, band = tile / per, at = tile - band * per;
+        const int rows = tiles_m - band * 8 < 8 ? tiles_m - band * 8 : 8;
+        split = (int)(unit - (uint32_t)tile * p.splits);
+        tn = at / rows;
+        m0 = (band * 8 + at - tn * rows) * BM;
     }
     const int n0 = tn * (UP ? UP_COLUMNS : BN), KB = p.KB;
     // blocks of K: of this split, and of this group (an odd one out is the first group's; the other walks as far, over zeros of x)

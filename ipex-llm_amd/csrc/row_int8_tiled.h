@@ -28,14 +28,14 @@ struct Int8Plan {
 };
 
 // One launch per form; the wave tiles are 64 x 128, 96 x 64, 64 x 64, 64 x 64, 32 x 64, 32 x 32 and 32 x 32.
-template <typename OT, Int8Mode MODE, bool BY_EXPERT = false> void launch_int8_form(const Int8Args &p, int form, hipStream_t st) {
-    if (form == INT8_256) launch_int8_tile<OT, MODE, BY_EXPERT, false, 4, 8, 4, 2, 2, 2>(p, st);
-    else if (form == INT8_192_256) launch_int8_tile<OT, MODE, BY_EXPERT, false, 6, 4, 2, 4, 2, 2>(p, st);
-    else if (form == INT8_128_256) launch_int8_tile<OT, MODE, BY_EXPERT, false, 4, 4, 2, 4, 3, 2>(p, st);
-    else if (form == INT8_128) launch_int8_tile<OT, MODE, BY_EXPERT, false, 4, 4, 2, 2, 2, 2>(p, st);
-    else if (form == INT8_64) launch_int8_tile<OT, MODE, BY_EXPERT, false, 2, 4, 2, 2, 3, 2>(p, st);
-    else if (form == INT8_32) launch_int8_tile<OT, MODE, BY_EXPERT, false, 2, 2, 1, 4, 3, 2>(p, st);
-    else if constexpr (!BY_EXPERT) launch_int8_tile<OT, MODE, BY_EXPERT, false, 2, 2, 2, 2, 3, 2, 2>(p, st);
+template <typename OT, Int8Mode MODE> void launch_int8_form(const Int8Args &p, int form, hipStream_t st) {
+    if (form == INT8_256) launch_int8_tile<OT, MODE, false, false, 4, 8, 4, 2, 2, 2>(p, st);
+    else if (form == INT8_192_256) launch_int8_tile<OT, MODE, false, false, 6, 4, 2, 4, 2, 2>(p, st);
+    else if (form == INT8_128_256) launch_int8_tile<OT, MODE, false, false, 4, 4, 2, 4, 3, 2>(p, st);
+    else if (form == INT8_128) launch_int8_tile<OT, MODE, false, false, 4, 4, 2, 2, 2, 2>(p, st);
+    else if (form == INT8_64) launch_int8_tile<OT, MODE, false, false, 2, 4, 2, 2, 3, 2>(p, st);
+    else if (form == INT8_32) launch_int8_tile<OT, MODE, false, false, 2, 2, 1, 4, 3, 2>(p, st);
+    else launch_int8_tile<OT, MODE, false, false, 2, 2, 2, 2, 3, 2, 2>(p, st);
 }
 
 void launch_int8_f16(const Int8Args &p, int form, hipStream_t st);
