@@ -8,6 +8,9 @@
 // lane (row l & 15, k = l >> 4): a lane loads eight neighbours of its row, k = 8 (l >> 4) .. + 7 of 32, and eight instructions take one of
 // them each, since the order of the terms is free as long as both operands agree.
 //
+// (Two waves per SIMD are asked for so that the sums stay in vector registers: left alone the compiler keeps them in accumulation registers and copies
+// them back and forth in every turn of the loops below.)
+//
 // The first launch sums a part of H for 16 tokens by 16 TN experts per workgroup, the second one, a wave per token, adds the parts and chooses.
 #include "row_int8.h"
 
@@ -29,7 +32,7 @@ template <typename AT> struct Octet {
 };
 
 template <typename AT, typename RT, int TN, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void route_logits_kernel(const RouteArgs p) {
+__global__ __launch_bounds__(64 * WAVES, 2) void route_logits_kernel(const RouteArgs p) {
     using X8 = typename Octet<AT>::type;
     using R8 = typename Octet<RT>::type;
     __shared__ double sums[WAVES - 1][64][TN * 4 + 1];
@@ -90,14 +93,19 @@ __global__ __launch_bounds__(64 * WAVES) void route_logits_kernel(const RouteArg
 
 // ---- a wave's doubles
 
-__device__ inline double wave_sum(double v) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
-    return v;
+template <int CTRL, int ROWS> __device__ inline double add_dpp(double v) {
+    const u32x2 b = __builtin_bit_cast(u32x2, v);
+    return v + __builtin_bit_cast(double, u32x2{(uint32_t)__builtin_amdgcn_update_dpp(0, (int)b[0], CTRL, ROWS, 0xf, false),
+                                                (uint32_t)__builtin_amdgcn_update_dpp(0, (int)b[1], CTRL, ROWS, 0xf, false)});
 }
 __device__ inline double from_lane(double v, int l) {
     const u32x2 b = __builtin_bit_cast(u32x2, v);
     return __builtin_bit_cast(double, u32x2{(uint32_t)__builtin_amdgcn_readlane((int)b[0], l), (uint32_t)__builtin_amdgcn_readlane((int)b[1], l)});
+}
+// the same in every lane: rows of 16, then the rows (max_of_wave)
+__device__ inline double wave_sum(double v) {
+    v = add_dpp<0x140, 0xf>(add_dpp<0x141, 0xf>(add_dpp<0x4E, 0xf>(add_dpp<0xB1, 0xf>(v))));
+    return from_lane(add_dpp<0x143, 0xc>(add_dpp<0x142, 0xa>(v)), 63);
 }
 // Whole numbers in the order of the doubles: a NaN above all, the zeros alike, nothing at 0.
 __device__ inline uint64_t ordered(double v) {
@@ -171,14 +179,17 @@ template <int NR> __global__ __launch_bounds__(256) void route_select_kernel(con
             if (p.z) p.z[t * p.E + e] = z[i];
         }
     }
-    const double sum = scores<NR>(z, s, p.E, p.sigmoid, lane);
+    // (the scores of all only where the choice or the weights go by them)
+    const bool of_chosen = p.renormalize && !p.bias;
+    double sum = 1.0;
+    if (!of_chosen) sum = scores<NR>(z, s, p.E, p.sigmoid, lane);
     uint64_t key[NR];
 #pragma unroll
     for (int i = 0; i < NR; i++) {
         const int e = lane + 64 * i;
         key[i] = e < p.E ? ordered(p.bias ? s[i] / sum + (double)p.bias[e] : z[i]) : 0;
     }
-    double chosen = 0.0, total = 0.0;                        // lane j: the score of choice j
+    double chosen = 0.0, total = 0.0;                        // lane j: the score of choice j (of_chosen: z)
     int index = 0;
     for (int j = 0; j < p.top_k; j++) {
         uint64_t best = 0;
@@ -188,7 +199,7 @@ template <int NR> __global__ __launch_bounds__(256) void route_select_kernel(con
         for (int i = 0; i < NR; i++)
             if (key[i] > best) {
                 best = key[i];
-                score = s[i];
+                score = of_chosen ? z[i] : s[i];
                 at = i;
             }
         const uint64_t most = wave_max(best);
@@ -203,6 +214,10 @@ template <int NR> __global__ __launch_bounds__(256) void route_select_kernel(con
 #pragma unroll
         for (int i = 0; i < NR; i++)
             if (lane + 64 * i == (int)e) key[i] = 0;
+    }
+    if (of_chosen) {                                         // (z of the first choice is the largest)
+        chosen = p.sigmoid ? 1.0 / (1.0 + exp(-chosen)) : exp(chosen - from_lane(chosen, 0));
+        total = wave_sum(lane < p.top_k ? chosen : 0.0);
     }
     if (lane < p.top_k) {
         p.w[t * p.top_k + lane] = (float)((double)p.factor * (chosen / (p.renormalize ? total : sum)));
@@ -270,7 +285,7 @@ struct OuterArgs {
 };
 
 template <typename BT, typename CT, int TM, bool ACROSS>
-__global__ __launch_bounds__(256) void route_outer_kernel(const OuterArgs p) {
+__global__ __launch_bounds__(256, 2) void route_outer_kernel(const OuterArgs p) {
     using B8 = typename Octet<BT>::type;
     __shared__ float sums[ACROSS ? 64 * (TM * 32 + 1) : 1];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;

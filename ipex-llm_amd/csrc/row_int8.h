@@ -79,11 +79,12 @@ template <int V> __device__ inline uint32_t largest_of(const float (&v)[V]) {
     for (int i = 0; i < V; i++) m = max_u32(m, magnitude(v[i]));
     return m;
 }
-// .. over the wave, the same in every lane
+// .. over the wave, the same in every lane: of rows of 16, handed on to the second and fourth, then to the last two
 __device__ inline uint32_t max_of_wave(uint32_t v) {
     v = max_of_16(v);
-    v = max_u32(v, (uint32_t)__builtin_amdgcn_ds_swizzle((int)v, 0x401f));       // lanes l ^ 16
-    return max_u32((uint32_t)__builtin_amdgcn_readlane((int)v, 0), (uint32_t)__builtin_amdgcn_readlane((int)v, 32));
+    v = max_u32(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false));
+    v = max_u32(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false));
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
 // One row of K values by the threads t of WAVES waves, 16 values per thread and piece; what lies past the first HELD pieces is read again behind

@@ -34,10 +34,11 @@ __device__ inline Codes load_block(const uint8_t *row, int kb, int g, int K) {
 constexpr size_t TOKEN_LDS = 65536 - 4096;                   // codes of a row of x, or of h of all pairs of a token
 
 // One pair's 16 columns of h per workgroup: 16 rows of the gate and 16 of u.  The blocks of K are dealt to the waves, STEPS of them in flight
-// per wave, whose sums meet in LDS.  x is quantized by each workgroup.
-template <typename AT>
-__global__ __launch_bounds__(512) void row_int8_expert_token_up_kernel(const Int8Experts p) {
-    constexpr int STEPS = 2, WAVES = 8, THREADS = 64 * WAVES, HELD = 2;
+// per wave, whose sums meet in LDS.  x is quantized by each workgroup.  Bound by memory: two experts of [14336 x 4096] 46.8 us, 5.0 TB/s (two steps in
+// flight 51.5); rows of up to 2048 in four waves of two steps, one of [7168 x 512] 10.4 us against 16.2 in eight.
+template <typename AT, int WAVES, int STEPS>
+__global__ __launch_bounds__(64 * WAVES, 2) void row_int8_expert_token_up_kernel(const Int8Experts p) {
+    constexpr int THREADS = 64 * WAVES, HELD = 2;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     __shared__ int32_t sums[WAVES][2][16];
     __shared__ uint32_t part[WAVES];
@@ -130,7 +131,8 @@ __global__ __launch_bounds__(512) void row_int8_expert_token_up_kernel(const Int
 }
 
 // One token's 16 columns per workgroup, which quantizes h of all its pairs; their blocks are dealt to the waves, STEPS of them in flight per
-// wave.  A wave's blocks of one pair are summed in whole numbers, then scaled into the sum over the pairs.
+// wave.  A wave's blocks of one pair are summed in whole numbers, then scaled into the sum over the pairs.  Two experts of [4096 x 14336] 28 us, 4.2
+// TB/s: ahead of the first product 115 KB of h come from L2 and become codes; six or eight steps in flight make no difference.
 template <typename AT, typename PT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void row_int8_expert_down_token_kernel(const Int8Experts p, const PT *__restrict__ weight, AT *__restrict__ out) {
     constexpr int STEPS = 4, HELD = 4, THREADS = 64 * WAVES;
@@ -255,17 +257,19 @@ __global__ __launch_bounds__(256) void row_int8_expert_rows_kernel(const AT *__r
     if (threadIdx.x == 0) scale[row] = s;
 }
 
-// Few pairs: each streams its expert's weights, which costs as many reads as there are pairs; the codes of a row of x and those of a token's
-// rows of h have to fit LDS.  Sorted by expert a weight is read once, by launches that take some 10 us more and leave a quarter of a round
-// of the first product's tiles idle.  The estimate counts the experts that tokens routed evenly would meet, at 5.5 TB/s.
+// Pair by pair or sorted, by estimated time in us, fitted to 110 sizes of 1 to 48 tokens; the pick is 0.3 % above the shorter way on average, 12 % at
+// worst.  Pair by pair: the reads, as many as there are pairs; workgroups of the first launch; of the second, and the codes of h that each of its
+// rounds makes.  Sorted: a weight is read once, of the experts that tokens routed evenly would meet.  The codes of a row of x and those of a
+// token's rows of h have to fit LDS.  2 tokens through 2 of 8 of [14336 x 4096] 150 us pair by pair, 110 sorted, 4 through 6 of 64 of [1408 x 2048]
+// 43 / 53, 8 81 / 79, 12 through 2 of 4 of [512 x 1024] 16 / 21.
 static size_t token_up_lds(int H) { return (size_t)int8_blocks(H) * INT8_BLOCK; }
 static size_t token_down_lds(int top_k, int I) { return (size_t)top_k * int8_blocks(I) * INT8_BLOCK; }
 static bool direct(int tokens, int top_k, int n_exp, int H, int I) {
-    if (token_up_lds(H) > TOKEN_LDS || token_down_lds(top_k, I) > TOKEN_LDS) return false;
-    if (tokens == 1) return true;
-    if ((int64_t)tokens * top_k > n_exp) return false;
-    const double expert_us = 3.0 * H * I / 5.5e6, met = n_exp * (1.0 - pow(1.0 - (double)top_k / n_exp, tokens));
-    return (tokens * top_k - met) * expert_us <= 10.0 + 64.0 * 2 * INT8_BLOCK * H / 5.5e6;
+    if (token_up_lds(H) > TOKEN_LDS || token_down_lds(top_k, I) > TOKEN_LDS || (int64_t)tokens * top_k > 4096) return false;
+    const double pairs = (double)tokens * top_k, expert = 3.0e-6 * H * I, met = n_exp * (1.0 - pow(1.0 - (double)top_k / n_exp, tokens));
+    const double rounds = tokens * (double)H / (16 * 256);
+    const double each = 6.6 + 0.08 * pairs * expert + 2.5 * pairs * I / (16 * 512) + 0.114 * rounds + 0.117 * top_k * int8_blocks(I) * fmax(1.0, rounds);
+    return each <= 20.1 + 0.1815 * met * expert + 0.0006 * pairs;
 }
 
 // The forms of the two products, by estimated time, with the row tiles that tokens routed evenly would make: of m rows for an expert, with a deviation
@@ -426,7 +430,9 @@ template <typename AT> static int launch_sorted(Int8Experts p, const ExpertsSpac
 template <typename AT> static int launch_experts_t(Int8Experts p, const ExpertsSpace &at, uint8_t *ws, const void *weight, int w_dtype, void *out,
                                                    int act_dtype, int tokens, hipStream_t st) {
     if (direct(tokens, p.top_k, p.n_exp, p.H, p.I)) {
-        hipLaunchKernelGGL((row_int8_expert_token_up_kernel<AT>), dim3(p.I / 16, tokens * p.top_k), dim3(512), token_up_lds(p.H), st, p);
+        const dim3 grid(p.I / 16, tokens * p.top_k);
+        if (int8_blocks(p.H) <= 16) hipLaunchKernelGGL((row_int8_expert_token_up_kernel<AT, 4, 2>), grid, dim3(256), token_up_lds(p.H), st, p);
+        else hipLaunchKernelGGL((row_int8_expert_token_up_kernel<AT, 8, 4>), grid, dim3(512), token_up_lds(p.H), st, p);
         if (w_dtype == DT_F32) launch_down_token(p, (const float *)weight, (AT *)out, tokens, st);
         else if (w_dtype == DT_F16) launch_down_token(p, (const _Float16 *)weight, (AT *)out, tokens, st);
         else launch_down_token(p, (const __bf16 *)weight, (AT *)out, tokens, st);

@@ -28,7 +28,7 @@ template <typename V8> __device__ inline void widen_to(const V8 &v, float (&f)[8
 }
 
 template <typename AT, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void row_int8_few_rows_kernel(const Int8Rows p) {
+__global__ __launch_bounds__(64 * WAVES, 2) void row_int8_few_rows_kernel(const Int8Rows p) {
     constexpr int STEPS = 4;                                 // blocks in flight per wave
     constexpr int HELD = sizeof(AT) == 4 ? 2 : 4;            // pieces of x per thread that are asked for ahead of the weights
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];

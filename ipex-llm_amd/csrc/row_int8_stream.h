@@ -13,7 +13,7 @@ constexpr int STREAM_ROWS = 32;
 
 // PART: the sums of split blockIdx.y's blocks of K.
 template <typename OT, bool PART, int MT, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void row_int8_stream_kernel(const Int8Args p) {
+__global__ __launch_bounds__(64 * WAVES, 2) void row_int8_stream_kernel(const Int8Args p) {
     constexpr int DEPTH = 4;
     __shared__ int32_t sums[WAVES][MT][64 * 4];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
