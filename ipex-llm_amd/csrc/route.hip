@@ -387,15 +387,18 @@ template <typename F> static void by_type(int dtype, F &&f) {
     else f((float *)nullptr);
 }
 
-// Columns of 16 experts per workgroup, and parts of H so that a few hundred workgroups run; a part has a chunk for each of the four waves at least.
+// Columns of 16 experts per workgroup, and parts of H so that about a thousand workgroups run, four per CU; a part has a chunk for each of the four
+// waves at least.  Two columns share a token's conversions and are taken once there are tokens enough: 500 tokens x 64 experts of 2048 take 5.7 us with
+// one in 8 parts and 5.8 with two, 1000 x 60 of 4096 14.0 and 13.6, 4096 x 64 of 2048 24.1 and 23.4; with four columns they take 6.6, 14.8 and 24.8,
+// and with 32 tokens by two columns 6.3, 15.4 and 26.3.  300 x 256 of 7168 takes 49 us in 512 workgroups and 32 in 1024.
 struct RoutePlan {
     int tn, splits, chunks;
 };
 static RoutePlan route_plan(int T, int E, int H) {
     RoutePlan p;
-    p.tn = E > 32 && T > 256 ? 4 : E > 16 && T > 64 ? 2 : 1;
+    p.tn = E > 16 && T > 500 ? 2 : 1;
     const int tiles = cdiv(T, 16) * cdiv(E, 16 * p.tn), all = cdiv(H, 32);
-    int splits = tiles < 512 ? 512 / tiles : 1;
+    int splits = tiles < 1024 ? cdiv(1024, tiles) : 1;
     splits = splits > 16 ? 16 : splits;
     if (splits > all / 4) splits = all / 4 > 0 ? all / 4 : 1;
     p.chunks = cdiv(all, splits);
@@ -428,8 +431,7 @@ int launch_route(const void *x, int x_dtype, const void *router, int r_dtype, co
         by_type(r_dtype, [&](auto *rt) {
             using AT = typename std::remove_pointer<decltype(xt)>::type;
             using RT = typename std::remove_pointer<decltype(rt)>::type;
-            if (plan.tn == 4) hipLaunchKernelGGL((route_logits_kernel<AT, RT, 4, 4>), grid, dim3(256), 0, st, a);
-            else if (plan.tn == 2) hipLaunchKernelGGL((route_logits_kernel<AT, RT, 2, 4>), grid, dim3(256), 0, st, a);
+            if (plan.tn == 2) hipLaunchKernelGGL((route_logits_kernel<AT, RT, 2, 4>), grid, dim3(256), 0, st, a);
             else hipLaunchKernelGGL((route_logits_kernel<AT, RT, 1, 4>), grid, dim3(256), 0, st, a);
         });
     });
