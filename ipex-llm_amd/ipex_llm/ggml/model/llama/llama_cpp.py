@@ -565,7 +565,7 @@ def lowbit_row_int8_plan(dtype, backward, m, n, k):
 
 
 def lowbit_row_int8_waves(m, n, k):
-    """Waves of a workgroup of the kernel of few rows, 0 where lowbit_row_int8_linear runs tiles."""
+    """Waves of a workgroup of the kernel of few rows or of the streaming one, 0 where lowbit_row_int8_linear runs tiles."""
     waves = _lib.lowbit_row_int8_waves(m, n, k)
     _check(min(waves, 0), "lowbit_row_int8_waves")
     return waves

@@ -96,6 +96,14 @@ def block_fp8_layers(state_dict):
     return names, any(n.endswith("q_proj") for n in names)
 
 
+def row_int8_layers(state_dict, low_bit):
+    """Module names whose saved weights are int8 codes with a scale for each row (a model saved as sym_int8)."""
+    if low_bit != "sym_int8":
+        return set()
+    return {k[:-len("." + w)] for w in ("weight", "gate_up_proj") for k, v in state_dict.items()
+            if k.endswith("." + w) and v.dtype == torch.int8 and k + "_scale" in state_dict}
+
+
 def unmerged_attentions(state_dict):
     """Names of the modules whose q_proj was saved by itself, not as part of a qkv_proj."""
     return {k.rpartition("q_proj.")[0].rstrip(".") for k in state_dict if ".q_proj." in "." + k}
@@ -111,9 +119,10 @@ def load_low_bit(model, model_path):
     if low_bit:
         from ipex_llm.transformers.convert import ggml_convert_low_bit
         qtype = ggml_tensor_qtype[low_bit]
+        rows = row_int8_layers(state_dict, low_bit)
         model = ggml_convert_low_bit(model, qtype=qtype, convert_shape_only=True,
-                                     modules_to_not_convert=unconverted_linears(state_dict),
-                                     keep_apart=unmerged_attentions(state_dict), block_fp8=block_fp8_layers(state_dict)[0])
+                                     modules_to_not_convert=[n for n in unconverted_linears(state_dict) if n not in rows],
+                                     keep_apart=unmerged_attentions(state_dict), block_fp8=block_fp8_layers(state_dict)[0], row_int8=rows)
     for param_name, param in state_dict.items():
         _assign(model, param_name, param)
     if low_bit:
@@ -126,7 +135,8 @@ def optimize_model(model, low_bit='sym_int4', optimize_llm=True, modules_to_not_
                    cpu_embedding=False, **kwargs):
     """Replaces every nn.Linear of a PyTorch model by its low-bit counterpart
     (reference: optimize.py:199-267; same arguments).  `block_fp8=True` with low_bit="fp8_e4m3": weights with a scale for each
-    128 x 128 block and activations quantized in the call (transformers/block_fp8.py)."""
+    128 x 128 block and activations quantized in the call (transformers/block_fp8.py).  `row_int8=True` with low_bit="sym_int8": int8 weights
+    with a scale for each row and activations quantized by row in the call (transformers/row_int8.py)."""
     invalidInputError(low_bit is None or low_bit in ggml_tensor_qtype,
                       f"Unknown load_in_low_bit value: {low_bit}, expected:"
                       f" sym_int4, asym_int4, sym_int5, asym_int5 or sym_int8.")
@@ -152,7 +162,8 @@ def optimize_model(model, low_bit='sym_int4', optimize_llm=True, modules_to_not_
                                  modules_to_not_convert=modules_to_not_convert,
                                  cpu_embedding=cpu_embedding,
                                  disable_optimize_pre=kwargs.pop("disable_optimize_pre", False),
-                                 block_fp8=kwargs.pop("block_fp8", False))
+                                 block_fp8=kwargs.pop("block_fp8", False),
+                                 row_int8=kwargs.pop("row_int8", False))
     model._bigdl_config = dict()
     model._bigdl_config["bigdl_transformers_low_bit"] = low_bit
     model.save_low_bit = types.MethodType(_save_low_bit, model)

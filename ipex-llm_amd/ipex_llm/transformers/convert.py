@@ -70,6 +70,32 @@ def check_block_fp8(module, full_name, names):
     invalidInputError(not more, f"{why} with weight, scales and bias; it holds {more} beside them (modules_to_not_convert leaves it out)")
 
 
+def is_row_int8(module, name="weight") -> bool:
+    """A layer (or, with the name of its 3-D parameter, an experts module) of a checkpoint in row-scaled int8: codes and a tensor of scales
+    beside them."""
+    w = getattr(module, name, None)
+    return isinstance(w, torch.Tensor) and w.dtype == torch.int8 and isinstance(getattr(module, name + "_scale", None), torch.Tensor)
+
+
+def check_row_int8(module, full_name, names):
+    """Refuses a layer of such a checkpoint (`names`: its weights that is_row_int8 knows) that computes something else than the product of
+    row_int8.py: scales of another shape, a fixed scale of the activations, zero points, groups of columns, tensors of its own."""
+    why = f"{full_name}: a layer in row-scaled int8 converts"
+    for n in names:
+        w, scale = getattr(module, n), getattr(module, n + "_scale")
+        invalidInputError(tuple(scale.shape) in (tuple(w.shape[:-1]), (*w.shape[:-1], 1)) and scale.is_floating_point(),
+                          f"{why} with a scale for each row, not {n}_scale {tuple(scale.shape)} for {tuple(w.shape)}")
+    groups = getattr(module, "n_groups", 1)
+    invalidInputError(getattr(module, "activation_scheme", "dynamic") == "dynamic",
+                      f"{why} with activation_scheme='dynamic': activations are quantized by their own rows")
+    invalidInputError(groups == 1, f"{why} where all of x meets all of the weight, not in {groups} groups")
+    own = {"bias"}.union(names, (n + "_scale" for n in names))
+    if "weight" not in names:
+        own |= {"gate_up_proj", "down_proj"}
+    more = [n for n, t in [*module._parameters.items(), *module._buffers.items()] if t is not None and n not in own]
+    invalidInputError(not more, f"{why} with weight, scales and bias; it holds {more} beside them (modules_to_not_convert leaves it out)")
+
+
 def is_linear_module(module):
     """(is_linear, (in_features, out_features, mp_group)): nn.Linear and 4-bit GPTQ / AWQ layers; the
     vLLM / DeepSpeed layer classes of the reference (convert.py:138-232) are not handled."""
@@ -168,29 +194,37 @@ def _replace_with_low_bit_linear(model, qtype, modules_to_not_convert=None,
                                  act_order=False,
                                  enable_scale_search=False,
                                  block_fp8=False,
+                                 row_int8=False,
                                  ):
     """block_fp8: which layers (True: all; or a set of their full names) get e4m3 weights with a scale for each 128 x 128 and
-    activations quantized in the call (block_fp8.py) in place of qtype's format."""
+    activations quantized in the call (block_fp8.py) in place of qtype's format; row_int8: which get int8 weights with a scale for each row
+    and activations quantized by row (row_int8.py)."""
     from ipex_llm.transformers.block_fp8 import BlockFP8Experts, BlockFP8Linear
     from ipex_llm.transformers.low_bit_linear import BF16Linear, FP16Linear, FP4Params, LowBitLinear
+    from ipex_llm.transformers.row_int8 import MOST_K, RowInt8Experts, RowInt8Linear
     modules_to_not_convert = modules_to_not_convert or []
     has_been_replaced = False
     only_fp8 = "layers with a scale for each 128 x 128 block hold e4m3: convert with load_in_low_bit='fp8_e4m3'"
+    only_int8 = "layers with int8 codes and a scale for each row: convert with load_in_low_bit='sym_int8'"
 
     for name, module in model.named_children():
         is_linear, linear_args = is_linear_module(module)
         full_module_name = prefix_name + '.' + name if prefix_name != '' else name
         wants_blocks = block_fp8 is True or (block_fp8 and full_module_name in block_fp8)
+        wants_rows = row_int8 is True or (row_int8 and full_module_name in row_int8)
 
         # sub-string match, as in the reference: "0" also matches "10"
         if any(key in full_module_name for key in modules_to_not_convert):
             continue
 
-        if isinstance(module, (BlockFP8Linear, BlockFP8Experts)):
+        if isinstance(module, (BlockFP8Linear, BlockFP8Experts, RowInt8Linear, RowInt8Experts)):
             continue
         scaled = [n for n in ("weight", "gate_up_proj", "down_proj") if is_block_fp8(module, n)]
+        rows = [n for n in ("weight", "gate_up_proj", "down_proj") if is_row_int8(module, n)]
         if isinstance(module, nn.Linear) or is_fused_experts(module):
             check_block_fp8(module, full_module_name, scaled)
+            if rows:
+                check_row_int8(module, full_module_name, rows)
 
         if isinstance(module, nn.Linear) and getattr(module, "n_groups", 1) != 1:
             continue   # a linear in groups, each of which meets its own columns of x, stays as it is
@@ -205,6 +239,12 @@ def _replace_with_low_bit_linear(model, qtype, modules_to_not_convert=None,
                     invalidInputError(not is_block_fp8(module), f"{full_module_name}: in_features must be a multiple of 16")
                     continue
                 new_linear = BlockFP8Linear.from_linear(module, convert_shape_only, mp_group, optimize_lm_head)
+            elif rows or (wants_rows and not is_gptq_linear(module)):
+                invalidInputError(qtype == ggml_tensor_qtype["sym_int8"], only_int8)
+                if in_features % 16 != 0 or in_features > MOST_K:
+                    invalidInputError(not rows, f"{full_module_name}: in_features must be a multiple of 16, at most {MOST_K}")
+                    continue
+                new_linear = RowInt8Linear.from_linear(module, convert_shape_only, mp_group, optimize_lm_head)
             elif is_gptq_linear(module):
                 # convert.py:511-545 of the reference: the codes are kept, only the packing changes
                 invalidInputError(qtype == ggml_tensor_qtype["asym_int4"],
@@ -282,15 +322,20 @@ def _replace_with_low_bit_linear(model, qtype, modules_to_not_convert=None,
             from ipex_llm.transformers.low_bit_linear import get_qk_size
             from ipex_llm.transformers.moe import LowBitExperts, gate_of
             _, two_i, hidden = module.gate_up_proj.shape
-            if not scaled and (not gate_of(module)[0] or any(getattr(module, n + "_bias", None) is not None for n in ("gate_up_proj", "down_proj"))):
+            if not scaled and not rows and (not gate_of(module)[0] or any(getattr(module, n + "_bias", None) is not None for n in ("gate_up_proj", "down_proj"))):
                 continue                                 # a gate that cannot be taken over, biases: the module stays dense
             if scaled or (wants_blocks and hidden % 16 == 0 and two_i % 256 == 0):
                 invalidInputError(qtype == ggml_tensor_qtype["fp8_e4m3"], only_fp8)
                 model._modules[name] = BlockFP8Experts.from_fused(module, convert_shape_only).requires_grad_(False)
                 has_been_replaced = True
                 continue
-            if wants_blocks:
-                continue                                 # sizes that do not divide into blocks stay dense
+            if rows or (wants_rows and hidden % 16 == 0 and two_i % 32 == 0 and max(hidden, two_i // 2) <= MOST_K):
+                invalidInputError(qtype == ggml_tensor_qtype["sym_int8"], only_int8)
+                model._modules[name] = RowInt8Experts.from_fused(module, convert_shape_only).requires_grad_(False)
+                has_been_replaced = True
+                continue
+            if wants_blocks or wants_rows:
+                continue                                 # sizes that do not fit the format stay dense
             qk = get_qk_size(qtype)
             if hidden % 64 == 0 and (two_i // 2) % 64 == 0 and (not qk or (hidden % qk == 0 and (two_i // 2) % qk == 0)):
                 model._modules[name] = LowBitExperts.from_fused(module, qtype, convert_shape_only=convert_shape_only,
@@ -311,7 +356,7 @@ def _replace_with_low_bit_linear(model, qtype, modules_to_not_convert=None,
                 prefix_name=full_module_name, imatrix_data=imatrix_data,
                 embedding_qtype=embedding_qtype, model_config=model_config, torch_dtype=torch_dtype,
                 mixed_precision=mixed_precision, act_order=act_order,
-                enable_scale_search=enable_scale_search, block_fp8=block_fp8)
+                enable_scale_search=enable_scale_search, block_fp8=block_fp8, row_int8=row_int8)
             has_been_replaced = _flag or has_been_replaced
     return model, has_been_replaced
 
@@ -386,9 +431,12 @@ def ggml_convert_low_bit(model, qtype, optimize_model=True,
                          mixed_precision=False,
                          disable_optimize_pre=False,
                          block_fp8=False,
-                         keep_apart=()):
+                         keep_apart=(),
+                         row_int8=False):
     invalidInputError(not block_fp8 or qtype == ggml_tensor_qtype["fp8_e4m3"],
                       "block_fp8 makes e4m3 weights: use it with fp8_e4m3")
+    invalidInputError(not row_int8 or qtype == ggml_tensor_qtype["sym_int8"],
+                      "row_int8 makes int8 weights: use it with sym_int8")
     if qtype in ggml_tensor_qtype.values():
         index = list(ggml_tensor_qtype.values()).index(qtype)
         logger.info(f"Converting the current model to {list(ggml_tensor_qtype.keys())[index]} format......")
@@ -407,7 +455,7 @@ def ggml_convert_low_bit(model, qtype, optimize_model=True,
             model, qtype, modules_to_not_convert, convert_shape_only, cpu_embedding,
             imatrix_data=imatrix_data, embedding_qtype=embedding_qtype, model_config=model_config,
             torch_dtype=torch_dtype, mixed_precision=mixed_precision, act_order=False,
-            enable_scale_search=enable_scale_search, block_fp8=block_fp8)
+            enable_scale_search=enable_scale_search, block_fp8=block_fp8, row_int8=row_int8)
         if not has_been_replaced:
             warnings.warn("No linear modules were found in your model. This can happen for some "
                           "architectures such as gpt2 that uses Conv1D instead of Linear layers.")
@@ -424,10 +472,11 @@ def convert_bigdl_other_module(model, dtype):
     of a checkpoint that was left out of the conversion, keeps them: as numbers of another type they would have lost their scales."""
     from ipex_llm.transformers.block_fp8 import BlockFP8Linear
     from ipex_llm.transformers.low_bit_linear import BF16Linear, FP16Linear, LowBitLinear
+    from ipex_llm.transformers.row_int8 import RowInt8Linear
     for module in model.modules():
         if list(module.children()) == []:
             codes = any(p.is_floating_point() and p.element_size() == 1 for p in module.parameters(recurse=False))
-            if not codes and not isinstance(module, (LowBitLinear, FP16Linear, BF16Linear, BlockFP8Linear)):
+            if not codes and not isinstance(module, (LowBitLinear, FP16Linear, BF16Linear, BlockFP8Linear, RowInt8Linear)):
                 module.to(dtype)
 
 

@@ -62,7 +62,8 @@ class _BaseAutoModelClass:
     def from_pretrained(cls, *args, **kwargs):
         """Hugging Face from_pretrained plus load_in_4bit / load_in_low_bit / optimize_model /
         modules_to_not_convert (reference: transformers/model.py:111-388), and block_fp8 (with "fp8_e4m3": weights with a
-        scale for each 128 x 128 block, activations quantized in the call)."""
+        scale for each 128 x 128 block, activations quantized in the call) or row_int8 (with "sym_int8": int8 weights with a
+        scale for each row, activations quantized by row)."""
         from transformers import PretrainedConfig
         pretrained_model_name_or_path = kwargs.get("pretrained_model_name_or_path", None) \
             if len(args) == 0 else args[0]
@@ -131,6 +132,7 @@ class _BaseAutoModelClass:
         disable_optimize_pre = kwargs.pop("disable_optimize_pre", False)
         embedding_qtype = kwargs.pop("embedding_qtype", None)
         block_fp8 = kwargs.pop("block_fp8", False)
+        row_int8 = kwargs.pop("row_int8", False)
         if embedding_qtype is not None:
             # the reference documents 'q2_k' / 'q4_k' here (model.py:148); any qtype with a kernel works
             invalidInputError(embedding_qtype in ("sym_int4", "asym_int4", "sym_int8", "nf4", "fp8_e4m3"),
@@ -156,7 +158,7 @@ class _BaseAutoModelClass:
                                      embedding_qtype=embedding_qtype,
                                      mixed_precision=mixed_precision,
                                      disable_optimize_pre=disable_optimize_pre,
-                                     block_fp8=block_fp8)
+                                     block_fp8=block_fp8, row_int8=row_int8)
         _release_quantizer(model)
         model.config.update({"bigdl_transformers_low_bit": q_k, "bigdl_disk_embedding": False})
         model.config.update({"tie_word_embeddings": False})
@@ -184,16 +186,17 @@ class _BaseAutoModelClass:
                           " serialize the model using save_low_bit first.")
         invalidInputError(low_bit in ggml_tensor_qtype, f"Unknown bigdl_transformers_low_bit value: {low_bit}")
         qtype = ggml_tensor_qtype[low_bit]
-        from ipex_llm.optimize import block_fp8_layers, unconverted_linears, unmerged_attentions
+        from ipex_llm.optimize import block_fp8_layers, row_int8_layers, unconverted_linears, unmerged_attentions
         state_dict = torch.load(os.path.join(pretrained_model_name_or_path, PYTORCH_MODEL_NAME),
                                 weights_only=True)
         with torch.device("meta"):
             model = cls.HF_Model.from_config(config)
-        skip = list(modules_to_not_convert or []) + unconverted_linears(state_dict)
+        rows = row_int8_layers(state_dict, low_bit)
+        skip = list(modules_to_not_convert or []) + [n for n in unconverted_linears(state_dict) if n not in rows]
         model = ggml_convert_low_bit(model, qtype, optimize_model, device="meta",
                                      convert_shape_only=True, modules_to_not_convert=skip,
                                      embedding_qtype=embedding_qtype, keep_apart=unmerged_attentions(state_dict),
-                                     block_fp8=block_fp8_layers(state_dict)[0])
+                                     block_fp8=block_fp8_layers(state_dict)[0], row_int8=rows)
         keys_file = os.path.join(pretrained_model_name_or_path, "load_keys.json")
         if os.path.isfile(keys_file):
             with open(keys_file) as f:

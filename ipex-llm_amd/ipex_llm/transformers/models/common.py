@@ -11,8 +11,10 @@ from ipex_llm.transformers.native_ops import ops
 
 def merge_linear(linears: List[torch.nn.Linear]) -> torch.nn.Linear:
     """One linear whose weight (and bias) is the row-wise concatenation of `linears`
-    (reference: models/common.py:22-37).  GPTQ layers (no `weight`) give None, and so do block-scaled ones, whose
-    scales would have to be merged too."""
+    (reference: models/common.py:22-37).  GPTQ layers (no `weight`) give None, and so do those of a checkpoint in
+    block-scaled fp8 or row-scaled int8, whose scales would have to be merged too."""
+    if any(getattr(lin, "weight", None) is not None and lin.weight.dtype == torch.int8 and hasattr(lin, "weight_scale") for lin in linears):
+        return None
     if not all(isinstance(lin, torch.nn.Linear) and hasattr(lin, "weight") and not hasattr(lin, "weight_scale_inv") for lin in linears):
         return None
     new_weight = torch.cat([lin.weight.data for lin in linears], dim=0)

@@ -11,8 +11,10 @@ Weights are frozen, as in LowBitLinear.  The gradient flows on to the activation
 """
 import torch
 import torch.nn.functional as F
+from torch import nn
 
 import ipex_llm.ggml.model.llama.llama_cpp as ggml
+from ipex_llm.transformers.block_fp8 import _frozen, _gated, _KeepsFormat
 from ipex_llm.transformers.native_ops import ops
 from ipex_llm.utils.common import invalidInputError
 
@@ -165,13 +167,6 @@ def _expert_loop(x, top_k_index, top_k_weights, gate_up, gate_up_scale, down, do
     return y.new_zeros((tokens * top_k, x.shape[1])).index_copy(0, order, y).view(tokens, top_k, -1).sum(1).to(x.dtype)
 
 
-def _gated(act_fn):
-    def gate(gu):
-        g, u = gu.chunk(2, dim=-1)
-        return act_fn(g) * u
-    return gate
-
-
 _ACTS = {0: F.silu, 1: lambda g: F.gelu(g, approximate="tanh")}
 
 
@@ -227,3 +222,120 @@ def row_int8_moe(x: torch.Tensor, router: torch.Tensor, top_k: int, gate_up: tor
         return x * 0
     weights, index = moe_route(x, router, top_k, bias, score, renormalize, scale)
     return row_int8_experts(x, index, weights, gate_up, gate_up_scale, down, down_scale, act)
+
+
+def _pack_weight(w, shape_only=False):
+    """Codes and scales of a dense weight on any device; a host weight is quantized on the GPU."""
+    if shape_only or w.device.type == "meta":
+        return torch.empty(w.shape, dtype=torch.int8, device=w.device), torch.empty(w.shape[:-1], dtype=torch.float32, device=w.device)
+    from ipex_llm.transformers.low_bit_linear import _require_gpu, _to_gpu
+    if w.device.type == _ACCEL:
+        return row_int8_quantize(w.detach())
+    _require_gpu("row_int8_quantize")
+    codes, scale = row_int8_quantize(_to_gpu(w.detach().contiguous()))
+    return codes.to(w.device), scale.to(w.device)
+
+
+def _taken(module, name, shape_only):
+    """(codes, scale) of a module's weight: its own where it holds `<name>_scale`, [.., N] or [.., N, 1]; else the dense weight's."""
+    w, scale = getattr(module, name).data, getattr(module, name + "_scale", None)
+    if scale is None:
+        return _pack_weight(w, shape_only)
+    scale = scale.data.to(torch.float32)
+    scale = scale.squeeze(-1) if scale.dim() == w.dim() and scale.shape[-1] == 1 else scale
+    invalidInputError(w.dtype == torch.int8 and scale.shape == w.shape[:-1],
+                      f"row-scaled int8 {name} {tuple(w.shape)} has one scale for each row, not {tuple(scale.shape)}")
+    # (the kernels load sixteen codes at once: a view that starts between two such groups is copied)
+    w = w.contiguous()
+    return (w.clone() if w.device.type != "meta" and w.data_ptr() % 16 else w), scale.contiguous()
+
+
+class RowInt8Linear(_KeepsFormat, nn.Linear):
+    """nn.Linear with an int8 weight and a scale for each of its rows (`weight`, `weight_scale`) and activations quantized by row in the call."""
+
+    _FORMAT = ("weight", "weight_scale")
+
+    def __init__(self, input_features, output_features, bias=True, mp_group=None, optimize_lm_head=False):
+        with torch.device("meta"):
+            super().__init__(input_features, output_features, bias)
+        invalidInputError(input_features % 16 == 0 and input_features <= MOST_K,
+                          f"RowInt8Linear needs in_features to be a multiple of 16, at most {MOST_K}")
+        self.weight = _frozen(torch.empty((output_features, input_features), dtype=torch.int8))
+        self.weight_scale = _frozen(torch.empty(output_features, dtype=torch.float32))
+        if bias:
+            self.bias = _frozen(torch.zeros(output_features))
+        self.in_len, self.out_len = input_features, output_features
+        self.weight_shape = (output_features, input_features)
+        self.mp_group = mp_group
+        self.compute_dtype = None                        # only for training
+        self.optimize_lm_head = optimize_lm_head
+
+    @classmethod
+    def from_linear(cls, linear, convert_shape_only=False, mp_group=None, optimize_lm_head=False):
+        """From an nn.Linear: a dense one is quantized; one that holds `weight_scale` keeps its codes and scales."""
+        w, scale = _taken(linear, "weight", convert_shape_only)
+        with torch.device("meta"):
+            new = cls(w.shape[1], w.shape[0], False, mp_group, optimize_lm_head)
+        new.weight, new.weight_scale = _frozen(w), _frozen(scale)
+        new.bias = None if linear.bias is None else _frozen(linear.bias.data)
+        return new.train(linear.training)
+
+    def forward(self, x: torch.Tensor):
+        invalidInputError(self.mp_group is None, "mp_group (tensor parallel all-reduce) is outside this single-GPU build")
+        if self.optimize_lm_head:
+            from ipex_llm.transformers.low_bit_linear import reshape_lm_head_input
+            x = reshape_lm_head_input(x)
+        given = x.dtype
+        if self.training and not torch.is_inference_mode_enabled() and self.compute_dtype is not None:
+            x = x.to(self.compute_dtype)
+        if self.bias is not None and self.bias.dtype != x.dtype:
+            self.bias.data = self.bias.data.to(x.dtype)
+        y = row_int8_linear(x, self.weight, self.weight_scale, self.bias)
+        return y if y.dtype == given else y.to(given)
+
+    def dequantize(self, dtype=torch.float32):
+        return row_int8_dequantize(self.weight.data, self.weight_scale.data, dtype)
+
+
+class RowInt8Experts(_KeepsFormat):
+    """The experts of a sparse mixture-of-experts block in row-scaled int8: takes the place of a module that holds `gate_up_proj` [E, 2 I, H]
+    and `down_proj` [E, H, I] (moe.LowBitExperts has the call)."""
+
+    _FORMAT = ("gate_up_proj", "gate_up_proj_scale", "down_proj", "down_proj_scale")
+
+    def __init__(self, num_experts, hidden_dim, intermediate_dim, act_fn):
+        super().__init__()
+        invalidInputError(hidden_dim % 16 == 0 and intermediate_dim % 16 == 0 and max(hidden_dim, intermediate_dim) <= MOST_K,
+                          f"RowInt8Experts needs hidden_dim and intermediate_dim to be multiples of 16, at most {MOST_K}")
+        self.num_experts, self.hidden_dim, self.intermediate_dim, self.act_fn = num_experts, hidden_dim, intermediate_dim, act_fn
+        self.own_gate = None                             # h of (g | u), where it is not act_fn(g) * u (moe.gate_of)
+        for name, n, k in (("gate_up_proj", 2 * intermediate_dim, hidden_dim), ("down_proj", hidden_dim, intermediate_dim)):
+            setattr(self, name, _frozen(torch.empty((num_experts, n, k), dtype=torch.int8)))
+            setattr(self, name + "_scale", _frozen(torch.empty((num_experts, n), dtype=torch.float32)))
+
+    @classmethod
+    def from_fused(cls, module, convert_shape_only=False):
+        """From a module with dense or row-scaled `gate_up_proj` and `down_proj` and an `act_fn`, or a gate of its own, which is kept."""
+        n_exp, two_i, hidden = module.gate_up_proj.shape
+        invalidInputError(tuple(module.down_proj.shape) == (n_exp, hidden, two_i // 2), "gate_up_proj / down_proj shapes do not fit together")
+        from ipex_llm.transformers.moe import gate_of
+        known, gate = gate_of(module)
+        invalidInputError(known, "the experts' gate depends on tensors of the module, which its row-scaled form does not have")
+        with torch.device("meta"):
+            new = cls(n_exp, hidden, two_i // 2, module.act_fn)
+        new.own_gate = gate
+        for name in ("gate_up_proj", "down_proj"):
+            w, scale = _taken(module, name, convert_shape_only)
+            setattr(new, name, _frozen(w))
+            setattr(new, name + "_scale", _frozen(scale))
+        return new.train(module.training)
+
+    def forward(self, hidden_states, top_k_index, top_k_weights):
+        from ipex_llm.transformers.moe import activation_code
+        if top_k_index.shape[0] == 0:
+            return torch.zeros_like(hidden_states)
+        weights = (self.gate_up_proj, self.gate_up_proj_scale, self.down_proj, self.down_proj_scale)
+        act = activation_code(self.act_fn)
+        if act is None or self.own_gate is not None:
+            return _expert_loop(hidden_states, top_k_index, top_k_weights, *weights, self.own_gate or _gated(self.act_fn))
+        return row_int8_experts(hidden_states, top_k_index, top_k_weights, *weights, act)

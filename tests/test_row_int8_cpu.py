@@ -87,7 +87,7 @@ def test_plans_cover_every_size():
         for n in (1, 64, 1000, 28672):
             for k in (16, 128, 144, 4096, 1 << 17):
                 rows, cols, splits, groups = ggml.lowbit_row_int8_plan(1, 0, m, n, k)
-                assert (rows == 0) == (ggml.lowbit_row_int8_waves(m, n, k) > 0)
+                assert (rows == 0 or cols == 16) == (ggml.lowbit_row_int8_waves(m, n, k) > 0)      # (few rows, or streamed)
                 assert 1 <= splits <= (k + 127) // 128 and groups in (1, 2)
                 if rows:
                     need = m * ((k + 127) // 128 * 128) + m * 4 + (splits * m * n * 4 if splits > 1 else 0)
