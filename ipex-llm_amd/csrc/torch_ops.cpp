@@ -490,8 +490,12 @@ bool plain_bias(const Tensor &bias, const Tensor &x, at::ScalarType dtype, int64
 }
 
 // The gradient that flows on to x, the quantization of x counting as the identity.  Holds the weight as ProductBackward does.
+// how often a tensor was changed in place (inference tensors do not count that)
+static int64_t changes(const Tensor &t) { return t.is_inference() ? 0 : (int64_t)t._version(); }
+
 struct RowInt8Backward : public torch::autograd::Node {
     Tensor w, scale;
+    int64_t w_changes = 0, scale_changes = 0;                // of the forward
     at::ScalarType x_dtype = at::kHalf;
     at::DimVector x_shape;
 
@@ -504,6 +508,8 @@ struct RowInt8Backward : public torch::autograd::Node {
                                                : at::zeros({c10::multiply_integers(x_shape) / K, N}, w.options().dtype(x_dtype));
         c10::DeviceGuard guard(grad.device());
         if (grad.device() != w.device()) throw Failed("the int8 weight is not where the forward found it");
+        if (changes(w) != w_changes || changes(scale) != scale_changes)
+            throw Failed("the int8 weight or its scales have been modified by an inplace operation since the forward");
         if (differentiable(grad) || !nothing_watches(grad))  // (a second derivative, a transform: the dense product)
             return {at::matmul(grad.to(at::kFloat), w.to(at::kFloat).mul_(scale.unsqueeze(-1))).to(x_dtype).view(x_shape)};
         const Tensor g = whole_rows(grad);
@@ -529,6 +535,8 @@ Tensor row_int8_linear(const Tensor &x_in, const Tensor &w, const Tensor &scale,
     node->set_next_edges(torch::autograd::collect_next_edges(x_in));
     node->w = w;
     node->scale = scale;
+    node->w_changes = changes(w);
+    node->scale_changes = changes(scale);
     node->x_dtype = x_in.scalar_type();
     node->x_shape.assign(x_in.sizes().begin(), x_in.sizes().end());
     {
