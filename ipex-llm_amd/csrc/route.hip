@@ -239,7 +239,7 @@ template <int NR> __global__ __launch_bounds__(256) void route_grad_kernel(const
     for (int i = 0; i < NR; i++) s[i] /= sum;
     const int id = lane < p.top_k ? (int)p.ids[t * p.top_k + lane] : 0;
     const double g = lane < p.top_k ? (double)p.grad[t * p.top_k + lane] * (double)p.factor : 0.0;
-    double total = 0.0, dot = 0.0;
+    double chosen = 0.0;                                     // lane j: the score of choice j
     for (int j = 0; j < p.top_k; j++) {
         const int e = __builtin_amdgcn_readlane(id, j);
         double own = 0.0;
@@ -247,13 +247,14 @@ template <int NR> __global__ __launch_bounds__(256) void route_grad_kernel(const
         for (int i = 0; i < NR; i++)
             if (i == e >> 6) own = s[i];
         const double c = from_lane(own, e & 63);
-        total += c;
-        dot += from_lane(g, j) * c;
+        if (lane == j) chosen = c;
     }
-    const double by = p.renormalize ? 1.0 / total : 1.0, less = p.renormalize ? dot * by : 0.0;
+    // (by c / C, which is 1 where one expert is chosen, whose gradient is zero)
+    const double total = p.renormalize ? wave_sum(chosen) : 1.0, less = p.renormalize ? wave_sum(lane < p.top_k ? g * (chosen / total) : 0.0) : 0.0;
+    const double mine = (g - less) / total;
     for (int j = 0; j < p.top_k; j++) {
         const int e = __builtin_amdgcn_readlane(id, j);
-        const double d = (from_lane(g, j) - less) * by;
+        const double d = from_lane(mine, j);
 #pragma unroll
         for (int i = 0; i < NR; i++)
             if (lane + 64 * i == e) ds[i] = d;

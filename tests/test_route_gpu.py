@@ -144,6 +144,17 @@ def test_gradients_against_differences():
             assert abs((ends[0] - ends[1]) / (2 * step) - grad.cpu().double()[at]) <= step ** 2 * size * g.abs().sum() + 2.0 ** -24 / step * g.abs().sum()
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_one_expert_has_a_weight_that_nothing_changes(score):
+    """top_k = 1, renormalized: the weight is the scale whatever x and the router are, and their gradients are zeros."""
+    x, router, _ = operands(50, 33, 264, torch.bfloat16, torch.bfloat16)
+    xd, rd = x.cuda().requires_grad_(), router.cuda().requires_grad_()
+    w, index = moe.moe_route(xd, rd, 1, score=score, scale=2.5)
+    assert torch.equal(index.cpu(), (x.double() @ router.double().t()).argmax(-1, keepdim=True)) and (w == 2.5).all()
+    gx, gr = torch.autograd.grad(w, (xd, rd), torch.randn((50, 1), generator=torch.Generator().manual_seed(1)).cuda())
+    assert not gx.any() and not gr.any()
+
+
 def test_leading_dimensions_strides_and_types():
     x, router, bias = operands(24, 20, 128, torch.bfloat16, torch.bfloat16)
     w, index = moe.moe_route(x.cuda(), router.cuda(), 3, bias.cuda())
