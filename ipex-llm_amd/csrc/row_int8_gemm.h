@@ -70,7 +70,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, MIN_WAVES) void row_int8_tiled_k
     constexpr int UP_COLUMNS = BN / 2;
     // Two buffers: a step in two halves, each with a barrier (see the loop)
     constexpr int HALVES = S == 2 ? 2 : 1, PH = PW / HALVES;
-    static_assert(KG == 1 || (KG == 2 && MODE != INT8_UP && !BY_EXPERT && S * (BM + BN) * INT8_BLOCK >= TM * TN * WAVES * 1024), "room for a group's sums");
+    static_assert(KG == 1 || (MODE != INT8_UP && !BY_EXPERT && S * (BM + BN) * INT8_BLOCK >= TM * TN * WAVES * 1024), "room for a group's sums");
     static_assert(WP % (WAVES * HALVES) == 0 && XP % WAVES == 0 && PX > 0 && TN % 2 == 0 && (S > 2 || TN % 4 == 0 || TN == 2), "whole pieces per wave");
     constexpr uint32_t BUFFER = (BM + BN) * INT8_BLOCK, OWN = S * BUFFER;            // a group's
     __shared__ __attribute__((aligned(16))) uint8_t shared[KG * OWN];
@@ -99,9 +99,9 @@ __global__ __launch_bounds__(64 * WM * WN * KG, MIN_WAVES) void row_int8_tiled_k
         m0 = (band * 8 + at - tn * rows) * BM;
     }
     const int n0 = tn * (UP ? UP_COLUMNS : BN), KB = p.KB;
-    // blocks of K: of this split, and of this group (an odd one out is the first group's; the other walks as far, over zeros of x)
+    // blocks of K: of this split, and of this group (the first ones have them all; the last walks as far, over zeros of x)
     const int from = split * p.split_blocks, to = MODE == INT8_PART && from + p.split_blocks < KB ? from + p.split_blocks : KB;
-    const int walk = (to - from + KG - 1) / KG, b0 = KG == 1 || group == 0 ? from : from + walk, stop = b0 + walk, b1 = stop < to ? stop : to;
+    const int walk = (to - from + KG - 1) / KG, b0 = from + group * walk, stop = b0 + walk, b1 = stop < to ? stop : to;
 
     // ---- sources of this wave's pieces of 8 rows
     uint32_t xoff[GATHER ? 1 : PX], woff[PW];
@@ -295,15 +295,18 @@ __global__ __launch_bounds__(64 * WM * WN * KG, MIN_WAVES) void row_int8_tiled_k
     }
     wait_all_loads();
     __syncthreads();
-    if constexpr (KG == 2) {
-        i32x4 *const sums = (i32x4 *)(shared + OWN) + wave * TN * TM * 64 + lane;
-        if (group == 1)
+    if constexpr (KG > 1) {
+        constexpr int NEXT = OWN / 16;
+        i32x4 *const sums = (i32x4 *)shared + wave * TN * TM * 64 + lane;
+        if (group > 0)
 #pragma unroll
-            for (int o = 0; o < COUNT; o++) sums[o * 64] = acc[o / TM][o % TM];
+            for (int o = 0; o < COUNT; o++) sums[group * NEXT + o * 64] = acc[o / TM][o % TM];
         __syncthreads();
-        if (group == 1) return;
+        if (group > 0) return;
 #pragma unroll
-        for (int o = 0; o < COUNT; o++) acc[o / TM][o % TM] += sums[o * 64];
+        for (int v = 1; v < KG; v++)
+#pragma unroll
+            for (int o = 0; o < COUNT; o++) acc[o / TM][o % TM] += sums[v * NEXT + o * 64];
     }
 
     // ---- results: lane = row r of tile i, columns 4 g .. 4 g + 3 of tile t's sixteen

@@ -42,16 +42,18 @@ template <typename OT, bool PART> static void launch_stream(const Int8Args &p, i
 
 // Estimated times in us, fitted to timed launches with weights from memory.
 //
-// Tiles: rounds of workgroups over the GPU, each a walk of blocks; what a launch, its first loads and its stores take, and again the first loads of
-// each further round; the results, which forms of two workgroups on a CU write while the other one multiplies; the sums of two groups; with splits the
-// sums written and read.  163 sizes, 5 to 8192 rows by 64 to 28672 by 128 to 16384.
+// Tiles: rounds of workgroups over the GPU, each a walk of blocks; a step with one workgroup on a CU is longer where the weight comes from memory, which one
+// of 2 MB starts to and one of 16 MB does; what a launch, its first loads and its stores take, and again the first loads of each further round; the
+// results, which forms of two workgroups on a CU write while the other one multiplies; the sums of groups; with splits the sums written and read.
+// 233 sizes, 5 to 8192 rows by 64 to 28672 by 128 to 16384, forms and splits of each: the pick is 1.7 % above the fastest on average.
 static float tiled_us(int form, int M, int N, int KB, int splits) {
     const Int8Form &f = INT8_FORMS[form];
     const int64_t units = (int64_t)cdiv(M, f.rows) * cdiv(N, f.cols) * splits, further = (units - 1) / (256 * f.per_cu);
-    float us = tiled_walk_us(f.step_us, f.alone_us, f.per_cu, units, cdiv(cdiv(KB, splits), f.groups)) + 3.2f + 0.56f * further;
-    us += (f.per_cu == 1 ? 0.39e-6f : 0.30e-6f) * 2.0f * M * N;
-    if (f.groups > 1) us += 0.3f;
-    if (splits > 1) us += 2.5f + (float)splits * M * N * 8.0f / 2.9e6f;
+    const float megabytes = (float)N * KB * INT8_BLOCK * 1e-6f, far = megabytes <= 2.0f ? 0.0f : megabytes >= 16.0f ? 1.0f : log2f(megabytes * 0.5f) / 3.0f;
+    float us = tiled_walk_us(f.step_us, f.alone_us + far * f.far_us, f.per_cu, units, cdiv(cdiv(KB, splits), f.groups)) + 3.24f + 0.11f * far + 0.83f * further;
+    us += (f.per_cu == 1 ? 0.38e-6f : 0.28e-6f) * 2.0f * M * N;
+    if (f.groups > 1) us += 0.5f;
+    if (splits > 1) us += 1.16f + 0.76f * log2f((float)splits) + (float)splits * M * N * 8.0f / 3.6e6f;
     return us;
 }
 // The streaming kernel: blocks of K that a CU walks, each with x, and what the other CUs leave it of the memory; 518 launches of 1 to 32 rows, within 9 %

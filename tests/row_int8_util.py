@@ -10,7 +10,8 @@ BACK_SHAPES = [(1, 1, 16), (1, 16, 16), (1, 130, 128), (5, 128, 272), (17, 300, 
 # .. and sizes of every form of tiles, of both streaming kernels by number of waves, alone and in parts (test_every_form_is_run), and of the gradient
 TILES = [(301, 702, 1040), (935, 1070, 144), (644, 1546, 1184), (653, 454, 4672), (1925, 4007, 144), (2250, 1806, 128), (3255, 2439, 144),
          (3466, 3630, 144), (1347, 1459, 128), (66, 2005, 7952), (2884, 130, 6560), (5000, 2050, 272), (6000, 4100, 144), (40, 3000, 4992), (20, 20011, 400), (48, 11009, 1040),
-         (1700, 3001, 544), (4761, 794, 544), (2660, 3090, 144), (5132, 2498, 272), (1103, 19, 2048), (36, 20, 15904)]
+         (1700, 3001, 544), (4761, 794, 544), (2660, 3090, 144), (5132, 2498, 272), (1103, 19, 2048), (36, 20, 15904),
+         (58, 7282, 720), (50, 5860, 1088), (150, 13824, 528), (1000, 4000, 1040), (513, 4090, 2064), (300, 5000, 1040), (500, 1700, 3216), (130, 2600, 8208)]
 STREAMED = [(1, 2003, 16400), (2, 200, 8208), (4, 77, 8512), (3, 1001, 14656), (6, 4099, 4096), (16, 4096, 4112), (17, 512, 4096), (32, 200, 8192), (29, 783, 272),
             (13, 3037, 144), (5, 2000, 1040), (25, 2001, 2064), (2, 6990, 8832), (4, 20000, 528), (5, 17, 1424),
             (17, 18, 2880), (1, 17, 3616), (5, 16, 8064), (8, 40, 11712), (18, 16, 11552)]

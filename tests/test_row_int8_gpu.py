@@ -131,7 +131,7 @@ def test_every_form_is_run():
     and in parts, and the kernel of few rows with each number of waves."""
     seen = {ggml.lowbit_row_int8_plan(1, 0, *s) + (ggml.lowbit_row_int8_waves(*s),) for s in u.SHAPES + u.TILES + u.STREAMED}
     forms = {(p[0], p[1], p[3]) for p in seen if p[1] > 16}
-    assert forms == {(256, 256, 1), (192, 256, 1), (128, 256, 1), (128, 128, 1), (64, 128, 1), (32, 128, 1), (64, 64, 2)}, forms
+    assert forms == {(256, 256, 1), (192, 256, 1), (128, 256, 1), (128, 128, 1), (64, 128, 1), (32, 128, 1), (64, 64, 2), (64, 32, 4)}, forms
     assert {p[2] > 1 for p in seen if p[1] > 16} == {False, True}
     assert {(p[0], p[4], p[2] > 1) for p in seen if p[1] == 16} == {(r, w, s) for r in (16, 32) for w in (4, 8) for s in (False, True)}
     assert {p[4] for p in seen if p[1] == 0} == {4, 8}
