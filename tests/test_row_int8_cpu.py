@@ -88,7 +88,7 @@ def test_plans_cover_every_size():
             for k in (16, 128, 144, 4096, 1 << 17):
                 rows, cols, splits, groups = ggml.lowbit_row_int8_plan(1, 0, m, n, k)
                 assert (rows == 0 or cols == 16) == (ggml.lowbit_row_int8_waves(m, n, k) > 0)      # (few rows, or streamed)
-                assert 1 <= splits <= (k + 127) // 128 and groups in (1, 2)
+                assert 1 <= splits <= (k + 127) // 128 and groups in (1, 2, 4)
                 if rows:
                     need = m * ((k + 127) // 128 * 128) + m * 4 + (splits * m * n * 4 if splits > 1 else 0)
                     assert ggml.lowbit_row_int8_linear_workspace_bytes(1, m, n, k) >= need
