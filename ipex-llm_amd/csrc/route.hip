@@ -92,6 +92,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void route_logits_kernel(const Route
 }
 
 // ---- a wave's doubles
+//
+// (Maxima and sums over a wave by moves between lanes: by way of LDS the selection of 6 of 64 took 4.0 us for 500 tokens, so 3.4.)
 
 template <int CTRL, int ROWS> __device__ inline double add_dpp(double v) {
     const u32x2 b = __builtin_bit_cast(u32x2, v);
@@ -276,7 +278,8 @@ template <int NR> __global__ __launch_bounds__(256) void route_grad_kernel(const
 //
 // A lane of B loads eight neighbours of a row, which are its column of eight tiles, so that a wave owns 128 columns and a lane stores
 // eight neighbours of a row of C.  ACROSS: A(m, k) = dz[k, m], the gradient of the router, whose waves take the rows k in turn and add their
-// sums in LDS, in order; else A(m, k) = dz[m, k], the gradient of x, whose waves take 128 columns each.
+// sums in LDS, in order; else A(m, k) = dz[m, k], the gradient of x, whose waves take 128 columns each.  1000 tokens x 60 experts of 4096: router 14.3 us and
+// the splits' sum 3.8, x 10.9, the gradient of the logits 4.2; loads a step ahead make it 15.3 and 13.0.
 struct OuterArgs {
     const float *dz;                                         // [T, lde]
     const void *b;                                           // [K, H]

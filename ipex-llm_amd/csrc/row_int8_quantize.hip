@@ -1,6 +1,8 @@
 // Codes and scales of rows (row_int8.h): activations by token, weights by output channel.
 //
-// Bound by memory: a row is read once, into registers, and its codes written once.
+// Bound by memory: a row is read once, into registers, and its codes written once.  [28672 x 8192] in bfloat16 124 us, 5.7 TB/s read and written, [8192 x
+// 8192] 47, [2048 x 11008] 15.5; 48 rows of 11008 take what a launch takes.  A wave per row up to 1024 values, so that no maximum waits for a barrier; eight
+// above 8192, so that a row stays in registers.
 #include "row_int8.h"
 
 #include <type_traits>

@@ -3,7 +3,7 @@
 // A workgroup owns 16 weight rows and all rows of x, MT * 16 at most.  Its waves take the blocks of K in turn, both operands from memory
 // straight to registers, DEPTH blocks in flight, and their whole sums meet in LDS: no barrier stands between a load and its use, which tiles pay for
 // in every step.  Each workgroup reads all of x from L2, so that tiles overtake it as rows and weight rows grow: 16 rows on [4096 x 4096] 7.4 us
-// against 9.6 in tiles, 32 8.8 / 10.1, 4 on [512 x 4096] 5.6 / 7.4; 16 on [11008 x 4096] 15.4 / 12.5, 64 on [4096 x 4096] 12.7 / 11.5.
+// against 8.9 in tiles, 4 on [512 x 4096] 5.6 / 7.4; 16 on [11008 x 4096] 15.4 / 12.5, 64 on [4096 x 4096] 12.7 / 10.2.
 #pragma once
 #include "row_int8_tiled.h"
 

@@ -489,10 +489,10 @@ bool plain_bias(const Tensor &bias, const Tensor &x, at::ScalarType dtype, int64
                                bias.is_contiguous() && !differentiable(bias));
 }
 
-// The gradient that flows on to x, the quantization of x counting as the identity.  Holds the weight as ProductBackward does.
 // how often a tensor was changed in place (inference tensors do not count that)
 static int64_t changes(const Tensor &t) { return t.is_inference() ? 0 : (int64_t)t._version(); }
 
+// The gradient that flows on to x, the quantization of x counting as the identity.  Holds the weight as ProductBackward does.
 struct RowInt8Backward : public torch::autograd::Node {
     Tensor w, scale;
     int64_t w_changes = 0, scale_changes = 0;                // of the forward

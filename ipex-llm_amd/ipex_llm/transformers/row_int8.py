@@ -161,7 +161,7 @@ def _expert_loop(x, top_k_index, top_k_weights, gate_up, gate_up_scale, down, do
             gu = row_int8_linear(rows[e], gate_up[e], gate_up_scale[e])
             ys.append(row_int8_linear(gate(gu), down[e], down_scale[e]))
     if not ys:
-        return x * 0 + top_k_weights.sum().to(x.dtype) * 0
+        return torch.zeros_like(x) + (x[:0].sum() + top_k_weights[:0].sum().to(x.dtype))       # (zeros that carry the gradients)
     order = order[:len(order) - counts[n_exp]]
     y = torch.cat(ys) * top_k_weights.reshape(-1)[order].float().unsqueeze(-1)
     return y.new_zeros((tokens * top_k, x.shape[1])).index_copy(0, order, y).view(tokens, top_k, -1).sum(1).to(x.dtype)

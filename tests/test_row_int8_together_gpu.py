@@ -136,6 +136,34 @@ def test_nan_stays_in_its_row_and_column(dtype, m, n, k):
     assert same(y, want)
 
 
+@pytest.mark.parametrize("m", [1, 3, 12, 30, 70, 300, 1200])
+def test_codes_of_minus_128(m):
+    """The quantizer makes none, a checkpoint may hold them."""
+    g = gen(m)
+    x, (w, ws) = torch.randn((m, 272), generator=g).bfloat16(), whole(g, 200, 272)
+    w[torch.rand(w.shape, generator=g) < 0.3] = -128
+    grad = torch.randint(-8, 9, (m, 200), generator=g).bfloat16()
+    leaf = x.cuda().requires_grad_()
+    y = ri.row_int8_linear(leaf, w.cuda(), ws.cuda())
+    assert torch.equal(y.detach().cpu(), u.product(x, w, ws))
+    assert torch.equal(torch.autograd.grad(y, leaf, grad.cuda())[0].cpu(), back(grad, w, ws).bfloat16())
+
+
+def test_tokens_whose_indices_name_no_expert_get_zeros_whatever_they_hold():
+    x, index, p, *weights = expert_case(2, 5, 2, 4, 64, 32, torch.float32)
+    x[1], x[2, 3] = math.nan, math.inf
+    index[:3] = 9
+    for leaf in (x, x.clone().requires_grad_()):
+        y = ri.row_int8_experts(leaf, index, p, *weights)
+        assert not y[:3].any() and y[3:].isfinite().all() and y[3:].any()
+    index[:] = -1
+    leaf, q = x.clone().requires_grad_(), p.clone().requires_grad_()
+    y = ri.row_int8_experts(leaf, index, q, *weights)
+    assert not y.any() and not ri.row_int8_experts(x, index, p, *weights).any()
+    gx, gp = torch.autograd.grad(y.sum(), (leaf, q))
+    assert not gx.any() and not gp.any()
+
+
 # ---------------------------------------------------------------- nothing is written past a result
 
 @pytest.mark.parametrize("m,n,k", [(1, 33, 256), (5, 40, 272), (20, 77, 400), (90, 130, 272), (300, 261, 144), (2, 16, 16384)])
