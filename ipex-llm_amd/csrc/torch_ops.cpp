@@ -309,6 +309,10 @@ Tensor whole_rows(const Tensor &t) {
     Tensor c = t.contiguous();
     return ((uintptr_t)c.const_data_ptr() & 15) ? c.clone() : c;
 }
+// the same, of a tensor whose history is left behind (a detached tensor is a tensor more, half a microsecond: made only where a copy is)
+Tensor whole_values(const Tensor &t) {
+    return t.is_contiguous() && !((uintptr_t)t.const_data_ptr() & 15) ? t : whole_rows(t.detach());
+}
 
 // w holds e4m3 codes [.., N, K] and scale their scales, one per block of 128 x 128, on x's device
 bool is_block_fp8(const Tensor &w, const Tensor &scale, const Tensor &x, int64_t matrices) {
@@ -455,7 +459,7 @@ constexpr int64_t ROW_INT8_MOST_K = 1 << 17;
 std::pair<Tensor, Tensor> row_int8_quantize(const Tensor &x_in) {
     if (!on_gpu(x_in) || x_in.dim() < 1 || x_in.numel() == 0 || x_in.size(-1) % 16 || dtype_code(x_in.scalar_type()) < 0 ||
         !nothing_watches(x_in)) return {};
-    const Tensor x = whole_rows(x_in.detach());
+    const Tensor x = whole_values(x_in);
     const int64_t K = x.size(-1);
     c10::DeviceGuard guard(x.device());
     const Tensor codes = at::empty(x.sizes(), x.options().dtype(at::kChar)),
@@ -541,7 +545,7 @@ Tensor row_int8_linear(const Tensor &x_in, const Tensor &w, const Tensor &scale,
     node->x_shape.assign(x_in.sizes().begin(), x_in.sizes().end());
     {
         c10::AutoGradMode no_grad(false);
-        y = row_int8_any_product(whole_rows(x_in.detach()), Tensor(), w, scale, bias, x_in.scalar_type());
+        y = row_int8_any_product(whole_values(x_in), Tensor(), w, scale, bias, x_in.scalar_type());
     }
     torch::autograd::set_history(y, node);
     return y;
@@ -647,7 +651,7 @@ struct RouteBackward : public torch::autograd::Node {
             auto g = torch::autograd::grad({w}, inputs, {grad}, /*retain_graph=*/true, create, /*allow_unused=*/false);
             return {want_x ? g[0] : Tensor(), want_r ? g[want_x ? 1 : 0] : Tensor()};
         }
-        const Tensor xr = whole_rows(x.detach()), rr = whole_rows(router.detach()), g = grad.to(at::kFloat).contiguous();
+        const Tensor xr = whole_values(x), rr = whole_values(router), g = grad.to(at::kFloat).contiguous();
         Tensor gx = want_x ? at::empty(xr.sizes(), xr.options()) : Tensor(), gr = want_r ? at::empty(rr.sizes(), rr.options()) : Tensor();
         const size_t bytes = api.route_backward_workspace_bytes(T, (int)E, H);
         const Tensor ws = at::empty({(int64_t)bytes}, xr.options().dtype(at::kByte));
@@ -668,7 +672,7 @@ std::pair<Tensor, Tensor> route(const Tensor &x_in, const Tensor &router_in, con
     Tensor w, ids, logits;
     {
         c10::AutoGradMode no_grad(false);
-        const Tensor x = whole_rows(x_in.detach()), router = whole_rows(router_in.detach()), bias = bias_in.defined() ? bias_in.detach().contiguous() : Tensor();
+        const Tensor x = whole_values(x_in), router = whole_values(router_in), bias = bias_in.defined() ? bias_in.detach().contiguous() : Tensor();
         w = at::empty({T, rule.top_k}, x.options().dtype(at::kFloat));
         ids = at::empty({T, rule.top_k}, x.options().dtype(at::kLong));
         if (wants) logits = at::empty({T, E}, x.options().dtype(at::kDouble));
