@@ -1,4 +1,4 @@
-// Up to four rows of activations times a weight with a scale for each row (row_int8.h): the weight streams past once, in one launch.
+// Up to sixteen rows of activations times a weight with a scale for each row (row_int8.h): the weight streams past once, in one launch.
 //
 // A workgroup owns 16 weight rows; its waves take the blocks of K in turn and their sums meet in LDS.  A wave's loads are 16 rows x 64
 // contiguous bytes, STEPS blocks ahead of their use.  x is quantized by each workgroup, into LDS, while the first weights are on their
@@ -7,7 +7,7 @@
 
 namespace lowbit {
 
-constexpr int FEW_ROWS = 4;
+constexpr int FEW_ROWS = 16;
 
 struct Int8Rows {
     const void *x;                                           // [M, K]
@@ -118,24 +118,24 @@ __global__ __launch_bounds__(64 * WAVES, 2) void row_int8_few_rows_kernel(const 
         }
     }
 
-    // the waves' sums, [wave][row][16 columns]
+    // the waves' sums, [wave][row of M][16 columns]
     __syncthreads();                                         // (they lie where the codes were)
     int32_t *const sums = (int32_t *)lds;
-    if (r < M) *(i32x4 *)(sums + (wave * FEW_ROWS + r) * 16 + g * 4) = acc;
+    if (r < M) *(i32x4 *)(sums + (wave * M + r) * 16 + g * 4) = acc;
     __syncthreads();
     if ((int)threadIdx.x >= M * 16) return;
     const int m = threadIdx.x >> 4, c = threadIdx.x & 15;
     if (n0 + c >= N) return;
     int32_t sum = 0;
 #pragma unroll
-    for (int w = 0; w < WAVES; w++) sum += sums[(w * FEW_ROWS + m) * 16 + c];
+    for (int w = 0; w < WAVES; w++) sum += sums[(w * M + m) * 16 + c];
     float v = (float)sum * row_scale(most[m]) * p.ws[n0 + c];
     if (p.bias) v += (float)((const AT *)p.bias)[n0 + c];
     ((AT *)p.y)[(int64_t)m * N + n0 + c] = Stored<AT>::of(v);
 }
 
 static size_t few_rows_lds(int M, int KB, int waves) {
-    const size_t codes = (size_t)M * (KB * INT8_BLOCK + 16), sums = (size_t)waves * FEW_ROWS * 16 * sizeof(int32_t);
+    const size_t codes = (size_t)M * (KB * INT8_BLOCK + 16), sums = (size_t)waves * M * 16 * sizeof(int32_t);
     return codes > sums ? codes : sums;
 }
 
@@ -149,7 +149,8 @@ template <typename AT> static void launch_few_rows(const Int8Rows &p, int waves,
 // Waves of a workgroup, by estimated time in us; 0 where codes of x, made by a launch of their own, and a product of those are estimated shorter,
 // or where x's codes do not fit 64 KiB of LDS.  What grows with the rows is x, which every workgroup reads and quantizes: on [4096 x 4096] one row
 // 6.1 against 6.3 and the launch ahead of it, 2.6; four 8.8 / 6.6 + 2.6; on [28672 x 8192] one 44.5 / 44.4 + 2.6, four 71 / 46 + 2.7; one on
-// [20000 x 512] 9.4 / 4.2 + 2.6.  Fitted to 80 sizes of 1 to 16 rows, within 11 and 17 % at rms; 16
+// [20000 x 512] 9.4 / 4.2 + 2.6.  With short rows sixteen of them are few: 11 on [64 x 128] 3.2 against 5.5 with the launch ahead, 9 on [730 x 384] 4.2 / 5.5, 5 on
+// [2086 x 1152] 5.1 / 6.7, 16 on [1024 x 1024] 7.4 / 6.9.  Fitted to 80 sizes of 1 to 16 rows, within 11 and 17 % at rms; 16
 // waves would be the shortest at one row of very long weights only, [4096 x 11008] 13.7 against 14.3.
 constexpr size_t FEW_LDS = 65536 - 64;
 constexpr float ROWS_LAUNCH_US = 2.6f;
@@ -164,7 +165,8 @@ static int few_rows_waves(int M, int N, int K, float codes_us) {
     int best = 0;
     for (const auto &f : fits) {
         if (M > FEW_ROWS || few_rows_lds(M, KB, f.waves) > FEW_LDS) continue;
-        const float us = f.launch + f.further * (load - 1.0f) + load * KB * (f.block + f.row * M / f.waves);
+        // (each further workgroup on a CU waits for its rows: half a microsecond where they are many)
+        const float us = f.launch + (f.further + (M > 4 ? 0.6f : 0.0f)) * (load - 1.0f) + load * KB * (f.block + f.row * M / f.waves);
         if (us < least) {
             least = us;
             best = f.waves;
