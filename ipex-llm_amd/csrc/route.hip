@@ -11,7 +11,8 @@
 // (Two waves per SIMD are asked for so that the sums stay in vector registers: left alone the compiler keeps them in accumulation registers and copies
 // them back and forth in every turn of the loops below.)
 //
-// The first launch sums a part of H for 16 tokens by 16 TN experts per workgroup, the second one, a wave per token, adds the parts and chooses.
+// The first launch sums a part of H for 16 tokens by 16 TN experts per workgroup, the second one, a wave per token, adds the parts and chooses.  Small routers
+// take one launch, a token per workgroup.
 #include "row_int8.h"
 
 #include <type_traits>
@@ -158,29 +159,9 @@ template <int NR> __device__ inline double scores(const double (&z)[NR], double 
     return wave_sum(sum);
 }
 
-// One token per wave; NR * 64 experts at most.
-template <int NR> __global__ __launch_bounds__(256) void route_select_kernel(const ScoreArgs p) {
-    const int lane = threadIdx.x & 63;
-    const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (t >= p.T) return;
-    double z[NR], s[NR];
-#pragma unroll
-    for (int i = 0; i < NR; i++) {
-        const int e = lane + 64 * i;
-        z[i] = 0.0;
-        if (e < p.E) {
-            const double *const from = p.part + t * p.E + e;
-            const int64_t stride = (int64_t)p.T * p.E;
-            for (int v = 0; v < p.splits; v += 8) {          // (the parts on their way together, added in order)
-                double part[8];
-#pragma unroll
-                for (int u = 0; u < 8; u++) part[u] = v + u < p.splits ? from[(v + u) * stride] : 0.0;
-#pragma unroll
-                for (int u = 0; u < 8; u++) z[i] += part[u];
-            }
-            if (p.z) p.z[t * p.E + e] = z[i];
-        }
-    }
+// The choice for token t by one wave, of logits z, lane + 64 i; NR * 64 experts at most.
+template <int NR> __device__ __forceinline__ void choose(const ScoreArgs &p, int64_t t, const double (&z)[NR], int lane) {
+    double s[NR];
     // (the scores of all only where the choice or the weights go by them)
     const bool of_chosen = p.renormalize && !p.bias;
     double sum = 1.0;
@@ -225,6 +206,88 @@ template <int NR> __global__ __launch_bounds__(256) void route_select_kernel(con
         p.w[t * p.top_k + lane] = (float)((double)p.factor * (chosen / (p.renormalize ? total : sum)));
         p.ids[t * p.top_k + lane] = index;
     }
+}
+
+// One token per wave.
+template <int NR> __global__ __launch_bounds__(256) void route_select_kernel(const ScoreArgs p) {
+    const int lane = threadIdx.x & 63;
+    const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (t >= p.T) return;
+    double z[NR];
+#pragma unroll
+    for (int i = 0; i < NR; i++) {
+        const int e = lane + 64 * i;
+        z[i] = 0.0;
+        if (e < p.E) {
+            const double *const from = p.part + t * p.E + e;
+            const int64_t stride = (int64_t)p.T * p.E;
+            for (int v = 0; v < p.splits; v += 8) {          // (the parts on their way together, added in order)
+                double part[8];
+#pragma unroll
+                for (int u = 0; u < 8; u++) part[u] = v + u < p.splits ? from[(v + u) * stride] : 0.0;
+#pragma unroll
+                for (int u = 0; u < 8; u++) z[i] += part[u];
+            }
+            if (p.z) p.z[t * p.E + e] = z[i];
+        }
+    }
+    choose<NR>(p, t, z, lane);
+}
+
+// A token per workgroup, logits and choice in one launch, where a router is small: a wave sums ROWS rows of it at a time, eight apart, in float64, and the first
+// wave chooses.  EIGHTS: pieces of 512 values on their way together.
+constexpr int SMALL_EXPERTS = 64;
+template <typename AT, typename RT, int ROWS> __global__ __launch_bounds__(512, 2) void route_small_kernel(const RouteArgs a, const ScoreArgs p) {
+    using X8 = typename Octet<AT>::type;
+    using R8 = typename Octet<RT>::type;
+    constexpr int EIGHTS = sizeof(RT) == 4 && ROWS == 4 ? 2 : 4;
+    __shared__ double logits[SMALL_EXPERTS];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t t = blockIdx.x;
+    const AT *const x = (const AT *)a.x + t * a.H;
+    for (int e0 = wave; e0 < a.E; e0 += 8 * ROWS) {
+        double sum[ROWS] = {};
+        const RT *rows[ROWS];                                // (past the last: it again, whose sum is not kept)
+#pragma unroll
+        for (int i = 0; i < ROWS; i++) rows[i] = (const RT *)a.r + (int64_t)(e0 + 8 * i < a.E ? e0 + 8 * i : a.E - 1) * a.H;
+        for (int h = 0; h < a.H; h += 512 * EIGHTS) {
+            X8 xv[EIGHTS];
+            R8 wv[ROWS][EIGHTS];
+#pragma unroll
+            for (int u = 0; u < EIGHTS; u++) {
+                const int k = h + u * 512 + lane * 8;
+                const bool in = k < a.H;
+                const X8 v = *(const X8 *)(x + (in ? k : 0));
+                xv[u] = in ? v : X8{};
+#pragma unroll
+                for (int i = 0; i < ROWS; i++) {
+                    const R8 w = *(const R8 *)(rows[i] + (in ? k : 0));
+                    wv[i][u] = in ? w : R8{};
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int u = 0; u < EIGHTS; u++) {
+                if (h + u * 512 >= a.H) break;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const double b = (double)(float)xv[u][j];
+#pragma unroll
+                    for (int i = 0; i < ROWS; i++) sum[i] = fma((double)(float)wv[i][u][j], b, sum[i]);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < ROWS; i++) sum[i] = wave_sum(sum[i]);
+#pragma unroll
+        for (int i = 0; i < ROWS; i++)
+            if (lane == 0 && e0 + 8 * i < a.E) logits[e0 + 8 * i] = sum[i];
+    }
+    __syncthreads();
+    if (wave > 0) return;
+    const double z[1] = {lane < a.E ? logits[lane] : 0.0};
+    if (p.z && lane < a.E) p.z[t * a.E + lane] = z[0];
+    choose<1>(p, t, z, lane);
 }
 
 // Gradients of z for gradients of the weights.  c: the chosen scores, w = factor c / C (C their sum, or 1):
@@ -410,7 +473,17 @@ static RoutePlan route_plan(int T, int E, int H) {
     return p;
 }
 
-size_t route_workspace_bytes(int T, int E, int H) { return (size_t)route_plan(T, E, H).splits * T * E * sizeof(double); }
+// One launch where a workgroup has a token's logits in 3.5 us at most: 512 values of one, two or four rows for each of its waves take 0.17, 0.28 and 0.58, of
+// which four in five are conversions to float64.  One token x 8 experts of 4096 4.6 us against 8.3 in two launches, 64 of 512 5.5 / 7.9, 64 of 1024 6.1 / 8.0, 64 of
+// 2048 7.7 / 7.8; 1024 tokens x 8 of 1024 5.5 / 8.8, 4096 x 8 of 512 10.3 / 9.5.
+static int small_rows(int E) { return E <= 8 ? 1 : E <= 16 ? 2 : 4; }
+static bool route_small(int T, int E, int H) {
+    if (E > SMALL_EXPERTS || T > 2048) return false;
+    const int rows = small_rows(E);
+    return cdiv(T, 512) * cdiv(E, 8 * rows) * cdiv(H, 512) * (rows == 1 ? 0.17f : rows == 2 ? 0.28f : 0.58f) <= 3.5f;
+}
+
+size_t route_workspace_bytes(int T, int E, int H) { return route_small(T, E, H) ? 0 : (size_t)route_plan(T, E, H).splits * T * E * sizeof(double); }
 
 template <int NR> static void launch_scores(const ScoreArgs &p, bool backward, hipStream_t st) {
     const dim3 grid((p.T + 3) / 4);
@@ -428,6 +501,21 @@ static void launch_scores(const ScoreArgs &p, bool backward, hipStream_t st) {
 // z: [T, E] for the backward, or null
 int launch_route(const void *x, int x_dtype, const void *router, int r_dtype, const float *bias, int T, int E, int H, int top_k, bool sigmoid,
                  bool renormalize, float factor, float *w, int64_t *ids, double *z, void *space, hipStream_t st) {
+    const ScoreArgs s = {(const double *)space, bias, nullptr, z, w, nullptr, ids, T, E, top_k, 0, 0, sigmoid, renormalize, factor};
+    if (route_small(T, E, H)) {
+        const RouteArgs a = {x, router, nullptr, T, E, H, 1, 0};
+        by_type(x_dtype, [&](auto *xt) {
+            by_type(r_dtype, [&](auto *rt) {
+                using AT = typename std::remove_pointer<decltype(xt)>::type;
+                using RT = typename std::remove_pointer<decltype(rt)>::type;
+                const int rows = small_rows(E);
+                if (rows == 1) hipLaunchKernelGGL((route_small_kernel<AT, RT, 1>), dim3(T), dim3(512), 0, st, a, s);
+                else if (rows == 2) hipLaunchKernelGGL((route_small_kernel<AT, RT, 2>), dim3(T), dim3(512), 0, st, a, s);
+                else hipLaunchKernelGGL((route_small_kernel<AT, RT, 4>), dim3(T), dim3(512), 0, st, a, s);
+            });
+        });
+        return 0;
+    }
     const RoutePlan plan = route_plan(T, E, H);
     const RouteArgs a = {x, router, (double *)space, T, E, H, plan.splits, plan.chunks};
     const dim3 grid(cdiv(T, 16), cdiv(E, 16 * plan.tn), plan.splits);
@@ -439,8 +527,9 @@ int launch_route(const void *x, int x_dtype, const void *router, int r_dtype, co
             else hipLaunchKernelGGL((route_logits_kernel<AT, RT, 1, 4>), grid, dim3(256), 0, st, a);
         });
     });
-    const ScoreArgs s = {(const double *)space, bias, nullptr, z, w, nullptr, ids, T, E, top_k, plan.splits, 0, sigmoid, renormalize, factor};
-    launch_scores(s, false, st);
+    ScoreArgs parts = s;
+    parts.splits = plan.splits;
+    launch_scores(parts, false, st);
     return 0;
 }
 

@@ -609,8 +609,8 @@ bool plain_route(const Tensor &x, const Tensor &router, const Tensor &bias, cons
         !nothing_watches(router) || x._fw_grad(/*level=*/0).defined() || router._fw_grad(/*level=*/0).defined()) return false;
     if (bias.defined() && (bias.device() != x.device() || bias.dim() != 1 || bias.size(0) != router.size(0) || bias.scalar_type() != at::kFloat ||
                            !nothing_watches(bias))) return false;
-    return rule.top_k >= 1 && rule.top_k <= 64 && rule.top_k <= router.size(0) &&
-           api.route_workspace_bytes(x.size(0), (int)std::min<int64_t>(router.size(0), 1 << 30), x.size(1)) > 0;
+    return rule.top_k >= 1 && rule.top_k <= 64 && rule.top_k <= router.size(0) && x.size(0) <= 1 << 21 && router.size(0) <= 1024 && x.size(1) % 8 == 0 &&
+           x.size(1) <= 1 << 20;                             // (what the library takes)
 }
 
 // the weights as torch operators of logits and choice, for a second derivative
@@ -677,10 +677,10 @@ std::pair<Tensor, Tensor> route(const Tensor &x_in, const Tensor &router_in, con
         ids = at::empty({T, rule.top_k}, x.options().dtype(at::kLong));
         if (wants) logits = at::empty({T, E}, x.options().dtype(at::kDouble));
         const size_t bytes = api.route_workspace_bytes(T, (int)E, H);
-        const Tensor ws = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
+        const Tensor ws = bytes ? at::empty({(int64_t)bytes}, x.options().dtype(at::kByte)) : Tensor();
         check(api.route(x.const_data_ptr(), dtype_code(x.scalar_type()), router.const_data_ptr(), dtype_code(router.scalar_type()),
                         bias.defined() ? bias.const_data_ptr<float>() : nullptr, T, (int)E, H, (int)rule.top_k, rule.sigmoid, rule.renormalize,
-                        (float)rule.factor, w.data_ptr<float>(), ids.data_ptr<int64_t>(), wants ? logits.data_ptr<double>() : nullptr, ws.data_ptr(), bytes,
+                        (float)rule.factor, w.data_ptr<float>(), ids.data_ptr<int64_t>(), wants ? logits.data_ptr<double>() : nullptr, bytes ? ws.data_ptr() : nullptr, bytes,
                         current_stream(x)), "lowbit_route");
     }
     if (wants) {

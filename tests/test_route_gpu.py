@@ -155,6 +155,24 @@ def test_one_expert_has_a_weight_that_nothing_changes(score):
     assert not gx.any() and not gr.any()
 
 
+@pytest.mark.parametrize("e,h", [(1, 8), (4, 1024), (8, 4096), (8, 10240), (13, 2056), (16, 4104), (17, 520), (33, 1032), (64, 512), (64, 1016)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32], ids=ids)
+@pytest.mark.parametrize("biased", [False, True])
+def test_small_routers_choose_as_larger_calls_do(biased, dtype, e, h):
+    """One launch for a few tokens, two for many: sums in float64 in another order, off by some 2^-50, so that the choice is the same and the weights differ by
+    a unit of float32 at most."""
+    from gpu_util import ggml
+    k = min(3, e)
+    x, router, bias = operands(2500, e, h, dtype, dtype)
+    x, router, bias = x.cuda(), router.cuda(), bias.cuda() if biased else None
+    assert ggml._lib.lowbit_route_workspace_bytes(7, e, h) == 0 < ggml._lib.lowbit_route_workspace_bytes(2500, e, h)
+    for score in ("softmax", "sigmoid"):
+        w, index = moe.moe_route(x, router, k, bias, score)
+        for rows in (slice(0, 1), slice(100, 107), slice(2400, 2500)):
+            ws, i = moe.moe_route(x[rows], router, k, bias, score)
+            assert torch.equal(i, index[rows]) and ((ws - w[rows]).abs() <= 2.0 ** -23 * w[rows]).all()
+
+
 def test_leading_dimensions_strides_and_types():
     x, router, bias = operands(24, 20, 128, torch.bfloat16, torch.bfloat16)
     w, index = moe.moe_route(x.cuda(), router.cuda(), 3, bias.cuda())

@@ -120,7 +120,8 @@ def test_experts_router_and_layer_refuse_before_they_touch_the_gpu():
     assert router(hidden=60) == ESHAPE and router(n_exp=1025) == ESIZE and router(top_k=9) == ESIZE and router(top_k=0) == ESIZE
     assert router(n_exp=100, top_k=65) == ESIZE and router(tokens=(1 << 21) + 1) == ESIZE
     assert router(x=P + 4) == EARG and router(bias=P + 2) == EARG and router(z=P + 4) == EARG and router(w=None) == EARG
-    assert router(bytes_=8) == ESIZE and router(ws=None) == ESIZE
+    assert router(n_exp=64, hidden=8192, bytes_=8) == ESIZE and router(n_exp=64, hidden=8192, ws=None) == ESIZE
+    assert lib.lowbit_route_workspace_bytes(2, 8, 64) == 0 < lib.lowbit_route_workspace_bytes(2, 64, 8192)       # (small routers need none)
     assert router(tokens=0, x=None, r=None) == 0
     assert back(P, P, P, P, 1, P, 1, 0, 8, 64, 2, 0, 1, 1.0, P, P, P, 1 << 40, None) == EARG
     assert back(P, None, P, P, 1, P, 1, 2, 8, 64, 2, 0, 1, 1.0, P, P, P, 1 << 40, None) == EARG
