@@ -473,14 +473,14 @@ static RoutePlan route_plan(int T, int E, int H) {
     return p;
 }
 
-// One launch where a workgroup has a token's logits in 3.5 us at most: 512 values of one, two or four rows for each of its waves take 0.17, 0.28 and 0.58, of
+// One launch where a workgroup has a token's logits in 2.5 us at most: 512 values of one, two or four rows for each of its waves take 0.17, 0.28 and 0.58, of
 // which four in five are conversions to float64.  One token x 8 experts of 4096 4.6 us against 8.3 in two launches, 64 of 512 5.5 / 7.9, 64 of 1024 6.1 / 8.0, 64 of
 // 2048 7.7 / 7.8; 1024 tokens x 8 of 1024 5.5 / 8.8, 4096 x 8 of 512 10.3 / 9.5.
 static int small_rows(int E) { return E <= 8 ? 1 : E <= 16 ? 2 : 4; }
 static bool route_small(int T, int E, int H) {
     if (E > SMALL_EXPERTS || T > 2048) return false;
     const int rows = small_rows(E);
-    return cdiv(T, 512) * cdiv(E, 8 * rows) * cdiv(H, 512) * (rows == 1 ? 0.17f : rows == 2 ? 0.28f : 0.58f) <= 3.5f;
+    return cdiv(T, 512) * cdiv(E, 8 * rows) * cdiv(H, 512) * (rows == 1 ? 0.17f : rows == 2 ? 0.28f : 0.58f) <= 2.5f;
 }
 
 size_t route_workspace_bytes(int T, int E, int H) { return route_small(T, E, H) ? 0 : (size_t)route_plan(T, E, H).splits * T * E * sizeof(double); }
