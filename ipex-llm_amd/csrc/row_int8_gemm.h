@@ -344,18 +344,39 @@ __global__ __launch_bounds__(64 * WM * WN * KG, MIN_WAVES) void row_int8_tiled_k
         }
     } else {
         const bool aligned = p.N % 8 == 0;
-        const float *const ws = p.ws + (BY_EXPERT ? (int64_t)expert * p.expert_rows : 0);
+        // the columns' scales and bias, all on their way together
+        float by[TN / 2][8], add[TN / 2][8] = {};
+        if constexpr (MODE == INT8_PLAIN) {
+            const float *const ws = p.ws + (BY_EXPERT ? (int64_t)expert * p.expert_rows : 0);
+            const int first = n0 + wn * TN * 16 + g * 8;
+            if (n0 + BN <= p.N) {
+#pragma unroll
+                for (int t = 0; t < TN / 2; t++) __builtin_memcpy(by[t], ws + first + t * 32, sizeof(by[t]));
+                if (p.bias) {
+                    typedef OT v8 __attribute__((ext_vector_type(8)));
+                    v8 given[TN / 2];
+#pragma unroll
+                    for (int t = 0; t < TN / 2; t++) __builtin_memcpy(&given[t], (const OT *)p.bias + first + t * 32, sizeof(v8));
+#pragma unroll
+                    for (int t = 0; t < TN / 2; t++)
+#pragma unroll
+                        for (int j = 0; j < 8; j++) add[t][j] = (float)given[t][j];
+                }
+            } else {
+#pragma unroll
+                for (int t = 0; t < TN / 2; t++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const int n = first + t * 32 + j < p.N ? first + t * 32 + j : p.N - 1;
+                        by[t][j] = ws[n];
+                        if (p.bias) add[t][j] = (float)((const OT *)p.bias)[n];
+                    }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
 #pragma unroll
         for (int t = 0; t < TN; t += 2) {
             const int n = n0 + wn * TN * 16 + (t >> 1) * 32 + g * 8;
-            float by[8], add[8] = {};
-            if constexpr (MODE == INT8_PLAIN) {
-#pragma unroll
-                for (int j = 0; j < 8; j++) by[j] = n + j < p.N ? ws[n + j] : 0.0f;
-                if (p.bias)
-#pragma unroll
-                    for (int j = 0; j < 8; j++) add[j] = n + j < p.N ? (float)((const OT *)p.bias)[n + j] : 0.0f;
-            }
 #pragma unroll
             for (int i = 0; i < TM; i++) {
                 const int m = m0 + (wm * TM + i) * 16 + r;
@@ -370,7 +391,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, MIN_WAVES) void row_int8_tiled_k
                     typedef OT out_v __attribute__((ext_vector_type(8)));
                     out_v o;
 #pragma unroll
-                    for (int j = 0; j < 8; j++) o[j] = Stored<OT>::of((float)acc[t + j / 4][i][j & 3] * xs[i] * by[j] + add[j]);
+                    for (int j = 0; j < 8; j++) o[j] = Stored<OT>::of((float)acc[t + j / 4][i][j & 3] * xs[i] * by[t / 2][j] + add[t / 2][j]);
                     // (one store of 8 results also where rows of y start at odd places)
                     if (aligned) {
                         if (n < p.N) *(out_v *)to = o;
