@@ -8,7 +8,7 @@
 //
 // Large products are bound by the clock that their data's power leaves: 8192^3 395 us, 2780 TOP/s, at 2.0 GHz with MFMAs on 63 % of the cycles and no
 // LDS conflict, the same launch on codes of zero 311, 3530 TOP/s.  Four waves of 128 x 128 results in instructions of 32 x 32 x 32, which read a third
-// less from LDS, take 471 at 1.87 GHz.  [28672 x 8192] by 8192 rows 1400 to 1480 us, where the library's largest product reaches 2150 TOP/s.  Products of a few hundred
+// less from LDS, take 471 at 1.87 GHz.  [28672 x 8192] by 8192 rows 1400 to 1430 us, where the library's largest product reaches 2150 TOP/s.  Products of a few hundred
 // rows are bound by the latency of a step and by how many CUs have a tile (row_int8_tiled.h).
 #pragma once
 #include "row_int8.h"
