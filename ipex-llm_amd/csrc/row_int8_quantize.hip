@@ -24,7 +24,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void row_int8_quanti
 int launch_row_int8_quantize(const void *x, int dtype, int64_t rows, int K, uint8_t *codes, int ldc, float *scale, const int32_t *limit, hipStream_t st) {
     if (dtype != DT_F16 && dtype != DT_BF16 && dtype != DT_F32) return -4;
     const bool one = K <= 1024;
-    const int64_t most = most_groups(256) * (one ? 4 : 1);
+    constexpr int64_t most = 1 << 22;                        // (of 512 threads each: a grid holds fewer than 2^32)
     for (; rows > most; rows -= most) {                      // (rows that a limit counts are fewer)
         if (int rc = launch_row_int8_quantize(x, dtype, most, K, codes, ldc, scale, limit, st)) return rc;
         x = (const uint8_t *)x + most * K * (dtype == DT_F32 ? 4 : 2);

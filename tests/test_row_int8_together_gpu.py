@@ -293,6 +293,18 @@ def test_a_changed_weight_is_noticed_and_trained_scales_are_refused():
         ri.row_int8_linear(leaf, w, ws)
 
 
+def test_rows_of_several_launches():
+    rows, few = (1 << 22) + 5, 7                                 # a launch takes 2^22
+    x = torch.zeros((rows, 16), dtype=torch.float16, device="cuda")
+    at = torch.cat([torch.arange(few), torch.arange((1 << 22) - few, rows)])
+    given = torch.randn((len(at), 16), generator=gen(24)).half()
+    x[at.cuda()] = given.cuda()
+    codes, scale = ri.row_int8_quantize(x)
+    want, by = u.quantize(given)
+    assert torch.equal(codes[at.cuda()].cpu(), want.to(torch.int8)) and torch.equal(scale[at.cuda()].cpu(), by)
+    assert int(codes.count_nonzero()) == int(want.count_nonzero())
+
+
 # ---------------------------------------------------------------- offsets past 32 bits
 
 def test_weights_of_more_than_2_to_32_codes():
