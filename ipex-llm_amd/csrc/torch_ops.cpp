@@ -499,7 +499,7 @@ static int64_t changes(const Tensor &t) { return t.is_inference() ? 0 : (int64_t
 // The gradient that flows on to x, the quantization of x counting as the identity.  Holds the weight as ProductBackward does.
 struct RowInt8Backward : public torch::autograd::Node {
     Tensor w, scale;
-    int64_t w_changes = 0, scale_changes = 0;                // of the forward
+    int64_t N = 0, K = 0, w_changes = 0, scale_changes = 0;  // of the forward
     at::ScalarType x_dtype = at::kHalf;
     at::DimVector x_shape;
 
@@ -507,11 +507,11 @@ struct RowInt8Backward : public torch::autograd::Node {
 
     torch::autograd::variable_list apply(torch::autograd::variable_list &&grads) override {
         if (!task_should_compute_output(0)) return {Tensor()};
-        const int64_t N = w.size(0), K = w.size(1);
         const Tensor grad = grads[0].defined() ? grads[0].to(x_dtype).reshape({-1, N})
                                                : at::zeros({c10::multiply_integers(x_shape) / K, N}, w.options().dtype(x_dtype));
         c10::DeviceGuard guard(grad.device());
-        if (grad.device() != w.device()) throw Failed("the int8 weight is not where the forward found it");
+        // (a tensor's data may have been replaced, also by some of another size, which counts no change)
+        if (!is_row_int8(w, scale, grad, 0) || w.size(0) != N || w.size(1) != K) throw Failed("the int8 weight is not what the forward found");
         if (changes(w) != w_changes || changes(scale) != scale_changes)
             throw Failed("the int8 weight or its scales have been modified by an inplace operation since the forward");
         if (differentiable(grad) || !nothing_watches(grad))  // (a second derivative, a transform: the dense product)
@@ -539,6 +539,8 @@ Tensor row_int8_linear(const Tensor &x_in, const Tensor &w, const Tensor &scale,
     node->set_next_edges(torch::autograd::collect_next_edges(x_in));
     node->w = w;
     node->scale = scale;
+    node->N = w.size(0);
+    node->K = w.size(1);
     node->w_changes = changes(w);
     node->scale_changes = changes(scale);
     node->x_dtype = x_in.scalar_type();
@@ -623,6 +625,7 @@ Tensor route_weights(const Tensor &x, const Tensor &router, const Tensor &ids, c
 struct RouteBackward : public torch::autograd::Node {
     torch::autograd::SavedVariable x_saved, router_saved;
     Tensor ids, logits;
+    int64_t hidden = 0;
     RouteRule rule{};
 
     std::string name() const override { return "MoeRouteBackward"; }
@@ -635,6 +638,10 @@ struct RouteBackward : public torch::autograd::Node {
 
     torch::autograd::variable_list apply(torch::autograd::variable_list &&grads) override {
         const Tensor x = x_saved.unpack(), router = router_saved.unpack();
+        // (a tensor's data may have been replaced, also by some of another size, which counts no change)
+        if (x.sizes() != at::IntArrayRef({logits.size(0), hidden}) || router.sizes() != at::IntArrayRef({logits.size(1), hidden}) ||
+            x.device() != logits.device() || router.device() != x.device() || dtype_code(x.scalar_type()) < 0 || dtype_code(router.scalar_type()) < 0)
+            throw Failed("the router's operands are not what the forward found");
         const int64_t T = x.size(0), H = x.size(1), E = router.size(0);
         c10::DeviceGuard guard(x.device());
         const Tensor grad = grads[0].defined() ? grads[0] : at::zeros(ids.sizes(), logits.options().dtype(at::kFloat));
@@ -690,6 +697,7 @@ std::pair<Tensor, Tensor> route(const Tensor &x_in, const Tensor &router_in, con
         node->router_saved = torch::autograd::SavedVariable(router_in, /*is_output=*/false);
         node->ids = ids;
         node->logits = logits;
+        node->hidden = H;
         node->rule = rule;
         torch::autograd::set_history(w, node);
     }

@@ -229,6 +229,16 @@ def test_a_changed_operand_is_noticed():
         w.sum().backward()
 
 
+@pytest.mark.parametrize("what", ["rows of the router", "length of its rows", "type"])
+def test_replaced_data_is_noticed(what):
+    x, router, _ = operands(4, 6, 32, torch.float32, torch.float32)
+    xd, rd = x.cuda().requires_grad_(), router.cuda()
+    w, _ = moe.moe_route(xd, rd, 2)
+    rd.data = {"rows of the router": rd[:4].clone(), "length of its rows": rd[:, :16].contiguous(), "type": rd.double()}[what]
+    with pytest.raises(RuntimeError, match="not what the forward found"):
+        w.sum().backward()
+
+
 def test_refusals():
     x, router, bias = (v.cuda() for v in operands(4, 6, 16, torch.float32, torch.float32))
     for call, why in ((lambda: moe.moe_route(x, router, 7), "top_k"), (lambda: moe.moe_route(x, router, 0), "top_k"),

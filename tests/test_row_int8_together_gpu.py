@@ -293,6 +293,24 @@ def test_a_changed_weight_is_noticed_and_trained_scales_are_refused():
         ri.row_int8_linear(leaf, w, ws)
 
 
+@pytest.mark.parametrize("what", ["fewer rows", "shorter rows", "other codes", "other scales"])
+def test_replaced_data_is_noticed(what):
+    g = gen(13)
+    (w, ws), x = u.weight(g, 48, 128), torch.randn((3, 128), generator=g)
+    w, ws, leaf = w.cuda(), ws.cuda(), x.cuda().requires_grad_()
+    y = ri.row_int8_linear(leaf, w, ws)
+    if what == "fewer rows":
+        w.data, ws.data = w[:32].clone(), ws[:32].clone()
+    elif what == "shorter rows":
+        w.data = w[:, :64].contiguous()
+    elif what == "other codes":
+        w.data = w.float()
+    else:
+        ws.data = ws.half()
+    with pytest.raises(RuntimeError, match="not what the forward found"):
+        y.sum().backward()
+
+
 def test_rows_of_several_launches():
     rows, few = (1 << 22) + 5, 7                                 # a launch takes 2^22
     x = torch.zeros((rows, 16), dtype=torch.float16, device="cuda")
