@@ -306,6 +306,8 @@ static Int8BackPlan back_plan(int M, int steps, int K) {
     float least = 0.0f;
     for (int form = 0; form < BACK_COUNT; form++) {
         const Int8BackForm &f = BACK_FORMS[form];
+        // (a tile's rows of g lie within 2^31 bytes, 64 of them whatever their length: from 2^21 columns of float32 on, 2^22 of 16 bits, not 256)
+        if ((int64_t)f.rows * steps * (BACK_STEP * 2) > (int64_t)1 << 31) continue;
         static const int tried[] = {1, 2, 3, 4, 6, 8};
         const int64_t tiles = (int64_t)cdiv(M, f.rows) * cdiv(K, f.cols);
         for (int splits : tried) {

@@ -98,6 +98,15 @@ def test_plans_cover_every_size():
                     assert ggml.lowbit_row_int8_backward_workspace_bytes(dtype, m, n, k) >= m * n * 2 * terms + (splits * m * k * 4 if splits > 1 else 0)
 
 
+@pytest.mark.parametrize("m", [2, 300, 2048, 20000])
+def test_gradient_tiles_of_very_long_rows_stay_within_32_bit_offsets(m):
+    for n in (5000, (1 << 21) - 64, (1 << 21) + 64, (1 << 22) + 1, (1 << 23) - 1):
+        for dtype, size in ((0, 2), (1, 2), (2, 4)):
+            for k in (16, 1024, 4096):
+                rows = ggml.lowbit_row_int8_plan(dtype, 1, m, n, k)[0]
+                assert rows * ((n + 63) // 64 * 64) * size <= 1 << 31
+
+
 def test_experts_router_and_layer_refuse_before_they_touch_the_gpu():
     ex, route, back, layer = lib.lowbit_row_int8_experts, lib.lowbit_route, lib.lowbit_route_backward, lib.lowbit_row_int8_moe
 
