@@ -75,7 +75,7 @@ def moe_route(x: torch.Tensor, router: torch.Tensor, top_k: int, bias: torch.Ten
             return both if x.dim() == 2 else tuple(t.view(*x.shape[:-1], top_k) for t in both)
     _check_route(x, router, top_k, bias, score, "moe_route")
     if x.numel() == 0:
-        return (x.float().sum(-1, keepdim=True) * 0 + torch.zeros(top_k, device=x.device),
+        return (x.float().sum(-1, keepdim=True) + router[:0].float().sum() + torch.zeros(top_k, device=x.device),     # (carries the gradients)
                 torch.zeros((*x.shape[:-1], top_k), dtype=torch.int64, device=x.device))
     return _route_steps(x, router, top_k, bias, score, renormalize, scale)
 

@@ -100,7 +100,8 @@ def row_int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.T
     invalidInputError(x.dim() >= 1 and x.shape[-1] == k, f"{what}: x has rows of {x.shape[-1] if x.dim() else 0} values, the weight of {k}")
     _check_bias(bias, n, x, what)
     if x.numel() == 0:
-        return x.new_empty((*x.shape[:-1], n)) + x.sum() * 0
+        y = x.new_empty((*x.shape[:-1], n)) + x.sum()        # (carries the gradients)
+        return y if bias is None else y + bias[:0].sum().to(x.dtype)
     if bias is not None and bias.dtype == x.dtype:           # strided, or one that wants a gradient itself
         fixed = bias.detach().contiguous()
         y = ops.row_int8_linear(x, weight, weight_scale, fixed)
@@ -219,7 +220,7 @@ def row_int8_moe(x: torch.Tensor, router: torch.Tensor, top_k: int, gate_up: tor
     _check_route(x, router, top_k, bias, score, what)
     invalidInputError(router.shape[0] == gate_up.shape[0], f"{what}: the router has {router.shape[0]} rows for {gate_up.shape[0]} experts")
     if x.numel() == 0:
-        return x * 0
+        return x + router[:0].sum().to(x.dtype)              # (carries the gradients)
     weights, index = moe_route(x, router, top_k, bias, score, renormalize, scale)
     return row_int8_experts(x, index, weights, gate_up, gate_up_scale, down, down_scale, act)
 
@@ -333,7 +334,7 @@ class RowInt8Experts(_KeepsFormat):
     def forward(self, hidden_states, top_k_index, top_k_weights):
         from ipex_llm.transformers.moe import activation_code
         if top_k_index.shape[0] == 0:
-            return torch.zeros_like(hidden_states)
+            return torch.zeros_like(hidden_states) + (hidden_states[:0].sum() + top_k_weights[:0].sum().to(hidden_states.dtype))
         weights = (self.gate_up_proj, self.gate_up_proj_scale, self.down_proj, self.down_proj_scale)
         act = activation_code(self.act_fn)
         if act is None or self.own_gate is not None:

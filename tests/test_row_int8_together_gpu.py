@@ -278,6 +278,22 @@ def test_second_derivative_tangent_and_transforms():
     assert (each - plain).norm() <= 1e-5 * plain.norm()
 
 
+def test_no_rows_carry_gradients_of_zero():
+    g = gen(14)
+    x = torch.empty((0, 64), dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    router = torch.randn((4, 64), generator=g).cuda().requires_grad_()
+    bias = torch.randn(32, generator=g).to(torch.bfloat16).cuda().requires_grad_()
+    (w, ws), (gu, gus), (d, ds) = (tuple(t.cuda() for t in u.weight(g, n, k, lead)) for n, k, lead in ((32, 64, ()), (96, 64, (4,)), (64, 48, (4,))))
+    p, index = moe.moe_route(x, router, 2)
+    experts = ri.RowInt8Experts(4, 64, 48, torch.nn.functional.silu)
+    for out, shape, leaves in ((ri.row_int8_linear(x, w, ws, bias), (0, 32), (x, bias)), (p, (0, 2), (x, router)),
+                               (ri.row_int8_experts(x, index, p, gu, gus, d, ds), (0, 64), (x, router)), (experts(x, index, p), (0, 64), (x, router)),
+                               (ri.row_int8_moe(x, router, 2, gu, gus, d, ds), (0, 64), (x, router))):
+        assert out.shape == shape
+        for leaf, grad in zip(leaves, torch.autograd.grad(out.sum(), leaves, retain_graph=True)):
+            assert grad.shape == leaf.shape and not grad.any()
+
+
 def test_a_changed_weight_is_noticed_and_trained_scales_are_refused():
     g = gen(12)
     (w, ws), x = u.weight(g, 32, 128), torch.randn((3, 128), generator=g)
