@@ -341,23 +341,25 @@ template <int NR> __global__ __launch_bounds__(256) void route_grad_kernel(const
 //
 // A lane of B loads eight neighbours of a row, which are its column of eight tiles, so that a wave owns 128 columns and a lane stores
 // eight neighbours of a row of C.  ACROSS: A(m, k) = dz[k, m], the gradient of the router, whose waves take the rows k in turn and add their
-// sums in LDS, in order; else A(m, k) = dz[m, k], the gradient of x, whose waves take 128 columns each.  1000 tokens x 60 experts of 4096: router 14.3 us and
-// the splits' sum 3.8, x 10.9, the gradient of the logits 4.2; loads a step ahead make it 15.3 and 13.0.
+// sums in LDS, in order; else A(m, k) = dz[m, k], the gradient of x, whose waves take 128 columns each.  1000 tokens x 60 experts of 4096: both in one
+// launch 19.7 us (alone 13.8 and 10.8, which loads a step ahead make 15.3 and 13.0), the splits' sum 3.5, the gradient of the logits 5.4; 2000 x 160 of 1024 24.6
+// (17.7 and 18.5).
 struct OuterArgs {
     const float *dz;                                         // [T, lde]
     const void *b;                                           // [K, H]
     void *c;                                                 // [M, H]
     float *part;                                             // ACROSS, several splits: [split][M][H]
     int M, K, H, lde, splits, steps;                         // steps of 16 rows k per split
+    uint32_t groups_h, groups_m, groups;                     // workgroups along H, along M, in all
 };
 
 template <typename BT, typename CT, int TM, bool ACROSS>
-__global__ __launch_bounds__(256, 2) void route_outer_kernel(const OuterArgs p) {
+__device__ __forceinline__ void route_outer(const OuterArgs &p, float *sums, uint32_t at) {
     using B8 = typename Octet<BT>::type;
-    __shared__ float sums[ACROSS ? 64 * (TM * 32 + 1) : 1];
+    const int at_h = at % p.groups_h, at_m = at / p.groups_h % p.groups_m, split = at / p.groups_h / p.groups_m;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
-    const int h = (ACROSS ? blockIdx.x : blockIdx.x * 4 + wave) * 128 + r * 8, m0 = blockIdx.y * 16 * TM;
-    const int all = (p.K + 15) / 16, first = ACROSS ? blockIdx.z * p.steps : 0, last = ACROSS && first + p.steps < all ? first + p.steps : all;
+    const int h = (ACROSS ? at_h : at_h * 4 + wave) * 128 + r * 8, m0 = at_m * 16 * TM;
+    const int all = (p.K + 15) / 16, first = ACROSS ? split * p.steps : 0, last = ACROSS && first + p.steps < all ? first + p.steps : all;
     const BT *const b = (const BT *)p.b + (h < p.H ? h : 0);
     f32x4 acc[TM][8] = {};
     for (int s = ACROSS ? first + wave : first; s < last; s += ACROSS ? 4 : 1) {
@@ -417,7 +419,7 @@ __global__ __launch_bounds__(256, 2) void route_outer_kernel(const OuterArgs p) 
             const int m = m0 + i * 16 + g * 4 + q;
             if (m >= p.M) continue;
             if (ACROSS && p.splits > 1) {
-                float *const to = p.part + ((int64_t)blockIdx.z * p.M + m) * p.H + h;
+                float *const to = p.part + ((int64_t)split * p.M + m) * p.H + h;
 #pragma unroll
                 for (int v = 0; v < 2; v++) *(f32x4 *)(to + 4 * v) = f32x4{acc[i][4 * v][q], acc[i][4 * v + 1][q], acc[i][4 * v + 2][q], acc[i][4 * v + 3][q]};
             } else {
@@ -428,6 +430,14 @@ __global__ __launch_bounds__(256, 2) void route_outer_kernel(const OuterArgs p) 
                 *(out8 *)((CT *)p.c + (int64_t)m * p.H + h) = o;
             }
         }
+}
+
+// Both gradients in one launch, the router's workgroups first, which take longer; either may have none.
+constexpr int OUTER_TM = 4, OUTER_X_TM = 2;
+template <typename XT, typename RT> __global__ __launch_bounds__(256, 2) void route_outer_kernel(const OuterArgs of_router, const OuterArgs of_x) {
+    __shared__ float sums[64 * (OUTER_TM * 32 + 1)];
+    if (blockIdx.x < of_router.groups) route_outer<XT, RT, OUTER_TM, true>(of_router, sums, blockIdx.x);
+    else route_outer<RT, XT, OUTER_X_TM, false>(of_x, sums, blockIdx.x - of_router.groups);
 }
 
 // the splits' sums in their order, rounded once; four values per thread
@@ -535,7 +545,6 @@ int launch_route(const void *x, int x_dtype, const void *router, int r_dtype, co
 
 // Splits of T for the gradient of the router: at most 512 rows for each of a workgroup's four waves, so that a float32 sum rounds little, and a few
 // hundred workgroups.
-constexpr int OUTER_TM = 4;
 static int outer_steps(int T, int E, int H) {
     const int tiles = cdiv(H, 128) * cdiv(E, 16 * OUTER_TM), all = cdiv(T, 16);
     int splits = tiles < 512 ? 512 / tiles : 1;
@@ -565,35 +574,25 @@ int launch_route_backward(const float *grad, const double *z, const int64_t *ids
     const int lde = router_columns(E);
     const ScoreArgs s = {nullptr, nullptr, grad, (double *)z, nullptr, (float *)space, (int64_t *)ids, T, E, top_k, 1, lde, sigmoid, renormalize, factor};
     launch_scores(s, true, st);
-    if (gx) {
-        OuterArgs a = {(const float *)space, router, gx, nullptr, T, E, H, lde, 1, 0};
-        by_type(x_dtype, [&](auto *xt) {
-            by_type(r_dtype, [&](auto *rt) {
-                using CT = typename std::remove_pointer<decltype(xt)>::type;
-                using BT = typename std::remove_pointer<decltype(rt)>::type;
-                for (int m = 0; m < T; m += 65535 * 32) {
-                    a.M = T - m < 65535 * 32 ? T - m : 65535 * 32;
-                    a.dz = (const float *)space + (int64_t)m * lde;
-                    a.c = (CT *)gx + (int64_t)m * H;
-                    hipLaunchKernelGGL((route_outer_kernel<BT, CT, 2, false>), dim3(cdiv(H, 512), cdiv(a.M, 32)), dim3(256), 0, st, a);
-                }
-            });
+    OuterArgs r = {(const float *)space, x, gr, (float *)(space + at.part), E, T, H, lde, at.splits, outer_steps(T, E, H), (uint32_t)cdiv(H, 128),
+                   (uint32_t)cdiv(E, 16 * OUTER_TM), 0};
+    OuterArgs o = {(const float *)space, router, gx, nullptr, T, E, H, lde, 1, 0, (uint32_t)cdiv(H, 512), (uint32_t)cdiv(T, 16 * OUTER_X_TM), 0};
+    const int64_t of_router = gr ? (int64_t)r.groups_h * r.groups_m * at.splits : 0, of_x = gx ? (int64_t)o.groups_h * o.groups_m : 0;
+    if (of_router + of_x > most_groups(256)) return -3;
+    if (of_router + of_x == 0) return 0;
+    r.groups = (uint32_t)of_router;
+    o.groups = (uint32_t)of_x;
+    by_type(x_dtype, [&](auto *xt) {
+        by_type(r_dtype, [&](auto *rt) {
+            using XT = typename std::remove_pointer<decltype(xt)>::type;
+            using RT = typename std::remove_pointer<decltype(rt)>::type;
+            hipLaunchKernelGGL((route_outer_kernel<XT, RT>), dim3(r.groups + o.groups), dim3(256), 0, st, r, o);
+            const int64_t quads = (int64_t)E * H / 4;
+            if (gr && at.splits > 1)
+                hipLaunchKernelGGL((route_outer_reduce_kernel<RT>), dim3((uint32_t)((quads + 255) / 256)), dim3(256), 0, st, (const f32x4 *)r.part, (RT *)gr, quads,
+                                   at.splits);
         });
-    }
-    if (gr) {
-        const OuterArgs a = {(const float *)space, x, gr, (float *)(space + at.part), E, T, H, lde, at.splits, outer_steps(T, E, H)};
-        by_type(x_dtype, [&](auto *xt) {
-            by_type(r_dtype, [&](auto *rt) {
-                using BT = typename std::remove_pointer<decltype(xt)>::type;
-                using CT = typename std::remove_pointer<decltype(rt)>::type;
-                hipLaunchKernelGGL((route_outer_kernel<BT, CT, OUTER_TM, true>), dim3(cdiv(H, 128), cdiv(E, 16 * OUTER_TM), at.splits), dim3(256), 0, st, a);
-                const int64_t quads = (int64_t)E * H / 4;
-                if (at.splits > 1)
-                    hipLaunchKernelGGL((route_outer_reduce_kernel<CT>), dim3((uint32_t)((quads + 255) / 256)), dim3(256), 0, st, (const f32x4 *)a.part, (CT *)gr,
-                                       quads, at.splits);
-            });
-        });
-    }
+    });
     return 0;
 }
 
