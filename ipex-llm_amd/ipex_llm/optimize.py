@@ -23,8 +23,11 @@ def _save_low_bit(self, save_dir, *args, **kwargs):
     # blobs are written in the ggml layout: GPU-resident weights go back through .to("cpu")
     state = {k: v.detach().to("cpu") for k, v in _cpu_state(self).items()}
     torch.save(state, os.path.join(save_dir, PYTORCH_MODEL_NAME))
+    config = dict(self._bigdl_config)
+    if config["bigdl_transformers_low_bit"] == "sym_int8":
+        config["row_int8_layers"] = row_int8_modules(self)
     with open(os.path.join(save_dir, CONFIG_NAME), "w") as json_file:
-        json.dump(self._bigdl_config, json_file)
+        json.dump(config, json_file)
 
 
 def _cpu_state(model):
@@ -96,12 +99,38 @@ def block_fp8_layers(state_dict):
     return names, any(n.endswith("q_proj") for n in names)
 
 
-def row_int8_layers(state_dict, low_bit):
-    """Module names whose saved weights are int8 codes with a scale for each row (a model saved as sym_int8)."""
+def row_int8_modules(model):
+    """Names of a model's modules in row-scaled int8: what a saved sym_int8 model lists, since a layer of a checkpoint that was left out of
+    the conversion may hold tensors of the same names."""
+    from ipex_llm.transformers.row_int8 import RowInt8Experts, RowInt8Linear
+    return [n for n, m in model.named_modules() if isinstance(m, (RowInt8Linear, RowInt8Experts))]
+
+
+def row_int8_layers(state_dict, low_bit, listed=None):
+    """Module names whose saved weights are int8 codes with a scale for each row (a model saved as sym_int8): those that the saved model lists.
+    Where it has no list, those that hold what a converted one does: a float32 scale for each row, and a bias at most."""
     if low_bit != "sym_int8":
         return set()
-    return {k[:-len("." + w)] for w in ("weight", "gate_up_proj") for k, v in state_dict.items()
-            if k.endswith("." + w) and v.dtype == torch.int8 and k + "_scale" in state_dict}
+    if listed is not None:
+        return set(listed)
+    own, names = {}, set()
+    for k in state_dict:
+        name, _, leaf = k.rpartition(".")
+        own.setdefault(name, set()).add(leaf)
+    for name, leaves in own.items():
+        weights = [w for w in ("weight", "gate_up_proj", "down_proj") if w in leaves]
+        held = [(state_dict[f"{name}.{w}"], state_dict.get(f"{name}.{w}_scale")) for w in weights]
+        if weights in (["weight"], ["gate_up_proj", "down_proj"]) and leaves <= {"bias", *weights, *(w + "_scale" for w in weights)} and \
+                all(w.dtype == torch.int8 and s is not None and s.dtype == torch.float32 and s.shape == w.shape[:-1] for w, s in held):
+            names.add(name)
+    return names
+
+
+def left_out_int8(state_dict, rows):
+    """Names of experts in int8 codes with scales that are not among the converted ones (`rows`): they were left out of the conversion, as
+    unconverted_linears' were."""
+    return sorted({k.rpartition(".")[0] for k, v in state_dict.items() if k.endswith((".gate_up_proj", ".down_proj")) and v.dtype == torch.int8
+                   and k + "_scale" in state_dict} - set(rows))
 
 
 def unmerged_attentions(state_dict):
@@ -119,9 +148,10 @@ def load_low_bit(model, model_path):
     if low_bit:
         from ipex_llm.transformers.convert import ggml_convert_low_bit
         qtype = ggml_tensor_qtype[low_bit]
-        rows = row_int8_layers(state_dict, low_bit)
-        model = ggml_convert_low_bit(model, qtype=qtype, convert_shape_only=True,
-                                     modules_to_not_convert=[n for n in unconverted_linears(state_dict) if n not in rows],
+        with open(os.path.join(model_path, CONFIG_NAME)) as f:
+            rows = row_int8_layers(state_dict, low_bit, json.load(f).get("row_int8_layers"))
+        skip = [n for n in unconverted_linears(state_dict) if n not in rows] + left_out_int8(state_dict, rows)
+        model = ggml_convert_low_bit(model, qtype=qtype, convert_shape_only=True, modules_to_not_convert=skip,
                                      keep_apart=unmerged_attentions(state_dict), block_fp8=block_fp8_layers(state_dict)[0], row_int8=rows)
     for param_name, param in state_dict.items():
         _assign(model, param_name, param)

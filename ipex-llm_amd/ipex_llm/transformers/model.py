@@ -29,7 +29,7 @@ def save_low_bit(self, *args, **kwargs):
                       " load_in_4bit or load_in_low_bit parameter to load a 4-bit model first.")
     save_dir = args[0] if args else kwargs["save_directory"]
     os.makedirs(save_dir, exist_ok=True)
-    from ipex_llm.optimize import _cpu_state
+    from ipex_llm.optimize import _cpu_state, row_int8_modules
     state = {k: v.detach().to("cpu").contiguous() for k, v in _cpu_state(self).items()}
     self.config.save_pretrained(save_dir)
     if getattr(self, "generation_config", None) is not None:
@@ -38,8 +38,11 @@ def save_low_bit(self, *args, **kwargs):
         except Exception:  # noqa: BLE001
             pass
     torch.save(state, os.path.join(save_dir, PYTORCH_MODEL_NAME))
+    keys = {"all_checkpoint_keys": list(state.keys())}
+    if self.config.bigdl_transformers_low_bit == "sym_int8":
+        keys["row_int8_layers"] = row_int8_modules(self)
     with open(os.path.join(save_dir, "load_keys.json"), "w") as json_file:
-        json.dump({"all_checkpoint_keys": list(state.keys())}, json_file)
+        json.dump(keys, json_file)
 
 
 def _release_quantizer(model):
@@ -186,22 +189,23 @@ class _BaseAutoModelClass:
                           " serialize the model using save_low_bit first.")
         invalidInputError(low_bit in ggml_tensor_qtype, f"Unknown bigdl_transformers_low_bit value: {low_bit}")
         qtype = ggml_tensor_qtype[low_bit]
-        from ipex_llm.optimize import block_fp8_layers, row_int8_layers, unconverted_linears, unmerged_attentions
+        from ipex_llm.optimize import block_fp8_layers, left_out_int8, row_int8_layers, unconverted_linears, unmerged_attentions
         state_dict = torch.load(os.path.join(pretrained_model_name_or_path, PYTORCH_MODEL_NAME),
                                 weights_only=True)
         with torch.device("meta"):
             model = cls.HF_Model.from_config(config)
-        rows = row_int8_layers(state_dict, low_bit)
-        skip = list(modules_to_not_convert or []) + [n for n in unconverted_linears(state_dict) if n not in rows]
+        keys_file, keys = os.path.join(pretrained_model_name_or_path, "load_keys.json"), {}
+        if os.path.isfile(keys_file):
+            with open(keys_file) as f:
+                keys = json.load(f)
+        rows = row_int8_layers(state_dict, low_bit, keys.get("row_int8_layers"))
+        skip = list(modules_to_not_convert or []) + [n for n in unconverted_linears(state_dict) if n not in rows] + left_out_int8(state_dict, rows)
         model = ggml_convert_low_bit(model, qtype, optimize_model, device="meta",
                                      convert_shape_only=True, modules_to_not_convert=skip,
                                      embedding_qtype=embedding_qtype, keep_apart=unmerged_attentions(state_dict),
                                      block_fp8=block_fp8_layers(state_dict)[0], row_int8=rows)
-        keys_file = os.path.join(pretrained_model_name_or_path, "load_keys.json")
-        if os.path.isfile(keys_file):
-            with open(keys_file) as f:
-                expected = json.load(f)["all_checkpoint_keys"]
-            invalidInputError(set(expected) == set(state_dict.keys()),
+        if keys:
+            invalidInputError(set(keys["all_checkpoint_keys"]) == set(state_dict.keys()),
                               "pytorch_model.bin does not hold the keys listed in load_keys.json")
         for name, tensor in state_dict.items():
             _assign(model, name, tensor)

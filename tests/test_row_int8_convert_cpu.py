@@ -222,3 +222,53 @@ def test_layers_left_out_of_another_format_stay_left_out(tmp_path):
     want.save_low_bit(str(tmp_path))
     again = load_low_bit(model(), str(tmp_path))
     assert type(again["left"]) is nn.Linear and again["left"].weight.dtype == torch.int8 and torch.equal(again["left"].weight, want["left"].weight)
+
+
+LEFT_OUT = {
+    "a column of scales": lambda: scaled_linear(32, 128, column=True),
+    "a row of scales": lambda: scaled_linear(32, 128, True),
+    "16-bit scales": lambda: scaled_linear(32, 128, dtype=torch.float16),
+    "fixed scale of the activations": lambda: held(scaled_linear(32, 128), activation_scheme="static"),
+    "zero points": lambda: held(scaled_linear(32, 128), weight_zero_point=torch.zeros(32)),
+    "experts": lambda: FusedExperts(2, 64, 32),
+    "experts with columns": lambda: FusedExperts(2, 64, 32, column=True),
+}
+
+
+def saved_and_loaded(model, folder, **kwargs):
+    want = optimize_model(model(), "sym_int8", modules_to_not_convert=["left"], **kwargs)
+    want.save_low_bit(str(folder))
+    return want, lambda: load_low_bit(model(), str(folder))
+
+
+@pytest.mark.parametrize("what", LEFT_OUT)
+def test_layers_left_out_of_a_sym_int8_model_stay_left_out(what, tmp_path):
+    """A checkpoint's int8 layers, some of them left out of the conversion: as they were after a model is saved and loaded, also where they hold the
+    tensors of a converted one."""
+    want, load = saved_and_loaded(lambda: nn.ModuleDict({"left": LEFT_OUT[what](), "other": scaled_linear(32, 64), "experts": FusedExperts(2, 64, 32)}).eval(),
+                                  tmp_path)
+    again = load()
+    assert type(again["left"]) is type(LEFT_OUT[what]()) and type(again["other"]) is ri.RowInt8Linear and type(again["experts"]) is ri.RowInt8Experts
+    assert want.state_dict().keys() == again.state_dict().keys()
+    for name, v in want.state_dict().items():
+        assert torch.equal(again.state_dict()[name], v) and again.state_dict()[name].dtype == v.dtype, name
+
+
+@pytest.mark.parametrize("what", ["a column of scales", "zero points", "experts with columns"])
+def test_models_saved_without_a_list_of_layers_load(what, tmp_path):
+    """What no converted layer holds was left out."""
+    import json
+    _, load = saved_and_loaded(lambda: nn.ModuleDict({"left": LEFT_OUT[what](), "other": scaled_linear(32, 64, True), "experts": FusedExperts(2, 64, 32)}).eval(),
+                               tmp_path)
+    config = json.loads((tmp_path / "bigdl_config.json").read_text())
+    assert config.pop("row_int8_layers") == ["other", "experts"]
+    (tmp_path / "bigdl_config.json").write_text(json.dumps(config))
+    again = load()
+    assert type(again["left"]) is type(LEFT_OUT[what]()) and type(again["other"]) is ri.RowInt8Linear and type(again["experts"]) is ri.RowInt8Experts
+
+
+def test_a_list_of_layers_goes_before_what_they_hold():
+    state = {"low.weight": torch.zeros(8, dtype=torch.uint8), "left.weight": torch.zeros(4, 4), "q.weight": torch.zeros((4, 16), dtype=torch.int8),
+             "q.weight_scale": torch.zeros(4)}
+    assert row_int8_layers(state, "sym_int8") == {"q"} and row_int8_layers(state, "sym_int8", []) == set()
+    assert row_int8_layers(state, "sym_int8", ["q"]) == {"q"} and row_int8_layers(state, "bf16", ["q"]) == set()
