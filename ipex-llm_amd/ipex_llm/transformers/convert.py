@@ -468,15 +468,20 @@ def ggml_convert_low_bit(model, qtype, optimize_model=True,
 
 
 def convert_bigdl_other_module(model, dtype):
-    """Every leaf that is not one of our linears follows `dtype` (convert.py:1174-1182).  One that holds 8-bit floating point codes, a layer
-    of a checkpoint that was left out of the conversion, keeps them: as numbers of another type they would have lost their scales."""
+    """Every leaf that is not one of our linears follows `dtype` (convert.py:1174-1182).  One that holds 8-bit codes, a layer of a checkpoint that was
+    left out of the conversion, keeps them and their scales: as numbers of another type those would be others.  Of one in int8 the bias follows."""
     from ipex_llm.transformers.block_fp8 import BlockFP8Linear
     from ipex_llm.transformers.low_bit_linear import BF16Linear, FP16Linear, LowBitLinear
     from ipex_llm.transformers.row_int8 import RowInt8Linear
     for module in model.modules():
         if list(module.children()) == []:
             codes = any(p.is_floating_point() and p.element_size() == 1 for p in module.parameters(recurse=False))
-            if not codes and not isinstance(module, (LowBitLinear, FP16Linear, BF16Linear, BlockFP8Linear, RowInt8Linear)):
+            if codes or isinstance(module, (LowBitLinear, FP16Linear, BF16Linear, BlockFP8Linear, RowInt8Linear)):
+                continue
+            if any(is_row_int8(module, n) for n in ("weight", "gate_up_proj", "down_proj")):
+                if module._parameters.get("bias") is not None:
+                    module.bias.data = module.bias.data.to(dtype)
+            else:
                 module.to(dtype)
 
 

@@ -272,3 +272,29 @@ def test_a_list_of_layers_goes_before_what_they_hold():
              "q.weight_scale": torch.zeros(4)}
     assert row_int8_layers(state, "sym_int8") == {"q"} and row_int8_layers(state, "sym_int8", []) == set()
     assert row_int8_layers(state, "sym_int8", ["q"]) == {"q"} and row_int8_layers(state, "bf16", ["q"]) == set()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+def test_layers_left_out_of_the_conversion_keep_their_scales(dtype, tmp_path):
+    """Scales that 16 bits do not hold, of a linear, of one with fixed scales of its activations and zero points, and of experts with and without a
+    module for their gate."""
+    def model():
+        def small(module):
+            for name, p in module.named_parameters():
+                if name.endswith("_scale"):
+                    p.data = torch.arange(1, p.numel() + 1).view(p.shape) * 1.234567e-8
+            return module
+        bare = FusedExperts(2, 64, 32)
+        bare.act_fn = None
+        del bare._modules["act_fn"]
+        static = held(scaled_linear(32, 128), input_scale=torch.tensor([1.234567e-3]), weight_zero_point=torch.full((32,), 0.1))
+        return nn.ModuleDict({"left": small(scaled_linear(32, 128, True)), "left_static": small(static), "left_experts": small(FusedExperts(2, 64, 32)),
+                              "left_bare": small(bare), "other": scaled_linear(32, 64), "norm": nn.LayerNorm(64)}).eval()
+    before = model()
+    after = optimize_model(model(), "sym_int8", modules_to_not_convert=["left"], torch_dtype=dtype)
+    assert after["norm"].weight.dtype == dtype and type(after["other"]) is ri.RowInt8Linear and after["left"].bias.dtype == dtype
+    after.save_low_bit(str(tmp_path))
+    for m in (after, load_low_bit(model(), str(tmp_path))):
+        for name, v in before.state_dict().items():
+            if name.startswith("left") and not name.endswith("bias"):
+                assert m.state_dict()[name].dtype == v.dtype and torch.equal(m.state_dict()[name], v), name
