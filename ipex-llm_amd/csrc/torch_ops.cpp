@@ -623,8 +623,8 @@ Tensor route_weights(const Tensor &x, const Tensor &router, const Tensor &ids, c
 }
 
 struct RouteBackward : public torch::autograd::Node {
-    torch::autograd::SavedVariable x_saved, router_saved;
-    Tensor ids, logits;
+    torch::autograd::SavedVariable x_saved, router_saved, ids_saved;         // (the ids are the caller's too, who may change them)
+    Tensor logits;
     int64_t hidden = 0;
     RouteRule rule{};
 
@@ -632,16 +632,18 @@ struct RouteBackward : public torch::autograd::Node {
     void release_variables() override {
         x_saved.reset_data();
         router_saved.reset_data();
-        ids.reset();
+        ids_saved.reset_data();
         logits.reset();
     }
 
     torch::autograd::variable_list apply(torch::autograd::variable_list &&grads) override {
-        const Tensor x = x_saved.unpack(), router = router_saved.unpack();
+        const Tensor x = x_saved.unpack(), router = router_saved.unpack(), ids = ids_saved.unpack();
         // (a tensor's data may have been replaced, also by some of another size, which counts no change)
         if (x.sizes() != at::IntArrayRef({logits.size(0), hidden}) || router.sizes() != at::IntArrayRef({logits.size(1), hidden}) ||
             x.device() != logits.device() || router.device() != x.device() || dtype_code(x.scalar_type()) < 0 || dtype_code(router.scalar_type()) < 0)
             throw Failed("the router's operands are not what the forward found");
+        if (ids.sizes() != at::IntArrayRef({logits.size(0), rule.top_k}) || ids.scalar_type() != at::kLong || ids.device() != x.device() || !ids.is_contiguous())
+            throw Failed("the indices of the router are not what the forward found");
         const int64_t T = x.size(0), H = x.size(1), E = router.size(0);
         c10::DeviceGuard guard(x.device());
         const Tensor grad = grads[0].defined() ? grads[0] : at::zeros(ids.sizes(), logits.options().dtype(at::kFloat));
@@ -695,7 +697,7 @@ std::pair<Tensor, Tensor> route(const Tensor &x_in, const Tensor &router_in, con
         node->set_next_edges(torch::autograd::collect_next_edges(x_in, router_in));
         node->x_saved = torch::autograd::SavedVariable(x_in, /*is_output=*/false);
         node->router_saved = torch::autograd::SavedVariable(router_in, /*is_output=*/false);
-        node->ids = ids;
+        node->ids_saved = torch::autograd::SavedVariable(ids, /*is_output=*/false);
         node->logits = logits;
         node->hidden = H;
         node->rule = rule;

@@ -248,3 +248,27 @@ def test_refusals():
                       (lambda: moe.moe_route(x.cpu(), router, 2), "no CPU implementation"), (lambda: moe.moe_route(x, router.cpu(), 2), "one GPU")):
         with pytest.raises(RuntimeError, match=why):
             call()
+
+
+@pytest.mark.parametrize("how", ["in place", "under no_grad", "through a view", "fewer of them", "another type"])
+def test_changed_indices_are_noticed(how):
+    """The weights' gradient goes by the choice: where a caller has changed the returned indices since (tokens dropped, an offset added) it is refused, as a
+    changed operand is; a changed copy is the caller's own."""
+    x, router, _ = operands(8, 6, 16, torch.float32, torch.float32)
+    xd, rd, g = x.cuda().requires_grad_(), router.cuda().requires_grad_(), torch.randn((8, 2), generator=gen(3)).cuda()
+    w, index = moe.moe_route(xd, rd, 2)
+    want = torch.autograd.grad(w, (xd, rd), g)
+    w, index = moe.moe_route(xd.view(2, 4, 16) if how == "through a view" else xd, rd, 2)
+    copied = index.clone()
+    copied[1] = -1
+    got = torch.autograd.grad(w, (xd, rd), g.view(w.shape), retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    if how == "fewer of them":
+        index.data = index[:, :1].contiguous()
+    elif how == "another type":
+        index.data = index.int()
+    else:
+        with torch.set_grad_enabled(how != "under no_grad"):
+            index[..., 0] = (index[..., 0] + 1) % 6
+    with pytest.raises(RuntimeError, match="indices.*not what the forward found" if how in ("fewer of them", "another type") else "modified by an inplace operation"):
+        torch.autograd.grad(w, (xd, rd), g.view(w.shape))
