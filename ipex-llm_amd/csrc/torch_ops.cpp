@@ -13,7 +13,6 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
-#include <torch/csrc/autograd/autograd.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <ATen/ATen.h>
@@ -615,13 +614,6 @@ bool plain_route(const Tensor &x, const Tensor &router, const Tensor &bias, cons
            x.size(1) <= 1 << 20;                             // (what the library takes)
 }
 
-// the weights as torch operators of logits and choice, for a second derivative
-Tensor route_weights(const Tensor &x, const Tensor &router, const Tensor &ids, const RouteRule &rule) {
-    const Tensor z = at::matmul(x.to(at::kDouble), router.to(at::kDouble).t());
-    const Tensor c = (rule.sigmoid ? z.sigmoid() : z.softmax(-1)).gather(1, ids);
-    return ((rule.renormalize ? c / c.sum(-1, true) : c) * rule.factor).to(at::kFloat);
-}
-
 struct RouteBackward : public torch::autograd::Node {
     torch::autograd::SavedVariable x_saved, router_saved, ids_saved;         // (the ids are the caller's too, who may change them)
     Tensor logits;
@@ -650,15 +642,17 @@ struct RouteBackward : public torch::autograd::Node {
         const bool want_x = task_should_compute_output(0), want_r = task_should_compute_output(1);
         if (!want_x && !want_r) return {Tensor(), Tensor()};
         if (differentiable(grad) || !nothing_watches(grad) || c10::GradMode::is_enabled()) {
-            c10::AutoGradMode enabled(true);                 // (a second derivative, a transform: torch operators)
-            const bool create = differentiable(grad) || differentiable(x) || differentiable(router);
-            const Tensor xl = want_x && !x.requires_grad() ? x.detach().requires_grad_() : x, rl = want_r && !router.requires_grad() ? router.detach().requires_grad_() : router;
-            const Tensor w = route_weights(xl, rl, ids, rule);
-            torch::autograd::variable_list inputs;
-            if (want_x) inputs.push_back(xl);
-            if (want_r) inputs.push_back(rl);
-            auto g = torch::autograd::grad({w}, inputs, {grad}, /*retain_graph=*/true, create, /*allow_unused=*/false);
-            return {want_x ? g[0] : Tensor(), want_r ? g[want_x ? 1 : 0] : Tensor()};
+            // A second derivative, a transform: the gradient's formula (route.hip) in torch operators on the caller's operands, so that what they were made
+            // from and their hooks come in where the engine walks on from here.
+            const Tensor xd = x.to(at::kDouble), rd = router.to(at::kDouble), z = at::matmul(xd, rd.t()), s = rule.sigmoid ? z.sigmoid() : z.softmax(-1);
+            const Tensor chosen = ids.clamp(0, E - 1);       // (numbers written past the version count, by .data: none out of range)
+            Tensor dc = grad.to(at::kDouble) * rule.factor;
+            if (rule.renormalize) {
+                const Tensor c = s.gather(1, chosen), sum = c.sum(-1, true);
+                dc = (dc - (dc * (c / sum)).sum(-1, true)) / sum;
+            }
+            const Tensor ds = at::zeros_like(s).scatter(1, chosen, dc), dz = rule.sigmoid ? ds * s * (1 - s) : s * (ds - (ds * s).sum(-1, true));
+            return {want_x ? at::matmul(dz, rd).to(x.scalar_type()) : Tensor(), want_r ? at::matmul(dz.t(), xd).to(router.scalar_type()) : Tensor()};
         }
         const Tensor xr = whole_values(x), rr = whole_values(router), g = grad.to(at::kFloat).contiguous();
         Tensor gx = want_x ? at::empty(xr.sizes(), xr.options()) : Tensor(), gr = want_r ? at::empty(rr.sizes(), rr.options()) : Tensor();

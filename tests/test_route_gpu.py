@@ -272,3 +272,42 @@ def test_changed_indices_are_noticed(how):
             index[..., 0] = (index[..., 0] + 1) % 6
     with pytest.raises(RuntimeError, match="indices.*not what the forward found" if how in ("fewer of them", "another type") else "modified by an inplace operation"):
         torch.autograd.grad(w, (xd, rd), g.view(w.shape))
+
+
+@pytest.mark.parametrize("score,renormalize,biased", RULES)
+@pytest.mark.parametrize("hooked", [False, True])
+def test_second_derivative_of_operands_that_depend_on_each_other(hooked, score, renormalize, biased):
+    """x made from the router, as below a layer that shares it: with a graph of the gradients the router's has both ways, each once, and a hook on x runs once.
+
+    float32 roundings, each 2^-24 of what it rounds: the weights, the gradients of both operands and their sum, twice over for the second derivative,
+    some ten; sums of terms of either sign that leave a sixteenth or more of them: 10 * 16 * 2^-24 = 1e-5."""
+    x, router, bias = operands(5, 6, 16, torch.float32, torch.float32)
+    mix, v = torch.randn((5, 6), generator=gen(4)) * 0.5, torch.randn((5, 2), generator=gen(5))
+    bias = bias if biased else None
+    answers, calls = [], []
+    for on_gpu in (False, True):
+        move = (lambda t: t.cuda()) if on_gpu else (lambda t: t.double())
+        leaf, r = move(x).requires_grad_(), move(router).requires_grad_()
+        inner = leaf + move(mix) @ r
+        if hooked:
+            inner.register_hook(lambda g: calls.append(on_gpu) or 2 * g)
+        b = None if bias is None else move(bias)
+        w = moe.moe_route(inner, r, 2, b, score, renormalize, 1.5)[0] if on_gpu else plain(inner, r, 2, b, score, renormalize, 1.5)[0]
+        first = torch.autograd.grad((w * move(v)).square().sum(), (leaf, r), create_graph=True)
+        if hooked:
+            assert calls.count(on_gpu) == 1
+        second = torch.autograd.grad(sum(g.square().sum() for g in first), (leaf, r))
+        answers.append([t.detach().cpu().double() for t in (*first, *second)])
+    for want, got in zip(*answers):
+        assert (got - want).norm() <= 1e-5 * want.norm(), (got - want).norm() / want.norm()
+
+
+def test_gradients_of_several_vectors_at_once():
+    x, router, _ = operands(5, 6, 16, torch.float32, torch.float32)
+    xd, rd = x.cuda().requires_grad_(), router.cuda().requires_grad_()
+    w, _ = moe.moe_route(xd, rd, 2)
+    vectors = torch.randn((3, 5, 2), generator=gen(6)).cuda()
+    got = torch.autograd.grad(w, (xd, rd), vectors, retain_graph=True, is_grads_batched=True)
+    for i in range(3):
+        for a, b in zip(got, torch.autograd.grad(w, (xd, rd), vectors[i], retain_graph=True)):
+            assert (a[i] - b).norm() <= 1e-5 * b.norm()      # (as above: some ten float32 roundings)
