@@ -445,11 +445,15 @@ Tensor block_fp8_experts(const Tensor &x_in, const Tensor &ids_in, const Tensor 
 // ---- int8 operands with a scale for each row
 
 // w holds int8 codes [.., N, K] and scale their scales [.., N], on x's device
-bool is_row_int8(const Tensor &w, const Tensor &scale, const Tensor &x, int64_t matrices) {
+bool holds_row_int8(const Tensor &w, const Tensor &scale, const Tensor &x, int64_t matrices) {
     if (w.device() != x.device() || scale.device() != x.device() || w.layout() != at::kStrided || scale.layout() != at::kStrided ||
         w.scalar_type() != at::kChar || scale.scalar_type() != at::kFloat || w.dim() != (matrices ? 3 : 2) || scale.dim() != w.dim() - 1 ||
         !w.is_contiguous() || !scale.is_contiguous() || ((uintptr_t)w.const_data_ptr() & 15) || w.numel() == 0 || w.size(-1) % 16) return false;
     return scale.sizes() == w.sizes().slice(0, w.dim() - 1) && (!matrices || w.size(0) == matrices) && !differentiable(scale);
+}
+// .. and no transform or trace is about, whose tensors have no pointers to ask for
+bool is_row_int8(const Tensor &w, const Tensor &scale, const Tensor &x, int64_t matrices) {
+    return nothing_watches(w) && nothing_watches(scale) && holds_row_int8(w, scale, x, matrices);
 }
 
 constexpr int64_t ROW_INT8_MOST_K = 1 << 17;
@@ -489,7 +493,7 @@ Tensor row_int8_any_product(const Tensor &x, const Tensor &xs, const Tensor &w, 
 // a bias that the kernels add themselves
 bool plain_bias(const Tensor &bias, const Tensor &x, at::ScalarType dtype, int64_t N) {
     return !bias.defined() || (bias.scalar_type() == dtype && bias.device() == x.device() && bias.dim() == 1 && bias.numel() == N &&
-                               bias.is_contiguous() && !differentiable(bias));
+                               bias.is_contiguous() && !differentiable(bias) && nothing_watches(bias));
 }
 
 // how often a tensor was changed in place (inference tensors do not count that)
@@ -510,7 +514,7 @@ struct RowInt8Backward : public torch::autograd::Node {
                                                : at::zeros({c10::multiply_integers(x_shape) / K, N}, w.options().dtype(x_dtype));
         c10::DeviceGuard guard(grad.device());
         // (a tensor's data may have been replaced, also by some of another size, which counts no change)
-        if (!is_row_int8(w, scale, grad, 0) || w.size(0) != N || w.size(1) != K) throw Failed("the int8 weight is not what the forward found");
+        if (!holds_row_int8(w, scale, grad, 0) || w.size(0) != N || w.size(1) != K) throw Failed("the int8 weight is not what the forward found");
         if (changes(w) != w_changes || changes(scale) != scale_changes)
             throw Failed("the int8 weight or its scales have been modified by an inplace operation since the forward");
         if (differentiable(grad) || !nothing_watches(grad))  // (a second derivative, a transform: the dense product)

@@ -33,6 +33,14 @@ def _check_input(x, what):
     invalidInputError(x.dtype in _FLOATS, f"{what}: unsupported dtype {x.dtype}")
 
 
+def _as_the_kernels_read(w, scale):
+    try:
+        start = w.data_ptr()
+    except RuntimeError:                                     # (a transform's or a trace's tensor, which has no storage and meets torch operators)
+        return True
+    return w.is_contiguous() and scale.is_contiguous() and start % 16 == 0
+
+
 def _check_weight(w, scale, x, what, dim=2):
     invalidInputError(isinstance(w, torch.Tensor) and isinstance(scale, torch.Tensor) and w.device == x.device
                       and scale.device == x.device, f"{what}: the weight and its scales must be on x's GPU")
@@ -40,7 +48,7 @@ def _check_weight(w, scale, x, what, dim=2):
     invalidInputError(w.dim() == dim and w.numel() > 0 and scale.shape == w.shape[:-1],
                       f"{what}: a weight {tuple(w.shape)} has one scale for each row, not {tuple(scale.shape)}")
     invalidInputError(w.shape[-1] % 16 == 0 and w.shape[-1] <= MOST_K, f"{what}: in_features must be a multiple of 16, at most {MOST_K}")
-    invalidInputError(w.is_contiguous() and scale.is_contiguous() and w.data_ptr() % 16 == 0,
+    invalidInputError(_as_the_kernels_read(w, scale),
                       f"{what}: weights and scales must be contiguous, codes from a 16-byte boundary on")
     invalidInputError(not (torch.is_grad_enabled() and scale.requires_grad), f"{what}: weights and scales are frozen")
 

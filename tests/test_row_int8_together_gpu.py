@@ -648,3 +648,42 @@ def test_a_layer_computes_what_its_function_does():
     layer.mp_group = object()
     with pytest.raises(RuntimeError, match="mp_group"):
         layer(x.cuda())
+
+
+def test_transforms_over_weights_biases_and_codes():
+    """Stacked weights by vmap, as of experts: each as by itself.  Both factors of a product, its sum of 128 and the scales in float32 in another order: five roundings
+    of 2^-24 of a product and sqrt(128) of its sum's, 1e-6 of the result's norm."""
+    g = gen(31)
+    (w, ws), x = u.weight(g, 32, 128, (3,)), torch.randn((5, 128), generator=g)
+    w, ws, x, bias = w.cuda(), ws.cuda(), x.cuda(), torch.randn((3, 32), generator=g).cuda()
+    want = torch.stack([ri.row_int8_linear(x, w[i], ws[i], bias[i]) for i in range(3)])
+    got = torch.func.vmap(lambda a, s, b: ri.row_int8_linear(x, a, s, b))(w, ws, bias)
+    assert (got - want).norm() <= 1e-6 * want.norm()
+    turned = torch.func.vmap(lambda a, s, b: ri.row_int8_linear(x, a, s, b), in_dims=(2, 1, 1))(w.permute(1, 2, 0).contiguous(), ws.t().contiguous(), bias.t().contiguous())
+    assert (turned - want).norm() <= 1e-6 * want.norm()
+    only = torch.func.vmap(lambda b: ri.row_int8_linear(x, w[0], ws[0], b))(bias)
+    assert (only - (want[0] - bias[0] + bias[:, None])).norm() <= 1e-6 * want.norm()
+    codes, xs = ri.row_int8_quantize(x)
+    got = torch.func.vmap(lambda a, s, b: ri.row_int8_product(codes, xs, a, s, b, torch.float32))(w, ws, bias)
+    assert (got - want).norm() <= 1e-6 * want.norm()
+    got = torch.func.vmap(lambda c, s: ri.row_int8_product(c, s, w[0], ws[0], dtype=torch.float32))(codes, xs)
+    assert (got - (want[0] - bias[0])).norm() <= 1e-6 * want.norm()
+
+
+def test_backwards_under_a_transform_or_a_mode():
+    """Several vectors at once, and a dispatch mode around the backward only: by the dense product, sums of 48 in float32 (as above)."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Watching(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+    g = gen(32)
+    (w, ws), leaf, v = u.weight(g, 48, 128), torch.randn((3, 128), generator=g), torch.randn((4, 3, 48), generator=g)
+    leaf, w, ws, v = leaf.cuda().requires_grad_(), w.cuda(), ws.cuda(), v.cuda()
+    y = ri.row_int8_linear(leaf, w, ws)
+    want = torch.stack([torch.autograd.grad(y, leaf, v[i], retain_graph=True)[0] for i in range(4)])
+    got, = torch.autograd.grad(y, leaf, v, retain_graph=True, is_grads_batched=True)
+    assert (got - want).norm() <= 1e-6 * want.norm()
+    with Watching():
+        got, = torch.autograd.grad(y, leaf, v[0])
+    assert (got - want[0]).norm() <= 1e-6 * want[0].norm()
