@@ -394,7 +394,7 @@ int lowbit_row_int8_quantize(const void *x, int dtype, int64_t rows, int64_t K, 
 size_t lowbit_row_int8_linear_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K);
 int lowbit_row_int8_linear(const void *x, const void *w, const float *w_scale, const void *bias, void *y, int dtype, int64_t M, int64_t N,
                            int64_t K, void *workspace, size_t workspace_bytes, void *stream);
-/* The same of rows that are codes [M, K] and scale [M] already; bias and y of `dtype`. */
+/* The same of rows that are codes [M, K] and scale [M] already; bias and y of `dtype`.  Any codes, -128 on both sides too. */
 size_t lowbit_row_int8_product_workspace_bytes(int dtype, int64_t M, int64_t N, int64_t K);
 int lowbit_row_int8_product(const void *codes, const float *scale, const void *w, const float *w_scale, const void *bias, void *y, int dtype,
                             int64_t M, int64_t N, int64_t K, void *workspace, size_t workspace_bytes, void *stream);

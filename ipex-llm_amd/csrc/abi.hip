@@ -901,7 +901,7 @@ int lowbit_block_fp8_experts(const void *x, const int64_t *topk_ids, const void 
 
 // ---- products of 8-bit integers with a scale for each row
 
-// Sizes that the kernels' arithmetic and grids hold: whole sums of K products of 127 * 127 in 32 bits, fewer than 2^22 rows of x.
+// Sizes that the kernels' arithmetic and grids hold: whole sums of K products of 127 * 128 in 32 bits, fewer than 2^22 rows of x.
 static int check_row_int8(const char *what, int dtype, int64_t M, int64_t N, int64_t K) {
     if (dtype != LOWBIT_DT_F16 && dtype != LOWBIT_DT_BF16 && dtype != LOWBIT_DT_F32) return fail(LOWBIT_EDTYPE, "%s: unsupported element type", what);
     if (M < 0 || N < 0 || K < 0) return fail(LOWBIT_EARG, "%s: negative shape", what);

@@ -4,7 +4,8 @@
 //     a = max |x[m, :]| (2^-100 at least), xs[m] = a / 127, xc[m, k] = x[m, k] * 127 / a to the nearest, ties to even, decided exactly
 //     y[m, n] = xs[m] * ws[n] * sum_k xc[m, k] * wc[n, k]
 // A row that holds a NaN or an infinity has the scale NaN and codes of zero.  The sum runs over all of K in 32-bit integers: it is exact in any
-// order up to K = 2^17 (127 * 127 * 2^17 < 2^31), and float32, float16 and bfloat16 rows go through the same product.
+// order up to K = 2^17 (127 * 128 * 2^17 < 2^31: a weight's code may be -128, one made here is 127 at most; where both are given, given_codes_plan in
+// row_int8_rows.hip), and float32, float16 and bfloat16 rows go through the same product.
 //
 // v_mfma_i32_16x16x64_i8 takes 16 bytes of a lane (row l & 15, g = l >> 4).  Two of them take 128 values of a row in the 16-byte chunks g and
 // 4 + g: the order of the terms is free as long as both operands agree, and a load of one chunk by 64 lanes covers 64 contiguous bytes of 16 rows.

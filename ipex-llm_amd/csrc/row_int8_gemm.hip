@@ -3,17 +3,21 @@
 
 namespace lowbit {
 
-// y = xs * ws * sum of the splits' sums (+ bias), rounded once; four columns per thread.  Whole numbers: exact in any order.
+// y = xs * ws * sum of the splits' sums (+ bias), rounded once; four columns per thread.  Whole numbers: exact in any order, and in float32 rounded once.
 template <typename OT>
 __global__ __launch_bounds__(256) void row_int8_reduce_kernel(const i32x4 *__restrict__ part, const float *__restrict__ xs, const float *__restrict__ ws,
-                                                              const OT *__restrict__ bias, OT *__restrict__ y, int M, int N, int quads, int splits) {
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+                                                              const OT *__restrict__ bias, OT *__restrict__ y, int M, int N, int quads, int splits, int64_t first) {
+    const int64_t id = first + (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (id >= (int64_t)M * quads) return;
     const int m = (int)(id / quads), n = (int)(id - (int64_t)m * quads) * 4;
     const int64_t stride = (int64_t)M * quads;
     const i32x4 *at = part + id;
-    i32x4 v = *at;
-    for (int s = 1; s < splits; s++) v += at[s * stride];
+    int64_t v[4] = {};                                       // (64 bits: given_codes_plan in row_int8_rows.hip)
+    for (int s = 0; s < splits; s++) {
+        const i32x4 one = at[s * stride];
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] += one[j];
+    }
     const float by = xs[m];
     OT *const to = y + (int64_t)m * N + n;
     typedef OT out4 __attribute__((ext_vector_type(4)));
@@ -96,8 +100,10 @@ size_t row_int8_part_bytes(const Int8Plan &plan, int M, int N) {
 
 template <typename OT> static void launch_reduce(const Int8Args &p, hipStream_t st) {
     const int quads = (p.N + 3) / 4;
-    hipLaunchKernelGGL((row_int8_reduce_kernel<OT>), dim3((uint32_t)(((int64_t)p.M * quads + 255) / 256)), dim3(256), 0, st, (const i32x4 *)p.part, p.xs,
-                       p.ws, (const OT *)p.bias, (OT *)p.y, p.M, p.N, quads, p.splits);
+    constexpr int64_t most = (int64_t)1 << 31;               // threads of a launch
+    for (int64_t first = 0, all = (int64_t)p.M * quads; first < all; first += most)
+        hipLaunchKernelGGL((row_int8_reduce_kernel<OT>), dim3((uint32_t)(((all - first < most ? all - first : most) + 255) / 256)), dim3(256), 0, st,
+                           (const i32x4 *)p.part, p.xs, p.ws, (const OT *)p.bias, (OT *)p.y, p.M, p.N, quads, p.splits, first);
 }
 
 // p: x (codes in rows of ldx bytes, zeros past K up to whole blocks), xs, w, ws, bias, y, M, N, K and, for splits, part

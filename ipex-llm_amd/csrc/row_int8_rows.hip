@@ -262,9 +262,17 @@ __global__ __launch_bounds__(256) void row_int8_pad_kernel(const u32x4 *__restri
 
 static bool whole_blocks(int K) { return K % INT8_BLOCK == 0; }
 
+// The plan of a product of codes that are given.  Those may be -128 on both sides: 128 * 128 * 2^17 is one more than 32 bits hold, so that the longest row goes in
+// two parts at least, whose sums row_int8_reduce_kernel adds in 64 bits.
+static Int8Plan given_codes_plan(int M, int N, int K) {
+    Int8Plan plan = linear_plan(M, N, K).plan;
+    if (K == INT8_MOST_K && plan.splits == 1) plan.splits = 2;
+    return plan;
+}
+
 size_t row_int8_product_workspace_bytes(int M, int N, int K) {
     const size_t padded = whole_blocks(K) ? 0 : (size_t)M * int8_blocks(K) * INT8_BLOCK;
-    return ((padded + 255) & ~(size_t)255) + row_int8_part_bytes(linear_plan(M, N, K).plan, M, N);
+    return ((padded + 255) & ~(size_t)255) + row_int8_part_bytes(given_codes_plan(M, N, K), M, N);
 }
 
 int launch_row_int8_product(const uint8_t *codes, const float *xs, const uint8_t *w, const float *ws, const void *bias, void *y, int dtype, int M, int N,
@@ -281,7 +289,7 @@ int launch_row_int8_product(const uint8_t *codes, const float *xs, const uint8_t
     }
     t.xs = xs; t.w = w; t.ws = ws; t.bias = bias; t.y = y; t.part = (int32_t *)space;
     t.M = M; t.N = N; t.K = K;
-    return launch_row_int8_codes(t, dtype, linear_plan(M, N, K).plan, st);
+    return launch_row_int8_codes(t, dtype, given_codes_plan(M, N, K), st);
 }
 
 }  // namespace lowbit

@@ -18,7 +18,7 @@ from ipex_llm.transformers.block_fp8 import _frozen, _gated, _KeepsFormat
 from ipex_llm.transformers.native_ops import ops
 from ipex_llm.utils.common import invalidInputError
 
-MOST_K = 1 << 17                                             # of a row, so that sums of 127 * 127 fit 32 bits
+MOST_K = 1 << 17                                             # of a row, so that sums of 127 * 128 fit 32 bits
 _ACCEL = "cuda"
 _FLOATS = {torch.float16: ggml.DT_F16, torch.bfloat16: ggml.DT_BF16, torch.float32: ggml.DT_F32}
 

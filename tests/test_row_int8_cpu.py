@@ -168,3 +168,10 @@ def test_route_steps_are_the_formula():
     w, index = moe._route_steps(x, router, 3, bias, "sigmoid", False, 1.0)
     assert torch.equal(index, (torch.sigmoid(z) + bias.double()).topk(3, dim=-1).indices)
     assert torch.allclose(w.double(), torch.sigmoid(z).gather(1, index), atol=1e-7)
+
+
+def test_the_longest_row_of_given_codes_goes_in_parts():
+    """Of given codes 128 * 128 * 2^17 does not fit 32 bits, so that their product has two parts at least, for which the workspace has room."""
+    for m, n in ((1, 17), (16, 300), (40, 33), (300, 3000), (2000, 2100)):
+        k = 1 << 17
+        assert ggml.lowbit_row_int8_product_workspace_bytes(0, m, n, k) >= 2 * m * ((n + 3) // 4 * 4) * 4

@@ -219,3 +219,19 @@ def test_gradient_against_differences():
         d = ((up - down) / 2 * grad.double()).sum()
         # 48 results, each rounded to 2^-24 of itself
         assert abs(gx[row, col].cpu().double() - d) <= 2.0 ** -22 * (up[row].abs() * grad[row].abs()).sum() + 1e-6 * gx[row].norm().cpu()
+
+
+@pytest.mark.parametrize("m", [1, 16, 40, 300])
+def test_every_code_in_the_longest_row(m):
+    """128 * 128 * 2^17 = 2^31, which a product of codes of -128 on both sides reaches and 32 bits do not hold; sums beside it, and one row shorter."""
+    for k in (1 << 17, (1 << 17) - 16):
+        codes, w = torch.full((m, k), -128, dtype=torch.int8), torch.full((33, k), -128, dtype=torch.int8)
+        w[1], w[2], w[3, 0], codes[m // 2, 5] = 127, 0, 0, -127
+        xs, ws, bias = torch.full((m,), 0.5), torch.arange(1.0, 34.0), torch.ones(33)
+        want = torch.full((m, 1), 0.5).double() * ws.double() * u.sums(codes, w)         # (whole numbers below 2^53)
+        for dtype in ALL[1:]:
+            for b in (None, bias):
+                y = ri.row_int8_product(codes.cuda(), xs.cuda(), w.cuda(), ws.cuda(), None if b is None else b.to(dtype).cuda(), dtype).cpu()
+                steps = u.sums(codes, w).float() * xs.unsqueeze(-1) * ws
+                assert torch.equal(y, (steps if b is None else steps + b).to(dtype))
+                assert ((y.double() - want).abs() <= want.abs() * torch.finfo(dtype).eps + 1).all()
