@@ -281,9 +281,12 @@ int launch_row_int8_product(const uint8_t *codes, const float *xs, const uint8_t
     t.ldx = (int64_t)int8_blocks(K) * INT8_BLOCK;
     t.x = codes;
     if (!whole_blocks(K)) {
-        const int64_t units = M * (t.ldx / 16);
-        hipLaunchKernelGGL(row_int8_pad_kernel, dim3((uint32_t)((units + 255) / 256)), dim3(256), 0, st, (const u32x4 *)codes, (u32x4 *)space, units, K / 16,
-                           (int)(t.ldx / 16));
+        constexpr int most = 1 << 18;                        // rows of a launch, of up to 2^13 threads each (a grid holds fewer than 2^32)
+        for (int m = 0; m < M; m += most) {
+            const int64_t units = (M - m < most ? M - m : most) * (t.ldx / 16);
+            hipLaunchKernelGGL(row_int8_pad_kernel, dim3((uint32_t)((units + 255) / 256)), dim3(256), 0, st, (const u32x4 *)(codes + (int64_t)m * K),
+                               (u32x4 *)(space + m * t.ldx), units, K / 16, (int)(t.ldx / 16));
+        }
         t.x = space;
         space += (M * t.ldx + 255) & ~(int64_t)255;
     }

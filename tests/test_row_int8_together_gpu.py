@@ -687,3 +687,22 @@ def test_backwards_under_a_transform_or_a_mode():
     with Watching():
         got, = torch.autograd.grad(y, leaf, v[0])
     assert (got - want[0]).norm() <= 1e-6 * want[0].norm()
+
+
+def test_codes_of_more_than_one_launch():
+    """Rows of 2^17 - 16 codes, which are copied to whole blocks, 2^32 pieces of 16 of them and more: rows of several launches, at both sides of a launch's end."""
+    k, rows = (1 << 17) - 16, (1 << 19) + 3
+    free = torch.cuda.mem_get_info()[0] / 2 ** 30
+    if free < 150:
+        pytest.skip(f"needs 150 GiB, {free:.0f} are free")
+    g = gen(33)
+    at = torch.tensor([0, 1, (1 << 18) - 1, 1 << 18, (1 << 19) - 1, 1 << 19, rows - 1])
+    given, (w, ws) = torch.randint(-127, 128, (len(at), k), generator=g, dtype=torch.int8), u.weight(g, 17, k)
+    codes, xs = torch.zeros((rows, k), dtype=torch.int8, device="cuda"), torch.ones(rows, device="cuda")
+    for i, row in enumerate(at.tolist()):
+        codes[row] = given[i].cuda()
+    y = ri.row_int8_product(codes, xs, w.cuda(), ws.cuda(), dtype=torch.float32)
+    assert torch.equal(y[at.cuda()].cpu(), u.sums(given, w).float() * ws)
+    assert int((y != 0).any(dim=1).sum()) == len(at)
+    del codes, y
+    torch.cuda.empty_cache()
