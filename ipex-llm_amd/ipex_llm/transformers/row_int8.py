@@ -297,9 +297,9 @@ class RowInt8Linear(_KeepsFormat, nn.Linear):
         given = x.dtype
         if self.training and not torch.is_inference_mode_enabled() and self.compute_dtype is not None:
             x = x.to(self.compute_dtype)
-        if self.bias is not None and self.bias.dtype != x.dtype:
-            self.bias.data = self.bias.data.to(x.dtype)
-        y = row_int8_linear(x, self.weight, self.weight_scale, self.bias)
+        # (in x's type for this call only: the bias stays as it was given)
+        bias = self.bias if self.bias is None or self.bias.dtype == x.dtype else self.bias.to(x.dtype)
+        y = row_int8_linear(x, self.weight, self.weight_scale, bias)
         return y if y.dtype == given else y.to(given)
 
     def dequantize(self, dtype=torch.float32):

@@ -706,3 +706,16 @@ def test_codes_of_more_than_one_launch():
     assert int((y != 0).any(dim=1).sum()) == len(at)
     del codes, y
     torch.cuda.empty_cache()
+
+
+def test_a_layer_keeps_its_bias():
+    """A float32 bias meets rows of any type, in that type, and stays what it was."""
+    g = gen(41)
+    lin = nn.Linear(144, 100)
+    (codes, scale), x = u.weight(g, 100, 144), torch.randn((7, 144), generator=g)
+    lin.weight, lin.weight_scale = nn.Parameter(codes, requires_grad=False), nn.Parameter(scale, requires_grad=False)
+    bias = lin.bias.data.clone()
+    layer = ri.RowInt8Linear.from_linear(lin).cuda().eval()
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        assert torch.equal(layer(x.to(dtype).cuda()).cpu(), u.product(x.to(dtype), codes, scale, bias.to(dtype)))
+        assert layer.bias.dtype == torch.float32 and torch.equal(layer.bias.cpu(), bias)
