@@ -235,3 +235,44 @@ def test_every_code_in_the_longest_row(m):
                 steps = u.sums(codes, w).float() * xs.unsqueeze(-1) * ws
                 assert torch.equal(y, (steps if b is None else steps + b).to(dtype))
                 assert ((y.double() - want).abs() <= want.abs() * torch.finfo(dtype).eps + 1).all()
+
+
+# Sizes of each form of tiles in parts (128 x 128: of four waves, then of eight), rows and columns that end inside a tile and K inside a block
+PARTS = [(33, 17, 3264, (32, 128, 1)), (2699, 71, 6800, (32, 128, 1)), (66, 1009, 16016, (64, 64, 2)), (34, 4299, 5232, (64, 64, 2)), (65, 2018, 6224, (64, 128, 1)),
+         (68, 4126, 3424, (64, 128, 1)), (34, 115, 3888, (64, 32, 4)), (4047, 442, 10192, (128, 128, 1)), (135, 5618, 5088, (128, 128, 1)), (67, 2711, 8416, (128, 128, 1)),
+         (195, 8228, 8624, (128, 256, 1)), (135, 5843, 12880, (192, 256, 1)), (267, 5396, 13200, (192, 256, 1)), (391, 4413, 17600, (256, 256, 1)), (417, 8380, 9008, (256, 256, 1))]
+
+
+@pytest.mark.parametrize("m,n,k,form", PARTS)
+def test_every_form_in_parts(form, m, n, k):
+    """Whole numbers of sixteenths up to 127 with a largest of 127 in each row: codes that every type holds, so that one sum serves all."""
+    rows, cols, parts, groups = ggml.lowbit_row_int8_plan(1, 0, m, n, k)
+    assert (rows, cols, groups) == form and parts > 1
+    g = gen(m + n)
+    codes = torch.randint(-127, 128, (m, k), generator=g, dtype=torch.int8)
+    codes[:, k // 2] = 127
+    w, ws = torch.randint(-128, 128, (n, k), generator=g, dtype=torch.int8), torch.rand(n, generator=g) * 0.01
+    sums, xs = u.sums(codes, w).float(), torch.full((m, 1), 127 / 16) / torch.tensor(127.0)
+    wd, sd, bias = w.cuda(), ws.cuda(), torch.randn(n, generator=g)
+    for dtype in ALL:
+        b = bias.to(dtype)
+        y = ri.row_int8_linear((codes.to(dtype) / 16).cuda(), wd, sd).cpu()
+        assert torch.equal(y, (sums * xs * ws).to(dtype))
+        y = ri.row_int8_product(codes.cuda(), xs.view(-1).cuda(), wd, sd, b.cuda(), dtype).cpu()
+        assert torch.equal(y, (sums * xs * ws + b.float()).to(dtype))
+
+
+BACK_PARTS = [(66, 4359, 6064, (128, 256)), (5757, 7598, 144, (192, 256)), (161, 4057, 11376, (192, 256)), (390, 5333, 10448, (256, 256)), (5950, 4975, 736, (256, 256))]
+
+
+@pytest.mark.parametrize("m,n,k,form", BACK_PARTS)
+def test_large_forms_of_the_gradient_in_parts(form, m, n, k):
+    assert ggml.lowbit_row_int8_plan(1, 1, m, n, k)[:2] == form and ggml.lowbit_row_int8_plan(1, 1, m, n, k)[2] > 1
+    g = gen(m + n)
+    x = torch.randn((m, k), generator=g).bfloat16().cuda().requires_grad_()
+    w, ws = u.weight(g, n, k)
+    grad = (torch.randn((m, n), generator=g) * torch.exp2(torch.randint(-9, 3, (m, 1), generator=g).float())).bfloat16()
+    gx, = torch.autograd.grad(ri.row_int8_linear(x, w.cuda(), ws.cuda()), x, grad.cuda())
+    want = (grad.double() * ws.double()) @ w.double()
+    off = (gx.cpu().double() - want).norm(dim=1)
+    assert (off <= back_tolerance(torch.bfloat16) * want.norm(dim=1)).all(), (off / want.norm(dim=1)).max()
