@@ -212,8 +212,12 @@ __global__ __launch_bounds__(64 * WAVES) void block_fp8_expert_down_token_kernel
 }
 
 // The rows of x in codes (as bfloat16 numbers, see EXACT) and scales, and the pairs' sort by expert or its first half, in one launch: the
-// first workgroups quantize (32 blocks each); one more sorts the pairs, or as many as there are chunks count them for the launch that does (expert_sort.h).
-template <typename AT, bool PLACES>
+// first workgroups quantize (32 blocks each); the rest place a pair for each wave, or one sorts them all, or as many as there are chunks count them for the launch
+// that places them (expert_sort.h).
+enum ExpertSort { SORT_EACH, SORT_ONE, SORT_CHUNKS };
+static ExpertSort expert_sort(int64_t pairs, int n_exp) { return counted_by_each(pairs, n_exp) ? SORT_EACH : one_sorts(pairs, n_exp) ? SORT_ONE : SORT_CHUNKS; }
+
+template <typename AT, ExpertSort SORT>
 __global__ __launch_bounds__(256) void block_fp8_expert_rows_kernel(const AT *__restrict__ x, const int64_t *__restrict__ ids, uint8_t *__restrict__ codes,
                                                                     float *__restrict__ scale, int32_t *__restrict__ offsets, int32_t *__restrict__ order,
                                                                     int32_t *__restrict__ pos, int32_t *__restrict__ counts, int tokens, int pairs,
@@ -228,7 +232,8 @@ __global__ __launch_bounds__(256) void block_fp8_expert_rows_kernel(const AT *__
         if ((threadIdx.x & 7) == 0) scale[(int64_t)kb * tokens + row] = s;
         return;
     }
-    if constexpr (PLACES) sort_pairs(ids, offsets, order, pos, pairs, n_exp);
+    if constexpr (SORT == SORT_EACH) count_for_each(ids, offsets, order, pos, pairs, n_exp, blockIdx.x - quantizing);
+    else if constexpr (SORT == SORT_ONE) sort_pairs(ids, offsets, order, pos, pairs, n_exp);
     else count_pairs(ids, counts, pairs, n_exp, chunk, blockIdx.x - quantizing);
 }
 
@@ -317,7 +322,7 @@ void block_fp8_experts_plan(int tokens, int top_k, int n_exp, int H, int I, int 
     plan4[0] = up_rows(pairs, n_exp, I);
     plan4[1] = down.rows;
     plan4[2] = down.cols;
-    plan4[3] = !one_sorts(pairs, n_exp);
+    plan4[3] = expert_sort(pairs, n_exp) == SORT_CHUNKS;
 }
 
 struct ExpertsSpace {
@@ -344,7 +349,7 @@ static ExpertsSpace experts_space(int tokens, int top_k, int n_exp, int H, int I
         w.offsets = take((size_t)(n_exp + 1) * 4);
         w.order = take((size_t)pairs * 4);
         w.pos = take((size_t)pairs * 4);
-        if (!one_sorts(pairs, n_exp)) w.counts = take((size_t)EXPERTS_CHUNKS * n_exp * 4);
+        if (expert_sort(pairs, n_exp) == SORT_CHUNKS) w.counts = take((size_t)EXPERTS_CHUNKS * n_exp * 4);
         w.y = take((size_t)pairs * down_columns(pairs, H) * sizeof(float));        // (rounded once, when a token's are summed: 16 bits would cost its precision twice)
     }
     w.bytes = at;
@@ -388,12 +393,16 @@ template <typename AT> static int launch_experts_t(ExpertsArgs p, const ExpertsS
     int32_t *const counts = (int32_t *)(ws + at.counts);
     const AT *const x = (const AT *)p.x;
     float *const xs = (float *)(ws + at.xs);
-    if (one_sorts(pairs, p.n_exp))
-        hipLaunchKernelGGL((block_fp8_expert_rows_kernel<AT, true>), dim3(quantizing + 1), dim3(256), sort_lds(p.n_exp), st, x, p.ids, ws + at.x,
+    const ExpertSort sort = expert_sort(pairs, p.n_exp);
+    if (sort == SORT_EACH)
+        hipLaunchKernelGGL((block_fp8_expert_rows_kernel<AT, SORT_EACH>), dim3(quantizing + (pairs + p.n_exp + 4) / 4), dim3(256), 0, st, x, p.ids, ws + at.x,
+                           xs, offsets, order, pos, nullptr, tokens, pairs, p.n_exp, p.H, KB, quantizing, 0);
+    else if (sort == SORT_ONE)
+        hipLaunchKernelGGL((block_fp8_expert_rows_kernel<AT, SORT_ONE>), dim3(quantizing + 1), dim3(256), sort_lds(p.n_exp), st, x, p.ids, ws + at.x,
                            xs, offsets, order, pos, nullptr, tokens, pairs, p.n_exp, p.H, KB, quantizing, 0);
     else {
         const int chunk = sort_chunk(pairs), chunks = (pairs + chunk - 1) / chunk;
-        hipLaunchKernelGGL((block_fp8_expert_rows_kernel<AT, false>), dim3(quantizing + chunks), dim3(256), (size_t)p.n_exp * 4, st, x, p.ids, ws + at.x,
+        hipLaunchKernelGGL((block_fp8_expert_rows_kernel<AT, SORT_CHUNKS>), dim3(quantizing + chunks), dim3(256), (size_t)p.n_exp * 4, st, x, p.ids, ws + at.x,
                            xs, offsets, order, pos, counts, tokens, pairs, p.n_exp, p.H, KB, quantizing, chunk);
         launch_expert_place(p.ids, counts, offsets, order, pos, pairs, p.n_exp, st);
     }

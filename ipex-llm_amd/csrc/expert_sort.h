@@ -4,6 +4,8 @@
 // Up to EXPERTS_SORT_PAIRS pairs one workgroup sorts them, beside others of its launch that do other work.  More, or more than EXPERTS_SORT_EXPERTS:
 // workgroups of that launch count a chunk of pairs each, and a second launch places them.  A whole block in int8, 4096 pairs over 64 experts of [512 x 1024]
 // 51.4 us with one workgroup and 55.7 with a second launch, 3300 over 8 of [256 x 512] 31 and 37.
+//
+// The block-scaled experts have a third way, counted_by_each: a wave for each pair and each expert counts what comes before it.
 #pragma once
 #include "lowbit_formats.h"
 
@@ -12,6 +14,12 @@ namespace lowbit {
 constexpr int EXPERTS_SORT_PAIRS = 4096, EXPERTS_SORT_EXPERTS = 2048, EXPERTS_CHUNKS = 256;
 
 inline bool one_sorts(int64_t pairs, int n_exp) { return pairs <= EXPERTS_SORT_PAIRS && n_exp <= EXPERTS_SORT_EXPERTS; }
+
+// Few pairs for the experts there are: each counted by a wave of its own.  That grows with pairs * pairs but not with the experts, of which one workgroup has
+// counts to clear, to sum and to find: a whole block-scaled block of [128 x 256] with 1600 pairs over 160 experts 27.4 us this way and 28.5 with one workgroup, over
+// 16 25.9 and 25.5; 1920 over 64 26.1 and 26.4; 2400 over 128 29.1 and 28.5, over 1024 114 and 118, over 2100, which one workgroup does not take, 255 and 362; 3000
+// over 8 34.8 and 31.3.
+inline bool counted_by_each(int64_t pairs, int n_exp) { return pairs <= 3200 && 5 * (int64_t)n_exp >= pairs - 1600; }
 inline size_t sort_lds(int n_exp) { return (size_t)n_exp * 4 * sizeof(int32_t); }
 
 // pairs of a chunk, whole waves of them
@@ -90,6 +98,33 @@ __device__ __forceinline__ void sort_pairs(const int64_t *__restrict__ ids, int3
         }
         if (b < pairs) pos[b] = place;
     }
+}
+
+// Workgroup `at` of (pairs + n_exp + 4) / 4 places four: a wave counts the pairs that come before its own - those of lower experts, and the earlier ones of its
+// expert -, and waves pairs + e write offsets[e].
+__device__ __forceinline__ void count_for_each(const int64_t *__restrict__ ids, int32_t *__restrict__ offsets, int32_t *__restrict__ order, int32_t *__restrict__ pos,
+                                               int pairs, int n_exp, int at) {
+    const int lane = threadIdx.x & 63, b = at * 4 + (threadIdx.x >> 6);
+    if (b > pairs + n_exp) return;
+    const bool is_pair = b < pairs;
+    const int64_t own = is_pair ? ids[b] : b - pairs;
+    int before = 0;
+    for (int j0 = lane; j0 - lane < pairs; j0 += 512) {
+        int64_t e[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) e[i] = j0 + i * 64 < pairs ? ids[j0 + i * 64] : -1;
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            before += __popcll(__ballot(e[i] >= 0 && e[i] < n_exp && (e[i] < own || (is_pair && e[i] == own && j0 + i * 64 < b))));
+    }
+    if (lane != 0) return;
+    if (!is_pair) {
+        offsets[own] = before;
+        return;
+    }
+    const bool valid = own >= 0 && own < n_exp;
+    pos[b] = valid ? before : -1;
+    if (valid) order[before] = b;
 }
 
 // Workgroup `at` of 256 counts its chunk's pairs by expert, counts[at][e], in n_exp words of dynamic LDS.

@@ -523,3 +523,12 @@ def test_fp8_weights_without_scales_that_were_left_out_stay_left_out(tmp_path):
     again = load_low_bit(model(), str(tmp_path))
     assert type(again["plain"]) is nn.Linear and type(again["scaled"]) is bf.BlockFP8Linear
     assert again["plain"].weight.dtype == u.E4M3 and torch.equal(again["plain"].weight.float(), want["plain"].weight.float())
+
+
+def test_experts_take_no_second_launch_for_few_pairs_of_many_experts():
+    """Up to 3200 pairs are placed in the rows' launch however many experts there are; where a second launch places them the workspace has 256 counts of each
+    expert beside what another expert takes elsewhere, its offset."""
+    for tokens, top_k, n_exp, apart in ((300, 8, 2100, 0), (800, 4, 4095, 0), (3200, 1, 2048, 0), (3201, 1, 2047, 0), (3201, 1, 2049, 1), (4097, 1, 900, 1)):
+        assert ggml.lowbit_block_fp8_experts_plan(tokens, top_k, n_exp, 16, 128)[3] == apart
+        size, more = (ggml._lib.lowbit_block_fp8_experts_workspace_bytes(tokens, top_k, e, 16, 128) for e in (n_exp, n_exp + 1))
+        assert more - size == 1024 * apart or more - size == 1024 * apart + 256

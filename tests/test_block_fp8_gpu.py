@@ -707,3 +707,15 @@ def test_a_block_scaled_checkpoint_layer_keeps_its_codes():
     assert type(model[0]) is bf.BlockFP8Linear and torch.equal(model[0].weight.cpu().float(), w.float())
     x = torch.randn((9, 272), generator=g)
     assert torch.equal(model(x.cuda()), bf.block_fp8_linear(x.cuda(), w.cuda(), ws.cuda()))
+
+
+@pytest.mark.parametrize("tokens,top_k,n_exp,apart", [(200, 8, 160, 0), (401, 4, 2, 0), (3200, 1, 400, 0), (3201, 1, 400, 0), (1600, 2, 321, 0), (1600, 2, 319, 0),
+                                                      (1600, 1, 1, 0), (300, 8, 2100, 0), (800, 4, 4096, 0), (801, 4, 2100, 1), (1025, 4, 9, 1)])
+def test_experts_sorted_in_every_way(tokens, top_k, n_exp, apart):
+    """Pairs counted each by a wave, sorted by one workgroup, or counted and placed by two launches, at the borders between them, some ids naming none."""
+    assert ggml.lowbit_block_fp8_experts_plan(tokens, top_k, n_exp, 16, 128)[3] == apart
+    case = list(expert_case(tokens + n_exp, tokens, top_k, n_exp, 16, 128, torch.bfloat16))
+    case[1][::7, 0], case[1][5::11, -1] = -1, n_exp
+    case[1][3] = 2 ** 33
+    got = check_experts(case, torch.bfloat16)
+    assert (got[3] == 0).all()
