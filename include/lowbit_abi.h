@@ -429,7 +429,8 @@ int lowbit_row_int8_experts_waves(int64_t tokens, int top_k, int n_experts, int6
  *
  * z = x[tokens, hidden] * router[n_experts, hidden]^T, s = softmax or sigmoid of z; topk_ids: the top_k largest z (s + bias[n_experts] where bias is
  * not null), in descending order, ties to the lowest index, NaN above all numbers; topk_weight = factor * s of those, divided by their
- * sum if renormalize.  Sums, z and s are float64, so that the choice depends on no order of summation.  hidden is a multiple of 8, n_experts at
+ * sum if renormalize.  Sums, z and s are float64: only logits within hidden * 2^-53 of both their sums of |x r| may be taken in
+ * another order in a call of another size.  hidden is a multiple of 8, n_experts at
  * most 1024, top_k 64.  logits: z [tokens, n_experts] for the backward, or null. */
 #define LOWBIT_SCORE_SOFTMAX 0
 #define LOWBIT_SCORE_SIGMOID 1

@@ -3,8 +3,9 @@
 //     ids[t, :]: the top_k largest z (s + bias where a bias is given), in descending order, ties to the lowest index, a NaN above all numbers
 //     w[t, j] = factor * s[ids_j] (/ sum of the chosen s where renormalized)
 //
-// z, s and the sums are float64: which of two near experts is taken does not depend on the order of a sum, nor on how many tokens a call holds.
-// Operands are float16, bfloat16 or float32, whose products are exact in float64; v_mfma_f64_16x16x4 adds them.  An operand of it is one value a
+// z, s and the sums are float64.  Operands are float16, bfloat16 or float32, whose products are exact in float64; v_mfma_f64_16x16x4 adds them.  A sum of H
+// products is off by H * 2^-53 of the sum of their magnitudes at most: of experts whose logits (biased scores) are farther apart than that, of both, every call takes the same,
+// whatever the order of its sums, which goes by how many tokens it holds.  An operand of it is one value a
 // lane (row l & 15, k = l >> 4): a lane loads eight neighbours of its row, k = 8 (l >> 4) .. + 7 of 32, and eight instructions take one of
 // them each, since the order of the terms is free as long as both operands agree.
 //

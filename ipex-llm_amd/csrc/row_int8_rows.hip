@@ -147,10 +147,10 @@ template <typename AT> static void launch_few_rows(const Int8Rows &p, int waves,
 }
 
 // Waves of a workgroup, by estimated time in us; 0 where codes of x, made by a launch of their own, and a product of those are estimated shorter,
-// or where x's codes do not fit 64 KiB of LDS.  What grows with the rows is x, which every workgroup reads and quantizes: on [4096 x 4096] one row
-// 6.1 against 6.3 and the launch ahead of it, 2.6; four 8.8 / 6.6 + 2.6; on [28672 x 8192] one 44.5 / 44.4 + 2.6, four 71 / 46 + 2.7; one on
-// [20000 x 512] 9.4 / 4.2 + 2.6.  With short rows sixteen of them are few: 11 on [64 x 128] 3.2 against 5.5 with the launch ahead, 9 on [730 x 384] 4.2 / 5.5, 5 on
-// [2086 x 1152] 5.1 / 6.7, 16 on [1024 x 1024] 7.4 / 6.9.  Fitted to 80 sizes of 1 to 16 rows, within 11 and 17 % at rms; 16
+// or where x's codes do not fit 64 KiB of LDS.  What grows with the rows is x, which every workgroup reads and quantizes.  With weights in turn from memory: on
+// [4096 x 4096] one row 6.1 against 5.9 and the launch ahead of it, 2.6 (5.3 where the one weight stays in the caches), four 8.9 / 6.2 + 2.6; one on
+// [20000 x 512] 9.0 / 5.2 + 2.6, on [4096 x 11008] 14.4 / 15.4 + 2.6; one on [28672 x 8192] goes through tiles, 58 with the launch.  With short rows sixteen of them
+// are few: 11 on [64 x 128] 3.2 against 5.4 with the launch ahead, 9 on [730 x 384] 4.5 to 5 / 5.5, 5 on [2086 x 1152] 5.2 / 6.1, 16 on [1024 x 1024] 7.4 / 7.3.  Fitted to 80 sizes of 1 to 16 rows, within 11 and 17 % at rms; 16
 // waves would be the shortest at one row of very long weights only, [4096 x 11008] 13.7 against 14.3.
 constexpr size_t FEW_LDS = 65536 - 64;
 constexpr float ROWS_LAUNCH_US = 2.6f;

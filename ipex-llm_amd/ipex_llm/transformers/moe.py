@@ -64,8 +64,8 @@ def moe_route(x: torch.Tensor, router: torch.Tensor, top_k: int, bias: torch.Ten
 
     z = x router^T (router [experts, hidden]) and s = softmax(z) or sigmoid(z); chosen are the top_k largest z, in descending order - of s + bias
     where a bias [experts] is given, a correction of the choice that the weights do not see -, ties to the lowest index, a NaN above all numbers.
-    weights = scale * s of those, divided by their sum if `renormalize`.  Sums and scores are float64 (csrc/route.hip), so that the choice depends on
-    no order of summation.  The gradient of the weights flows on to x and the router; the choice and the bias count as constant.  It goes
+    weights = scale * s of those, divided by their sum if `renormalize`.  Sums and scores are float64 (csrc/route.hip): only experts whose
+    logits are within hidden * 2^-53 of both their sums of |x r| may change places in a call of another size.  A bias is taken in float32.  The gradient of the weights flows on to x and the router; the choice and the bias count as constant.  It goes
     by the indices returned: where they are changed in place ahead of it (tokens dropped by -1, an offset added) it is refused; a copy may be."""
     invalidInputError(score in _SCORES, f"moe_route: score is 'softmax' or 'sigmoid', not {score!r}")
     if isinstance(x, torch.Tensor) and isinstance(router, torch.Tensor):
