@@ -719,3 +719,26 @@ def test_a_layer_keeps_its_bias():
     for dtype in (torch.bfloat16, torch.float16, torch.float32):
         assert torch.equal(layer(x.to(dtype).cuda()).cpu(), u.product(x.to(dtype), codes, scale, bias.to(dtype)))
         assert layer.bias.dtype == torch.float32 and torch.equal(layer.bias.cpu(), bias)
+
+
+def test_parts_added_in_more_than_one_launch():
+    """The longest row goes in parts (any codes), whose sums are added four results a thread, 2^31 threads a launch: rows 65536 on of 2^17 results each are the second's."""
+    k, n, m = 1 << 17, 1 << 17, 65600
+    free = torch.cuda.mem_get_info()[0] / 2 ** 30
+    if free < 150:
+        pytest.skip(f"needs 150 GiB, {free:.0f} are free")
+    g = gen(34)
+    rows, cols = torch.tensor([0, 1, 65535, 65536, m - 1]), torch.tensor([0, 5, n - 1])
+    a, b = torch.randint(-128, 128, (len(rows), k), generator=g, dtype=torch.int8), torch.randint(-128, 128, (len(cols), k), generator=g, dtype=torch.int8)
+    a[3], b[2] = -128, -128
+    codes, w = (torch.zeros((r, k), dtype=torch.int8, device="cuda") for r in (m, n))
+    for i, row in enumerate(rows.tolist()):
+        codes[row] = a[i].cuda()
+    for i, col in enumerate(cols.tolist()):
+        w[col] = b[i].cuda()
+    y = ri.row_int8_product(codes, torch.ones(m, device="cuda"), w, torch.full((n,), 0.5, device="cuda"), dtype=torch.bfloat16)
+    got = y[rows.cuda()][:, cols.cuda()].cpu()
+    assert torch.equal(got, (u.sums(a, b).float() * 0.5).bfloat16()) and got[3, 2] == 2.0 ** 30
+    assert int(y[rows.cuda()].count_nonzero()) == int(got.count_nonzero()) and not y[2:65535:1013].any() and not y[65537:m - 1].any()
+    del codes, w, y
+    torch.cuda.empty_cache()
