@@ -311,3 +311,15 @@ def test_gradients_of_several_vectors_at_once():
     for i in range(3):
         for a, b in zip(got, torch.autograd.grad(w, (xd, rd), vectors[i], retain_graph=True)):
             assert (a[i] - b).norm() <= 1e-5 * b.norm()      # (as above: some ten float32 roundings)
+
+
+def test_saved_tensors_that_hooks_move_or_a_checkpoint_makes_again():
+    from torch.utils.checkpoint import checkpoint
+    x, router, _ = operands(8, 6, 16, torch.bfloat16, torch.float32)
+    xd, rd, g = x.cuda().requires_grad_(), router.cuda().requires_grad_(), torch.randn((8, 2), generator=gen(3)).cuda()
+    want = torch.autograd.grad(moe.moe_route(xd, rd, 2)[0], (xd, rd), g)
+    with torch.autograd.graph.save_on_cpu():
+        w, index = moe.moe_route(xd, rd, 2)
+    index.fill_(-1)                                          # (the hook's copy is the one that counts)
+    for got in (torch.autograd.grad(w, (xd, rd), g), torch.autograd.grad(checkpoint(lambda a: moe.moe_route(a, rd, 2)[0], xd, use_reentrant=False), (xd, rd), g)):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
